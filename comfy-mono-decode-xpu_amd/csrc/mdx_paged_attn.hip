@@ -1,0 +1,985 @@
+// Attention over the paged cache (layout: mdx_pages.hip): single tokens, drafted trees and prompt rows of several
+// sequences (mdx_attn_paged), and the same over the blocks of a long context that a score selects (mdx_attn_blocks).
+//
+// Row (b, s, h) attends the committed tokens t < n = length[b] and the rows' own tokens n + j (j < S, their K/V in the
+// pages already) that bit j of mask[b][s] admits, or j <= s without masks: softmax(q . k / sqrt(D)) v, 0 where no token
+// is admitted. A token in a page that the table does not have is not admitted; what a place holds that a row does not
+// admit never reaches it, infinities and NaN included.
+//
+// Work. A unit is (sequence, kv head, block of query rows); its tokens go in steps of 32 per token part. The steps of
+// all units stand in one line and every work-group takes an equal share of it (one work-group per CU: the ring takes most
+// of its LDS), so unequal lengths, one long sequence and many short ones keep all CUs busy alike, and the lengths are
+// read on the device alone. A share that begins or ends inside a unit leaves a partial (maximum, sum, O in fp32), which
+// the second launch joins; a unit inside one share is written at once.
+//
+// A step of a wave: its 32 tokens' K and V come to LDS by direct loads (1 KiB per wave instruction); S^T = K Q^T with
+// A = 16 tokens x 32 dims and B = Q^T in registers (v_mfma_f32_16x16x32), so that the four lanes of a query row hold its
+// scores; softmax with a running maximum; O^T += V^T P^T with A = V^T by transposing LDS reads in the token order the
+// S^T accumulators hold, B = P^T from registers. A wave holds up to four tiles of 16 query rows and reads each K and V
+// operand once for all of them. Sums, maxima and O in fp32; P is rounded to the cache's type for the product (half a
+// step of each weight; the normaliser sums the rounded weights, so that equal values come out unchanged).
+//
+// Reference: none for the pages; the rows' contract is csrc/attn_dpas.sycl:269-342's.
+#include <math.h>
+
+#include "mdx_common.hpp"
+
+namespace mdx {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+
+// The two element types: their MFMA, and P's rounding. fp16 holds weights down to 2^-14 at full precision only: P is
+// scaled by 2^14 there (exact; numerator and normaliser alike), so weights down to 2^-28 of the largest keep theirs.
+struct Bf16 {
+    static constexpr float SHIFT = 0.f;
+    static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pair(float a, float b) {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(mdx_f32x2{a, b}, mdx_bf16x2));
+    }
+    static __device__ __forceinline__ float add_pair(uint32_t p, float c) {
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(mdx_bf16x2, p), mdx_bf16x2{(__bf16)1.f, (__bf16)1.f}, c, false);
+    }
+    static __device__ __forceinline__ float to_f32(uint16_t x) { return bf2f(x); }
+    static constexpr uint32_t EXP = 0x7F807F80u, ONE = 0x00800080u;  // two elements' exponents, one step of them
+};
+struct Fp16 {
+    static constexpr float SHIFT = 14.f;
+    static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pair(float a, float b) {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(mdx_f32x2{a, b}, f16x2));
+    }
+    static __device__ __forceinline__ float add_pair(uint32_t p, float c) {
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, p), f16x2{(_Float16)1.f, (_Float16)1.f}, c, false);
+    }
+    static __device__ __forceinline__ float to_f32(uint16_t x) { return fp16_to_f32(x); }
+    static constexpr uint32_t EXP = 0x7C007C00u, ONE = 0x04000400u;
+};
+
+struct PagedArgs {
+    const uint16_t* q;  // [B, S, H, D], strides qb, qs, qh
+    int64_t qb, qs, qh;
+    const uint16_t* key;  // [Hk, P, T, D], strides kh, kp, kt
+    int64_t kh, kp, kt;
+    const uint16_t* value;
+    int64_t vh, vp, vt;
+    const int32_t* table;  // [B, W], row stride ts
+    int64_t ts;
+    const int32_t* length;  // [B]
+    const int64_t* mask;    // [B, S] or null (a chain)
+    uint16_t* out;          // [B, S, H, D]
+    // selected blocks (mdx_attn_blocks): page indices of the table and pages of the pool, [B, S, Hk, most]
+    int32_t* sel;
+    int32_t* page;
+    int most, sink, local;
+    const uint16_t* ksum;  // [Hk, P, D], strides sh, sp
+    int64_t sh, sp;
+    uint64_t* keys;  // [B, S, Hk, W]
+    int4* info;      // [work-groups]: the unit left open, and the shares it has from there
+    float* part;     // [2 work-groups][rows][D + 2]: O, maximum, sum
+    int B, S, H, Hk, G, W, P, lt;
+    int units;  // units of a sequence and kv head: row blocks, or rows with a selection each
+    int rows;   // query rows of a kv head in a unit's family: S G, or G with a selection
+    float zs;   // scale * log2(e)
+};
+
+constexpr int MAX_SEQS = 1024;
+constexpr int STEP = 32;
+constexpr int GRID = 256;
+constexpr int RING_BYTES = 128 * 1024;
+
+__device__ __forceinline__ uint32_t lds_addr(const void* p) {
+    return uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const unsigned char*)p));
+}
+
+// LDS layout of a 32-token stage, K and V alike: [dims 32 kk ..][token half][16 tokens][64 B], written by direct loads of
+// 16 tokens x 64 B. K: lane (token c16, k-group g) reads its 16 bytes at c16 * 64 + g * 16 of block (kk, half): one
+// contiguous KiB. V: the two 32-byte halves of a token's 64 bytes are exchanged in every second group of four tokens (the
+// loads fetch them so), so that the transposing reads of two lane groups meet different banks; lane s of group g points
+// at token 4 g + s / 4, dims 16 dt + 4 (s % 4) .. + 3, and receives dim c16 of tokens 4 g .. 4 g + 3.
+// The reads are inline asm that ends with its wait: the builtins would wait for every direct load in flight.
+template <int D>
+__device__ __forceinline__ void read_k(u32x4 (&kf)[2][D / 32], uint32_t base) {
+    if constexpr (D == 256) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            asm volatile(
+                "ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:2048\n\tds_read_b128 %2, %8 offset:4096\n\t"
+                "ds_read_b128 %3, %8 offset:6144\n\tds_read_b128 %4, %8 offset:8192\n\tds_read_b128 %5, %8 offset:10240\n\t"
+                "ds_read_b128 %6, %8 offset:12288\n\tds_read_b128 %7, %8 offset:14336\n\ts_waitcnt lgkmcnt(0)"
+                : "=&v"(kf[h][0]), "=&v"(kf[h][1]), "=&v"(kf[h][2]), "=&v"(kf[h][3]), "=&v"(kf[h][4]), "=&v"(kf[h][5]),
+                  "=&v"(kf[h][6]), "=&v"(kf[h][7])
+                : "v"(base + h * 1024)
+                : "memory");
+    } else if constexpr (D == 128) {
+        asm volatile(
+            "ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:2048\n\tds_read_b128 %2, %8 offset:4096\n\t"
+            "ds_read_b128 %3, %8 offset:6144\n\tds_read_b128 %4, %8 offset:1024\n\tds_read_b128 %5, %8 offset:3072\n\t"
+            "ds_read_b128 %6, %8 offset:5120\n\tds_read_b128 %7, %8 offset:7168\n\ts_waitcnt lgkmcnt(0)"
+            : "=&v"(kf[0][0]), "=&v"(kf[0][1]), "=&v"(kf[0][2]), "=&v"(kf[0][3]), "=&v"(kf[1][0]), "=&v"(kf[1][1]),
+              "=&v"(kf[1][2]), "=&v"(kf[1][3])
+            : "v"(base)
+            : "memory");
+    } else {
+        static_assert(D == 64, "head_dim 64, 128 or 256");
+        asm volatile(
+            "ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:2048\n\tds_read_b128 %2, %4 offset:1024\n\t"
+            "ds_read_b128 %3, %4 offset:3072\n\ts_waitcnt lgkmcnt(0)"
+            : "=&v"(kf[0][0]), "=&v"(kf[0][1]), "=&v"(kf[1][0]), "=&v"(kf[1][1])
+            : "v"(base)
+            : "memory");
+    }
+}
+// dim tiles 4 X .. 4 X + 3 of V^T (ev / od: the lane's base for even and odd dim tiles)
+template <int X, int DT>
+__device__ __forceinline__ void read_v4(u32x2 (&va)[DT], u32x2 (&vb)[DT], uint32_t ev, uint32_t od) {
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %9\n\tds_read_b64_tr_b16 %2, %8 offset:2048\n\t"
+        "ds_read_b64_tr_b16 %3, %9 offset:2048\n\tds_read_b64_tr_b16 %4, %8 offset:1024\n\tds_read_b64_tr_b16 %5, %9 offset:1024\n\t"
+        "ds_read_b64_tr_b16 %6, %8 offset:3072\n\tds_read_b64_tr_b16 %7, %9 offset:3072\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(va[4 * X]), "=&v"(va[4 * X + 1]), "=&v"(va[4 * X + 2]), "=&v"(va[4 * X + 3]), "=&v"(vb[4 * X]),
+          "=&v"(vb[4 * X + 1]), "=&v"(vb[4 * X + 2]), "=&v"(vb[4 * X + 3])
+        : "v"(ev + X * 4096), "v"(od + X * 4096)
+        : "memory");
+}
+template <int D>
+__device__ __forceinline__ void read_v(u32x2 (&va)[D / 16], u32x2 (&vb)[D / 16], uint32_t ev, uint32_t od) {
+    read_v4<0>(va, vb, ev, od);
+    if constexpr (D >= 128) read_v4<1>(va, vb, ev, od);
+    if constexpr (D == 256) {
+        read_v4<2>(va, vb, ev, od);
+        read_v4<3>(va, vb, ev, od);
+    }
+}
+
+typedef __attribute__((address_space(4))) const int32_t* const_i32p;
+__device__ __forceinline__ int uload(const int32_t* p) { return *(const_i32p)(p); }  // (a scalar load: uniform addresses)
+
+// what a wave may have in flight behind the load it waits for (vmcnt only)
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+    static_assert(N <= 63, "vmcnt");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// The tokens a unit's steps run over. Without a selection: [0, n + own rows). With one: the selected blocks' tokens, then
+// the tail behind the full pages and the rows' own (virtual tokens v; tree0 = the first own row's).
+struct Span {
+    int n;      // committed tokens
+    int tree0;  // virtual token of own row 0
+    int nsel;   // tokens of selected blocks (0: none)
+    int tail;   // token at which the tail starts
+};
+template <bool SEL>
+__device__ __forceinline__ Span span_of(const PagedArgs& a, int n) {
+    n = n < 0 ? 0 : (n > (a.W << a.lt) ? a.W << a.lt : n);
+    if constexpr (!SEL) return {n, n, 0, 0};
+    const int c = n >> a.lt, k = c < a.most ? c : a.most;
+    return {n, (k << a.lt) + (n - (c << a.lt)), k << a.lt, c << a.lt};
+}
+// steps of unit u of a sequence (RPW: query rows of a row block)
+template <bool SEL>
+__device__ __forceinline__ int steps_of(const PagedArgs& a, const Span& s, int u, int rpw, int tokens_per_step) {
+    int own = a.S;
+    if (!SEL && !a.mask) {  // (a chain's row block ends with its last row's own token)
+        const int last = min(a.rows, (u + 1) * rpw) - 1;
+        own = last / a.G + 1;
+    }
+    if (SEL && !a.mask) own = u + 1;  // (unit u is row u)
+    return (s.tree0 + own + tokens_per_step - 1) / tokens_per_step;
+}
+
+// One work-group: RTW waves of row tiles (TPW tiles of 16 query rows each) times P token parts.
+template <class E, int D, int TPW, int RTW, int P, bool SEL>
+struct Geometry {
+    static constexpr int NT = 64 * RTW * P;
+    static constexpr int RPW = 16 * TPW * RTW;
+    static constexpr int STAGE = STEP * 2 * D;                    // bytes of K (or V) per stage
+    static constexpr int NS = RING_BYTES / (2 * STAGE * P);       // ring stages per part
+    static constexpr int PER = STAGE / 1024 / RTW;                // direct loads per wave, stage and matrix
+    static_assert(NS >= 1 && (NS & (NS - 1)) == 0 && PER >= 1 && (RTW == 1 || NS >= 2), "ring geometry");
+};
+
+template <class E, int D, int TPW, int RTW, int P, bool SEL>
+__global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
+    using Geo = Geometry<E, D, TPW, RTW, P, SEL>;
+    constexpr int NT = Geo::NT, RPW = Geo::RPW, STAGE = Geo::STAGE, NS = Geo::NS, PER = Geo::PER;
+    constexpr int KK = D / 32, DT = D / 16, TOK = STEP * P;
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ int sh_sum[NT / 64], sh_at[3];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, c16 = lane & 15;
+    const int rw = w % RTW, part = w / RTW;
+
+    // ---- this work-group's share of the line of steps: [begin, end), and the sequence it begins in
+    int begin, end, quota, b, in_b;
+    {
+        constexpr int EACH = (MAX_SEQS + NT - 1) / NT;
+        int mine[EACH], sum = 0;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int bb = tid * EACH + i;
+            mine[i] = 0;
+            if (bb < a.B) {
+                const Span s = span_of<SEL>(a, a.length[bb]);
+                int t = 0;
+                for (int u = 0; u < a.units; ++u) t += steps_of<SEL>(a, s, u, RPW, TOK);
+                mine[i] = t * a.Hk;
+            }
+            sum += mine[i];
+        }
+        int incl = sum;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int u = __shfl_up(incl, d, 64);
+            if (lane >= d) incl += u;
+        }
+        if (lane == 63) sh_sum[w] = incl;
+        __syncthreads();
+        int total = 0, before = incl - sum;
+#pragma unroll
+        for (int i = 0; i < NT / 64; ++i) {
+            const int x = sh_sum[i];
+            before += i < w ? x : 0;
+            total += x;
+        }
+        quota = (total + int(gridDim.x) - 1) / int(gridDim.x);
+        begin = int(blockIdx.x) * quota;
+        end = min(total, begin + quota);
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            if (begin >= before && begin < before + mine[i]) {
+                sh_at[0] = tid * EACH + i;
+                sh_at[1] = before;
+            }
+            before += mine[i];
+        }
+        __syncthreads();
+        b = __builtin_amdgcn_readfirstlane(sh_at[0]);
+        in_b = begin - __builtin_amdgcn_readfirstlane(sh_at[1]);
+    }
+    if (tid == 0) a.info[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (begin >= end) return;  // (uniform)
+    begin = __builtin_amdgcn_readfirstlane(begin);
+    end = __builtin_amdgcn_readfirstlane(end);
+
+    // the unit the share begins in
+    Span sp = span_of<SEL>(a, uload(a.length + b));
+    int kh = 0, u = 0;
+    {
+        int all = 0;
+        for (int i = 0; i < a.units; ++i) all += steps_of<SEL>(a, sp, i, RPW, TOK);
+        kh = in_b / all;
+        in_b -= kh * all;
+        for (;; ++u) {
+            const int n = steps_of<SEL>(a, sp, u, RPW, TOK);
+            if (in_b < n) break;
+            in_b -= n;
+        }
+    }
+    int at = begin, step0 = in_b;  // line position, and the unit's step there
+
+    unsigned char* ring = smem + part * NS * 2 * STAGE;
+    const uint32_t ring_lds = lds_addr(ring);
+    const uint32_t k_lane = c16 * 64 + g * 16;
+    const uint32_t v_lane = (4 * g + (c16 >> 2)) * 64 + (c16 & 3) * 8;
+    const uint32_t v_even = v_lane + (g & 1) * 32, v_odd = v_lane + ((g & 1) ^ 1) * 32;
+    // the lane's place within a direct load: token lane / 4 of the half, 16-byte piece lane % 4 (V: exchanged halves)
+    const int k_voff = (lane >> 2) * int(a.kt) * 2 + (lane & 3) * 16;
+    const int v_voff = (lane >> 2) * int(a.vt) * 2 + ((lane & 3) ^ (((lane >> 4) & 1) << 1)) * 16;
+
+    while (true) {
+        const int n_unit = steps_of<SEL>(a, sp, u, RPW, TOK);
+        const int nst = min(n_unit - step0, end - at);  // steps of this unit in the share
+        const int own = (!a.mask && !SEL) ? (min(a.rows, (u + 1) * RPW) - 1) / a.G + 1 : (!a.mask ? u + 1 : a.S);
+        const int t_end = sp.tree0 + own;
+
+        // ---- query rows and what they admit
+        u32x4 qf[TPW][KK];
+        uint64_t bits[TPW];
+        int lim[TPW];
+#pragma unroll
+        for (int t = 0; t < TPW; ++t) {
+            const int r = (SEL ? 0 : u * RPW) + (rw * TPW + t) * 16 + c16;
+            const bool live = r < a.rows;
+            const int rr = live ? r : 0;
+            const int s = SEL ? u : rr / a.G, h = kh * a.G + (SEL ? rr : rr % a.G);
+            const uint16_t* src = a.q + b * a.qb + s * a.qs + h * a.qh + 8 * g;
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) qf[t][kk] = *reinterpret_cast<const u32x4*>(src + 32 * kk);
+            bits[t] = a.mask ? uint64_t(a.mask[int64_t(b) * a.S + s]) : 0;
+            if (a.S < 64) bits[t] &= (uint64_t(1) << a.S) - 1;
+            lim[t] = s;
+        }
+        // they have arrived before the first direct load goes out: the compiler waits for all of those before it uses a
+        // register that a load among them wrote
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int t = 0; t < TPW; ++t) {
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) asm volatile("" : "+v"(qf[t][kk]));
+            asm volatile("" : "+v"(bits[t]));
+        }
+
+        // ---- the stages
+        const unsigned char* kbase = reinterpret_cast<const unsigned char*>(a.key + kh * a.kh);
+        const unsigned char* vbase = reinterpret_cast<const unsigned char*>(a.value + kh * a.vh);
+        const int32_t* row = a.table + b * a.ts;
+        const int64_t unit_row = (int64_t(b) * a.S + u) * a.Hk + kh;  // (with a selection)
+        uint32_t hist = 0;  // two bits per stage issued: its halves stand in pages
+        const unsigned char *kp_[2], *vp_[2];
+        // the pages of stage s (scalar loads), for issue_k / issue_v
+        auto pages = [&](int s) {
+            const int v0 = (step0 + s) * TOK + part * STEP;
+            uint32_t ok = 0;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int v = v0 + 16 * h;
+                int e = -1, r = 0;
+                if (v < t_end) {
+                    if (SEL && v < sp.nsel) {
+                        e = uload(a.page + unit_row * a.most + (v >> a.lt));
+                        r = v & ((1 << a.lt) - 1);
+                    } else {
+                        const int t = SEL ? sp.tail + (v - sp.nsel) : v;
+                        if ((t >> a.lt) < a.W) e = uload(row + (t >> a.lt));
+                        r = t & ((1 << a.lt) - 1);
+                    }
+                }
+                const bool in = e >= 0 && e < a.P;
+                ok |= in ? 1u << h : 0u;
+                // (a half without a page reads the pool's first rows: in bounds, and masked)
+                kp_[h] = kbase + (in ? (e * a.kp + r * a.kt) * 2 : 0);
+                vp_[h] = vbase + (in ? (e * a.vp + r * a.vt) * 2 : 0);
+            }
+            hist = (hist << 2) | ok;
+        };
+        auto issue_k = [&](int s) {
+            unsigned char* dst = ring + (s & (NS - 1)) * 2 * STAGE;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const int i = rw * PER + j;
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kp_[i & 1] + k_voff + (i >> 1) * 64),
+                                                 (__attribute__((address_space(3))) void*)(dst + i * 1024), 16, 0, 0);
+            }
+        };
+        auto issue_v = [&](int s) {
+            unsigned char* dst = ring + (s & (NS - 1)) * 2 * STAGE + STAGE;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const int i = rw * PER + j;
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(vp_[i & 1] + v_voff + (i >> 1) * 64),
+                                                 (__attribute__((address_space(3))) void*)(dst + i * 1024), 16, 0, 0);
+            }
+        };
+
+        f32x4 acc[TPW][DT];
+        float m[TPW], l[TPW];
+#pragma unroll
+        for (int t = 0; t < TPW; ++t) {
+            m[t] = -INFINITY;
+            l[t] = 0.f;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) acc[t][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        // A wave with a ring of its own (RTW == 1) fills the whole ring ahead, refills K's slot once it has read K and V's
+        // once it has read V, and meets no barrier. Waves that share a ring fill NS - 1 stages ahead and refill the slot of
+        // the stage before at the top of a stage, behind the one barrier.
+        constexpr int AHEAD = RTW == 1 ? NS : NS - 1;
+        for (int s = 0; s < AHEAD && s < nst; ++s) {
+            pages(s);
+            issue_k(s);
+            issue_v(s);
+        }
+        for (int s = 0; s < nst; ++s) {
+            const uint32_t slot = ring_lds + (s & (NS - 1)) * 2 * STAGE;
+            // (stages issued when stage s is read: AHEAD more, as far as there are any)
+            const int behind = min(nst - s, AHEAD) - 1;
+            const uint32_t ok = (hist >> (2 * behind)) & 3u;
+            u32x4 kf[2][KK];
+            u32x2 va[DT], vb[DT];
+            const bool more = s + AHEAD < nst;
+            if constexpr (RTW == 1) {
+                if (s + AHEAD - 1 < nst) wait_vm<PER * (2 * NS - 1)>();
+                else wait_vm<0>();
+                read_k<D>(kf, slot + k_lane);
+                if (more) {
+                    pages(s + AHEAD);
+                    issue_k(s + AHEAD);
+                }
+            } else {
+                if (s + AHEAD - 1 < nst) wait_vm<2 * PER * (AHEAD - 1)>();
+                else wait_vm<0>();
+                __builtin_amdgcn_s_barrier();  // everyone's share of stage s has landed, everyone is done with stage s - 1
+                if (more) {
+                    pages(s + AHEAD);
+                    issue_k(s + AHEAD);
+                    issue_v(s + AHEAD);
+                }
+                read_k<D>(kf, slot + k_lane);
+            }
+            f32x4 st[TPW][2];
+#pragma unroll
+            for (int t = 0; t < TPW; ++t)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    st[t][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int kk = 0; kk < KK; ++kk) st[t][h] = E::mfma(kf[h][kk], qf[t][kk], st[t][h]);
+                }
+            if constexpr (RTW == 1) {
+                if (more) wait_vm<PER * (2 * NS - 1)>();
+                else wait_vm<0>();
+            }
+            read_v<D>(va, vb, slot + STAGE + v_even, slot + STAGE + v_odd);
+            if constexpr (RTW == 1)
+                if (more) issue_v(s + AHEAD);
+
+            const int v0 = (step0 + s) * TOK + part * STEP;
+            const bool whole = ok == 3u && v0 + STEP <= sp.tree0;  // (uniform) every row admits all 32 tokens
+            // A weight of 0 times an infinity or a NaN in a place that a row does not admit would reach the row: where such
+            // a stage holds one, its tokens go one by one to the rows that admit them.
+            bool clean = true;
+            if (!whole) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+                    top |= ((va[dt].x & E::EXP) + E::ONE) | ((va[dt].y & E::EXP) + E::ONE) | ((vb[dt].x & E::EXP) + E::ONE) |
+                           ((vb[dt].y & E::EXP) + E::ONE);
+                clean = __builtin_amdgcn_ballot_w64((top & 0x80008000u) != 0) == 0;
+            }
+#pragma unroll
+            for (int t = 0; t < TPW; ++t) {
+                uint32_t in = ~0u;
+                if (!whole) {
+                    const int p = sp.tree0 - v0;  // tokens of the prefix in the stage
+                    if (a.mask) {
+                        const uint64_t own_bits = p >= 32 ? 0 : (p >= 0 ? bits[t] << p : (-p < 64 ? bits[t] >> -p : 0));
+                        in = (p >= 32 ? ~0u : (p > 0 ? (1u << p) - 1u : 0u)) | uint32_t(own_bits);
+                    } else {
+                        const int nv = p + lim[t] + 1;
+                        in = nv >= 32 ? ~0u : (nv > 0 ? (1u << nv) - 1u : 0u);
+                    }
+                    in &= ((ok & 1u) ? 0x0000FFFFu : 0u) | ((ok & 2u) ? 0xFFFF0000u : 0u);
+                    if (__builtin_amdgcn_ballot_w64(in != 0u) == 0) continue;  // (uniform: nothing for this tile)
+                    const uint32_t lb = in >> (4 * g);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (!((lb >> (16 * h + i)) & 1u)) st[t][h][i] = -INFINITY;
+                }
+                float mx = fmaxf(fmaxf(fmaxf(st[t][0][0], st[t][0][1]), fmaxf(st[t][0][2], st[t][0][3])),
+                                 fmaxf(fmaxf(st[t][1][0], st[t][1][1]), fmaxf(st[t][1][2], st[t][1][3])));
+                mx = max_x32(max_x16(mx));
+                const float mnew = fmaxf(m[t], mx);
+                // a row with nothing admitted yet subtracts 0, so -inf - -inf never forms
+                const float mz = (mnew == -INFINITY ? 0.f : mnew) * a.zs - E::SHIFT;
+                const float alpha = __builtin_amdgcn_exp2f(fmaf(m[t], a.zs, -mz) - E::SHIFT);
+                m[t] = mnew;
+                u32x4 pf;
+                float ps = 0.f;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; i += 2) {
+                        const float p0 = __builtin_amdgcn_exp2f(fmaf(st[t][h][i], a.zs, -mz));
+                        const float p1 = __builtin_amdgcn_exp2f(fmaf(st[t][h][i + 1], a.zs, -mz));
+                        pf[2 * h + i / 2] = E::pair(p0, p1);
+                        ps = E::add_pair(pf[2 * h + i / 2], ps);
+                    }
+                l[t] = l[t] * alpha + ps;  // (this lane's tokens; the row's four lanes meet at the end)
+                if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0)
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) acc[t][dt] *= alpha;
+                if (clean) {
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt)
+                        acc[t][dt] = E::mfma(u32x4{va[dt].x, va[dt].y, vb[dt].x, vb[dt].y}, pf, acc[t][dt]);
+                } else {
+                    for (int j = 0; j < 32; ++j) {
+                        // token j's k-slot: lane group (j / 4) % 4, element 4 (j / 16) + j % 4
+                        const bool mine = g == ((j >> 2) & 3);
+                        const uint32_t half = mine ? ((j & 1) ? 0xFFFF0000u : 0x0000FFFFu) : 0u;
+                        const uint32_t m0 = j < 16 && !(j & 2) ? half : 0u, m1 = j < 16 && (j & 2) ? half : 0u;
+                        const uint32_t m2 = j >= 16 && !(j & 2) ? half : 0u, m3 = j >= 16 && (j & 2) ? half : 0u;
+                        const bool admits = (in >> j) & 1u;
+#pragma unroll
+                        for (int dt = 0; dt < DT; ++dt) {
+                            const f32x4 x = E::mfma(u32x4{va[dt].x & m0, va[dt].y & m1, vb[dt].x & m2, vb[dt].y & m3}, pf,
+                                                    f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) acc[t][dt][i] += admits ? x[i] : 0.f;
+                        }
+                    }
+                }
+            }
+        }
+
+        // ---- the parts of a row tile meet in LDS, tile by tile; rows D + 4 floats apart (no two rows of an access in one bank)
+        const bool first = step0 == 0, last = step0 + nst == n_unit;
+        constexpr int OR = D + 4;
+        float* const lo = reinterpret_cast<float*>(smem);               // [RTW][P][16][OR]
+        float* const lm = lo + RTW * P * 16 * OR;                       // [RTW][P][16] maxima (log2 units), then sums
+        float* rec = a.part + (int64_t(blockIdx.x) * 2 + (first ? 1 : 0)) * RPW * (D + 2);
+        __syncthreads();  // the ring is free
+#pragma unroll
+        for (int t = 0; t < TPW; ++t) {
+            float* mo = lo + (rw * P + part) * 16 * OR + c16 * OR + 4 * g;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(mo + 16 * dt) = acc[t][dt];
+            const float sl = sum_x32(sum_x16(l[t]));
+            if (g == 0) {
+                lm[(rw * P + part) * 16 + c16] = m[t] * a.zs;
+                lm[RTW * P * 16 + (rw * P + part) * 16 + c16] = sl;
+            }
+            __syncthreads();
+            // thread: row x / (D / 4) of the RTW tiles' 16 each, four dims
+            for (int x = tid; x < RTW * 16 * (D / 4); x += NT) {
+                const int rt = x / (16 * (D / 4)), rr = x / (D / 4) % 16, d = x % (D / 4) * 4;
+                const int r = (rt * TPW + t) * 16 + rr;  // row of the unit's block
+                const int rg = (SEL ? 0 : u * RPW) + r;
+                if (rg >= a.rows) continue;
+                float M = -INFINITY;
+#pragma unroll
+                for (int p = 0; p < P; ++p) M = fmaxf(M, lm[(rt * P + p) * 16 + rr]);
+                float sum = 0.f;
+                f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    const float mp = lm[(rt * P + p) * 16 + rr];
+                    const float wp = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mp - M);
+                    sum += lm[RTW * P * 16 + (rt * P + p) * 16 + rr] * wp;
+                    o += *reinterpret_cast<const f32x4*>(lo + (rt * P + p) * 16 * OR + rr * OR + d) * wp;
+                }
+                if (first && last) {
+                    const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+                    const int s = SEL ? u : rg / a.G, h = kh * a.G + (SEL ? rg : rg % a.G);
+                    // (no token admitted: 0, whatever o holds)
+                    *reinterpret_cast<uint2*>(a.out + ((int64_t(b) * a.S + s) * a.H + h) * D + d) =
+                        sum == 0.f ? make_uint2(0u, 0u) : make_uint2(E::pair(o[0] * inv, o[1] * inv), E::pair(o[2] * inv, o[3] * inv));
+                } else {
+                    *reinterpret_cast<f32x4*>(rec + int64_t(r) * D + d) = o;
+                    if (d == 0) {
+                        rec[int64_t(RPW) * D + r] = M;
+                        rec[int64_t(RPW) * (D + 1) + r] = sum;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        if (first && !last && tid == 0) {
+            // the unit goes on in the shares behind: how many in all
+            const int left = n_unit - nst;
+            a.info[blockIdx.x] = make_int4(b, kh, u, 1 + (left + quota - 1) / quota);
+        }
+
+        // ---- the next unit
+        at += nst;
+        if (at >= end) break;
+        step0 = 0;
+        if (++u == a.units) {
+            u = 0;
+            if (++kh == a.Hk) {
+                kh = 0;
+                ++b;
+                sp = span_of<SEL>(a, uload(a.length + b));
+            }
+        }
+    }
+}
+
+// The units that several shares worked on: one wave per query row, work-groups (share, four rows). D / 4 lanes take a
+// partial's row in 16-byte pieces, 256 / D partials at once.
+template <class E, int D, bool SEL>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int rpw) {
+    const int4 x = a.info[blockIdx.x];
+    const int nseg = x.w, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int r = int(blockIdx.y) * 4 + w, rg = (SEL ? 0 : x.z * rpw) + r;
+    if (nseg == 0 || rg >= a.rows) return;  // (uniform in the wave)
+    constexpr int TPR = D / 4, NG = 64 / TPR;
+    const int gi = lane / TPR, d = lane % TPR * 4;
+    const int64_t rec = int64_t(rpw) * (D + 2);
+    const float* base = a.part + int64_t(blockIdx.x) * 2 * rec;
+    auto seg = [&](int i) { return base + (i == 0 ? 1 : 2 * i) * rec; };
+    float M = -INFINITY;
+    for (int i = lane; i < nseg; i += 64) M = fmaxf(M, seg(i)[int64_t(rpw) * D + r]);
+    for (int k = 32; k; k >>= 1) M = fmaxf(M, __shfl_xor(M, k, 64));
+    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f;
+#pragma unroll 4
+    for (int i = gi; i < nseg; i += NG) {
+        const float* p = seg(i);
+        const float mi = p[int64_t(rpw) * D + r];
+        const float wi = mi == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi - M);
+        sum += p[int64_t(rpw) * (D + 1) + r] * wi;
+        o += *reinterpret_cast<const f32x4*>(p + int64_t(r) * D + d) * wi;
+    }
+    for (int k = TPR; k < 64; k <<= 1) {
+        sum += __shfl_xor(sum, k, 64);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], k, 64);
+    }
+    if (gi != 0) return;
+    const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+    const int s = SEL ? x.z : rg / a.G, h = x.y * a.G + (SEL ? rg : rg % a.G);
+    *reinterpret_cast<uint2*>(a.out + ((int64_t(x.x) * a.S + s) * a.H + h) * D + d) =
+        sum == 0.f ? make_uint2(0u, 0u) : make_uint2(E::pair(o[0] * inv, o[1] * inv), E::pair(o[2] * inv, o[3] * inv));
+}
+
+// ---- the selection ----------------------------------------------------------------------------------------
+// Scores of the full pages between the forced ones: (sum of the group's queries) . mean key, in float64 (the order of
+// scores decides, and 32-bit sums in another order would swap neighbours), as keys whose unsigned order is the scores'
+// (NaN lowest). One thread per page, the queries' sums in LDS.
+constexpr int SCORE_ROWS = 8;
+template <class E, int D>
+__global__ __launch_bounds__(256) void block_score_kernel(PagedArgs a) {
+    __shared__ double qs[SCORE_ROWS][D];
+    const int b = blockIdx.z / a.Hk, kh = blockIdx.z % a.Hk, s0 = blockIdx.y * SCORE_ROWS, ns = min(SCORE_ROWS, a.S - s0);
+    const int c = span_of<true>(a, a.length[b]).tail >> a.lt;
+    const int j = a.sink + int(blockIdx.x) * 256 + int(threadIdx.x), j_end = c - a.local;
+    if (c <= a.most || a.sink + int(blockIdx.x) * 256 >= j_end) return;  // (uniform; all pages are selected, or none is scored here)
+    for (int i = threadIdx.x; i < ns * D; i += 256) {
+        const int s = i / D, d = i % D;
+        const uint16_t* p = a.q + b * a.qb + (s0 + s) * a.qs + kh * a.G * a.qh + d;
+        double t = 0;
+        for (int h = 0; h < a.G; ++h) t += double(E::to_f32(p[h * a.qh]));
+        qs[s][d] = t;
+    }
+    __syncthreads();
+    if (j >= j_end) return;
+    const int e = a.table[b * a.ts + j];
+    double dot[SCORE_ROWS];
+#pragma unroll
+    for (int s = 0; s < SCORE_ROWS; ++s) dot[s] = 0;
+    const bool in = e >= 0 && e < a.P;
+    if (in) {
+        const uint16_t* k = a.ksum + kh * a.sh + e * a.sp;
+        for (int d = 0; d < D; d += 8) {
+            const u32x4 v = *reinterpret_cast<const u32x4*>(k + d);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const double x = double(E::to_f32(uint16_t(v[i / 2] >> (16 * (i & 1)))));
+#pragma unroll
+                for (int s = 0; s < SCORE_ROWS; ++s)
+                    if (s < ns) dot[s] = fma(x, qs[s][d + i], dot[s]);
+            }
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < SCORE_ROWS; ++s)
+        if (s < ns) {
+            const double z = dot[s] + 0.0;  // (-0 and 0 are one score)
+            const uint64_t u = __builtin_bit_cast(uint64_t, z);
+            a.keys[((int64_t(b) * a.S + s0 + s) * a.Hk + kh) * a.W + j] =
+                !in || z != z ? 0 : (u >> 63 ? ~u : u | (uint64_t(1) << 63));
+        }
+}
+
+// The `blocks` best of the scored pages (ties to the lowest index) and the forced ones, ascending: one work-group per
+// (sequence, row, kv head). The threshold by bytes from the top (a histogram in LDS per byte, stopping where a byte's
+// pages are all taken), then one pass in index order.
+__global__ __launch_bounds__(256) void block_select_kernel(PagedArgs a) {
+    __shared__ int hist[256], tmp[4], pick[3];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int64_t unit = blockIdx.x;
+    const int b = int(unit / (int64_t(a.S) * a.Hk));
+    const int c = span_of<true>(a, a.length[b]).tail >> a.lt;
+    int32_t* sel = a.sel + unit * a.most;
+    int32_t* page = a.page + unit * a.most;
+    const int32_t* row = a.table + b * a.ts;
+    if (c <= a.most) {  // every full page
+        for (int i = tid; i < a.most; i += 256) {
+            sel[i] = i < c ? i : -1;
+            page[i] = i < c ? row[i] : -1;
+        }
+        return;
+    }
+    const uint64_t* keys = a.keys + unit * a.W;
+    const int j0 = a.sink, j1 = c - a.local, want = a.most - a.sink - a.local;
+    uint64_t prefix = 0;  // the threshold's bytes so far
+    int left = want, shift = 64;
+    bool exact = want == 0;  // every page of the last byte's bin is taken
+    while (!exact && shift > 0) {
+        shift -= 8;
+        hist[tid] = 0;
+        __syncthreads();
+        for (int j = j0 + tid; j < j1; j += 256) {
+            const uint64_t k = keys[j];
+            if (shift == 56 || (k >> (shift + 8)) == prefix) atomicAdd(&hist[int(k >> shift) & 255], 1);
+        }
+        __syncthreads();
+        // the bin that holds the left-th from the top: sums from bin 255 downwards
+        int v = hist[255 - tid];
+        const int own = v;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int u = __shfl_up(v, d, 64);
+            if (lane >= d) v += u;
+        }
+        if (lane == 63) tmp[w] = v;
+        __syncthreads();
+        for (int i = 0; i < w; ++i) v += tmp[i];
+        if (v >= left && v - own < left) {
+            pick[0] = 255 - tid;
+            pick[1] = left - (v - own);
+            pick[2] = own;
+        }
+        __syncthreads();
+        prefix = (prefix << 8) | uint64_t(pick[0]);
+        left = pick[1];
+        exact = pick[2] == left;
+    }
+    // pages whose key's first bytes lie above the prefix, and `left` of those at it (all of them, or the first in order)
+    int taken = 0, ties = 0;  // (running counts, uniform)
+    for (int i = tid; i < a.sink; i += 256) {
+        sel[i] = i;
+        page[i] = row[i];
+    }
+    for (int i = tid; i < a.local; i += 256) {
+        sel[a.sink + want + i] = j1 + i;
+        page[a.sink + want + i] = row[j1 + i];
+    }
+    if (want == 0) return;
+    for (int base = j0; base < j1; base += 256) {
+        const int j = base + tid;
+        const uint64_t k = j < j1 ? keys[j] >> shift : 0;
+        const bool above = j < j1 && k > prefix, at = j < j1 && k == prefix;
+        const uint64_t ma = __builtin_amdgcn_ballot_w64(above), mt = __builtin_amdgcn_ballot_w64(at);
+        const uint64_t under = (uint64_t(1) << lane) - 1;
+        __syncthreads();
+        if (lane == 0) {
+            hist[w] = __popcll(ma);
+            hist[4 + w] = __popcll(mt);
+        }
+        __syncthreads();
+        int na = 0, nt = 0, all_a = 0, all_t = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            na += i < w ? hist[i] : 0;
+            nt += i < w ? hist[4 + i] : 0;
+            all_a += hist[i];
+            all_t += hist[4 + i];
+        }
+        na += __popcll(ma & under);
+        nt += __popcll(mt & under);
+        // its place: pages above before it, and of the ties before it those that are taken
+        const bool take = above || (at && ties + nt < left);
+        if (take) {
+            const int to = a.sink + taken + na + min(ties + nt, left);
+            sel[to] = j;
+            page[to] = row[j];
+        }
+        taken += all_a;
+        ties += all_t;
+    }
+}
+
+// ---- launches ---------------------------------------------------------------------------------------------
+template <class E, int D, int TPW, int RTW, int P, bool SEL>
+int launch(const PagedArgs& a, hipStream_t st) {
+    using Geo = Geometry<E, D, TPW, RTW, P, SEL>;
+    constexpr int joined = (RTW * P * 16 * (D + 4) + 2 * RTW * P * 16) * 4;
+    constexpr int lds = RING_BYTES > joined ? RING_BYTES : joined;
+    const void* fn = reinterpret_cast<const void*>(&paged_attn_kernel<E, D, TPW, RTW, P, SEL>);
+    allow_smem(fn, lds);
+    hipLaunchKernelGGL((paged_attn_kernel<E, D, TPW, RTW, P, SEL>), dim3(GRID), dim3(Geo::NT), lds, st, a);
+    MDX_LAUNCHED();
+    const int rows = a.rows < Geo::RPW ? a.rows : Geo::RPW;
+    hipLaunchKernelGGL((paged_join_kernel<E, D, SEL>), dim3(GRID, unsigned((rows + 3) / 4)), dim3(256), 0, st, a, Geo::RPW);
+    MDX_LAUNCHED();
+    return MDX_OK;
+}
+
+// query rows of a work-group: what covers the rows of a kv head with as few row blocks as registers allow
+template <int D>
+int rows_per_wg(int rows) {
+    if (rows <= 16) return 16;
+    if (rows <= 32) return 32;
+    if (rows <= 64) return 64;
+    return 128;
+}
+
+template <class E, int D, bool SEL>
+int launch_rows(const PagedArgs& a, hipStream_t st) {
+    if (a.rows <= 16) return launch<E, D, 1, 1, 4, SEL>(a, st);
+    if (a.rows <= 32) return launch<E, D, 2, 1, 4, SEL>(a, st);
+    if constexpr (D == 256) {
+        if (a.rows <= 64) return launch<E, D, 2, 2, 2, SEL>(a, st);
+        if constexpr (!SEL) return launch<E, D, 2, 4, 1, SEL>(a, st);
+    } else {
+        if (a.rows <= 64) return launch<E, D, 4, 1, 4, SEL>(a, st);
+        if constexpr (!SEL) return launch<E, D, 2, 4, 2, SEL>(a, st);
+    }
+    set_error("at most 64 query heads per kv head");
+    return MDX_EINVAL;
+}
+
+template <bool SEL>
+int launch_any(const PagedArgs& a, int D, int dtype, hipStream_t st) {
+    if (dtype == MDX_DT_BF16) {
+        if (D == 64) return launch_rows<Bf16, 64, SEL>(a, st);
+        if (D == 128) return launch_rows<Bf16, 128, SEL>(a, st);
+        return launch_rows<Bf16, 256, SEL>(a, st);
+    }
+    if (D == 64) return launch_rows<Fp16, 64, SEL>(a, st);
+    if (D == 128) return launch_rows<Fp16, 128, SEL>(a, st);
+    return launch_rows<Fp16, 256, SEL>(a, st);
+}
+
+int rpw_of(int64_t rows) { return rows_per_wg<128>(int(rows > 128 ? 128 : rows)); }
+
+size_t base_bytes(int64_t rows, int64_t D) {
+    return size_t(GRID) * sizeof(int4) + size_t(GRID) * 2 * rpw_of(rows) * (D + 2) * 4;
+}
+
+int log2_of(int64_t T) {
+    for (int i = 4; i <= 10; ++i)
+        if (T == int64_t(1) << i) return i;
+    return -1;
+}
+
+// what both entry points check and set
+int fill(PagedArgs& a, const void* q, int64_t q_seq_stride, int64_t q_row_stride, int64_t q_head_stride, const void* key,
+         int64_t k_head_stride, int64_t k_page_stride, int64_t k_row_stride, const void* value, int64_t v_head_stride,
+         int64_t v_page_stride, int64_t v_row_stride, int32_t dtype, const int32_t* table, int64_t table_stride,
+         const int32_t* length, const int64_t* mask, void* out, int64_t B, int64_t S, int64_t H, int64_t Hk, int64_t D,
+         int64_t P, int64_t T, int64_t W, float scale) {
+    MDX_CHECK(q && key && value && table && length && out, "null pointer");
+    MDX_CHECK(dtype == MDX_DT_BF16 || dtype == MDX_DT_F16, "bf16 or fp16");
+    MDX_CHECK(D == 64 || D == 128 || D == 256, "head_dim must be 64, 128 or 256");
+    const int lt = log2_of(T);
+    MDX_CHECK(lt >= 0, "page rows: a power of two in 16..1024");
+    MDX_CHECK(B >= 1 && B <= MAX_SEQS && Hk >= 1 && Hk <= 1024 && H >= 1 && H % Hk == 0 && H <= 65536, "1..1024 sequences, heads");
+    MDX_CHECK(P >= 1 && P <= (int64_t(1) << 30) && W >= 1 && (W << lt) < (int64_t(1) << 30) && table_stride >= W &&
+                  table_stride <= (int64_t(1) << 26),
+              "pages, table [sequences, W], under 2^30 tokens a sequence");
+    const int64_t lim = int64_t(1) << 40;
+    MDX_CHECK(k_row_stride >= D && v_row_stride >= D && k_row_stride <= (int64_t(1) << 24) && v_row_stride <= (int64_t(1) << 24) &&
+                  k_head_stride >= 0 && v_head_stride >= 0 && k_page_stride >= 0 && v_page_stride >= 0 && k_head_stride < lim &&
+                  v_head_stride < lim && k_page_stride < lim && v_page_stride < lim,
+              "cache strides (rows of D elements or further apart)");
+    MDX_CHECK(aligned(q, 16) && aligned(key, 16) && aligned(value, 16) && aligned(out, 8) && q_seq_stride % 8 == 0 &&
+                  q_row_stride % 8 == 0 && q_head_stride % 8 == 0 && k_head_stride % 8 == 0 && k_page_stride % 8 == 0 &&
+                  k_row_stride % 8 == 0 && v_head_stride % 8 == 0 && v_page_stride % 8 == 0 && v_row_stride % 8 == 0,
+              "16-byte aligned rows");
+    MDX_CHECK(scale > 0.f && scale < INFINITY, "a positive, finite scale");
+    a.q = static_cast<const uint16_t*>(q);
+    a.qb = q_seq_stride, a.qs = q_row_stride, a.qh = q_head_stride;
+    a.key = static_cast<const uint16_t*>(key);
+    a.kh = k_head_stride, a.kp = k_page_stride, a.kt = k_row_stride;
+    a.value = static_cast<const uint16_t*>(value);
+    a.vh = v_head_stride, a.vp = v_page_stride, a.vt = v_row_stride;
+    a.table = table;
+    a.ts = table_stride;
+    a.length = length;
+    a.mask = mask;
+    a.out = static_cast<uint16_t*>(out);
+    a.B = int(B), a.S = int(S), a.H = int(H), a.Hk = int(Hk), a.G = int(H / Hk), a.W = int(W), a.P = int(P), a.lt = lt;
+    a.zs = float(double(scale) * 1.4426950408889634);
+    return MDX_OK;
+}
+
+}  // namespace
+}  // namespace mdx
+
+using namespace mdx;
+
+extern "C" size_t mdx_attn_paged_workspace(int64_t S, int64_t H, int64_t Hk, int64_t D) {
+    if (S < 1 || Hk < 1 || H < 1 || H % Hk != 0 || D < 1) return 0;
+    return base_bytes(S * (H / Hk), D);
+}
+
+extern "C" int mdx_attn_paged(const void* q, int64_t q_seq_stride, int64_t q_row_stride, int64_t q_head_stride, const void* key,
+                              int64_t k_head_stride, int64_t k_page_stride, int64_t k_row_stride, const void* value,
+                              int64_t v_head_stride, int64_t v_page_stride, int64_t v_row_stride, int32_t dtype,
+                              const int32_t* table, int64_t table_stride, const int32_t* length, const int64_t* mask, void* out,
+                              int64_t B, int64_t S, int64_t H, int64_t Hk, int64_t D, int64_t P, int64_t T, int64_t W,
+                              float scale, void* workspace, size_t workspace_bytes, void* stream) {
+    MDX_CHECK(S >= 1 && (mask ? S <= 64 : S <= 65535), "1..64 rows with masks, 1..65535 without");
+    PagedArgs a{};
+    const int rc = fill(a, q, q_seq_stride, q_row_stride, q_head_stride, key, k_head_stride, k_page_stride, k_row_stride, value,
+                        v_head_stride, v_page_stride, v_row_stride, dtype, table, table_stride, length, mask, out, B, S, H, Hk, D, P,
+                        T, W, scale);
+    if (rc != MDX_OK) return rc;
+    const int64_t rows = S * (H / Hk);
+    const int rpw = rpw_of(rows);
+    const int64_t blocks = (rows + rpw - 1) / rpw;
+    MDX_CHECK(rows < (int64_t(1) << 30) && B * Hk * blocks * ((W * T + S) / STEP + 1) < (int64_t(1) << 31),
+              "too many rows times tokens for one call");
+    MDX_CHECK(workspace && aligned(workspace, 16) && workspace_bytes >= base_bytes(rows, D), "workspace: %zu bytes, 16-byte aligned",
+              base_bytes(rows, D));
+    a.rows = int(rows);
+    a.units = int(blocks);
+    a.info = static_cast<int4*>(workspace);
+    a.part = reinterpret_cast<float*>(a.info + GRID);
+    return launch_any<false>(a, int(D), dtype, static_cast<hipStream_t>(stream));
+}
+
+extern "C" size_t mdx_attn_blocks_workspace(int64_t B, int64_t S, int64_t H, int64_t Hk, int64_t D, int64_t W, int64_t most) {
+    if (B < 1 || S < 1 || Hk < 1 || H < 1 || H % Hk != 0 || D < 1 || W < 1 || most < 1) return 0;
+    return base_bytes(H / Hk, D) + size_t(B * S * Hk) * (size_t(W) * 8 + size_t((most + 3) / 4 * 4) * 4);
+}
+
+extern "C" int mdx_attn_blocks(const void* q, int64_t q_seq_stride, int64_t q_row_stride, int64_t q_head_stride, const void* key,
+                               int64_t k_head_stride, int64_t k_page_stride, int64_t k_row_stride, const void* value,
+                               int64_t v_head_stride, int64_t v_page_stride, int64_t v_row_stride, const void* ksum,
+                               int64_t s_head_stride, int64_t s_page_stride, int32_t dtype, const int32_t* table,
+                               int64_t table_stride, const int32_t* length, const int64_t* mask, void* out, int32_t* sel,
+                               int64_t blocks, int64_t sink, int64_t local, int64_t B, int64_t S, int64_t H, int64_t Hk,
+                               int64_t D, int64_t P, int64_t T, int64_t W, float scale, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+    MDX_CHECK(S >= 1 && S <= 64, "1..64 rows");
+    MDX_CHECK(ksum && sel, "null pointer");
+    MDX_CHECK(blocks >= 0 && sink >= 0 && local >= 0 && blocks + sink + local >= 1 && blocks + sink + local <= 65536,
+              "1..65536 selected blocks");
+    MDX_CHECK(aligned(ksum, 16) && s_head_stride % 8 == 0 && s_page_stride % 8 == 0 && s_head_stride >= 0 && s_page_stride >= D,
+              "mean keys: 16-byte aligned rows");
+    PagedArgs a{};
+    const int rc = fill(a, q, q_seq_stride, q_row_stride, q_head_stride, key, k_head_stride, k_page_stride, k_row_stride, value,
+                        v_head_stride, v_page_stride, v_row_stride, dtype, table, table_stride, length, mask, out, B, S, H, Hk, D, P,
+                        T, W, scale);
+    if (rc != MDX_OK) return rc;
+    const int64_t most = blocks + sink + local, units = B * S * Hk;
+    MDX_CHECK(H / Hk <= 64, "at most 64 query heads per kv head");
+    MDX_CHECK(B * Hk <= 65535 && units < (int64_t(1) << 24) && units * (((most < W ? most : W) + 1) * T + S) / STEP + units < (int64_t(1) << 31),
+              "too many rows times tokens for one call");
+    const size_t need = mdx_attn_blocks_workspace(B, S, H, Hk, D, W, most);
+    MDX_CHECK(workspace && aligned(workspace, 16) && workspace_bytes >= need, "workspace: %zu bytes, 16-byte aligned", need);
+    a.rows = int(H / Hk);
+    a.units = int(S);
+    a.most = int(most), a.sink = int(sink), a.local = int(local);
+    a.ksum = static_cast<const uint16_t*>(ksum);
+    a.sh = s_head_stride, a.sp = s_page_stride;
+    a.sel = sel;
+    a.info = static_cast<int4*>(workspace);
+    a.part = reinterpret_cast<float*>(a.info + GRID);
+    a.keys = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + base_bytes(a.rows, D));
+    a.page = reinterpret_cast<int32_t*>(a.keys + units * W);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (W > most) {  // (else every full page is selected)
+        const dim3 grid(unsigned((W + 255) / 256), unsigned((S + SCORE_ROWS - 1) / SCORE_ROWS), unsigned(B * Hk));
+        if (dtype == MDX_DT_BF16) {
+            if (D == 64) hipLaunchKernelGGL((block_score_kernel<Bf16, 64>), grid, dim3(256), 0, st, a);
+            else if (D == 128) hipLaunchKernelGGL((block_score_kernel<Bf16, 128>), grid, dim3(256), 0, st, a);
+            else hipLaunchKernelGGL((block_score_kernel<Bf16, 256>), grid, dim3(256), 0, st, a);
+        } else {
+            if (D == 64) hipLaunchKernelGGL((block_score_kernel<Fp16, 64>), grid, dim3(256), 0, st, a);
+            else if (D == 128) hipLaunchKernelGGL((block_score_kernel<Fp16, 128>), grid, dim3(256), 0, st, a);
+            else hipLaunchKernelGGL((block_score_kernel<Fp16, 256>), grid, dim3(256), 0, st, a);
+        }
+        MDX_LAUNCHED();
+    }
+    hipLaunchKernelGGL(block_select_kernel, dim3(unsigned(units)), dim3(256), 0, st, a);
+    MDX_LAUNCHED();
+    return launch_any<true>(a, int(D), dtype, st);
+}

@@ -1282,3 +1282,170 @@ def draft_pick_bf16(approx, x, w, nout, argmax_first, top, top_values, token, vt
               N, K, int(nout), int(bool(argmax_first)), _lib.ptr(top) if _present(top) else None,
               _lib.ptr(top_values), _lib.ptr(token), _lib.ptr(vtok), vtok.numel(), ch, nch, _lib.ptr(calls), _lib.ptr(ws),
               ws.numel(), _lib.stream_of(approx))
+
+
+# ---- the paged cache of several sequences ---------------------------------------------------------------
+# kv [L, 2, Hk, P, T, D] bf16 / fp16 (keys, values of every layer), ksum [L, Hk, P, D] (the full pages' mean keys, or None),
+# table int32 [B, W] (page of token t: table[b, t // T]; -1: none), length int32 [B], refs int32 [P] (0: free). Workspaces are
+# taken from torch's allocator per call, so calls on several streams and captured graphs share none.
+_PAGE_DT = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
+
+
+def _ints(t, what, *shape):
+    if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.shape == shape and t.is_contiguous()):
+        raise RuntimeError(f"{what}: contiguous int32 {list(shape)}")
+
+
+def _same_device(t, **others):
+    d = t.get_device()
+    if d < 0:
+        raise RuntimeError("expected tensors on the ROCm device")
+    for n, o in others.items():
+        if o is not None and (not isinstance(o, torch.Tensor) or o.get_device() != d):
+            raise RuntimeError(f"{n} must be a tensor on the same ROCm device")
+
+
+def _pool(kv, ksum, table, length, refs):
+    """The cache's tensors checked; (L, Hk, P, T, D, B, W)."""
+    _same_device(kv, ksum=ksum, table=table, length=length, refs=refs)
+    _check(kv.dtype in _PAGE_DT and kv.dim() == 6 and kv.shape[1] == 2 and kv.is_contiguous(),
+           "kv: contiguous bf16 / fp16 [layers, 2, kv_heads, pages, page rows, head_dim]")
+    L, _, Hk, P, T, D = kv.shape
+    if ksum is not None:
+        _check(ksum.dtype == kv.dtype and ksum.shape == (L, Hk, P, D) and ksum.is_contiguous(),
+               "ksum: contiguous [layers, kv_heads, pages, head_dim] of the cache's type")
+    _check(table.dtype == torch.int32 and table.dim() == 2 and table.stride(1) == 1 and table.stride(0) >= table.shape[1],
+           "table: int32 [sequences, W], rows contiguous")
+    B, W = table.shape
+    _ints(length, "length", B)
+    _ints(refs, "refs", P)
+    return L, Hk, P, T, D, B, W
+
+
+def page_fork(kv, ksum, table, length, refs, dst, src, room=0, share=True, slots=None):
+    """Sequence dst[i] becomes a continuation of src[i] (src[i] == -1: an empty sequence), in place, for every pair i at once:
+    share=True: it names src's full pages too (their references go up) and gets a copy of the page that src's length ends
+    in; share=False: copies of all of src's pages (and of their mean keys). It gets pages for `room` more tokens; the pages it
+    had go back. dst[i] == src[i]: the sequence stays, only its room is given. All pairs read the state before the call;
+    pages are the lowest free ones, in the pairs' order, and pages given back by this call are free for the next.
+    slots (int64 [pairs, room], optional): the cache rows page * T + row of its next tokens, -1 where there is no page.
+    Returns int32 [pairs]: 1 done, 0 too few free pages (for this pair with those before it), -1 refused (a place outside the
+    table or named twice, a length and room past the table's width); pairs that are not done change nothing.
+    No counterpart in the reference (one sequence, one contiguous cache)."""
+    L, Hk, P, T, D, B, W = _pool(kv, ksum, table, length, refs)
+    _same_device(kv, dst=dst, src=src, slots=slots)
+    M = dst.numel()
+    _ints(dst, "dst", M)
+    _ints(src, "src", M)
+    room = int(room)
+    if slots is not None:
+        _check(slots.dtype == torch.int64 and slots.shape == (M, room) and slots.is_contiguous(), "slots: contiguous int64 [pairs, room]")
+    status = torch.empty(M, dtype=torch.int32, device=kv.device)
+    if M == 0:
+        return status
+    ws = torch.empty(_lib.lib().mdx_page_fork_workspace(M, W) or 16, dtype=torch.uint8, device=kv.device)
+    _lib.call_on(kv, "mdx_page_fork", kv.data_ptr(), _lib.ptr(ksum), L, Hk, P, T, D, table.data_ptr(), table.stride(0), B, W,
+                 length.data_ptr(), refs.data_ptr(), dst.data_ptr(), src.data_ptr(), M, room, 1 if share else 0,
+                 _lib.ptr(slots), status.data_ptr(), ws.data_ptr(), ws.numel())
+    return status
+
+
+def page_commit(kv, ksum, table, length, refs, count, path=None, room=0, new_length=None, slots=None):
+    """The step's rows of every sequence become committed: row length[b] + path[b, k] of the cache moves to length[b] + k for
+    k < count[b] (all layers, keys and values; path int32 [B, R] ascending from 0 <= path, R <= 64; None: the rows stand
+    in order already), the length grows by count[b] (into new_length, default: in place), the mean keys of the pages that
+    fill up are taken (ksum not None), and missing pages for `room` more tokens are given (the lowest free ones, in the
+    sequences' order). slots (int64 [B, room], optional): the cache rows page * T + row of the next tokens (the positions
+    that qk_norm_rope_kv writes in a [1, Hk, P * T, D] view of a layer), -1 where there is no page.
+    count[b] < 0: the sequence is left alone (status 1). Returns int32 [B]: 1 done, 0 committed but not all of the room
+    given, -1 refused (a path out of order or range, rows without pages, a length past the table): nothing of that sequence
+    moves or grows. The move of mtp_accept (csrc/mtp_loop.sycl:160-196 of the reference) over pages, for a batch."""
+    L, Hk, P, T, D, B, W = _pool(kv, ksum, table, length, refs)
+    _same_device(kv, count=count, path=path, new_length=new_length, slots=slots)
+    _ints(count, "count", B)
+    R = 0
+    if path is not None:
+        R = path.shape[-1]
+        _ints(path, "path", B, R)
+    if new_length is None:
+        new_length = length
+    else:
+        _ints(new_length, "new_length", B)
+    room = int(room)
+    if slots is not None:
+        _check(slots.dtype == torch.int64 and slots.shape == (B, room) and slots.is_contiguous(), "slots: contiguous int64 [B, room]")
+    status = torch.empty(B, dtype=torch.int32, device=kv.device)
+    ws = torch.empty(_lib.lib().mdx_page_commit_workspace(B, W) or 16, dtype=torch.uint8, device=kv.device)
+    _lib.call_on(kv, "mdx_page_commit", kv.data_ptr(), _lib.ptr(ksum), _PAGE_DT[kv.dtype], L, Hk, P, T, D, table.data_ptr(),
+                 table.stride(0), B, W, length.data_ptr(), new_length.data_ptr(), refs.data_ptr(), count.data_ptr(),
+                 _lib.ptr(path), R, room, _lib.ptr(slots), status.data_ptr(), ws.data_ptr(), ws.numel())
+    return status
+
+
+def _paged(q, key, value, table, length, mask, out):
+    """The operands of the paged attention checked; (out, the C arguments up to value's strides, sizes)."""
+    _same_device(q, key=key, value=value, table=table, length=length, mask=mask, out=out)
+    dt = _PAGE_DT.get(q.dtype)
+    _check(dt is not None and key.dtype == q.dtype and value.dtype == q.dtype, "q, key and value: bf16 or fp16, one type")
+    _check(q.dim() == 4 and q.stride(3) == 1, "q: [sequences, rows, heads, head_dim], the last dim contiguous")
+    B, S, H, D = q.shape
+    _check(key.dim() == 4 and key.shape[3] == D and value.shape == key.shape and key.stride(3) == 1 and value.stride(3) == 1,
+           "key / value: [kv_heads, pages, page rows, head_dim], the last dim contiguous")
+    Hk, P, T, _ = key.shape
+    _check(Hk >= 1 and H % Hk == 0, "query heads: a multiple of the kv heads")
+    _check(table.dtype == torch.int32 and table.dim() == 2 and table.shape[0] == B and table.stride(1) == 1
+           and table.stride(0) >= table.shape[1], "table: int32 [sequences, W], rows contiguous")
+    _ints(length, "length", B)
+    if mask is not None:
+        _check(mask.dtype == torch.int64 and mask.shape == (B, S) and mask.is_contiguous() and S <= 64,
+               "mask: contiguous int64 [sequences, rows], at most 64 rows")
+    if out is None:
+        out = torch.empty(B, S, H, D, dtype=q.dtype, device=q.device)
+    else:
+        _check(out.dtype == q.dtype and out.shape == q.shape and out.is_contiguous(), "out: contiguous, q's shape and type")
+    qs, ks, vs = q.stride(), key.stride(), value.stride()
+    return out, (q.data_ptr(), qs[0], qs[1], qs[2], key.data_ptr(), ks[0], ks[1], ks[2], value.data_ptr(), vs[0], vs[1], vs[2]), \
+        (dt, B, S, H, Hk, D, P, T, table.shape[1])
+
+
+def attn_paged(q, key, value, table, length, mask=None, scale=None, out=None):
+    """Attention of S rows of each of B sequences over their pages: row (b, s) attends the committed tokens t < length[b] and
+    those of the rows' own tokens length[b] + j (j < S, their K / V in the pages already) whose bit j its mask has (int64
+    [B, S], S <= 64: a tree's ancestors), or j <= s without masks (a chain: decode and prompt rows). q [B, S, H, D] (any
+    strides of 8 elements), key / value [Hk, P, T, D] views of the cache (kv[layer, 0], kv[layer, 1]; any strides of 8
+    elements), table, length as page_commit keeps them. out [B, S, H, D]; a row that admits nothing is 0. Tokens in pages that
+    the table does not have are not attended; what stands in places a row does not attend is never seen.
+    The form of attn_dpas (csrc/attn_dpas.sycl:269-342 of the reference) for a batch, pages, and any rows."""
+    out, args, (dt, B, S, H, Hk, D, P, T, W) = _paged(q, key, value, table, length, mask, out)
+    if B == 0 or S == 0:
+        return out
+    ws = torch.empty(_lib.lib().mdx_attn_paged_workspace(S, H, Hk, D), dtype=torch.uint8, device=q.device)
+    _lib.call_on(q, "mdx_attn_paged", *args, dt, table.data_ptr(), table.stride(0), length.data_ptr(), _lib.ptr(mask),
+                 out.data_ptr(), B, S, H, Hk, D, P, T, W, D ** -0.5 if scale is None else float(scale), ws.data_ptr(), ws.numel())
+    return out
+
+
+def attn_blocks(q, key, value, ksum, table, length, blocks, sink=1, local=1, mask=None, scale=None, out=None, sel=None):
+    """attn_paged over a selection of the context's full pages: of the length[b] // T full pages of a sequence, each row and
+    kv head attends the first `sink`, the last `local` and, of the others, the `blocks` whose score is highest (ties: the
+    lowest), score = (sum of the kv head's query heads) . ksum[page], in float64; and always the tokens behind the full
+    pages and the rows' own. ksum [Hk, P, D]: the full pages' mean keys (page_commit's, one layer). At most 64 rows.
+    Returns (out [B, S, H, D], sel int32 [B, S, Hk, sink + local + blocks]): the selected pages of the sequence, ascending,
+    -1 behind them. No counterpart in the reference."""
+    out, args, (dt, B, S, H, Hk, D, P, T, W) = _paged(q, key, value, table, length, mask, out)
+    _same_device(q, ksum=ksum, sel=sel)
+    _check(ksum.dtype == q.dtype and ksum.shape == (Hk, P, D) and ksum.stride(2) == 1, "ksum: [kv_heads, pages, head_dim] of the cache's type")
+    blocks, sink, local = int(blocks), int(sink), int(local)
+    _check(min(blocks, sink, local) >= 0 and 1 <= blocks + sink + local <= 65536, "1..65536 selected blocks")
+    most = blocks + sink + local
+    if sel is None:
+        sel = torch.empty(B, S, Hk, most, dtype=torch.int32, device=q.device)
+    else:
+        _ints(sel, "sel", B, S, Hk, most)
+    if B == 0 or S == 0:
+        return out, sel
+    ws = torch.empty(_lib.lib().mdx_attn_blocks_workspace(B, S, H, Hk, D, W, most) or 16, dtype=torch.uint8, device=q.device)
+    _lib.call_on(q, "mdx_attn_blocks", *args, ksum.data_ptr(), ksum.stride(0), ksum.stride(1), dt, table.data_ptr(),
+                 table.stride(0), length.data_ptr(), _lib.ptr(mask), out.data_ptr(), sel.data_ptr(), blocks, sink, local, B, S, H,
+                 Hk, D, P, T, W, D ** -0.5 if scale is None else float(scale), ws.data_ptr(), ws.numel())
+    return out, sel

@@ -147,6 +147,25 @@ SIGNATURES = {
     "mdx_gdn_run": (ctypes.c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
                                    c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, ctypes.c_float, c_void_p,
                                    c_void_p, c_void_p, c_int64, c_int64, c_int32, c_int64, c_int64, c_int64, c_void_p]),
+    "mdx_page_fork_workspace": (c_size_t, [c_int64, c_int64]),
+    "mdx_page_fork": (ctypes.c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64,
+                                     c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int32, c_void_p,
+                                     c_void_p, c_void_p, c_size_t, c_void_p]),
+    "mdx_page_commit_workspace": (c_size_t, [c_int64, c_int64]),
+    "mdx_page_commit": (ctypes.c_int, [c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p,
+                                       c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+                                       c_int64, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "mdx_attn_paged_workspace": (c_size_t, [c_int64, c_int64, c_int64, c_int64]),
+    "mdx_attn_paged": (ctypes.c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p,
+                                      c_int64, c_int64, c_int64, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
+                                      c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, ctypes.c_float,
+                                      c_void_p, c_size_t, c_void_p]),
+    "mdx_attn_blocks_workspace": (c_size_t, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64]),
+    "mdx_attn_blocks": (ctypes.c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p,
+                                       c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32, c_void_p, c_int64,
+                                       c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64,
+                                       c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, ctypes.c_float, c_void_p, c_size_t,
+                                       c_void_p]),
     "mdx_stream_read": (ctypes.c_int, [c_void_p, c_int64, c_int32, c_void_p, c_void_p]),
     "mdx_gemv_trace": (c_int32, [c_void_p, c_int32]),
     "mdx_check_bf16_round": (ctypes.c_int, [c_void_p, c_void_p, c_void_p]),
@@ -227,3 +246,11 @@ def stream_of(t: torch.Tensor):
 
 def ptr(t):
     return None if t is None else t.data_ptr()
+
+
+def call_on(t, name, *args):
+    """call() with t's device as the current one (a launch belongs to the current device, its stream to t's)."""
+    if t.get_device() == torch.cuda.current_device():
+        return call(name, *args, stream_of(t))
+    with torch.cuda.device(t.device):
+        return call(name, *args, stream_of(t))

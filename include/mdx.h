@@ -584,6 +584,69 @@ int mdx_gdn_run(const uint16_t* proj, const uint16_t* xn, const uint16_t* wa, co
                 uint16_t* qkv, float* gates, uint16_t* core, int64_t rows, int64_t tail, int32_t tail_parity, int64_t HK,
                 int64_t HV, int64_t slots, void* stream);
 
+/* ---- the paged cache of several sequences -----------------------------------------------------
+ * kv [L][2][Hk][P][T][D] 16-bit elements (keys, then values of every layer); table int32 [B][W] (row stride
+ * table_stride): token t of sequence b is row t % T of page table[b][t / T], -1: no page; length int32 [B]: committed
+ * tokens; refs int32 [P]: table entries that name a page, 0: free; ksum [L][Hk][P][D]: the mean key of every full page
+ * (may be NULL). T a power of two in 16..1024. A page that holds a position at or past a sequence's length is that
+ * sequence's alone. All decisions are made on the device from these arrays. Entries outside 0..P - 1 are no pages.
+ * Workspaces need no initial value and hold nothing between calls. */
+
+/* Sequence dst[i] <- src[i] (-1: empty) for every pair i < pairs (<= 1024) at once, with pages for `room` more tokens:
+ * with share, src's full pages are named by dst too and the page its length ends in is copied; without, every page (and
+ * mean key) is copied. dst[i] == src[i]: only the room is given. Fresh pages are the lowest free ones, in pair order;
+ * pages that dst gives back are free from the next call on. slots int64 [pairs][room] (may be NULL): page * T + row of
+ * the next tokens, or -1. status int32 [pairs]: 1 done; 0 too few free pages for the pairs up to this one; -1 refused (dst
+ * outside 0..B - 1 or named by an earlier pair, src >= B, tokens and room past W pages). Pairs not done change nothing. */
+size_t mdx_page_fork_workspace(int64_t pairs, int64_t W);
+int mdx_page_fork(void* kv, void* ksum, int64_t L, int64_t Hk, int64_t P, int64_t T, int64_t D, int32_t* table,
+                  int64_t table_stride, int64_t B, int64_t W, int32_t* length, int32_t* refs, const int32_t* dst,
+                  const int32_t* src, int64_t pairs, int64_t room, int32_t share, int64_t* slots, int32_t* status,
+                  void* workspace, size_t workspace_bytes, void* stream);
+
+/* Per sequence b (B <= 1024): the rows at length[b] + path[b][k] move to length[b] + k for k < count[b] (path int32 [B][R],
+ * strictly ascending in 0..R - 1, R <= 64; NULL: nothing moves), new_length[b] = length[b] + count[b] (may be length), the
+ * mean keys of the pages that fill are written (ksum, fp32 sums), missing pages up to `room` more tokens are given (lowest
+ * free first, in sequence order), slots int64 [B][room] (may be NULL) as above. count[b] < 0: left alone. status int32 [B]:
+ * 1 done; 0 committed, room not all given; -1 refused (bad path, rows without pages, past the table): that sequence stays
+ * (the mean keys of its pages past its length may have been written). Replaces, over pages and for a batch, the KV move of
+ * _C.mtp_accept (csrc/mtp_loop.sycl:160-196). dtype MDX_DT_BF16 or MDX_DT_F16; D in {64, 128, 256}. */
+size_t mdx_page_commit_workspace(int64_t B, int64_t W);
+int mdx_page_commit(void* kv, void* ksum, int32_t dtype, int64_t L, int64_t Hk, int64_t P, int64_t T, int64_t D,
+                    int32_t* table, int64_t table_stride, int64_t B, int64_t W, const int32_t* length, int32_t* new_length,
+                    int32_t* refs, const int32_t* count, const int32_t* path, int64_t R, int64_t room, int64_t* slots,
+                    int32_t* status, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Attention over pages. Row (b, s, h) of q [B, S, H, D]: softmax(scale q . k) v over the committed tokens t < length[b] and
+ * the rows' own tokens length[b] + j, j < S, of bit j of mask[b][s] (int64 [B][S], S <= 64) or, with mask NULL, of j <= s
+ * (S <= 65535); 0 if there are none. Own tokens are read from the pages too. key / value [Hk, P, T, D] (strides in elements;
+ * head, page, row; multiples of 8). out [B, S, H, D] contiguous. fp32 sums, P rounded to the element type. A token in no
+ * page is not attended; the contents of places that a row does not attend (non-finite ones too) do not reach it.
+ * dtype MDX_DT_BF16 or MDX_DT_F16; D in {64, 128, 256}; B <= 1024. The contract of mdx_attn_decode (csrc/attn_dpas.sycl:269-342)
+ * for a batch over pages. */
+size_t mdx_attn_paged_workspace(int64_t S, int64_t H, int64_t Hk, int64_t D);
+int mdx_attn_paged(const void* q, int64_t q_seq_stride, int64_t q_row_stride, int64_t q_head_stride, const void* key,
+                   int64_t k_head_stride, int64_t k_page_stride, int64_t k_row_stride, const void* value,
+                   int64_t v_head_stride, int64_t v_page_stride, int64_t v_row_stride, int32_t dtype, const int32_t* table,
+                   int64_t table_stride, const int32_t* length, const int64_t* mask, void* out, int64_t B, int64_t S, int64_t H,
+                   int64_t Hk, int64_t D, int64_t P, int64_t T, int64_t W, float scale, void* workspace, size_t workspace_bytes,
+                   void* stream);
+
+/* mdx_attn_paged over selected pages: of the c = length[b] / T full pages, row s and kv head g attend the first `sink`, the
+ * last `local` and the `blocks` best of the others by score (sum over the group's heads of q[b][s][h]) . ksum[g][page] in
+ * float64 (ties: the lowest page; NaN last; all pages if c <= sink + local + blocks), then the tokens past the full pages and
+ * the rows' own as above. ksum [Hk, P, D] (strides as given, rows contiguous). sel int32 [B, S, Hk, sink + local + blocks]
+ * receives the selected page numbers of the sequence, ascending, -1 behind. S <= 64, H / Hk <= 64. No counterpart in the
+ * reference. */
+size_t mdx_attn_blocks_workspace(int64_t B, int64_t S, int64_t H, int64_t Hk, int64_t D, int64_t W, int64_t most);
+int mdx_attn_blocks(const void* q, int64_t q_seq_stride, int64_t q_row_stride, int64_t q_head_stride, const void* key,
+                    int64_t k_head_stride, int64_t k_page_stride, int64_t k_row_stride, const void* value,
+                    int64_t v_head_stride, int64_t v_page_stride, int64_t v_row_stride, const void* ksum, int64_t s_head_stride,
+                    int64_t s_page_stride, int32_t dtype, const int32_t* table, int64_t table_stride, const int32_t* length,
+                    const int64_t* mask, void* out, int32_t* sel, int64_t blocks, int64_t sink, int64_t local, int64_t B,
+                    int64_t S, int64_t H, int64_t Hk, int64_t D, int64_t P, int64_t T, int64_t W, float scale, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
 /* Calibration: one streaming read of `bytes` (a multiple of 1024) from `src` with the W4A8 GEMV's load
  * pattern (1 KiB per wave instruction, four loads in flight per wave), over `work_groups` work-groups
  * of 256 threads; `sink` (4 bytes) is written only if the data hashes to a marker value. It has no

@@ -938,3 +938,170 @@ def seeded_uniform(seed, counter, r, j):
     z = splitmix64_mix((int(seed) + (n + 1) * SPLITMIX_GAMMA) & _M64)
     return np.float32((float(z >> 41) + 0.5) * 2.0 ** -23)
 
+
+
+# ---- the paged cache of several sequences -----------------------------------------------------------
+def paged_tokens(table, length, T, P, b, own):
+    """Positions 0 .. length + own - 1 of sequence b that stand in pages: (positions, pages, rows)."""
+    pos = [t for t in range(int(length[b]) + own)
+           if t // T < table.shape[1] and 0 <= table[b, t // T] < P]
+    return (np.array(pos, dtype=np.int64), np.array([table[b, t // T] for t in pos], dtype=np.int64),
+            np.array([t % T for t in pos], dtype=np.int64))
+
+
+def paged_attention(q, key, value, table, length, mask, scale, keep=None):
+    """float64 attention over pages. q [B, S, H, D], key / value [Hk, P, T, D] (float64), table int [B, W], length [B], mask
+    int [B, S] (bit j: own row j) or None (a chain). keep(b, s, kh, positions) -> bool: which positions of a row and kv head
+    take part (None: all). Only the values at admitted positions enter. Returns (out, spread, mass, heft): per element
+    sum w |v - out| and sum w |v|, per row max over its tokens of scale * sum |q k|; rows without tokens are 0."""
+    B, S, H, D = q.shape
+    Hk, P, T, _ = key.shape
+    G = H // Hk
+    out, spread, mass = (np.zeros((B, S, H, D)) for _ in range(3))
+    heft = np.zeros((B, S, H))
+    for b in range(B):
+        n = int(length[b])
+        pos, page, row = paged_tokens(table, length, T, P, b, S)
+        for s in range(S):
+            own = pos - n
+            if mask is None:
+                seen = own <= s
+            else:
+                m = int(mask[b, s])
+                seen = np.array([o < 0 or (m >> int(o)) & 1 == 1 for o in own], dtype=bool)
+            for kh in range(Hk):
+                use = seen if keep is None else seen & keep(b, s, kh, pos)
+                if not use.any():
+                    continue
+                k, v = key[kh, page[use], row[use]], value[kh, page[use], row[use]]
+                for h in range(kh * G, (kh + 1) * G):
+                    z = (k @ q[b, s, h]) * scale
+                    with np.errstate(invalid="ignore"):
+                        w = np.exp(z - z.max())
+                        w = w / w.sum()
+                        out[b, s, h] = (w[:, None] * v).sum(0)
+                        spread[b, s, h] = (w[:, None] * np.abs(v - out[b, s, h])).sum(0)
+                        mass[b, s, h] = (w[:, None] * np.abs(v)).sum(0)
+                        heft[b, s, h] = scale * (np.abs(k) @ np.abs(q[b, s, h])).max()
+    return out, spread, mass, heft
+
+
+def block_selection(q, ksum, table, length, T, blocks, sink, local):
+    """The pages that each row and kv head selects: int [B, S, Hk, sink + local + blocks], ascending, -1 behind. q [B, S, H, D]
+    and ksum [Hk, P, D] float64."""
+    B, S, H, D = q.shape
+    Hk, P = ksum.shape[:2]
+    G, most = H // Hk, sink + local + blocks
+    sel = np.full((B, S, Hk, most), -1, dtype=np.int64)
+    for b in range(B):
+        c = int(length[b]) // T
+        for s in range(S):
+            for kh in range(Hk):
+                if c <= most:
+                    sel[b, s, kh, :c] = np.arange(c)
+                    continue
+                total = q[b, s, kh * G:(kh + 1) * G].sum(0)
+                worth = []
+                for j in range(sink, c - local):
+                    e = int(table[b, j])
+                    x = float((total * ksum[kh, e]).sum()) if 0 <= e < P else float("nan")
+                    worth.append((x != x, -x if x == x else 0.0, j))
+                got = sorted(j for _, _, j in sorted(worth)[:blocks])
+                sel[b, s, kh] = list(range(sink)) + got + list(range(c - local, c))
+    return sel
+
+
+def page_fork(kv, ksum, table, length, refs, dst, src, room, share):
+    """The pairs of a fork one after the other, every read from the state before the call. kv [L, 2, Hk, P, T, D], ksum
+    [L, Hk, P, D]. Returns the new (kv, ksum, table, length, refs), the status and the slots."""
+    T, (B, W) = kv.shape[4], table.shape
+    kv, ksum, refs = kv.copy(), ksum.copy(), refs.copy()
+    new_table, new_length = table.copy(), length.copy()
+    free = [p for p in range(len(refs)) if refs[p] == 0]
+    status, slots, wanted, seen = [], [], 0, set()
+    for d, s in zip(dst, src):
+        d, s = int(d), int(s)
+        n = 0 if s < 0 or s >= B else min(max(int(length[s]), 0), W * T)
+        total = -(-(n + room) // T)
+        if d < 0 or d >= B or d in seen or s >= B or total > W:
+            seen.add(d)
+            status.append(-1)
+            slots.append([-1] * room)
+            continue
+        seen.add(d)
+        full, used = n // T, -(-n // T)
+        kept = W if s == d else full if share else 0
+        places = [j for j in range(full, total) if table[d, j] < 0] if s == d else list(range(kept, total))
+        wanted += len(places)
+        if wanted > len(free):
+            status.append(0)
+            slots.append([-1] * room)
+            continue
+        given = free[wanted - len(places):wanted]
+        row = [-1] * W
+        for j in range(W):
+            if s == d:
+                row[j] = int(table[d, j])
+            elif j < kept:
+                e = int(table[s, j])
+                if 0 <= e < len(refs):
+                    row[j] = e
+                    refs[e] += 1
+        for j, e in zip(places, given):
+            row[j] = e
+            refs[e] += 1
+            old = int(table[s, j]) if s != d and j < used else -1
+            if 0 <= old < len(refs):
+                kv[:, :, :, e] = kv[:, :, :, old]
+                if not share:
+                    ksum[:, :, e] = ksum[:, :, old]
+        if s != d:
+            for e in table[d]:
+                if 0 <= e < len(refs):
+                    refs[e] -= 1
+        new_table[d], new_length[d] = row, n
+        status.append(1)
+        at = [row[t // T] for t in range(n, n + room)]
+        slots.append([e * T + t % T if e >= 0 else -1 for e, t in zip(at, range(n, n + room))])
+    return kv, ksum, new_table, new_length, refs, np.array(status), np.array(slots).reshape(len(status), room)
+
+
+def page_commit(kv, table, length, refs, count, path, room):
+    """A commit, sequence by sequence. Returns the new (kv, table, length, refs), the status, the slots and the pages that filled:
+    a list of (page, float64 mean of its keys [L, Hk, D])."""
+    T, (B, W), P = kv.shape[4], table.shape, kv.shape[3]
+    kv, table, refs, new_length = kv.copy(), table.copy(), refs.copy(), length.copy()
+    free = [p for p in range(P) if refs[p] == 0]
+    status, slots, filled, wanted = np.zeros(B, dtype=np.int64), np.full((B, room), -1, dtype=np.int64), [], 0
+    for b in range(B):
+        n, c = int(length[b]), int(count[b])
+        if c < 0:
+            status[b] = 1
+            continue
+        rows = list(range(c)) if path is None else [int(x) for x in path[b][:c]]
+        ok = n >= 0 and n + c <= W * T and (path is None or c <= len(path[b]))
+        ok = ok and all(x > y for x, y in zip(rows, [-1] + rows)) and (path is None or all(x < len(path[b]) for x in rows))
+        places = (sorted({t // T for t in range(n // T * T, n + c)} | {(n + x) // T for x in rows}) if c else ([n // T] if n % T else [])) if ok else []
+        ok = ok and all(j < W and 0 <= table[b, j] < P for j in places)
+        if not ok:
+            status[b] = -1
+            continue
+        moved = [(kv[:, :, :, table[b, (n + x) // T], (n + x) % T]).copy() for x in rows]
+        for k, x in enumerate(moved):
+            kv[:, :, :, table[b, (n + k) // T], (n + k) % T] = x
+        new_length[b] = n + c
+        for j in range(n // T, (n + c) // T):
+            filled.append((int(table[b, j]), kv[:, 0, :, table[b, j]].astype(np.float64).mean(-2)))
+        last = -(-(n + c + room) // T)
+        need = [j for j in range(-(-(n + c) // T), min(last, W)) if not 0 <= table[b, j] < P]
+        wanted += len(need)
+        status[b] = 1 if wanted <= len(free) and last <= W else 0
+        if wanted <= len(free):
+            for j, e in zip(need, free[wanted - len(need):wanted]):
+                table[b, j] = e
+                refs[e] = 1
+        for r in range(room):
+            t = n + c + r
+            if t // T < W and 0 <= table[b, t // T] < P:
+                slots[b, r] = table[b, t // T] * T + t % T
+    return kv, table, new_length, refs, status, slots, filled

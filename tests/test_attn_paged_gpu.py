@@ -1,0 +1,218 @@
+"""attn_paged on the GPU against the float64 oracle (bounds: tests/paged_cases.py), over pages whose unused rows hold NaN."""
+import pytest
+import torch
+
+from paged_cases import cache, check, tree_masks
+
+pytestmark = pytest.mark.gpu
+BF, FH = torch.bfloat16, torch.float16
+
+
+def _run(C, dev, dt, H, Hk, D, T, lens, S, tree, seed=0):
+    print(f"attn_paged {dt} H={H} Hk={Hk} D={D} T={T} lens={lens} S={S} tree={tree}", flush=True)
+    g = torch.Generator().manual_seed(seed + D + T + S)
+    key, value, table = cache(g, dt, Hk, T, D, lens, S)
+    q = (torch.randn(len(lens), S, H, D, generator=g) * 1.5).to(dt)
+    mask = tree_masks(g, len(lens), S) if tree else None
+    n = torch.tensor(lens, dtype=torch.int32, device=dev)
+    got = C.attn_paged(q.to(dev), key.to(dev), value.to(dev), table.to(dev), n, None if mask is None else mask.to(dev))
+    check(got, dt, q, key, value, table, lens, mask, D ** -0.5)
+
+
+@pytest.mark.parametrize("dt", [BF, FH])
+@pytest.mark.parametrize("H,Hk,D", [(32, 8, 128), (16, 4, 256), (16, 8, 64), (32, 4, 128), (3, 3, 64), (7, 1, 128), (5, 1, 256)])
+def test_single_tokens(C, dev, dt, H, Hk, D):
+    _run(C, dev, dt, H, Hk, D, 16, [0, 1, 15, 16, 17, 31, 32, 33, 127, 128, 300], 1, False)
+
+
+@pytest.mark.parametrize("T", [16, 32, 64, 128, 1024])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_page_sizes(C, dev, T, D):
+    _run(C, dev, BF, 8, 2, D, T, [T - 1, T, T + 1, 3 * T + 5, 0], 3, True, T)
+
+
+@pytest.mark.parametrize("H,Hk,D,S", [(32, 8, 128, 16), (16, 4, 256, 8), (16, 4, 256, 16), (16, 4, 256, 17), (16, 8, 64, 9), (32, 8, 128, 17),
+                                      (32, 4, 128, 64), (8, 8, 64, 64), (4, 4, 256, 63), (4, 1, 128, 33), (12, 4, 64, 5)])
+@pytest.mark.parametrize("dt", [BF, FH])
+def test_trees(C, dev, dt, H, Hk, D, S):
+    _run(C, dev, dt, H, Hk, D, 64, [0, 70, 257], S, True, H)
+
+
+@pytest.mark.parametrize("H,Hk,D,S,lens", [(32, 8, 128, 65, [0, 40]), (8, 2, 128, 300, [129]), (4, 1, 256, 130, [7, 64]), (8, 4, 64, 513, [0]),
+                                           (6, 2, 128, 100, [33, 0, 1]), (16, 1, 128, 9, [50]), (8, 1, 64, 40, [500, 3])])
+def test_chains(C, dev, H, Hk, D, S, lens):
+    _run(C, dev, BF, H, Hk, D, 32, lens, S, False, 5)
+
+
+@pytest.mark.parametrize("D,n", [(128, 5000), (256, 3100), (64, 9001)])
+def test_one_long_sequence_among_short_ones(C, dev, D, n):
+    """Shares of the line of steps that begin and end inside units, and units of a single step."""
+    _run(C, dev, BF, 4, 2, D, 64, [3, n, 0, 40, 1], 2, True, 7)
+
+
+def test_many_sequences(C, dev):
+    g = torch.Generator().manual_seed(2)
+    lens = [int(x) for x in torch.randint(0, 90, (300,), generator=g)]
+    _run(C, dev, BF, 4, 2, 64, 16, lens, 1, False, 9)
+
+
+def _small(dev, dt=BF, D=128, H=8, Hk=2, T=16, lens=(40, 0, 33), S=4, seed=11):
+    g = torch.Generator().manual_seed(seed)
+    lens = list(lens)
+    key, value, table = cache(g, dt, Hk, T, D, lens, S)
+    q = (torch.randn(len(lens), S, H, D, generator=g) * 1.5).to(dt)
+    mask = tree_masks(g, len(lens), S)
+    return g, q, key, value, table, lens, torch.tensor(lens, dtype=torch.int32, device=dev), mask
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_strides(C, dev, D):
+    """A cache of token-major pages, q as a slice of wider rows, a table of wider rows, out given."""
+    g, q, key, value, table, lens, n, mask = _small(dev, D=D)
+    both = torch.stack([key, value], 0).permute(2, 3, 0, 1, 4).contiguous().to(dev)  # [P, T, 2, Hk, D]
+    wide_q = torch.randn(3, 4, 8, 2 * D, generator=g).to(BF)
+    wide_q[..., D:] = q
+    wide_t = torch.full((3, table.shape[1] + 5), -1, dtype=torch.int32)
+    wide_t[:, :table.shape[1]] = table
+    out = torch.empty(3, 4, 8, D, dtype=BF, device=dev)
+    got = C.attn_paged(wide_q.to(dev)[..., D:], both[:, :, 0].permute(2, 0, 1, 3), both[:, :, 1].permute(2, 0, 1, 3),
+                       wide_t.to(dev)[:, :table.shape[1]], n, mask.to(dev), out=out)
+    assert got is out
+    check(got, BF, q, key, value, table, lens, mask, D ** -0.5)
+
+
+def test_scale(C, dev):
+    _, q, key, value, table, lens, n, mask = _small(dev)
+    got = C.attn_paged(q.to(dev), key.to(dev), value.to(dev), table.to(dev), n, mask.to(dev), scale=0.31)
+    check(got, BF, q, key, value, table, lens, mask, 0.31)
+
+
+def test_rows_that_admit_nothing_are_zero(C, dev):
+    _, q, key, value, table, lens, n, mask = _small(dev)
+    mask[1, 2] = 0
+    mask[2, 1] = 0
+    got = C.attn_paged(q.to(dev), key.to(dev), value.to(dev), table.to(dev), n, mask.to(dev))
+    assert (got[1, 2] == 0).all() and (got[2, 1] != 0).any()
+    check(got, BF, q, key, value, table, lens, mask, 128 ** -0.5)
+
+
+@pytest.mark.parametrize("T,S", [(16, 4), (64, 20)])
+def test_bad_pages_are_not_attended(C, dev, T, S):
+    """Entries that are no page (negative, past the pool) inside and behind the prefix, a sequence without pages, lengths out of
+    range: nothing of them is read, the other tokens count as ever."""
+    g, q, key, value, table, lens, n, mask = _small(dev, T=T, lens=(5 * T + 3, T, 2 * T, 0), S=S)
+    P = key.shape[1]
+    table[0, 1], table[0, 3], table[1, 0], table[2] = -7, P, 2 ** 31 - 1, -1
+    table[3, 0] = P + 3
+    got = C.attn_paged(q.to(dev), key.to(dev), value.to(dev), table.to(dev), n, mask.to(dev))
+    check(got, BF, q, key, value, table, lens, mask, 128 ** -0.5)
+    assert (got[2] == 0).all() and (got[3] == 0).all()
+    n2 = torch.tensor([-5, 2 ** 31 - 1, -2 ** 31, 0], dtype=torch.int32, device=dev)
+    W = table.shape[1]
+    got = C.attn_paged(q.to(dev), torch.zeros_like(key).to(dev), torch.ones_like(value).to(dev), table.to(dev), n2, mask.to(dev))
+    assert got.isfinite().all()
+    assert W * T < 2 ** 30
+
+
+@pytest.mark.parametrize("dt", [BF, FH])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_non_finite_in_places_that_are_not_admitted(C, dev, dt, D, bad):
+    """K and V of one own row non-finite: the rows that do not admit it are as without it; a row that admits it shows it."""
+    _, q, key, value, table, lens, n, _ = _small(dev, dt=dt, D=D, lens=(40, 0, 31), S=4)
+    mask = torch.tensor([[1, 3, 5, 9]] * 3)  # rows 1, 2, 3 children of 0
+    for b, t in enumerate(lens):
+        key[:, table[b, (t + 2) // 16], (t + 2) % 16] = bad
+        value[:, table[b, (t + 2) // 16], (t + 2) % 16] = bad
+    got = C.attn_paged(q.to(dev), key.to(dev), value.to(dev), table.to(dev), n, mask.to(dev)).cpu()
+    clean_k, clean_v = key.nan_to_num(0, 0, 0), value.nan_to_num(0, 0, 0)
+    check(got, dt, q, clean_k, clean_v, table, lens, mask, D ** -0.5, rows=[0, 1, 3])
+    assert not got[:, 2].isfinite().all(-1).any()
+
+
+def test_non_finite_values_that_are_admitted(C, dev):
+    """An infinite value of the prefix reaches every row, with its sign; a NaN makes that dim NaN and no other."""
+    _, q, key, value, table, lens, n, mask = _small(dev, lens=(40, 0, 33))
+    value[:, table[0, 0], 3, 5] = float("inf")
+    value[:, table[0, 2], 1, 9] = float("nan")
+    got = C.attn_paged(q.to(dev), key.to(dev), value.to(dev), table.to(dev), n, mask.to(dev)).cpu().float()
+    assert (got[0, :, :, 5] == float("inf")).all() and got[0, :, :, 9].isnan().all()
+    rest = [d for d in range(128) if d not in (5, 9)]
+    assert got[0][..., rest].isfinite().all() and got[1:].isfinite().all()
+
+
+def test_large_scores(C, dev):
+    """One token far above the others takes the row, whatever stands before it."""
+    _, q, key, value, table, lens, n, mask = _small(dev, lens=(200, 100, 33), S=1)
+    q, key = q * 30, key
+    got = C.attn_paged(q.to(dev), key.to(dev), value.to(dev), table.to(dev), n, mask.to(dev))
+    check(got, BF, q, key, value, table, lens, mask, 128 ** -0.5)
+
+
+def test_same_bits_again_and_on_another_stream(C, dev):
+    _, q, key, value, table, lens, n, mask = _small(dev, lens=(3000, 10, 500))
+    a = [x.to(dev) for x in (q, key, value, table)] + [n, mask.to(dev)]
+    one = C.attn_paged(*a)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        two = [C.attn_paged(*a) for _ in range(3)]
+    main = [C.attn_paged(*a) for _ in range(3)]  # both streams at once: each call has a workspace of its own
+    torch.cuda.synchronize()
+    assert all(torch.equal(one, x) for x in two + main)
+
+
+def test_graph_replay_follows_the_lengths(C, dev):
+    """Two captured calls (their workspaces apart) replayed in turn and over lengths and tables written between replays."""
+    _, q, key, value, table, lens, n, mask = _small(dev, lens=(400, 64, 33), S=2)
+    qd, kd, vd, td, md = (x.to(dev) for x in (q, key, value, table, mask))
+    C.attn_paged(qd, kd, vd, td, n, md)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for m in (md, None):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(C.attn_paged(qd, kd, vd, td, n, m))
+        graphs.append(gr)
+    for now in ((400, 64, 33), (1, 0, 20), (399, 60, 33), (17, 33, 0)):
+        n.copy_(torch.tensor(now, dtype=torch.int32))
+        for gr in graphs:
+            gr.replay()
+        torch.cuda.synchronize()
+        for o, m in zip(outs, (md, None)):
+            want = C.attn_paged(qd, kd, vd, td, n, m)
+            assert torch.equal(o, want), now
+
+
+def test_offsets_past_32_bits(C, dev):
+    """A pool of more than 4 GiB a matrix, the sequence in its last pages."""
+    T, D, P = 64, 128, 270000
+    pool = torch.empty(2, 1, P, T, D, dtype=BF, device=dev)
+    g = torch.Generator().manual_seed(4)
+    n = 150
+    table = torch.tensor([[P - 1, P - 3, P - 2, -1]], dtype=torch.int32)
+    small = torch.full((2, 1, 4, T, D), float("nan")).to(BF)
+    small_table = torch.tensor([[3, 1, 2, -1]], dtype=torch.int32)
+    t = torch.arange(n + 1)
+    for i in range(2):
+        small[i][:, small_table[0].long()[t // T], t % T] = torch.randn(1, n + 1, D, generator=g).to(BF)
+    pool[:, :, P - 4:] = small.to(dev)
+    q = torch.randn(1, 1, 4, D, generator=g).to(BF)
+    length = torch.tensor([n], dtype=torch.int32, device=dev)
+    got = C.attn_paged(q.to(dev), pool[0], pool[1], table.to(dev), length)
+    check(got, BF, q, small[0], small[1], small_table, [n], None, D ** -0.5)
+
+
+def test_refusals(C, dev):
+    _, q, key, value, table, lens, n, mask = _small(dev)
+    q, key, value, table, mask = (x.to(dev) for x in (q, key, value, table, mask))
+    for args, kw, match in [((q.float(), key, value, table, n), {}, "bf16 or fp16"), ((q, key.half(), value, table, n), {}, "one type"),
+                            ((q[:, :, :7], key, value, table, n), {}, "multiple"), ((q, key, value[:, 1:], table, n), {}, "head_dim"),
+                            ((q, key, value, table.long(), n), {}, "int32"), ((q, key, value, table[:2], n), {}, "table"),
+                            ((q, key, value, table, n[:2]), {}, "length"), ((q, key, value, table, n.long()), {}, "int32"),
+                            ((q, key, value, table, n, mask.int()), {}, "mask"), ((q, key, value, table, n, mask[:, :3]), {}, "mask"),
+                            ((q, key, value, table, n, mask.cpu()), {}, "same ROCm device"), ((q, key, value, table, n), dict(scale=-1.0), "scale"),
+                            ((q, key, value, table, n), dict(out=q[:, :, :4]), "out"), ((q[0], key, value, table, n), {}, "q:"),
+                            ((q.transpose(2, 3), key, value, table, n), {}, "contiguous")]:
+        with pytest.raises(RuntimeError, match=match):
+            C.attn_paged(*args, **kw)
