@@ -22,6 +22,8 @@
 // Reference: none for the pages; the rows' contract is csrc/attn_dpas.sycl:269-342's.
 #include <math.h>
 
+#include <atomic>
+
 #include "mdx_common.hpp"
 
 namespace mdx {
@@ -639,57 +641,82 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int rpw) {
 // ---- the selection ----------------------------------------------------------------------------------------
 // Scores of the full pages between the forced ones: (sum of the group's queries) . mean key, in float64 (the order of
 // scores decides, and 32-bit sums in another order would swap neighbours), as keys whose unsigned order is the scores'
-// (NaN lowest). One thread per page, the queries' sums in LDS.
-constexpr int SCORE_ROWS = 8;
+// (NaN lowest). Products of 16 rows and 16 pages by v_mfma_f64_16x16x4 (A: lane (row c16, k g), B: lane (page c16, k g),
+// the four dims of a product being dim e of the four 8-dim pieces that the lanes of a page hold; D: lane (row 4 r + g, page
+// c16) in element r): a wave takes 16 pages, so the longest context spreads over all CUs. (One thread per page on the vector
+// units: 94.8 us for 8 rows over 250 pages of head_dim 256, 21 us for 1 row over 2046 of 128.)
+constexpr int SCORE_ROWS = 16;
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+typedef double f64x2 __attribute__((ext_vector_type(2)));
 template <class E, int D>
 __global__ __launch_bounds__(256) void block_score_kernel(PagedArgs a) {
-    __shared__ double qs[SCORE_ROWS][D];
+    constexpr int QR = D + 2;  // (rows two doubles further apart: no bank conflicts)
+    __shared__ __align__(16) double qs[SCORE_ROWS * QR];
     const int b = blockIdx.z / a.Hk, kh = blockIdx.z % a.Hk, s0 = blockIdx.y * SCORE_ROWS, ns = min(SCORE_ROWS, a.S - s0);
-    const int c = span_of<true>(a, a.length[b]).tail >> a.lt;
-    const int j = a.sink + int(blockIdx.x) * 256 + int(threadIdx.x), j_end = c - a.local;
-    if (c <= a.most || a.sink + int(blockIdx.x) * 256 >= j_end) return;  // (uniform; all pages are selected, or none is scored here)
+    const int c = span_of<true>(a, a.length[b]).tail >> a.lt, j_end = c - a.local;
+    if (c <= a.most || a.sink + int(blockIdx.x) * 64 >= j_end) return;  // (uniform: all pages are selected, or none is scored here)
+    const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
+    const int j = a.sink + int(blockIdx.x) * 64 + int(threadIdx.x >> 6) * 16 + c16;
+    const int e = j < j_end ? a.table[b * a.ts + j] : -1;
+    const bool in = e >= 0 && e < a.P;
+    u32x4 k[D / 32];  // (the page's mean key goes out ahead of the queries; a page that is none reads page 0)
+    const uint16_t* kp = a.ksum + kh * a.sh + (in ? e : 0) * a.sp + 8 * g;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) k[i] = *reinterpret_cast<const u32x4*>(kp + 32 * i);
     for (int i = threadIdx.x; i < ns * D; i += 256) {
         const int s = i / D, d = i % D;
         const uint16_t* p = a.q + b * a.qb + (s0 + s) * a.qs + kh * a.G * a.qh + d;
         double t = 0;
+#pragma unroll 4
         for (int h = 0; h < a.G; ++h) t += double(E::to_f32(p[h * a.qh]));
-        qs[s][d] = t;
+        qs[s * QR + d] = t;
     }
     __syncthreads();
+    const double* q = qs + min(c16, ns - 1) * QR + 8 * g;  // (rows past the last repeat it: their products are not written)
+    f64x4 dot = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const f64x2 qq = *reinterpret_cast<const f64x2*>(q + 32 * i + 2 * x);
+            dot = __builtin_amdgcn_mfma_f64_16x16x4f64(qq[0], double(E::to_f32(uint16_t(k[i][x] & 0xFFFFu))), dot, 0, 0, 0);
+            dot = __builtin_amdgcn_mfma_f64_16x16x4f64(qq[1], double(E::to_f32(uint16_t(k[i][x] >> 16))), dot, 0, 0, 0);
+        }
     if (j >= j_end) return;
-    const int e = a.table[b * a.ts + j];
-    double dot[SCORE_ROWS];
 #pragma unroll
-    for (int s = 0; s < SCORE_ROWS; ++s) dot[s] = 0;
-    const bool in = e >= 0 && e < a.P;
-    if (in) {
-        const uint16_t* k = a.ksum + kh * a.sh + e * a.sp;
-        for (int d = 0; d < D; d += 8) {
-            const u32x4 v = *reinterpret_cast<const u32x4*>(k + d);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const double x = double(E::to_f32(uint16_t(v[i / 2] >> (16 * (i & 1)))));
-#pragma unroll
-                for (int s = 0; s < SCORE_ROWS; ++s)
-                    if (s < ns) dot[s] = fma(x, qs[s][d + i], dot[s]);
-            }
-        }
+    for (int r = 0; r < 4; ++r) {
+        const int s = 4 * r + g;
+        const double z = dot[r] + 0.0;  // (-0 and 0 are one score)
+        const uint64_t u = __builtin_bit_cast(uint64_t, z);
+        if (s < ns)
+            a.keys[((int64_t(b) * a.S + s0 + s) * a.Hk + kh) * a.W + j] = !in || z != z ? 0 : (u >> 63 ? ~u : u | (uint64_t(1) << 63));
     }
+}
+
+__device__ __forceinline__ int wave_incl_sum(int v, int lane) {
 #pragma unroll
-    for (int s = 0; s < SCORE_ROWS; ++s)
-        if (s < ns) {
-            const double z = dot[s] + 0.0;  // (-0 and 0 are one score)
-            const uint64_t u = __builtin_bit_cast(uint64_t, z);
-            a.keys[((int64_t(b) * a.S + s0 + s) * a.Hk + kh) * a.W + j] =
-                !in || z != z ? 0 : (u >> 63 ? ~u : u | (uint64_t(1) << 63));
-        }
+    for (int d = 1; d < 64; d <<= 1) {
+        const int u = __shfl_up(v, d, 64);
+        if (lane >= d) v += u;
+    }
+    return v;
 }
 
 // The `blocks` best of the scored pages (ties to the lowest index) and the forced ones, ascending: one work-group per
-// (sequence, row, kv head). The threshold by bytes from the top (a histogram in LDS per byte, stopping where a byte's
-// pages are all taken), then one pass in index order.
-__global__ __launch_bounds__(256) void block_select_kernel(PagedArgs a) {
-    __shared__ int hist[256], tmp[4], pick[3];
+// (sequence, row, kv head), the keys in registers (W <= NT EACH; past 16 per thread they are read again). The threshold: a histogram of 1024 bins over the range
+// that the keys' upper words span, then the keys of the one bin that holds it by their ranks; where that bin has more than
+// NT keys (ties), by bytes from the top instead. Then one pass in index order. Bound by latency (barriers and LDS): 9 us
+// with a byte-wise threshold and a barrier pair per NT keys of the last pass, at 2046 pages.
+template <int NT, int EACH>
+__global__ __launch_bounds__(NT) void block_select_kernel(PagedArgs a) {
+    constexpr int NW = NT / 64, BINS = 1024;
+    constexpr bool REG = EACH <= 16;
+    constexpr int U = REG ? EACH : 1;
+    __shared__ int hist[BINS];
+    __shared__ int tmp[NW], pick[3], found;
+    __shared__ uint32_t lo_w[NW], hi_w[NW];
+    __shared__ uint64_t cand[NT], thr;
+    __shared__ int pre[2][NW * EACH];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const int64_t unit = blockIdx.x;
     const int b = int(unit / (int64_t(a.S) * a.Hk));
@@ -698,89 +725,181 @@ __global__ __launch_bounds__(256) void block_select_kernel(PagedArgs a) {
     int32_t* page = a.page + unit * a.most;
     const int32_t* row = a.table + b * a.ts;
     if (c <= a.most) {  // every full page
-        for (int i = tid; i < a.most; i += 256) {
+        for (int i = tid; i < a.most; i += NT) {
             sel[i] = i < c ? i : -1;
             page[i] = i < c ? row[i] : -1;
         }
         return;
     }
-    const uint64_t* keys = a.keys + unit * a.W;
     const int j0 = a.sink, j1 = c - a.local, want = a.most - a.sink - a.local;
-    uint64_t prefix = 0;  // the threshold's bytes so far
-    int left = want, shift = 64;
-    bool exact = want == 0;  // every page of the last byte's bin is taken
-    while (!exact && shift > 0) {
-        shift -= 8;
-        hist[tid] = 0;
-        __syncthreads();
-        for (int j = j0 + tid; j < j1; j += 256) {
-            const uint64_t k = keys[j];
-            if (shift == 56 || (k >> (shift + 8)) == prefix) atomicAdd(&hist[int(k >> shift) & 255], 1);
-        }
-        __syncthreads();
-        // the bin that holds the left-th from the top: sums from bin 255 downwards
-        int v = hist[255 - tid];
-        const int own = v;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int u = __shfl_up(v, d, 64);
-            if (lane >= d) v += u;
-        }
-        if (lane == 63) tmp[w] = v;
-        __syncthreads();
-        for (int i = 0; i < w; ++i) v += tmp[i];
-        if (v >= left && v - own < left) {
-            pick[0] = 255 - tid;
-            pick[1] = left - (v - own);
-            pick[2] = own;
-        }
-        __syncthreads();
-        prefix = (prefix << 8) | uint64_t(pick[0]);
-        left = pick[1];
-        exact = pick[2] == left;
-    }
-    // pages whose key's first bytes lie above the prefix, and `left` of those at it (all of them, or the first in order)
-    int taken = 0, ties = 0;  // (running counts, uniform)
-    for (int i = tid; i < a.sink; i += 256) {
+    for (int i = tid; i < a.sink; i += NT) {
         sel[i] = i;
         page[i] = row[i];
     }
-    for (int i = tid; i < a.local; i += 256) {
+    for (int i = tid; i < a.local; i += NT) {
         sel[a.sink + want + i] = j1 + i;
         page[a.sink + want + i] = row[j1 + i];
     }
     if (want == 0) return;
-    for (int base = j0; base < j1; base += 256) {
-        const int j = base + tid;
-        const uint64_t k = j < j1 ? keys[j] >> shift : 0;
-        const bool above = j < j1 && k > prefix, at = j < j1 && k == prefix;
-        const uint64_t ma = __builtin_amdgcn_ballot_w64(above), mt = __builtin_amdgcn_ballot_w64(at);
-        const uint64_t under = (uint64_t(1) << lane) - 1;
-        __syncthreads();
-        if (lane == 0) {
-            hist[w] = __popcll(ma);
-            hist[4 + w] = __popcll(mt);
-        }
-        __syncthreads();
-        int na = 0, nt = 0, all_a = 0, all_t = 0;
+    const uint64_t* keys = a.keys + unit * a.W;
+    uint64_t kept[U];
+    uint32_t lo = 0xFFFFFFFFu, hi = 0;
+    if constexpr (REG)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            na += i < w ? hist[i] : 0;
-            nt += i < w ? hist[4 + i] : 0;
-            all_a += hist[i];
-            all_t += hist[4 + i];
+        for (int i = 0; i < EACH; ++i) {
+            const int j = j0 + i * NT + tid;
+            kept[i] = j < j1 ? keys[j] : 0;
         }
-        na += __popcll(ma & under);
-        nt += __popcll(mt & under);
-        // its place: pages above before it, and of the ties before it those that are taken
-        const bool take = above || (at && ties + nt < left);
-        if (take) {
-            const int to = a.sink + taken + na + min(ties + nt, left);
+    auto live = [&](int i) { return j0 + i * NT + tid < j1; };
+    auto key = [&](int i) -> uint64_t {
+        if constexpr (REG) return kept[i];
+        return live(i) ? keys[j0 + i * NT + tid] : 0;
+    };
+#pragma unroll U
+    for (int i = 0; i < EACH; ++i)
+        if (live(i)) {
+            const uint32_t x = uint32_t(key(i) >> 32);
+            lo = min(lo, x);
+            hi = max(hi, x);
+        }
+    for (int d = 32; d; d >>= 1) {
+        lo = min(lo, uint32_t(__shfl_xor(int(lo), d, 64)));
+        hi = max(hi, uint32_t(__shfl_xor(int(hi), d, 64)));
+    }
+    for (int i = tid; i < BINS; i += NT) hist[i] = 0;
+    if (lane == 0) {
+        lo_w[w] = lo;
+        hi_w[w] = hi;
+    }
+    if (tid == 0) found = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+        lo = min(lo, lo_w[i]);
+        hi = max(hi, hi_w[i]);
+    }
+    const int sh = max(0, 22 - int(__builtin_clz((hi - lo) | 1u)));  // (hi - lo) >> sh < 1024
+    auto bin = [&](uint64_t x) { return int((uint32_t(x >> 32) - lo) >> sh); };
+#pragma unroll U
+    for (int i = 0; i < EACH; ++i)
+        if (live(i)) atomicAdd(&hist[bin(key(i))], 1);
+    __syncthreads();
+    // the bin that holds the want-th key from the top
+    {
+        constexpr int PB = BINS / NT;  // bins per thread, from the top
+        int sum = 0;
+#pragma unroll
+        for (int i = 0; i < PB; ++i) sum += hist[BINS - 1 - (tid * PB + i)];
+        const int incl = wave_incl_sum(sum, lane);
+        if (lane == 63) tmp[w] = incl;
+        __syncthreads();
+        int before = incl - sum;
+        for (int i = 0; i < w; ++i) before += tmp[i];
+#pragma unroll
+        for (int i = 0; i < PB; ++i) {
+            const int x = hist[BINS - 1 - (tid * PB + i)];
+            if (before < want && before + x >= want) {
+                pick[0] = BINS - 1 - (tid * PB + i);
+                pick[1] = want - before;
+                pick[2] = x;
+            }
+            before += x;
+        }
+    }
+    __syncthreads();
+    const int at_bin = pick[0], in_bin = pick[2];
+    int left = pick[1], shift = 0;
+    uint64_t prefix;
+    if (in_bin <= NT) {
+#pragma unroll U
+        for (int i = 0; i < EACH; ++i)
+            if (live(i) && bin(key(i)) == at_bin) cand[atomicAdd(&found, 1)] = key(i);
+        __syncthreads();
+        if (tid < in_bin) {  // (equal keys find the same threshold and count: whichever thread writes last)
+            const uint64_t mine = cand[tid];
+            int above = 0, same = 0;
+            for (int i = 0; i < in_bin; ++i) {
+                above += cand[i] > mine;
+                same += cand[i] == mine;
+            }
+            if (above < left && left <= above + same) {
+                thr = mine;
+                pick[1] = left - above;
+            }
+        }
+        __syncthreads();
+        prefix = thr;
+        left = pick[1];
+    } else {
+        // by bytes, among the keys of that bin; `left` of them are wanted
+        prefix = 0;
+        shift = 64;
+        bool exact = false;  // every key of the last byte's value is taken
+        while (!exact && shift > 0) {
+            shift -= 8;
+            __syncthreads();
+            for (int i = tid; i < 256; i += NT) hist[i] = 0;
+            __syncthreads();
+#pragma unroll U
+            for (int i = 0; i < EACH; ++i)
+                if (live(i) && bin(key(i)) == at_bin && (shift == 56 || (key(i) >> (shift + 8)) == prefix))
+                    atomicAdd(&hist[int(key(i) >> shift) & 255], 1);
+            __syncthreads();
+            if (w == 0) {  // four bytes' values per lane, from 255 downwards
+                int v[4], sum = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum += v[i] = hist[255 - (lane * 4 + i)];
+                int before = wave_incl_sum(sum, lane) - sum;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (before < left && before + v[i] >= left) {
+                        pick[0] = 255 - (lane * 4 + i);
+                        pick[1] = left - before;
+                        pick[2] = v[i];
+                    }
+                    before += v[i];
+                }
+            }
+            __syncthreads();
+            prefix = (prefix << 8) | uint64_t(pick[0]);
+            left = pick[1];
+            exact = pick[2] == left;
+        }
+    }
+    // keys above the threshold (a higher bin, or its bin and higher in the bytes above `shift`), and `left` of those at it, the
+    // first in index order
+    auto side = [&](int i) { return !live(i) || bin(key(i)) < at_bin ? 0 : bin(key(i)) > at_bin || (key(i) >> shift) > prefix ? 2 : (key(i) >> shift) == prefix ? 1 : 0; };
+#pragma unroll U
+    for (int i = 0; i < EACH; ++i) {
+        const int x = side(i);
+        const uint64_t above = __builtin_amdgcn_ballot_w64(x == 2), ties = __builtin_amdgcn_ballot_w64(x == 1);
+        if (lane == 0) {
+            pre[0][i * NW + w] = __popcll(above);
+            pre[1][i * NW + w] = __popcll(ties);
+        }
+    }
+    __syncthreads();
+    if (w < 2) {  // exclusive sums over (i, wave), in index order
+        int carry = 0;
+        for (int r = 0; r < NW * EACH; r += 64) {
+            const int x = r + lane < NW * EACH ? pre[w][r + lane] : 0;
+            const int incl = wave_incl_sum(x, lane);
+            if (r + lane < NW * EACH) pre[w][r + lane] = carry + incl - x;
+            carry += __shfl(incl, 63, 64);
+        }
+    }
+    __syncthreads();
+    const uint64_t under = (uint64_t(1) << lane) - 1;
+#pragma unroll U
+    for (int i = 0; i < EACH; ++i) {
+        const int x = side(i);
+        const uint64_t above = __builtin_amdgcn_ballot_w64(x == 2), tie = __builtin_amdgcn_ballot_w64(x == 1);
+        const int ties = pre[1][i * NW + w] + __popcll(tie & under);
+        if (x == 2 || (x == 1 && ties < left)) {
+            const int j = j0 + i * NT + tid, to = a.sink + pre[0][i * NW + w] + __popcll(above & under) + min(ties, left);
             sel[to] = j;
             page[to] = row[j];
         }
-        taken += all_a;
-        ties += all_t;
     }
 }
 
@@ -790,8 +909,15 @@ int launch(const PagedArgs& a, hipStream_t st) {
     using Geo = Geometry<E, D, TPW, RTW, P, SEL>;
     constexpr int joined = (RTW * P * 16 * (D + 4) + 2 * RTW * P * 16) * 4;
     constexpr int lds = RING_BYTES > joined ? RING_BYTES : joined;
-    const void* fn = reinterpret_cast<const void*>(&paged_attn_kernel<E, D, TPW, RTW, P, SEL>);
-    allow_smem(fn, lds);
+    // (once per device and kernel: the call costs about a microsecond)
+    static std::atomic<uint64_t> allowed{0};
+    int dev = 0;
+    MDX_HIP(hipGetDevice(&dev));
+    const uint64_t bit = uint64_t(1) << (dev & 63);
+    if (dev > 63 || !(allowed.load(std::memory_order_relaxed) & bit)) {
+        allow_smem(reinterpret_cast<const void*>(&paged_attn_kernel<E, D, TPW, RTW, P, SEL>), lds);
+        allowed.fetch_or(bit, std::memory_order_relaxed);
+    }
     hipLaunchKernelGGL((paged_attn_kernel<E, D, TPW, RTW, P, SEL>), dim3(GRID), dim3(Geo::NT), lds, st, a);
     MDX_LAUNCHED();
     const int rows = a.rows < Geo::RPW ? a.rows : Geo::RPW;
@@ -951,6 +1077,7 @@ extern "C" int mdx_attn_blocks(const void* q, int64_t q_seq_stride, int64_t q_ro
     if (rc != MDX_OK) return rc;
     const int64_t most = blocks + sink + local, units = B * S * Hk;
     MDX_CHECK(H / Hk <= 64, "at most 64 query heads per kv head");
+    MDX_CHECK(W <= 65536, "at most 65536 pages a sequence");
     MDX_CHECK(B * Hk <= 65535 && units < (int64_t(1) << 24) && units * (((most < W ? most : W) + 1) * T + S) / STEP + units < (int64_t(1) << 31),
               "too many rows times tokens for one call");
     const size_t need = mdx_attn_blocks_workspace(B, S, H, Hk, D, W, most);
@@ -967,7 +1094,7 @@ extern "C" int mdx_attn_blocks(const void* q, int64_t q_seq_stride, int64_t q_ro
     a.page = reinterpret_cast<int32_t*>(a.keys + units * W);
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (W > most) {  // (else every full page is selected)
-        const dim3 grid(unsigned((W + 255) / 256), unsigned((S + SCORE_ROWS - 1) / SCORE_ROWS), unsigned(B * Hk));
+        const dim3 grid(unsigned((W + 63) / 64), unsigned((S + SCORE_ROWS - 1) / SCORE_ROWS), unsigned(B * Hk));
         if (dtype == MDX_DT_BF16) {
             if (D == 64) hipLaunchKernelGGL((block_score_kernel<Bf16, 64>), grid, dim3(256), 0, st, a);
             else if (D == 128) hipLaunchKernelGGL((block_score_kernel<Bf16, 128>), grid, dim3(256), 0, st, a);
@@ -979,7 +1106,11 @@ extern "C" int mdx_attn_blocks(const void* q, int64_t q_seq_stride, int64_t q_ro
         }
         MDX_LAUNCHED();
     }
-    hipLaunchKernelGGL(block_select_kernel, dim3(unsigned(units)), dim3(256), 0, st, a);
+    // (keys in registers: the smallest form that holds a row's)
+    if (W <= 1024) hipLaunchKernelGGL((block_select_kernel<256, 4>), dim3(unsigned(units)), dim3(256), 0, st, a);
+    else if (W <= 4096) hipLaunchKernelGGL((block_select_kernel<512, 8>), dim3(unsigned(units)), dim3(512), 0, st, a);
+    else if (W <= 16384) hipLaunchKernelGGL((block_select_kernel<1024, 16>), dim3(unsigned(units)), dim3(1024), 0, st, a);
+    else hipLaunchKernelGGL((block_select_kernel<1024, 64>), dim3(unsigned(units)), dim3(1024), 0, st, a);
     MDX_LAUNCHED();
     return launch_any<true>(a, int(D), dtype, st);
 }

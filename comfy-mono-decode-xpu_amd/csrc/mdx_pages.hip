@@ -22,6 +22,7 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 constexpr int PLAN_T = 1024;      // threads of the planning work-group
 constexpr int MAX_SEQS = 1024;    // pairs of a fork, sequences of a commit: one planning thread each
 constexpr int MAX_PATH = 64;      // rows of a committed path
+constexpr int SUM_T = PLAN_T;     // threads of a work-group of commit's second launch
 
 // ---- the free pages -------------------------------------------------------------------------------------
 // Inclusive sum over the work-group's threads (16 waves), and the total; `tmp` of 16 ints. Every thread calls it.
@@ -105,9 +106,53 @@ __device__ __forceinline__ int clamp_len(int n, int W, int lt) {
     return n < 0 ? 0 : (n > most ? most : n);
 }
 
-// Plan: one thread per pair. Pages of old rows are released by the last launch, so pages given out here are never ones
+// New table rows, the references they add, the list of copies: `nt` threads (t of them, whole waves) for pair i.
+__device__ void fork_rows(const ForkArgs& a, int i, int t, int nt) {
+    const int4 p = reinterpret_cast<const int4*>(a.pair)[i];
+    if (p.x != 1) return;
+    const int d = a.dst[i], s = a.src[i], n = p.y;
+    const int full = n >> a.lt, used = (n + a.T - 1) >> a.lt, total = int((int64_t(n) + a.room + a.T - 1) >> a.lt);
+    int32_t* row = a.rows + int64_t(i) * a.W;
+    if (s == d) {
+        // (its missing entries in order: the whole row by the first wave, a ballot per 64 entries)
+        if (t >= 64) return;
+        int given = p.z;
+        for (int j0 = 0; j0 < a.W; j0 += 64) {
+            const int j = j0 + t;
+            int e = j < a.W ? a.table[d * a.ts + j] : -1;
+            const bool miss = j < a.W && j >= full && j < total && e < 0;
+            const uint64_t m = __builtin_amdgcn_ballot_w64(miss);
+            if (miss) {
+                e = a.fresh[given + __popcll(m & ((uint64_t(1) << t) - 1))];
+                a.refs[e] = 1;
+            }
+            given += __popcll(m);
+            if (j < a.W) row[j] = e;
+        }
+        return;
+    }
+    const int kept = a.share ? full : 0;
+    for (int j = t; j < a.W; j += nt) {
+        int e = -1;
+        if (j < used) e = a.table[s * a.ts + j];
+        if (j < kept) {
+            if (e >= 0 && e < a.P) atomicAdd(a.refs + e, 1);
+            else e = -1;
+        } else if (j < total) {
+            const int from = e;
+            e = a.fresh[p.z + j - kept];
+            a.refs[e] = 1;
+            if (j < used)  // (an entry that is no page leaves its copy as it was)
+                a.copies[p.w + j - kept] = make_int2(from >= 0 && from < a.P ? from : -1, e);
+        }
+        row[j] = e;
+    }
+}
+__global__ __launch_bounds__(256) void fork_rows_kernel(ForkArgs a) { fork_rows(a, blockIdx.x, threadIdx.x, 256); }
+
+// Plan: one thread per pair; with `rows` (few pairs and entries) the new rows in the same launch, a wave per pair. Pages of old rows are released by the last launch, so pages given out here are never ones
 // that a copy still reads.
-__global__ __launch_bounds__(PLAN_T) void fork_plan_kernel(ForkArgs a) {
+__global__ __launch_bounds__(PLAN_T) void fork_plan_kernel(ForkArgs a, int rows) {
     __shared__ int tmp[PLAN_T / 64];
     __shared__ int sdst[MAX_SEQS];
     const int i = threadIdx.x;
@@ -142,50 +187,9 @@ __global__ __launch_bounds__(PLAN_T) void fork_plan_kernel(ForkArgs a) {
         a.status[i] = valid ? (served ? 1 : 0) : -1;
     }
     if (i == 0) a.head[0] = all;
-}
-
-// New table rows, the references they add, the list of copies: one work-group per pair.
-__global__ __launch_bounds__(256) void fork_rows_kernel(ForkArgs a) {
-    const int i = blockIdx.x;
-    const int4 p = reinterpret_cast<const int4*>(a.pair)[i];
-    if (p.x != 1) return;
-    const int d = a.dst[i], s = a.src[i], n = p.y;
-    const int full = n >> a.lt, used = (n + a.T - 1) >> a.lt, total = int((int64_t(n) + a.room + a.T - 1) >> a.lt);
-    int32_t* row = a.rows + int64_t(i) * a.W;
-    if (s == d) {
-        // (its missing entries in order: the whole row by wave 0, a ballot per 64 entries)
-        if (threadIdx.x >= 64) return;
-        int given = p.z;
-        for (int j0 = 0; j0 < a.W; j0 += 64) {
-            const int j = j0 + int(threadIdx.x);
-            int e = j < a.W ? a.table[d * a.ts + j] : -1;
-            const bool miss = j < a.W && j >= full && j < total && e < 0;
-            const uint64_t m = __builtin_amdgcn_ballot_w64(miss);
-            if (miss) {
-                e = a.fresh[given + __popcll(m & ((uint64_t(1) << threadIdx.x) - 1))];
-                a.refs[e] = 1;
-            }
-            given += __popcll(m);
-            if (j < a.W) row[j] = e;
-        }
-        return;
-    }
-    const int kept = a.share ? full : 0;
-    for (int j = threadIdx.x; j < a.W; j += 256) {
-        int e = -1;
-        if (j < used) e = a.table[s * a.ts + j];
-        if (j < kept) {
-            if (e >= 0 && e < a.P) atomicAdd(a.refs + e, 1);
-            else e = -1;
-        } else if (j < total) {
-            const int from = e;
-            e = a.fresh[p.z + j - kept];
-            a.refs[e] = 1;
-            if (j < used)  // (an entry that is no page leaves its copy as it was)
-                a.copies[p.w + j - kept] = make_int2(from >= 0 && from < a.P ? from : -1, e);
-        }
-        row[j] = e;
-    }
+    if (!rows) return;  // (uniform)
+    __syncthreads();
+    for (int x = i >> 6; x < a.M; x += PLAN_T / 64) fork_rows(a, x, i & 63, 64);
 }
 
 // The copies (work-groups past the pairs', in pieces of 16 KiB) and, by the first `pairs` work-groups, what the call
@@ -263,41 +267,43 @@ struct CommitArgs {
     int32_t* status;
     int B, W, P, T, lt, D, L, Hk, R, room, half;  // half: fp16 elements, else bf16
     int per_wg;           // chunks a work-group of the move takes
+    int32_t* state;       // [B]: a sequence's tokens before the commit, -1 where it is refused or left alone (the first launch's)
     int32_t* fresh;
 };
 
-// A sequence whose rows can be committed: its tokens, or -1. The path is checked by its callers.
-__device__ __forceinline__ int commit_tokens(const CommitArgs& a, int b) {
-    const int c = a.count[b], n = a.length[b];
-    if (c < 0 || n < 0 || (a.path && c > a.R) || int64_t(n) + c > int64_t(a.W) << a.lt) return -1;
-    return n;
-}
 __device__ __forceinline__ int page_at(const CommitArgs& a, int b, int64_t t) {
     const int64_t j = t >> a.lt;
     const int e = j < a.W ? a.table[b * a.ts + j] : -1;
     return e >= 0 && e < a.P ? e : -1;
 }
 
-// Rows n + path[k] to n + k. A work-group holds every row of its chunks in registers before it writes one, so no order
-// among the rows matters; chunks do not meet. Bound by latency (three dependent round trips), hence many small
-// work-groups: 32 sequences of 8 rows over 128 chunks are 512.
+// First launch: which sequences can be committed (`state`: the second launch may overwrite the lengths), and rows
+// n + path[k] to n + k. Work-group (x, b); every one checks its sequence for itself. One holds every row of its chunks in
+// registers before it writes one, so no order among the rows matters; chunks do not meet. Bound by latency (dependent
+// round trips), hence many small work-groups: 32 sequences of 8 rows over 128 chunks are 1024.
 __global__ __launch_bounds__(256) void commit_move_kernel(CommitArgs a) {
     __shared__ int64_t from[MAX_PATH], to[MAX_PATH];
     __shared__ int bad;
-    const int b = blockIdx.y, n = commit_tokens(a, b), c = a.count[b], t = threadIdx.x;
-    if (n < 0 || c <= 0) return;  // (uniform)
-    if (t == 0) bad = 0;
+    const int b = blockIdx.y, n = a.length[b], c = a.count[b], t = threadIdx.x;
+    const bool fits = c >= 0 && n >= 0 && !(a.path && c > a.R) && int64_t(n) + c <= int64_t(a.W) << a.lt;
+    if (t == 0) bad = !fits;
     __syncthreads();
-    if (t < c) {
-        const int32_t* path = a.path + int64_t(b) * a.R;
-        const int k = path[t], before = t ? path[t - 1] : -1;
-        const int p = k >= 0 && k < a.R ? page_at(a, b, int64_t(n) + k) : -1, q = page_at(a, b, int64_t(n) + t);
-        from[t] = k == t ? -1 : (int64_t(p) << a.lt) + ((n + k) & (a.T - 1));
-        to[t] = (int64_t(q) << a.lt) + ((n + t) & (a.T - 1));
-        if (k <= before || p < 0 || q < 0) bad = 1;
+    if (fits) {
+        if (a.path && t < c) {
+            const int32_t* path = a.path + int64_t(b) * a.R;
+            const int k = path[t], before = t ? path[t - 1] : -1;
+            const int p = k >= 0 && k < a.R ? page_at(a, b, int64_t(n) + k) : -1, q = page_at(a, b, int64_t(n) + t);
+            from[t] = k == t ? -1 : (int64_t(p) << a.lt) + ((n + k) & (a.T - 1));
+            to[t] = (int64_t(q) << a.lt) + ((n + t) & (a.T - 1));
+            if (k <= before || p < 0 || q < 0) bad = 1;
+        }
+        // the entries of the committed rows have to be pages
+        for (int j = (n >> a.lt) + t; j < (n + c + a.T - 1) >> a.lt; j += 256)
+            if (page_at(a, b, int64_t(j) << a.lt) < 0) bad = 1;
     }
     __syncthreads();
-    if (bad) return;
+    if (blockIdx.x == 0 && t == 0) a.state[b] = bad ? -1 : n;
+    if (bad || !a.path) return;  // (uniform)
     const int lanes = a.D / 8, items = c * lanes;  // 16-byte pieces of a chunk's rows
     const int chunks = a.L * 2 * a.Hk, c0 = blockIdx.x * a.per_wg;
     const int live = min(a.per_wg, chunks - c0) * items;
@@ -310,6 +316,7 @@ __global__ __launch_bounds__(256) void commit_move_kernel(CommitArgs a) {
     };
 #pragma unroll
     for (int i = 0; i < MOST; ++i) {
+        if (i * 256 >= live) break;  // (uniform)
         const int x = i * 256 + t;
         unsigned char* p = x < live ? place(x, from) : nullptr;
         if (p) v[i] = *reinterpret_cast<const u32x4*>(p);
@@ -317,6 +324,7 @@ __global__ __launch_bounds__(256) void commit_move_kernel(CommitArgs a) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < MOST; ++i) {
+        if (i * 256 >= live) break;
         const int x = i * 256 + t;
         unsigned char* p = x < live ? place(x, to) : nullptr;
         if (p) *reinterpret_cast<u32x4*>(p) = v[i];
@@ -332,17 +340,18 @@ __device__ __forceinline__ uint16_t to_el(float f, int half) {
 // (64 / (D / 8))-th row, fp32 sums, the row groups joined by lane exchanges, one rounding to the cache's type. The pages
 // of all sequences are numbered through (their counts summed in every work-group), so a batch of short tails and one
 // long prompt spread alike. Bound by the bytes of the keys.
-__global__ __launch_bounds__(256) void commit_sum_kernel(CommitArgs a) {
+__device__ void commit_sums(const CommitArgs& a, int block, int blocks) {
+    constexpr int EACH = MAX_SEQS / SUM_T;
     __shared__ int upto[MAX_SEQS];  // pages filled in sequences 0..b
-    __shared__ int wsum[4];
+    __shared__ int wsum[SUM_T / 64];
     const int t = threadIdx.x, lane = t & 63;
-    int mine[MAX_SEQS / 256], sum = 0;
+    int mine[EACH], sum = 0;
 #pragma unroll
-    for (int i = 0; i < MAX_SEQS / 256; ++i) {
-        const int b = t * (MAX_SEQS / 256) + i;
+    for (int i = 0; i < EACH; ++i) {
+        const int b = t * EACH + i;
         int f = 0;
         if (b < a.B) {
-            const int n = commit_tokens(a, b);
+            const int n = a.state[b];
             if (n >= 0) f = ((n + a.count[b]) >> a.lt) - (n >> a.lt);
         }
         sum += f;
@@ -359,12 +368,12 @@ __global__ __launch_bounds__(256) void commit_sum_kernel(CommitArgs a) {
     int before = incl - sum;
     for (int w = 0; w < (t >> 6); ++w) before += wsum[w];
 #pragma unroll
-    for (int i = 0; i < MAX_SEQS / 256; ++i) upto[t * (MAX_SEQS / 256) + i] = before + mine[i];
+    for (int i = 0; i < EACH; ++i) upto[t * EACH + i] = before + mine[i];
     __syncthreads();
     const int64_t keys = int64_t(a.L) * a.Hk, jobs = upto[MAX_SEQS - 1] * keys;
     const int lanes = a.D / 8, step = 64 / lanes, sub = lane / lanes, d8 = lane % lanes * 8;
     const float inv = 1.f / float(a.T);  // (a power of two: exact)
-    for (int64_t job = int64_t(blockIdx.x) * 4 + (t >> 6); job < jobs; job += int64_t(gridDim.x) * 4) {
+    for (int64_t job = int64_t(block) * (SUM_T / 64) + (t >> 6); job < jobs; job += int64_t(blocks) * (SUM_T / 64)) {
         const int page_no = int(job / keys);
         const int64_t kc = job % keys;
         int lo = 0, hi = a.B - 1;  // the sequence: the first whose sum passes page_no
@@ -373,7 +382,7 @@ __global__ __launch_bounds__(256) void commit_sum_kernel(CommitArgs a) {
             if (upto[mid] > page_no) hi = mid;
             else lo = mid + 1;
         }
-        const int j = (a.length[lo] >> a.lt) + page_no - (lo ? upto[lo - 1] : 0);
+        const int j = (a.state[lo] >> a.lt) + page_no - (lo ? upto[lo - 1] : 0);
         const int e = page_at(a, lo, int64_t(j) << a.lt);
         if (e < 0) continue;
         const int64_t layer = kc / a.Hk, h = kc % a.Hk;
@@ -404,12 +413,11 @@ __global__ __launch_bounds__(256) void commit_sum_kernel(CommitArgs a) {
 }
 
 // Lengths, pages for the next rows and their slots: one thread per sequence (a span of many entries by a whole wave).
-__global__ __launch_bounds__(PLAN_T) void commit_plan_kernel(CommitArgs a) {
-    __shared__ int tmp[PLAN_T / 64];
+__device__ void commit_plan(const CommitArgs& a) {
+    __shared__ int tmp[PLAN_T / 64], ends[MAX_SEQS];
     const int b = threadIdx.x, lane = b & 63;
-    int n = b < a.B ? commit_tokens(a, b) : -1, c = b < a.B ? a.count[b] : 0;
-    const bool idle = c < 0;
-    bool valid = n >= 0;
+    const int n = b < a.B ? a.state[b] : -1, c = b < a.B ? a.count[b] : 0, was = b < a.B ? a.length[b] : 0;
+    const bool valid = n >= 0;
     int64_t total = 0;
     bool narrow = false;  // (room past the table's width gets no page)
     if (valid) {
@@ -417,56 +425,30 @@ __global__ __launch_bounds__(PLAN_T) void commit_plan_kernel(CommitArgs a) {
         narrow = total > a.W;
         if (narrow) total = a.W;
     }
-    if (valid && a.path) {  // the checks of the move
-        int before = -1;
-        for (int k = 0; k < c; ++k) {
-            const int p = a.path[int64_t(b) * a.R + k];
-            valid = valid && p > before && p < a.R && page_at(a, b, int64_t(n) + (p < 0 ? 0 : p)) >= 0;
-            before = p;
-        }
-    }
-    // entries of the committed rows have to be pages; missing ones behind them are given
-    const int j0 = n >> a.lt, j1 = valid ? (n + c + a.T - 1) >> a.lt : 0, j2 = int(total);
+    // missing entries behind the committed rows' are given
+    const int j1 = valid ? (n + c + a.T - 1) >> a.lt : 0, j2 = int(total);
     int need = 0;
-    bool hole = false;
-    const bool wide = valid && j2 - j0 > 8;
+    const bool wide = valid && j2 - j1 > 8;
     if (valid && !wide)
-        for (int j = j0; j < j2; ++j) {
-            const bool miss = page_at(a, b, int64_t(j) << a.lt) < 0;
-            hole = hole || (miss && j < j1);
-            need += miss && j >= j1;
-        }
+        for (int j = j1; j < j2; ++j) need += page_at(a, b, int64_t(j) << a.lt) < 0;
     uint64_t todo = __builtin_amdgcn_ballot_w64(wide);
     while (todo) {  // (uniform in the wave)
         const int l = __builtin_ctzll(todo);
         todo &= todo - 1;
-        const int bb = __builtin_amdgcn_readlane(b, l), x0 = __builtin_amdgcn_readlane(j0, l), x1 = __builtin_amdgcn_readlane(j1, l),
-                  x2 = __builtin_amdgcn_readlane(j2, l);
-        int miss_in = 0, miss_behind = 0;
+        const int bb = __builtin_amdgcn_readlane(b, l), x1 = __builtin_amdgcn_readlane(j1, l), x2 = __builtin_amdgcn_readlane(j2, l);
+        int miss = 0;
 #pragma unroll 4
-        for (int j = x0 + lane; j < x2; j += 64) {
-            const bool miss = page_at(a, bb, int64_t(j) << a.lt) < 0;
-            miss_in += miss && j < x1;
-            miss_behind += miss && j >= x1;
-        }
-        for (int d = 32; d; d >>= 1) {
-            miss_in += __shfl_xor(miss_in, d, 64);
-            miss_behind += __shfl_xor(miss_behind, d, 64);
-        }
-        if (lane == l) {
-            hole = miss_in > 0;
-            need = miss_behind;
-        }
+        for (int j = x1 + lane; j < x2; j += 64) miss += page_at(a, bb, int64_t(j) << a.lt) < 0;
+        for (int d = 32; d; d >>= 1) miss += __shfl_xor(miss, d, 64);
+        if (lane == l) need = miss;
     }
-    valid = valid && !hole;
-    if (!valid) need = 0;
     int want;
     const int upto = block_sum_incl(need, tmp, want);
     const int have = want > 0 ? free_pages(a.refs, a.P, want, a.fresh, tmp) : 0;
     __syncthreads();  // (the list, written by other threads)
     const bool served = valid && upto <= have;
     const int end = valid ? n + c : 0;
-    if (served && need) {
+    if (served && need && !wide) {
         int at = upto - need;
         for (int j = j1; j < j2; ++j)
             if (page_at(a, b, int64_t(j) << a.lt) < 0) {
@@ -475,15 +457,43 @@ __global__ __launch_bounds__(PLAN_T) void commit_plan_kernel(CommitArgs a) {
                 a.refs[e] = 1;
             }
     }
-    if (b >= a.B) return;
-    a.status[b] = valid ? (served && !narrow ? 1 : 0) : (idle ? 1 : -1);
-    a.new_length[b] = valid ? end : a.length[b];
-    if (a.slots)
-        for (int r = 0; r < a.room; ++r) {
-            const int64_t t = int64_t(end) + r;
-            const int e = valid ? page_at(a, b, t) : -1;
-            a.slots[int64_t(b) * a.room + r] = e >= 0 ? (int64_t(e) << a.lt) + (t & (a.T - 1)) : -1;
+    todo = __builtin_amdgcn_ballot_w64(wide && served && need);
+    while (todo) {  // (uniform in the wave)
+        const int l = __builtin_ctzll(todo);
+        todo &= todo - 1;
+        const int bb = __builtin_amdgcn_readlane(b, l), x1 = __builtin_amdgcn_readlane(j1, l), x2 = __builtin_amdgcn_readlane(j2, l);
+        int at = __builtin_amdgcn_readlane(upto - need, l);
+        for (int j0 = x1; j0 < x2; j0 += 64) {
+            const int j = j0 + lane;
+            const bool miss = j < x2 && page_at(a, bb, int64_t(j) << a.lt) < 0;
+            const uint64_t m = __builtin_amdgcn_ballot_w64(miss);
+            if (miss) {
+                const int e = a.fresh[at + __popcll(m & ((uint64_t(1) << lane) - 1))];
+                a.table[bb * a.ts + j] = e;
+                a.refs[e] = 1;
+            }
+            at += __popcll(m);
         }
+    }
+    ends[b] = valid ? end : -1;
+    if (b < a.B) {
+        a.status[b] = valid ? (served && !narrow ? 1 : 0) : (c < 0 ? 1 : -1);
+        a.new_length[b] = valid ? end : was;
+    }
+    if (!a.slots) return;
+    __syncthreads();  // (ends, and the entries given above)
+    for (int x = b; x < a.B * a.room; x += PLAN_T) {
+        const int q = x / a.room;
+        const int64_t t = int64_t(ends[q]) + x % a.room;
+        const int e = ends[q] >= 0 ? page_at(a, q, t) : -1;
+        a.slots[x] = e >= 0 ? (int64_t(e) << a.lt) + (t & (a.T - 1)) : -1;
+    }
+}
+
+// Second launch: work-group 0 plans, the others (none without mean keys) sum.
+__global__ __launch_bounds__(SUM_T) void commit_plan_kernel(CommitArgs a) {
+    if (blockIdx.x == 0) commit_plan(a);
+    else commit_sums(a, blockIdx.x - 1, gridDim.x - 1);
 }
 
 int log2_of(int64_t T) {
@@ -542,10 +552,13 @@ extern "C" int mdx_page_fork(void* kv, void* ksum, int64_t L, int64_t Hk, int64_
     a.rows = a.fresh + pairs * W;
     a.copies = reinterpret_cast<int2*>(a.head + (fork_ints(pairs, W) + 3) / 4 * 4);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(fork_plan_kernel, dim3(1), dim3(PLAN_T), 0, st, a);
+    const bool few = pairs * W <= 4096;  // (at most four rounds of the planning work-group's waves)
+    hipLaunchKernelGGL(fork_plan_kernel, dim3(1), dim3(PLAN_T), 0, st, a, few ? 1 : 0);
     MDX_LAUNCHED();
-    hipLaunchKernelGGL(fork_rows_kernel, dim3(unsigned(pairs)), dim3(256), 0, st, a);
-    MDX_LAUNCHED();
+    if (!few) {
+        hipLaunchKernelGGL(fork_rows_kernel, dim3(unsigned(pairs)), dim3(256), 0, st, a);
+        MDX_LAUNCHED();
+    }
     hipLaunchKernelGGL(fork_copy_kernel, dim3(unsigned(pairs + 2048)), dim3(256), 0, st, a);
     MDX_LAUNCHED();
     return MDX_OK;
@@ -553,7 +566,7 @@ extern "C" int mdx_page_fork(void* kv, void* ksum, int64_t L, int64_t Hk, int64_
 
 extern "C" size_t mdx_page_commit_workspace(int64_t B, int64_t W) {
     if (B < 1 || B > MAX_SEQS || W < 1 || W > (int64_t(1) << 26)) return 0;
-    return size_t(B * W) * 4;
+    return size_t(B * W + (B + 3) / 4 * 4) * 4;
 }
 
 extern "C" int mdx_page_commit(void* kv, void* ksum, int32_t dtype, int64_t L, int64_t Hk, int64_t P, int64_t T, int64_t D,
@@ -570,7 +583,7 @@ extern "C" int mdx_page_commit(void* kv, void* ksum, int32_t dtype, int64_t L, i
     MDX_CHECK(B >= 1 && B <= MAX_SEQS && W >= 1 && (W << lt) < (int64_t(1) << 30) && table_stride >= W && table_stride <= (int64_t(1) << 26),
               "table [1..1024 sequences, W], under 2^30 tokens a sequence");
     MDX_CHECK(!path || (R >= 1 && R <= MAX_PATH), "a path has 1..64 rows");
-    MDX_CHECK(room >= 0 && room <= 65536, "room 0..65536");
+    MDX_CHECK(room >= 0 && room <= 65536 && B * room < (int64_t(1) << 30), "room 0..65536");
     MDX_CHECK(aligned(kv, 16) && aligned(ksum, 16), "16-byte aligned cache");
     MDX_CHECK(workspace && aligned(workspace, 16) && workspace_bytes >= mdx_page_commit_workspace(B, W),
               "workspace: %zu bytes, 16-byte aligned", mdx_page_commit_workspace(B, W));
@@ -588,21 +601,17 @@ extern "C" int mdx_page_commit(void* kv, void* ksum, int32_t dtype, int64_t L, i
     a.status = status;
     a.B = int(B), a.W = int(W), a.P = int(P), a.T = int(T), a.lt = lt, a.D = int(D), a.L = int(L), a.Hk = int(Hk);
     a.R = int(path ? R : 0), a.room = int(room), a.half = dtype == MDX_DT_F16;
-    a.fresh = static_cast<int32_t*>(workspace);
+    a.state = static_cast<int32_t*>(workspace);
+    a.fresh = a.state + (B + 3) / 4 * 4;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int64_t chunks = L * 2 * Hk;
-    if (path) {
-        // chunks per work-group: 512 pieces of 16 bytes where that is more than one chunk's (two in flight per thread)
-        const int64_t items = R * D / 8;
-        a.per_wg = int(items >= 512 ? 1 : 512 / items);
-        hipLaunchKernelGGL(commit_move_kernel, dim3(unsigned((chunks + a.per_wg - 1) / a.per_wg), unsigned(B)), dim3(256), 0, st, a);
-        MDX_LAUNCHED();
-    }
-    if (ksum) {
-        hipLaunchKernelGGL(commit_sum_kernel, dim3(1024), dim3(256), 0, st, a);
-        MDX_LAUNCHED();
-    }
-    hipLaunchKernelGGL(commit_plan_kernel, dim3(1), dim3(PLAN_T), 0, st, a);
+    // chunks per work-group: 512 pieces of 16 bytes where that is more than one chunk's (two in flight per thread)
+    const int64_t items = (path ? R : 1) * D / 8;
+    a.per_wg = int(items >= 512 ? 1 : 512 / items);
+    const int64_t wgs = path ? (chunks + a.per_wg - 1) / a.per_wg : 1;
+    hipLaunchKernelGGL(commit_move_kernel, dim3(unsigned(wgs), unsigned(B)), dim3(256), 0, st, a);
+    MDX_LAUNCHED();
+    hipLaunchKernelGGL(commit_plan_kernel, dim3(ksum ? 257 : 1), dim3(PLAN_T), 0, st, a);
     MDX_LAUNCHED();
     return MDX_OK;
 }

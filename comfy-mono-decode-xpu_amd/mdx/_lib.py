@@ -248,9 +248,14 @@ def ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def call_on(t, name, *args):
-    """call() with t's device as the current one (a launch belongs to the current device, its stream to t's)."""
-    if t.get_device() == torch.cuda.current_device():
-        return call(name, *args, stream_of(t))
-    with torch.cuda.device(t.device):
-        return call(name, *args, stream_of(t))
+_device_now = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def call_on(d, name, *args):
+    """call() on device d's current stream, with d as the current device (a launch belongs to that one)."""
+    if d != _device_now():
+        with torch.cuda.device(d):
+            return call_on(d, name, *args)
+    stream = torch.cuda.current_stream(d).cuda_stream if _raw_stream is None else _raw_stream(d)
+    if (_fns.get(name) or getattr(lib(), name))(*args, stream) != MDX_OK:
+        raise MdxError(f"{name}: {lib().mdx_last_error().decode(errors='replace')}")

@@ -63,9 +63,23 @@ def test_chain_rows(C, dev):
     _run(C, dev, BF, 8, 2, 128, 32, [500, 40], 6, False, 3, 1, 1, 5)
 
 
-def test_many_pages(C, dev):
-    """Thousands of candidates: several rounds of the histogram and of the pass in index order."""
-    _run(C, dev, BF, 4, 1, 64, 16, [16 * 5000 + 7, 16 * 1500], 1, False, 40, 1, 2, 6)
+@pytest.mark.parametrize("pages", [1024, 1025, 3000, 5000, 17000])
+def test_many_pages(C, dev, pages):
+    """Every size class of the selection, a full table and a short sequence in it."""
+    _run(C, dev, BF, 4, 1, 64, 16, [16 * (pages - 1) + 7, 16 * 150], 1, False, 40, 1, 2, 6)
+
+
+@pytest.mark.parametrize("pages", [900, 3000, 17000])
+@pytest.mark.parametrize("levels", [1, 2, 5])
+def test_few_levels_of_scores(C, dev, pages, levels):
+    """More equal scores at the threshold than one work-group's threads; scores that share all but their last bits."""
+    def edit(q, key, value, table, ksum):
+        q.fill_(1.0)
+        ksum.zero_()
+        ksum[:, table[0].long().clamp(min=0), 0] = (torch.arange(table.shape[1]) * 7 % levels).float().to(BF)
+        ksum[:, table[0, 500], 1] = 2.0 ** -40
+        ksum[:, table[0, 700], 1] = -(2.0 ** -40)
+    _run(C, dev, BF, 4, 2, 64, 16, [16 * (pages - 1) + 3], 1, False, 450, 1, 1, 13, edit)
 
 
 @pytest.mark.parametrize("equal", [1.0, 0.0])

@@ -189,6 +189,15 @@ def test_commit_without_pages(C, dev):
     assert _commit(C, dev, st, [4, 1], None, 5) == [0, 1]
 
 
+def test_commit_large_room(C, dev):
+    """Room of many pages for one sequence beside small ones, not all of it in the table for another."""
+    st = State(21, [14, 300, 0], P=900, held=2, W=300, L=1, Hk=1)
+    assert _commit(C, dev, st, [2, 1, 0], None, 4000) == [1, 1, 1]
+    st = State(22, [14, 900, 0], P=900, held=2, W=300, L=1, Hk=1)
+    st.table[2, 5], st.table[2, 100] = st.table[1, 50], 10 ** 6
+    assert _commit(C, dev, st, [2, 1, 0], None, 4000) == [1, 0, 1]
+
+
 def test_commit_many_sequences(C, dev):
     g = torch.Generator().manual_seed(5)
     lens = [int(x) for x in torch.randint(0, 60, (1000,), generator=g)]
