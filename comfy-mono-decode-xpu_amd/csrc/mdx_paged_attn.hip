@@ -103,63 +103,88 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
     return uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const unsigned char*)p));
 }
 
-// LDS layout of a 32-token stage, K and V alike: [dims 32 kk ..][token half][16 tokens][64 B], written by direct loads of
-// 16 tokens x 64 B. K: lane (token c16, k-group g) reads its 16 bytes at c16 * 64 + g * 16 of block (kk, half): one
-// contiguous KiB. V: the two 32-byte halves of a token's 64 bytes are exchanged in every second group of four tokens (the
-// loads fetch them so), so that the transposing reads of two lane groups meet different banks; lane s of group g points
-// at token 4 g + s / 4, dims 16 dt + 4 (s % 4) .. + 3, and receives dim c16 of tokens 4 g .. 4 g + 3.
+// LDS layout of a 32-token stage, K and V alike: the tokens' rows of 2 D bytes one after the other, as they stand in a page,
+// so that a direct load's KiB is one KiB of the page (64-byte pieces of 16 tokens per load: 5 % slower, 200 us against
+// PIECES for 64 single-token sequences of 262 thousand tokens in all). Within a row the 16-byte pieces are exchanged by
+// an exclusive or with the token (swizzle), which the loads' source addresses follow, so that
+//   K: lane (token c16 of the half, k-group g) reads piece 4 kk + g, 16 tokens of one piece meeting all banks once;
+//   V: the transposing reads (lane s of group g points at token 4 g + s / 4 of the half, dims 16 dt + 4 (s % 4) .. + 3, and
+//      receives dim c16 of tokens 4 g .. 4 g + 3) meet every bank alike;
+// both from one lane address: piece bits above the lane's own enter by an exclusive or with a constant.
 // The reads are inline asm that ends with its wait: the builtins would wait for every direct load in flight.
 template <int D>
-__device__ __forceinline__ void read_k(u32x4 (&kf)[2][D / 32], uint32_t base) {
+__device__ __forceinline__ int swizzle(int token) {  // exchanged piece = piece ^ swizzle(token)
+    return D == 64 ? (token >> 1) & 7 : token & 15;
+}
+// tokens of half h: k-operands kk of the D / 32
+template <int D>
+__device__ __forceinline__ void read_k(u32x4 (&kf)[D / 32], uint32_t at) {
     if constexpr (D == 256) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-            asm volatile(
-                "ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:2048\n\tds_read_b128 %2, %8 offset:4096\n\t"
-                "ds_read_b128 %3, %8 offset:6144\n\tds_read_b128 %4, %8 offset:8192\n\tds_read_b128 %5, %8 offset:10240\n\t"
-                "ds_read_b128 %6, %8 offset:12288\n\tds_read_b128 %7, %8 offset:14336\n\ts_waitcnt lgkmcnt(0)"
-                : "=&v"(kf[h][0]), "=&v"(kf[h][1]), "=&v"(kf[h][2]), "=&v"(kf[h][3]), "=&v"(kf[h][4]), "=&v"(kf[h][5]),
-                  "=&v"(kf[h][6]), "=&v"(kf[h][7])
-                : "v"(base + h * 1024)
-                : "memory");
+        asm volatile(
+            "ds_read_b128 %0, %8\n\tds_read_b128 %1, %9\n\tds_read_b128 %2, %10\n\tds_read_b128 %3, %11\n\t"
+            "ds_read_b128 %4, %8 offset:256\n\tds_read_b128 %5, %9 offset:256\n\tds_read_b128 %6, %10 offset:256\n\t"
+            "ds_read_b128 %7, %11 offset:256\n\ts_waitcnt lgkmcnt(0)"
+            : "=&v"(kf[0]), "=&v"(kf[1]), "=&v"(kf[2]), "=&v"(kf[3]), "=&v"(kf[4]), "=&v"(kf[5]), "=&v"(kf[6]), "=&v"(kf[7])
+            : "v"(at), "v"(at ^ 64), "v"(at ^ 128), "v"(at ^ 192)
+            : "memory");
     } else if constexpr (D == 128) {
         asm volatile(
-            "ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:2048\n\tds_read_b128 %2, %8 offset:4096\n\t"
-            "ds_read_b128 %3, %8 offset:6144\n\tds_read_b128 %4, %8 offset:1024\n\tds_read_b128 %5, %8 offset:3072\n\t"
-            "ds_read_b128 %6, %8 offset:5120\n\tds_read_b128 %7, %8 offset:7168\n\ts_waitcnt lgkmcnt(0)"
-            : "=&v"(kf[0][0]), "=&v"(kf[0][1]), "=&v"(kf[0][2]), "=&v"(kf[0][3]), "=&v"(kf[1][0]), "=&v"(kf[1][1]),
-              "=&v"(kf[1][2]), "=&v"(kf[1][3])
-            : "v"(base)
+            "ds_read_b128 %0, %4\n\tds_read_b128 %1, %5\n\tds_read_b128 %2, %6\n\tds_read_b128 %3, %7\n\ts_waitcnt lgkmcnt(0)"
+            : "=&v"(kf[0]), "=&v"(kf[1]), "=&v"(kf[2]), "=&v"(kf[3])
+            : "v"(at), "v"(at ^ 64), "v"(at ^ 128), "v"(at ^ 192)
             : "memory");
     } else {
         static_assert(D == 64, "head_dim 64, 128 or 256");
-        asm volatile(
-            "ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:2048\n\tds_read_b128 %2, %4 offset:1024\n\t"
-            "ds_read_b128 %3, %4 offset:3072\n\ts_waitcnt lgkmcnt(0)"
-            : "=&v"(kf[0][0]), "=&v"(kf[0][1]), "=&v"(kf[1][0]), "=&v"(kf[1][1])
-            : "v"(base)
-            : "memory");
+        asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %3\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(kf[0]), "=&v"(kf[1])
+                     : "v"(at), "v"(at ^ 64)
+                     : "memory");
     }
 }
-// dim tiles 4 X .. 4 X + 3 of V^T (ev / od: the lane's base for even and odd dim tiles)
-template <int X, int DT>
-__device__ __forceinline__ void read_v4(u32x2 (&va)[DT], u32x2 (&vb)[DT], uint32_t ev, uint32_t od) {
-    asm volatile(
-        "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %9\n\tds_read_b64_tr_b16 %2, %8 offset:2048\n\t"
-        "ds_read_b64_tr_b16 %3, %9 offset:2048\n\tds_read_b64_tr_b16 %4, %8 offset:1024\n\tds_read_b64_tr_b16 %5, %9 offset:1024\n\t"
-        "ds_read_b64_tr_b16 %6, %8 offset:3072\n\tds_read_b64_tr_b16 %7, %9 offset:3072\n\ts_waitcnt lgkmcnt(0)"
-        : "=&v"(va[4 * X]), "=&v"(va[4 * X + 1]), "=&v"(va[4 * X + 2]), "=&v"(va[4 * X + 3]), "=&v"(vb[4 * X]),
-          "=&v"(vb[4 * X + 1]), "=&v"(vb[4 * X + 2]), "=&v"(vb[4 * X + 3])
-        : "v"(ev + X * 4096), "v"(od + X * 4096)
-        : "memory");
-}
+// both halves at once
 template <int D>
-__device__ __forceinline__ void read_v(u32x2 (&va)[D / 16], u32x2 (&vb)[D / 16], uint32_t ev, uint32_t od) {
-    read_v4<0>(va, vb, ev, od);
-    if constexpr (D >= 128) read_v4<1>(va, vb, ev, od);
-    if constexpr (D == 256) {
-        read_v4<2>(va, vb, ev, od);
-        read_v4<3>(va, vb, ev, od);
+__device__ __forceinline__ void read_k2(u32x4 (&kf)[2][D / 32], uint32_t at) {
+    if constexpr (D == 128) {
+        asm volatile(
+            "ds_read_b128 %0, %8\n\tds_read_b128 %1, %9\n\tds_read_b128 %2, %10\n\tds_read_b128 %3, %11\n\t"
+            "ds_read_b128 %4, %8 offset:4096\n\tds_read_b128 %5, %9 offset:4096\n\tds_read_b128 %6, %10 offset:4096\n\t"
+            "ds_read_b128 %7, %11 offset:4096\n\ts_waitcnt lgkmcnt(0)"
+            : "=&v"(kf[0][0]), "=&v"(kf[0][1]), "=&v"(kf[0][2]), "=&v"(kf[0][3]), "=&v"(kf[1][0]), "=&v"(kf[1][1]),
+              "=&v"(kf[1][2]), "=&v"(kf[1][3])
+            : "v"(at), "v"(at ^ 64), "v"(at ^ 128), "v"(at ^ 192)
+            : "memory");
+    } else {
+        read_k<D>(kf[0], at);
+        read_k<D>(kf[1], at + 16 * 2 * D);
+    }
+}
+// V^T of dim tiles 8 X .. 8 X + 7 (D = 64: the four there are): va tokens of half 0, vb of half 1
+template <int D, int X>
+__device__ __forceinline__ void read_v(u32x2 (&va)[D == 64 ? 4 : 8], u32x2 (&vb)[D == 64 ? 4 : 8], uint32_t at) {
+    if constexpr (D == 64) {
+        asm volatile(
+            "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %9\n\tds_read_b64_tr_b16 %2, %10\n\t"
+            "ds_read_b64_tr_b16 %3, %11\n\tds_read_b64_tr_b16 %4, %8 offset:2048\n\tds_read_b64_tr_b16 %5, %9 offset:2048\n\t"
+            "ds_read_b64_tr_b16 %6, %10 offset:2048\n\tds_read_b64_tr_b16 %7, %11 offset:2048\n\ts_waitcnt lgkmcnt(0)"
+            : "=&v"(va[0]), "=&v"(va[1]), "=&v"(va[2]), "=&v"(va[3]), "=&v"(vb[0]), "=&v"(vb[1]), "=&v"(vb[2]), "=&v"(vb[3])
+            : "v"(at), "v"(at ^ 32), "v"(at ^ 64), "v"(at ^ 96)
+            : "memory");
+    } else {
+        static_assert(D == 128 || D == 256, "");
+        asm volatile(
+            "ds_read_b64_tr_b16 %0, %16 offset:%24\n\tds_read_b64_tr_b16 %1, %17 offset:%24\n\t"
+            "ds_read_b64_tr_b16 %2, %18 offset:%24\n\tds_read_b64_tr_b16 %3, %19 offset:%24\n\t"
+            "ds_read_b64_tr_b16 %4, %20 offset:%24\n\tds_read_b64_tr_b16 %5, %21 offset:%24\n\t"
+            "ds_read_b64_tr_b16 %6, %22 offset:%24\n\tds_read_b64_tr_b16 %7, %23 offset:%24\n\t"
+            "ds_read_b64_tr_b16 %8, %16 offset:%25\n\tds_read_b64_tr_b16 %9, %17 offset:%25\n\t"
+            "ds_read_b64_tr_b16 %10, %18 offset:%25\n\tds_read_b64_tr_b16 %11, %19 offset:%25\n\t"
+            "ds_read_b64_tr_b16 %12, %20 offset:%25\n\tds_read_b64_tr_b16 %13, %21 offset:%25\n\t"
+            "ds_read_b64_tr_b16 %14, %22 offset:%25\n\tds_read_b64_tr_b16 %15, %23 offset:%25\n\ts_waitcnt lgkmcnt(0)"
+            : "=&v"(va[0]), "=&v"(va[1]), "=&v"(va[2]), "=&v"(va[3]), "=&v"(va[4]), "=&v"(va[5]), "=&v"(va[6]), "=&v"(va[7]),
+              "=&v"(vb[0]), "=&v"(vb[1]), "=&v"(vb[2]), "=&v"(vb[3]), "=&v"(vb[4]), "=&v"(vb[5]), "=&v"(vb[6]), "=&v"(vb[7])
+            : "v"(at), "v"(at ^ 32), "v"(at ^ 64), "v"(at ^ 96), "v"(at ^ 128), "v"(at ^ 160), "v"(at ^ 192), "v"(at ^ 224),
+              "n"(X * 256), "n"(X * 256 + 16 * 2 * D)
+            : "memory");
     }
 }
 
@@ -216,8 +241,8 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
     using Geo = Geometry<E, D, TPW, RTW, P, SEL>;
     constexpr int NT = Geo::NT, RPW = Geo::RPW, STAGE = Geo::STAGE, NS = Geo::NS, PER = Geo::PER;
     constexpr int KK = D / 32, DT = D / 16, TOK = STEP * P;
-    extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ int sh_sum[NT / 64], sh_at[3];
+    extern __shared__ __align__(256) unsigned char smem[];  // (the reads' exclusive ors need rows aligned to 256 bytes)
+    __shared__ int sh_sum[NT / 64], sh_at[3], odd;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, c16 = lane & 15;
     const int rw = w % RTW, part = w / RTW;
@@ -269,8 +294,12 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
         b = __builtin_amdgcn_readfirstlane(sh_at[0]);
         in_b = begin - __builtin_amdgcn_readfirstlane(sh_at[1]);
     }
-    if (tid == 0) a.info[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (tid == 0) {
+        a.info[blockIdx.x] = make_int4(0, 0, 0, 0);
+        odd = 0;
+    }
     if (begin >= end) return;  // (uniform)
+    __syncthreads();
     begin = __builtin_amdgcn_readfirstlane(begin);
     end = __builtin_amdgcn_readfirstlane(end);
 
@@ -292,18 +321,83 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
 
     unsigned char* ring = smem + part * NS * 2 * STAGE;
     const uint32_t ring_lds = lds_addr(ring);
-    const uint32_t k_lane = c16 * 64 + g * 16;
-    const uint32_t v_lane = (4 * g + (c16 >> 2)) * 64 + (c16 & 3) * 8;
-    const uint32_t v_even = v_lane + (g & 1) * 32, v_odd = v_lane + ((g & 1) ^ 1) * 32;
-    // the lane's place within a direct load: token lane / 4 of the half, 16-byte piece lane % 4 (V: exchanged halves)
-    const int k_voff = (lane >> 2) * int(a.kt) * 2 + (lane & 3) * 16;
-    const int v_voff = (lane >> 2) * int(a.vt) * 2 + ((lane & 3) ^ (((lane >> 4) & 1) << 1)) * 16;
+    constexpr int RB = 2 * D, LPR = RB / 16, TPL = 64 / LPR;  // bytes and pieces of a token's row, tokens per direct load
+    const uint32_t k_lane = c16 * RB + ((g ^ swizzle<D>(c16)) * 16);
+    const int v_tok = 4 * g + (c16 >> 2);
+    const uint32_t v_lane = v_tok * RB + ((((c16 & 3) >> 1) ^ swizzle<D>(v_tok)) * 16) + (c16 & 1) * 8;
+    // The lane's place within a direct load: token lane / LPR, piece lane % LPR as exchanged; load i of a matrix covers the
+    // tokens from TPL i, whose swizzle enters by an exclusive or (swizzle(TPL i + x) = swizzle(TPL i) ^ swizzle(x)).
+    const uint32_t piece = ((lane % LPR) ^ swizzle<D>(lane / LPR)) * 16;
+    const uint32_t k_row = (lane / LPR) * uint32_t(a.kt) * 2, v_row = (lane / LPR) * uint32_t(a.vt) * 2;
 
     while (true) {
         const int n_unit = steps_of<SEL>(a, sp, u, RPW, TOK);
         const int nst = min(n_unit - step0, end - at);  // steps of this unit in the share
         const int own = (!a.mask && !SEL) ? (min(a.rows, (u + 1) * RPW) - 1) / a.G + 1 : (!a.mask ? u + 1 : a.S);
         const int t_end = sp.tree0 + own;
+
+        // ---- the pages of a stage (scalar loads ahead of their use), and its direct loads
+        const unsigned char* kbase = reinterpret_cast<const unsigned char*>(a.key + kh * a.kh);
+        const unsigned char* vbase = reinterpret_cast<const unsigned char*>(a.value + kh * a.vh);
+        const int32_t* row = a.table + b * a.ts;
+        const int32_t* picked = SEL ? a.page + ((int64_t(b) * a.S + u) * a.Hk + kh) * a.most : nullptr;
+        struct Two {
+            int e[2];
+        };
+        auto entries = [&](int s) {
+            const int v0 = (step0 + s) * TOK + part * STEP;
+            Two x;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int v = v0 + 16 * h;
+                x.e[h] = -1;
+                if (v < t_end) {
+                    if (SEL && v < sp.nsel) {
+                        x.e[h] = uload(picked + (v >> a.lt));
+                    } else {
+                        const int t = SEL ? sp.tail + (v - sp.nsel) : v;
+                        if ((t >> a.lt) < a.W) x.e[h] = uload(row + (t >> a.lt));
+                    }
+                }
+            }
+            return x;
+        };
+        uint32_t hist = 0;  // two bits per stage issued: its halves stand in pages
+        const unsigned char *kp_[2], *vp_[2];
+        auto place = [&](int s, Two x) {
+            const int v0 = (step0 + s) * TOK + part * STEP;
+            uint32_t ok = 0;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int v = v0 + 16 * h, t = SEL && v >= sp.nsel ? v - sp.nsel : v;
+                const int64_t e = x.e[h], r = t & ((1 << a.lt) - 1);
+                const bool in = x.e[h] >= 0 && x.e[h] < a.P;
+                ok |= in ? 1u << h : 0u;
+                // (a half without a page reads the pool's first rows: in bounds, and masked)
+                kp_[h] = kbase + (in ? (e * a.kp + r * a.kt) * 2 : 0);
+                vp_[h] = vbase + (in ? (e * a.vp + r * a.vt) * 2 : 0);
+            }
+            hist = (hist << 2) | ok;
+        };
+        auto load = [&](const unsigned char* const (&from)[2], uint32_t lane_row, uint32_t stride, unsigned char* dst) {
+            constexpr int HALF = 16 / TPL;  // loads of a half
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const int i = rw * PER + j;  // tokens TPL i ..
+                const unsigned char* src = from[i / HALF] + (lane_row + uint32_t((i % HALF) * TPL) * stride + (piece ^ (swizzle<D>(TPL * i) * 16)));
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                                 (__attribute__((address_space(3))) void*)(dst + i * 1024), 16, 0, 0);
+            }
+        };
+        auto issue_k = [&](int s) { load(kp_, k_row, uint32_t(a.kt) * 2, ring + (s & (NS - 1)) * 2 * STAGE); };
+        auto issue_v = [&](int s) { load(vp_, v_row, uint32_t(a.vt) * 2, ring + (s & (NS - 1)) * 2 * STAGE + STAGE); };
+        // A wave with a ring of its own (RTW == 1) fills the whole ring ahead, refills K's slot once it has read K and V's
+        // once it has read V, and meets no barrier. Waves that share a ring fill NS - 1 stages ahead and refill the slot of
+        // the stage before at the top of a stage, behind the one barrier.
+        constexpr int AHEAD = RTW == 1 ? NS : NS - 1;
+        Two first_e[AHEAD];
+#pragma unroll
+        for (int s = 0; s < AHEAD; ++s) first_e[s] = entries(s);
 
         // ---- query rows and what they admit
         u32x4 qf[TPW][KK];
@@ -332,58 +426,6 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
             asm volatile("" : "+v"(bits[t]));
         }
 
-        // ---- the stages
-        const unsigned char* kbase = reinterpret_cast<const unsigned char*>(a.key + kh * a.kh);
-        const unsigned char* vbase = reinterpret_cast<const unsigned char*>(a.value + kh * a.vh);
-        const int32_t* row = a.table + b * a.ts;
-        const int64_t unit_row = (int64_t(b) * a.S + u) * a.Hk + kh;  // (with a selection)
-        uint32_t hist = 0;  // two bits per stage issued: its halves stand in pages
-        const unsigned char *kp_[2], *vp_[2];
-        // the pages of stage s (scalar loads), for issue_k / issue_v
-        auto pages = [&](int s) {
-            const int v0 = (step0 + s) * TOK + part * STEP;
-            uint32_t ok = 0;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int v = v0 + 16 * h;
-                int e = -1, r = 0;
-                if (v < t_end) {
-                    if (SEL && v < sp.nsel) {
-                        e = uload(a.page + unit_row * a.most + (v >> a.lt));
-                        r = v & ((1 << a.lt) - 1);
-                    } else {
-                        const int t = SEL ? sp.tail + (v - sp.nsel) : v;
-                        if ((t >> a.lt) < a.W) e = uload(row + (t >> a.lt));
-                        r = t & ((1 << a.lt) - 1);
-                    }
-                }
-                const bool in = e >= 0 && e < a.P;
-                ok |= in ? 1u << h : 0u;
-                // (a half without a page reads the pool's first rows: in bounds, and masked)
-                kp_[h] = kbase + (in ? (e * a.kp + r * a.kt) * 2 : 0);
-                vp_[h] = vbase + (in ? (e * a.vp + r * a.vt) * 2 : 0);
-            }
-            hist = (hist << 2) | ok;
-        };
-        auto issue_k = [&](int s) {
-            unsigned char* dst = ring + (s & (NS - 1)) * 2 * STAGE;
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                const int i = rw * PER + j;
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kp_[i & 1] + k_voff + (i >> 1) * 64),
-                                                 (__attribute__((address_space(3))) void*)(dst + i * 1024), 16, 0, 0);
-            }
-        };
-        auto issue_v = [&](int s) {
-            unsigned char* dst = ring + (s & (NS - 1)) * 2 * STAGE + STAGE;
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                const int i = rw * PER + j;
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(vp_[i & 1] + v_voff + (i >> 1) * 64),
-                                                 (__attribute__((address_space(3))) void*)(dst + i * 1024), 16, 0, 0);
-            }
-        };
-
         f32x4 acc[TPW][DT];
         float m[TPW], l[TPW];
 #pragma unroll
@@ -393,87 +435,86 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) acc[t][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
-        // A wave with a ring of its own (RTW == 1) fills the whole ring ahead, refills K's slot once it has read K and V's
-        // once it has read V, and meets no barrier. Waves that share a ring fill NS - 1 stages ahead and refill the slot of
-        // the stage before at the top of a stage, behind the one barrier.
-        constexpr int AHEAD = RTW == 1 ? NS : NS - 1;
-        for (int s = 0; s < AHEAD && s < nst; ++s) {
-            pages(s);
-            issue_k(s);
-            issue_v(s);
-        }
+#pragma unroll
+        for (int s = 0; s < AHEAD; ++s)
+            if (s < nst) {
+                place(s, first_e[s]);
+                issue_k(s);
+                issue_v(s);
+            }
+        Two next_e = entries(AHEAD);  // of the stage issued next
         for (int s = 0; s < nst; ++s) {
             const uint32_t slot = ring_lds + (s & (NS - 1)) * 2 * STAGE;
             // (stages issued when stage s is read: AHEAD more, as far as there are any)
             const int behind = min(nst - s, AHEAD) - 1;
             const uint32_t ok = (hist >> (2 * behind)) & 3u;
-            u32x4 kf[2][KK];
-            u32x2 va[DT], vb[DT];
             const bool more = s + AHEAD < nst;
             if constexpr (RTW == 1) {
                 if (s + AHEAD - 1 < nst) wait_vm<PER * (2 * NS - 1)>();
                 else wait_vm<0>();
-                read_k<D>(kf, slot + k_lane);
-                if (more) {
-                    pages(s + AHEAD);
-                    issue_k(s + AHEAD);
-                }
             } else {
                 if (s + AHEAD - 1 < nst) wait_vm<2 * PER * (AHEAD - 1)>();
                 else wait_vm<0>();
                 __builtin_amdgcn_s_barrier();  // everyone's share of stage s has landed, everyone is done with stage s - 1
                 if (more) {
-                    pages(s + AHEAD);
+                    place(s + AHEAD, next_e);
                     issue_k(s + AHEAD);
                     issue_v(s + AHEAD);
+                    next_e = entries(s + AHEAD + 1);
                 }
-                read_k<D>(kf, slot + k_lane);
             }
             f32x4 st[TPW][2];
+            auto scores = [&](const u32x4 (&k)[KK], int h) {
 #pragma unroll
-            for (int t = 0; t < TPW; ++t)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int t = 0; t < TPW; ++t) {
                     st[t][h] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int kk = 0; kk < KK; ++kk) st[t][h] = E::mfma(kf[h][kk], qf[t][kk], st[t][h]);
+                    for (int kk = 0; kk < KK; ++kk) st[t][h] = E::mfma(k[kk], qf[t][kk], st[t][h]);
                 }
-            if constexpr (RTW == 1) {
-                if (more) wait_vm<PER * (2 * NS - 1)>();
-                else wait_vm<0>();
+            };
+            auto refill_k = [&]() {
+                if (RTW == 1 && more) {
+                    place(s + AHEAD, next_e);
+                    issue_k(s + AHEAD);
+                }
+            };
+            if constexpr (D == 256) {  // (half by half: the operands of one half are 32 registers)
+                u32x4 kf[KK];
+                read_k<D>(kf, slot + k_lane);
+                scores(kf, 0);
+                read_k<D>(kf, slot + k_lane + 16 * RB);
+                refill_k();
+                scores(kf, 1);
+            } else {
+                u32x4 kf[2][KK];
+                read_k2<D>(kf, slot + k_lane);
+                refill_k();
+                scores(kf[0], 0);
+                scores(kf[1], 1);
             }
-            read_v<D>(va, vb, slot + STAGE + v_even, slot + STAGE + v_odd);
-            if constexpr (RTW == 1)
-                if (more) issue_v(s + AHEAD);
 
             const int v0 = (step0 + s) * TOK + part * STEP;
             const bool whole = ok == 3u && v0 + STEP <= sp.tree0;  // (uniform) every row admits all 32 tokens
-            // A weight of 0 times an infinity or a NaN in a place that a row does not admit would reach the row: where such
-            // a stage holds one, its tokens go one by one to the rows that admit them.
-            bool clean = true;
-            if (!whole) {
-                uint32_t top = 0;
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
-                    top |= ((va[dt].x & E::EXP) + E::ONE) | ((va[dt].y & E::EXP) + E::ONE) | ((vb[dt].x & E::EXP) + E::ONE) |
-                           ((vb[dt].y & E::EXP) + E::ONE);
-                clean = __builtin_amdgcn_ballot_w64((top & 0x80008000u) != 0) == 0;
-            }
+            u32x4 pf[TPW];
+            uint32_t in[TPW];
 #pragma unroll
             for (int t = 0; t < TPW; ++t) {
-                uint32_t in = ~0u;
+                in[t] = ~0u;
                 if (!whole) {
                     const int p = sp.tree0 - v0;  // tokens of the prefix in the stage
                     if (a.mask) {
                         const uint64_t own_bits = p >= 32 ? 0 : (p >= 0 ? bits[t] << p : (-p < 64 ? bits[t] >> -p : 0));
-                        in = (p >= 32 ? ~0u : (p > 0 ? (1u << p) - 1u : 0u)) | uint32_t(own_bits);
+                        in[t] = (p >= 32 ? ~0u : (p > 0 ? (1u << p) - 1u : 0u)) | uint32_t(own_bits);
                     } else {
                         const int nv = p + lim[t] + 1;
-                        in = nv >= 32 ? ~0u : (nv > 0 ? (1u << nv) - 1u : 0u);
+                        in[t] = nv >= 32 ? ~0u : (nv > 0 ? (1u << nv) - 1u : 0u);
                     }
-                    in &= ((ok & 1u) ? 0x0000FFFFu : 0u) | ((ok & 2u) ? 0xFFFF0000u : 0u);
-                    if (__builtin_amdgcn_ballot_w64(in != 0u) == 0) continue;  // (uniform: nothing for this tile)
-                    const uint32_t lb = in >> (4 * g);
+                    in[t] &= ((ok & 1u) ? 0x0000FFFFu : 0u) | ((ok & 2u) ? 0xFFFF0000u : 0u);
+                    if (__builtin_amdgcn_ballot_w64(in[t] != 0u) == 0) {  // (uniform: nothing for this tile)
+                        pf[t] = u32x4{0, 0, 0, 0};
+                        continue;
+                    }
+                    const uint32_t lb = in[t] >> (4 * g);
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -488,7 +529,6 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
                 const float mz = (mnew == -INFINITY ? 0.f : mnew) * a.zs - E::SHIFT;
                 const float alpha = __builtin_amdgcn_exp2f(fmaf(m[t], a.zs, -mz) - E::SHIFT);
                 m[t] = mnew;
-                u32x4 pf;
                 float ps = 0.f;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
@@ -496,35 +536,56 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
                     for (int i = 0; i < 4; i += 2) {
                         const float p0 = __builtin_amdgcn_exp2f(fmaf(st[t][h][i], a.zs, -mz));
                         const float p1 = __builtin_amdgcn_exp2f(fmaf(st[t][h][i + 1], a.zs, -mz));
-                        pf[2 * h + i / 2] = E::pair(p0, p1);
-                        ps = E::add_pair(pf[2 * h + i / 2], ps);
+                        pf[t][2 * h + i / 2] = E::pair(p0, p1);
+                        ps = E::add_pair(pf[t][2 * h + i / 2], ps);
                     }
                 l[t] = l[t] * alpha + ps;  // (this lane's tokens; the row's four lanes meet at the end)
                 if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0)
 #pragma unroll
                     for (int dt = 0; dt < DT; ++dt) acc[t][dt] *= alpha;
-                if (clean) {
+            }
+            if constexpr (RTW == 1) {
+                if (more) wait_vm<PER * (2 * NS - 1)>();
+                else wait_vm<0>();
+            }
+            constexpr int VT = D == 64 ? 4 : 8;  // dim tiles read at once
+            u32x2 va[VT], vb[VT];
+            auto weigh = [&](int dt0) {
+                // A weight of 0 times an infinity or a NaN in a place that a row does not admit would reach the row: in a
+                // stage that not every row admits whole, such values count as 0 here, and where there are any the rows
+                // that do admit them get them when the unit's parts meet (`odd`).
+                if (!whole) {
+                    uint32_t top = 0;
 #pragma unroll
-                    for (int dt = 0; dt < DT; ++dt)
-                        acc[t][dt] = E::mfma(u32x4{va[dt].x, va[dt].y, vb[dt].x, vb[dt].y}, pf, acc[t][dt]);
-                } else {
-                    for (int j = 0; j < 32; ++j) {
-                        // token j's k-slot: lane group (j / 4) % 4, element 4 (j / 16) + j % 4
-                        const bool mine = g == ((j >> 2) & 3);
-                        const uint32_t half = mine ? ((j & 1) ? 0xFFFF0000u : 0x0000FFFFu) : 0u;
-                        const uint32_t m0 = j < 16 && !(j & 2) ? half : 0u, m1 = j < 16 && (j & 2) ? half : 0u;
-                        const uint32_t m2 = j >= 16 && !(j & 2) ? half : 0u, m3 = j >= 16 && (j & 2) ? half : 0u;
-                        const bool admits = (in >> j) & 1u;
+                    for (int x = 0; x < VT; ++x)
+                        top |= ((va[x].x & E::EXP) + E::ONE) | ((va[x].y & E::EXP) + E::ONE) | ((vb[x].x & E::EXP) + E::ONE) |
+                               ((vb[x].y & E::EXP) + E::ONE);
+                    if (__builtin_amdgcn_ballot_w64((top & 0x80008000u) != 0) != 0) {
+                        auto finite = [](uint32_t v) { return v & ~(((((v & E::EXP) + E::ONE) & 0x80008000u) >> 15) * 0xFFFFu); };
 #pragma unroll
-                        for (int dt = 0; dt < DT; ++dt) {
-                            const f32x4 x = E::mfma(u32x4{va[dt].x & m0, va[dt].y & m1, vb[dt].x & m2, vb[dt].y & m3}, pf,
-                                                    f32x4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) acc[t][dt][i] += admits ? x[i] : 0.f;
+                        for (int x = 0; x < VT; ++x) {
+                            va[x] = u32x2{finite(va[x].x), finite(va[x].y)};
+                            vb[x] = u32x2{finite(vb[x].x), finite(vb[x].y)};
                         }
+                        odd = 1;
                     }
                 }
+#pragma unroll
+                for (int t = 0; t < TPW; ++t)
+#pragma unroll
+                    for (int x = 0; x < VT; ++x)
+                        acc[t][dt0 + x] = E::mfma(u32x4{va[x].x, va[x].y, vb[x].x, vb[x].y}, pf[t], acc[t][dt0 + x]);
+            };
+            read_v<D, 0>(va, vb, slot + STAGE + v_lane);
+            if constexpr (D == 256) {
+                weigh(0);
+                read_v<D, 1>(va, vb, slot + STAGE + v_lane);
             }
+            if (RTW == 1 && more) {
+                issue_v(s + AHEAD);
+                next_e = entries(s + AHEAD + 1);
+            }
+            weigh(D == 256 ? 8 : 0);
         }
 
         // ---- the parts of a row tile meet in LDS, tile by tile; rows D + 4 floats apart (no two rows of an access in one bank)
@@ -563,6 +624,24 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
                     sum += lm[RTW * P * 16 + (rt * P + p) * 16 + rr] * wp;
                     o += *reinterpret_cast<const f32x4*>(lo + (rt * P + p) * 16 * OR + rr * OR + d) * wp;
                 }
+                if (odd) {  // (uniform: what the stages left out, for the rows that admit it)
+                    const int s = SEL ? u : rg / a.G;
+                    for (int v = step0 * TOK; v < min(t_end, (step0 + nst) * TOK); ++v) {
+                        const int own_row = v - sp.tree0;
+                        if (own_row >= 0 && !(a.mask ? (uint64_t(a.mask[int64_t(b) * a.S + s]) >> own_row) & 1 : own_row <= s)) continue;
+                        const int tok = SEL && v >= sp.nsel ? v - sp.nsel + sp.tail : v;
+                        const bool chosen = SEL && v < sp.nsel;
+                        if (!chosen && (tok >> a.lt) >= a.W) continue;
+                        const int64_t e = chosen ? picked[v >> a.lt] : row[tok >> a.lt];
+                        if (e < 0 || e >= a.P) continue;
+                        const uint16_t* src = a.value + kh * a.vh + e * a.vp + (tok & ((1 << a.lt) - 1)) * a.vt + d;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float x = E::to_f32(src[i]);
+                            if (!(__builtin_fabsf(x) < INFINITY)) o[i] += x;
+                        }
+                    }
+                }
                 if (first && last) {
                     const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
                     const int s = SEL ? u : rg / a.G, h = kh * a.G + (SEL ? rg : rg % a.G);
@@ -588,6 +667,11 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
         // ---- the next unit
         at += nst;
         if (at >= end) break;
+        if (odd) {  // (uniform: every thread is past its last use)
+            __syncthreads();
+            if (tid == 0) odd = 0;
+            __syncthreads();
+        }
         step0 = 0;
         if (++u == a.units) {
             u = 0;
@@ -703,9 +787,10 @@ __device__ __forceinline__ int wave_incl_sum(int v, int lane) {
 }
 
 // The `blocks` best of the scored pages (ties to the lowest index) and the forced ones, ascending: one work-group per
-// (sequence, row, kv head), the keys in registers (W <= NT EACH; past 16 per thread they are read again). The threshold: a histogram of 1024 bins over the range
-// that the keys' upper words span, then the keys of the one bin that holds it by their ranks; where that bin has more than
-// NT keys (ties), by bytes from the top instead. Then one pass in index order. Bound by latency (barriers and LDS): 9 us
+// (sequence, row, kv head), the keys in registers (W <= NT EACH; past 16 per thread they are read again). The threshold: a
+// histogram of 1024 bins, even steps between the lowest and the highest score (in fp32: rounding keeps their order), then
+// the keys of the one bin that holds it by their ranks; where that bin has more than NT keys (ties, or an infinity that
+// stretches the range), by bytes from the top instead. Then one pass in index order. Bound by latency (barriers and LDS): 9 us
 // with a byte-wise threshold and a barrier pair per NT keys of the last pass, at 2046 pages.
 template <int NT, int EACH>
 __global__ __launch_bounds__(NT) void block_select_kernel(PagedArgs a) {
@@ -714,7 +799,7 @@ __global__ __launch_bounds__(NT) void block_select_kernel(PagedArgs a) {
     constexpr int U = REG ? EACH : 1;
     __shared__ int hist[BINS];
     __shared__ int tmp[NW], pick[3], found;
-    __shared__ uint32_t lo_w[NW], hi_w[NW];
+    __shared__ float lo_w[NW], hi_w[NW];
     __shared__ uint64_t cand[NT], thr;
     __shared__ int pre[2][NW * EACH];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
@@ -743,7 +828,7 @@ __global__ __launch_bounds__(NT) void block_select_kernel(PagedArgs a) {
     if (want == 0) return;
     const uint64_t* keys = a.keys + unit * a.W;
     uint64_t kept[U];
-    uint32_t lo = 0xFFFFFFFFu, hi = 0;
+    float lo = INFINITY, hi = -INFINITY;
     if constexpr (REG)
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
@@ -755,16 +840,22 @@ __global__ __launch_bounds__(NT) void block_select_kernel(PagedArgs a) {
         if constexpr (REG) return kept[i];
         return live(i) ? keys[j0 + i * NT + tid] : 0;
     };
+    // a key's score in fp32, a quarter of it (the range stays finite); a NaN's is the lowest there is
+    auto score = [](uint64_t x) {
+        if (x == 0) return -0.25f * 3.402823466e38f;
+        const double d = __builtin_bit_cast(double, x >> 63 ? x & ~(uint64_t(1) << 63) : ~x);
+        return 0.25f * fminf(fmaxf(float(d), -3.402823466e38f), 3.402823466e38f);
+    };
 #pragma unroll U
     for (int i = 0; i < EACH; ++i)
         if (live(i)) {
-            const uint32_t x = uint32_t(key(i) >> 32);
-            lo = min(lo, x);
-            hi = max(hi, x);
+            const float x = score(key(i));
+            lo = fminf(lo, x);
+            hi = fmaxf(hi, x);
         }
     for (int d = 32; d; d >>= 1) {
-        lo = min(lo, uint32_t(__shfl_xor(int(lo), d, 64)));
-        hi = max(hi, uint32_t(__shfl_xor(int(hi), d, 64)));
+        lo = fminf(lo, __shfl_xor(lo, d, 64));
+        hi = fmaxf(hi, __shfl_xor(hi, d, 64));
     }
     for (int i = tid; i < BINS; i += NT) hist[i] = 0;
     if (lane == 0) {
@@ -775,11 +866,11 @@ __global__ __launch_bounds__(NT) void block_select_kernel(PagedArgs a) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < NW; ++i) {
-        lo = min(lo, lo_w[i]);
-        hi = max(hi, hi_w[i]);
+        lo = fminf(lo, lo_w[i]);
+        hi = fmaxf(hi, hi_w[i]);
     }
-    const int sh = max(0, 22 - int(__builtin_clz((hi - lo) | 1u)));  // (hi - lo) >> sh < 1024
-    auto bin = [&](uint64_t x) { return int((uint32_t(x >> 32) - lo) >> sh); };
+    const float per = hi - lo > 1e-30f ? float(BINS - 1) / (hi - lo) : 0.f;
+    auto bin = [&](uint64_t x) { return int(fminf((score(x) - lo) * per, float(BINS - 1))); };
 #pragma unroll U
     for (int i = 0; i < EACH; ++i)
         if (live(i)) atomicAdd(&hist[bin(key(i))], 1);
