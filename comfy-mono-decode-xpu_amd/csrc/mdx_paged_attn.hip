@@ -91,6 +91,7 @@ struct PagedArgs {
     int B, S, H, Hk, G, W, P, lt;
     int units;  // units of a sequence and kv head: row blocks, or rows with a selection each
     int rows;   // query rows of a kv head in a unit's family: S G, or G with a selection
+    int whole;  // every work-group takes one whole unit (no join)
     float zs;   // scale * log2(e)
 };
 
@@ -98,6 +99,8 @@ constexpr int MAX_SEQS = 1024;
 constexpr int STEP = 32;
 constexpr int GRID = 256;
 constexpr int RING_BYTES = 128 * 1024;
+constexpr int64_t FEW_STEPS = 2048;  // 128-token steps of a call at most, for the forms that go by latency
+constexpr int64_t WHOLE_TOKENS = 640;  // tokens a unit can have at most, for one work-group per unit
 
 __device__ __forceinline__ uint32_t lds_addr(const void* p) {
     return uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const unsigned char*)p));
@@ -248,8 +251,17 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
     const int rw = w % RTW, part = w / RTW;
 
     // ---- this work-group's share of the line of steps: [begin, end), and the sequence it begins in
-    int begin, end, quota, b, in_b;
-    {
+    int begin, end, quota, b, in_b, kh = 0, u = 0;
+    Span sp;
+    if (a.whole) {  // unit (b, kh, u) of the grid
+        u = int(blockIdx.x) % a.units;
+        kh = int(blockIdx.x) / a.units % a.Hk;
+        b = int(blockIdx.x) / a.units / a.Hk;
+        sp = span_of<SEL>(a, uload(a.length + b));
+        begin = in_b = 0;
+        end = quota = steps_of<SEL>(a, sp, u, RPW, TOK);
+        if (tid == 0) odd = 0;
+    } else {
         constexpr int EACH = (MAX_SEQS + NT - 1) / NT;
         int mine[EACH], sum = 0;
 #pragma unroll
@@ -293,20 +305,15 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
         __syncthreads();
         b = __builtin_amdgcn_readfirstlane(sh_at[0]);
         in_b = begin - __builtin_amdgcn_readfirstlane(sh_at[1]);
-    }
-    if (tid == 0) {
-        a.info[blockIdx.x] = make_int4(0, 0, 0, 0);
-        odd = 0;
-    }
-    if (begin >= end) return;  // (uniform)
-    __syncthreads();
-    begin = __builtin_amdgcn_readfirstlane(begin);
-    end = __builtin_amdgcn_readfirstlane(end);
-
-    // the unit the share begins in
-    Span sp = span_of<SEL>(a, uload(a.length + b));
-    int kh = 0, u = 0;
-    {
+        if (tid == 0) {
+            a.info[blockIdx.x] = make_int4(0, 0, 0, 0);
+            odd = 0;
+        }
+        if (begin >= end) return;  // (uniform)
+        begin = __builtin_amdgcn_readfirstlane(begin);
+        end = __builtin_amdgcn_readfirstlane(end);
+        // the unit the share begins in
+        sp = span_of<SEL>(a, uload(a.length + b));
         int all = 0;
         for (int i = 0; i < a.units; ++i) all += steps_of<SEL>(a, sp, i, RPW, TOK);
         kh = in_b / all;
@@ -317,6 +324,7 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
             in_b -= n;
         }
     }
+    __syncthreads();  // (odd)
     int at = begin, step0 = in_b;  // line position, and the unit's step there
 
     unsigned char* ring = smem + part * NS * 2 * STAGE;
@@ -1009,6 +1017,11 @@ int launch(const PagedArgs& a, hipStream_t st) {
         allow_smem(reinterpret_cast<const void*>(&paged_attn_kernel<E, D, TPW, RTW, P, SEL>), lds);
         allowed.fetch_or(bit, std::memory_order_relaxed);
     }
+    if (a.whole) {
+        hipLaunchKernelGGL((paged_attn_kernel<E, D, TPW, RTW, P, SEL>), dim3(unsigned(a.B * a.Hk * a.units)), dim3(Geo::NT), lds, st, a);
+        MDX_LAUNCHED();
+        return MDX_OK;
+    }
     hipLaunchKernelGGL((paged_attn_kernel<E, D, TPW, RTW, P, SEL>), dim3(GRID), dim3(Geo::NT), lds, st, a);
     MDX_LAUNCHED();
     const int rows = a.rows < Geo::RPW ? a.rows : Geo::RPW;
@@ -1017,32 +1030,38 @@ int launch(const PagedArgs& a, hipStream_t st) {
     return MDX_OK;
 }
 
-// query rows of a work-group: what covers the rows of a kv head with as few row blocks as registers allow
-template <int D>
-int rows_per_wg(int rows) {
-    if (rows <= 16) return 16;
-    if (rows <= 32) return 32;
-    if (rows <= 64) return 64;
-    return 128;
+// Query rows of a work-group: what covers the rows of a kv head with as few row blocks as registers allow.
+int rpw_of(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+
+// The most tokens a unit can have: all that the table (or a selection) holds, and the rows' own.
+int64_t most_tokens(const PagedArgs& a, bool sel) {
+    const int64_t pages = sel && a.most < a.W ? a.most + 1 : a.W;
+    return (pages << a.lt) + a.S;
 }
 
+// Row tiles in one wave's registers (each K and V operand read from LDS once for all) where there is much to stream, in
+// waves of their own where a unit's few steps count by their latency.
 template <class E, int D, bool SEL>
-int launch_rows(const PagedArgs& a, hipStream_t st) {
+int launch_rows(PagedArgs& a, hipStream_t st) {
+    const int64_t steps = int64_t(a.B) * a.Hk * a.units * ((most_tokens(a, SEL) + 127) / 128);
+    const bool few = steps <= FEW_STEPS;
     if (a.rows <= 16) return launch<E, D, 1, 1, 4, SEL>(a, st);
-    if (a.rows <= 32) return launch<E, D, 2, 1, 4, SEL>(a, st);
-    if constexpr (D == 256) {
-        if (a.rows <= 64) return launch<E, D, 2, 2, 2, SEL>(a, st);
-        if constexpr (!SEL) return launch<E, D, 2, 4, 1, SEL>(a, st);
-    } else {
-        if (a.rows <= 64) return launch<E, D, 4, 1, 4, SEL>(a, st);
-        if constexpr (!SEL) return launch<E, D, 2, 4, 2, SEL>(a, st);
+    if (a.rows <= 32) {
+        if (few) return launch<E, D, 1, 2, (D == 256 ? 2 : 4), SEL>(a, st);
+        return launch<E, D, 2, 1, 4, SEL>(a, st);
     }
+    if (a.rows <= 64) {
+        if (few) return launch<E, D, 1, 4, (D == 256 ? 1 : 2), SEL>(a, st);
+        if constexpr (D == 256) return launch<E, D, 2, 2, 2, SEL>(a, st);
+        else return launch<E, D, 4, 1, 4, SEL>(a, st);
+    }
+    if constexpr (!SEL) return launch<E, D, 2, 4, (D == 256 ? 1 : 2), SEL>(a, st);
     set_error("at most 64 query heads per kv head");
     return MDX_EINVAL;
 }
 
 template <bool SEL>
-int launch_any(const PagedArgs& a, int D, int dtype, hipStream_t st) {
+int launch_any(PagedArgs& a, int D, int dtype, hipStream_t st) {
     if (dtype == MDX_DT_BF16) {
         if (D == 64) return launch_rows<Bf16, 64, SEL>(a, st);
         if (D == 128) return launch_rows<Bf16, 128, SEL>(a, st);
@@ -1052,8 +1071,6 @@ int launch_any(const PagedArgs& a, int D, int dtype, hipStream_t st) {
     if (D == 128) return launch_rows<Fp16, 128, SEL>(a, st);
     return launch_rows<Fp16, 256, SEL>(a, st);
 }
-
-int rpw_of(int64_t rows) { return rows_per_wg<128>(int(rows > 128 ? 128 : rows)); }
 
 size_t base_bytes(int64_t rows, int64_t D) {
     return size_t(GRID) * sizeof(int4) + size_t(GRID) * 2 * rpw_of(rows) * (D + 2) * 4;
@@ -1111,9 +1128,15 @@ int fill(PagedArgs& a, const void* q, int64_t q_seq_stride, int64_t q_row_stride
 
 using namespace mdx;
 
-extern "C" size_t mdx_attn_paged_workspace(int64_t S, int64_t H, int64_t Hk, int64_t D) {
-    if (S < 1 || Hk < 1 || H < 1 || H % Hk != 0 || D < 1) return 0;
-    return base_bytes(S * (H / Hk), D);
+// One work-group per unit, without a join: where a unit has few steps at most.
+static bool whole_units(int64_t B, int64_t S, int64_t H, int64_t Hk, int64_t T, int64_t W) {
+    const int64_t rows = S * (H / Hk), rpw = rpw_of(rows);
+    return W * T + S <= WHOLE_TOKENS && B * Hk * ((rows + rpw - 1) / rpw) <= 65536;
+}
+
+extern "C" size_t mdx_attn_paged_workspace(int64_t B, int64_t S, int64_t H, int64_t Hk, int64_t D, int64_t T, int64_t W) {
+    if (B < 1 || S < 1 || Hk < 1 || H < 1 || H % Hk != 0 || D < 1 || T < 1 || W < 1 || W > (int64_t(1) << 30)) return 0;
+    return whole_units(B, S, H, Hk, T, W) ? 0 : base_bytes(S * (H / Hk), D);
 }
 
 extern "C" int mdx_attn_paged(const void* q, int64_t q_seq_stride, int64_t q_row_stride, int64_t q_head_stride, const void* key,
@@ -1133,8 +1156,9 @@ extern "C" int mdx_attn_paged(const void* q, int64_t q_seq_stride, int64_t q_row
     const int64_t blocks = (rows + rpw - 1) / rpw;
     MDX_CHECK(rows < (int64_t(1) << 30) && B * Hk * blocks * ((W * T + S) / STEP + 1) < (int64_t(1) << 31),
               "too many rows times tokens for one call");
-    MDX_CHECK(workspace && aligned(workspace, 16) && workspace_bytes >= base_bytes(rows, D), "workspace: %zu bytes, 16-byte aligned",
-              base_bytes(rows, D));
+    a.whole = whole_units(B, S, H, Hk, T, W);
+    MDX_CHECK(a.whole || (workspace && aligned(workspace, 16) && workspace_bytes >= base_bytes(rows, D)),
+              "workspace: %zu bytes, 16-byte aligned", base_bytes(rows, D));
     a.rows = int(rows);
     a.units = int(blocks);
     a.info = static_cast<int4*>(workspace);

@@ -1297,7 +1297,7 @@ def _ws_bytes(name, *sizes):
     if n is None:
         if len(_WS_BYTES) > 4096:
             _WS_BYTES.clear()
-        n = _WS_BYTES[name, sizes] = getattr(_lib.lib(), name)(*sizes) or 16
+        n = _WS_BYTES[name, sizes] = getattr(_lib.lib(), name)(*sizes)
     return n
 
 
@@ -1441,10 +1441,10 @@ def attn_paged(q, key, value, table, length, mask=None, scale=None, out=None):
     d, out, args, (dt, B, S, H, Hk, D, P, T, W, ts) = _paged(q, key, value, table, length, mask, out)
     if B == 0 or S == 0:
         return out
-    nb = _ws_bytes("mdx_attn_paged_workspace", S, H, Hk, D)
-    ws = torch.empty(nb, dtype=torch.uint8, device=q.device)
+    nb = _ws_bytes("mdx_attn_paged_workspace", B, S, H, Hk, D, T, W)
+    ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
     _lib.call_on(d, "mdx_attn_paged", *args, dt, table.data_ptr(), ts, length.data_ptr(), _lib.ptr(mask), out.data_ptr(), B, S, H,
-                 Hk, D, P, T, W, D ** -0.5 if scale is None else float(scale), ws.data_ptr(), nb)
+                 Hk, D, P, T, W, D ** -0.5 if scale is None else float(scale), _lib.ptr(ws), nb)
     return out
 
 

@@ -155,7 +155,7 @@ SIGNATURES = {
     "mdx_page_commit": (ctypes.c_int, [c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p,
                                        c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
                                        c_int64, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
-    "mdx_attn_paged_workspace": (c_size_t, [c_int64, c_int64, c_int64, c_int64]),
+    "mdx_attn_paged_workspace": (c_size_t, [c_int64] * 7),
     "mdx_attn_paged": (ctypes.c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p,
                                       c_int64, c_int64, c_int64, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
                                       c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, ctypes.c_float,

@@ -8,10 +8,10 @@ pytestmark = pytest.mark.gpu
 BF, FH = torch.bfloat16, torch.float16
 
 
-def _run(C, dev, dt, H, Hk, D, T, lens, S, tree, seed=0):
-    print(f"attn_paged {dt} H={H} Hk={Hk} D={D} T={T} lens={lens} S={S} tree={tree}", flush=True)
+def _run(C, dev, dt, H, Hk, D, T, lens, S, tree, seed=0, width=1):
+    print(f"attn_paged {dt} H={H} Hk={Hk} D={D} T={T} lens={lens} S={S} tree={tree} width={width}", flush=True)
     g = torch.Generator().manual_seed(seed + D + T + S)
-    key, value, table = cache(g, dt, Hk, T, D, lens, S)
+    key, value, table = cache(g, dt, Hk, T, D, lens, S, width=width)
     q = (torch.randn(len(lens), S, H, D, generator=g) * 1.5).to(dt)
     mask = tree_masks(g, len(lens), S) if tree else None
     n = torch.tensor(lens, dtype=torch.int32, device=dev)
@@ -36,6 +36,15 @@ def test_page_sizes(C, dev, T, D):
 @pytest.mark.parametrize("dt", [BF, FH])
 def test_trees(C, dev, dt, H, Hk, D, S):
     _run(C, dev, dt, H, Hk, D, 64, [0, 70, 257], S, True, H)
+
+
+@pytest.mark.parametrize("H,Hk,D,S", [(32, 8, 128, 1), (32, 8, 128, 5), (32, 8, 128, 16), (16, 4, 256, 3), (16, 4, 256, 8), (16, 4, 256, 16),
+                                      (16, 8, 64, 3), (16, 8, 64, 12), (16, 8, 64, 30), (8, 8, 256, 64)])
+@pytest.mark.parametrize("dt", [BF, FH])
+@pytest.mark.parametrize("width", [12, 6000])
+def test_tables_wider_than_the_sequences(C, dev, dt, H, Hk, D, S, width):
+    """The forms go by what the table could hold: the same rows through those for much to stream."""
+    _run(C, dev, dt, H, Hk, D, 64, [0, 70, 400, 129], S, S > 1, H, width)
 
 
 @pytest.mark.parametrize("H,Hk,D,S,lens", [(32, 8, 128, 65, [0, 40]), (8, 2, 128, 300, [129]), (4, 1, 256, 130, [7, 64]), (8, 4, 64, 513, [0]),
@@ -116,10 +125,11 @@ def test_bad_pages_are_not_attended(C, dev, T, S):
 
 @pytest.mark.parametrize("dt", [BF, FH])
 @pytest.mark.parametrize("D", [64, 128, 256])
-@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
-def test_non_finite_in_places_that_are_not_admitted(C, dev, dt, D, bad):
+@pytest.mark.parametrize("bad,width", [(float("nan"), 1), (float("inf"), 1), (float("-inf"), 1), (float("nan"), 40), (float("nan"), 20000)])
+def test_non_finite_in_places_that_are_not_admitted(C, dev, dt, D, bad, width):
     """K and V of one own row non-finite: the rows that do not admit it are as without it; a row that admits it shows it."""
     _, q, key, value, table, lens, n, _ = _small(dev, dt=dt, D=D, lens=(40, 0, 31), S=4)
+    table = torch.nn.functional.pad(table, (0, width), value=-1)
     mask = torch.tensor([[1, 3, 5, 9]] * 3)  # rows 1, 2, 3 children of 0
     for b, t in enumerate(lens):
         key[:, table[b, (t + 2) // 16], (t + 2) % 16] = bad

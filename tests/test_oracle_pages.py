@@ -90,8 +90,8 @@ def test_refusals_before_any_device_work():
     from mdx import _lib
     A = 1 << 12  # an aligned address that nothing reads
 
-    def attn(q=A, key=A, value=A, dt=_lib.DT_BF16, table=A, length=A, mask=None, out=A, B=1, S=1, H=4, Hk=2, D=128, P=8, T=16, W=4,
-             scale=0.1, ws=A, nb=1 << 40, kt=128, kp=2048, qs=512, ts=4):
+    def attn(q=A, key=A, value=A, dt=_lib.DT_BF16, table=A, length=A, mask=None, out=A, B=1, S=1, H=4, Hk=2, D=128, P=8, T=16, W=400,
+             scale=0.1, ws=A, nb=1 << 40, kt=128, kp=2048, qs=512, ts=400):
         return _lib.lib().mdx_attn_paged(q, 512, qs, 128, key, kp * 8, kp, kt, value, kp * 8, kp, kt, dt, table, ts, length, mask,
                                          out, B, S, H, Hk, D, P, T, W, scale, ws, nb, None)
 
