@@ -89,8 +89,8 @@ struct PagedArgs {
     int4* info;      // [work-groups]: the unit left open, and the shares it has from there
     float* part;     // [2 work-groups][rows][D + 2]: O, maximum, sum
     int B, S, H, Hk, G, W, P, lt;
-    int units;  // units of a sequence and kv head: row blocks, or rows with a selection each
-    int rows;   // query rows of a kv head in a unit's family: S G, or G with a selection
+    int units;  // units of a sequence and kv head: blocks of spb rows s (1 with a selection each)
+    int spb;    // a unit's query rows: s from u spb, each with the kv head's G heads
     int whole;  // every work-group takes one whole unit (no join)
     float zs;   // scale * log2(e)
 };
@@ -194,6 +194,13 @@ __device__ __forceinline__ void read_v(u32x2 (&va)[D == 64 ? 4 : 8], u32x2 (&vb)
 typedef __attribute__((address_space(4))) const int32_t* const_i32p;
 __device__ __forceinline__ int uload(const int32_t* p) { return *(const_i32p)(p); }  // (a scalar load: uniform addresses)
 
+// the largest of three (a NaN counts as the smallest; fmaxf would first make every operand a quiet one)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
 // what a wave may have in flight behind the load it waits for (vmcnt only)
 template <int N>
 __device__ __forceinline__ void wait_vm() {
@@ -216,16 +223,10 @@ __device__ __forceinline__ Span span_of(const PagedArgs& a, int n) {
     const int c = n >> a.lt, k = c < a.most ? c : a.most;
     return {n, (k << a.lt) + (n - (c << a.lt)), k << a.lt, c << a.lt};
 }
-// steps of unit u of a sequence (RPW: query rows of a row block)
-template <bool SEL>
-__device__ __forceinline__ int steps_of(const PagedArgs& a, const Span& s, int u, int rpw, int tokens_per_step) {
-    int own = a.S;
-    if (!SEL && !a.mask) {  // (a chain's row block ends with its last row's own token)
-        const int last = min(a.rows, (u + 1) * rpw) - 1;
-        own = last / a.G + 1;
-    }
-    if (SEL && !a.mask) own = u + 1;  // (unit u is row u)
-    return (s.tree0 + own + tokens_per_step - 1) / tokens_per_step;
+// own tokens that unit u attends at most (a chain's unit ends with its last row's), and its steps
+__device__ __forceinline__ int own_of(const PagedArgs& a, int u) { return a.mask ? a.S : min(a.S, (u + 1) * a.spb); }
+__device__ __forceinline__ int steps_of(const PagedArgs& a, const Span& s, int u, int tokens_per_step) {
+    return (s.tree0 + own_of(a, u) + tokens_per_step - 1) / tokens_per_step;
 }
 
 // One work-group: RTW waves of row tiles (TPW tiles of 16 query rows each) times P token parts.
@@ -245,10 +246,13 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
     constexpr int NT = Geo::NT, RPW = Geo::RPW, STAGE = Geo::STAGE, NS = Geo::NS, PER = Geo::PER;
     constexpr int KK = D / 32, DT = D / 16, TOK = STEP * P;
     extern __shared__ __align__(256) unsigned char smem[];  // (the reads' exclusive ors need rows aligned to 256 bytes)
-    __shared__ int sh_sum[NT / 64], sh_at[3], odd;
+    __shared__ int sh_sum[NT / 64], sh_at[4], odd;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, c16 = lane & 15;
     const int rw = w % RTW, part = w / RTW;
+    // Work-groups go to the 8 XCDs in turn: each XCD takes neighbouring shares, so that the row blocks of a kv head, which
+    // read the same K and V, find them in one L2 (a prompt's 2048 rows: 164 us with the shares in turn).
+    const int share = a.whole ? int(blockIdx.x) : int(blockIdx.x) % 8 * (GRID / 8) + int(blockIdx.x) / 8;
 
     // ---- this work-group's share of the line of steps: [begin, end), and the sequence it begins in
     int begin, end, quota, b, in_b, kh = 0, u = 0;
@@ -259,28 +263,33 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
         b = int(blockIdx.x) / a.units / a.Hk;
         sp = span_of<SEL>(a, uload(a.length + b));
         begin = in_b = 0;
-        end = quota = steps_of<SEL>(a, sp, u, RPW, TOK);
+        end = quota = steps_of(a, sp, u, TOK);
         if (tid == 0) odd = 0;
     } else {
-        constexpr int EACH = (MAX_SEQS + NT - 1) / NT;
-        int mine[EACH], sum = 0;
-#pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-            const int bb = tid * EACH + i;
-            mine[i] = 0;
-            if (bb < a.B) {
-                const Span s = span_of<SEL>(a, a.length[bb]);
-                int t = 0;
-                for (int u = 0; u < a.units; ++u) t += steps_of<SEL>(a, s, u, RPW, TOK);
-                mine[i] = t * a.Hk;
+        // The units in the line's order (sequence, kv head, block), a run of neighbouring ones per thread (where a kv head
+        // is one unit, its sequence's kv heads together); the threads' sums, and the unit that the share begins in.
+        const int per_kh = a.units == 1 ? a.Hk : 1, n_items = a.units == 1 ? a.B : a.B * a.Hk * a.units;
+        const int each = (n_items + NT - 1) / NT, i0 = min(tid * each, n_items), i1 = min(i0 + each, n_items);
+        const int per_b = a.units == 1 ? 1 : a.Hk * a.units;
+        // (f(item's sequence, its unit, its steps) over this thread's items)
+        auto walk = [&](auto f) {
+            int bb = i0 / per_b, rest = i0 % per_b, uu = rest % a.units;
+            for (int i = i0; i < i1; ++i) {
+                f(bb, rest, steps_of(a, span_of<SEL>(a, a.length[bb]), uu, TOK));
+                if (++uu == a.units) uu = 0;
+                if (++rest == per_b) {
+                    rest = 0;
+                    ++bb;
+                }
             }
-            sum += mine[i];
-        }
+        };
+        int sum = 0;
+        walk([&](int, int, int n) { sum += n * per_kh; });
         int incl = sum;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
-            const int u = __shfl_up(incl, d, 64);
-            if (lane >= d) incl += u;
+            const int x = __shfl_up(incl, d, 64);
+            if (lane >= d) incl += x;
         }
         if (lane == 63) sh_sum[w] = incl;
         __syncthreads();
@@ -292,37 +301,33 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
             total += x;
         }
         quota = (total + int(gridDim.x) - 1) / int(gridDim.x);
-        begin = int(blockIdx.x) * quota;
+        begin = share * quota;
         end = min(total, begin + quota);
-#pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-            if (begin >= before && begin < before + mine[i]) {
-                sh_at[0] = tid * EACH + i;
-                sh_at[1] = before;
-            }
-            before += mine[i];
-        }
-        __syncthreads();
-        b = __builtin_amdgcn_readfirstlane(sh_at[0]);
-        in_b = begin - __builtin_amdgcn_readfirstlane(sh_at[1]);
+        if (begin >= before && begin < before + sum)
+            walk([&](int bb, int rest, int n) {
+                const int in = begin - before;
+                if (in >= 0 && in < n * per_kh) {
+                    sh_at[0] = bb;
+                    sh_at[1] = a.units == 1 ? in / n : rest / a.units;
+                    sh_at[2] = a.units == 1 ? 0 : rest % a.units;
+                    sh_at[3] = in % n;
+                }
+                before += n * per_kh;
+            });
         if (tid == 0) {
-            a.info[blockIdx.x] = make_int4(0, 0, 0, 0);
+            a.info[share] = make_int4(0, 0, 0, 0);
             odd = 0;
         }
         if (begin >= end) return;  // (uniform)
+        __syncthreads();
         begin = __builtin_amdgcn_readfirstlane(begin);
         end = __builtin_amdgcn_readfirstlane(end);
-        // the unit the share begins in
+        quota = __builtin_amdgcn_readfirstlane(quota);
+        b = __builtin_amdgcn_readfirstlane(sh_at[0]);
+        kh = __builtin_amdgcn_readfirstlane(sh_at[1]);
+        u = __builtin_amdgcn_readfirstlane(sh_at[2]);
+        in_b = __builtin_amdgcn_readfirstlane(sh_at[3]);
         sp = span_of<SEL>(a, uload(a.length + b));
-        int all = 0;
-        for (int i = 0; i < a.units; ++i) all += steps_of<SEL>(a, sp, i, RPW, TOK);
-        kh = in_b / all;
-        in_b -= kh * all;
-        for (;; ++u) {
-            const int n = steps_of<SEL>(a, sp, u, RPW, TOK);
-            if (in_b < n) break;
-            in_b -= n;
-        }
     }
     __syncthreads();  // (odd)
     int at = begin, step0 = in_b;  // line position, and the unit's step there
@@ -336,13 +341,19 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
     // The lane's place within a direct load: token lane / LPR, piece lane % LPR as exchanged; load i of a matrix covers the
     // tokens from TPL i, whose swizzle enters by an exclusive or (swizzle(TPL i + x) = swizzle(TPL i) ^ swizzle(x)).
     const uint32_t piece = ((lane % LPR) ^ swizzle<D>(lane / LPR)) * 16;
+    const uint64_t page_k = uint64_t(a.kp) * 2, page_v = uint64_t(a.vp) * 2;  // (bytes)
+    const uint32_t row_k = uint32_t(a.kt) * 2, row_v = uint32_t(a.vt) * 2;
     const uint32_t k_row = (lane / LPR) * uint32_t(a.kt) * 2, v_row = (lane / LPR) * uint32_t(a.vt) * 2;
 
     while (true) {
-        const int n_unit = steps_of<SEL>(a, sp, u, RPW, TOK);
+        const int n_unit = steps_of(a, sp, u, TOK);
         const int nst = min(n_unit - step0, end - at);  // steps of this unit in the share
-        const int own = (!a.mask && !SEL) ? (min(a.rows, (u + 1) * RPW) - 1) / a.G + 1 : (!a.mask ? u + 1 : a.S);
-        const int t_end = sp.tree0 + own;
+        const int t_end = sp.tree0 + own_of(a, u);
+        const int s_first = u * a.spb, rows = min(a.spb, a.S - s_first) * a.G;  // query rows of the unit
+
+        // tokens that every row of the wave admits (a chain's first row in the wave its own too)
+        const int t_all = sp.tree0 + (a.mask ? 0 : min(a.S, s_first + rw * TPW * 16 / a.G + 1));
+        const int t_none = a.mask ? t_end : min(t_end, sp.tree0 + s_first + ((rw + 1) * TPW * 16 - 1) / a.G + 1);  // from here none
 
         // ---- the pages of a stage (scalar loads ahead of their use), and its direct loads
         const unsigned char* kbase = reinterpret_cast<const unsigned char*>(a.key + kh * a.kh);
@@ -352,40 +363,40 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
         struct Two {
             int e[2];
         };
+        const bool one_page = a.lt >= 5;  // (a stage's 32 tokens stand in one page)
+        auto entry = [&](int v) {
+            if (v >= t_end) return -1;
+            if (SEL && v < sp.nsel) return uload(picked + (v >> a.lt));
+            const int j = (SEL ? sp.tail + (v - sp.nsel) : v) >> a.lt;
+            return j < a.W ? uload(row + j) : -1;
+        };
         auto entries = [&](int s) {
             const int v0 = (step0 + s) * TOK + part * STEP;
             Two x;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int v = v0 + 16 * h;
-                x.e[h] = -1;
-                if (v < t_end) {
-                    if (SEL && v < sp.nsel) {
-                        x.e[h] = uload(picked + (v >> a.lt));
-                    } else {
-                        const int t = SEL ? sp.tail + (v - sp.nsel) : v;
-                        if ((t >> a.lt) < a.W) x.e[h] = uload(row + (t >> a.lt));
-                    }
-                }
-            }
+            x.e[0] = entry(v0);
+            x.e[1] = one_page ? x.e[0] : entry(v0 + 16);
             return x;
         };
         uint32_t hist = 0;  // two bits per stage issued: its halves stand in pages
         const unsigned char *kp_[2], *vp_[2];
         auto place = [&](int s, Two x) {
             const int v0 = (step0 + s) * TOK + part * STEP;
-            uint32_t ok = 0;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int v = v0 + 16 * h, t = SEL && v >= sp.nsel ? v - sp.nsel : v;
-                const int64_t e = x.e[h], r = t & ((1 << a.lt) - 1);
-                const bool in = x.e[h] >= 0 && x.e[h] < a.P;
-                ok |= in ? 1u << h : 0u;
-                // (a half without a page reads the pool's first rows: in bounds, and masked)
-                kp_[h] = kbase + (in ? (e * a.kp + r * a.kt) * 2 : 0);
-                vp_[h] = vbase + (in ? (e * a.vp + r * a.vt) * 2 : 0);
+            const uint32_t r = uint32_t(SEL && v0 >= sp.nsel ? v0 - sp.nsel : v0) & ((1u << a.lt) - 1u);
+            // (a half without a page reads the pool's first rows: in bounds, and masked)
+            const bool in = uint32_t(x.e[0]) < uint32_t(a.P);
+            kp_[0] = kbase + (in ? uint64_t(uint32_t(x.e[0])) * page_k + uint64_t(r) * row_k : 0);
+            vp_[0] = vbase + (in ? uint64_t(uint32_t(x.e[0])) * page_v + uint64_t(r) * row_v : 0);
+            if (one_page) {
+                kp_[1] = kp_[0] + 16 * row_k;
+                vp_[1] = vp_[0] + 16 * row_v;
+                hist = (hist << 2) | (in ? 3u : 0u);
+            } else {
+                const uint32_t r1 = (r + 16) & ((1u << a.lt) - 1u);
+                const bool in1 = uint32_t(x.e[1]) < uint32_t(a.P);
+                kp_[1] = kbase + (in1 ? uint64_t(uint32_t(x.e[1])) * page_k + uint64_t(r1) * row_k : 0);
+                vp_[1] = vbase + (in1 ? uint64_t(uint32_t(x.e[1])) * page_v + uint64_t(r1) * row_v : 0);
+                hist = (hist << 2) | (in ? 1u : 0u) | (in1 ? 2u : 0u);
             }
-            hist = (hist << 2) | ok;
         };
         auto load = [&](const unsigned char* const (&from)[2], uint32_t lane_row, uint32_t stride, unsigned char* dst) {
             constexpr int HALF = 16 / TPL;  // loads of a half
@@ -397,8 +408,8 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
                                                  (__attribute__((address_space(3))) void*)(dst + i * 1024), 16, 0, 0);
             }
         };
-        auto issue_k = [&](int s) { load(kp_, k_row, uint32_t(a.kt) * 2, ring + (s & (NS - 1)) * 2 * STAGE); };
-        auto issue_v = [&](int s) { load(vp_, v_row, uint32_t(a.vt) * 2, ring + (s & (NS - 1)) * 2 * STAGE + STAGE); };
+        auto issue_k = [&](int s) { load(kp_, k_row, row_k, ring + (s & (NS - 1)) * 2 * STAGE); };
+        auto issue_v = [&](int s) { load(vp_, v_row, row_v, ring + (s & (NS - 1)) * 2 * STAGE + STAGE); };
         // A wave with a ring of its own (RTW == 1) fills the whole ring ahead, refills K's slot once it has read K and V's
         // once it has read V, and meets no barrier. Waves that share a ring fill NS - 1 stages ahead and refill the slot of
         // the stage before at the top of a stage, behind the one barrier.
@@ -413,10 +424,8 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
         int lim[TPW];
 #pragma unroll
         for (int t = 0; t < TPW; ++t) {
-            const int r = (SEL ? 0 : u * RPW) + (rw * TPW + t) * 16 + c16;
-            const bool live = r < a.rows;
-            const int rr = live ? r : 0;
-            const int s = SEL ? u : rr / a.G, h = kh * a.G + (SEL ? rr : rr % a.G);
+            const int r = (rw * TPW + t) * 16 + c16, rr = r < rows ? r : 0;
+            const int s = s_first + rr / a.G, h = kh * a.G + rr % a.G;
             const uint16_t* src = a.q + b * a.qb + s * a.qs + h * a.qh + 8 * g;
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk) qf[t][kk] = *reinterpret_cast<const u32x4*>(src + 32 * kk);
@@ -471,6 +480,8 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
                     next_e = entries(s + AHEAD + 1);
                 }
             }
+            const int v0 = (step0 + s) * TOK + part * STEP;
+            if (RTW > 1 && v0 >= t_none) continue;  // (uniform in the wave: only its loads and the barriers are left)
             f32x4 st[TPW][2];
             auto scores = [&](const u32x4 (&k)[KK], int h) {
 #pragma unroll
@@ -501,8 +512,7 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
                 scores(kf[1], 1);
             }
 
-            const int v0 = (step0 + s) * TOK + part * STEP;
-            const bool whole = ok == 3u && v0 + STEP <= sp.tree0;  // (uniform) every row admits all 32 tokens
+            const bool whole = ok == 3u && v0 + STEP <= t_all;  // (uniform in the wave) every row admits all 32 tokens
             u32x4 pf[TPW];
             uint32_t in[TPW];
 #pragma unroll
@@ -529,13 +539,12 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
                         for (int i = 0; i < 4; ++i)
                             if (!((lb >> (16 * h + i)) & 1u)) st[t][h][i] = -INFINITY;
                 }
-                float mx = fmaxf(fmaxf(fmaxf(st[t][0][0], st[t][0][1]), fmaxf(st[t][0][2], st[t][0][3])),
-                                 fmaxf(fmaxf(st[t][1][0], st[t][1][1]), fmaxf(st[t][1][2], st[t][1][3])));
-                mx = max_x32(max_x16(mx));
-                const float mnew = fmaxf(m[t], mx);
+                float mx = max3(max3(st[t][0][0], st[t][0][1], st[t][0][2]), max3(st[t][0][3], st[t][1][0], st[t][1][1]),
+                                max3(st[t][1][2], st[t][1][3], m[t]));
+                const float mnew = max_x32(max_x16(mx));
                 // a row with nothing admitted yet subtracts 0, so -inf - -inf never forms
-                const float mz = (mnew == -INFINITY ? 0.f : mnew) * a.zs - E::SHIFT;
-                const float alpha = __builtin_amdgcn_exp2f(fmaf(m[t], a.zs, -mz) - E::SHIFT);
+                const float msub = mnew == -INFINITY ? 0.f : mnew, mz = msub * a.zs - E::SHIFT;
+                const float alpha = __builtin_amdgcn_exp2f((m[t] - msub) * a.zs);  // (exactly 1 where the maximum stays)
                 m[t] = mnew;
                 float ps = 0.f;
 #pragma unroll
@@ -601,7 +610,7 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
         constexpr int OR = D + 4;
         float* const lo = reinterpret_cast<float*>(smem);               // [RTW][P][16][OR]
         float* const lm = lo + RTW * P * 16 * OR;                       // [RTW][P][16] maxima (log2 units), then sums
-        float* rec = a.part + (int64_t(blockIdx.x) * 2 + (first ? 1 : 0)) * RPW * (D + 2);
+        float* rec = a.part + (int64_t(share) * 2 + (first ? 1 : 0)) * RPW * (D + 2);
         __syncthreads();  // the ring is free
 #pragma unroll
         for (int t = 0; t < TPW; ++t) {
@@ -618,8 +627,8 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
             for (int x = tid; x < RTW * 16 * (D / 4); x += NT) {
                 const int rt = x / (16 * (D / 4)), rr = x / (D / 4) % 16, d = x % (D / 4) * 4;
                 const int r = (rt * TPW + t) * 16 + rr;  // row of the unit's block
-                const int rg = (SEL ? 0 : u * RPW) + r;
-                if (rg >= a.rows) continue;
+                if (r >= rows) continue;
+                const int s = s_first + r / a.G, h = kh * a.G + r % a.G;
                 float M = -INFINITY;
 #pragma unroll
                 for (int p = 0; p < P; ++p) M = fmaxf(M, lm[(rt * P + p) * 16 + rr]);
@@ -633,7 +642,6 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
                     o += *reinterpret_cast<const f32x4*>(lo + (rt * P + p) * 16 * OR + rr * OR + d) * wp;
                 }
                 if (odd) {  // (uniform: what the stages left out, for the rows that admit it)
-                    const int s = SEL ? u : rg / a.G;
                     for (int v = step0 * TOK; v < min(t_end, (step0 + nst) * TOK); ++v) {
                         const int own_row = v - sp.tree0;
                         if (own_row >= 0 && !(a.mask ? (uint64_t(a.mask[int64_t(b) * a.S + s]) >> own_row) & 1 : own_row <= s)) continue;
@@ -652,7 +660,6 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
                 }
                 if (first && last) {
                     const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
-                    const int s = SEL ? u : rg / a.G, h = kh * a.G + (SEL ? rg : rg % a.G);
                     // (no token admitted: 0, whatever o holds)
                     *reinterpret_cast<uint2*>(a.out + ((int64_t(b) * a.S + s) * a.H + h) * D + d) =
                         sum == 0.f ? make_uint2(0u, 0u) : make_uint2(E::pair(o[0] * inv, o[1] * inv), E::pair(o[2] * inv, o[3] * inv));
@@ -669,7 +676,7 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
         if (first && !last && tid == 0) {
             // the unit goes on in the shares behind: how many in all
             const int left = n_unit - nst;
-            a.info[blockIdx.x] = make_int4(b, kh, u, 1 + (left + quota - 1) / quota);
+            a.info[share] = make_int4(b, kh, u, 1 + (left + quota - 1) / quota);
         }
 
         // ---- the next unit
@@ -694,12 +701,12 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
 
 // The units that several shares worked on: one wave per query row, work-groups (share, four rows). D / 4 lanes take a
 // partial's row in 16-byte pieces, 256 / D partials at once.
-template <class E, int D, bool SEL>
+template <class E, int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int rpw) {
     const int4 x = a.info[blockIdx.x];
     const int nseg = x.w, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int r = int(blockIdx.y) * 4 + w, rg = (SEL ? 0 : x.z * rpw) + r;
-    if (nseg == 0 || rg >= a.rows) return;  // (uniform in the wave)
+    const int r = int(blockIdx.y) * 4 + w, s = x.z * a.spb + r / a.G, h = x.y * a.G + r % a.G;
+    if (nseg == 0 || r >= a.spb * a.G || s >= a.S) return;  // (uniform in the wave)
     constexpr int TPR = D / 4, NG = 64 / TPR;
     const int gi = lane / TPR, d = lane % TPR * 4;
     const int64_t rec = int64_t(rpw) * (D + 2);
@@ -725,7 +732,6 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int rpw) {
     }
     if (gi != 0) return;
     const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
-    const int s = SEL ? x.z : rg / a.G, h = x.y * a.G + (SEL ? rg : rg % a.G);
     *reinterpret_cast<uint2*>(a.out + ((int64_t(x.x) * a.S + s) * a.H + h) * D + d) =
         sum == 0.f ? make_uint2(0u, 0u) : make_uint2(E::pair(o[0] * inv, o[1] * inv), E::pair(o[2] * inv, o[3] * inv));
 }
@@ -1024,8 +1030,8 @@ int launch(const PagedArgs& a, hipStream_t st) {
     }
     hipLaunchKernelGGL((paged_attn_kernel<E, D, TPW, RTW, P, SEL>), dim3(GRID), dim3(Geo::NT), lds, st, a);
     MDX_LAUNCHED();
-    const int rows = a.rows < Geo::RPW ? a.rows : Geo::RPW;
-    hipLaunchKernelGGL((paged_join_kernel<E, D, SEL>), dim3(GRID, unsigned((rows + 3) / 4)), dim3(256), 0, st, a, Geo::RPW);
+    const int rows = (a.spb < a.S ? a.spb : a.S) * a.G;
+    hipLaunchKernelGGL((paged_join_kernel<E, D>), dim3(GRID, unsigned((rows + 3) / 4)), dim3(256), 0, st, a, Geo::RPW);
     MDX_LAUNCHED();
     return MDX_OK;
 }
@@ -1043,14 +1049,15 @@ int64_t most_tokens(const PagedArgs& a, bool sel) {
 // waves of their own where a unit's few steps count by their latency.
 template <class E, int D, bool SEL>
 int launch_rows(PagedArgs& a, hipStream_t st) {
+    const int rows = SEL ? a.G : a.units > 1 ? 128 : a.S * a.G;
     const int64_t steps = int64_t(a.B) * a.Hk * a.units * ((most_tokens(a, SEL) + 127) / 128);
     const bool few = steps <= FEW_STEPS;
-    if (a.rows <= 16) return launch<E, D, 1, 1, 4, SEL>(a, st);
-    if (a.rows <= 32) {
+    if (rows <= 16) return launch<E, D, 1, 1, 4, SEL>(a, st);
+    if (rows <= 32) {
         if (few) return launch<E, D, 1, 2, (D == 256 ? 2 : 4), SEL>(a, st);
         return launch<E, D, 2, 1, 4, SEL>(a, st);
     }
-    if (a.rows <= 64) {
+    if (rows <= 64) {
         if (few) return launch<E, D, 1, 4, (D == 256 ? 1 : 2), SEL>(a, st);
         if constexpr (D == 256) return launch<E, D, 2, 2, 2, SEL>(a, st);
         else return launch<E, D, 4, 1, 4, SEL>(a, st);
@@ -1128,10 +1135,13 @@ int fill(PagedArgs& a, const void* q, int64_t q_seq_stride, int64_t q_row_stride
 
 using namespace mdx;
 
+// Rows s of a unit (a work-group's rows hold whole groups of heads), and a kv head's units.
+static int64_t rows_of_unit(int64_t S, int64_t G) { return rpw_of(S * G) / G; }
+static int64_t blocks_of(int64_t S, int64_t G) { return G > 128 ? 0 : (S + rows_of_unit(S, G) - 1) / rows_of_unit(S, G); }
+
 // One work-group per unit, without a join: where a unit has few steps at most.
 static bool whole_units(int64_t B, int64_t S, int64_t H, int64_t Hk, int64_t T, int64_t W) {
-    const int64_t rows = S * (H / Hk), rpw = rpw_of(rows);
-    return W * T + S <= WHOLE_TOKENS && B * Hk * ((rows + rpw - 1) / rpw) <= 65536;
+    return W * T + S <= WHOLE_TOKENS && B * Hk * blocks_of(S, H / Hk) <= 65536;
 }
 
 extern "C" size_t mdx_attn_paged_workspace(int64_t B, int64_t S, int64_t H, int64_t Hk, int64_t D, int64_t T, int64_t W) {
@@ -1151,15 +1161,14 @@ extern "C" int mdx_attn_paged(const void* q, int64_t q_seq_stride, int64_t q_row
                         v_head_stride, v_page_stride, v_row_stride, dtype, table, table_stride, length, mask, out, B, S, H, Hk, D, P,
                         T, W, scale);
     if (rc != MDX_OK) return rc;
-    const int64_t rows = S * (H / Hk);
-    const int rpw = rpw_of(rows);
-    const int64_t blocks = (rows + rpw - 1) / rpw;
-    MDX_CHECK(rows < (int64_t(1) << 30) && B * Hk * blocks * ((W * T + S) / STEP + 1) < (int64_t(1) << 31),
+    MDX_CHECK(H / Hk <= 128, "at most 128 query heads per kv head");
+    const int64_t rows = S * (H / Hk), blocks = blocks_of(S, H / Hk);
+    MDX_CHECK(rows < (int64_t(1) << 30) && B * Hk * blocks < (int64_t(1) << 30) && B * Hk * blocks * ((W * T + S) / STEP + 1) < (int64_t(1) << 31),
               "too many rows times tokens for one call");
     a.whole = whole_units(B, S, H, Hk, T, W);
     MDX_CHECK(a.whole || (workspace && aligned(workspace, 16) && workspace_bytes >= base_bytes(rows, D)),
               "workspace: %zu bytes, 16-byte aligned", base_bytes(rows, D));
-    a.rows = int(rows);
+    a.spb = int(rows_of_unit(S, H / Hk));
     a.units = int(blocks);
     a.info = static_cast<int4*>(workspace);
     a.part = reinterpret_cast<float*>(a.info + GRID);
@@ -1197,7 +1206,7 @@ extern "C" int mdx_attn_blocks(const void* q, int64_t q_seq_stride, int64_t q_ro
               "too many rows times tokens for one call");
     const size_t need = mdx_attn_blocks_workspace(B, S, H, Hk, D, W, most);
     MDX_CHECK(workspace && aligned(workspace, 16) && workspace_bytes >= need, "workspace: %zu bytes, 16-byte aligned", need);
-    a.rows = int(H / Hk);
+    a.spb = 1;
     a.units = int(S);
     a.most = int(most), a.sink = int(sink), a.local = int(local);
     a.ksum = static_cast<const uint16_t*>(ksum);
@@ -1205,7 +1214,7 @@ extern "C" int mdx_attn_blocks(const void* q, int64_t q_seq_stride, int64_t q_ro
     a.sel = sel;
     a.info = static_cast<int4*>(workspace);
     a.part = reinterpret_cast<float*>(a.info + GRID);
-    a.keys = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + base_bytes(a.rows, D));
+    a.keys = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + base_bytes(a.G, D));
     a.page = reinterpret_cast<int32_t*>(a.keys + units * W);
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (W > most) {  // (else every full page is selected)

@@ -622,7 +622,7 @@ int mdx_page_commit(void* kv, void* ksum, int32_t dtype, int64_t L, int64_t Hk, 
  * (S <= 65535); 0 if there are none. Own tokens are read from the pages too. key / value [Hk, P, T, D] (strides in elements;
  * head, page, row; multiples of 8). out [B, S, H, D] contiguous. fp32 sums, P rounded to the element type. A token in no
  * page is not attended; the contents of places that a row does not attend (non-finite ones too) do not reach it.
- * dtype MDX_DT_BF16 or MDX_DT_F16; D in {64, 128, 256}; B <= 1024; a workspace of 0 bytes may be NULL. The contract of mdx_attn_decode (csrc/attn_dpas.sycl:269-342)
+ * dtype MDX_DT_BF16 or MDX_DT_F16; D in {64, 128, 256}; B <= 1024, H / Hk <= 128; a workspace of 0 bytes may be NULL. The contract of mdx_attn_decode (csrc/attn_dpas.sycl:269-342)
  * for a batch over pages. */
 size_t mdx_attn_paged_workspace(int64_t B, int64_t S, int64_t H, int64_t Hk, int64_t D, int64_t T, int64_t W);
 int mdx_attn_paged(const void* q, int64_t q_seq_stride, int64_t q_row_stride, int64_t q_head_stride, const void* key,

@@ -48,7 +48,8 @@ def test_tables_wider_than_the_sequences(C, dev, dt, H, Hk, D, S, width):
 
 
 @pytest.mark.parametrize("H,Hk,D,S,lens", [(32, 8, 128, 65, [0, 40]), (8, 2, 128, 300, [129]), (4, 1, 256, 130, [7, 64]), (8, 4, 64, 513, [0]),
-                                           (6, 2, 128, 100, [33, 0, 1]), (16, 1, 128, 9, [50]), (8, 1, 64, 40, [500, 3])])
+                                           (6, 2, 128, 100, [33, 0, 1]), (10, 2, 64, 111, [77, 0, 400]), (128, 1, 128, 5, [40]), (100, 1, 64, 3, [0, 70]), (33, 1, 256, 12, [90]),
+                                           (14, 2, 256, 41, [65, 3]), (16, 1, 128, 9, [50]), (8, 1, 64, 40, [500, 3])])
 def test_chains(C, dev, H, Hk, D, S, lens):
     _run(C, dev, BF, H, Hk, D, 32, lens, S, False, 5)
 

@@ -106,7 +106,7 @@ def test_refusals_before_any_device_work():
         return _lib.lib().mdx_page_commit(kv, A, dt, 2, 2, 8, T, D, A, ts, B, W, A, A, A, count, path, R, room, None, A, A, nb, None)
 
     bad = [(attn, dict(q=None)), (attn, dict(length=None)), (attn, dict(dt=_lib.DT_F32)), (attn, dict(D=192)), (attn, dict(T=24)),
-           (attn, dict(T=8)), (attn, dict(T=2048)), (attn, dict(H=5)), (attn, dict(B=0)), (attn, dict(B=1025)), (attn, dict(S=0)),
+           (attn, dict(T=8)), (attn, dict(T=2048)), (attn, dict(H=5)), (attn, dict(H=258)), (attn, dict(B=0)), (attn, dict(B=1025)), (attn, dict(S=0)),
            (attn, dict(S=65, mask=A)), (attn, dict(S=65536)), (attn, dict(W=0)), (attn, dict(ts=3)), (attn, dict(W=1 << 28)),
            (attn, dict(scale=0.0)), (attn, dict(scale=float("inf"))), (attn, dict(scale=float("nan"))), (attn, dict(q=A + 8)),
            (attn, dict(kt=64)), (attn, dict(kt=132)), (attn, dict(kp=-2048)), (attn, dict(qs=516)), (attn, dict(ws=None)),
