@@ -38,8 +38,10 @@ typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 
 // The two element types: their MFMA, and P's rounding. fp16 holds weights down to 2^-14 at full precision only: P is
 // scaled by 2^14 there (exact; numerator and normaliser alike), so weights down to 2^-28 of the largest keep theirs.
+// SLACK: how far (log2) scores may pass the row's reference before the sums are brought to a new one; fp16 holds weights up
+// to 2^(14 + SLACK).
 struct Bf16 {
-    static constexpr float SHIFT = 0.f;
+    static constexpr float SHIFT = 0.f, SLACK = 8.f;
     static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
@@ -53,7 +55,7 @@ struct Bf16 {
     static constexpr uint32_t EXP = 0x7F807F80u, ONE = 0x00800080u;  // two elements' exponents, one step of them
 };
 struct Fp16 {
-    static constexpr float SHIFT = 14.f;
+    static constexpr float SHIFT = 14.f, SLACK = 1.5f;
     static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
@@ -97,8 +99,8 @@ struct PagedArgs {
 
 constexpr int MAX_SEQS = 1024;
 constexpr int STEP = 32;
-constexpr int GRID = 256;
-constexpr int RING_BYTES = 128 * 1024;
+constexpr int CUS = 256;
+constexpr int RING_BYTES = 128 * 1024;  // of a CU's work-groups together
 constexpr int64_t FEW_STEPS = 2048;  // 128-token steps of a call at most, for the forms that go by latency
 constexpr int64_t WHOLE_TOKENS = 640;  // tokens a unit can have at most, for one work-group per unit
 
@@ -230,19 +232,21 @@ __device__ __forceinline__ int steps_of(const PagedArgs& a, const Span& s, int u
 }
 
 // One work-group: RTW waves of row tiles (TPW tiles of 16 query rows each) times P token parts.
-template <class E, int D, int TPW, int RTW, int P, bool SEL>
+// (WPC of them share a CU: waves that meet at a barrier are then not all of the CU's)
+template <int D, int TPW, int RTW, int P, int WPC>
 struct Geometry {
     static constexpr int NT = 64 * RTW * P;
     static constexpr int RPW = 16 * TPW * RTW;
     static constexpr int STAGE = STEP * 2 * D;                    // bytes of K (or V) per stage
-    static constexpr int NS = RING_BYTES / (2 * STAGE * P);       // ring stages per part
+    static constexpr int RING = RING_BYTES / WPC;
+    static constexpr int NS = RING / (2 * STAGE * P);             // ring stages per part
     static constexpr int PER = STAGE / 1024 / RTW;                // direct loads per wave, stage and matrix
     static_assert(NS >= 1 && (NS & (NS - 1)) == 0 && PER >= 1 && (RTW == 1 || NS >= 2), "ring geometry");
 };
 
-template <class E, int D, int TPW, int RTW, int P, bool SEL>
-__global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
-    using Geo = Geometry<E, D, TPW, RTW, P, SEL>;
+template <class E, int D, int TPW, int RTW, int P, int WPC, bool SEL>
+__global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_kernel(PagedArgs a) {
+    using Geo = Geometry<D, TPW, RTW, P, WPC>;
     constexpr int NT = Geo::NT, RPW = Geo::RPW, STAGE = Geo::STAGE, NS = Geo::NS, PER = Geo::PER;
     constexpr int KK = D / 32, DT = D / 16, TOK = STEP * P;
     extern __shared__ __align__(256) unsigned char smem[];  // (the reads' exclusive ors need rows aligned to 256 bytes)
@@ -252,7 +256,7 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
     const int rw = w % RTW, part = w / RTW;
     // Work-groups go to the 8 XCDs in turn: each XCD takes neighbouring shares, so that the row blocks of a kv head, which
     // read the same K and V, find them in one L2 (a prompt's 2048 rows: 164 us with the shares in turn).
-    const int share = a.whole ? int(blockIdx.x) : int(blockIdx.x) % 8 * (GRID / 8) + int(blockIdx.x) / 8;
+    const int share = a.whole ? int(blockIdx.x) : int(blockIdx.x) % 8 * (CUS * WPC / 8) + int(blockIdx.x) / 8;
 
     // ---- this work-group's share of the line of steps: [begin, end), and the sequence it begins in
     int begin, end, quota, b, in_b, kh = 0, u = 0;
@@ -374,38 +378,44 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
             const int v0 = (step0 + s) * TOK + part * STEP;
             Two x;
             x.e[0] = entry(v0);
-            x.e[1] = one_page ? x.e[0] : entry(v0 + 16);
+            x.e[1] = one_page ? 0 : entry(v0 + 16);  // (one page: unused; a copy would wait for the load here)
             return x;
         };
         uint32_t hist = 0;  // two bits per stage issued: its halves stand in pages
-        const unsigned char *kp_[2], *vp_[2];
+        // A wave's loads of a stage lie in one half where several waves share them: only that half's address is formed.
+        constexpr int HALF = 16 / TPL;  // loads of a half
+        constexpr int HW = PER <= HALF ? 1 : 2;
+        const int h_own = HW == 1 ? rw * PER / HALF : 0;  // (the wave's half)
+        const unsigned char *kp_[HW], *vp_[HW];
         auto place = [&](int s, Two x) {
             const int v0 = (step0 + s) * TOK + part * STEP;
-            const uint32_t r = uint32_t(SEL && v0 >= sp.nsel ? v0 - sp.nsel : v0) & ((1u << a.lt) - 1u);
-            // (a half without a page reads the pool's first rows: in bounds, and masked)
-            const bool in = uint32_t(x.e[0]) < uint32_t(a.P);
-            kp_[0] = kbase + (in ? uint64_t(uint32_t(x.e[0])) * page_k + uint64_t(r) * row_k : 0);
-            vp_[0] = vbase + (in ? uint64_t(uint32_t(x.e[0])) * page_v + uint64_t(r) * row_v : 0);
-            if (one_page) {
-                kp_[1] = kp_[0] + 16 * row_k;
-                vp_[1] = vp_[0] + 16 * row_v;
-                hist = (hist << 2) | (in ? 3u : 0u);
-            } else {
-                const uint32_t r1 = (r + 16) & ((1u << a.lt) - 1u);
-                const bool in1 = uint32_t(x.e[1]) < uint32_t(a.P);
-                kp_[1] = kbase + (in1 ? uint64_t(uint32_t(x.e[1])) * page_k + uint64_t(r1) * row_k : 0);
-                vp_[1] = vbase + (in1 ? uint64_t(uint32_t(x.e[1])) * page_v + uint64_t(r1) * row_v : 0);
-                hist = (hist << 2) | (in ? 1u : 0u) | (in1 ? 2u : 0u);
+            const uint32_t r0 = uint32_t(SEL && v0 >= sp.nsel ? v0 - sp.nsel : v0);
+            const bool in0 = uint32_t(x.e[0]) < uint32_t(a.P), in1 = one_page ? in0 : uint32_t(x.e[1]) < uint32_t(a.P);
+            hist = (hist << 2) | (in0 ? 1u : 0u) | (in1 ? 2u : 0u);
+#pragma unroll
+            for (int i = 0; i < HW; ++i) {
+                const int h = HW == 1 ? h_own : i;
+                if (i == 1 && one_page) {
+                    kp_[HW - 1] = kp_[0] + 16 * row_k;
+                    vp_[HW - 1] = vp_[0] + 16 * row_v;
+                    break;
+                }
+                // (a half without a page reads the pool's first rows: in bounds, and masked)
+                const bool in = h ? in1 : in0;
+                const uint32_t e = in ? uint32_t(h && !one_page ? x.e[1] : x.e[0]) : 0u;
+                const uint32_t r = in ? (r0 + 16 * h) & ((1u << a.lt) - 1u) : 0u;
+                kp_[i] = kbase + (uint64_t(e) * page_k + uint64_t(r) * row_k);
+                vp_[i] = vbase + (uint64_t(e) * page_v + uint64_t(r) * row_v);
             }
         };
-        auto load = [&](const unsigned char* const (&from)[2], uint32_t lane_row, uint32_t stride, unsigned char* dst) {
-            constexpr int HALF = 16 / TPL;  // loads of a half
+        auto load = [&](const unsigned char* const (&from)[HW], uint32_t lane_row, uint32_t stride, unsigned char* dst) {
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
-                const int i = rw * PER + j;  // tokens TPL i ..
-                const unsigned char* src = from[i / HALF] + (lane_row + uint32_t((i % HALF) * TPL) * stride + (piece ^ (swizzle<D>(TPL * i) * 16)));
+                const int i = HW == 1 ? rw * PER % HALF + j : j;  // load of its half, or of the stage: tokens TPL i ..
+                const unsigned char* src = from[HW == 1 ? 0 : j / HALF] +
+                                           (lane_row + uint32_t((i % HALF) * TPL) * stride + (piece ^ uint32_t(swizzle<D>(TPL * (i % HALF)) * 16)));
                 __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                                 (__attribute__((address_space(3))) void*)(dst + i * 1024), 16, 0, 0);
+                                                 (__attribute__((address_space(3))) void*)(dst + (rw * PER + j) * 1024), 16, 0, 0);
             }
         };
         auto issue_k = [&](int s) { load(kp_, k_row, row_k, ring + (s & (NS - 1)) * 2 * STAGE); };
@@ -444,10 +454,14 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
         }
 
         f32x4 acc[TPW][DT];
-        float m[TPW], l[TPW];
+        // per row: the score up to which its reference serves (-inf: none yet), the reference in log2 units (0 as long as nothing
+        // is admitted, so that -inf - -inf never forms), the sum of weights
+        float m_lim[TPW], m_z[TPW], l[TPW];
+        const float slack = E::SLACK / a.zs;
 #pragma unroll
         for (int t = 0; t < TPW; ++t) {
-            m[t] = -INFINITY;
+            m_lim[t] = -INFINITY;
+            m_z[t] = 0.f;
             l[t] = 0.f;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) acc[t][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -513,64 +527,64 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
             }
 
             const bool whole = ok == 3u && v0 + STEP <= t_all;  // (uniform in the wave) every row admits all 32 tokens
-            u32x4 pf[TPW];
-            uint32_t in[TPW];
-#pragma unroll
-            for (int t = 0; t < TPW; ++t) {
-                in[t] = ~0u;
+            // tile t's weights of the stage, as the B operand of O^T += V^T P^T
+            auto weights = [&](int t) -> u32x4 {
                 if (!whole) {
-                    const int p = sp.tree0 - v0;  // tokens of the prefix in the stage
+                    int p = sp.tree0 - v0;  // tokens of the prefix in the stage
+                    asm volatile("" : "+s"(p));  // (none of this ahead of the branch)
+                    uint32_t in;
                     if (a.mask) {
                         const uint64_t own_bits = p >= 32 ? 0 : (p >= 0 ? bits[t] << p : (-p < 64 ? bits[t] >> -p : 0));
-                        in[t] = (p >= 32 ? ~0u : (p > 0 ? (1u << p) - 1u : 0u)) | uint32_t(own_bits);
+                        in = (p >= 32 ? ~0u : (p > 0 ? (1u << p) - 1u : 0u)) | uint32_t(own_bits);
                     } else {
                         const int nv = p + lim[t] + 1;
-                        in[t] = nv >= 32 ? ~0u : (nv > 0 ? (1u << nv) - 1u : 0u);
+                        in = nv >= 32 ? ~0u : (nv > 0 ? (1u << nv) - 1u : 0u);
                     }
-                    in[t] &= ((ok & 1u) ? 0x0000FFFFu : 0u) | ((ok & 2u) ? 0xFFFF0000u : 0u);
-                    if (__builtin_amdgcn_ballot_w64(in[t] != 0u) == 0) {  // (uniform: nothing for this tile)
-                        pf[t] = u32x4{0, 0, 0, 0};
-                        continue;
-                    }
-                    const uint32_t lb = in[t] >> (4 * g);
+                    in &= ((ok & 1u) ? 0x0000FFFFu : 0u) | ((ok & 2u) ? 0xFFFF0000u : 0u);
+                    if (__builtin_amdgcn_ballot_w64(in != 0u) == 0) return u32x4{0, 0, 0, 0};  // (uniform: nothing for this tile)
+                    const uint32_t lb = in >> (4 * g);
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             if (!((lb >> (16 * h + i)) & 1u)) st[t][h][i] = -INFINITY;
                 }
-                float mx = max3(max3(st[t][0][0], st[t][0][1], st[t][0][2]), max3(st[t][0][3], st[t][1][0], st[t][1][1]),
-                                max3(st[t][1][2], st[t][1][3], m[t]));
-                const float mnew = max_x32(max_x16(mx));
-                // a row with nothing admitted yet subtracts 0, so -inf - -inf never forms
-                const float msub = mnew == -INFINITY ? 0.f : mnew, mz = msub * a.zs - E::SHIFT;
-                const float alpha = __builtin_amdgcn_exp2f((m[t] - msub) * a.zs);  // (exactly 1 where the maximum stays)
-                m[t] = mnew;
-                float ps = 0.f;
+                u32x4 pf;
+                // Weights are taken against the row's reference, an earlier maximum, as long as no score passes it by more
+                // than SLACK: the sums are fp32 and a weight's rounding is relative, so nothing is lost, and the common
+                // stage has neither an exchange between lanes nor a rescale.
+                const float mx = max3(max3(st[t][0][0], st[t][0][1], st[t][0][2]), max3(st[t][0][3], st[t][1][0], st[t][1][1]),
+                                      max3(st[t][1][2], st[t][1][3], st[t][1][3]));
+                if (__builtin_amdgcn_ballot_w64(mx > m_lim[t]) != 0) {  // (uniform)
+                    const float top = max_x32(max_x16(mx));
+                    if (top > m_lim[t]) {  // (a row's four lanes alike)
+                        const float mz = top * a.zs;
+                        const float alpha = m_lim[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_z[t] - mz);
+                        m_z[t] = mz;
+                        m_lim[t] = top + slack;
+                        l[t] *= alpha;
+#pragma unroll
+                        for (int dt = 0; dt < DT; ++dt) acc[t][dt] *= alpha;
+                    }
+                }
+                const float sub = m_z[t] - E::SHIFT;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int i = 0; i < 4; i += 2) {
-                        const float p0 = __builtin_amdgcn_exp2f(fmaf(st[t][h][i], a.zs, -mz));
-                        const float p1 = __builtin_amdgcn_exp2f(fmaf(st[t][h][i + 1], a.zs, -mz));
-                        pf[t][2 * h + i / 2] = E::pair(p0, p1);
-                        ps = E::add_pair(pf[t][2 * h + i / 2], ps);
+                        const float p0 = __builtin_amdgcn_exp2f(fmaf(st[t][h][i], a.zs, -sub));
+                        const float p1 = __builtin_amdgcn_exp2f(fmaf(st[t][h][i + 1], a.zs, -sub));
+                        pf[2 * h + i / 2] = E::pair(p0, p1);
+                        l[t] = E::add_pair(pf[2 * h + i / 2], l[t]);  // (this lane's tokens; the row's four lanes meet at the end)
                     }
-                l[t] = l[t] * alpha + ps;  // (this lane's tokens; the row's four lanes meet at the end)
-                if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0)
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) acc[t][dt] *= alpha;
-            }
-            if constexpr (RTW == 1) {
-                if (more) wait_vm<PER * (2 * NS - 1)>();
-                else wait_vm<0>();
-            }
+                return pf;
+            };
             constexpr int VT = D == 64 ? 4 : 8;  // dim tiles read at once
             u32x2 va[VT], vb[VT];
-            auto weigh = [&](int dt0) {
-                // A weight of 0 times an infinity or a NaN in a place that a row does not admit would reach the row: in a
-                // stage that not every row admits whole, such values count as 0 here, and where there are any the rows
-                // that do admit them get them when the unit's parts meet (`odd`).
+            // A weight of 0 times an infinity or a NaN in a place that a row does not admit would reach the row: in a stage that
+            // not every row admits whole, such values count as 0 here, and where there are any the rows that do admit them
+            // get them when the unit's parts meet (`odd`).
+            auto sift = [&]() {
                 if (!whole) {
                     uint32_t top = 0;
 #pragma unroll
@@ -587,22 +601,50 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
                         odd = 1;
                     }
                 }
-#pragma unroll
-                for (int t = 0; t < TPW; ++t)
-#pragma unroll
-                    for (int x = 0; x < VT; ++x)
-                        acc[t][dt0 + x] = E::mfma(u32x4{va[x].x, va[x].y, vb[x].x, vb[x].y}, pf[t], acc[t][dt0 + x]);
             };
-            read_v<D, 0>(va, vb, slot + STAGE + v_lane);
-            if constexpr (D == 256) {
-                weigh(0);
-                read_v<D, 1>(va, vb, slot + STAGE + v_lane);
+            auto weigh = [&](int t, int dt0, u32x4 pf) {
+#pragma unroll
+                for (int x = 0; x < VT; ++x)
+                    acc[t][dt0 + x] = E::mfma(u32x4{va[x].x, va[x].y, vb[x].x, vb[x].y}, pf, acc[t][dt0 + x]);
+            };
+            auto wait_v = [&]() {
+                if constexpr (RTW == 1) {
+                    if (more) wait_vm<PER * (2 * NS - 1)>();
+                    else wait_vm<0>();
+                }
+            };
+            auto refill_v = [&]() {
+                if (RTW == 1 && more) {
+                    issue_v(s + AHEAD);
+                    next_e = entries(s + AHEAD + 1);
+                }
+            };
+            if constexpr (D != 256 && TPW <= 2) {
+                // V's reads behind the scores' MFMAs, a tile's products behind the next tile's weights
+                wait_v();
+                read_v<D, 0>(va, vb, slot + STAGE + v_lane);
+                refill_v();
+                sift();
+#pragma unroll
+                for (int t = 0; t < TPW; ++t) weigh(t, 0, weights(t));
+            } else {
+                // (V's operands only once the scores' registers are free; at head_dim 256 in halves)
+                u32x4 pf[TPW];
+#pragma unroll
+                for (int t = 0; t < TPW; ++t) pf[t] = weights(t);
+                wait_v();
+                read_v<D, 0>(va, vb, slot + STAGE + v_lane);
+                if constexpr (D == 256) {
+                    sift();
+#pragma unroll
+                    for (int t = 0; t < TPW; ++t) weigh(t, 0, pf[t]);
+                    read_v<D, 1>(va, vb, slot + STAGE + v_lane);
+                }
+                refill_v();
+                sift();
+#pragma unroll
+                for (int t = 0; t < TPW; ++t) weigh(t, D == 256 ? 8 : 0, pf[t]);
             }
-            if (RTW == 1 && more) {
-                issue_v(s + AHEAD);
-                next_e = entries(s + AHEAD + 1);
-            }
-            weigh(D == 256 ? 8 : 0);
         }
 
         // ---- the parts of a row tile meet in LDS, tile by tile; rows D + 4 floats apart (no two rows of an access in one bank)
@@ -619,7 +661,7 @@ __global__ __launch_bounds__(64 * RTW * P) void paged_attn_kernel(PagedArgs a) {
             for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(mo + 16 * dt) = acc[t][dt];
             const float sl = sum_x32(sum_x16(l[t]));
             if (g == 0) {
-                lm[(rw * P + part) * 16 + c16] = m[t] * a.zs;
+                lm[(rw * P + part) * 16 + c16] = m_lim[t] == -INFINITY ? -INFINITY : m_z[t];
                 lm[RTW * P * 16 + (rw * P + part) * 16 + c16] = sl;
             }
             __syncthreads();
@@ -1009,29 +1051,26 @@ __global__ __launch_bounds__(NT) void block_select_kernel(PagedArgs a) {
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------
-template <class E, int D, int TPW, int RTW, int P, bool SEL>
-int launch(const PagedArgs& a, hipStream_t st) {
-    using Geo = Geometry<E, D, TPW, RTW, P, SEL>;
+template <class E, int D, int TPW, int RTW, int P, int WPC, bool SEL>
+int launch(PagedArgs& a, hipStream_t st) {
+    using Geo = Geometry<D, TPW, RTW, P, WPC>;
     constexpr int joined = (RTW * P * 16 * (D + 4) + 2 * RTW * P * 16) * 4;
-    constexpr int lds = RING_BYTES > joined ? RING_BYTES : joined;
+    constexpr int lds = Geo::RING > joined ? Geo::RING : joined;
     // (once per device and kernel: the call costs about a microsecond)
     static std::atomic<uint64_t> allowed{0};
     int dev = 0;
     MDX_HIP(hipGetDevice(&dev));
     const uint64_t bit = uint64_t(1) << (dev & 63);
     if (dev > 63 || !(allowed.load(std::memory_order_relaxed) & bit)) {
-        allow_smem(reinterpret_cast<const void*>(&paged_attn_kernel<E, D, TPW, RTW, P, SEL>), lds);
+        allow_smem(reinterpret_cast<const void*>(&paged_attn_kernel<E, D, TPW, RTW, P, WPC, SEL>), lds);
         allowed.fetch_or(bit, std::memory_order_relaxed);
     }
-    if (a.whole) {
-        hipLaunchKernelGGL((paged_attn_kernel<E, D, TPW, RTW, P, SEL>), dim3(unsigned(a.B * a.Hk * a.units)), dim3(Geo::NT), lds, st, a);
-        MDX_LAUNCHED();
-        return MDX_OK;
-    }
-    hipLaunchKernelGGL((paged_attn_kernel<E, D, TPW, RTW, P, SEL>), dim3(GRID), dim3(Geo::NT), lds, st, a);
+    const int grid = a.whole ? a.B * a.Hk * a.units : CUS * WPC;
+    hipLaunchKernelGGL((paged_attn_kernel<E, D, TPW, RTW, P, WPC, SEL>), dim3(unsigned(grid)), dim3(Geo::NT), lds, st, a);
     MDX_LAUNCHED();
+    if (a.whole) return MDX_OK;
     const int rows = (a.spb < a.S ? a.spb : a.S) * a.G;
-    hipLaunchKernelGGL((paged_join_kernel<E, D>), dim3(GRID, unsigned((rows + 3) / 4)), dim3(256), 0, st, a, Geo::RPW);
+    hipLaunchKernelGGL((paged_join_kernel<E, D>), dim3(unsigned(grid), unsigned((rows + 3) / 4)), dim3(256), 0, st, a, Geo::RPW);
     MDX_LAUNCHED();
     return MDX_OK;
 }
@@ -1052,17 +1091,17 @@ int launch_rows(PagedArgs& a, hipStream_t st) {
     const int rows = SEL ? a.G : a.units > 1 ? 128 : a.S * a.G;
     const int64_t steps = int64_t(a.B) * a.Hk * a.units * ((most_tokens(a, SEL) + 127) / 128);
     const bool few = steps <= FEW_STEPS;
-    if (rows <= 16) return launch<E, D, 1, 1, 4, SEL>(a, st);
+    if (rows <= 16) return launch<E, D, 1, 1, 4, 1, SEL>(a, st);
     if (rows <= 32) {
-        if (few) return launch<E, D, 1, 2, (D == 256 ? 2 : 4), SEL>(a, st);
-        return launch<E, D, 2, 1, 4, SEL>(a, st);
+        if (few) return launch<E, D, 1, 2, (D == 256 ? 2 : 4), 1, SEL>(a, st);
+        return launch<E, D, 2, 1, 4, 1, SEL>(a, st);
     }
     if (rows <= 64) {
-        if (few) return launch<E, D, 1, 4, (D == 256 ? 1 : 2), SEL>(a, st);
-        if constexpr (D == 256) return launch<E, D, 2, 2, 2, SEL>(a, st);
-        else return launch<E, D, 4, 1, 4, SEL>(a, st);
+        if (few) return launch<E, D, 1, 4, (D == 256 ? 1 : 2), 1, SEL>(a, st);
+        if constexpr (D == 256) return launch<E, D, 2, 2, 2, 1, SEL>(a, st);
+        else return launch<E, D, 4, 1, 4, 1, SEL>(a, st);
     }
-    if constexpr (!SEL) return launch<E, D, 2, 4, (D == 256 ? 1 : 2), SEL>(a, st);
+    if constexpr (!SEL) return launch<E, D, 2, 4, 1, (D == 256 ? 1 : 2), SEL>(a, st);
     set_error("at most 64 query heads per kv head");
     return MDX_EINVAL;
 }
@@ -1080,7 +1119,8 @@ int launch_any(PagedArgs& a, int D, int dtype, hipStream_t st) {
 }
 
 size_t base_bytes(int64_t rows, int64_t D) {
-    return size_t(GRID) * sizeof(int4) + size_t(GRID) * 2 * rpw_of(rows) * (D + 2) * 4;
+    const int rpw = rpw_of(rows), shares = rpw == 128 && D != 256 ? 2 * CUS : CUS;
+    return size_t(2 * CUS) * sizeof(int4) + size_t(shares) * 2 * rpw * (D + 2) * 4;
 }
 
 int log2_of(int64_t T) {
@@ -1171,7 +1211,7 @@ extern "C" int mdx_attn_paged(const void* q, int64_t q_seq_stride, int64_t q_row
     a.spb = int(rows_of_unit(S, H / Hk));
     a.units = int(blocks);
     a.info = static_cast<int4*>(workspace);
-    a.part = reinterpret_cast<float*>(a.info + GRID);
+    a.part = reinterpret_cast<float*>(a.info + 2 * CUS);
     return launch_any<false>(a, int(D), dtype, static_cast<hipStream_t>(stream));
 }
 
@@ -1213,7 +1253,7 @@ extern "C" int mdx_attn_blocks(const void* q, int64_t q_seq_stride, int64_t q_ro
     a.sh = s_head_stride, a.sp = s_page_stride;
     a.sel = sel;
     a.info = static_cast<int4*>(workspace);
-    a.part = reinterpret_cast<float*>(a.info + GRID);
+    a.part = reinterpret_cast<float*>(a.info + 2 * CUS);
     a.keys = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + base_bytes(a.G, D));
     a.page = reinterpret_cast<int32_t*>(a.keys + units * W);
     hipStream_t st = static_cast<hipStream_t>(stream);
