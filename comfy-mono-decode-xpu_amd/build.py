@@ -1,4 +1,5 @@
-"""Build libmdx.so (every HIP kernel of the package, gfx950) in-tree, next to the Python shim.
+"""Build libmdx.so (every HIP kernel of the package, gfx950) and _bind.so (the torch binding of the paged cache's calls)
+in-tree, next to the Python shim.
 
     python comfy-mono-decode-xpu_amd/build.py [--jobs N]
 
@@ -18,6 +19,8 @@ import tempfile
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "mdx", "libmdx.so")
+BIND = os.path.join(CSRC, "mdx_bind.cpp")  # host code over torch's headers: a module of its own
+BIND_OUT = os.path.join(HERE, "mdx", "_bind.so")
 ARCH = os.environ.get("MDX_ARCH", "gfx950")
 
 # -ffp-contract=off: every rounding the operator contracts name is an explicit single op; the
@@ -35,7 +38,23 @@ def hipcc():
 
 
 def sources():
-    return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".hip", ".cpp")))
+    return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".hip", ".cpp")) and f != os.path.basename(BIND))
+
+
+def _bind(tmp_out):
+    """The torch binding, with the host compiler; torch's libraries are in the process before it loads (no run path)."""
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    rocm = os.path.dirname(os.path.dirname(os.path.realpath(hipcc())))
+    cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I" + sysconfig.get_paths()["include"],
+           f"-I{root}/include", f"-I{root}/include/torch/csrc/api/include", f"-I{rocm}/include", BIND, "-o", tmp_out, f"-L{root}/lib",
+           "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
 
 
 def _compile(cc, src, obj):
@@ -53,15 +72,18 @@ def build(jobs: int | None = None, verbose: bool = False) -> str:
     with tempfile.TemporaryDirectory(prefix="mdx_build_") as tmp:
         objs = [os.path.join(tmp, os.path.basename(s) + ".o") for s in srcs]
         with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
+            bind = ex.submit(_bind, BIND_OUT + ".tmp")
             list(ex.map(lambda so: _compile(cc, *so), zip(srcs, objs)))
+            bind.result()
         tmp_out = OUT + ".tmp"
         cmd = [cc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", tmp_out]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
         os.replace(tmp_out, OUT)
+        os.replace(BIND_OUT + ".tmp", BIND_OUT)
     if verbose:
-        print(f"built {OUT} from {len(srcs)} sources")
+        print(f"built {OUT} from {len(srcs)} sources, {BIND_OUT}")
     return OUT
 
 

@@ -1286,53 +1286,16 @@ def draft_pick_bf16(approx, x, w, nout, argmax_first, top, top_values, token, vt
 
 # ---- the paged cache of several sequences ---------------------------------------------------------------
 # kv [L, 2, Hk, P, T, D] bf16 / fp16 (keys, values of every layer), ksum [L, Hk, P, D] (the full pages' mean keys, or None),
-# table int32 [B, W] (page of token t: table[b, t // T]; -1: none), length int32 [B], refs int32 [P] (0: free). Workspaces are
-# taken from torch's allocator per call, so calls on several streams and captured graphs share none.
-_PAGE_DT = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
-_WS_BYTES = {}  # (entry, sizes) -> workspace bytes
+# table int32 [B, W] (page of token t: table[b, t // T]; -1: none), length int32 [B], refs int32 [P] (0: free). The operands are
+# checked in mdx._bind, and workspaces come from torch's allocator per call, so calls on several streams and captured graphs
+# share none. Called before libmdx and the binding are loaded, every function loads them (_lib.bind).
+_bind = None
 
 
-def _ws_bytes(name, *sizes):
-    n = _WS_BYTES.get((name, sizes))
-    if n is None:
-        if len(_WS_BYTES) > 4096:
-            _WS_BYTES.clear()
-        n = _WS_BYTES[name, sizes] = getattr(_lib.lib(), name)(*sizes)
-    return n
-
-
-def _ints(t, what, shape):
-    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
-        raise RuntimeError(f"{what}: contiguous int32 {list(shape)}")
-
-
-def _off_device(d, **tensors):
-    """Raises for the tensor that is not one on device d."""
-    if d < 0:
-        raise RuntimeError("expected tensors on the ROCm device")
-    for n, t in tensors.items():
-        if t is not None and (not isinstance(t, torch.Tensor) or t.get_device() != d):
-            raise RuntimeError(f"{n} must be a tensor on the same ROCm device")
-
-
-def _pool(kv, ksum, table, length, refs):
-    """The cache's tensors checked; their device and (L, Hk, P, T, D, B, W)."""
-    d = kv.get_device()
-    if d < 0 or table.get_device() != d or length.get_device() != d or refs.get_device() != d \
-            or (ksum is not None and ksum.get_device() != d):
-        _off_device(d, ksum=ksum, table=table, length=length, refs=refs)
-    shape = kv.shape
-    if kv.dtype not in _PAGE_DT or len(shape) != 6 or shape[1] != 2 or not kv.is_contiguous():
-        raise RuntimeError("kv: contiguous bf16 / fp16 [layers, 2, kv_heads, pages, page rows, head_dim]")
-    L, _, Hk, P, T, D = shape
-    if ksum is not None and (ksum.dtype is not kv.dtype or ksum.shape != (L, Hk, P, D) or not ksum.is_contiguous()):
-        raise RuntimeError("ksum: contiguous [layers, kv_heads, pages, head_dim] of the cache's type")
-    if table.dtype is not torch.int32 or table.dim() != 2 or table.stride(1) != 1 or table.stride(0) < table.shape[1]:
-        raise RuntimeError("table: int32 [sequences, W], rows contiguous")
-    B, W = table.shape
-    _ints(length, "length", (B,))
-    _ints(refs, "refs", (P,))
-    return d, L, Hk, P, T, D, B, W
+def _bound():
+    global _bind
+    _bind = _lib.bind()
+    return _bind
 
 
 def page_fork(kv, ksum, table, length, refs, dst, src, room=0, share=True, slots=None):
@@ -1345,23 +1308,7 @@ def page_fork(kv, ksum, table, length, refs, dst, src, room=0, share=True, slots
     Returns int32 [pairs]: 1 done, 0 too few free pages (for this pair with those before it), -1 refused (a place outside the
     table or named twice, a length and room past the table's width); pairs that are not done change nothing.
     No counterpart in the reference (one sequence, one contiguous cache)."""
-    d, L, Hk, P, T, D, B, W = _pool(kv, ksum, table, length, refs)
-    if dst.get_device() != d or src.get_device() != d or (slots is not None and slots.get_device() != d):
-        _off_device(d, dst=dst, src=src, slots=slots)
-    M = dst.numel()
-    _ints(dst, "dst", (M,))
-    _ints(src, "src", (M,))
-    room = int(room)
-    if slots is not None:
-        _check(slots.dtype == torch.int64 and slots.shape == (M, room) and slots.is_contiguous(), "slots: contiguous int64 [pairs, room]")
-    status = torch.empty(M, dtype=torch.int32, device=kv.device)
-    if M == 0:
-        return status
-    ws = torch.empty(_ws_bytes("mdx_page_fork_workspace", M, W), dtype=torch.uint8, device=kv.device)
-    _lib.call_on(d, "mdx_page_fork", kv.data_ptr(), _lib.ptr(ksum), L, Hk, P, T, D, table.data_ptr(), table.stride(0), B, W,
-                 length.data_ptr(), refs.data_ptr(), dst.data_ptr(), src.data_ptr(), M, room, 1 if share else 0,
-                 _lib.ptr(slots), status.data_ptr(), ws.data_ptr(), ws.numel())
-    return status
+    return (_bind or _bound()).page_fork(kv, ksum, table, length, refs, dst, src, room, share, slots)
 
 
 def page_commit(kv, ksum, table, length, refs, count, path=None, room=0, new_length=None, slots=None):
@@ -1374,60 +1321,7 @@ def page_commit(kv, ksum, table, length, refs, count, path=None, room=0, new_len
     count[b] < 0: the sequence is left alone (status 1). Returns int32 [B]: 1 done, 0 committed but not all of the room
     given, -1 refused (a path out of order or range, rows without pages, a length past the table): nothing of that sequence
     moves or grows. The move of mtp_accept (csrc/mtp_loop.sycl:160-196 of the reference) over pages, for a batch."""
-    d, L, Hk, P, T, D, B, W = _pool(kv, ksum, table, length, refs)
-    if count.get_device() != d or any(t is not None and t.get_device() != d for t in (path, new_length, slots)):
-        _off_device(d, count=count, path=path, new_length=new_length, slots=slots)
-    _ints(count, "count", (B,))
-    R = 0
-    if path is not None:
-        R = path.shape[-1]
-        _ints(path, "path", (B, R))
-    if new_length is None:
-        new_length = length
-    else:
-        _ints(new_length, "new_length", (B,))
-    room = int(room)
-    if slots is not None:
-        _check(slots.dtype == torch.int64 and slots.shape == (B, room) and slots.is_contiguous(), "slots: contiguous int64 [B, room]")
-    status = torch.empty(B, dtype=torch.int32, device=kv.device)
-    ws = torch.empty(_ws_bytes("mdx_page_commit_workspace", B, W), dtype=torch.uint8, device=kv.device)
-    _lib.call_on(d, "mdx_page_commit", kv.data_ptr(), _lib.ptr(ksum), _PAGE_DT[kv.dtype], L, Hk, P, T, D, table.data_ptr(),
-                 table.stride(0), B, W, length.data_ptr(), new_length.data_ptr(), refs.data_ptr(), count.data_ptr(),
-                 _lib.ptr(path), R, room, _lib.ptr(slots), status.data_ptr(), ws.data_ptr(), ws.numel())
-    return status
-
-
-def _paged(q, key, value, table, length, mask, out):
-    """The operands of the paged attention checked: their device, out, the C arguments up to value's strides, sizes."""
-    d = q.get_device()
-    if d < 0 or key.get_device() != d or value.get_device() != d or table.get_device() != d or length.get_device() != d \
-            or (mask is not None and mask.get_device() != d) or (out is not None and out.get_device() != d):
-        _off_device(d, key=key, value=value, table=table, length=length, mask=mask, out=out)
-    dt = q.dtype
-    code = _PAGE_DT.get(dt)
-    if code is None or key.dtype is not dt or value.dtype is not dt:
-        raise RuntimeError("q, key and value: bf16 or fp16, one type")
-    shape, kshape, qs, ks, vs = q.shape, key.shape, q.stride(), key.stride(), value.stride()
-    if len(shape) != 4 or qs[3] != 1:
-        raise RuntimeError("q: [sequences, rows, heads, head_dim], the last dim contiguous")
-    B, S, H, D = shape
-    if len(kshape) != 4 or kshape[3] != D or value.shape != kshape or ks[3] != 1 or vs[3] != 1:
-        raise RuntimeError("key / value: [kv_heads, pages, page rows, head_dim], the last dim contiguous")
-    Hk, P, T, _ = kshape
-    if Hk < 1 or H % Hk != 0:
-        raise RuntimeError("query heads: a multiple of the kv heads")
-    tshape, ts = table.shape, table.stride()
-    if table.dtype is not torch.int32 or len(tshape) != 2 or tshape[0] != B or ts[1] != 1 or ts[0] < tshape[1]:
-        raise RuntimeError("table: int32 [sequences, W], rows contiguous")
-    _ints(length, "length", (B,))
-    if mask is not None and (mask.dtype is not torch.int64 or mask.shape != (B, S) or not mask.is_contiguous() or S > 64):
-        raise RuntimeError("mask: contiguous int64 [sequences, rows], at most 64 rows")
-    if out is None:
-        out = torch.empty(shape, dtype=dt, device=q.device)
-    elif out.dtype is not dt or out.shape != shape or not out.is_contiguous():
-        raise RuntimeError("out: contiguous, q's shape and type")
-    return d, out, (q.data_ptr(), qs[0], qs[1], qs[2], key.data_ptr(), ks[0], ks[1], ks[2], value.data_ptr(), vs[0], vs[1], vs[2]), \
-        (code, B, S, H, Hk, D, P, T, tshape[1], ts[0])
+    return (_bind or _bound()).page_commit(kv, ksum, table, length, refs, count, path, room, new_length, slots)
 
 
 def attn_paged(q, key, value, table, length, mask=None, scale=None, out=None):
@@ -1438,14 +1332,7 @@ def attn_paged(q, key, value, table, length, mask=None, scale=None, out=None):
     elements), table, length as page_commit keeps them. out [B, S, H, D]; a row that admits nothing is 0. Tokens in pages that
     the table does not have are not attended; what stands in places a row does not attend is never seen.
     The form of attn_dpas (csrc/attn_dpas.sycl:269-342 of the reference) for a batch, pages, and any rows."""
-    d, out, args, (dt, B, S, H, Hk, D, P, T, W, ts) = _paged(q, key, value, table, length, mask, out)
-    if B == 0 or S == 0:
-        return out
-    nb = _ws_bytes("mdx_attn_paged_workspace", B, S, H, Hk, D, T, W)
-    ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
-    _lib.call_on(d, "mdx_attn_paged", *args, dt, table.data_ptr(), ts, length.data_ptr(), _lib.ptr(mask), out.data_ptr(), B, S, H,
-                 Hk, D, P, T, W, D ** -0.5 if scale is None else float(scale), _lib.ptr(ws), nb)
-    return out
+    return (_bind or _bound()).attn_paged(q, key, value, table, length, mask, scale, out)
 
 
 def attn_blocks(q, key, value, ksum, table, length, blocks, sink=1, local=1, mask=None, scale=None, out=None, sel=None):
@@ -1455,25 +1342,4 @@ def attn_blocks(q, key, value, ksum, table, length, blocks, sink=1, local=1, mas
     pages and the rows' own. ksum [Hk, P, D]: the full pages' mean keys (page_commit's, one layer). At most 64 rows.
     Returns (out [B, S, H, D], sel int32 [B, S, Hk, sink + local + blocks]): the selected pages of the sequence, ascending,
     -1 behind them. No counterpart in the reference."""
-    d, out, args, (dt, B, S, H, Hk, D, P, T, W, ts) = _paged(q, key, value, table, length, mask, out)
-    if ksum.get_device() != d or (sel is not None and sel.get_device() != d):
-        _off_device(d, ksum=ksum, sel=sel)
-    ss = ksum.stride()
-    if ksum.dtype is not q.dtype or ksum.shape != (Hk, P, D) or ss[2] != 1:
-        raise RuntimeError("ksum: [kv_heads, pages, head_dim] of the cache's type")
-    blocks, sink, local = int(blocks), int(sink), int(local)
-    most = blocks + sink + local
-    if blocks < 0 or sink < 0 or local < 0 or not 1 <= most <= 65536:
-        raise RuntimeError("1..65536 selected blocks")
-    if sel is None:
-        sel = torch.empty((B, S, Hk, most), dtype=torch.int32, device=q.device)
-    else:
-        _ints(sel, "sel", (B, S, Hk, most))
-    if B == 0 or S == 0:
-        return out, sel
-    nb = _ws_bytes("mdx_attn_blocks_workspace", B, S, H, Hk, D, W, most)
-    ws = torch.empty(nb, dtype=torch.uint8, device=q.device)
-    _lib.call_on(d, "mdx_attn_blocks", *args, ksum.data_ptr(), ss[0], ss[1], dt, table.data_ptr(), ts, length.data_ptr(),
-                 _lib.ptr(mask), out.data_ptr(), sel.data_ptr(), blocks, sink, local, B, S, H, Hk, D, P, T, W,
-                 D ** -0.5 if scale is None else float(scale), ws.data_ptr(), nb)
-    return out, sel
+    return (_bind or _bound()).attn_blocks(q, key, value, ksum, table, length, blocks, sink, local, mask, scale, out, sel)

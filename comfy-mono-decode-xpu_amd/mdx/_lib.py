@@ -248,14 +248,20 @@ def ptr(t):
     return None if t is None else t.data_ptr()
 
 
-_device_now = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_bound = None
 
 
-def call_on(d, name, *args):
-    """call() on device d's current stream, with d as the current device (a launch belongs to that one)."""
-    if d != _device_now():
-        with torch.cuda.device(d):
-            return call_on(d, name, *args)
-    stream = torch.cuda.current_stream(d).cuda_stream if _raw_stream is None else _raw_stream(d)
-    if (_fns.get(name) or getattr(lib(), name))(*args, stream) != MDX_OK:
-        raise MdxError(f"{name}: {lib().mdx_last_error().decode(errors='replace')}")
+def bind():
+    """The module mdx._bind with this library's entry points (raises if it was not built: there is no other path)."""
+    global _bound
+    if _bound is None:
+        L = lib()
+        try:
+            from . import _bind as m
+        except ImportError as e:
+            raise MdxError(f"mdx/_bind.so not built or not loadable ({e}); run comfy-mono-decode-xpu_amd/build.py") from None
+        names = ("last_error", "page_fork_workspace", "page_fork", "page_commit_workspace", "page_commit", "attn_paged_workspace",
+                 "attn_paged", "attn_blocks_workspace", "attn_blocks")
+        m.init(*(ctypes.cast(getattr(L, "mdx_" + n), c_void_p).value for n in names), MdxError)
+        _bound = m
+    return _bound
