@@ -88,7 +88,8 @@ struct PagedArgs {
     const uint16_t* ksum;  // [Hk, P, D], strides sh, sp
     int64_t sh, sp;
     uint64_t* keys;  // [B, S, Hk, W]
-    int4* info;      // [work-groups]: the unit left open, and the shares it has from there
+    int4* info;      // the units left open to join: (unit, first share, shares), by unit (where they are few) or by share
+    int by_unit;
     float* part;     // [2 work-groups][rows][D + 2]: O, maximum, sum
     int B, S, H, Hk, G, W, P, lt;
     int units;  // units of a sequence and kv head: blocks of spb rows s (1 with a selection each)
@@ -262,9 +263,13 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
     int begin, end, quota, b, in_b, kh = 0, u = 0;
     Span sp;
     if (a.whole) {  // unit (b, kh, u) of the grid
-        u = int(blockIdx.x) % a.units;
-        kh = int(blockIdx.x) / a.units % a.Hk;
-        b = int(blockIdx.x) / a.units / a.Hk;
+        // kv heads in turn (neighbouring work-groups go to different XCDs), a chain's blocks with the most tokens first; every
+        // second round of the CUs the other way, so that a CU's work-groups have about as much to do together.
+        kh = int(blockIdx.x) % a.Hk;
+        const int rest = int(blockIdx.x) / a.Hk, all = a.B * a.units, turn = CUS / a.Hk > 0 ? CUS / a.Hk : 1, q = rest / turn;
+        const int rank = (q & 1) && (q + 1) * turn <= all ? 2 * q * turn + turn - 1 - rest : rest;
+        b = rank % a.B;
+        u = a.units - 1 - rank / a.B;
         sp = span_of<SEL>(a, uload(a.length + b));
         begin = in_b = 0;
         end = quota = steps_of(a, sp, u, TOK);
@@ -319,7 +324,7 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
                 before += n * per_kh;
             });
         if (tid == 0) {
-            a.info[share] = make_int4(0, 0, 0, 0);
+            if (!a.by_unit) a.info[share] = make_int4(0, 0, 0, 0);
             odd = 0;
         }
         if (begin >= end) return;  // (uniform)
@@ -715,10 +720,10 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
             }
             __syncthreads();
         }
-        if (first && !last && tid == 0) {
-            // the unit goes on in the shares behind: how many in all
-            const int left = n_unit - nst;
-            a.info[share] = make_int4(b, kh, u, 1 + (left + quota - 1) / quota);
+        if (first && tid == 0 && !a.whole && (a.by_unit || !last)) {
+            // the unit goes on in the shares behind: how many in all (1: it is done)
+            const int unit = (b * a.Hk + kh) * a.units + u, left = n_unit - nst;
+            a.info[a.by_unit ? unit : share] = make_int4(unit, share, 1 + (left + quota - 1) / quota, 0);
         }
 
         // ---- the next unit
@@ -741,41 +746,72 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
     }
 }
 
-// The units that several shares worked on: one wave per query row, work-groups (share, four rows). D / 4 lanes take a
-// partial's row in 16-byte pieces, 256 / D partials at once.
+// The units that several shares worked on: a wave per query row, `per_wave` rows one after the other (many rows: fewer
+// work-groups, most of which find no open unit). D / 4 lanes take a partial's row in 16-byte pieces, 256 / D partials at
+// once; the maxima, sums and pieces of up to eight each go out together, so that few partials cost one memory round trip
+// behind the share's entry.
 template <class E, int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int rpw) {
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int rpw, int per_wave) {
     const int4 x = a.info[blockIdx.x];
-    const int nseg = x.w, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int r = int(blockIdx.y) * 4 + w, s = x.z * a.spb + r / a.G, h = x.y * a.G + r % a.G;
-    if (nseg == 0 || r >= a.spb * a.G || s >= a.S) return;  // (uniform in the wave)
-    constexpr int TPR = D / 4, NG = 64 / TPR;
+    const int nseg = x.z, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    if (nseg <= 1) return;
+    const int u = x.x % a.units, kh = x.x / a.units % a.Hk, b = x.x / a.units / a.Hk;
+    constexpr int TPR = D / 4, NG = 64 / TPR, U = 8;
     const int gi = lane / TPR, d = lane % TPR * 4;
     const int64_t rec = int64_t(rpw) * (D + 2);
-    const float* base = a.part + int64_t(blockIdx.x) * 2 * rec;
-    auto seg = [&](int i) { return base + (i == 0 ? 1 : 2 * i) * rec; };
-    float M = -INFINITY;
-    for (int i = lane; i < nseg; i += 64) M = fmaxf(M, seg(i)[int64_t(rpw) * D + r]);
-    for (int k = 32; k; k >>= 1) M = fmaxf(M, __shfl_xor(M, k, 64));
-    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-    float sum = 0.f;
-#pragma unroll 4
-    for (int i = gi; i < nseg; i += NG) {
-        const float* p = seg(i);
-        const float mi = p[int64_t(rpw) * D + r];
-        const float wi = mi == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi - M);
-        sum += p[int64_t(rpw) * (D + 1) + r] * wi;
-        o += *reinterpret_cast<const f32x4*>(p + int64_t(r) * D + d) * wi;
-    }
-    for (int k = TPR; k < 64; k <<= 1) {
-        sum += __shfl_xor(sum, k, 64);
+    const float* base = a.part + int64_t(x.y) * 2 * rec;
+    for (int k = 0; k < per_wave; ++k) {
+        const int r = (int(blockIdx.y) * per_wave + k) * 4 + w, s = u * a.spb + r / a.G, h = kh * a.G + r % a.G;
+        if (r >= a.spb * a.G || s >= a.S) return;  // (uniform in the wave)
+        f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+        float M = -INFINITY, sum = 0.f;
+        for (int i0 = 0; i0 < nseg; i0 += U * NG) {
+            f32x4 v[U];
+            float mi[U], li[U];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], k, 64);
+            for (int i = 0; i < U; ++i) {
+                const int sg = min(i0 + i * NG + gi, nseg - 1);  // (past the last: read again, not counted)
+                const float* p = base + (sg == 0 ? 1 : 2 * sg) * rec;
+                mi[i] = p[int64_t(rpw) * D + r];
+                li[i] = p[int64_t(rpw) * (D + 1) + r];
+                v[i] = *reinterpret_cast<const f32x4*>(p + int64_t(r) * D + d);
+            }
+            float top = M;
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                if (i0 + i * NG + gi >= nseg) mi[i] = -INFINITY;
+                top = fmaxf(top, mi[i]);
+            }
+            const float was = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - top);
+            o *= was;
+            sum *= was;
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                if (i0 + i * NG + gi >= nseg) continue;
+                // (a partial without an admitted token has sum 0 and O 0)
+                const float wi = mi[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi[i] - top);
+                sum += li[i] * wi;
+                o += v[i] * wi;
+            }
+            M = top;
+        }
+        float top = M;
+#pragma unroll
+        for (int j = TPR; j < 64; j <<= 1) top = fmaxf(top, __shfl_xor(top, j, 64));
+        const float own = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - top);
+        o *= own;
+        sum *= own;
+#pragma unroll
+        for (int j = TPR; j < 64; j <<= 1) {
+            sum += __shfl_xor(sum, j, 64);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], j, 64);
+        }
+        if (gi != 0) continue;
+        const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+        *reinterpret_cast<uint2*>(a.out + ((int64_t(b) * a.S + s) * a.H + h) * D + d) =
+            sum == 0.f ? make_uint2(0u, 0u) : make_uint2(E::pair(o[0] * inv, o[1] * inv), E::pair(o[2] * inv, o[3] * inv));
     }
-    if (gi != 0) return;
-    const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
-    *reinterpret_cast<uint2*>(a.out + ((int64_t(x.x) * a.S + s) * a.H + h) * D + d) =
-        sum == 0.f ? make_uint2(0u, 0u) : make_uint2(E::pair(o[0] * inv, o[1] * inv), E::pair(o[2] * inv, o[3] * inv));
 }
 
 // ---- the selection ----------------------------------------------------------------------------------------
@@ -786,6 +822,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int rpw) {
 // c16) in element r): a wave takes 16 pages, so the longest context spreads over all CUs. (One thread per page on the vector
 // units: 94.8 us for 8 rows over 250 pages of head_dim 256, 21 us for 1 row over 2046 of 128.)
 constexpr int SCORE_ROWS = 16;
+constexpr int FEW_ROWS = 4;  // rows up to which the vector units take them: an MFMA of one row takes as long as of 16
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 typedef double f64x2 __attribute__((ext_vector_type(2)));
 template <class E, int D>
@@ -812,6 +849,35 @@ __global__ __launch_bounds__(256) void block_score_kernel(PagedArgs a) {
         qs[s * QR + d] = t;
     }
     __syncthreads();
+    auto put = [&](int s, double z) {
+        z += 0.0;  // (-0 and 0 are one score)
+        const uint64_t x = __builtin_bit_cast(uint64_t, z);
+        a.keys[((int64_t(b) * a.S + s0 + s) * a.Hk + kh) * a.W + j] = !in || z != z ? 0 : (x >> 63 ? ~x : x | (uint64_t(1) << 63));
+    };
+    if (ns <= FEW_ROWS) {  // (uniform)
+        double kd[D / 4];
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+            for (int x = 0; x < 8; ++x) kd[8 * i + x] = double(E::to_f32(uint16_t(k[i][x / 2] >> (16 * (x & 1)))));
+        for (int s = 0; s < ns; ++s) {
+            const double* q = qs + s * QR + 8 * g;
+            double t0 = 0, t1 = 0;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const f64x2 qq = *reinterpret_cast<const f64x2*>(q + 32 * i + 2 * x);
+                    t0 = fma(qq[0], kd[8 * i + 2 * x], t0);
+                    t1 = fma(qq[1], kd[8 * i + 2 * x + 1], t1);
+                }
+            t0 += t1;
+            t0 += __shfl_xor(t0, 16, 64);
+            t0 += __shfl_xor(t0, 32, 64);
+            if (g == 0 && j < j_end) put(s, t0);
+        }
+        return;
+    }
     const double* q = qs + min(c16, ns - 1) * QR + 8 * g;  // (rows past the last repeat it: their products are not written)
     f64x4 dot = {0, 0, 0, 0};
 #pragma unroll
@@ -824,13 +890,8 @@ __global__ __launch_bounds__(256) void block_score_kernel(PagedArgs a) {
         }
     if (j >= j_end) return;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int s = 4 * r + g;
-        const double z = dot[r] + 0.0;  // (-0 and 0 are one score)
-        const uint64_t u = __builtin_bit_cast(uint64_t, z);
-        if (s < ns)
-            a.keys[((int64_t(b) * a.S + s0 + s) * a.Hk + kh) * a.W + j] = !in || z != z ? 0 : (u >> 63 ? ~u : u | (uint64_t(1) << 63));
-    }
+    for (int r = 0; r < 4; ++r)
+        if (4 * r + g < ns) put(4 * r + g, dot[r]);
 }
 
 __device__ __forceinline__ int wave_incl_sum(int v, int lane) {
@@ -1065,12 +1126,18 @@ int launch(PagedArgs& a, hipStream_t st) {
         allow_smem(reinterpret_cast<const void*>(&paged_attn_kernel<E, D, TPW, RTW, P, WPC, SEL>), lds);
         allowed.fetch_or(bit, std::memory_order_relaxed);
     }
-    const int grid = a.whole ? a.B * a.Hk * a.units : CUS * WPC;
+    // (units enough for every work-group there is room for: whole ones, without partials)
+    const int units = a.B * a.Hk * a.units;
+    if (a.units > 1 && units >= CUS * WPC) a.whole = 1;
+    const int grid = a.whole ? units : CUS * WPC;
+    a.by_unit = units <= grid;  // (every unit is begun by one share, which writes its entry)
     hipLaunchKernelGGL((paged_attn_kernel<E, D, TPW, RTW, P, WPC, SEL>), dim3(unsigned(grid)), dim3(Geo::NT), lds, st, a);
     MDX_LAUNCHED();
     if (a.whole) return MDX_OK;
     const int rows = (a.spb < a.S ? a.spb : a.S) * a.G;
-    hipLaunchKernelGGL((paged_join_kernel<E, D>), dim3(unsigned(grid), unsigned((rows + 3) / 4)), dim3(256), 0, st, a, Geo::RPW);
+    const int per_wave = rows > 64 ? 4 : 1;
+    hipLaunchKernelGGL((paged_join_kernel<E, D>), dim3(unsigned(units < grid ? units : grid), unsigned((rows + 4 * per_wave - 1) / (4 * per_wave))), dim3(256), 0, st,
+                       a, Geo::RPW, per_wave);
     MDX_LAUNCHED();
     return MDX_OK;
 }
