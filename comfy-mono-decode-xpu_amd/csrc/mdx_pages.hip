@@ -22,7 +22,6 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 constexpr int PLAN_T = 1024;      // threads of the planning work-group
 constexpr int MAX_SEQS = 1024;    // pairs of a fork, sequences of a commit: one planning thread each
 constexpr int MAX_PATH = 64;      // rows of a committed path
-constexpr int SUM_T = PLAN_T;     // threads of a work-group of commit's second launch
 
 // ---- the free pages -------------------------------------------------------------------------------------
 // Inclusive sum over the work-group's threads (16 waves), and the total; `tmp` of 16 ints. Every thread calls it.
@@ -177,11 +176,13 @@ __global__ __launch_bounds__(PLAN_T) void fork_plan_kernel(ForkArgs a, int rows)
         }
     }
     if (!valid) n = need = copies = 0;
-    int want, all;
-    const int upto = block_sum_incl(need, tmp, want);
-    const int have = want > 0 ? free_pages(a.refs, a.P, want, a.fresh, tmp) : 0;
+    int want = 0, all = 0, upto = 0, have = 0, cend = 0;
+    if (__syncthreads_or(need)) {
+        upto = block_sum_incl(need, tmp, want);
+        have = free_pages(a.refs, a.P, want, a.fresh, tmp);
+    }
     const bool served = valid && upto <= have;
-    const int cend = block_sum_incl(served ? copies : 0, tmp, all);
+    if (__syncthreads_or(served ? copies : 0)) cend = block_sum_incl(served ? copies : 0, tmp, all);
     if (i < a.M) {
         reinterpret_cast<int4*>(a.pair)[i] = make_int4(valid ? (served ? 1 : 0) : -1, n, upto - need, cend - copies);
         a.status[i] = valid ? (served ? 1 : 0) : -1;
@@ -266,8 +267,7 @@ struct CommitArgs {
     int64_t* slots;       // [B][room] or null
     int32_t* status;
     int B, W, P, T, lt, D, L, Hk, R, room, half;  // half: fp16 elements, else bf16
-    int per_wg;           // chunks a work-group of the move takes
-    int32_t* state;       // [B]: a sequence's tokens before the commit, -1 where it is refused or left alone (the first launch's)
+    int per_wg, wgs;      // chunks a work-group of the move takes, and such work-groups per sequence
     int32_t* fresh;
 };
 
@@ -277,37 +277,71 @@ __device__ __forceinline__ int page_at(const CommitArgs& a, int b, int64_t t) {
     return e >= 0 && e < a.P ? e : -1;
 }
 
-// First launch: which sequences can be committed (`state`: the second launch may overwrite the lengths), and rows
-// n + path[k] to n + k. Work-group (x, b); every one checks its sequence for itself. One holds every row of its chunks in
-// registers before it writes one, so no order among the rows matters; chunks do not meet. Bound by latency (dependent
-// round trips), hence many small work-groups: 32 sequences of 8 rows over 128 chunks are 1024.
-__global__ __launch_bounds__(256) void commit_move_kernel(CommitArgs a) {
+__device__ __forceinline__ float el(uint16_t x, int half) { return half ? fp16_to_f32(x) : bf2f(x); }
+__device__ __forceinline__ uint16_t to_el(float f, int half) {
+    return half ? __builtin_bit_cast(uint16_t, static_cast<_Float16>(f)) : f2bf(f);
+}
+
+__device__ __forceinline__ bool commit_fits(const CommitArgs& a, int n, int c) {
+    return c >= 0 && n >= 0 && !(a.path && c > a.R) && int64_t(n) + c <= int64_t(a.W) << a.lt;
+}
+
+// The mean key of page e in chunk kc (layer, kv head), by one wave: a lane holds eight dims of every (64 / (D / 8))-th row,
+// fp32 sums, the row groups joined by lane exchanges, one rounding to the cache's type.
+__device__ void mean_key(const CommitArgs& a, int64_t kc, int e, int lane) {
+    const int lanes = a.D / 8, step = 64 / lanes, sub = lane / lanes, d8 = lane % lanes * 8;
+    const float inv = 1.f / float(a.T);  // (a power of two: exact)
+    const int64_t layer = kc / a.Hk, h = kc % a.Hk;
+    const uint16_t* keys = reinterpret_cast<const uint16_t*>(a.kv) + (((layer * 2 * a.Hk + h) * a.P + e) << a.lt) * a.D + d8;
+    float s[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] = 0.f;
+#pragma unroll 8
+    for (int r = sub; r < a.T; r += step) {
+        const u32x4 v = *reinterpret_cast<const u32x4*>(keys + int64_t(r) * a.D);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            s[2 * i] += el(uint16_t(v[i] & 0xFFFFu), a.half);
+            s[2 * i + 1] += el(uint16_t(v[i] >> 16), a.half);
+        }
+    }
+    for (int d = lanes; d < 64; d <<= 1)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i] += __shfl_xor(s[i], d, 64);
+    if (sub == 0) {
+        u32x4 o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            o[i] = unsigned(to_el(s[2 * i] * inv, a.half)) | (unsigned(to_el(s[2 * i + 1] * inv, a.half)) << 16);
+        *reinterpret_cast<u32x4*>(a.ksum + (kc * a.P + e) * a.D + d8) = o;
+    }
+}
+
+// Sequence b's rows n + path[k] to n + k, and the mean keys of the pages that fill, for the chunks from c0. The work-group
+// holds every row of its chunks in registers before it writes one, so no order among the rows matters; chunks do not meet.
+// Bound by latency (dependent round trips), hence many work-groups: 32 sequences of 8 rows over 128 chunks are 256.
+__device__ void commit_move(const CommitArgs& a, int b, int c0) {
     __shared__ int64_t from[MAX_PATH], to[MAX_PATH];
     __shared__ int bad;
-    const int b = blockIdx.y, n = a.length[b], c = a.count[b], t = threadIdx.x;
-    const bool fits = c >= 0 && n >= 0 && !(a.path && c > a.R) && int64_t(n) + c <= int64_t(a.W) << a.lt;
-    if (t == 0) bad = !fits;
+    const int n = a.length[b], c = a.count[b], t = threadIdx.x;
+    if (!commit_fits(a, n, c)) return;  // (uniform)
+    if (t == 0) bad = 0;
     __syncthreads();
-    if (fits) {
-        if (a.path && t < c) {
-            const int32_t* path = a.path + int64_t(b) * a.R;
-            const int k = path[t], before = t ? path[t - 1] : -1;
-            const int p = k >= 0 && k < a.R ? page_at(a, b, int64_t(n) + k) : -1, q = page_at(a, b, int64_t(n) + t);
-            from[t] = k == t ? -1 : (int64_t(p) << a.lt) + ((n + k) & (a.T - 1));
-            to[t] = (int64_t(q) << a.lt) + ((n + t) & (a.T - 1));
-            if (k <= before || p < 0 || q < 0) bad = 1;
-        }
-        // the entries of the committed rows have to be pages
-        for (int j = (n >> a.lt) + t; j < (n + c + a.T - 1) >> a.lt; j += 256)
-            if (page_at(a, b, int64_t(j) << a.lt) < 0) bad = 1;
+    const int j0 = n >> a.lt, j1 = (n + c + a.T - 1) >> a.lt;
+    if (t < c) {
+        const int32_t* path = a.path + int64_t(b) * a.R;
+        const int k = path[t], before = t ? path[t - 1] : -1;
+        const int p = k >= 0 && k < a.R ? page_at(a, b, int64_t(n) + k) : -1, q = page_at(a, b, int64_t(n) + t);
+        from[t] = k == t ? -1 : (int64_t(p) << a.lt) + ((n + k) & (a.T - 1));
+        to[t] = (int64_t(q) << a.lt) + ((n + t) & (a.T - 1));
+        if (k <= before || p < 0 || q < 0) bad = 1;
     }
+    if (t >= MAX_PATH && t - MAX_PATH < j1 - j0 && page_at(a, b, int64_t(j0 + t - MAX_PATH) << a.lt) < 0) bad = 1;
     __syncthreads();
-    if (blockIdx.x == 0 && t == 0) a.state[b] = bad ? -1 : n;
-    if (bad || !a.path) return;  // (uniform)
+    if (bad) return;
     const int lanes = a.D / 8, items = c * lanes;  // 16-byte pieces of a chunk's rows
-    const int chunks = a.L * 2 * a.Hk, c0 = blockIdx.x * a.per_wg;
-    const int live = min(a.per_wg, chunks - c0) * items;
-    constexpr int MOST = 8;  // 64 rows of 32 pieces over 256 threads
+    const int chunks = a.L * 2 * a.Hk, mine = min(a.per_wg, chunks - c0), live = mine * items;
+    constexpr int MOST = 2;  // 64 rows of 32 pieces
     u32x4 v[MOST];
     const int64_t chunk_bytes = (int64_t(a.P) << a.lt) * a.D * 2;
     auto place = [&](int x, const int64_t* rows) -> unsigned char* {
@@ -316,108 +350,64 @@ __global__ __launch_bounds__(256) void commit_move_kernel(CommitArgs a) {
     };
 #pragma unroll
     for (int i = 0; i < MOST; ++i) {
-        if (i * 256 >= live) break;  // (uniform)
-        const int x = i * 256 + t;
+        const int x = i * PLAN_T + t;
         unsigned char* p = x < live ? place(x, from) : nullptr;
         if (p) v[i] = *reinterpret_cast<const u32x4*>(p);
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < MOST; ++i) {
-        if (i * 256 >= live) break;
-        const int x = i * 256 + t;
+        const int x = i * PLAN_T + t;
         unsigned char* p = x < live ? place(x, to) : nullptr;
         if (p) *reinterpret_cast<u32x4*>(p) = v[i];
     }
+    const int filled = ((n + c) >> a.lt) - j0;
+    if (!a.ksum || filled == 0) return;
+    __syncthreads();  // (the rows above, read by other waves)
+    for (int x = t >> 6; x < filled * mine; x += PLAN_T / 64) {
+        const int chunk = c0 + x % mine, kc = chunk / (2 * a.Hk) * a.Hk + chunk % (2 * a.Hk);
+        if (chunk % (2 * a.Hk) >= a.Hk) continue;  // (values)
+        mean_key(a, kc, page_at(a, b, int64_t(j0 + x / mine) << a.lt), t & 63);
+    }
 }
 
-__device__ __forceinline__ float el(uint16_t x, int half) { return half ? fp16_to_f32(x) : bf2f(x); }
-__device__ __forceinline__ uint16_t to_el(float f, int half) {
-    return half ? __builtin_bit_cast(uint16_t, static_cast<_Float16>(f)) : f2bf(f);
-}
-
-// Mean keys of the pages that the commit fills. One wave per (page, layer, kv head): a lane holds eight dims of every
-// (64 / (D / 8))-th row, fp32 sums, the row groups joined by lane exchanges, one rounding to the cache's type. The pages
-// of all sequences are numbered through (their counts summed in every work-group), so a batch of short tails and one
-// long prompt spread alike. Bound by the bytes of the keys.
+// Mean keys of the pages that a commit without a path fills, one wave per (page, layer, kv head). The pages of all sequences
+// are numbered through (their counts summed in every work-group), so a batch of short tails and one long prompt spread
+// alike. Bound by the bytes of the keys.
 __device__ void commit_sums(const CommitArgs& a, int block, int blocks) {
-    constexpr int EACH = MAX_SEQS / SUM_T;
-    __shared__ int upto[MAX_SEQS];  // pages filled in sequences 0..b
-    __shared__ int wsum[SUM_T / 64];
-    const int t = threadIdx.x, lane = t & 63;
-    int mine[EACH], sum = 0;
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-        const int b = t * EACH + i;
-        int f = 0;
-        if (b < a.B) {
-            const int n = a.state[b];
-            if (n >= 0) f = ((n + a.count[b]) >> a.lt) - (n >> a.lt);
-        }
-        sum += f;
-        mine[i] = sum;
+    __shared__ int upto[MAX_SEQS], first[MAX_SEQS], tmp[PLAN_T / 64];  // pages filled in sequences 0..b, their first
+    const int t = threadIdx.x;
+    int f = 0;
+    if (t < a.B) {
+        const int n = a.length[t], c = a.count[t];
+        first[t] = n >> a.lt;
+        if (commit_fits(a, n, c)) f = ((n + c) >> a.lt) - (n >> a.lt);
     }
-    int incl = sum;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int u = __shfl_up(incl, d, 64);
-        if (lane >= d) incl += u;
-    }
-    if (lane == 63) wsum[t >> 6] = incl;
+    int total;
+    upto[t] = block_sum_incl(f, tmp, total);
     __syncthreads();
-    int before = incl - sum;
-    for (int w = 0; w < (t >> 6); ++w) before += wsum[w];
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) upto[t * EACH + i] = before + mine[i];
-    __syncthreads();
-    const int64_t keys = int64_t(a.L) * a.Hk, jobs = upto[MAX_SEQS - 1] * keys;
-    const int lanes = a.D / 8, step = 64 / lanes, sub = lane / lanes, d8 = lane % lanes * 8;
-    const float inv = 1.f / float(a.T);  // (a power of two: exact)
-    for (int64_t job = int64_t(block) * (SUM_T / 64) + (t >> 6); job < jobs; job += int64_t(blocks) * (SUM_T / 64)) {
+    const int64_t keys = int64_t(a.L) * a.Hk, jobs = total * keys;
+    for (int64_t job = int64_t(block) * (PLAN_T / 64) + (t >> 6); job < jobs; job += int64_t(blocks) * (PLAN_T / 64)) {
         const int page_no = int(job / keys);
-        const int64_t kc = job % keys;
         int lo = 0, hi = a.B - 1;  // the sequence: the first whose sum passes page_no
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
             if (upto[mid] > page_no) hi = mid;
             else lo = mid + 1;
         }
-        const int j = (a.state[lo] >> a.lt) + page_no - (lo ? upto[lo - 1] : 0);
-        const int e = page_at(a, lo, int64_t(j) << a.lt);
-        if (e < 0) continue;
-        const int64_t layer = kc / a.Hk, h = kc % a.Hk;
-        const uint16_t* keys_ = reinterpret_cast<const uint16_t*>(a.kv) + (((layer * 2 * a.Hk + h) * a.P + e) << a.lt) * a.D + d8;
-        float s[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s[i] = 0.f;
-#pragma unroll 8
-        for (int r = sub; r < a.T; r += step) {
-            const u32x4 v = *reinterpret_cast<const u32x4*>(keys_ + int64_t(r) * a.D);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                s[2 * i] += el(uint16_t(v[i] & 0xFFFFu), a.half);
-                s[2 * i + 1] += el(uint16_t(v[i] >> 16), a.half);
-            }
-        }
-        for (int d = lanes; d < 64; d <<= 1)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s[i] += __shfl_xor(s[i], d, 64);
-        if (sub == 0) {
-            u32x4 o;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                o[i] = unsigned(to_el(s[2 * i] * inv, a.half)) | (unsigned(to_el(s[2 * i + 1] * inv, a.half)) << 16);
-            *reinterpret_cast<u32x4*>(a.ksum + (kc * a.P + e) * a.D + d8) = o;
-        }
+        const int e = page_at(a, lo, int64_t(first[lo] + page_no - (lo ? upto[lo - 1] : 0)) << a.lt);
+        if (e >= 0) mean_key(a, job % keys, e, t & 63);
     }
 }
 
 // Lengths, pages for the next rows and their slots: one thread per sequence (a span of many entries by a whole wave).
 __device__ void commit_plan(const CommitArgs& a) {
-    __shared__ int tmp[PLAN_T / 64], ends[MAX_SEQS];
+    __shared__ int tmp[PLAN_T / 64], ends[MAX_SEQS], bad[MAX_SEQS];
     const int b = threadIdx.x, lane = b & 63;
-    const int n = b < a.B ? a.state[b] : -1, c = b < a.B ? a.count[b] : 0, was = b < a.B ? a.length[b] : 0;
-    const bool valid = n >= 0;
+    const int n = b < a.B ? a.length[b] : -1, c = b < a.B ? a.count[b] : 0;
+    bad[b] = 0;
+    ends[b] = n;
+    bool valid = b < a.B && commit_fits(a, n, c);
     int64_t total = 0;
     bool narrow = false;  // (room past the table's width gets no page)
     if (valid) {
@@ -425,29 +415,61 @@ __device__ void commit_plan(const CommitArgs& a) {
         narrow = total > a.W;
         if (narrow) total = a.W;
     }
-    // missing entries behind the committed rows' are given
-    const int j1 = valid ? (n + c + a.T - 1) >> a.lt : 0, j2 = int(total);
-    int need = 0;
-    const bool wide = valid && j2 - j1 > 8;
-    if (valid && !wide)
-        for (int j = j1; j < j2; ++j) need += page_at(a, b, int64_t(j) << a.lt) < 0;
+    // the committed rows' entries have to be pages; missing ones behind them are given
+    const int j0 = n >> a.lt, j1 = valid ? (n + c + a.T - 1) >> a.lt : 0, j2 = int(total);
+    int need = 0, holes = 0;
+    const bool wide = valid && j2 - j0 > 8;
+    if (valid && !wide) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int j = j0 + i;
+            const bool miss = j < j2 && page_at(a, b, int64_t(j) << a.lt) < 0;
+            holes += miss && j < j1;
+            need += miss && j >= j1;
+        }
+    }
+    if (a.path) {  // the checks of the move, a thread per row
+        __syncthreads();
+        for (int x = b; x < a.B * a.R; x += PLAN_T) {
+            const int q = x / a.R, k = x % a.R, cq = a.count[q], nq = ends[q];
+            if (!commit_fits(a, nq, cq) || k >= cq) continue;
+            const int p = a.path[x], before = k ? a.path[x - 1] : -1;
+            if (p <= before || p >= a.R || page_at(a, q, int64_t(nq) + p) < 0) bad[q] = 1;
+        }
+        __syncthreads();
+    }
     uint64_t todo = __builtin_amdgcn_ballot_w64(wide);
     while (todo) {  // (uniform in the wave)
         const int l = __builtin_ctzll(todo);
         todo &= todo - 1;
-        const int bb = __builtin_amdgcn_readlane(b, l), x1 = __builtin_amdgcn_readlane(j1, l), x2 = __builtin_amdgcn_readlane(j2, l);
-        int miss = 0;
+        const int bb = __builtin_amdgcn_readlane(b, l), x0 = __builtin_amdgcn_readlane(j0, l), x1 = __builtin_amdgcn_readlane(j1, l),
+                  x2 = __builtin_amdgcn_readlane(j2, l);
+        int in = 0, behind = 0;
 #pragma unroll 4
-        for (int j = x1 + lane; j < x2; j += 64) miss += page_at(a, bb, int64_t(j) << a.lt) < 0;
-        for (int d = 32; d; d >>= 1) miss += __shfl_xor(miss, d, 64);
-        if (lane == l) need = miss;
+        for (int j = x0 + lane; j < x2; j += 64) {
+            const bool miss = page_at(a, bb, int64_t(j) << a.lt) < 0;
+            in += miss && j < x1;
+            behind += miss && j >= x1;
+        }
+        for (int d = 32; d; d >>= 1) {
+            in += __shfl_xor(in, d, 64);
+            behind += __shfl_xor(behind, d, 64);
+        }
+        if (lane == l) {
+            holes = in;
+            need = behind;
+        }
     }
-    int want;
-    const int upto = block_sum_incl(need, tmp, want);
-    const int have = want > 0 ? free_pages(a.refs, a.P, want, a.fresh, tmp) : 0;
-    __syncthreads();  // (the list, written by other threads)
+    valid = valid && holes == 0 && bad[b] == 0;
+    if (!valid) need = 0;
+    int upto = 0, have = 0;
+    if (__syncthreads_or(need)) {  // (most steps stay in their pages)
+        int want;
+        upto = block_sum_incl(need, tmp, want);
+        have = free_pages(a.refs, a.P, want, a.fresh, tmp);
+        __syncthreads();  // (the list, written by other threads)
+    }
     const bool served = valid && upto <= have;
-    const int end = valid ? n + c : 0;
     if (served && need && !wide) {
         int at = upto - need;
         for (int j = j1; j < j2; ++j)
@@ -463,8 +485,8 @@ __device__ void commit_plan(const CommitArgs& a) {
         todo &= todo - 1;
         const int bb = __builtin_amdgcn_readlane(b, l), x1 = __builtin_amdgcn_readlane(j1, l), x2 = __builtin_amdgcn_readlane(j2, l);
         int at = __builtin_amdgcn_readlane(upto - need, l);
-        for (int j0 = x1; j0 < x2; j0 += 64) {
-            const int j = j0 + lane;
+        for (int k0 = x1; k0 < x2; k0 += 64) {
+            const int j = k0 + lane;
             const bool miss = j < x2 && page_at(a, bb, int64_t(j) << a.lt) < 0;
             const uint64_t m = __builtin_amdgcn_ballot_w64(miss);
             if (miss) {
@@ -475,10 +497,10 @@ __device__ void commit_plan(const CommitArgs& a) {
             at += __popcll(m);
         }
     }
-    ends[b] = valid ? end : -1;
+    ends[b] = valid ? n + c : -1;
     if (b < a.B) {
         a.status[b] = valid ? (served && !narrow ? 1 : 0) : (c < 0 ? 1 : -1);
-        a.new_length[b] = valid ? end : was;
+        a.new_length[b] = valid ? n + c : n;
     }
     if (!a.slots) return;
     __syncthreads();  // (ends, and the entries given above)
@@ -490,10 +512,14 @@ __device__ void commit_plan(const CommitArgs& a) {
     }
 }
 
-// Second launch: work-group 0 plans, the others (none without mean keys) sum.
-__global__ __launch_bounds__(SUM_T) void commit_plan_kernel(CommitArgs a) {
-    if (blockIdx.x == 0) commit_plan(a);
-    else commit_sums(a, blockIdx.x - 1, gridDim.x - 1);
+// The plan (`plans` work-groups, 1 or 0) and the moves and means, in one launch where the new lengths go elsewhere than the
+// old ones. They do not meet: the plan changes entries behind the committed rows' alone, of sequences whose rows all have
+// pages already, and each checks a sequence alike.
+__global__ __launch_bounds__(PLAN_T) void commit_kernel(CommitArgs a, int plans) {
+    const int x = int(blockIdx.x) - plans;
+    if (x < 0) commit_plan(a);
+    else if (a.path) commit_move(a, x / a.wgs, x % a.wgs * a.per_wg);
+    else commit_sums(a, x, int(gridDim.x) - plans);
 }
 
 int log2_of(int64_t T) {
@@ -566,7 +592,7 @@ extern "C" int mdx_page_fork(void* kv, void* ksum, int64_t L, int64_t Hk, int64_
 
 extern "C" size_t mdx_page_commit_workspace(int64_t B, int64_t W) {
     if (B < 1 || B > MAX_SEQS || W < 1 || W > (int64_t(1) << 26)) return 0;
-    return size_t(B * W + (B + 3) / 4 * 4) * 4;
+    return size_t(B * W) * 4;
 }
 
 extern "C" int mdx_page_commit(void* kv, void* ksum, int32_t dtype, int64_t L, int64_t Hk, int64_t P, int64_t T, int64_t D,
@@ -601,17 +627,22 @@ extern "C" int mdx_page_commit(void* kv, void* ksum, int32_t dtype, int64_t L, i
     a.status = status;
     a.B = int(B), a.W = int(W), a.P = int(P), a.T = int(T), a.lt = lt, a.D = int(D), a.L = int(L), a.Hk = int(Hk);
     a.R = int(path ? R : 0), a.room = int(room), a.half = dtype == MDX_DT_F16;
-    a.state = static_cast<int32_t*>(workspace);
-    a.fresh = a.state + (B + 3) / 4 * 4;
+    a.fresh = static_cast<int32_t*>(workspace);
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int64_t chunks = L * 2 * Hk;
-    // chunks per work-group: 512 pieces of 16 bytes where that is more than one chunk's (two in flight per thread)
+    // chunks per work-group of the move: 2048 pieces of 16 bytes (two in flight per thread)
     const int64_t items = (path ? R : 1) * D / 8;
-    a.per_wg = int(items >= 512 ? 1 : 512 / items);
-    const int64_t wgs = path ? (chunks + a.per_wg - 1) / a.per_wg : 1;
-    hipLaunchKernelGGL(commit_move_kernel, dim3(unsigned(wgs), unsigned(B)), dim3(256), 0, st, a);
-    MDX_LAUNCHED();
-    hipLaunchKernelGGL(commit_plan_kernel, dim3(ksum ? 257 : 1), dim3(PLAN_T), 0, st, a);
+    a.per_wg = int(2048 / items);
+    a.wgs = int((chunks + a.per_wg - 1) / a.per_wg);
+    const int64_t work = path ? B * a.wgs : ksum ? 256 : 0;
+    MDX_CHECK(work < (int64_t(1) << 30), "too many chunks times sequences");
+    if (work && new_length == length) {
+        hipLaunchKernelGGL(commit_kernel, dim3(unsigned(work)), dim3(PLAN_T), 0, st, a, 0);
+        MDX_LAUNCHED();
+        hipLaunchKernelGGL(commit_kernel, dim3(1), dim3(PLAN_T), 0, st, a, 1);
+    } else {
+        hipLaunchKernelGGL(commit_kernel, dim3(unsigned(1 + work)), dim3(PLAN_T), 0, st, a, 1);
+    }
     MDX_LAUNCHED();
     return MDX_OK;
 }

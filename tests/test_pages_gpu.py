@@ -258,3 +258,13 @@ def test_refusals(C, dev):
         C.page_fork(kv, ksum, table, length, refs, two, i32([0]))
     with pytest.raises(RuntimeError, match="room"):
         C.page_fork(kv, ksum, table, length, refs, two, two, -1)
+
+
+@pytest.mark.parametrize("with_path", [True, False])
+def test_commit_into_other_lengths(C, dev, with_path):
+    """One launch for the move, the means and the plan: the same as in place, refused and starved sequences among them."""
+    st = State(23, [10, 20, 30, 40, 47, 60, 5, 0], P=26, held=8, W=5)
+    st.table[4, 3], st.table[5, 4] = -1, 70
+    path = [[0, 1, 2, 3], [0, 2, 3, 3], [1, 0, 2, 3], [0, 1, 2, 4], [0, 1, 2, 3], [0, 1, 2, 3], [0, 3, 3, 3], [0, 1, 2, 3]]
+    assert _commit(C, dev, st, [4, 3, 2, 4, 2, 4, 2, 0], path if with_path else None, 13, in_place=False)
+    assert _commit(C, dev, st, [4, 3, 2, 4, 2, 4, -1, 0], path if with_path else None, 13)
