@@ -234,22 +234,22 @@ __device__ __forceinline__ int steps_of(const PagedArgs& a, const Span& s, int u
 
 // One work-group: RTW waves of row tiles (TPW tiles of 16 query rows each) times P token parts.
 // (WPC of them share a CU: waves that meet at a barrier are then not all of the CU's)
-template <int D, int TPW, int RTW, int P, int WPC>
+template <int D, int TPW, int RTW, int P, int WPC, int SUB>
 struct Geometry {
     static constexpr int NT = 64 * RTW * P;
     static constexpr int RPW = 16 * TPW * RTW;
-    static constexpr int STAGE = STEP * 2 * D;                    // bytes of K (or V) per stage
+    static constexpr int STAGE = STEP * SUB * 2 * D;              // bytes of K (or V) per stage of SUB 32-token pieces
     static constexpr int RING = RING_BYTES / WPC;
     static constexpr int NS = RING / (2 * STAGE * P);             // ring stages per part
     static constexpr int PER = STAGE / 1024 / RTW;                // direct loads per wave, stage and matrix
-    static_assert(NS >= 1 && (NS & (NS - 1)) == 0 && PER >= 1 && (RTW == 1 || NS >= 2), "ring geometry");
+    static_assert(NS >= 1 && (NS & (NS - 1)) == 0 && PER >= 1 && (RTW == 1 ? SUB == 1 : NS >= 2) && (SUB == 1 || D != 256), "ring geometry");
 };
 
-template <class E, int D, int TPW, int RTW, int P, int WPC, bool SEL>
+template <class E, int D, int TPW, int RTW, int P, int WPC, int SUB, bool SEL>
 __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_kernel(PagedArgs a) {
-    using Geo = Geometry<D, TPW, RTW, P, WPC>;
+    using Geo = Geometry<D, TPW, RTW, P, WPC, SUB>;
     constexpr int NT = Geo::NT, RPW = Geo::RPW, STAGE = Geo::STAGE, NS = Geo::NS, PER = Geo::PER;
-    constexpr int KK = D / 32, DT = D / 16, TOK = STEP * P;
+    constexpr int KK = D / 32, DT = D / 16, ST = STEP * SUB, TOK = ST * P;
     extern __shared__ __align__(256) unsigned char smem[];  // (the reads' exclusive ors need rows aligned to 256 bytes)
     __shared__ int sh_sum[NT / 64], sh_at[4], odd;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -369,10 +369,11 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
         const unsigned char* vbase = reinterpret_cast<const unsigned char*>(a.value + kh * a.vh);
         const int32_t* row = a.table + b * a.ts;
         const int32_t* picked = SEL ? a.page + ((int64_t(b) * a.S + u) * a.Hk + kh) * a.most : nullptr;
-        struct Two {
-            int e[2];
+        constexpr int QT = 2 * SUB;  // 16-token pieces of a stage, each of one page
+        struct Pages {
+            int e[QT];
         };
-        const bool one_page = a.lt >= 5;  // (a stage's 32 tokens stand in one page)
+        const bool one_page = a.lt >= (SUB == 1 ? 5 : 6);  // (a stage's tokens stand in one page)
         auto entry = [&](int v) {
             if (v >= t_end) return -1;
             if (SEL && v < sp.nsel) return uload(picked + (v >> a.lt));
@@ -380,34 +381,46 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
             return j < a.W ? uload(row + j) : -1;
         };
         auto entries = [&](int s) {
-            const int v0 = (step0 + s) * TOK + part * STEP;
-            Two x;
+            const int v0 = (step0 + s) * TOK + part * ST;
+            Pages x;
             x.e[0] = entry(v0);
-            x.e[1] = one_page ? 0 : entry(v0 + 16);  // (one page: unused; a copy would wait for the load here)
+#pragma unroll
+            for (int h = 1; h < QT; ++h) x.e[h] = one_page ? 0 : entry(v0 + 16 * h);  // (one page: unused; a copy would wait here)
             return x;
         };
-        uint32_t hist = 0;  // two bits per stage issued: its halves stand in pages
-        // A wave's loads of a stage lie in one half where several waves share them: only that half's address is formed.
-        constexpr int HALF = 16 / TPL;  // loads of a half
+        uint32_t hist = 0;  // QT bits per stage issued: its 16-token pieces stand in pages
+        // A wave's loads of a stage lie in one piece where several waves share them: only that piece's address is formed.
+        constexpr int HALF = 16 / TPL;  // loads of a piece
         constexpr int HW = PER <= HALF ? 1 : 2;
-        const int h_own = HW == 1 ? rw * PER / HALF : 0;  // (the wave's half)
+        static_assert(HW == 1 || SUB == 1, "");
+        const int h_own = HW == 1 ? rw * PER / HALF : 0;  // (the wave's piece)
         const unsigned char *kp_[HW], *vp_[HW];
-        auto place = [&](int s, Two x) {
-            const int v0 = (step0 + s) * TOK + part * STEP;
+        auto place = [&](int s, Pages x) {
+            const int v0 = (step0 + s) * TOK + part * ST;
             const uint32_t r0 = uint32_t(SEL && v0 >= sp.nsel ? v0 - sp.nsel : v0);
-            const bool in0 = uint32_t(x.e[0]) < uint32_t(a.P), in1 = one_page ? in0 : uint32_t(x.e[1]) < uint32_t(a.P);
-            hist = (hist << 2) | (in0 ? 1u : 0u) | (in1 ? 2u : 0u);
+            const bool in0 = uint32_t(x.e[0]) < uint32_t(a.P);
+            uint32_t ok = in0 ? (1u << QT) - 1u : 0u;
+            int e_own = x.e[0];
+            if (!one_page) {
+                ok = in0 ? 1u : 0u;
+#pragma unroll
+                for (int h = 1; h < QT; ++h) {
+                    ok |= uint32_t(x.e[h]) < uint32_t(a.P) ? 1u << h : 0u;
+                    e_own = h_own == h ? x.e[h] : e_own;
+                }
+            }
+            hist = (hist << QT) | ok;
 #pragma unroll
             for (int i = 0; i < HW; ++i) {
-                const int h = HW == 1 ? h_own : i;
                 if (i == 1 && one_page) {
                     kp_[HW - 1] = kp_[0] + 16 * row_k;
                     vp_[HW - 1] = vp_[0] + 16 * row_v;
                     break;
                 }
-                // (a half without a page reads the pool's first rows: in bounds, and masked)
-                const bool in = h ? in1 : in0;
-                const uint32_t e = in ? uint32_t(h && !one_page ? x.e[1] : x.e[0]) : 0u;
+                // (a piece without a page reads the pool's first rows: in bounds, and masked)
+                const int h = HW == 1 ? h_own : i, own = HW == 1 ? e_own : x.e[i];
+                const bool in = uint32_t(own) < uint32_t(a.P);
+                const uint32_t e = in ? uint32_t(own) : 0u;
                 const uint32_t r = in ? (r0 + 16 * h) & ((1u << a.lt) - 1u) : 0u;
                 kp_[i] = kbase + (uint64_t(e) * page_k + uint64_t(r) * row_k);
                 vp_[i] = vbase + (uint64_t(e) * page_v + uint64_t(r) * row_v);
@@ -429,7 +442,7 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
         // once it has read V, and meets no barrier. Waves that share a ring fill NS - 1 stages ahead and refill the slot of
         // the stage before at the top of a stage, behind the one barrier.
         constexpr int AHEAD = RTW == 1 ? NS : NS - 1;
-        Two first_e[AHEAD];
+        Pages first_e[AHEAD];
 #pragma unroll
         for (int s = 0; s < AHEAD; ++s) first_e[s] = entries(s);
 
@@ -478,12 +491,12 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
                 issue_k(s);
                 issue_v(s);
             }
-        Two next_e = entries(AHEAD);  // of the stage issued next
+        Pages next_e = entries(AHEAD);  // of the stage issued next
         for (int s = 0; s < nst; ++s) {
             const uint32_t slot = ring_lds + (s & (NS - 1)) * 2 * STAGE;
             // (stages issued when stage s is read: AHEAD more, as far as there are any)
             const int behind = min(nst - s, AHEAD) - 1;
-            const uint32_t ok = (hist >> (2 * behind)) & 3u;
+            const uint32_t ok = (hist >> (QT * behind)) & ((1u << QT) - 1u);
             const bool more = s + AHEAD < nst;
             if constexpr (RTW == 1) {
                 if (s + AHEAD - 1 < nst) wait_vm<PER * (2 * NS - 1)>();
@@ -499,15 +512,15 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
                     next_e = entries(s + AHEAD + 1);
                 }
             }
-            const int v0 = (step0 + s) * TOK + part * STEP;
+            const int v0 = (step0 + s) * TOK + part * ST;
             if (RTW > 1 && v0 >= t_none) continue;  // (uniform in the wave: only its loads and the barriers are left)
-            f32x4 st[TPW][2];
-            auto scores = [&](const u32x4 (&k)[KK], int h) {
+            f32x4 st[SUB][TPW][2];
+            auto scores = [&](const u32x4 (&k)[KK], int x, int h) {
 #pragma unroll
                 for (int t = 0; t < TPW; ++t) {
-                    st[t][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    st[x][t][h] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int kk = 0; kk < KK; ++kk) st[t][h] = E::mfma(k[kk], qf[t][kk], st[t][h]);
+                    for (int kk = 0; kk < KK; ++kk) st[x][t][h] = E::mfma(k[kk], qf[t][kk], st[x][t][h]);
                 }
             };
             auto refill_k = [&]() {
@@ -519,47 +532,66 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
             if constexpr (D == 256) {  // (half by half: the operands of one half are 32 registers)
                 u32x4 kf[KK];
                 read_k<D>(kf, slot + k_lane);
-                scores(kf, 0);
+                scores(kf, 0, 0);
                 read_k<D>(kf, slot + k_lane + 16 * RB);
                 refill_k();
-                scores(kf, 1);
+                scores(kf, 0, 1);
             } else {
-                u32x4 kf[2][KK];
-                read_k2<D>(kf, slot + k_lane);
-                refill_k();
-                scores(kf[0], 0);
-                scores(kf[1], 1);
+                u32x4 kf[SUB][2][KK];
+#pragma unroll
+                for (int x = 0; x < SUB; ++x) {
+                    read_k2<D>(kf[x], slot + k_lane + x * STEP * RB);
+                    if (x == SUB - 1) refill_k();
+                    scores(kf[x][0], x, 0);
+                    scores(kf[x][1], x, 1);
+                }
             }
 
-            const bool whole = ok == 3u && v0 + STEP <= t_all;  // (uniform in the wave) every row admits all 32 tokens
-            // tile t's weights of the stage, as the B operand of O^T += V^T P^T
-            auto weights = [&](int t) -> u32x4 {
+            const bool whole = ok == (1u << QT) - 1u && v0 + ST <= t_all;  // (uniform in the wave) every row admits every token
+            // tile t's weights of the stage, as the B operands of O^T += V^T P^T
+            struct Weights {
+                u32x4 p[SUB];
+            };
+            auto weights = [&](int t) -> Weights {
+                Weights r;
                 if (!whole) {
-                    int p = sp.tree0 - v0;  // tokens of the prefix in the stage
-                    asm volatile("" : "+s"(p));  // (none of this ahead of the branch)
-                    uint32_t in;
-                    if (a.mask) {
-                        const uint64_t own_bits = p >= 32 ? 0 : (p >= 0 ? bits[t] << p : (-p < 64 ? bits[t] >> -p : 0));
-                        in = (p >= 32 ? ~0u : (p > 0 ? (1u << p) - 1u : 0u)) | uint32_t(own_bits);
-                    } else {
-                        const int nv = p + lim[t] + 1;
-                        in = nv >= 32 ? ~0u : (nv > 0 ? (1u << nv) - 1u : 0u);
+                    bool any = false;
+#pragma unroll
+                    for (int x = 0; x < SUB; ++x) {
+                        int p = sp.tree0 - v0 - STEP * x;  // tokens of the prefix in the piece
+                        asm volatile("" : "+s"(p));        // (none of this ahead of the branch)
+                        uint32_t in;
+                        if (a.mask) {
+                            const uint64_t own_bits = p >= 32 ? 0 : (p >= 0 ? bits[t] << p : (-p < 64 ? bits[t] >> -p : 0));
+                            in = (p >= 32 ? ~0u : (p > 0 ? (1u << p) - 1u : 0u)) | uint32_t(own_bits);
+                        } else {
+                            const int nv = p + lim[t] + 1;
+                            in = nv >= 32 ? ~0u : (nv > 0 ? (1u << nv) - 1u : 0u);
+                        }
+                        const uint32_t here = ok >> (2 * x);
+                        in &= ((here & 1u) ? 0x0000FFFFu : 0u) | ((here & 2u) ? 0xFFFF0000u : 0u);
+                        any = any || __builtin_amdgcn_ballot_w64(in != 0u) != 0;
+                        const uint32_t lb = in >> (4 * g);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (!((lb >> (16 * h + i)) & 1u)) st[x][t][h][i] = -INFINITY;
                     }
-                    in &= ((ok & 1u) ? 0x0000FFFFu : 0u) | ((ok & 2u) ? 0xFFFF0000u : 0u);
-                    if (__builtin_amdgcn_ballot_w64(in != 0u) == 0) return u32x4{0, 0, 0, 0};  // (uniform: nothing for this tile)
-                    const uint32_t lb = in >> (4 * g);
+                    if (!any) {  // (uniform: nothing for this tile)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (!((lb >> (16 * h + i)) & 1u)) st[t][h][i] = -INFINITY;
+                        for (int x = 0; x < SUB; ++x) r.p[x] = u32x4{0, 0, 0, 0};
+                        return r;
+                    }
                 }
-                u32x4 pf;
                 // Weights are taken against the row's reference, an earlier maximum, as long as no score passes it by more
                 // than SLACK: the sums are fp32 and a weight's rounding is relative, so nothing is lost, and the common
                 // stage has neither an exchange between lanes nor a rescale.
-                const float mx = max3(max3(st[t][0][0], st[t][0][1], st[t][0][2]), max3(st[t][0][3], st[t][1][0], st[t][1][1]),
-                                      max3(st[t][1][2], st[t][1][3], st[t][1][3]));
+                float mx = max3(max3(st[0][t][0][0], st[0][t][0][1], st[0][t][0][2]), max3(st[0][t][0][3], st[0][t][1][0], st[0][t][1][1]),
+                                max3(st[0][t][1][2], st[0][t][1][3], st[0][t][1][3]));
+                if constexpr (SUB == 2)
+                    mx = max3(max3(st[1][t][0][0], st[1][t][0][1], st[1][t][0][2]), max3(st[1][t][0][3], st[1][t][1][0], st[1][t][1][1]),
+                              max3(st[1][t][1][2], st[1][t][1][3], mx));
                 if (__builtin_amdgcn_ballot_w64(mx > m_lim[t]) != 0) {  // (uniform)
                     const float top = max_x32(max_x16(mx));
                     if (top > m_lim[t]) {  // (a row's four lanes alike)
@@ -574,15 +606,17 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
                 }
                 const float sub = m_z[t] - E::SHIFT;
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                for (int x = 0; x < SUB; ++x)
 #pragma unroll
-                    for (int i = 0; i < 4; i += 2) {
-                        const float p0 = __builtin_amdgcn_exp2f(fmaf(st[t][h][i], a.zs, -sub));
-                        const float p1 = __builtin_amdgcn_exp2f(fmaf(st[t][h][i + 1], a.zs, -sub));
-                        pf[2 * h + i / 2] = E::pair(p0, p1);
-                        l[t] = E::add_pair(pf[2 * h + i / 2], l[t]);  // (this lane's tokens; the row's four lanes meet at the end)
-                    }
-                return pf;
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < 4; i += 2) {
+                            const float p0 = __builtin_amdgcn_exp2f(fmaf(st[x][t][h][i], a.zs, -sub));
+                            const float p1 = __builtin_amdgcn_exp2f(fmaf(st[x][t][h][i + 1], a.zs, -sub));
+                            r.p[x][2 * h + i / 2] = E::pair(p0, p1);
+                            l[t] = E::add_pair(r.p[x][2 * h + i / 2], l[t]);  // (this lane's tokens; the row's four lanes meet at the end)
+                        }
+                return r;
             };
             constexpr int VT = D == 64 ? 4 : 8;  // dim tiles read at once
             u32x2 va[VT], vb[VT];
@@ -624,31 +658,34 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
                     next_e = entries(s + AHEAD + 1);
                 }
             };
-            if constexpr (D != 256 && TPW <= 2) {
+            if constexpr (D != 256 && TPW <= 2 && SUB == 1) {
                 // V's reads behind the scores' MFMAs, a tile's products behind the next tile's weights
                 wait_v();
                 read_v<D, 0>(va, vb, slot + STAGE + v_lane);
                 refill_v();
                 sift();
 #pragma unroll
-                for (int t = 0; t < TPW; ++t) weigh(t, 0, weights(t));
+                for (int t = 0; t < TPW; ++t) weigh(t, 0, weights(t).p[0]);
             } else {
                 // (V's operands only once the scores' registers are free; at head_dim 256 in halves)
-                u32x4 pf[TPW];
+                Weights pf[TPW];
 #pragma unroll
                 for (int t = 0; t < TPW; ++t) pf[t] = weights(t);
                 wait_v();
-                read_v<D, 0>(va, vb, slot + STAGE + v_lane);
-                if constexpr (D == 256) {
+#pragma unroll
+                for (int x = 0; x < SUB; ++x) {
+                    read_v<D, 0>(va, vb, slot + STAGE + v_lane + x * STEP * RB);
+                    if constexpr (D == 256) {
+                        sift();
+#pragma unroll
+                        for (int t = 0; t < TPW; ++t) weigh(t, 0, pf[t].p[x]);
+                        read_v<D, 1>(va, vb, slot + STAGE + v_lane);
+                    }
+                    if (x == SUB - 1) refill_v();
                     sift();
 #pragma unroll
-                    for (int t = 0; t < TPW; ++t) weigh(t, 0, pf[t]);
-                    read_v<D, 1>(va, vb, slot + STAGE + v_lane);
+                    for (int t = 0; t < TPW; ++t) weigh(t, D == 256 ? 8 : 0, pf[t].p[x]);
                 }
-                refill_v();
-                sift();
-#pragma unroll
-                for (int t = 0; t < TPW; ++t) weigh(t, D == 256 ? 8 : 0, pf[t]);
             }
         }
 
@@ -1112,9 +1149,9 @@ __global__ __launch_bounds__(NT) void block_select_kernel(PagedArgs a) {
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------
-template <class E, int D, int TPW, int RTW, int P, int WPC, bool SEL>
+template <class E, int D, int TPW, int RTW, int P, int WPC, bool SEL, int SUB = 1>
 int launch(PagedArgs& a, hipStream_t st) {
-    using Geo = Geometry<D, TPW, RTW, P, WPC>;
+    using Geo = Geometry<D, TPW, RTW, P, WPC, SUB>;
     constexpr int joined = (RTW * P * 16 * (D + 4) + 2 * RTW * P * 16) * 4;
     constexpr int lds = Geo::RING > joined ? Geo::RING : joined;
     // (once per device and kernel: the call costs about a microsecond)
@@ -1123,7 +1160,7 @@ int launch(PagedArgs& a, hipStream_t st) {
     MDX_HIP(hipGetDevice(&dev));
     const uint64_t bit = uint64_t(1) << (dev & 63);
     if (dev > 63 || !(allowed.load(std::memory_order_relaxed) & bit)) {
-        allow_smem(reinterpret_cast<const void*>(&paged_attn_kernel<E, D, TPW, RTW, P, WPC, SEL>), lds);
+        allow_smem(reinterpret_cast<const void*>(&paged_attn_kernel<E, D, TPW, RTW, P, WPC, SUB, SEL>), lds);
         allowed.fetch_or(bit, std::memory_order_relaxed);
     }
     // (units enough for every work-group there is room for: whole ones, without partials)
@@ -1131,7 +1168,7 @@ int launch(PagedArgs& a, hipStream_t st) {
     if (a.units > 1 && units >= CUS * WPC) a.whole = 1;
     const int grid = a.whole ? units : CUS * WPC;
     a.by_unit = units <= grid;  // (every unit is begun by one share, which writes its entry)
-    hipLaunchKernelGGL((paged_attn_kernel<E, D, TPW, RTW, P, WPC, SEL>), dim3(unsigned(grid)), dim3(Geo::NT), lds, st, a);
+    hipLaunchKernelGGL((paged_attn_kernel<E, D, TPW, RTW, P, WPC, SUB, SEL>), dim3(unsigned(grid)), dim3(Geo::NT), lds, st, a);
     MDX_LAUNCHED();
     if (a.whole) return MDX_OK;
     const int rows = (a.spb < a.S ? a.spb : a.S) * a.G;
@@ -1173,7 +1210,7 @@ int launch_rows(PagedArgs& a, hipStream_t st) {
         if constexpr (D == 256) return launch<E, D, 2, 2, 2, 1, SEL>(a, st);
         else return launch<E, D, 4, 1, 4, 1, SEL>(a, st);
     }
-    if constexpr (!SEL) return launch<E, D, 2, 4, 1, (D == 256 ? 1 : 2), SEL>(a, st);
+    if constexpr (!SEL) return launch<E, D, 2, 4, 1, (D == 256 ? 1 : 2), SEL, (D == 256 ? 1 : 2)>(a, st);
     set_error("at most 64 query heads per kv head");
     return MDX_EINVAL;
 }
