@@ -104,6 +104,7 @@ constexpr int CUS = 256;
 constexpr int RING_BYTES = 128 * 1024;  // of a CU's work-groups together
 constexpr int64_t FEW_STEPS = 2048;  // 128-token steps of a call at most, for the forms that go by latency
 constexpr int64_t WHOLE_TOKENS = 640;  // tokens a unit can have at most, for one work-group per unit
+constexpr int64_t EVEN_TOKENS = 4096;  // and where there are as many row blocks as work-groups
 
 __device__ __forceinline__ uint32_t lds_addr(const void* p) {
     return uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const unsigned char*)p));
@@ -242,6 +243,11 @@ struct Geometry {
     static constexpr int RING = RING_BYTES / WPC;
     static constexpr int NS = RING / (2 * STAGE * P);             // ring stages per part
     static constexpr int PER = STAGE / 1024 / RTW;                // direct loads per wave, stage and matrix
+    // What a unit costs beside its steps (its queries, the ring's first stage, the meeting of its parts), in steps: without
+    // it the share that takes the shortest units ends last. 16 prompts of 128 rows over 0 to 6000 tokens: 408 -> 166 us a
+    // call, 64 trees of 16 rows over at most 900: 104 -> 59, 32 of 8 rows over at most 8000: 130 -> 115; of 64 sequences'
+    // selections, one with 256 blocks and the others with 4: 199 -> 223; equal lengths: up to 8 % less.
+    static constexpr int FIXED = RPW == 16 ? 2 : RPW == 128 ? 6 : 4;
     static_assert(NS >= 1 && (NS & (NS - 1)) == 0 && PER >= 1 && (RTW == 1 ? SUB == 1 : NS >= 2) && (SUB == 1 || D != 256), "ring geometry");
 };
 
@@ -259,9 +265,20 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
     // read the same K and V, find them in one L2 (a prompt's 2048 rows: 164 us with the shares in turn).
     const int share = a.whole ? int(blockIdx.x) : int(blockIdx.x) % 8 * (CUS * WPC / 8) + int(blockIdx.x) / 8;
 
-    // ---- this work-group's share of the line of steps: [begin, end), and the sequence it begins in
     int begin, end, quota, b, in_b, kh = 0, u = 0;
     Span sp;
+    auto next_unit = [&]() {
+        if (++u == a.units) {
+            u = 0;
+            if (++kh == a.Hk) {
+                kh = 0;
+                ++b;
+                sp = span_of<SEL>(a, uload(a.length + b));
+            }
+        }
+    };
+
+    // ---- this work-group's share of the line of steps: [begin, end), and the sequence it begins in
     if (a.whole) {  // unit (b, kh, u) of the grid
         // kv heads in turn (neighbouring work-groups go to different XCDs), a chain's blocks with the most tokens first; every
         // second round of the CUs the other way, so that a CU's work-groups have about as much to do together.
@@ -284,7 +301,7 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
         auto walk = [&](auto f) {
             int bb = i0 / per_b, rest = i0 % per_b, uu = rest % a.units;
             for (int i = i0; i < i1; ++i) {
-                f(bb, rest, steps_of(a, span_of<SEL>(a, a.length[bb]), uu, TOK));
+                f(bb, rest, steps_of(a, span_of<SEL>(a, a.length[bb]), uu, TOK) + Geo::FIXED);
                 if (++uu == a.units) uu = 0;
                 if (++rest == per_b) {
                     rest = 0;
@@ -337,6 +354,13 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
         u = __builtin_amdgcn_readfirstlane(sh_at[2]);
         in_b = __builtin_amdgcn_readfirstlane(sh_at[3]);
         sp = span_of<SEL>(a, uload(a.length + b));
+        const int past = in_b - steps_of(a, sp, u, TOK);
+        if (past >= 0) {  // (behind the unit's last step: the next unit)
+            begin += Geo::FIXED - past;
+            if (begin >= end) return;
+            in_b = 0;
+            next_unit();
+        }
     }
     __syncthreads();  // (odd)
     int at = begin, step0 = in_b;  // line position, and the unit's step there
@@ -764,7 +788,7 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
         }
 
         // ---- the next unit
-        at += nst;
+        at += nst + (last ? Geo::FIXED : 0);
         if (at >= end) break;
         if (odd) {  // (uniform: every thread is past its last use)
             __syncthreads();
@@ -772,23 +796,16 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
             __syncthreads();
         }
         step0 = 0;
-        if (++u == a.units) {
-            u = 0;
-            if (++kh == a.Hk) {
-                kh = 0;
-                ++b;
-                sp = span_of<SEL>(a, uload(a.length + b));
-            }
-        }
+        next_unit();
     }
 }
 
-// The units that several shares worked on: a wave per query row, `per_wave` rows one after the other (many rows: fewer
-// work-groups, most of which find no open unit). D / 4 lanes take a partial's row in 16-byte pieces, 256 / D partials at
+// The units that several shares worked on: a wave per query row (four rows one after the other where there are many:
+// 37 us against 20 for 64 blocks of 128). D / 4 lanes take a partial's row in 16-byte pieces, 256 / D partials at
 // once; the maxima, sums and pieces of up to eight each go out together, so that few partials cost one memory round trip
 // behind the share's entry.
 template <class E, int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int rpw, int per_wave) {
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int rpw) {
     const int4 x = a.info[blockIdx.x];
     const int nseg = x.z, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
     if (nseg <= 1) return;
@@ -797,58 +814,56 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int rpw, i
     const int gi = lane / TPR, d = lane % TPR * 4;
     const int64_t rec = int64_t(rpw) * (D + 2);
     const float* base = a.part + int64_t(x.y) * 2 * rec;
-    for (int k = 0; k < per_wave; ++k) {
-        const int r = (int(blockIdx.y) * per_wave + k) * 4 + w, s = u * a.spb + r / a.G, h = kh * a.G + r % a.G;
-        if (r >= a.spb * a.G || s >= a.S) return;  // (uniform in the wave)
-        f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-        float M = -INFINITY, sum = 0.f;
-        for (int i0 = 0; i0 < nseg; i0 += U * NG) {
-            f32x4 v[U];
-            float mi[U], li[U];
+    const int r = int(blockIdx.y) * 4 + w, s = u * a.spb + r / a.G, h = kh * a.G + r % a.G;
+    if (r >= a.spb * a.G || s >= a.S) return;  // (uniform in the wave)
+    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+    float M = -INFINITY, sum = 0.f;
+    for (int i0 = 0; i0 < nseg; i0 += U * NG) {
+        f32x4 v[U];
+        float mi[U], li[U];
 #pragma unroll
-            for (int i = 0; i < U; ++i) {
-                const int sg = min(i0 + i * NG + gi, nseg - 1);  // (past the last: read again, not counted)
-                const float* p = base + (sg == 0 ? 1 : 2 * sg) * rec;
-                mi[i] = p[int64_t(rpw) * D + r];
-                li[i] = p[int64_t(rpw) * (D + 1) + r];
-                v[i] = *reinterpret_cast<const f32x4*>(p + int64_t(r) * D + d);
-            }
-            float top = M;
-#pragma unroll
-            for (int i = 0; i < U; ++i) {
-                if (i0 + i * NG + gi >= nseg) mi[i] = -INFINITY;
-                top = fmaxf(top, mi[i]);
-            }
-            const float was = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - top);
-            o *= was;
-            sum *= was;
-#pragma unroll
-            for (int i = 0; i < U; ++i) {
-                if (i0 + i * NG + gi >= nseg) continue;
-                // (a partial without an admitted token has sum 0 and O 0)
-                const float wi = mi[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi[i] - top);
-                sum += li[i] * wi;
-                o += v[i] * wi;
-            }
-            M = top;
+        for (int i = 0; i < U; ++i) {
+            const int sg = min(i0 + i * NG + gi, nseg - 1);  // (past the last: read again, not counted)
+            const float* p = base + (sg == 0 ? 1 : 2 * sg) * rec;
+            mi[i] = p[int64_t(rpw) * D + r];
+            li[i] = p[int64_t(rpw) * (D + 1) + r];
+            v[i] = *reinterpret_cast<const f32x4*>(p + int64_t(r) * D + d);
         }
         float top = M;
 #pragma unroll
-        for (int j = TPR; j < 64; j <<= 1) top = fmaxf(top, __shfl_xor(top, j, 64));
-        const float own = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - top);
-        o *= own;
-        sum *= own;
-#pragma unroll
-        for (int j = TPR; j < 64; j <<= 1) {
-            sum += __shfl_xor(sum, j, 64);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], j, 64);
+        for (int i = 0; i < U; ++i) {
+            if (i0 + i * NG + gi >= nseg) mi[i] = -INFINITY;
+            top = fmaxf(top, mi[i]);
         }
-        if (gi != 0) continue;
-        const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
-        *reinterpret_cast<uint2*>(a.out + ((int64_t(b) * a.S + s) * a.H + h) * D + d) =
-            sum == 0.f ? make_uint2(0u, 0u) : make_uint2(E::pair(o[0] * inv, o[1] * inv), E::pair(o[2] * inv, o[3] * inv));
+        const float was = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - top);
+        o *= was;
+        sum *= was;
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            if (i0 + i * NG + gi >= nseg) continue;
+            // (a partial without an admitted token has sum 0 and O 0)
+            const float wi = mi[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi[i] - top);
+            sum += li[i] * wi;
+            o += v[i] * wi;
+        }
+        M = top;
     }
+    float top = M;
+#pragma unroll
+    for (int j = TPR; j < 64; j <<= 1) top = fmaxf(top, __shfl_xor(top, j, 64));
+    const float own = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - top);
+    o *= own;
+    sum *= own;
+#pragma unroll
+    for (int j = TPR; j < 64; j <<= 1) {
+        sum += __shfl_xor(sum, j, 64);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], j, 64);
+    }
+    if (gi != 0) return;
+    const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+    *reinterpret_cast<uint2*>(a.out + ((int64_t(b) * a.S + s) * a.H + h) * D + d) =
+        sum == 0.f ? make_uint2(0u, 0u) : make_uint2(E::pair(o[0] * inv, o[1] * inv), E::pair(o[2] * inv, o[3] * inv));
 }
 
 // ---- the selection ----------------------------------------------------------------------------------------
@@ -1149,6 +1164,12 @@ __global__ __launch_bounds__(NT) void block_select_kernel(PagedArgs a) {
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------
+// The most tokens a unit can have: all that the table (or a selection) holds, and the rows' own.
+int64_t most_tokens(const PagedArgs& a, bool sel) {
+    const int64_t pages = sel && a.most < a.W ? a.most + 1 : a.W;
+    return (pages << a.lt) + a.S;
+}
+
 template <class E, int D, int TPW, int RTW, int P, int WPC, bool SEL, int SUB = 1>
 int launch(PagedArgs& a, hipStream_t st) {
     using Geo = Geometry<D, TPW, RTW, P, WPC, SUB>;
@@ -1163,30 +1184,26 @@ int launch(PagedArgs& a, hipStream_t st) {
         allow_smem(reinterpret_cast<const void*>(&paged_attn_kernel<E, D, TPW, RTW, P, WPC, SUB, SEL>), lds);
         allowed.fetch_or(bit, std::memory_order_relaxed);
     }
-    // (units enough for every work-group there is room for: whole ones, without partials)
+    // Row blocks enough for every work-group there is room for: whole ones, without partials, as long as no unit can be much
+    // longer than the others (2048 rows over 1000 tokens: 122 us in shares, 90 whole; 16 x 128 rows over 1000 each: 87 and 52;
+    // over 0 to 6000: 166 and 161; but with one sequence of 60000 among 15 of 500: 211 and 1437).
     const int units = a.B * a.Hk * a.units;
-    if (a.units > 1 && units >= CUS * WPC) a.whole = 1;
+    const int64_t most = most_tokens(a, SEL);
+    if (a.units > 1 && units >= CUS * WPC && (a.B == 1 || most <= EVEN_TOKENS || int64_t(units) * a.S >= most * CUS * WPC)) a.whole = 1;
     const int grid = a.whole ? units : CUS * WPC;
     a.by_unit = units <= grid;  // (every unit is begun by one share, which writes its entry)
     hipLaunchKernelGGL((paged_attn_kernel<E, D, TPW, RTW, P, WPC, SUB, SEL>), dim3(unsigned(grid)), dim3(Geo::NT), lds, st, a);
     MDX_LAUNCHED();
     if (a.whole) return MDX_OK;
     const int rows = (a.spb < a.S ? a.spb : a.S) * a.G;
-    const int per_wave = rows > 64 ? 4 : 1;
-    hipLaunchKernelGGL((paged_join_kernel<E, D>), dim3(unsigned(units < grid ? units : grid), unsigned((rows + 4 * per_wave - 1) / (4 * per_wave))), dim3(256), 0, st,
-                       a, Geo::RPW, per_wave);
+    hipLaunchKernelGGL((paged_join_kernel<E, D>), dim3(unsigned(units < grid ? units : grid), unsigned((rows + 3) / 4)), dim3(256), 0, st, a,
+                       Geo::RPW);
     MDX_LAUNCHED();
     return MDX_OK;
 }
 
 // Query rows of a work-group: what covers the rows of a kv head with as few row blocks as registers allow.
 int rpw_of(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
-
-// The most tokens a unit can have: all that the table (or a selection) holds, and the rows' own.
-int64_t most_tokens(const PagedArgs& a, bool sel) {
-    const int64_t pages = sel && a.most < a.W ? a.most + 1 : a.W;
-    return (pages << a.lt) + a.S;
-}
 
 // Row tiles in one wave's registers (each K and V operand read from LDS once for all) where there is much to stream, in
 // waves of their own where a unit's few steps count by their latency.
@@ -1312,7 +1329,7 @@ extern "C" int mdx_attn_paged(const void* q, int64_t q_seq_stride, int64_t q_row
     if (rc != MDX_OK) return rc;
     MDX_CHECK(H / Hk <= 128, "at most 128 query heads per kv head");
     const int64_t rows = S * (H / Hk), blocks = blocks_of(S, H / Hk);
-    MDX_CHECK(rows < (int64_t(1) << 30) && B * Hk * blocks < (int64_t(1) << 30) && B * Hk * blocks * ((W * T + S) / STEP + 1) < (int64_t(1) << 31),
+    MDX_CHECK(rows < (int64_t(1) << 30) && B * Hk * blocks < (int64_t(1) << 30) && B * Hk * blocks * ((W * T + S) / STEP + 8) < (int64_t(1) << 31),
               "too many rows times tokens for one call");
     a.whole = whole_units(B, S, H, Hk, T, W);
     MDX_CHECK(a.whole || (workspace && aligned(workspace, 16) && workspace_bytes >= base_bytes(rows, D)),
@@ -1351,7 +1368,7 @@ extern "C" int mdx_attn_blocks(const void* q, int64_t q_seq_stride, int64_t q_ro
     const int64_t most = blocks + sink + local, units = B * S * Hk;
     MDX_CHECK(H / Hk <= 64, "at most 64 query heads per kv head");
     MDX_CHECK(W <= 65536, "at most 65536 pages a sequence");
-    MDX_CHECK(B * Hk <= 65535 && units < (int64_t(1) << 24) && units * (((most < W ? most : W) + 1) * T + S) / STEP + units < (int64_t(1) << 31),
+    MDX_CHECK(B * Hk <= 65535 && units < (int64_t(1) << 24) && units * (((most < W ? most : W) + 1) * T + S) / STEP + 8 * units < (int64_t(1) << 31),
               "too many rows times tokens for one call");
     const size_t need = mdx_attn_blocks_workspace(B, S, H, Hk, D, W, most);
     MDX_CHECK(workspace && aligned(workspace, 16) && workspace_bytes >= need, "workspace: %zu bytes, 16-byte aligned", need);

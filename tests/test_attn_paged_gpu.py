@@ -66,6 +66,15 @@ def test_many_sequences(C, dev):
     _run(C, dev, BF, 4, 2, 64, 16, lens, 1, False, 9)
 
 
+@pytest.mark.parametrize("H,Hk,D,S,B,top,tree", [(4, 2, 64, 1, 300, 90, False), (8, 8, 128, 1, 130, 200, False), (8, 2, 128, 16, 150, 90, True),
+                                                 (8, 4, 256, 9, 150, 60, True), (8, 2, 128, 70, 24, 300, False), (16, 8, 64, 100, 40, 70, False)])
+def test_more_units_than_work_groups(C, dev, H, Hk, D, S, B, top, tree):
+    """Shares of several units, that begin and end in, between and behind the steps of a unit; tables that could hold much more."""
+    g = torch.Generator().manual_seed(B)
+    lens = [int(x) for x in torch.randint(0, top, (B,), generator=g)]
+    _run(C, dev, BF, H, Hk, D, 32, lens, S, tree, 13, 200)
+
+
 def _small(dev, dt=BF, D=128, H=8, Hk=2, T=16, lens=(40, 0, 33), S=4, seed=11):
     g = torch.Generator().manual_seed(seed)
     lens = list(lens)
