@@ -6,18 +6,25 @@
 // is admitted. A token in a page that the table does not have is not admitted; what a place holds that a row does not
 // admit never reaches it, infinities and NaN included.
 //
-// Work. A unit is (sequence, kv head, block of query rows); its tokens go in steps of 32 per token part. The steps of
-// all units stand in one line and every work-group takes an equal share of it (one work-group per CU: the ring takes most
-// of its LDS), so unequal lengths, one long sequence and many short ones keep all CUs busy alike, and the lengths are
-// read on the device alone. A share that begins or ends inside a unit leaves a partial (maximum, sum, O in fp32), which
-// the second launch joins; a unit inside one share is written at once.
+// Work. A unit is (sequence, kv head, block of query rows); its tokens go in steps of 32 or 64 per token part. The steps of
+// all units stand in one line and every work-group takes an equal share of it (one or two work-groups per CU: their rings
+// take most of its LDS), so unequal lengths, one long sequence and many short ones keep all CUs busy alike, and the lengths
+// are read on the device alone. A share that begins or ends inside a unit leaves a partial (maximum, sum, O in fp32), which
+// the second launch joins; a unit inside one share is written at once. Where units are short, or enough of them about equally
+// long, a work-group takes a whole one and there is no second launch.
 //
 // A step of a wave: its 32 tokens' K and V come to LDS by direct loads (1 KiB per wave instruction); S^T = K Q^T with
 // A = 16 tokens x 32 dims and B = Q^T in registers (v_mfma_f32_16x16x32), so that the four lanes of a query row hold its
-// scores; softmax with a running maximum; O^T += V^T P^T with A = V^T by transposing LDS reads in the token order the
+// scores; softmax against an earlier maximum, renewed when a score passes it by a slack; O^T += V^T P^T with A = V^T by transposing LDS reads in the token order the
 // S^T accumulators hold, B = P^T from registers. A wave holds up to four tiles of 16 query rows and reads each K and V
 // operand once for all of them. Sums, maxima and O in fp32; P is rounded to the cache's type for the product (half a
 // step of each weight; the normaliser sums the rounded weights, so that equal values come out unchanged).
+//
+// What bounds it. Few rows: the cache's bytes, where there are many (64 single tokens over 262 thousand: 193 us, 5.6 TB/s),
+// else the latency of one work-group's chain of queries, pages, first stage, products, meeting and join (one token of a
+// short sequence: 6 us in a whole unit). Many rows: the matrix units' and the softmax's instructions in turn, with two waves per
+// SIMD to overlap them (2048 rows over 30000 tokens: 1027 us, 1.0 PFLOP/s of the 1.2 that a large matrix product reaches;
+// 64 tokens a stage instead of 32: 128 -> 99 us for 2048 rows over 1000).
 //
 // Reference: none for the pages; the rows' contract is csrc/attn_dpas.sycl:269-342's.
 #include <math.h>
@@ -102,8 +109,13 @@ constexpr int MAX_SEQS = 1024;
 constexpr int STEP = 32;
 constexpr int CUS = 256;
 constexpr int RING_BYTES = 128 * 1024;  // of a CU's work-groups together
-constexpr int64_t FEW_STEPS = 2048;  // 128-token steps of a call at most, for the forms that go by latency
-constexpr int64_t WHOLE_TOKENS = 640;  // tokens a unit can have at most, for one work-group per unit
+// 128-token steps of a call at most, for the forms that go by latency (below: launch_rows)
+constexpr int64_t FEW_STEPS = 2048;
+// Tokens a unit can have at most, for one work-group per unit: 8 units of one token over 500: 9.4 us a call, 12.6 in shares
+// with their join; of 16 rows over 500: 15.5 and 13.9, 128 of them 16.5 and 25.3. Twice as many where the units fill half of
+// the CUs and no more than all (128 units of one token over 1000: 15.7 and 20.2, of 16 rows 23.0 and 29.3; 8 units of one
+// token over 1000: 13.2 and 11.7).
+constexpr int64_t WHOLE_TOKENS = 640;
 constexpr int64_t EVEN_TOKENS = 4096;  // and where there are as many row blocks as work-groups
 
 __device__ __forceinline__ uint32_t lds_addr(const void* p) {
@@ -111,8 +123,8 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
 }
 
 // LDS layout of a 32-token stage, K and V alike: the tokens' rows of 2 D bytes one after the other, as they stand in a page,
-// so that a direct load's KiB is one KiB of the page (64-byte pieces of 16 tokens per load: 5 % slower, 200 us against
-// PIECES for 64 single-token sequences of 262 thousand tokens in all). Within a row the 16-byte pieces are exchanged by
+// so that a direct load's KiB is one KiB of the page (64-byte pieces of 16 tokens per load took 2 % longer, 200 us against 196
+// for 64 single-token sequences of 262 thousand tokens in all). Within a row the 16-byte pieces are exchanged by
 // an exclusive or with the token (swizzle), which the loads' source addresses follow, so that
 //   K: lane (token c16 of the half, k-group g) reads piece 4 kk + g, 16 tokens of one piece meeting all banks once;
 //   V: the transposing reads (lane s of group g points at token 4 g + s / 4 of the half, dims 16 dt + 4 (s % 4) .. + 3, and
@@ -262,7 +274,8 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
     const int g = lane >> 4, c16 = lane & 15;
     const int rw = w % RTW, part = w / RTW;
     // Work-groups go to the 8 XCDs in turn: each XCD takes neighbouring shares, so that the row blocks of a kv head, which
-    // read the same K and V, find them in one L2 (a prompt's 2048 rows: 164 us with the shares in turn).
+    // read the same K and V, find them in one L2 (a prompt's 2048 rows in shares: 144 us, and 164 with the shares in turn; both
+    // before the steps of 64 tokens).
     const int share = a.whole ? int(blockIdx.x) : int(blockIdx.x) % 8 * (CUS * WPC / 8) + int(blockIdx.x) / 8;
 
     int begin, end, quota, b, in_b, kh = 0, u = 0;
@@ -874,7 +887,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int rpw) {
 // c16) in element r): a wave takes 16 pages, so the longest context spreads over all CUs. (One thread per page on the vector
 // units: 94.8 us for 8 rows over 250 pages of head_dim 256, 21 us for 1 row over 2046 of 128.)
 constexpr int SCORE_ROWS = 16;
-constexpr int FEW_ROWS = 4;  // rows up to which the vector units take them: an MFMA of one row takes as long as of 16
+// Rows up to which the vector units take them, an MFMA of one row taking as long as of 16 (a call with one row over 60000
+// pages: 115 us, 124 by MFMA; 16 x 1 over 500: 43.6 and 46.9; 4 rows over 2046: 31.0 and 30.4; 8: 37.4 and 34.9).
+constexpr int FEW_ROWS = 2;
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 typedef double f64x2 __attribute__((ext_vector_type(2)));
 template <class E, int D>
@@ -1205,27 +1220,27 @@ int launch(PagedArgs& a, hipStream_t st) {
 // Query rows of a work-group: what covers the rows of a kv head with as few row blocks as registers allow.
 int rpw_of(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
-// Row tiles in one wave's registers (each K and V operand read from LDS once for all) where there is much to stream, in
-// waves of their own where a unit's few steps count by their latency.
+// The form by the rows of a unit. A unit's row tiles lie in waves of their own, which read each K and V operand from LDS again
+// but have fewer instructions one after the other (32 and 64 rows in one wave's registers: 20 against 15 us for 16 rows over
+// 1000 tokens of 8 kv heads, 120 against 106 for 16 sequences over 8000); only at head_dim 64 LDS is what bounds 64 rows where
+// there is much to stream (32 sequences of 16 rows over 8000: 106 us in one wave's registers, 117 in waves of their own).
 template <class E, int D, bool SEL>
 int launch_rows(PagedArgs& a, hipStream_t st) {
     const int rows = SEL ? a.G : a.units > 1 ? 128 : a.S * a.G;
     const int64_t steps = int64_t(a.B) * a.Hk * a.units * ((most_tokens(a, SEL) + 127) / 128);
     const bool few = steps <= FEW_STEPS;
-    // (two work-groups per CU: one streams while the other changes units. 64 single tokens over 262 thousand: 198 -> 193 us;
-    // 32 selections of 1000 tokens: 6 -> 8 us a launch; at head_dim 256 a stage of 32 KiB leaves no ring for it)
+    // Two work-groups per CU where there is much to stream: one goes on while the other changes units (16 x 8 rows' selections
+    // of 16 blocks: 121 -> 109 us, 200 single tokens over 10 to 500: 50 -> 46, 64 over at most 8192 at head_dim 64: 98 -> 93, at
+    // 128: 195 -> 198; one token over 2000: 11.7 -> 12.1; at head_dim 256 a stage of 32 KiB leaves no ring for it).
     if (rows <= 16) {
         if (few || D == 256) return launch<E, D, 1, 1, 4, 1, SEL>(a, st);
         if constexpr (D != 256) return launch<E, D, 1, 1, 4, 2, SEL>(a, st);
     }
-    if (rows <= 32) {
-        if (few) return launch<E, D, 1, 2, (D == 256 ? 2 : 4), 1, SEL>(a, st);
-        return launch<E, D, 2, 1, 4, 1, SEL>(a, st);
-    }
+    if (rows <= 32) return launch<E, D, 1, 2, (D == 256 ? 2 : 4), 1, SEL>(a, st);
     if (rows <= 64) {
-        if (few) return launch<E, D, 1, 4, (D == 256 ? 1 : 2), 1, SEL>(a, st);
-        if constexpr (D == 256) return launch<E, D, 2, 2, 2, 1, SEL>(a, st);
-        else return launch<E, D, 4, 1, 4, 1, SEL>(a, st);
+        if constexpr (D == 64)
+            if (!few) return launch<E, D, 4, 1, 4, 1, SEL>(a, st);
+        return launch<E, D, 1, 4, (D == 256 ? 1 : 2), 1, SEL>(a, st);
     }
     if constexpr (!SEL) return launch<E, D, 2, 4, 1, (D == 256 ? 1 : 2), SEL, (D == 256 ? 1 : 2)>(a, st);
     set_error("at most 64 query heads per kv head");
@@ -1280,6 +1295,12 @@ int fill(PagedArgs& a, const void* q, int64_t q_seq_stride, int64_t q_row_stride
                   k_row_stride % 8 == 0 && v_head_stride % 8 == 0 && v_page_stride % 8 == 0 && v_row_stride % 8 == 0,
               "16-byte aligned rows");
     MDX_CHECK(scale > 0.f && scale < INFINITY, "a positive, finite scale");
+    MDX_CHECK(q_seq_stride >= 0 && q_row_stride >= 0 && q_head_stride >= 0 && q_seq_stride < lim && q_row_stride < lim && q_head_stride < lim,
+              "query strides");
+    // (a row is written while work-groups that have a part of it may still have its query to read)
+    const uintptr_t q0 = reinterpret_cast<uintptr_t>(q), o0 = reinterpret_cast<uintptr_t>(out);
+    const uint64_t q_bytes = uint64_t((B - 1) * q_seq_stride + (S - 1) * q_row_stride + (H - 1) * q_head_stride + D) * 2;
+    MDX_CHECK(o0 + uint64_t(B * S * H * D) * 2 <= q0 || q0 + q_bytes <= o0, "out: apart from q");
     a.q = static_cast<const uint16_t*>(q);
     a.qb = q_seq_stride, a.qs = q_row_stride, a.qh = q_head_stride;
     a.key = static_cast<const uint16_t*>(key);
@@ -1307,7 +1328,8 @@ static int64_t blocks_of(int64_t S, int64_t G) { return G > 128 ? 0 : (S + rows_
 
 // One work-group per unit, without a join: where a unit has few steps at most.
 static bool whole_units(int64_t B, int64_t S, int64_t H, int64_t Hk, int64_t T, int64_t W) {
-    return W * T + S <= WHOLE_TOKENS && B * Hk * blocks_of(S, H / Hk) <= 65536;
+    const int64_t units = B * Hk * blocks_of(S, H / Hk);
+    return W * T + S <= (2 * units >= CUS && units <= CUS ? 2 : 1) * WHOLE_TOKENS && units <= 65536;
 }
 
 extern "C" size_t mdx_attn_paged_workspace(int64_t B, int64_t S, int64_t H, int64_t Hk, int64_t D, int64_t T, int64_t W) {
@@ -1396,7 +1418,8 @@ extern "C" int mdx_attn_blocks(const void* q, int64_t q_seq_stride, int64_t q_ro
         }
         MDX_LAUNCHED();
     }
-    // (keys in registers: the smallest form that holds a row's)
+    // (keys in registers: the smallest form that holds a row's. A call at 1000 pages: 21.6 us, 23.6 with the third form, 42.4 with
+    // the fourth; at 4000: 24.3, 26.1, 46.4; at 16000: 34.6 and 62.5)
     if (W <= 1024) hipLaunchKernelGGL((block_select_kernel<256, 4>), dim3(unsigned(units)), dim3(256), 0, st, a);
     else if (W <= 4096) hipLaunchKernelGGL((block_select_kernel<512, 8>), dim3(unsigned(units)), dim3(512), 0, st, a);
     else if (W <= 16384) hipLaunchKernelGGL((block_select_kernel<1024, 16>), dim3(unsigned(units)), dim3(1024), 0, st, a);

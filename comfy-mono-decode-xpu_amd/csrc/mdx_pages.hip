@@ -149,8 +149,9 @@ __device__ void fork_rows(const ForkArgs& a, int i, int t, int nt) {
 }
 __global__ __launch_bounds__(256) void fork_rows_kernel(ForkArgs a) { fork_rows(a, blockIdx.x, threadIdx.x, 256); }
 
-// Plan: one thread per pair; with `rows` (few pairs and entries) the new rows in the same launch, a wave per pair. Pages of old rows are released by the last launch, so pages given out here are never ones
-// that a copy still reads.
+// Plan: one thread per pair; with `rows` (few pairs and entries) the new rows in the same launch, a wave per pair. Pages of old
+// rows are released by the last launch, so pages given out here are never ones that a copy still reads.
+// Bound by latency (references, sums, list, rows: dependent round trips of one work-group): 6 to 7 us for 8 pairs of 32 pages.
 __global__ __launch_bounds__(PLAN_T) void fork_plan_kernel(ForkArgs a, int rows) {
     __shared__ int tmp[PLAN_T / 64];
     __shared__ int sdst[MAX_SEQS];
@@ -195,8 +196,8 @@ __global__ __launch_bounds__(PLAN_T) void fork_plan_kernel(ForkArgs a, int rows)
 
 // The copies (work-groups past the pairs', in pieces of 16 KiB) and, by the first `pairs` work-groups, what the call
 // changes in the tables: the old rows' references given back, the new rows, lengths and slots.
-// Bound by the bytes: 16 bytes per lane and load, four loads in flight per wave. 66 pages of 4 MiB: see the table of
-// measurements.
+// Bound by the bytes: 16 bytes per lane and load, four loads in flight per wave. 66 pages of 4 MiB: 130 us a call, 4.3 TB/s
+// read and written together (4.8 in one large copy).
 constexpr int PIECE = 256 * 16 * 4;
 __device__ __forceinline__ void copy_piece(const unsigned char* from, unsigned char* to, int64_t bytes) {
     u32x4 v[4];
@@ -553,6 +554,7 @@ extern "C" int mdx_page_fork(void* kv, void* ksum, int64_t L, int64_t Hk, int64_
     MDX_CHECK(B >= 1 && B <= (int64_t(1) << 24) && W >= 1 && (W << lt) < (int64_t(1) << 30) && table_stride >= W && table_stride <= (int64_t(1) << 26),
               "table [sequences, W], under 2^30 tokens a sequence");
     MDX_CHECK(pairs >= 1 && pairs <= MAX_SEQS && room >= 0 && room < (int64_t(1) << 30), "1..1024 pairs, room");
+    MDX_CHECK(pairs * W < (int64_t(1) << 30), "too many pairs times table entries");
     MDX_CHECK(aligned(kv, 16) && aligned(ksum, 16), "16-byte aligned cache");
     MDX_CHECK(workspace && aligned(workspace, 16) && workspace_bytes >= mdx_page_fork_workspace(pairs, W),
               "workspace: %zu bytes, 16-byte aligned", mdx_page_fork_workspace(pairs, W));
@@ -578,7 +580,9 @@ extern "C" int mdx_page_fork(void* kv, void* ksum, int64_t L, int64_t Hk, int64_
     a.rows = a.fresh + pairs * W;
     a.copies = reinterpret_cast<int2*>(a.head + (fork_ints(pairs, W) + 3) / 4 * 4);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const bool few = pairs * W <= 4096;  // (at most four rounds of the planning work-group's waves)
+    // (the planning work-group builds the rows too: 512 entries 9.8 us a call, 12.3 with a launch for them; 4096: 14.0 and 12.8;
+    // 8192: 20.2 and 14.6)
+    const bool few = pairs * W <= 2048;
     hipLaunchKernelGGL(fork_plan_kernel, dim3(1), dim3(PLAN_T), 0, st, a, few ? 1 : 0);
     MDX_LAUNCHED();
     if (!few) {
@@ -608,6 +612,8 @@ extern "C" int mdx_page_commit(void* kv, void* ksum, int32_t dtype, int64_t L, i
     MDX_CHECK(L >= 1 && Hk >= 1 && P >= 1 && L * Hk <= 65536 && P <= (int64_t(1) << 30), "layers, heads, pages");
     MDX_CHECK(B >= 1 && B <= MAX_SEQS && W >= 1 && (W << lt) < (int64_t(1) << 30) && table_stride >= W && table_stride <= (int64_t(1) << 26),
               "table [1..1024 sequences, W], under 2^30 tokens a sequence");
+    MDX_CHECK(B * W < (int64_t(1) << 30), "too many sequences times table entries");
+    MDX_CHECK(new_length == length || new_length + B <= length || length + B <= new_length, "new_length: length itself, or apart from it");
     MDX_CHECK(!path || (R >= 1 && R <= MAX_PATH), "a path has 1..64 rows");
     MDX_CHECK(room >= 0 && room <= 65536 && B * room < (int64_t(1) << 30), "room 0..65536");
     MDX_CHECK(aligned(kv, 16) && aligned(ksum, 16), "16-byte aligned cache");

@@ -1312,15 +1312,15 @@ def page_fork(kv, ksum, table, length, refs, dst, src, room=0, share=True, slots
 
 
 def page_commit(kv, ksum, table, length, refs, count, path=None, room=0, new_length=None, slots=None):
-    """The step's rows of every sequence become committed: row length[b] + path[b, k] of the cache moves to length[b] + k for
-    k < count[b] (all layers, keys and values; path int32 [B, R] ascending from 0 <= path, R <= 64; None: the rows stand
-    in order already), the length grows by count[b] (into new_length, default: in place), the mean keys of the pages that
-    fill up are taken (ksum not None), and missing pages for `room` more tokens are given (the lowest free ones, in the
-    sequences' order). slots (int64 [B, room], optional): the cache rows page * T + row of the next tokens (the positions
-    that qk_norm_rope_kv writes in a [1, Hk, P * T, D] view of a layer), -1 where there is no page.
-    count[b] < 0: the sequence is left alone (status 1). Returns int32 [B]: 1 done, 0 committed but not all of the room
-    given, -1 refused (a path out of order or range, rows without pages, a length past the table): nothing of that sequence
-    moves or grows. The move of mtp_accept (csrc/mtp_loop.sycl:160-196 of the reference) over pages, for a batch."""
+    """The step's rows of every sequence become committed: row length[b] + path[b, k] of the cache moves to length[b] + k for k
+    < count[b] (all layers, keys and values; path int32 [B, R] ascending from 0 <= path, R <= 64; None: the rows stand in
+    order already), the length grows by count[b] (into new_length, apart from length; default: in place), the mean keys of
+    the pages that fill up are taken (ksum not None), and missing pages for `room` more tokens are given (the lowest free
+    ones, in the sequences' order). slots (int64 [B, room], optional): the cache rows page * T + row of the next tokens (the
+    positions that qk_norm_rope_kv writes in a [1, Hk, P * T, D] view of a layer), -1 where there is no page. count[b] < 0:
+    the sequence is left alone (status 1). Returns int32 [B]: 1 done, 0 committed but not all of the room given, -1 refused
+    (a path out of order or range, rows without pages, a length past the table): nothing of that sequence moves or grows.
+    The move of mtp_accept (csrc/mtp_loop.sycl:160-196 of the reference) over pages, for a batch."""
     return (_bind or _bound()).page_commit(kv, ksum, table, length, refs, count, path, room, new_length, slots)
 
 
@@ -1329,9 +1329,9 @@ def attn_paged(q, key, value, table, length, mask=None, scale=None, out=None):
     those of the rows' own tokens length[b] + j (j < S, their K / V in the pages already) whose bit j its mask has (int64
     [B, S], S <= 64: a tree's ancestors), or j <= s without masks (a chain: decode and prompt rows). q [B, S, H, D] (any
     strides of 8 elements), key / value [Hk, P, T, D] views of the cache (kv[layer, 0], kv[layer, 1]; any strides of 8
-    elements), table, length as page_commit keeps them. out [B, S, H, D]; a row that admits nothing is 0. Tokens in pages that
-    the table does not have are not attended; what stands in places a row does not attend is never seen.
-    The form of attn_dpas (csrc/attn_dpas.sycl:269-342 of the reference) for a batch, pages, and any rows."""
+    elements), table, length as page_commit keeps them. out [B, S, H, D], apart from q; a row that admits nothing is 0.
+    Tokens in pages that the table does not have are not attended; what stands in places a row does not attend is never
+    seen. The form of attn_dpas (csrc/attn_dpas.sycl:269-342 of the reference) for a batch, pages, and any rows."""
     return (_bind or _bound()).attn_paged(q, key, value, table, length, mask, scale, out)
 
 

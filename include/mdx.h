@@ -604,13 +604,14 @@ int mdx_page_fork(void* kv, void* ksum, int64_t L, int64_t Hk, int64_t P, int64_
                   const int32_t* src, int64_t pairs, int64_t room, int32_t share, int64_t* slots, int32_t* status,
                   void* workspace, size_t workspace_bytes, void* stream);
 
-/* Per sequence b (B <= 1024): the rows at length[b] + path[b][k] move to length[b] + k for k < count[b] (path int32 [B][R],
- * strictly ascending in 0..R - 1, R <= 64; NULL: nothing moves), new_length[b] = length[b] + count[b] (may be length), the
- * mean keys of the pages that fill are written (ksum, fp32 sums), missing pages up to `room` more tokens are given (lowest
- * free first, in sequence order), slots int64 [B][room] (may be NULL) as above. count[b] < 0: left alone. status int32 [B]:
- * 1 done; 0 committed, room not all given; -1 refused (bad path, rows without pages, past the table): that sequence stays
- * (the mean keys of its pages past its length may have been written). Replaces, over pages and for a batch, the KV move of
- * _C.mtp_accept (csrc/mtp_loop.sycl:160-196). dtype MDX_DT_BF16 or MDX_DT_F16; D in {64, 128, 256}. */
+/* Per sequence b (B <= 1024): the rows at length[b] + path[b][k] move to length[b] + k for k < count[b] (path int32
+ * [B][R], strictly ascending in 0..R - 1, R <= 64; NULL: nothing moves), new_length[b] = length[b] + count[b] (length
+ * itself or apart from it), the mean keys of the pages that fill are written (ksum, fp32 sums), missing pages up to
+ * `room` more tokens are given (lowest free first, in sequence order), slots int64 [B][room] (may be NULL) as above.
+ * count[b] < 0: left alone. status int32 [B]: 1 done; 0 committed, room not all given; -1 refused (bad path, rows
+ * without pages, past the table): that sequence stays (the mean keys of its pages past its length may have been
+ * written). Replaces, over pages and for a batch, the KV move of _C.mtp_accept (csrc/mtp_loop.sycl:160-196). dtype
+ * MDX_DT_BF16 or MDX_DT_F16; D in {64, 128, 256}. */
 size_t mdx_page_commit_workspace(int64_t B, int64_t W);
 int mdx_page_commit(void* kv, void* ksum, int32_t dtype, int64_t L, int64_t Hk, int64_t P, int64_t T, int64_t D,
                     int32_t* table, int64_t table_stride, int64_t B, int64_t W, const int32_t* length, int32_t* new_length,
@@ -620,10 +621,10 @@ int mdx_page_commit(void* kv, void* ksum, int32_t dtype, int64_t L, int64_t Hk, 
 /* Attention over pages. Row (b, s, h) of q [B, S, H, D]: softmax(scale q . k) v over the committed tokens t < length[b] and
  * the rows' own tokens length[b] + j, j < S, of bit j of mask[b][s] (int64 [B][S], S <= 64) or, with mask NULL, of j <= s
  * (S <= 65535); 0 if there are none. Own tokens are read from the pages too. key / value [Hk, P, T, D] (strides in elements;
- * head, page, row; multiples of 8). out [B, S, H, D] contiguous. fp32 sums, P rounded to the element type. A token in no
- * page is not attended; the contents of places that a row does not attend (non-finite ones too) do not reach it.
- * dtype MDX_DT_BF16 or MDX_DT_F16; D in {64, 128, 256}; B <= 1024, H / Hk <= 128; a workspace of 0 bytes may be NULL. The contract of mdx_attn_decode (csrc/attn_dpas.sycl:269-342)
- * for a batch over pages. */
+ * head, page, row; multiples of 8). out [B, S, H, D] contiguous, apart from q. fp32 sums, P rounded to the element type. A
+ * token in no page is not attended; the contents of places that a row does not attend (non-finite ones too) do not reach
+ * it. dtype MDX_DT_BF16 or MDX_DT_F16; D in {64, 128, 256}; B <= 1024, H / Hk <= 128; a workspace of 0 bytes may be NULL.
+ * The contract of mdx_attn_decode (csrc/attn_dpas.sycl:269-342) for a batch over pages. */
 size_t mdx_attn_paged_workspace(int64_t B, int64_t S, int64_t H, int64_t Hk, int64_t D, int64_t T, int64_t W);
 int mdx_attn_paged(const void* q, int64_t q_seq_stride, int64_t q_row_stride, int64_t q_head_stride, const void* key,
                    int64_t k_head_stride, int64_t k_page_stride, int64_t k_row_stride, const void* value,

@@ -236,3 +236,17 @@ def test_refusals(C, dev):
                             ((q.transpose(2, 3), key, value, table, n), {}, "contiguous")]:
         with pytest.raises(RuntimeError, match=match):
             C.attn_paged(*args, **kw)
+    with pytest.raises(RuntimeError, match="apart from q"):
+        C.attn_paged(q, key, value, table, n, out=q)
+    two = torch.empty(2 * q.numel(), dtype=q.dtype, device=dev)
+    with pytest.raises(RuntimeError, match="apart from q"):
+        C.attn_paged(two[:q.numel()].view_as(q), key, value, table, n, out=two[q.numel() - 8:-8].view_as(q))
+    assert C.attn_paged(two[:q.numel()].view_as(q).copy_(q), key, value, table, n, out=two[q.numel():].view_as(q)).isfinite().all()
+
+
+def test_queries_of_all_sequences_are_one(C, dev):
+    """A broadcast query (strides of 0)."""
+    _, q, key, value, table, lens, n, _ = _small(dev, lens=(90, 3, 700))
+    q = q[:1, :, :1].expand(3, 4, 8, 128)
+    got = C.attn_paged(q[:1, :, :1].to(dev).expand(3, 4, 8, 128), key.to(dev), value.to(dev), table.to(dev), n)
+    check(got, BF, q, key, value, table, lens, None, 128 ** -0.5)

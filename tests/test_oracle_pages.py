@@ -90,20 +90,20 @@ def test_refusals_before_any_device_work():
     from mdx import _lib
     A = 1 << 12  # an aligned address that nothing reads
 
-    def attn(q=A, key=A, value=A, dt=_lib.DT_BF16, table=A, length=A, mask=None, out=A, B=1, S=1, H=4, Hk=2, D=128, P=8, T=16, W=400,
+    def attn(q=A, key=A, value=A, dt=_lib.DT_BF16, table=A, length=A, mask=None, out=1 << 44, B=1, S=1, H=4, Hk=2, D=128, P=8, T=16, W=400,
              scale=0.1, ws=A, nb=1 << 40, kt=128, kp=2048, qs=512, ts=400):
         return _lib.lib().mdx_attn_paged(q, 512, qs, 128, key, kp * 8, kp, kt, value, kp * 8, kp, kt, dt, table, ts, length, mask,
                                          out, B, S, H, Hk, D, P, T, W, scale, ws, nb, None)
 
-    def blocks(blocks=4, sink=1, local=1, ksum=A, sel=A, S=1, H=4, sp=128, nb=1 << 40):
+    def blocks(blocks=4, sink=1, local=1, ksum=A, sel=A, out=1 << 44, S=1, H=4, sp=128, nb=1 << 40):
         return _lib.lib().mdx_attn_blocks(A, 512, 512, 128, A, 16384, 2048, 128, A, 16384, 2048, 128, ksum, 1024, sp, _lib.DT_BF16,
-                                          A, 4, A, None, A, sel, blocks, sink, local, 1, S, H, 2, 128, 8, 16, 4, 0.1, A, nb, None)
+                                          A, 4, A, None, out, sel, blocks, sink, local, 1, S, H, 2, 128, 8, 16, 4, 0.1, A, nb, None)
 
     def fork(kv=A, ksum=A, L=2, Hk=2, P=8, T=16, D=128, table=A, ts=4, B=4, W=4, pairs=2, room=1, ws=A, nb=1 << 20, refs=A):
         return _lib.lib().mdx_page_fork(kv, ksum, L, Hk, P, T, D, table, ts, B, W, A, refs, A, A, pairs, room, 1, None, A, ws, nb, None)
 
-    def commit(kv=A, dt=_lib.DT_BF16, T=16, D=128, B=4, W=4, ts=4, path=A, R=8, room=1, count=A, nb=1 << 20):
-        return _lib.lib().mdx_page_commit(kv, A, dt, 2, 2, 8, T, D, A, ts, B, W, A, A, A, count, path, R, room, None, A, A, nb, None)
+    def commit(kv=A, dt=_lib.DT_BF16, T=16, D=128, B=4, W=4, ts=4, path=A, R=8, room=1, count=A, nb=1 << 20, new=A):
+        return _lib.lib().mdx_page_commit(kv, A, dt, 2, 2, 8, T, D, A, ts, B, W, A, new, A, count, path, R, room, None, A, A, nb, None)
 
     bad = [(attn, dict(q=None)), (attn, dict(length=None)), (attn, dict(dt=_lib.DT_F32)), (attn, dict(D=192)), (attn, dict(T=24)),
            (attn, dict(T=8)), (attn, dict(T=2048)), (attn, dict(H=5)), (attn, dict(H=258)), (attn, dict(B=0)), (attn, dict(B=1025)), (attn, dict(S=0)),
@@ -118,7 +118,10 @@ def test_refusals_before_any_device_work():
            (fork, dict(ws=None)), (fork, dict(P=0)),
            (commit, dict(kv=None)), (commit, dict(count=None)), (commit, dict(dt=_lib.DT_F32)), (commit, dict(T=17)), (commit, dict(D=96)),
            (commit, dict(B=1025)), (commit, dict(R=0)), (commit, dict(R=65)), (commit, dict(room=-1)), (commit, dict(nb=16)),
-           (commit, dict(ts=2))]
+           (commit, dict(ts=2)),
+           (attn, dict(out=A)), (attn, dict(out=A + 1008)), (blocks, dict(out=A)), (attn, dict(qs=-512)),
+           (fork, dict(pairs=1024, W=1 << 20, ts=1 << 20, nb=1 << 40)), (commit, dict(B=1024, W=1 << 20, ts=1 << 20, nb=1 << 40)),
+           (commit, dict(new=A + 4)), (commit, dict(new=A - 12))]
     for f, kw in bad:
         assert f(**kw) == _lib.MDX_EINVAL, (f.__name__, kw)
         assert _lib.lib().mdx_last_error(), (f.__name__, kw)

@@ -268,3 +268,30 @@ def test_commit_into_other_lengths(C, dev, with_path):
     path = [[0, 1, 2, 3], [0, 2, 3, 3], [1, 0, 2, 3], [0, 1, 2, 4], [0, 1, 2, 3], [0, 1, 2, 3], [0, 3, 3, 3], [0, 1, 2, 3]]
     assert _commit(C, dev, st, [4, 3, 2, 4, 2, 4, 2, 0], path if with_path else None, 13, in_place=False)
     assert _commit(C, dev, st, [4, 3, 2, 4, 2, 4, -1, 0], path if with_path else None, 13)
+
+
+@pytest.mark.parametrize("share", [True, False])
+def test_fork_replay(C, dev, share):
+    """A captured fork and one on another stream in turn with eager calls: the same tables, references and pages."""
+    st = State(29, [37, 70, 0], P=90, held=8, W=10)
+    d, e, w = st.dev(dev), st.dev(dev), st.dev(dev)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    dst, src, slots, slots_e = i32(2, 0), i32(0, 1), *(torch.empty(2, 5, dtype=torch.int64, device=dev) for _ in range(2))
+    C.page_fork(*w, dst, src, 5, share, slots)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        status = C.page_fork(*d, dst, src, 5, share, slots)
+    side = torch.cuda.Stream()
+    for k in range(4):
+        src.copy_(i32(*[(0, 1), (1, -1), (1, 0), (2, 2)][k]))
+        torch.cuda.synchronize()
+        if k == 2:
+            with torch.cuda.stream(side):
+                status.copy_(C.page_fork(*d, dst, src, 5, share, slots))
+        else:
+            gr.replay()
+        torch.cuda.synchronize()
+        want = C.page_fork(*e, dst, src, 5, share, slots_e)
+        for a, b in zip(d + [slots, status], e + [slots_e, want]):
+            assert torch.equal(a.view(torch.int16) if a.dtype == torch.bfloat16 else a, b.view(torch.int16) if b.dtype == torch.bfloat16 else b), k
