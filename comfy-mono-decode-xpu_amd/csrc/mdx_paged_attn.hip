@@ -732,67 +732,86 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
         float* const lo = reinterpret_cast<float*>(smem);               // [RTW][P][16][OR]
         float* const lm = lo + RTW * P * 16 * OR;                       // [RTW][P][16] maxima (log2 units), then sums
         float* rec = a.part + (int64_t(share) * 2 + (first ? 1 : 0)) * RPW * (D + 2);
-        __syncthreads();  // the ring is free
-#pragma unroll
-        for (int t = 0; t < TPW; ++t) {
-            float* mo = lo + (rw * P + part) * 16 * OR + c16 * OR + 4 * g;
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(mo + 16 * dt) = acc[t][dt];
-            const float sl = sum_x32(sum_x16(l[t]));
-            if (g == 0) {
-                lm[(rw * P + part) * 16 + c16] = m_lim[t] == -INFINITY ? -INFINITY : m_z[t];
-                lm[RTW * P * 16 + (rw * P + part) * 16 + c16] = sl;
+        // row r of the unit's block (row s, head h), dims d .. d + 3: done, or to its partial
+        auto put = [&](int r, int s, int h, int d, float M, float sum, f32x4 o) {
+            if (first && last) {
+                const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+                // (no token admitted: 0, whatever o holds)
+                *reinterpret_cast<uint2*>(a.out + ((int64_t(b) * a.S + s) * a.H + h) * D + d) =
+                    sum == 0.f ? make_uint2(0u, 0u) : make_uint2(E::pair(o[0] * inv, o[1] * inv), E::pair(o[2] * inv, o[3] * inv));
+            } else {
+                *reinterpret_cast<f32x4*>(rec + int64_t(r) * D + d) = o;
+                if (d == 0) {
+                    rec[int64_t(RPW) * D + r] = M;
+                    rec[int64_t(RPW) * (D + 1) + r] = sum;
+                }
             }
-            __syncthreads();
-            // thread: row x / (D / 4) of the RTW tiles' 16 each, four dims
-            for (int x = tid; x < RTW * 16 * (D / 4); x += NT) {
-                const int rt = x / (16 * (D / 4)), rr = x / (D / 4) % 16, d = x % (D / 4) * 4;
-                const int r = (rt * TPW + t) * 16 + rr;  // row of the unit's block
+        };
+        __syncthreads();  // the ring is free
+        // One part: nothing to meet, each lane has its row's four dims of every dim tile (4 x 1024 rows over 1000: 125 us through
+        // LDS, 119; `odd` is set again behind the next unit's first barrier only).
+        static_assert(P > 1 || RTW > 1, "");
+        if (P == 1 && !odd) {
+#pragma unroll
+            for (int t = 0; t < TPW; ++t) {
+                const int r = (rw * TPW + t) * 16 + c16;
+                const float sl = sum_x32(sum_x16(l[t])), M = m_lim[t] == -INFINITY ? -INFINITY : m_z[t];
                 if (r >= rows) continue;
                 const int s = s_first + r / a.G, h = kh * a.G + r % a.G;
-                float M = -INFINITY;
 #pragma unroll
-                for (int p = 0; p < P; ++p) M = fmaxf(M, lm[(rt * P + p) * 16 + rr]);
-                float sum = 0.f;
-                f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int dt = 0; dt < DT; ++dt) put(r, s, h, 16 * dt + 4 * g, M, sl, acc[t][dt]);
+            }
+        } else {
 #pragma unroll
-                for (int p = 0; p < P; ++p) {
-                    const float mp = lm[(rt * P + p) * 16 + rr];
-                    const float wp = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mp - M);
-                    sum += lm[RTW * P * 16 + (rt * P + p) * 16 + rr] * wp;
-                    o += *reinterpret_cast<const f32x4*>(lo + (rt * P + p) * 16 * OR + rr * OR + d) * wp;
+            for (int t = 0; t < TPW; ++t) {
+                float* mo = lo + (rw * P + part) * 16 * OR + c16 * OR + 4 * g;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(mo + 16 * dt) = acc[t][dt];
+                const float sl = sum_x32(sum_x16(l[t]));
+                if (g == 0) {
+                    lm[(rw * P + part) * 16 + c16] = m_lim[t] == -INFINITY ? -INFINITY : m_z[t];
+                    lm[RTW * P * 16 + (rw * P + part) * 16 + c16] = sl;
                 }
-                if (odd) {  // (uniform: what the stages left out, for the rows that admit it)
-                    for (int v = step0 * TOK; v < min(t_end, (step0 + nst) * TOK); ++v) {
-                        const int own_row = v - sp.tree0;
-                        if (own_row >= 0 && !(a.mask ? (uint64_t(a.mask[int64_t(b) * a.S + s]) >> own_row) & 1 : own_row <= s)) continue;
-                        const int tok = SEL && v >= sp.nsel ? v - sp.nsel + sp.tail : v;
-                        const bool chosen = SEL && v < sp.nsel;
-                        if (!chosen && (tok >> a.lt) >= a.W) continue;
-                        const int64_t e = chosen ? picked[v >> a.lt] : row[tok >> a.lt];
-                        if (e < 0 || e >= a.P) continue;
-                        const uint16_t* src = a.value + kh * a.vh + e * a.vp + (tok & ((1 << a.lt) - 1)) * a.vt + d;
+                __syncthreads();
+                // thread: row x / (D / 4) of the RTW tiles' 16 each, four dims
+                for (int x = tid; x < RTW * 16 * (D / 4); x += NT) {
+                    const int rt = x / (16 * (D / 4)), rr = x / (D / 4) % 16, d = x % (D / 4) * 4;
+                    const int r = (rt * TPW + t) * 16 + rr;  // row of the unit's block
+                    if (r >= rows) continue;
+                    const int s = s_first + r / a.G, h = kh * a.G + r % a.G;
+                    float M = -INFINITY;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float x = E::to_f32(src[i]);
-                            if (!(__builtin_fabsf(x) < INFINITY)) o[i] += x;
+                    for (int p = 0; p < P; ++p) M = fmaxf(M, lm[(rt * P + p) * 16 + rr]);
+                    float sum = 0.f;
+                    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int p = 0; p < P; ++p) {
+                        const float mp = lm[(rt * P + p) * 16 + rr];
+                        const float wp = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mp - M);
+                        sum += lm[RTW * P * 16 + (rt * P + p) * 16 + rr] * wp;
+                        o += *reinterpret_cast<const f32x4*>(lo + (rt * P + p) * 16 * OR + rr * OR + d) * wp;
+                    }
+                    if (odd) {  // (uniform: what the stages left out, for the rows that admit it)
+                        for (int v = step0 * TOK; v < min(t_end, (step0 + nst) * TOK); ++v) {
+                            const int own_row = v - sp.tree0;
+                            if (own_row >= 0 && !(a.mask ? (uint64_t(a.mask[int64_t(b) * a.S + s]) >> own_row) & 1 : own_row <= s)) continue;
+                            const int tok = SEL && v >= sp.nsel ? v - sp.nsel + sp.tail : v;
+                            const bool chosen = SEL && v < sp.nsel;
+                            if (!chosen && (tok >> a.lt) >= a.W) continue;
+                            const int64_t e = chosen ? picked[v >> a.lt] : row[tok >> a.lt];
+                            if (e < 0 || e >= a.P) continue;
+                            const uint16_t* src = a.value + kh * a.vh + e * a.vp + (tok & ((1 << a.lt) - 1)) * a.vt + d;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float x = E::to_f32(src[i]);
+                                if (!(__builtin_fabsf(x) < INFINITY)) o[i] += x;
+                            }
                         }
                     }
+                    put(r, s, h, d, M, sum, o);
                 }
-                if (first && last) {
-                    const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
-                    // (no token admitted: 0, whatever o holds)
-                    *reinterpret_cast<uint2*>(a.out + ((int64_t(b) * a.S + s) * a.H + h) * D + d) =
-                        sum == 0.f ? make_uint2(0u, 0u) : make_uint2(E::pair(o[0] * inv, o[1] * inv), E::pair(o[2] * inv, o[3] * inv));
-                } else {
-                    *reinterpret_cast<f32x4*>(rec + int64_t(r) * D + d) = o;
-                    if (d == 0) {
-                        rec[int64_t(RPW) * D + r] = M;
-                        rec[int64_t(RPW) * (D + 1) + r] = sum;
-                    }
-                }
+                __syncthreads();
             }
-            __syncthreads();
         }
         if (first && tid == 0 && !a.whole && (a.by_unit || !last)) {
             // the unit goes on in the shares behind: how many in all (1: it is done)
