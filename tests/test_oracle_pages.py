@@ -137,3 +137,15 @@ def test_host_tensors_are_refused():
                  lambda: _C.attn_blocks(z(2, 1, 4, 64, dtype=torch.bfloat16), kv[0, 0], kv[0, 1], ks[0], i(2, 4), i(2), 1)):
         with pytest.raises(RuntimeError, match="ROCm device"):
             call()
+
+
+def test_a_missing_binding_is_an_error(monkeypatch):
+    import sys
+
+    import mdx
+    from mdx import _lib
+    monkeypatch.setitem(sys.modules, "mdx._bind", None)
+    monkeypatch.delattr(mdx, "_bind", raising=False)
+    monkeypatch.setattr(_lib, "_bound", None)
+    with pytest.raises(_lib.MdxError, match="build.py"):
+        _lib.bind()
