@@ -1437,10 +1437,11 @@ extern "C" int mdx_attn_blocks(const void* q, int64_t q_seq_stride, int64_t q_ro
         }
         MDX_LAUNCHED();
     }
-    // (keys in registers: the smallest form that holds a row's. A call at 1000 pages: 21.6 us, 23.6 with the third form, 42.4 with
-    // the fourth; at 4000: 24.3, 26.1, 46.4; at 16000: 34.6 and 62.5)
-    if (W <= 1024) hipLaunchKernelGGL((block_select_kernel<256, 4>), dim3(unsigned(units)), dim3(256), 0, st, a);
-    else if (W <= 4096) hipLaunchKernelGGL((block_select_kernel<512, 8>), dim3(unsigned(units)), dim3(512), 0, st, a);
+    // (keys in registers: the smallest form that holds a row's. A call at 1000 pages: 20.3 us, 21.7 by 256 threads of four keys,
+    // 23.6 with the third form, 42.4 with the fourth; at 4000: 22.8, 24.1 by 512 threads of eight, 26.1, 46.4; at 16000: 34.6
+    // with the third form and 62.5 with the fourth)
+    if (W <= 1024) hipLaunchKernelGGL((block_select_kernel<512, 2>), dim3(unsigned(units)), dim3(512), 0, st, a);
+    else if (W <= 4096) hipLaunchKernelGGL((block_select_kernel<1024, 4>), dim3(unsigned(units)), dim3(1024), 0, st, a);
     else if (W <= 16384) hipLaunchKernelGGL((block_select_kernel<1024, 16>), dim3(unsigned(units)), dim3(1024), 0, st, a);
     else hipLaunchKernelGGL((block_select_kernel<1024, 64>), dim3(unsigned(units)), dim3(1024), 0, st, a);
     MDX_LAUNCHED();
