@@ -926,13 +926,18 @@ __global__ __launch_bounds__(256) void block_score_kernel(PagedArgs a) {
     const uint16_t* kp = a.ksum + kh * a.sh + (in ? e : 0) * a.sp + 8 * g;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) k[i] = *reinterpret_cast<const u32x4*>(kp + 32 * i);
-    for (int i = threadIdx.x; i < ns * D; i += 256) {
-        const int s = i / D, d = i % D;
+    for (int i = threadIdx.x; i < ns * (D / 8); i += 256) {  // (eight dims each: one round of loads for 8 rows of 256)
+        const int s = i / (D / 8), d = i % (D / 8) * 8;
         const uint16_t* p = a.q + b * a.qb + (s0 + s) * a.qs + kh * a.G * a.qh + d;
-        double t = 0;
+        double t[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll 4
-        for (int h = 0; h < a.G; ++h) t += double(E::to_f32(p[h * a.qh]));
-        qs[s * QR + d] = t;
+        for (int h = 0; h < a.G; ++h) {
+            const u32x4 v = *reinterpret_cast<const u32x4*>(p + h * a.qh);
+#pragma unroll
+            for (int x = 0; x < 8; ++x) t[x] += double(E::to_f32(uint16_t(v[x / 2] >> (16 * (x & 1)))));
+        }
+#pragma unroll
+        for (int x = 0; x < 8; x += 2) *reinterpret_cast<f64x2*>(qs + s * QR + d + x) = f64x2{t[x], t[x + 1]};
     }
     __syncthreads();
     auto put = [&](int s, double z) {
