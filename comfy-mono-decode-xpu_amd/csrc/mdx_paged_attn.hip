@@ -256,10 +256,11 @@ struct Geometry {
     static constexpr int NS = RING / (2 * STAGE * P);             // ring stages per part
     static constexpr int PER = STAGE / 1024 / RTW;                // direct loads per wave, stage and matrix
     // What a unit costs beside its steps (its queries, the ring's first stage, the meeting of its parts), in steps: without
-    // it the share that takes the shortest units ends last. 16 prompts of 128 rows over 0 to 6000 tokens: 408 -> 166 us a
-    // call, 64 trees of 16 rows over at most 900: 104 -> 59, 32 of 8 rows over at most 8000: 130 -> 115; of 64 sequences'
-    // selections, one with 256 blocks and the others with 4: 199 -> 223; equal lengths: up to 8 % less.
-    static constexpr int FIXED = RPW == 16 ? 2 : RPW == 128 ? 6 : 4;
+    // it the share that takes the shortest units ends last. 16 prompts of 128 rows over 0 to 6000 tokens: 408 us a call with
+    // 0, 167 with 6, 160 with 5; 64 trees of 16 rows over at most 900: 104 with 0, 59 with 4; 48 over at most 8192 at head_dim
+    // 64: 119 with 4, 112 with 5; trees of 8 rows: 159 with 4, 156 with 3; 16 single tokens over at most 8192: 48 with 0, 44
+    // with 2; of 64 sequences' selections, one with 256 blocks and the others with 4: 199 with 0, 223 with 2.
+    static constexpr int FIXED = RPW == 16 ? 2 : RPW == 32 ? 3 : 5;
     static_assert(NS >= 1 && (NS & (NS - 1)) == 0 && PER >= 1 && (RTW == 1 ? SUB == 1 : NS >= 2) && (SUB == 1 || D != 256), "ring geometry");
 };
 
