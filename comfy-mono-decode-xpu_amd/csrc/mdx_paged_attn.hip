@@ -749,10 +749,14 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
             }
         };
         __syncthreads();  // the ring is free
-        // One part: nothing to meet, each lane has its row's four dims of every dim tile (4 x 1024 rows over 1000: 125 us through
-        // LDS, 119; `odd` is set again behind the next unit's first barrier only).
+        // The flag is read here alone. A wave that is ahead sets it again for the next unit without waiting for the others where
+        // it has a ring of its own, but not before the barriers below (several parts) or that unit's first stage (waves that share
+        // a ring), which a wave that has yet to read it here holds up; so it is one value for all, as the barriers under it need.
         static_assert(P > 1 || RTW > 1, "");
-        if (P == 1 && !odd) {
+        const bool left_out = odd != 0;
+        // One part: nothing to meet, each lane has its row's four dims of every dim tile (4 x 1024 rows over 1000: 125 us through
+        // LDS, 119).
+        if (P == 1 && !left_out) {
 #pragma unroll
             for (int t = 0; t < TPW; ++t) {
                 const int r = (rw * TPW + t) * 16 + c16;
@@ -792,7 +796,7 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
                         sum += lm[RTW * P * 16 + (rt * P + p) * 16 + rr] * wp;
                         o += *reinterpret_cast<const f32x4*>(lo + (rt * P + p) * 16 * OR + rr * OR + d) * wp;
                     }
-                    if (odd) {  // (uniform: what the stages left out, for the rows that admit it)
+                    if (left_out) {  // (what the stages left out, for the rows that admit it)
                         for (int v = step0 * TOK; v < min(t_end, (step0 + nst) * TOK); ++v) {
                             const int own_row = v - sp.tree0;
                             if (own_row >= 0 && !(a.mask ? (uint64_t(a.mask[int64_t(b) * a.S + s]) >> own_row) & 1 : own_row <= s)) continue;
@@ -823,9 +827,8 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
         // ---- the next unit
         at += nst + (last ? Geo::FIXED : 0);
         if (at >= end) break;
-        if (odd) {  // (uniform: every thread is past its last use)
-            __syncthreads();
-            if (tid == 0) odd = 0;
+        if (left_out) {  // (uniform)
+            if (tid == 0) odd = 0;  // (every wave has read it: the barriers of the meeting lie between)
             __syncthreads();
         }
         step0 = 0;

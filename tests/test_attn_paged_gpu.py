@@ -250,3 +250,28 @@ def test_queries_of_all_sequences_are_one(C, dev):
     q = q[:1, :, :1].expand(3, 4, 8, 128)
     got = C.attn_paged(q[:1, :, :1].to(dev).expand(3, 4, 8, 128), key.to(dev), value.to(dev), table.to(dev), n)
     check(got, BF, q, key, value, table, lens, None, 128 ** -0.5)
+
+
+@pytest.mark.parametrize("H,Hk,D,S,B,tree", [(4, 2, 64, 1, 400, False), (8, 4, 128, 3, 300, True), (4, 2, 256, 5, 200, True), (32, 4, 64, 6, 160, True)])
+def test_infinite_values_in_every_other_unit(C, dev, H, Hk, D, S, B, tree):
+    """Shares of several units, of which some hold an infinite value that their rows attend and others none: what a stage leaves out
+    for one unit is not taken for the next one's, call after call."""
+    print(f"infinite values: H={H} Hk={Hk} D={D} S={S} B={B}", flush=True)
+    g = torch.Generator().manual_seed(D + S)
+    lens = [int(x) for x in torch.randint(0, 150, (B,), generator=g)]
+    key, value, table = cache(g, BF, Hk, 16, D, lens, S, width=200)
+    q = (torch.randn(B, S, H, D, generator=g) * 1.5).to(BF)
+    mask = tree_masks(g, B, S) if tree else None
+    clean = value.clone()
+    some = [b for b in range(B) if b % 3 != 1]
+    for b in some:
+        t = lens[b]  # (own row 0, the root: every row attends it)
+        value[:, table[b, t // 16], t % 16, 7] = float("inf")
+    a = [x.to(dev) for x in (q, key, value, table)] + [torch.tensor(lens, dtype=torch.int32, device=dev), None if mask is None else mask.to(dev)]
+    got = [C.attn_paged(*a) for _ in range(10)]
+    assert all(torch.equal(got[0].view(torch.int16), x.view(torch.int16)) for x in got[1:])
+    out = got[0].cpu()
+    assert (out[some][..., 7] == float("inf")).all()
+    want = C.attn_paged(a[0], a[1], clean.to(dev), *a[3:]).cpu()
+    out[some, :, :, 7] = want[some][..., 7]
+    check(out, BF, q, key, clean, table, lens, mask, D ** -0.5)
