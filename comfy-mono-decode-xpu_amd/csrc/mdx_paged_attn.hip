@@ -27,6 +27,7 @@
 // 64 tokens a stage instead of 32: 128 -> 99 us for 2048 rows over 1000).
 //
 // Reference: none for the pages; the rows' contract is csrc/attn_dpas.sycl:269-342's.
+#include <limits.h>
 #include <math.h>
 
 #include <atomic>
@@ -270,7 +271,8 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
     constexpr int NT = Geo::NT, RPW = Geo::RPW, STAGE = Geo::STAGE, NS = Geo::NS, PER = Geo::PER;
     constexpr int KK = D / 32, DT = D / 16, ST = STEP * SUB, TOK = ST * P;
     extern __shared__ __align__(256) unsigned char smem[];  // (the reads' exclusive ors need rows aligned to 256 bytes)
-    __shared__ int sh_sum[NT / 64], sh_at[4], odd;
+    __shared__ int sh_sum[NT / 64], sh_at[4];
+    __shared__ int odd[2];  // the first and the last stage of the unit that left values out which a row attends (none: -1 last)
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, c16 = lane & 15;
     const int rw = w % RTW, part = w / RTW;
@@ -304,7 +306,7 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
         sp = span_of<SEL>(a, uload(a.length + b));
         begin = in_b = 0;
         end = quota = steps_of(a, sp, u, TOK);
-        if (tid == 0) odd = 0;
+        if (tid == 0) odd[0] = INT_MAX, odd[1] = -1;
     } else {
         // The units in the line's order (sequence, kv head, block), a run of neighbouring ones per thread (where a kv head
         // is one unit, its sequence's kv heads together); the threads' sums, and the unit that the share begins in.
@@ -356,7 +358,7 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
             });
         if (tid == 0) {
             if (!a.by_unit) a.info[share] = make_int4(0, 0, 0, 0);
-            odd = 0;
+            odd[0] = INT_MAX, odd[1] = -1;
         }
         if (begin >= end) return;  // (uniform)
         __syncthreads();
@@ -659,9 +661,12 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
             constexpr int VT = D == 64 ? 4 : 8;  // dim tiles read at once
             u32x2 va[VT], vb[VT];
             // A weight of 0 times an infinity or a NaN in a place that a row does not admit would reach the row: in a stage that
-            // not every row admits whole, such values count as 0 here, and where there are any the rows that do admit them
-            // get them when the unit's parts meet (`odd`).
-            auto sift = [&]() {
+            // not every row admits whole, such values count as 0 here (piece y of the stage). Those that some row of the wave
+            // admits it gets when the unit's parts meet, from the stages noted in `odd`. What no row admits (rows behind the
+            // last token of a page, the stand-in for a missing page) notes nothing: a cache holds anything there, and the
+            // search through a whole share takes milliseconds (a prompt's 2048 rows over 1000, NaN in the unused rows: 103 us as
+            // with zeros there, 16.8 ms with every such stage noted and searched from the share's first).
+            auto sift = [&](int y) {
                 if (!whole) {
                     uint32_t top = 0;
 #pragma unroll
@@ -669,13 +674,39 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
                         top |= ((va[x].x & E::EXP) + E::ONE) | ((va[x].y & E::EXP) + E::ONE) | ((vb[x].x & E::EXP) + E::ONE) |
                                ((vb[x].y & E::EXP) + E::ONE);
                     if (__builtin_amdgcn_ballot_w64((top & 0x80008000u) != 0) != 0) {
-                        auto finite = [](uint32_t v) { return v & ~(((((v & E::EXP) + E::ONE) & 0x80008000u) >> 15) * 0xFFFFu); };
+                        // by token: va.x, va.y, vb.x, vb.y hold tokens 4 g, 4 g + 2, 16 + 4 g, 16 + 4 g + 2 and the ones behind
+                        auto high = [](uint32_t v) { return ((v & E::EXP) + E::ONE) & 0x80008000u; };
+                        auto finite = [&](uint32_t v) { return v & ~((high(v) >> 15) * 0xFFFFu); };
+                        uint32_t t0 = 0, t2 = 0, t16 = 0, t18 = 0;
 #pragma unroll
                         for (int x = 0; x < VT; ++x) {
+                            t0 |= high(va[x].x), t2 |= high(va[x].y), t16 |= high(vb[x].x), t18 |= high(vb[x].y);
                             va[x] = u32x2{finite(va[x].x), finite(va[x].y)};
                             vb[x] = u32x2{finite(vb[x].x), finite(vb[x].y)};
                         }
-                        odd = 1;
+                        // the piece's tokens that a row of the wave admits (without masks: up to the last row's own)
+                        const int p = sp.tree0 - v0 - STEP * y;
+                        uint32_t in;
+                        if (a.mask) {
+                            uint64_t all = 0;
+#pragma unroll
+                            for (int t = 0; t < TPW; ++t) all |= bits[t];
+#pragma unroll
+                            for (int d = 1; d < 16; d <<= 1) all |= __shfl_xor(all, d, 64);
+                            const uint64_t own_bits = p >= 32 ? 0 : (p >= 0 ? all << p : (-p < 64 ? all >> -p : 0));
+                            in = (p >= 32 ? ~0u : (p > 0 ? (1u << p) - 1u : 0u)) | uint32_t(own_bits);
+                        } else {
+                            const int nv = t_none - v0 - STEP * y;
+                            in = nv >= 32 ? ~0u : (nv > 0 ? (1u << nv) - 1u : 0u);
+                        }
+                        const uint32_t here = ok >> (2 * y);
+                        in &= ((here & 1u) ? 0x0000FFFFu : 0u) | ((here & 2u) ? 0xFFFF0000u : 0u);
+                        auto two = [](uint32_t v) { return ((v >> 15) & 1u) | ((v >> 30) & 2u); };
+                        const uint32_t found = (two(t0) | (two(t2) << 2) | (two(t16) << 16) | (two(t18) << 18)) << (4 * g);
+                        if (__builtin_amdgcn_ballot_w64((found & in) != 0) != 0 && lane == 0) {
+                            atomicMin(&odd[0], s);
+                            atomicMax(&odd[1], s);
+                        }
                     }
                 }
             };
@@ -701,7 +732,7 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
                 wait_v();
                 read_v<D, 0>(va, vb, slot + STAGE + v_lane);
                 refill_v();
-                sift();
+                sift(0);
 #pragma unroll
                 for (int t = 0; t < TPW; ++t) weigh(t, 0, weights(t).p[0]);
             } else {
@@ -714,13 +745,13 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
                 for (int x = 0; x < SUB; ++x) {
                     read_v<D, 0>(va, vb, slot + STAGE + v_lane + x * STEP * RB);
                     if constexpr (D == 256) {
-                        sift();
+                        sift(x);
 #pragma unroll
                         for (int t = 0; t < TPW; ++t) weigh(t, 0, pf[t].p[x]);
                         read_v<D, 1>(va, vb, slot + STAGE + v_lane);
                     }
                     if (x == SUB - 1) refill_v();
-                    sift();
+                    sift(x);
 #pragma unroll
                     for (int t = 0; t < TPW; ++t) weigh(t, D == 256 ? 8 : 0, pf[t].p[x]);
                 }
@@ -749,11 +780,12 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
             }
         };
         __syncthreads();  // the ring is free
-        // The flag is read here alone. A wave that is ahead sets it again for the next unit without waiting for the others where
-        // it has a ring of its own, but not before the barriers below (several parts) or that unit's first stage (waves that share
-        // a ring), which a wave that has yet to read it here holds up; so it is one value for all, as the barriers under it need.
+        // The stages are read here alone. A wave that is ahead notes the next unit's without waiting for the others where it has
+        // a ring of its own, but not before the barriers below (several parts) or that unit's first stage (waves that share a
+        // ring), which a wave that has yet to read them here holds up; so all have one value, as the barriers under it need.
         static_assert(P > 1 || RTW > 1, "");
-        const bool left_out = odd != 0;
+        const int odd_from = odd[0], odd_to = odd[1];
+        const bool left_out = odd_to >= 0;
         // One part: nothing to meet, each lane has its row's four dims of every dim tile (4 x 1024 rows over 1000: 125 us through
         // LDS, 119).
         if (P == 1 && !left_out) {
@@ -797,7 +829,7 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
                         o += *reinterpret_cast<const f32x4*>(lo + (rt * P + p) * 16 * OR + rr * OR + d) * wp;
                     }
                     if (left_out) {  // (what the stages left out, for the rows that admit it)
-                        for (int v = step0 * TOK; v < min(t_end, (step0 + nst) * TOK); ++v) {
+                        for (int v = (step0 + odd_from) * TOK; v < min(t_end, (step0 + odd_to + 1) * TOK); ++v) {
                             const int own_row = v - sp.tree0;
                             if (own_row >= 0 && !(a.mask ? (uint64_t(a.mask[int64_t(b) * a.S + s]) >> own_row) & 1 : own_row <= s)) continue;
                             const int tok = SEL && v >= sp.nsel ? v - sp.nsel + sp.tail : v;
@@ -828,7 +860,7 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
         at += nst + (last ? Geo::FIXED : 0);
         if (at >= end) break;
         if (left_out) {  // (uniform)
-            if (tid == 0) odd = 0;  // (every wave has read it: the barriers of the meeting lie between)
+            if (tid == 0) odd[0] = INT_MAX, odd[1] = -1;  // (every wave has read it: the barriers of the meeting lie between)
             __syncthreads();
         }
         step0 = 0;

@@ -275,3 +275,63 @@ def test_infinite_values_in_every_other_unit(C, dev, H, Hk, D, S, B, tree):
     want = C.attn_paged(a[0], a[1], clean.to(dev), *a[3:]).cpu()
     out[some, :, :, 7] = want[some][..., 7]
     check(out, BF, q, key, clean, table, lens, mask, D ** -0.5)
+
+
+def _median_us(f, n=15):
+    for _ in range(3):
+        f()
+    torch.cuda.synchronize()
+    took = []
+    for _ in range(n):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        f()
+        b.record()
+        torch.cuda.synchronize()
+        took.append(a.elapsed_time(b) * 1e3)
+    return sorted(took)[n // 2]
+
+
+@pytest.mark.parametrize("H,Hk,D,T,S,lens,tree", [(32, 8, 128, 64, 1, [100 + 120 * i for i in range(64)], False), (16, 4, 256, 16, 8, [1001 + 401 * i for i in range(16)], True),
+                                                  (32, 8, 128, 64, 2048, [1000], False), (16, 8, 64, 32, 16, [3000, 500, 77], True)])
+def test_what_no_row_attends_costs_nothing(C, dev, H, Hk, D, T, S, lens, tree):
+    """NaN and infinities in the rows behind the sequences' tokens and in free pages: the bits of the same call over zeros, and its
+    time. The bound of the time is twice the other's: a search through the tokens took 8 to 160 times as long."""
+    print(f"unused rows: H={H} Hk={Hk} D={D} T={T} S={S} sequences={len(lens)}", flush=True)
+    g = torch.Generator().manual_seed(3)
+    out, us = [], []
+    key, value, table = cache(g, BF, Hk, T, D, lens, S, junk=float("nan"))
+    q = torch.randn(len(lens), S, H, D, generator=g).to(BF).to(dev)
+    mask = tree_masks(g, len(lens), S).to(dev) if tree else None
+    n = torch.tensor(lens, dtype=torch.int32, device=dev)
+    for junk in (0.0, float("nan"), float("-inf")):
+        k, v = (torch.where(x.isnan(), torch.tensor(junk, dtype=BF), x).to(dev) for x in (key, value))
+        a = (q, k, v, table.to(dev), n, mask)
+        out.append(C.attn_paged(*a))
+        us.append(_median_us(lambda: C.attn_paged(*a)))
+    assert all(torch.equal(out[0], x) for x in out[1:])
+    assert max(us[1:]) < 2 * us[0], us
+
+
+@pytest.mark.parametrize("H,Hk,D,S,tree", [(8, 2, 128, 6, True), (4, 2, 64, 40, True), (8, 2, 128, 150, False), (4, 1, 256, 200, False), (8, 4, 64, 300, False)])
+def test_values_that_some_rows_attend(C, dev, H, Hk, D, S, tree):
+    """Infinite values at many of the rows' own tokens, far apart: every row that attends one shows it with its sign, no other does."""
+    print(f"values attended by some: H={H} Hk={Hk} D={D} S={S}", flush=True)
+    g = torch.Generator().manual_seed(S)
+    lens = [300, 0, 41]
+    key, value, table = cache(g, BF, Hk, 32, D, lens, S)
+    q = torch.randn(3, S, H, D, generator=g).to(BF)
+    mask = tree_masks(g, 3, S) if tree else None
+    clean, hit = value.clone(), torch.zeros(3, S, D, dtype=torch.bool)
+    for j in range(1, S, max(2, S // 7)):
+        d = 5 * j % D
+        for b, m in enumerate(lens):
+            value[:, table[b, (m + j) // 32], (m + j) % 32, d] = float("-inf")
+            sees = (mask[b] >> j) & 1 == 1 if tree else torch.arange(S) >= j
+            hit[b, :, d] |= sees
+    a = (q.to(dev), key.to(dev), value.to(dev), table.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev), None if mask is None else mask.to(dev))
+    got = C.attn_paged(*a).cpu()
+    hit = hit[:, :, None, :].expand_as(got)
+    assert hit.any() and (got[hit] == float("-inf")).all() and got[~hit].isfinite().all()
+    want = C.attn_paged(a[0], a[1], clean.to(dev), *a[3:]).cpu()
+    check(torch.where(hit, want, got), BF, q, key, clean, table, lens, mask, D ** -0.5)
