@@ -27,6 +27,7 @@
 // 64 tokens a stage instead of 32: 128 -> 99 us for 2048 rows over 1000).
 //
 // Reference: none for the pages; the rows' contract is csrc/attn_dpas.sycl:269-342's.
+#include <float.h>
 #include <limits.h>
 #include <math.h>
 
@@ -108,6 +109,11 @@ struct PagedArgs {
 
 constexpr int MAX_SEQS = 1024;
 constexpr int STEP = 32;
+// References (log2 units) past which scores are taken less the reference in score units first. A weight's exponent is
+// score * zs - reference * zs, the first product unrounded, the second one fp32 number: its rounding (2^-9 up to here) is a
+// factor that numerator and normaliser share. Further out it grows past what the weights' type holds (fp16 from 2^26 on, bf16
+// from 2^32: NaN for finite inputs).
+constexpr float FAR_REF = 65536.f;
 constexpr int CUS = 256;
 constexpr int RING_BYTES = 128 * 1024;  // of a CU's work-groups together
 // 128-token steps of a call at most, for the forms that go by latency (below: launch_rows)
@@ -512,14 +518,15 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
         }
 
         f32x4 acc[TPW][DT];
-        // per row: the score up to which its reference serves (-inf: none yet), the reference in log2 units (0 as long as nothing
-        // is admitted, so that -inf - -inf never forms), the sum of weights
-        float m_lim[TPW], m_z[TPW], l[TPW];
+        // per row: the score up to which its reference serves (-inf: none yet; the lowest number: past FAR_REF, every stage
+        // looks), the reference, an earlier maximal score (0 as long as nothing is admitted, so that -inf - -inf never forms), the
+        // sum of weights
+        float m_lim[TPW], m_ref[TPW], l[TPW];
         const float slack = E::SLACK / a.zs;
 #pragma unroll
         for (int t = 0; t < TPW; ++t) {
             m_lim[t] = -INFINITY;
-            m_z[t] = 0.f;
+            m_ref[t] = 0.f;
             l[t] = 0.f;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) acc[t][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -632,19 +639,27 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
                 if constexpr (SUB == 2)
                     mx = max3(max3(st[1][t][0][0], st[1][t][0][1], st[1][t][0][2]), max3(st[1][t][0][3], st[1][t][1][0], st[1][t][1][1]),
                               max3(st[1][t][1][2], st[1][t][1][3], mx));
+                float ref = m_ref[t];
                 if (__builtin_amdgcn_ballot_w64(mx > m_lim[t]) != 0) {  // (uniform)
                     const float top = max_x32(max_x16(mx));
-                    if (top > m_lim[t]) {  // (a row's four lanes alike)
-                        const float mz = top * a.zs;
-                        const float alpha = m_lim[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_z[t] - mz);
-                        m_z[t] = mz;
-                        m_lim[t] = top + slack;
+                    if (top > m_lim[t] && (top > ref || m_lim[t] == -INFINITY)) {  // (a row's four lanes alike)
+                        const float alpha = m_lim[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ref - top) * a.zs);
+                        m_ref[t] = ref = top;
+                        m_lim[t] = __builtin_fabsf(top * a.zs) > FAR_REF ? -FLT_MAX : top + slack;
                         l[t] *= alpha;
 #pragma unroll
                         for (int dt = 0; dt < DT; ++dt) acc[t][dt] *= alpha;
                     }
+                    if (__builtin_amdgcn_ballot_w64(m_lim[t] == -FLT_MAX) != 0) {  // (uniform)
+                        const float less = m_lim[t] == -FLT_MAX ? ref : 0.f;
+                        ref -= less;
+#pragma unroll
+                        for (int x = 0; x < SUB; ++x)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) st[x][t][h] -= less;
+                    }
                 }
-                const float sub = m_z[t] - E::SHIFT;
+                const float sub = fmaf(ref, a.zs, -E::SHIFT);
 #pragma unroll
                 for (int x = 0; x < SUB; ++x)
 #pragma unroll
@@ -792,7 +807,7 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
 #pragma unroll
             for (int t = 0; t < TPW; ++t) {
                 const int r = (rw * TPW + t) * 16 + c16;
-                const float sl = sum_x32(sum_x16(l[t])), M = m_lim[t] == -INFINITY ? -INFINITY : m_z[t];
+                const float sl = sum_x32(sum_x16(l[t])), M = m_lim[t] == -INFINITY ? -INFINITY : m_ref[t] * a.zs;
                 if (r >= rows) continue;
                 const int s = s_first + r / a.G, h = kh * a.G + r % a.G;
 #pragma unroll
@@ -806,7 +821,7 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
                 for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(mo + 16 * dt) = acc[t][dt];
                 const float sl = sum_x32(sum_x16(l[t]));
                 if (g == 0) {
-                    lm[(rw * P + part) * 16 + c16] = m_lim[t] == -INFINITY ? -INFINITY : m_z[t];
+                    lm[(rw * P + part) * 16 + c16] = m_lim[t] == -INFINITY ? -INFINITY : m_ref[t] * a.zs;
                     lm[RTW * P * 16 + (rw * P + part) * 16 + c16] = sl;
                 }
                 __syncthreads();

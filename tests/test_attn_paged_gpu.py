@@ -335,3 +335,36 @@ def test_values_that_some_rows_attend(C, dev, H, Hk, D, S, tree):
     assert hit.any() and (got[hit] == float("-inf")).all() and got[~hit].isfinite().all()
     want = C.attn_paged(a[0], a[1], clean.to(dev), *a[3:]).cpu()
     check(torch.where(hit, want, got), BF, q, key, clean, table, lens, mask, D ** -0.5)
+
+
+@pytest.mark.parametrize("dt,top", [(BF, 2.0 ** 18), (BF, 2.0 ** 33), (BF, 2.0 ** 62), (BF, 2.0 ** 90), (FH, 2.0 ** 18), (FH, 2.0 ** 28)])
+@pytest.mark.parametrize("H,Hk,D,S,width", [(8, 2, 128, 1, 1), (8, 4, 64, 3, 6000), (4, 1, 256, 5, 1), (8, 2, 128, 40, 1), (4, 2, 256, 70, 6000)])
+def test_scores_past_the_accuracy_of_their_exponent(C, dev, dt, top, H, Hk, D, S, width):
+    """Scores of up to `top` whose product with scale log2(e) no fp32 number holds to a few units: one token takes the row, or
+    several equal ones share it. The scores are exact in fp32 (two dims of 16 powers of two times integers below 256), an integer
+    apart at least top / 2^9 before the scale, so every other weight is 0 in fp32 and the result is the token's value, or the mean
+    of the sharing tokens' (each weight 1 / count and their sum exact but for fp32, one rounding to the type)."""
+    print(f"large scores: {dt} top={top} H={H} Hk={Hk} D={D} S={S} width={width}", flush=True)
+    g = torch.Generator().manual_seed(D + S)
+    lens, T = [300, 33, 700], 32
+    key, value, table = cache(g, dt, Hk, T, D, lens, S, junk=0.0, width=width)
+    half = (top / 2 ** 12) ** 0.5  # 16 dims of q times k, integers to 255: 2^12 half^2
+    a = 2.0 ** int(torch.tensor(half).log2().floor())
+    b = 2.0 ** int(torch.tensor(top / 2 ** 12 / a).log2().floor())
+    key[:] = 0
+    q = torch.zeros(3, S, H, D, dtype=dt)
+    q[..., 3:19] = a
+    worth = []
+    for i, m in enumerate(lens):
+        w = torch.randint(-255, 200 if i < 2 else -20, (Hk, m + S), generator=g)
+        w[:, m // 2] = w[:, m - 1] = 230 if i < 2 else -3  # two tokens above all others (the third sequence's scores are all negative)
+        t = torch.arange(m + S)
+        key[:, table[i, t // T].long(), t % T, 3:19] = (w[..., None] * b).to(dt)
+        worth.append(w)
+    for scale in (D ** -0.5, 0.31, 0.0137):
+        got = C.attn_paged(q.to(dev), key.to(dev), value.to(dev), table.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev), scale=scale).cpu().double()
+        for i, m in enumerate(lens):
+            at = torch.tensor([m // 2, m - 1])
+            v = value[:, table[i, at // T].long(), at % T].double().mean(1)  # [Hk, D]
+            want = v.repeat_interleave(H // Hk, 0).expand(S, H, D)
+            assert ((got[i] - want).abs() <= (torch.finfo(dt).eps / 2 + 2.0 ** -20) * want.abs() + 2.0 ** -24).all(), (scale, i, got[i][0, 0, :4], want[0, 0, :4])
