@@ -113,13 +113,13 @@ __device__ void fork_rows(const ForkArgs& a, int i, int t, int nt) {
     const int full = n >> a.lt, used = (n + a.T - 1) >> a.lt, total = int((int64_t(n) + a.room + a.T - 1) >> a.lt);
     int32_t* row = a.rows + int64_t(i) * a.W;
     if (s == d) {
-        // (its missing entries in order: the whole row by the first wave, a ballot per 64 entries)
+        // (its missing entries, -1 or otherwise no page, in order: the whole row by the first wave, a ballot per 64 entries)
         if (t >= 64) return;
         int given = p.z;
         for (int j0 = 0; j0 < a.W; j0 += 64) {
             const int j = j0 + t;
             int e = j < a.W ? a.table[d * a.ts + j] : -1;
-            const bool miss = j < a.W && j >= full && j < total && e < 0;
+            const bool miss = j < a.W && j >= full && j < total && uint32_t(e) >= uint32_t(a.P);
             const uint64_t m = __builtin_amdgcn_ballot_w64(miss);
             if (miss) {
                 e = a.fresh[given + __popcll(m & ((uint64_t(1) << t) - 1))];
@@ -170,7 +170,7 @@ __global__ __launch_bounds__(PLAN_T) void fork_plan_kernel(ForkArgs a, int rows)
         if (total > a.W) {
             valid = false;
         } else if (s == d) {  // a sequence that stays: only the pages of its room
-            for (int j = full; j < int(total); ++j) need += a.table[d * a.ts + j] < 0;
+            for (int j = full; j < int(total); ++j) need += uint32_t(a.table[d * a.ts + j]) >= uint32_t(a.P);
         } else {
             need = int(total) - (a.share ? full : 0);
             copies = a.share ? used - full : used;

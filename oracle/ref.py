@@ -1031,7 +1031,7 @@ def page_fork(kv, ksum, table, length, refs, dst, src, room, share):
         seen.add(d)
         full, used = n // T, -(-n // T)
         kept = W if s == d else full if share else 0
-        places = [j for j in range(full, total) if table[d, j] < 0] if s == d else list(range(kept, total))
+        places = [j for j in range(full, total) if not 0 <= table[d, j] < len(refs)] if s == d else list(range(kept, total))
         wanted += len(places)
         if wanted > len(free):
             status.append(0)

@@ -83,6 +83,15 @@ def test_fork_and_commit_by_hand():
     assert st.tolist() == [1, -1] and n5.tolist() == [21, 20]
 
 
+def test_a_kept_sequence_gets_pages_for_entries_that_are_none():
+    """dst == src: an entry past the pool is no page, as one below 0 is none: both are given a page, and the slots lie in the cache."""
+    kv, ksum = np.zeros((1, 2, 1, 6, 16, 1)), np.zeros((1, 1, 6, 1))
+    table = np.array([[4, 9, -3, 2 ** 31 - 1]])
+    *_, t2, n2, r2, st, sl = ref.page_fork(kv, ksum, table, np.array([16]), np.array([0, 1, 0, 0, 1, 0]), [0], [0], 20, True)
+    assert st.tolist() == [1] and t2.tolist() == [[4, 0, 2, 2 ** 31 - 1]] and r2.tolist() == [1, 1, 1, 0, 1, 0]
+    assert sl[0].tolist() == list(range(16)) + [32, 33, 34, 35]
+
+
 # ---- refusals --------------------------------------------------------------------------------------
 @pytest.mark.skipif(not os.path.exists(os.path.join(PKG, "mdx", "libmdx.so")), reason="libmdx.so not built")
 def test_refusals_before_any_device_work():

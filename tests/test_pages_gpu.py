@@ -295,3 +295,17 @@ def test_fork_replay(C, dev, share):
         want = C.page_fork(*e, dst, src, 5, share, slots_e)
         for a, b in zip(d + [slots, status], e + [slots_e, want]):
             assert torch.equal(a.view(torch.int16) if a.dtype == torch.bfloat16 else a, b.view(torch.int16) if b.dtype == torch.bfloat16 else b), k
+
+
+@pytest.mark.parametrize("past", [40, 41, 99, 2 ** 31 - 1])
+def test_fork_kept_sequence_with_entries_past_the_pool(C, dev, past):
+    """dst == src: entries that are no page are given one like missing ones, and every slot lies inside the cache."""
+    st = State(31, [20, 37, 5], P=40, held=2, W=8)
+    st.table[0, 3], st.table[1, 4], st.table[2, 1], st.table[2, 2] = past, past, past, -9
+    assert _fork(C, dev, st, [0, 1, 2], [0, 1, 2], 60) == [1, 1, 1]
+    d = st.dev(dev)
+    slots = torch.empty(3, 60, dtype=torch.int64, device=dev)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    C.page_fork(*d, i32([0, 1, 2]), i32([0, 1, 2]), 60, True, slots)
+    assert (slots >= 0).all() and (slots < 40 * 16).all()
+    assert int((d[4] > 0).sum()) == 2 + 3 + 1 + (5 - 2) + (7 - 3) + (5 - 1)
