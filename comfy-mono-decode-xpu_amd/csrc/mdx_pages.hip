@@ -470,7 +470,7 @@ __device__ void commit_plan(const CommitArgs& a) {
         have = free_pages(a.refs, a.P, want, a.fresh, tmp);
         __syncthreads();  // (the list, written by other threads)
     }
-    const bool served = valid && upto <= have;
+    const bool served = valid && (need == 0 || upto <= have);
     if (served && need && !wide) {
         int at = upto - need;
         for (int j = j1; j < j2; ++j)

@@ -1318,8 +1318,10 @@ def page_commit(kv, ksum, table, length, refs, count, path=None, room=0, new_len
     the pages that fill up are taken (ksum not None), and missing pages for `room` more tokens are given (the lowest free
     ones, in the sequences' order). slots (int64 [B, room], optional): the cache rows page * T + row of the next tokens (the
     positions that qk_norm_rope_kv writes in a [1, Hk, P * T, D] view of a layer), -1 where there is no page. count[b] < 0:
-    the sequence is left alone (status 1). Returns int32 [B]: 1 done, 0 committed but not all of the room given, -1 refused
-    (a path out of order or range, rows without pages, a length past the table): nothing of that sequence moves or grows.
+    the sequence is left alone (status 1). Returns int32 [B]: 1 done, 0 committed but not all of the room given (too few free
+    pages for this sequence with those before it: none are given; or room past the table's width), -1 refused (a path out of
+    order or range, rows without pages, a length past the table): nothing of that sequence moves or grows. A sequence that
+    needs no page is done whatever the others need.
     The move of mtp_accept (csrc/mtp_loop.sycl:160-196 of the reference) over pages, for a batch."""
     return (_bind or _bound()).page_commit(kv, ksum, table, length, refs, count, path, room, new_length, slots)
 

@@ -608,9 +608,9 @@ int mdx_page_fork(void* kv, void* ksum, int64_t L, int64_t Hk, int64_t P, int64_
  * [B][R], strictly ascending in 0..R - 1, R <= 64; NULL: nothing moves), new_length[b] = length[b] + count[b] (length
  * itself or apart from it), the mean keys of the pages that fill are written (ksum, fp32 sums), missing pages up to
  * `room` more tokens are given (lowest free first, in sequence order), slots int64 [B][room] (may be NULL) as above.
- * count[b] < 0: left alone. status int32 [B]: 1 done; 0 committed, room not all given; -1 refused (bad path, rows
- * without pages, past the table): that sequence stays (the mean keys of its pages past its length may have been
- * written). Replaces, over pages and for a batch, the KV move of _C.mtp_accept (csrc/mtp_loop.sycl:160-196). dtype
+ * count[b] < 0: left alone. status int32 [B]: 1 done; 0 committed, room not all given (too few free pages for the
+ * sequences up to this one, if it needs any: none are given; or room past the table); -1 refused (bad path, rows without
+ * pages, past the table): that sequence stays (the mean keys of its pages past its length may have been written). Replaces, over pages and for a batch, the KV move of _C.mtp_accept (csrc/mtp_loop.sycl:160-196). dtype
  * MDX_DT_BF16 or MDX_DT_F16; D in {64, 128, 256}. */
 size_t mdx_page_commit_workspace(int64_t B, int64_t W);
 int mdx_page_commit(void* kv, void* ksum, int32_t dtype, int64_t L, int64_t Hk, int64_t P, int64_t T, int64_t D,

@@ -1095,7 +1095,7 @@ def page_commit(kv, table, length, refs, count, path, room):
         last = -(-(n + c + room) // T)
         need = [j for j in range(-(-(n + c) // T), min(last, W)) if not 0 <= table[b, j] < P]
         wanted += len(need)
-        status[b] = 1 if wanted <= len(free) and last <= W else 0
+        status[b] = 1 if (not need or wanted <= len(free)) and last <= W else 0
         if wanted <= len(free):
             for j, e in zip(need, free[wanted - len(need):wanted]):
                 table[b, j] = e

@@ -92,6 +92,17 @@ def test_a_kept_sequence_gets_pages_for_entries_that_are_none():
     assert sl[0].tolist() == list(range(16)) + [32, 33, 34, 35]
 
 
+def test_a_commit_that_needs_no_page_is_done_whatever_the_others_need():
+    """One free page; 17 more tokens take the first sequence two, the second none, the third one: only the second has all its room."""
+    kv = np.zeros((1, 2, 1, 6, 16, 1))
+    table = np.array([[0, -1, -1, -1], [1, 2, 4, -1], [3, -1, -1, -1]])
+    refs = np.array([1, 1, 1, 1, 1, 0])
+    _, t2, n2, _, st, sl, _ = ref.page_commit(kv, table, np.array([10, 16, 14]), refs, [6, 2, 1], None, 17)
+    assert st.tolist() == [0, 1, 0] and n2.tolist() == [16, 18, 15] and (t2 == table).all() and (sl[1] >= 0).all()
+    _, t2, _, _, st, _, _ = ref.page_commit(kv, table, np.array([10, 16, 14]), refs, [-1, 2, 1], None, 17)
+    assert st.tolist() == [1, 1, 1] and t2[2].tolist() == [3, 5, -1, -1]
+
+
 # ---- refusals --------------------------------------------------------------------------------------
 @pytest.mark.skipif(not os.path.exists(os.path.join(PKG, "mdx", "libmdx.so")), reason="libmdx.so not built")
 def test_refusals_before_any_device_work():

@@ -309,3 +309,17 @@ def test_fork_kept_sequence_with_entries_past_the_pool(C, dev, past):
     C.page_fork(*d, i32([0, 1, 2]), i32([0, 1, 2]), 60, True, slots)
     assert (slots >= 0).all() and (slots < 40 * 16).all()
     assert int((d[4] > 0).sum()) == 2 + 3 + 1 + (5 - 2) + (7 - 3) + (5 - 1)
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("path", [None, [[0, 1, 2, 3]] * 5])
+def test_commit_of_sequences_that_need_no_page_beside_starved_ones(C, dev, in_place, path):
+    """Status 0 is for sequences whose own room is not all given: not for those behind them that have all their pages."""
+    st = State(33, [14, 30, 0, 40, 8], P=10, held=4, W=6)
+    assert int((st.refs == 0).sum()) == 0
+    assert _commit(C, dev, st, [2, 2, 1, 3, 4], path, 4, in_place) == [1, 1, 1, 1, 1]
+    st = State(34, [14, 30, 0, 40, 8], P=12, held=4, W=6)
+    st.table[2, 1] = int((st.refs == 0).nonzero()[0])
+    st.refs[st.table[2, 1].long()] = 1  # (the third sequence has its pages; one is free for the other four)
+    assert _commit(C, dev, st, [2, 2, 1, 3, 4], path, 17, in_place) == [1, 0, 1, 0, 0]
+    assert _commit(C, dev, st, [2, 0, 1, 3, -1], path, 17, in_place) == [1, 1, 1, 0, 1]
