@@ -182,7 +182,7 @@ __global__ __launch_bounds__(PLAN_T) void fork_plan_kernel(ForkArgs a, int rows)
         upto = block_sum_incl(need, tmp, want);
         have = free_pages(a.refs, a.P, want, a.fresh, tmp);
     }
-    const bool served = valid && upto <= have;
+    const bool served = valid && (need == 0 || upto <= have);  // (a drop frees pages: it waits for none)
     if (__syncthreads_or(served ? copies : 0)) cend = block_sum_incl(served ? copies : 0, tmp, all);
     if (i < a.M) {
         reinterpret_cast<int4*>(a.pair)[i] = make_int4(valid ? (served ? 1 : 0) : -1, n, upto - need, cend - copies);

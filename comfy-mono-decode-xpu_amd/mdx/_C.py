@@ -1306,7 +1306,8 @@ def page_fork(kv, ksum, table, length, refs, dst, src, room=0, share=True, slots
     pages are the lowest free ones, in the pairs' order, and pages given back by this call are free for the next.
     slots (int64 [pairs, room], optional): the cache rows page * T + row of its next tokens, -1 where there is no page.
     Returns int32 [pairs]: 1 done, 0 too few free pages (for this pair with those before it), -1 refused (a place outside the
-    table or named twice, a length and room past the table's width); pairs that are not done change nothing.
+    table or named twice, a length and room past the table's width); pairs that are not done change nothing. A pair that
+    needs no page (a drop) is done whatever the others need.
     No counterpart in the reference (one sequence, one contiguous cache)."""
     return (_bind or _bound()).page_fork(kv, ksum, table, length, refs, dst, src, room, share, slots)
 

@@ -596,8 +596,9 @@ int mdx_gdn_run(const uint16_t* proj, const uint16_t* xn, const uint16_t* wa, co
  * with share, src's full pages are named by dst too and the page its length ends in is copied; without, every page (and
  * mean key) is copied. dst[i] == src[i]: only the room is given. Fresh pages are the lowest free ones, in pair order;
  * pages that dst gives back are free from the next call on. slots int64 [pairs][room] (may be NULL): page * T + row of
- * the next tokens, or -1. status int32 [pairs]: 1 done; 0 too few free pages for the pairs up to this one; -1 refused (dst
- * outside 0..B - 1 or named by an earlier pair, src >= B, tokens and room past W pages). Pairs not done change nothing. */
+ * the next tokens, or -1. status int32 [pairs]: 1 done; 0 too few free pages for the pairs up to this one (if it
+ * needs any: a drop is always done); -1 refused (dst outside 0..B - 1 or named by an earlier pair, src >= B, tokens and room
+ * past W pages). Pairs not done change nothing. */
 size_t mdx_page_fork_workspace(int64_t pairs, int64_t W);
 int mdx_page_fork(void* kv, void* ksum, int64_t L, int64_t Hk, int64_t P, int64_t T, int64_t D, int32_t* table,
                   int64_t table_stride, int64_t B, int64_t W, int32_t* length, int32_t* refs, const int32_t* dst,

@@ -1033,7 +1033,7 @@ def page_fork(kv, ksum, table, length, refs, dst, src, room, share):
         kept = W if s == d else full if share else 0
         places = [j for j in range(full, total) if not 0 <= table[d, j] < len(refs)] if s == d else list(range(kept, total))
         wanted += len(places)
-        if wanted > len(free):
+        if places and wanted > len(free):
             status.append(0)
             slots.append([-1] * room)
             continue

@@ -103,6 +103,17 @@ def test_a_commit_that_needs_no_page_is_done_whatever_the_others_need():
     assert st.tolist() == [1, 1, 1] and t2[2].tolist() == [3, 5, -1, -1]
 
 
+def test_a_drop_behind_a_starved_pair_is_done():
+    """A pair that needs no page (a drop, a share without a tail, a sequence that has its room) is done where others find too few;
+    the pages it gives back serve the next call."""
+    kv, ksum = np.zeros((1, 2, 1, 5, 16, 1)), np.zeros((1, 1, 5, 1))
+    table = np.array([[0, 1], [2, 3], [-1, -1], [-1, -1], [4, -1]])
+    length, refs = np.array([20, 32, 0, 0, 3]), np.ones(5, dtype=np.int64)
+    _, _, t2, n2, r2, st, _ = ref.page_fork(kv, ksum, table, length, refs, [2, 0, 3, 4, 1], [0, -1, 1, 4, 4], 0, True)
+    assert st.tolist() == [0, 1, 1, 1, 0] and n2.tolist() == [0, 32, 0, 32, 3]
+    assert t2.tolist() == [[-1, -1], [2, 3], [-1, -1], [2, 3], [4, -1]] and r2.tolist() == [0, 0, 2, 2, 1]
+
+
 # ---- refusals --------------------------------------------------------------------------------------
 @pytest.mark.skipif(not os.path.exists(os.path.join(PKG, "mdx", "libmdx.so")), reason="libmdx.so not built")
 def test_refusals_before_any_device_work():

@@ -323,3 +323,16 @@ def test_commit_of_sequences_that_need_no_page_beside_starved_ones(C, dev, in_pl
     st.refs[st.table[2, 1].long()] = 1  # (the third sequence has its pages; one is free for the other four)
     assert _commit(C, dev, st, [2, 2, 1, 3, 4], path, 17, in_place) == [1, 0, 1, 0, 0]
     assert _commit(C, dev, st, [2, 0, 1, 3, -1], path, 17, in_place) == [1, 1, 1, 0, 1]
+
+
+def test_fork_pairs_that_need_no_page_beside_starved_ones(C, dev):
+    """Drops, shares of full pages and sequences that stay are done where pairs in front of them find too few pages."""
+    st = State(35, [20, 32, 0, 0, 3], P=5, W=4)
+    assert int((st.refs == 0).sum()) == 0
+    assert _fork(C, dev, st, [2, 0, 3, 4, 1], [0, -1, 1, 4, 4], 0) == [0, 1, 1, 1, 0]
+    assert _fork(C, dev, st, [2, 0, 3, 4, 1], [0, -1, 1, 4, -1], 0, False) == [0, 1, 0, 1, 1]
+    lens = [20 + i % 29 for i in range(400)]
+    st = State(36, lens, P=sum(-(-n // 16) for n in lens) + 40, W=3, L=1, Hk=1, D=8)  # (40 free pages for some 130 copies)
+    pairs = [(200 + i, i if i % 3 else -1) for i in range(200)]
+    done = _fork(C, dev, st, [d for d, _ in pairs], [s for _, s in pairs], 0)
+    assert all(x == 1 for x, (_, s) in zip(done, pairs) if s < 0) and 0 in done
