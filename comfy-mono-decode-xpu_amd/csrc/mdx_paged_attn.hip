@@ -115,6 +115,9 @@ constexpr int STEP = 32;
 // from 2^32: NaN for finite inputs).
 constexpr float FAR_REF = 65536.f;
 constexpr int CUS = 256;
+// Steps of all units together, with their fixed cost: positions are 32-bit numbers, and the last shares' ends pass the line's by
+// up to one step for each of 2 CUS shares.
+constexpr int64_t MAX_LINE = (int64_t(1) << 31) - 4 * CUS;
 constexpr int RING_BYTES = 128 * 1024;  // of a CU's work-groups together
 // 128-token steps of a call at most, for the forms that go by latency (below: launch_rows)
 constexpr int64_t FEW_STEPS = 2048;
@@ -1426,7 +1429,7 @@ extern "C" int mdx_attn_paged(const void* q, int64_t q_seq_stride, int64_t q_row
     if (rc != MDX_OK) return rc;
     MDX_CHECK(H / Hk <= 128, "at most 128 query heads per kv head");
     const int64_t rows = S * (H / Hk), blocks = blocks_of(S, H / Hk);
-    MDX_CHECK(rows < (int64_t(1) << 30) && B * Hk * blocks < (int64_t(1) << 30) && B * Hk * blocks * ((W * T + S) / STEP + 8) < (int64_t(1) << 31),
+    MDX_CHECK(rows < (int64_t(1) << 30) && B * Hk * blocks < (int64_t(1) << 30) && B * Hk * blocks * ((W * T + S) / STEP + 8) < MAX_LINE,
               "too many rows times tokens for one call");
     a.whole = whole_units(B, S, H, Hk, T, W);
     MDX_CHECK(a.whole || (workspace && aligned(workspace, 16) && workspace_bytes >= base_bytes(rows, D)),
@@ -1465,7 +1468,7 @@ extern "C" int mdx_attn_blocks(const void* q, int64_t q_seq_stride, int64_t q_ro
     const int64_t most = blocks + sink + local, units = B * S * Hk;
     MDX_CHECK(H / Hk <= 64, "at most 64 query heads per kv head");
     MDX_CHECK(W <= 65536, "at most 65536 pages a sequence");
-    MDX_CHECK(B * Hk <= 65535 && units < (int64_t(1) << 24) && units * (((most < W ? most : W) + 1) * T + S) / STEP + 8 * units < (int64_t(1) << 31),
+    MDX_CHECK(B * Hk <= 65535 && units < (int64_t(1) << 24) && units * (((most < W ? most : W) + 1) * T + S) / STEP + 8 * units < MAX_LINE,
               "too many rows times tokens for one call");
     const size_t need = mdx_attn_blocks_workspace(B, S, H, Hk, D, W, most);
     MDX_CHECK(workspace && aligned(workspace, 16) && workspace_bytes >= need, "workspace: %zu bytes, 16-byte aligned", need);

@@ -158,6 +158,20 @@ def test_refusals_before_any_device_work():
         assert _lib.lib().mdx_last_error(), (f.__name__, kw)
 
 
+@pytest.mark.skipif(not os.path.exists(os.path.join(PKG, "mdx", "libmdx.so")), reason="libmdx.so not built")
+def test_a_line_of_steps_that_nearly_fills_32_bits_is_refused():
+    """64 units of 2^30 - 288 tokens are 2^31 - 192 steps of 32 with their fixed cost; of 256 shares the last begins at 255 * 2^23 and
+    its end, 2^31, is no 32-bit number."""
+    from mdx import _lib
+    A, tokens = 1 << 12, (1 << 30) - 288
+    steps = 64 * (-(-(tokens + 1) // 32) + 5)
+    share = -(-steps // 256)
+    assert steps == (1 << 31) - 192 and 256 * share >= 1 << 31
+    rc = _lib.lib().mdx_attn_paged(A, 80 * 256, 80 * 256, 256, A, 1 << 20, 4096, 256, A, 1 << 20, 4096, 256, _lib.DT_BF16, A, tokens // 16, A, None,
+                                   1 << 44, 64, 1, 80, 1, 256, 8, 16, tokens // 16, 0.1, A, 1 << 40, None)
+    assert rc == _lib.MDX_EINVAL and b"too many" in _lib.lib().mdx_last_error()
+
+
 def test_host_tensors_are_refused():
     from mdx import _C
     z = torch.zeros
