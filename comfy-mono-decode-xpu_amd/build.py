@@ -74,14 +74,21 @@ def build(jobs: int | None = None, verbose: bool = False) -> str:
         with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
             bind = ex.submit(_bind, BIND_OUT + ".tmp")
             list(ex.map(lambda so: _compile(cc, *so), zip(srcs, objs)))
-            bind.result()
         tmp_out = OUT + ".tmp"
         cmd = [cc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", tmp_out]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
         os.replace(tmp_out, OUT)
-        os.replace(BIND_OUT + ".tmp", BIND_OUT)
+    # The library is whole without the binding, which needs a host compiler and torch's headers; without it the paged cache's
+    # calls raise (mdx._lib.bind), and an older one does not stay beside a newer library.
+    try:
+        bind.result()
+    except Exception as e:
+        if os.path.exists(BIND_OUT):
+            os.remove(BIND_OUT)
+        raise RuntimeError(f"{OUT} is built, {os.path.basename(BIND_OUT)} is not: {e}") from e
+    os.replace(BIND_OUT + ".tmp", BIND_OUT)
     if verbose:
         print(f"built {OUT} from {len(srcs)} sources, {BIND_OUT}")
     return OUT
