@@ -48,13 +48,16 @@ def _bind(tmp_out):
     import torch
     root = os.path.dirname(torch.__file__)
     rocm = os.path.dirname(os.path.dirname(os.path.realpath(hipcc())))
-    cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I" + sysconfig.get_paths()["include"],
-           f"-I{root}/include", f"-I{root}/include/torch/csrc/api/include", f"-I{rocm}/include", BIND, "-o", tmp_out, f"-L{root}/lib",
+    cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(x for d in (sysconfig.get_paths()["include"], f"{root}/include", f"{root}/include/torch/csrc/api/include", f"{rocm}/include")
+             for x in ("-isystem", d)), BIND, "-o", tmp_out, f"-L{root}/lib",
            "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    if r.stderr:
+        print(r.stderr, file=sys.stderr)  # (warnings)
 
 
 def _compile(cc, src, obj):

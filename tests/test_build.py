@@ -56,3 +56,13 @@ def test_a_kernel_that_does_not_compile_leaves_both(built):
     with pytest.raises(RuntimeError, match="compile failed"):
         mod.build()
     assert (out / "libmdx.so").read_text() == "old"
+
+
+def test_the_binding_is_compiled_with_warnings(built, monkeypatch):
+    mod, _, out = built
+    seen = []
+    inner = mod.subprocess.run
+    monkeypatch.setattr(mod.subprocess, "run", lambda cmd, **kw: (seen.append(cmd), inner(cmd, **kw))[1])
+    mod.build()
+    bind = [c for c in seen if any("mdx_bind.cpp" in x for x in c)]
+    assert len(bind) == 1 and "-w" not in bind[0] and "-Wall" in bind[0]
