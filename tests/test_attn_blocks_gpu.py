@@ -250,3 +250,13 @@ def test_a_run_of_the_operators_together(C, dev):
                 assert (at - mean).abs().max() <= 2.0 ** -7 * mean.abs().max()
     C.page_fork(kv, ksum, table, length, refs, i32([0, 1, 2, 3]), i32([-1] * 4))
     assert (refs == 0).all() and (table == -1).all()
+
+
+@pytest.mark.parametrize("H,Hk,D,S", [(8, 2, 128, 5), (16, 4, 256, 8), (8, 4, 64, 17), (16, 8, 64, 3)])
+def test_trees_fp16(C, dev, H, Hk, D, S):
+    """Scores of several rows from fp16 mean keys, selections and attention of each row."""
+    _run(C, dev, FH, H, Hk, D, 16, [30 * 16 + 3, 0, 9 * 16, 700], S, True, 5, 1, 2, 14)
+
+
+def test_chain_rows_fp16(C, dev):
+    _run(C, dev, FH, 8, 2, 128, 32, [700, 40], 6, False, 3, 1, 1, 15)

@@ -368,3 +368,43 @@ def test_scores_past_the_accuracy_of_their_exponent(C, dev, dt, top, H, Hk, D, S
             v = value[:, table[i, at // T].long(), at % T].double().mean(1)  # [Hk, D]
             want = v.repeat_interleave(H // Hk, 0).expand(S, H, D)
             assert ((got[i] - want).abs() <= (torch.finfo(dt).eps / 2 + 2.0 ** -20) * want.abs() + 2.0 ** -24).all(), (scale, i, got[i][0, 0, :4], want[0, 0, :4])
+
+
+def _sampled(C, dev, dt, H, Hk, D, T, lens, S, width, rows, seed=0):
+    """A chain of S rows, checked at some rows: row s is a single token behind length + s tokens."""
+    print(f"attn_paged {dt} H={H} Hk={Hk} D={D} T={T} lens={lens} S={S} width={width}", flush=True)
+    g = torch.Generator().manual_seed(seed + D + S)
+    key, value, table = cache(g, dt, Hk, T, D, lens, S, width=width)
+    q = (torch.randn(len(lens), S, H, D, generator=g) * 1.5).to(dt)
+    got = C.attn_paged(q.to(dev), key.to(dev), value.to(dev), table.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev)).cpu()
+    assert got.isfinite().all()
+    for s in rows:
+        check(got[:, s:s + 1], dt, q[:, s:s + 1], key, value, table, [n + s for n in lens], None, D ** -0.5)
+
+
+@pytest.mark.parametrize("dt", [BF, FH])
+@pytest.mark.parametrize("H,Hk,D,S,lens,width", [(32, 32, 64, 2085, [70], 1), (32, 8, 128, 2048, [100], 1), (32, 8, 128, 700, [90, 0, 333], 1), (32, 8, 128, 671, [90, 0, 333], 1),
+                                                 (16, 4, 256, 1000, [33, 500], 1), (16, 4, 256, 991, [33, 500], 1), (20, 4, 128, 770, [40, 8, 900, 123], 1), (32, 8, 64, 600, [5] * 8, 50)])
+def test_whole_units_of_many_rows(C, dev, dt, H, Hk, D, S, lens, width):
+    """Row blocks enough for every work-group (512 at two per CU, 256 at head_dim 256) and just fewer; counts of rows that are no
+    multiple of a block's; unequal sequences; the rows at a block's ends and in the last one."""
+    spb = 128 // (H // Hk)
+    _sampled(C, dev, dt, H, Hk, D, 32, lens, S, width, sorted({0, spb - 1, spb, S // 2, (S - 1) // spb * spb - 1, (S - 1) // spb * spb, S - 1}))
+
+
+@pytest.mark.parametrize("H,Hk,D,S,lens", [(32, 8, 128, 65, [0, 40]), (8, 4, 64, 200, [0, 77]), (4, 1, 256, 130, [7, 64]), (8, 8, 128, 2, [100, 31])])
+def test_chains_fp16(C, dev, H, Hk, D, S, lens):
+    _run(C, dev, FH, H, Hk, D, 32, lens, S, False, 5)
+
+
+@pytest.mark.parametrize("width", [1, 4000])
+def test_lengths_out_of_range_are_clamped(C, dev, width):
+    """Below 0: no committed token. Past the table: all that it holds; the rows' own have no place there."""
+    g, q, key, value, table, _, _, mask = _small(dev, lens=(44, 44, 44, 12))
+    table = torch.nn.functional.pad(table[:, :3], (0, width - 1), value=-1)
+    W = table.shape[1]
+    n = [-5, 2 ** 31 - 1, W * 16 + 1, -2 ** 31]
+    got = C.attn_paged(q.to(dev), key.to(dev), value.to(dev), table.to(dev), torch.tensor(n, dtype=torch.int32, device=dev), mask.to(dev))
+    # (own rows of sequences 0 and 3 stand at tokens 0..3; sequences 1 and 2 have 44 + 4 tokens in their pages)
+    check(got, BF, q, key, value, table, [min(max(x, 0), W * 16) for x in n], mask, 128 ** -0.5)
+    assert (got != 0).any(-1).all()
