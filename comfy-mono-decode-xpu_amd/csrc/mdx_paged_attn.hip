@@ -121,6 +121,8 @@ constexpr int64_t MAX_LINE = (int64_t(1) << 31) - 4 * CUS;
 constexpr int RING_BYTES = 128 * 1024;  // of a CU's work-groups together
 // 128-token steps of a call at most, for the forms that go by latency (below: launch_rows)
 constexpr int64_t FEW_STEPS = 2048;
+// The forms go by what the table could hold, the lengths being on the device alone; a caller with a bound on them passes a table
+// of fewer columns (all rules measured with tables as wide as the lengths).
 // Tokens a unit can have at most, for one work-group per unit: 8 units of one token over 500: 9.4 us a call, 12.6 in shares
 // with their join; of 16 rows over 500: 15.5 and 13.9, 128 of them 16.5 and 25.3. Twice as many where the units fill half of
 // the CUs and no more than all (128 units of one token over 1000: 15.7 and 20.2, of 16 rows 23.0 and 29.3; 8 units of one

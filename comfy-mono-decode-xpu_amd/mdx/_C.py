@@ -1315,11 +1315,11 @@ def page_fork(kv, ksum, table, length, refs, dst, src, room=0, share=True, slots
 def page_commit(kv, ksum, table, length, refs, count, path=None, room=0, new_length=None, slots=None):
     """The step's rows of every sequence become committed: row length[b] + path[b, k] of the cache moves to length[b] + k for k
     < count[b] (all layers, keys and values; path int32 [B, R] ascending from 0 <= path, R <= 64; None: the rows stand in
-    order already), the length grows by count[b] (into new_length, apart from length; default: in place), the mean keys of
-    the pages that fill up are taken (ksum not None), and missing pages for `room` more tokens are given (the lowest free
-    ones, in the sequences' order). slots (int64 [B, room], optional): the cache rows page * T + row of the next tokens (the
-    positions that qk_norm_rope_kv writes in a [1, Hk, P * T, D] view of a layer), -1 where there is no page. count[b] < 0:
-    the sequence is left alone (status 1). Returns int32 [B]: 1 done, 0 committed but not all of the room given (too few free
+    order already), the length grows by count[b] (into new_length, apart from length: one launch; default: in place, two: 4 to
+    9 us more), the mean keys of the pages that fill up are taken (ksum not None), and missing pages for `room` more tokens
+    are given (the lowest free ones, in the sequences' order). slots (int64 [B, room], optional): the cache rows page * T +
+    row of the next tokens (the positions that qk_norm_rope_kv writes in a [1, Hk, P * T, D] view of a layer), -1 where there
+    is no page. count[b] < 0: the sequence is left alone (status 1). Returns int32 [B]: 1 done, 0 committed but not all of the room given (too few free
     pages for this sequence with those before it: none are given; or room past the table's width), -1 refused (a path out of
     order or range, rows without pages, a length past the table): nothing of that sequence moves or grows. A sequence that
     needs no page is done whatever the others need.
@@ -1334,7 +1334,8 @@ def attn_paged(q, key, value, table, length, mask=None, scale=None, out=None):
     strides of 8 elements), key / value [Hk, P, T, D] views of the cache (kv[layer, 0], kv[layer, 1]; any strides of 8
     elements), table, length as page_commit keeps them. out [B, S, H, D], apart from q; a row that admits nothing is 0.
     Tokens in pages that the table does not have are not attended; what stands in places a row does not attend is never
-    seen. The form of attn_dpas (csrc/attn_dpas.sycl:269-342 of the reference) for a batch, pages, and any rows."""
+    seen. The launches go by what the table could hold: with a bound on the lengths, pass table[:, :pages]. The form of
+    attn_dpas (csrc/attn_dpas.sycl:269-342 of the reference) for a batch, pages, and any rows."""
     return (_bind or _bound()).attn_paged(q, key, value, table, length, mask, scale, out)
 
 
