@@ -260,3 +260,8 @@ def test_trees_fp16(C, dev, H, Hk, D, S):
 
 def test_chain_rows_fp16(C, dev):
     _run(C, dev, FH, 8, 2, 128, 32, [700, 40], 6, False, 3, 1, 1, 15)
+
+
+def test_the_most_pages(C, dev):
+    """A table of 65536 entries (one of them spare), a million tokens in each sequence."""
+    _run(C, dev, BF, 2, 1, 64, 16, [16 * 65534 + 7, 16 * 65533], 1, False, 40, 1, 2, 16)

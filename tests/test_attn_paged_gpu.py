@@ -408,3 +408,16 @@ def test_lengths_out_of_range_are_clamped(C, dev, width):
     # (own rows of sequences 0 and 3 stand at tokens 0..3; sequences 1 and 2 have 44 + 4 tokens in their pages)
     check(got, BF, q, key, value, table, [min(max(x, 0), W * 16) for x in n], mask, 128 ** -0.5)
     assert (got != 0).any(-1).all()
+
+
+@pytest.mark.parametrize("H,Hk,D,T,lens,S", [(1, 1, 64, 1024, [100], 65535), (2, 2, 128, 16, [7], 20001)])
+def test_longest_chains(C, dev, H, Hk, D, T, lens, S):
+    _sampled(C, dev, BF, H, Hk, D, T, lens, S, 1, [0, 127, 128, S // 2, S - 2, S - 1])
+
+
+@pytest.mark.parametrize("D,S,tree", [(64, 1, False), (128, 2, True)])
+def test_the_most_sequences(C, dev, D, S, tree):
+    g = torch.Generator().manual_seed(17)
+    lens = [int(x) for x in torch.randint(0, 40, (1024,), generator=g)]
+    lens[::7] = [0] * len(lens[::7])
+    _run(C, dev, BF, 2, 1, D, 16, lens, S, tree, 17)

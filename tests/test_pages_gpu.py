@@ -336,3 +336,14 @@ def test_fork_pairs_that_need_no_page_beside_starved_ones(C, dev):
     pairs = [(200 + i, i if i % 3 else -1) for i in range(200)]
     done = _fork(C, dev, st, [d for d, _ in pairs], [s for _, s in pairs], 0)
     assert all(x == 1 for x, (_, s) in zip(done, pairs) if s < 0) and 0 in done
+
+
+def test_the_most_pairs_and_sequences(C, dev):
+    """1024 pairs of a fork, 1024 sequences of a commit with paths of 64 rows."""
+    g = torch.Generator().manual_seed(9)
+    lens = [int(x) for x in torch.randint(1, 60, (1024,), generator=g)]
+    st = State(37, lens + [0] * 1024, P=9000, W=5, L=1, Hk=1, D=8)
+    assert _fork(C, dev, st, list(range(1024, 2048)), list(range(1024)), 3) == [1] * 1024
+    st = State(38, lens, P=9000, held=64, W=9, L=1, Hk=1)
+    path = [list(range(i % 3, 64)) + [0] * (i % 3) for i in range(1024)]
+    assert _commit(C, dev, st, [64 - i % 3 for i in range(1024)], path, 3) == [1] * 1024
