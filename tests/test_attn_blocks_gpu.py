@@ -265,3 +265,27 @@ def test_chain_rows_fp16(C, dev):
 def test_the_most_pages(C, dev):
     """A table of 65536 entries (one of them spare), a million tokens in each sequence."""
     _run(C, dev, BF, 2, 1, 64, 16, [16 * 65534 + 7, 16 * 65533], 1, False, 40, 1, 2, 16)
+
+
+@pytest.mark.parametrize("H,Hk,D,T,S", [(8, 2, 64, 16, 5), (8, 2, 128, 64, 4), (16, 4, 256, 32, 8), (64, 1, 64, 16, 3), (40, 2, 128, 16, 3)])
+def test_values_that_some_rows_attend(C, dev, H, Hk, D, T, S):
+    """Infinite values in a page that some selections hold, in the tail and at an own row: in the rows that attend them, no others."""
+    g = torch.Generator().manual_seed(S + D)
+    n = 20 * T + 5
+    key, value, table = cache(g, BF, Hk, T, D, [n], S)
+    q = (torch.randn(1, S, H, D, generator=g) * 1.5).to(BF)
+    mask = torch.tensor([[(1 << s) | 1 for s in range(S)]])
+    ksum = _means(key, table, [n], T, BF)
+    dirty = value.clone()
+    at = {3: (9 * T + T - 1, "page"), 7: (20 * T + 2, "tail"), 11: (n + 1, "own row 1")}  # dim: token
+    for d, (t, _) in at.items():
+        dirty[:, table[0, t // T], t % T, d] = float("inf")
+    call = lambda v: C.attn_blocks(*(x.to(dev) for x in (q, key, v, ksum, table)), torch.tensor([n], dtype=torch.int32, device=dev), 8, 1, 1, mask.to(dev))  # noqa: E731
+    (got, sel), (clean, _) = call(dirty), call(value)
+    got, clean, sel = got.cpu(), clean.cpu(), sel.cpu()
+    hit = torch.zeros(1, S, H, D, dtype=torch.bool)
+    hit[0, :, :, 3] = (sel[0] == 9).any(-1).repeat_interleave(H // Hk, 1)
+    hit[..., 7] = True
+    hit[0, 1, :, 11] = True
+    assert (got[hit] == float("inf")).all() and got[~hit].isfinite().all()
+    assert torch.equal(got[~hit], clean[~hit])

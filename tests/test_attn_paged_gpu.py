@@ -313,13 +313,15 @@ def test_what_no_row_attends_costs_nothing(C, dev, H, Hk, D, T, S, lens, tree):
     assert max(us[1:]) < 2 * us[0], us
 
 
-@pytest.mark.parametrize("H,Hk,D,S,tree", [(8, 2, 128, 6, True), (4, 2, 64, 40, True), (8, 2, 128, 150, False), (4, 1, 256, 200, False), (8, 4, 64, 300, False)])
-def test_values_that_some_rows_attend(C, dev, H, Hk, D, S, tree):
+@pytest.mark.parametrize("H,Hk,D,S,tree,width", [(8, 2, 128, 6, True, 1), (4, 2, 64, 40, True, 1), (8, 2, 128, 150, False, 1), (4, 1, 256, 200, False, 1), (8, 4, 64, 300, False, 1),
+                                                 (16, 8, 64, 30, True, 9000), (16, 8, 64, 30, False, 9000), (32, 8, 128, 16, True, 9000), (8, 2, 128, 8, False, 9000), (16, 4, 256, 16, True, 9000),
+                                                 (8, 2, 256, 4, True, 9000), (8, 4, 64, 3, True, 9000)])
+def test_values_that_some_rows_attend(C, dev, H, Hk, D, S, tree, width):
     """Infinite values at many of the rows' own tokens, far apart: every row that attends one shows it with its sign, no other does."""
-    print(f"values attended by some: H={H} Hk={Hk} D={D} S={S}", flush=True)
+    print(f"values attended by some: H={H} Hk={Hk} D={D} S={S} width={width}", flush=True)
     g = torch.Generator().manual_seed(S)
     lens = [300, 0, 41]
-    key, value, table = cache(g, BF, Hk, 32, D, lens, S)
+    key, value, table = cache(g, BF, Hk, 32, D, lens, S, width=width)
     q = torch.randn(3, S, H, D, generator=g).to(BF)
     mask = tree_masks(g, 3, S) if tree else None
     clean, hit = value.clone(), torch.zeros(3, S, D, dtype=torch.bool)
