@@ -31,7 +31,10 @@ struct Entries {
     decltype(&mdx_attn_paged) paged;
     decltype(&mdx_attn_blocks_workspace) blocks_workspace;
     decltype(&mdx_attn_blocks) blocks;
+    decltype(&mdx_verify_drafts_workspace) verify_workspace;
+    decltype(&mdx_verify_drafts) verify;
 } g;
+constexpr int ENTRIES = 11;
 PyObject* g_error = nullptr;  // _lib.MdxError
 
 struct Refused : std::runtime_error {
@@ -328,11 +331,73 @@ PyObject* attn_blocks(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     });
 }
 
-// init(addresses: nine ints in the order of Entries, error class)
+// ---- a step's answers ----
+// logits, tokens, uniform, draft, parent, temperature -> (count, path, next)
+PyObject* verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    EXPECT(6, "verify_drafts")
+    return guarded([&]() -> PyObject* {
+        const at::Tensor& logits = tensor(a[0], "logits");
+        const c10::Device d = rocm_device(logits);
+        const int32_t dt = logits.scalar_type() == at::kFloat ? MDX_DT_F32 : code_of(logits);
+        check(dt >= 0 && logits.dim() == 3 && logits.size(2) >= 1 && logits.stride(2) == 1,
+              "logits: bf16, fp16 or fp32 [sequences, rows, vocabulary], rows contiguous");
+        const int64_t B = logits.size(0), R = logits.size(1), V = logits.size(2);
+        const at::Tensor &tokens = on(a[1], "tokens", d), &uniform = on(a[2], "uniform", d);
+        check(tokens.scalar_type() == at::kLong && tokens.sizes() == at::IntArrayRef({B, R}) && tokens.is_contiguous(),
+              "tokens: contiguous int64 [sequences, rows]");
+        check(uniform.scalar_type() == at::kDouble && uniform.sizes() == at::IntArrayRef({B, R + 1}) && uniform.is_contiguous(),
+              "uniform: contiguous float64 [sequences, rows + 1]");
+        const void* draft = nullptr;
+        int64_t db = 0, dr = 0;
+        if (given(a[3])) {
+            const at::Tensor& t = on(a[3], "draft", d);
+            check(R >= 1 && t.scalar_type() == logits.scalar_type() && t.sizes() == at::IntArrayRef({B, R - 1, V}) && t.stride(2) == 1,
+                  "draft: [sequences, rows - 1, vocabulary] of the logits' type, rows contiguous");
+            check(!given(a[4]), "drafts with probabilities: a chain (no parents)");
+            if (R > 1) draft = data(t), db = t.stride(0), dr = t.stride(1);
+        }
+        const int32_t* parent = nullptr;
+        if (given(a[4])) {
+            const at::Tensor& t = on(a[4], "parent", d);
+            ints(t, "parent", {B, R});
+            parent = t.data_ptr<int32_t>();
+        }
+        const float* heats = nullptr;
+        double heat = 0;
+        if (THPVariable_Check(a[5])) {
+            const at::Tensor& t = on(a[5], "temperature", d);
+            check(t.scalar_type() == at::kFloat && t.sizes() == at::IntArrayRef({B}) && t.is_contiguous(), "temperature: a number, or contiguous float32 [sequences]");
+            heats = t.data_ptr<float>();
+        } else {
+            heat = PyFloat_AsDouble(a[5]);
+            if (heat == -1.0 && PyErr_Occurred()) throw Refused("");
+        }
+        const auto kind = at::TensorOptions().device(d);
+        at::Tensor count = at::empty({B}, kind.dtype(at::kInt)), path = at::empty({B, R}, kind.dtype(at::kInt)), next = at::empty({B}, kind.dtype(at::kLong));
+        if (B > 0) {
+            const size_t n = g.verify_workspace(B, R, V, draft != nullptr);
+            at::Tensor ws = scratch(n, d);
+            call("mdx_verify_drafts", d, [&](void* st) {
+                return g.verify(data(logits), logits.stride(0), logits.stride(1), draft, db, dr, dt, tokens.data_ptr<int64_t>(), parent,
+                                uniform.data_ptr<double>(), heats, float(heat), count.data_ptr<int32_t>(), path.data_ptr<int32_t>(),
+                                next.data_ptr<int64_t>(), B, R, V, data(ws), n, st);
+            });
+        }
+        PyObject* o[3] = {THPVariable_Wrap(std::move(count)), THPVariable_Wrap(std::move(path)), THPVariable_Wrap(std::move(next))};
+        PyObject* all = o[0] && o[1] && o[2] ? PyTuple_Pack(3, o[0], o[1], o[2]) : nullptr;
+        for (PyObject* x : o) Py_XDECREF(x);
+        return all;
+    });
+}
+
+// init(the entry points' addresses in the order of Entries, error class)
 PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
-    EXPECT(10, "init")
-    void* p[9];
-    for (int i = 0; i < 9; ++i) {
+    if (nargs != ENTRIES + 1) {
+        PyErr_SetString(PyExc_TypeError, "init takes the entry points and the error class");
+        return nullptr;
+    }
+    void* p[ENTRIES];
+    for (int i = 0; i < ENTRIES; ++i) {
         p[i] = PyLong_AsVoidPtr(a[i]);
         if (!p[i]) {
             if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "null entry point");
@@ -349,9 +414,11 @@ PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     g.paged = reinterpret_cast<decltype(g.paged)>(p[i++]);
     g.blocks_workspace = reinterpret_cast<decltype(g.blocks_workspace)>(p[i++]);
     g.blocks = reinterpret_cast<decltype(g.blocks)>(p[i++]);
-    Py_XINCREF(a[9]);
+    g.verify_workspace = reinterpret_cast<decltype(g.verify_workspace)>(p[i++]);
+    g.verify = reinterpret_cast<decltype(g.verify)>(p[i++]);
+    Py_XINCREF(a[ENTRIES]);
     Py_XDECREF(g_error);
-    g_error = a[9];
+    g_error = a[ENTRIES];
     Py_RETURN_NONE;
 }
 
@@ -361,6 +428,7 @@ PyMethodDef methods[] = {{"init", FAST(init), METH_FASTCALL, nullptr},
                          {"page_commit", FAST(page_commit), METH_FASTCALL, nullptr},
                          {"attn_paged", FAST(attn_paged), METH_FASTCALL, nullptr},
                          {"attn_blocks", FAST(attn_blocks), METH_FASTCALL, nullptr},
+                         {"verify_drafts", FAST(verify_drafts), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_bind", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1347,3 +1347,21 @@ def attn_blocks(q, key, value, ksum, table, length, blocks, sink=1, local=1, mas
     Returns (out [B, S, H, D], sel int32 [B, S, Hk, sink + local + blocks]): the selected pages of the sequence, ascending,
     -1 behind them. No counterpart in the reference."""
     return (_bind or _bound()).attn_blocks(q, key, value, ksum, table, length, blocks, sink, local, mask, scale, out, sel)
+
+
+def verify_drafts(logits, tokens, uniform, draft=None, parent=None, temperature=1.0):
+    """The step's drafted tokens against the target's probabilities p_r = softmax(logits[b, r] / temperature): logits [B, R, V]
+    (bf16, fp16 or fp32), row 0 the last committed token's, row r >= 1 holding the drafted token tokens[b, r] (int64; outside
+    the vocabulary: none) behind row parent[b, r] < r (int32; None: a chain). draft [B, R - 1, V], of the same type: the
+    logits of q_r, which the token of row r + 1 was drawn from (a chain): it is accepted if uniform[b, r] q_r(x) < p_r(x),
+    and the first refusal's answer is drawn from max(p_r - q_r, 0), so that the answers are distributed as the target's.
+    Without draft (drafts that are no samples; trees): of a row's children, in row order, the first is accepted whose token,
+    with the distinct ones ahead of it, has more of p_r than uniform[b, r]; if none has, the answer is drawn from p_r without
+    their tokens. A row with no drafted token behind it answers from p_r. Drawn: the lowest index whose cumulative weight
+    passes uniform[b, R] of the whole, in 64-bit sums. uniform float64 [B, R + 1] in [0, 1). temperature: a number, or float32
+    [B]; 0: the lowest index of the largest logit has all of p_r. A logit of -inf or NaN has no probability; +inf counts as
+    the largest finite number.
+    Returns (count int32 [B]: row 0 and the accepted rows, path int32 [B, R]: those rows, -1 behind, next int64 [B]: the
+    answer, -1 where no token has a probability); count and path are page_commit's. The role of mtp_accept's walk
+    (csrc/mtp_loop.sycl:86-196 of the reference), by probabilities and for a batch."""
+    return (_bind or _bound()).verify_drafts(logits, tokens, uniform, draft, parent, temperature)

@@ -649,6 +649,26 @@ int mdx_attn_blocks(const void* q, int64_t q_seq_stride, int64_t q_row_stride, i
                     int64_t S, int64_t H, int64_t Hk, int64_t D, int64_t P, int64_t T, int64_t W, float scale, void* workspace,
                     size_t workspace_bytes, void* stream);
 
+/* ---- a step's answers --------------------------------------------------------------------------------
+ * Verification of drafted tokens against the target's probabilities. p_r = softmax(logits[b][r] / T), T the sequence's
+ * temperature (temperatures f32 [B], or `temperature` for all with NULL; 0 and below: 1 at the lowest index of the maximum); a
+ * NaN counts as -inf, +inf as the largest finite number. Row 0 is the last committed token's; row r >= 1 holds the drafted
+ * token tokens[b][r] (outside 0..V - 1: none) behind row parent[b][r] < r (NULL: r - 1; another value: never reached). With
+ * draft [B][R - 1][V], q_r = softmax(draft[b][r] / T) is what row r + 1's token was drawn from (parent NULL): accepted if
+ * uniform[b][r] q_r(x) < p_r(x); the first refusal's answer is drawn from max(p_r - q_r, 0) (p_r if that is empty). Without:
+ * of a row's children, in row order, the first with uniform[b][r] < the sum of p_r over the distinct tokens up to it is
+ * accepted; if none is, the answer is drawn from p_r without their tokens. A row with no drafted token behind it answers
+ * from p_r. Drawn is the lowest index whose cumulative weight passes uniform[b][R] of the whole (the last with a weight where
+ * rounding leaves none; -1 where there is no weight). 64-bit sums. logits, draft: dtype MDX_DT_BF16, _F16 or _F32, rows
+ * contiguous, any strides; uniform f64 [B][R + 1] in [0, 1). count int32 [B]: row 0 and the accepted rows; path int32 [B][R]:
+ * those rows, -1 behind (mdx_page_commit's); next int64 [B]: the answer. B <= 1024, R <= 64, V < 2^24. The role of
+ * mdx_mtp_accept's walk (csrc/mtp_loop.sycl:86-196), by probabilities and for a batch. */
+size_t mdx_verify_drafts_workspace(int64_t B, int64_t R, int64_t V, int32_t drafted);
+int mdx_verify_drafts(const void* logits, int64_t seq_stride, int64_t row_stride, const void* draft, int64_t draft_seq_stride,
+                      int64_t draft_row_stride, int32_t dtype, const int64_t* tokens, const int32_t* parent, const double* uniform,
+                      const float* temperatures, float temperature, int32_t* count, int32_t* path, int64_t* next, int64_t B,
+                      int64_t R, int64_t V, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Calibration: one streaming read of `bytes` (a multiple of 1024) from `src` with the W4A8 GEMV's load
  * pattern (1 KiB per wave instruction, four loads in flight per wave), over `work_groups` work-groups
  * of 256 threads; `sink` (4 bytes) is written only if the data hashes to a marker value. It has no

@@ -1105,3 +1105,71 @@ def page_commit(kv, table, length, refs, count, path, room):
             if t // T < W and 0 <= table[b, t // T] < P:
                 slots[b, r] = table[b, t // T] * T + t % T
     return kv, table, new_length, refs, status, slots, filled
+
+
+# ---- a step's answers ------------------------------------------------------------------------------------
+def token_probabilities(logits, heat):
+    """softmax(logits / heat) of one row in float64; heat 0 (or less): 1 at the lowest index of the maximum. NaN and -inf have no
+    probability, +inf counts as the largest finite number; all zeros where nothing has one."""
+    x = np.asarray(logits, dtype=np.float64)
+    x = np.where(np.isnan(x), -np.inf, np.minimum(x, float(np.finfo(np.float32).max)))
+    top = x.max()
+    if top == -np.inf:
+        return np.zeros_like(x)
+    if not heat > 0:
+        p = np.zeros_like(x)
+        p[int(np.argmax(x))] = 1.0
+        return p
+    with np.errstate(under="ignore", over="ignore", invalid="ignore"):
+        z = (x - top) / float(heat)
+        e = np.where(x == -np.inf, 0.0, np.exp(z))
+    return e / e.sum()
+
+
+def draw_token(w, u):
+    """The lowest index whose cumulative weight passes u of the whole; the last with a weight where none does; -1: no weight."""
+    c = np.cumsum(w)
+    if not c[-1] > 0:
+        return -1
+    past = np.flatnonzero((c > u * c[-1]) & (w > 0))
+    return int(past[0]) if past.size else int(np.flatnonzero(w > 0)[-1])
+
+
+def verify_drafts(logits, tokens, uniform, draft=None, parent=None, heat=1.0):
+    """The verification of drafted tokens: (count [B], path [B, R], next [B]). logits [B, R, V], draft [B, R - 1, V] or None,
+    parent [B, R] or None (a chain), uniform [B, R + 1], heat a number or [B]."""
+    B, R, V = logits.shape
+    heats = np.broadcast_to(np.asarray(heat, dtype=np.float32), (B,))
+    counts, paths, answers = [], np.full((B, R), -1, dtype=np.int64), []
+    for b in range(B):
+        up = [int(parent[b][r]) if parent is not None else r - 1 for r in range(R)]
+        drafted = [r > 0 and 0 <= up[r] < r and 0 <= int(tokens[b][r]) < V for r in range(R)]
+        line, at = [0], 0
+        while True:
+            p = token_probabilities(logits[b, at], heats[b])
+            kids = [r for r in range(at + 1, R) if drafted[r] and up[r] == at]
+            step = None
+            if draft is not None and kids:
+                q, x = token_probabilities(draft[b, at], heats[b]), int(tokens[b][kids[0]])
+                if uniform[b, at] * q[x] < p[x]:
+                    step = kids[0]
+                else:
+                    rest = np.maximum(p - q, 0.0)
+                    p = rest if rest.sum() > 0 else p
+            elif draft is None:
+                passed = 0.0
+                for r in kids:
+                    x = int(tokens[b][r])
+                    passed += p[x]
+                    if p[x] > 0 and uniform[b, at] < passed:
+                        step = r
+                        break
+                    p[x] = 0.0
+            if step is None:
+                break
+            at = step
+            line.append(at)
+        counts.append(len(line))
+        paths[b, :len(line)] = line
+        answers.append(draw_token(p, uniform[b, R]))
+    return np.array(counts), paths, np.array(answers)

@@ -1,0 +1,181 @@
+"""verify_drafts against its oracle in float64: every output is a whole number and has to be equal. (A draw or an acceptance could
+only differ where a uniform lies within about 1e-13 of a border, relative to the whole: with the fixed inputs here none does.)"""
+import numpy as np
+import pytest
+import torch
+
+from oracle import ref
+
+pytestmark = pytest.mark.gpu
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def f64(t):
+    return t.detach().cpu().double().numpy()
+
+
+def inputs(seed, B, R, V, dt, spread=3.0):
+    g = torch.Generator().manual_seed(seed)
+    base = torch.randn(B, R, V, generator=g) * spread
+    logits = (base + 0.5 * torch.randn(B, R, V, generator=g)).to(DT[dt])
+    draft = (base[:, :R - 1] + 0.5 * torch.randn(B, R - 1, V, generator=g)).to(DT[dt])
+    tokens = torch.zeros(B, R, dtype=torch.int64)
+    if R > 1:
+        noise = torch.empty(B, R - 1, V).exponential_(generator=g)
+        tokens[:, 1:] = (draft.float() - noise.log()).argmax(-1)
+    return logits, draft, tokens, torch.rand(B, R + 1, generator=g, dtype=torch.float64)
+
+
+def check(C, logits, tokens, uniform, draft=None, parent=None, heat=1.0, dev="cuda"):
+    up = lambda t: t.to(dev) if torch.is_tensor(t) else t  # noqa: E731
+    got = C.verify_drafts(up(logits), up(tokens), up(uniform), draft=up(draft), parent=up(parent), temperature=up(heat))
+    want = ref.verify_drafts(f64(logits), tokens.numpy(), uniform.numpy(), None if draft is None else f64(draft),
+                             None if parent is None else parent.numpy(), heat.numpy() if torch.is_tensor(heat) else heat)
+    for g, w, what in zip(got, want, ("count", "path", "next")):
+        assert g.cpu().numpy().tolist() == w.tolist(), what
+    return want
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("B,R,V", [(1, 2, 1), (3, 4, 7), (2, 5, 4097), (5, 3, 8185), (2, 2, 8193), (1, 8, 32768), (2, 3, 151936), (33, 2, 501)])
+def test_chains_with_draft_probabilities(C, dt, B, R, V):
+    logits, draft, tokens, uniform = inputs(V + R, B, R, V, dt)
+    check(C, logits, tokens, uniform, draft, heat=torch.linspace(0.6, 1.4, B))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("B,R,V", [(1, 1, 9), (4, 8, 1000), (2, 16, 8191), (1, 64, 257), (3, 5, 40000)])
+def test_trees(C, dt, B, R, V):
+    """Random trees whose children carry likely tokens, some of them twice, some none, some rows behind no row ahead of them."""
+    logits, _, tokens, uniform = inputs(V * 3 + R, B, R, V, dt, spread=2.0)
+    g = torch.Generator().manual_seed(R)
+    parent = (torch.rand(B, R, generator=g) * torch.arange(R)).to(torch.int32)
+    best = logits.float().topk(min(4, V), -1).indices
+    for b in range(B):
+        for r in range(1, R):
+            tokens[b, r] = best[b, parent[b, r], int(torch.randint(0, best.shape[-1], (1,), generator=g))]
+    if R > 4:
+        tokens[0, 3], tokens[0, 4] = -1, V
+        parent[-1, 2], parent[-1, 4] = 2, -7
+    check(C, logits, tokens, uniform, parent=parent, heat=0.5)
+    low = uniform.clone()
+    low[:, :R] *= 0.05  # (the first children: long paths)
+    check(C, logits, tokens, low, parent=parent, heat=torch.full((B,), 0.5))
+    check(C, logits, tokens, uniform, heat=0.5)  # a chain of drafts that are no samples
+
+
+def test_long_accepted_chains(C):
+    """Draft and target alike: every token is accepted, the answer comes from the last row."""
+    logits, _, tokens, uniform = inputs(5, 4, 9, 3000, "bf16")
+    same = logits[:, :8].contiguous()
+    g = torch.Generator().manual_seed(1)
+    tokens[:, 1:] = torch.randint(0, 3000, (4, 8), generator=g)
+    assert (check(C, logits, tokens, uniform, same)[0] == 9).all()
+
+
+def test_greedy(C):
+    logits, draft, tokens, uniform = inputs(9, 4, 5, 20000, "bf16")
+    logits[:, :, 777] = logits[:, :, 15000] = 60.0  # a tie: the lowest index
+    tokens[0, 1:] = 777
+    tokens[1, 1:3] = 777
+    heat = torch.tensor([0.0, 0.0, -1.0, 0.7])
+    want = check(C, logits, tokens, uniform, draft, heat=heat)
+    assert want[0][0] == 5 and want[2][0] == 777 and want[2][2] == 777
+    assert check(C, logits, tokens, uniform, heat=0.0)[0].tolist()[:2] == [5, 3]
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+def test_masked_and_odd_logits(C, dt):
+    """-inf over most of the vocabulary, rows of nothing, NaN, +inf, the type's lowest value, all logits alike."""
+    logits, draft, tokens, uniform = inputs(11, 8, 3, 9000, dt)
+    logits[0, :, :8990] = float("-inf")
+    logits[1] = float("-inf")
+    logits[2, :, ::2] = float("nan")
+    logits[3, :, 55] = logits[3, :, 8600] = float("inf")
+    logits[4] = torch.finfo(DT[dt]).min
+    logits[4, :, 4000] = torch.finfo(DT[dt]).max
+    logits[5] = 0.0
+    logits[6, 0, :8192] = float("-inf")
+    draft[7] = float("-inf")
+    tokens[0, 1] = 8995
+    for heat in (1.0, torch.linspace(0.5, 2.0, 8), 0.0):
+        want = check(C, logits, tokens, uniform, draft, heat=heat)
+        assert want[2][1] == -1
+        check(C, logits, tokens, uniform, heat=heat)
+
+
+def test_refused_without_a_rest(C):
+    """A token without probability in p and q, and p == q: p answers; uniforms at the ends of their range."""
+    logits, _, tokens, uniform = inputs(13, 6, 2, 20000, "fp16")
+    logits[:, :, 123] = float("-inf")
+    tokens[:, 1] = 123
+    uniform[0], uniform[1] = 0.0, 1.0 - 2.0 ** -53
+    assert (check(C, logits, tokens, uniform, logits[:, :1].contiguous())[0] == 1).all()
+
+
+def test_extreme_temperatures(C):
+    logits, draft, tokens, uniform = inputs(14, 5, 3, 5000, "fp32")
+    heat = torch.tensor([1e-30, 1e-3, 50.0, 1e30, 2.0 ** -140])
+    check(C, logits, tokens, uniform, draft, heat=heat)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_strided_rows(C, dev, dt):
+    """Rows of a wider buffer that stand at every offset to the 16-byte boundaries, the draft's otherwise than the target's."""
+    logits, draft, tokens, uniform = inputs(15, 3, 4, 8190, dt)
+    for off, pad in ((1, 3), (3, 0), (5, 8), (7, 1)):
+        wide = torch.full((3, 4, 8190 + off + pad), 99.0, dtype=DT[dt], device=dev)
+        view = wide[:, :, off:off + 8190]
+        view.copy_(logits)
+        dwide = torch.full((3, 3, 8191 + pad), 99.0, dtype=DT[dt], device=dev)
+        dview = dwide[:, :, 1:8191]
+        dview.copy_(draft)
+        got = C.verify_drafts(view, tokens.to(dev), uniform.to(dev), draft=dview, temperature=0.9)
+        want = ref.verify_drafts(f64(logits), tokens.numpy(), uniform.numpy(), f64(draft), heat=0.9)
+        assert [g.cpu().tolist() for g in got] == [w.tolist() for w in want]
+    # one row of logits for every sequence and row
+    one = logits[:1, :1].to(dev).expand(3, 4, 8190)
+    got = C.verify_drafts(one, tokens.to(dev), uniform.to(dev))
+    want = ref.verify_drafts(f64(one), tokens.numpy(), uniform.numpy())
+    assert [g.cpu().tolist() for g in got] == [w.tolist() for w in want]
+
+
+def test_captured_and_replayed_beside_another_stream(C, dev):
+    """Two calls of one shape at once, one of them a captured graph that is replayed over changing inputs."""
+    a = [inputs(20 + i, 6, 5, 30000, "bf16") for i in range(4)]
+    hold = [t.to(dev) for t in a[0]]
+    other = [t.to(dev) for t in a[3]]
+    C.verify_drafts(hold[0], hold[2], hold[3], draft=hold[1])
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        out = C.verify_drafts(hold[0], hold[2], hold[3], draft=hold[1])
+    want_other = ref.verify_drafts(f64(a[3][0]), a[3][2].numpy(), a[3][3].numpy(), f64(a[3][1]))
+    for i in (1, 2, 0, 1):
+        for h, t in zip(hold, a[i]):
+            h.copy_(t)
+        torch.cuda.synchronize()
+        graph.replay()
+        with torch.cuda.stream(side):
+            beside = C.verify_drafts(other[0], other[2], other[3], draft=other[1])
+        torch.cuda.synchronize()
+        want = ref.verify_drafts(f64(a[i][0]), a[i][2].numpy(), a[i][3].numpy(), f64(a[i][1]))
+        assert [g.cpu().tolist() for g in out] == [w.tolist() for w in want]
+        assert [g.cpu().tolist() for g in beside] == [w.tolist() for w in want_other]
+
+
+def test_refusals(C, dev):
+    logits, draft, tokens, uniform = (t.to(dev) for t in inputs(30, 2, 3, 64, "bf16"))
+    parent = torch.zeros(2, 3, dtype=torch.int32, device=dev)
+    for args, kw in (((logits.half(), tokens, uniform), dict(draft=draft)), ((logits.transpose(1, 2), tokens, uniform), {}),
+                     ((logits, tokens.int(), uniform), {}), ((logits, tokens, uniform.float()), {}), ((logits, tokens, uniform[:, :3]), {}),
+                     ((logits, tokens, uniform), dict(draft=draft, parent=parent)), ((logits, tokens, uniform), dict(parent=parent.long())),
+                     ((logits, tokens, uniform), dict(draft=draft[:, :1])), ((logits, tokens, uniform), dict(temperature=-1.0)),
+                     ((logits, tokens, uniform), dict(temperature=torch.ones(3, device=dev))), ((logits, tokens.cpu(), uniform), {}),
+                     ((logits.double(), tokens, uniform), {})):
+        with pytest.raises(RuntimeError):
+            C.verify_drafts(*args, **kw)
+    with pytest.raises((RuntimeError, TypeError)):
+        C.verify_drafts(logits, tokens, uniform, temperature="warm")
+    count, path, answer = C.verify_drafts(logits[:0], tokens[:0], uniform[:0])
+    assert count.shape == (0,) and path.shape == (0, 3) and answer.shape == (0,)
