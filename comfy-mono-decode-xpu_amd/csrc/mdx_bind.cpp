@@ -33,8 +33,10 @@ struct Entries {
     decltype(&mdx_attn_blocks) blocks;
     decltype(&mdx_verify_drafts_workspace) verify_workspace;
     decltype(&mdx_verify_drafts) verify;
+    decltype(&mdx_attn_window_workspace) window_workspace;
+    decltype(&mdx_attn_window) window;
 } g;
-constexpr int ENTRIES = 11;
+constexpr int ENTRIES = 13;
 PyObject* g_error = nullptr;  // _lib.MdxError
 
 struct Refused : std::runtime_error {
@@ -331,6 +333,49 @@ PyObject* attn_blocks(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     });
 }
 
+// a window's length (None: everything)
+int64_t window_of(PyObject* o) {
+    const int64_t window = given(o) ? number(o) : int64_t(1) << 30;
+    check(window >= 1 && window <= (int64_t(1) << 30), "window: 1..2^30 tokens, or None");
+    return window;
+}
+
+// q, key, value, table, length, window, sinks, mask, scale, out, lse -> (out, lse)
+PyObject* attn_window(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    EXPECT(11, "attn_window")
+    return guarded([&]() -> PyObject* {
+        Attn x = attn(a[0], a[1], a[2], a[3], a[4], a[7], a[9]);
+        const int64_t window = window_of(a[5]), sinks = number(a[6]);
+        check(sinks >= 0 && sinks <= (int64_t(1) << 30), "sinks: 0..2^30 tokens");
+        const float scale = scale_of(a[8], x.D);
+        at::Tensor lse;
+        if (given(a[10])) {
+            lse = on(a[10], "lse", x.d);
+            check(lse.scalar_type() == at::kFloat && lse.sizes() == at::IntArrayRef({x.B, x.S, x.H}) && lse.is_contiguous(),
+                  "lse: contiguous float32 [sequences, rows, heads]");
+        } else {
+            lse = at::empty({x.B, x.S, x.H}, at::TensorOptions().dtype(at::kFloat).device(x.d));
+        }
+        if (x.B > 0 && x.S > 0) {
+            const size_t n = g.window_workspace(x.B, x.S, x.H, x.Hk, x.D, x.T, x.W, window, sinks);
+            at::Tensor ws;
+            if (n) ws = scratch(n, x.d);
+            call("mdx_attn_window", x.d, [&](void* st) {
+                return g.window(data(x.q), x.q.stride(0), x.q.stride(1), x.q.stride(2), data(x.key), x.key.stride(0), x.key.stride(1),
+                                x.key.stride(2), data(x.value), x.value.stride(0), x.value.stride(1), x.value.stride(2), x.dt,
+                                x.table.data_ptr<int32_t>(), x.ts, x.length.data_ptr<int32_t>(), x.mask, data(x.out), lse.data_ptr<float>(),
+                                window, sinks, x.B, x.S, x.H, x.Hk, x.D, x.P, x.T, x.W, scale, n ? data(ws) : nullptr, n, st);
+            });
+        }
+        PyObject* o = same_or_new(a[9], x.out);
+        PyObject* l = o ? same_or_new(a[10], lse) : nullptr;
+        PyObject* both = l ? PyTuple_Pack(2, o, l) : nullptr;
+        Py_XDECREF(o);
+        Py_XDECREF(l);
+        return both;
+    });
+}
+
 // ---- a step's answers ----
 // logits, tokens, uniform, draft, parent, temperature -> (count, path, next)
 PyObject* verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
@@ -416,6 +461,8 @@ PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     g.blocks = reinterpret_cast<decltype(g.blocks)>(p[i++]);
     g.verify_workspace = reinterpret_cast<decltype(g.verify_workspace)>(p[i++]);
     g.verify = reinterpret_cast<decltype(g.verify)>(p[i++]);
+    g.window_workspace = reinterpret_cast<decltype(g.window_workspace)>(p[i++]);
+    g.window = reinterpret_cast<decltype(g.window)>(p[i++]);
     Py_XINCREF(a[ENTRIES]);
     Py_XDECREF(g_error);
     g_error = a[ENTRIES];
@@ -428,6 +475,7 @@ PyMethodDef methods[] = {{"init", FAST(init), METH_FASTCALL, nullptr},
                          {"page_commit", FAST(page_commit), METH_FASTCALL, nullptr},
                          {"attn_paged", FAST(attn_paged), METH_FASTCALL, nullptr},
                          {"attn_blocks", FAST(attn_blocks), METH_FASTCALL, nullptr},
+                         {"attn_window", FAST(attn_window), METH_FASTCALL, nullptr},
                          {"verify_drafts", FAST(verify_drafts), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_bind", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -105,7 +105,16 @@ struct PagedArgs {
     int spb;    // a unit's query rows: s from u spb, each with the kv head's G heads
     int whole;  // every work-group takes one whole unit (no join)
     float zs;   // scale * log2(e)
+    // a row's first `first` and last `window` tokens (mdx_attn_window), and its log-sum-exp [B, S, H]
+    int first, window;
+    float* lse;
 };
+
+// What a row's tokens are: all that are admitted, those of selected blocks (mdx_attn_blocks), or its first and last ones
+// (mdx_attn_window).
+enum class Kind { ALL, SEL, WIN };
+// fp32 numbers of a partial beside O: maximum, sum (windows: and the sum of the weights before their rounding)
+constexpr int extra_of(Kind k) { return k == Kind::WIN ? 3 : 2; }
 
 constexpr int MAX_SEQS = 1024;
 constexpr int STEP = 32;
@@ -236,25 +245,51 @@ __device__ __forceinline__ void wait_vm() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-// The tokens a unit's steps run over. Without a selection: [0, n + own rows). With one: the selected blocks' tokens, then
-// the tail behind the full pages and the rows' own (virtual tokens v; tree0 = the first own row's).
+// The tokens a unit's steps run over, as virtual tokens v: the first `nsel` of them are selected blocks' (Kind::SEL) or the
+// sequence's first ones (Kind::WIN), the others are tokens tail + (v - nsel) in a row. Kind::ALL: [0, n + own rows).
 struct Span {
     int n;      // committed tokens
-    int tree0;  // virtual token of own row 0
-    int nsel;   // tokens of selected blocks (0: none)
+    int tree0;  // virtual token of own row 0 (of a window that begins among the rows' own tokens: negative)
+    int nsel;   // tokens of selected blocks, or first ones in whole stages (0: none)
     int tail;   // token at which the tail starts
 };
-template <bool SEL>
-__device__ __forceinline__ Span span_of(const PagedArgs& a, int n) {
+constexpr int WIN_STEP = 64;  // a window's parts begin at multiples of the longest stage
+// own tokens that unit u attends at most (a chain's unit ends with its last row's)
+__device__ __forceinline__ int own_of(const PagedArgs& a, int u) { return a.mask ? a.S : min(a.S, (u + 1) * a.spb); }
+template <Kind KIND>
+__device__ __forceinline__ Span span_of(const PagedArgs& a, int n, int u) {
     n = n < 0 ? 0 : (n > (a.W << a.lt) ? a.W << a.lt : n);
-    if constexpr (!SEL) return {n, n, 0, 0};
+    if constexpr (KIND == Kind::ALL) return {n, n, 0, 0};
+    if constexpr (KIND == Kind::WIN) {
+        // the window of the unit's first row (under a mask: of a row without own tokens), and the first tokens, as one part
+        // where they meet
+        const int lo = n + (a.mask ? 0 : u * a.spb + 1) - a.window, tail = lo > 0 ? lo & ~(WIN_STEP - 1) : 0;
+        const int nsel = (min(a.first, n + own_of(a, u)) + WIN_STEP - 1) & ~(WIN_STEP - 1);
+        if (tail <= nsel) return {n, n, 0, 0};
+        return {n, nsel + n - tail, nsel, tail};
+    }
     const int c = n >> a.lt, k = c < a.most ? c : a.most;
     return {n, (k << a.lt) + (n - (c << a.lt)), k << a.lt, c << a.lt};
 }
-// own tokens that unit u attends at most (a chain's unit ends with its last row's), and its steps
-__device__ __forceinline__ int own_of(const PagedArgs& a, int u) { return a.mask ? a.S : min(a.S, (u + 1) * a.spb); }
+// A row's own tokens under a mask (bits) that a window leaves: of all its tokens, the n committed and these in order, the first
+// `first` and the last `window`.
+__device__ __forceinline__ uint64_t own_in_window(const PagedArgs& a, uint64_t bits, int n) {
+    uint64_t left = bits;
+    for (int i = 0, gone = __popcll(bits) - a.window; i < gone; ++i) {
+        const uint64_t low = left & (0 - left);
+        left ^= low;
+        if (n + i >= a.first) bits ^= low;
+    }
+    return bits;
+}
 __device__ __forceinline__ int steps_of(const PagedArgs& a, const Span& s, int u, int tokens_per_step) {
     return (s.tree0 + own_of(a, u) + tokens_per_step - 1) / tokens_per_step;
+}
+
+// log(sum of exp(scores)) of weights that are taken against M (log2 units), times 2^SHIFT; -inf for none
+template <class E>
+__device__ __forceinline__ float log_sum(float M, float sum) {
+    return sum == 0.f ? -INFINITY : (M + (__builtin_amdgcn_logf(sum) - E::SHIFT)) * 0.69314718055994530942f;
 }
 
 // One work-group: RTW waves of row tiles (TPW tiles of 16 query rows each) times P token parts.
@@ -276,8 +311,9 @@ struct Geometry {
     static_assert(NS >= 1 && (NS & (NS - 1)) == 0 && PER >= 1 && (RTW == 1 ? SUB == 1 : NS >= 2) && (SUB == 1 || D != 256), "ring geometry");
 };
 
-template <class E, int D, int TPW, int RTW, int P, int WPC, int SUB, bool SEL>
+template <class E, int D, int TPW, int RTW, int P, int WPC, int SUB, Kind KIND>
 __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_kernel(PagedArgs a) {
+    constexpr bool SEL = KIND == Kind::SEL, WIN = KIND == Kind::WIN;
     using Geo = Geometry<D, TPW, RTW, P, WPC, SUB>;
     constexpr int NT = Geo::NT, RPW = Geo::RPW, STAGE = Geo::STAGE, NS = Geo::NS, PER = Geo::PER;
     constexpr int KK = D / 32, DT = D / 16, ST = STEP * SUB, TOK = ST * P;
@@ -300,9 +336,10 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
             if (++kh == a.Hk) {
                 kh = 0;
                 ++b;
-                sp = span_of<SEL>(a, uload(a.length + b));
+                sp = span_of<KIND>(a, uload(a.length + b), u);
             }
         }
+        if constexpr (WIN) sp = span_of<KIND>(a, sp.n, u);
     };
 
     // ---- this work-group's share of the line of steps: [begin, end), and the sequence it begins in
@@ -314,7 +351,7 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
         const int rank = (q & 1) && (q + 1) * turn <= all ? 2 * q * turn + turn - 1 - rest : rest;
         b = rank % a.B;
         u = a.units - 1 - rank / a.B;
-        sp = span_of<SEL>(a, uload(a.length + b));
+        sp = span_of<KIND>(a, uload(a.length + b), u);
         begin = in_b = 0;
         end = quota = steps_of(a, sp, u, TOK);
         if (tid == 0) odd[0] = INT_MAX, odd[1] = -1;
@@ -328,7 +365,7 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
         auto walk = [&](auto f) {
             int bb = i0 / per_b, rest = i0 % per_b, uu = rest % a.units;
             for (int i = i0; i < i1; ++i) {
-                f(bb, rest, steps_of(a, span_of<SEL>(a, a.length[bb]), uu, TOK) + Geo::FIXED);
+                f(bb, rest, steps_of(a, span_of<KIND>(a, a.length[bb], uu), uu, TOK) + Geo::FIXED);
                 if (++uu == a.units) uu = 0;
                 if (++rest == per_b) {
                     rest = 0;
@@ -380,7 +417,7 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
         kh = __builtin_amdgcn_readfirstlane(sh_at[1]);
         u = __builtin_amdgcn_readfirstlane(sh_at[2]);
         in_b = __builtin_amdgcn_readfirstlane(sh_at[3]);
-        sp = span_of<SEL>(a, uload(a.length + b));
+        sp = span_of<KIND>(a, uload(a.length + b), u);
         const int past = in_b - steps_of(a, sp, u, TOK);
         if (past >= 0) {  // (behind the unit's last step: the next unit)
             begin += Geo::FIXED - past;
@@ -414,6 +451,9 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
         // tokens that every row of the wave admits (a chain's first row in the wave its own too)
         const int t_all = sp.tree0 + (a.mask ? 0 : min(a.S, s_first + rw * TPW * 16 / a.G + 1));
         const int t_none = a.mask ? t_end : min(t_end, sp.tree0 + s_first + ((rw + 1) * TPW * 16 - 1) / a.G + 1);  // from here none
+        // windows: tokens from which the wave's first and its last row attend (under masks: rows of no own tokens, of all)
+        const int lo_first = WIN ? sp.n - a.window + (a.mask ? 0 : s_first + rw * TPW * 16 / a.G + 1) : 0;
+        const int lo_last = WIN ? sp.n - a.window + (a.mask ? a.S : min(a.S, s_first + ((rw + 1) * TPW * 16 - 1) / a.G + 1)) : 0;
 
         // ---- the pages of a stage (scalar loads ahead of their use), and its direct loads
         const unsigned char* kbase = reinterpret_cast<const unsigned char*>(a.key + kh * a.kh);
@@ -428,7 +468,7 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
         auto entry = [&](int v) {
             if (v >= t_end) return -1;
             if (SEL && v < sp.nsel) return uload(picked + (v >> a.lt));
-            const int j = (SEL ? sp.tail + (v - sp.nsel) : v) >> a.lt;
+            const int j = (SEL || (WIN && v >= sp.nsel) ? sp.tail + (v - sp.nsel) : v) >> a.lt;
             return j < a.W ? uload(row + j) : -1;
         };
         auto entries = [&](int s) {
@@ -448,7 +488,7 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
         const unsigned char *kp_[HW], *vp_[HW];
         auto place = [&](int s, Pages x) {
             const int v0 = (step0 + s) * TOK + part * ST;
-            const uint32_t r0 = uint32_t(SEL && v0 >= sp.nsel ? v0 - sp.nsel : v0);
+            const uint32_t r0 = uint32_t(SEL && v0 >= sp.nsel ? v0 - sp.nsel : WIN && v0 >= sp.nsel ? v0 - sp.nsel + sp.tail : v0);
             const bool in0 = uint32_t(x.e[0]) < uint32_t(a.P);
             uint32_t ok = in0 ? (1u << QT) - 1u : 0u;
             int e_own = x.e[0];
@@ -500,7 +540,7 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
         // ---- query rows and what they admit
         u32x4 qf[TPW][KK];
         uint64_t bits[TPW];
-        int lim[TPW];
+        int lim[TPW], lo[TPW];  // a chain's row; the first token of its window
 #pragma unroll
         for (int t = 0; t < TPW; ++t) {
             const int r = (rw * TPW + t) * 16 + c16, rr = r < rows ? r : 0;
@@ -511,6 +551,7 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
             bits[t] = a.mask ? uint64_t(a.mask[int64_t(b) * a.S + s]) : 0;
             if (a.S < 64) bits[t] &= (uint64_t(1) << a.S) - 1;
             lim[t] = s;
+            lo[t] = 0;
         }
         // they have arrived before the first direct load goes out: the compiler waits for all of those before it uses a
         // register that a load among them wrote
@@ -520,6 +561,10 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk) asm volatile("" : "+v"(qf[t][kk]));
             asm volatile("" : "+v"(bits[t]));
+            if constexpr (WIN) {
+                lo[t] = sp.n - a.window + (a.mask ? __popcll(bits[t]) : lim[t] + 1);
+                if (a.mask) bits[t] = own_in_window(a, bits[t], sp.n);
+            }
         }
 
         f32x4 acc[TPW][DT];
@@ -527,12 +572,13 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
         // looks), the reference, an earlier maximal score (0 as long as nothing is admitted, so that -inf - -inf never forms), the
         // sum of weights
         float m_lim[TPW], m_ref[TPW], l[TPW];
+        float lx[TPW];  // windows: the sum of the weights before their rounding (the log-sum-exp's)
         const float slack = E::SLACK / a.zs;
 #pragma unroll
         for (int t = 0; t < TPW; ++t) {
             m_lim[t] = -INFINITY;
             m_ref[t] = 0.f;
-            l[t] = 0.f;
+            l[t] = lx[t] = 0.f;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) acc[t][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
@@ -566,6 +612,9 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
             }
             const int v0 = (step0 + s) * TOK + part * ST;
             if (RTW > 1 && v0 >= t_none) continue;  // (uniform in the wave: only its loads and the barriers are left)
+            // windows: the token of v0, the virtual one of own row 0 in this part of the span
+            const int r0 = WIN && v0 >= sp.nsel ? v0 - sp.nsel + sp.tail : v0, tree0 = WIN && v0 < sp.nsel ? sp.n : sp.tree0;
+            if (WIN && RTW > 1 && r0 >= a.first && r0 + ST <= lo_first && r0 + ST <= sp.n + (a.mask ? 0 : a.S)) continue;
             f32x4 st[SUB][TPW][2];
             auto scores = [&](const u32x4 (&k)[KK], int x, int h) {
 #pragma unroll
@@ -599,7 +648,14 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
                 }
             }
 
-            const bool whole = ok == (1u << QT) - 1u && v0 + ST <= t_all;  // (uniform in the wave) every row admits every token
+            // (uniform in the wave) every row admits every token
+            const bool whole = ok == (1u << QT) - 1u && v0 + ST <= (WIN ? t_all - sp.tree0 + tree0 : t_all) &&
+                               (!WIN || r0 + ST <= a.first || r0 >= lo_last);
+            // which of the 32 tokens from r on are among the first, or from `from` on (Kind::WIN)
+            auto in_window = [&](int r, int from) -> uint32_t {
+                const int f = a.first - r, k = from - r;
+                return (f >= 32 ? ~0u : (f > 0 ? (1u << f) - 1u : 0u)) | (k <= 0 ? ~0u : (k < 32 ? ~0u << k : 0u));
+            };
             // tile t's weights of the stage, as the B operands of O^T += V^T P^T
             struct Weights {
                 u32x4 p[SUB];
@@ -610,15 +666,16 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
                     bool any = false;
 #pragma unroll
                     for (int x = 0; x < SUB; ++x) {
-                        int p = sp.tree0 - v0 - STEP * x;  // tokens of the prefix in the piece
+                        int p = (WIN ? tree0 : sp.tree0) - v0 - STEP * x;  // tokens of the prefix in the piece
                         asm volatile("" : "+s"(p));        // (none of this ahead of the branch)
+                        const uint32_t near = WIN ? in_window(r0 + STEP * x, lo[t]) : ~0u;
                         uint32_t in;
                         if (a.mask) {
                             const uint64_t own_bits = p >= 32 ? 0 : (p >= 0 ? bits[t] << p : (-p < 64 ? bits[t] >> -p : 0));
-                            in = (p >= 32 ? ~0u : (p > 0 ? (1u << p) - 1u : 0u)) | uint32_t(own_bits);
+                            in = ((p >= 32 ? ~0u : (p > 0 ? (1u << p) - 1u : 0u)) & near) | uint32_t(own_bits);
                         } else {
                             const int nv = p + lim[t] + 1;
-                            in = nv >= 32 ? ~0u : (nv > 0 ? (1u << nv) - 1u : 0u);
+                            in = (nv >= 32 ? ~0u : (nv > 0 ? (1u << nv) - 1u : 0u)) & near;
                         }
                         const uint32_t here = ok >> (2 * x);
                         in &= ((here & 1u) ? 0x0000FFFFu : 0u) | ((here & 2u) ? 0xFFFF0000u : 0u);
@@ -652,6 +709,7 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
                         m_ref[t] = ref = top;
                         m_lim[t] = __builtin_fabsf(top * a.zs) > FAR_REF ? -FLT_MAX : top + slack;
                         l[t] *= alpha;
+                        if constexpr (WIN) lx[t] *= alpha;
 #pragma unroll
                         for (int dt = 0; dt < DT; ++dt) acc[t][dt] *= alpha;
                     }
@@ -675,6 +733,7 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
                             const float p1 = __builtin_amdgcn_exp2f(fmaf(st[x][t][h][i + 1], a.zs, -sub));
                             r.p[x][2 * h + i / 2] = E::pair(p0, p1);
                             l[t] = E::add_pair(r.p[x][2 * h + i / 2], l[t]);  // (this lane's tokens; the row's four lanes meet at the end)
+                            if constexpr (WIN) lx[t] += p0 + p1;
                         }
                 return r;
             };
@@ -705,7 +764,8 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
                             vb[x] = u32x2{finite(vb[x].x), finite(vb[x].y)};
                         }
                         // the piece's tokens that a row of the wave admits (without masks: up to the last row's own)
-                        const int p = sp.tree0 - v0 - STEP * y;
+                        const int p = (WIN ? tree0 : sp.tree0) - v0 - STEP * y;
+                        const uint32_t near = WIN ? in_window(r0 + STEP * y, lo_first) : ~0u;
                         uint32_t in;
                         if (a.mask) {
                             uint64_t all = 0;
@@ -714,10 +774,10 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
 #pragma unroll
                             for (int d = 1; d < 16; d <<= 1) all |= __shfl_xor(all, d, 64);
                             const uint64_t own_bits = p >= 32 ? 0 : (p >= 0 ? all << p : (-p < 64 ? all >> -p : 0));
-                            in = (p >= 32 ? ~0u : (p > 0 ? (1u << p) - 1u : 0u)) | uint32_t(own_bits);
+                            in = ((p >= 32 ? ~0u : (p > 0 ? (1u << p) - 1u : 0u)) & near) | uint32_t(own_bits);
                         } else {
-                            const int nv = t_none - v0 - STEP * y;
-                            in = nv >= 32 ? ~0u : (nv > 0 ? (1u << nv) - 1u : 0u);
+                            const int nv = (WIN ? t_none - sp.tree0 + tree0 : t_none) - v0 - STEP * y;
+                            in = (nv >= 32 ? ~0u : (nv > 0 ? (1u << nv) - 1u : 0u)) & near;
                         }
                         const uint32_t here = ok >> (2 * y);
                         in &= ((here & 1u) ? 0x0000FFFFu : 0u) | ((here & 2u) ? 0xFFFF0000u : 0u);
@@ -781,12 +841,14 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
         // ---- the parts of a row tile meet in LDS, tile by tile; rows D + 4 floats apart (no two rows of an access in one bank)
         const bool first = step0 == 0, last = step0 + nst == n_unit;
         constexpr int OR = D + 4;
-        float* const lo = reinterpret_cast<float*>(smem);               // [RTW][P][16][OR]
-        float* const lm = lo + RTW * P * 16 * OR;                       // [RTW][P][16] maxima (log2 units), then sums
-        float* rec = a.part + (int64_t(share) * 2 + (first ? 1 : 0)) * RPW * (D + 2);
+        float* const lds_o = reinterpret_cast<float*>(smem);            // [RTW][P][16][OR]
+        float* const lm = lds_o + RTW * P * 16 * OR;                    // [RTW][P][16] maxima (log2 units), then sums
+        constexpr int MR = RTW * P * 16;
+        float* rec = a.part + (int64_t(share) * 2 + (first ? 1 : 0)) * RPW * (D + extra_of(KIND));
         // row r of the unit's block (row s, head h), dims d .. d + 3: done, or to its partial
-        auto put = [&](int r, int s, int h, int d, float M, float sum, f32x4 o) {
+        auto put = [&](int r, int s, int h, int d, float M, float sum, float sumx, f32x4 o) {
             if (first && last) {
+                if (WIN && d == 0) a.lse[(int64_t(b) * a.S + s) * a.H + h] = log_sum<E>(M, sumx);
                 const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
                 // (no token admitted: 0, whatever o holds)
                 *reinterpret_cast<uint2*>(a.out + ((int64_t(b) * a.S + s) * a.H + h) * D + d) =
@@ -796,6 +858,7 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
                 if (d == 0) {
                     rec[int64_t(RPW) * D + r] = M;
                     rec[int64_t(RPW) * (D + 1) + r] = sum;
+                    if (WIN) rec[int64_t(RPW) * (D + 2) + r] = sumx;
                 }
             }
         };
@@ -812,22 +875,24 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
 #pragma unroll
             for (int t = 0; t < TPW; ++t) {
                 const int r = (rw * TPW + t) * 16 + c16;
+                const float sx = WIN ? sum_x32(sum_x16(lx[t])) : 0.f;
                 const float sl = sum_x32(sum_x16(l[t])), M = m_lim[t] == -INFINITY ? -INFINITY : m_ref[t] * a.zs;
                 if (r >= rows) continue;
                 const int s = s_first + r / a.G, h = kh * a.G + r % a.G;
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) put(r, s, h, 16 * dt + 4 * g, M, sl, acc[t][dt]);
+                for (int dt = 0; dt < DT; ++dt) put(r, s, h, 16 * dt + 4 * g, M, sl, sx, acc[t][dt]);
             }
         } else {
 #pragma unroll
             for (int t = 0; t < TPW; ++t) {
-                float* mo = lo + (rw * P + part) * 16 * OR + c16 * OR + 4 * g;
+                float* mo = lds_o + (rw * P + part) * 16 * OR + c16 * OR + 4 * g;
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(mo + 16 * dt) = acc[t][dt];
-                const float sl = sum_x32(sum_x16(l[t]));
+                const float sl = sum_x32(sum_x16(l[t])), sx = WIN ? sum_x32(sum_x16(lx[t])) : 0.f;
                 if (g == 0) {
                     lm[(rw * P + part) * 16 + c16] = m_lim[t] == -INFINITY ? -INFINITY : m_ref[t] * a.zs;
                     lm[RTW * P * 16 + (rw * P + part) * 16 + c16] = sl;
+                    if (WIN) lm[2 * MR + (rw * P + part) * 16 + c16] = sx;
                 }
                 __syncthreads();
                 // thread: row x / (D / 4) of the RTW tiles' 16 each, four dims
@@ -839,20 +904,29 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
                     float M = -INFINITY;
 #pragma unroll
                     for (int p = 0; p < P; ++p) M = fmaxf(M, lm[(rt * P + p) * 16 + rr]);
-                    float sum = 0.f;
+                    float sum = 0.f, sumx = 0.f;
                     f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int p = 0; p < P; ++p) {
                         const float mp = lm[(rt * P + p) * 16 + rr];
                         const float wp = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mp - M);
                         sum += lm[RTW * P * 16 + (rt * P + p) * 16 + rr] * wp;
-                        o += *reinterpret_cast<const f32x4*>(lo + (rt * P + p) * 16 * OR + rr * OR + d) * wp;
+                        if (WIN) sumx += lm[2 * MR + (rt * P + p) * 16 + rr] * wp;
+                        o += *reinterpret_cast<const f32x4*>(lds_o + (rt * P + p) * 16 * OR + rr * OR + d) * wp;
                     }
                     if (left_out) {  // (what the stages left out, for the rows that admit it)
+                        uint64_t own = a.mask ? uint64_t(a.mask[int64_t(b) * a.S + s]) : 0;
+                        int lo_row = 0;
+                        if constexpr (WIN) {
+                            if (a.S < 64) own &= (uint64_t(1) << a.S) - 1;
+                            lo_row = sp.n - a.window + (a.mask ? __popcll(own) : s + 1);
+                            own = own_in_window(a, own, sp.n);
+                        }
                         for (int v = (step0 + odd_from) * TOK; v < min(t_end, (step0 + odd_to + 1) * TOK); ++v) {
-                            const int own_row = v - sp.tree0;
-                            if (own_row >= 0 && !(a.mask ? (uint64_t(a.mask[int64_t(b) * a.S + s]) >> own_row) & 1 : own_row <= s)) continue;
-                            const int tok = SEL && v >= sp.nsel ? v - sp.nsel + sp.tail : v;
+                            const int tok = (SEL || WIN) && v >= sp.nsel ? v - sp.nsel + sp.tail : v;
+                            const int own_row = WIN ? tok - sp.n : v - sp.tree0;
+                            if (own_row >= 0 && !(a.mask ? own_row < 64 && ((own >> own_row) & 1) : own_row <= s)) continue;
+                            if (WIN && !(a.mask && own_row >= 0) && tok >= a.first && tok < lo_row) continue;
                             const bool chosen = SEL && v < sp.nsel;
                             if (!chosen && (tok >> a.lt) >= a.W) continue;
                             const int64_t e = chosen ? picked[v >> a.lt] : row[tok >> a.lt];
@@ -865,7 +939,7 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
                             }
                         }
                     }
-                    put(r, s, h, d, M, sum, o);
+                    put(r, s, h, d, M, sum, sumx, o);
                 }
                 __syncthreads();
             }
@@ -892,29 +966,31 @@ __global__ __launch_bounds__(64 * RTW * P, RTW * P * WPC / 4) void paged_attn_ke
 // 37 us against 20 for 64 blocks of 128). D / 4 lanes take a partial's row in 16-byte pieces, 256 / D partials at
 // once; the maxima, sums and pieces of up to eight each go out together, so that few partials cost one memory round trip
 // behind the share's entry.
-template <class E, int D>
+template <class E, int D, Kind KIND>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int rpw) {
+    constexpr bool WIN = KIND == Kind::WIN;
     const int4 x = a.info[blockIdx.x];
     const int nseg = x.z, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
     if (nseg <= 1) return;
     const int u = x.x % a.units, kh = x.x / a.units % a.Hk, b = x.x / a.units / a.Hk;
     constexpr int TPR = D / 4, NG = 64 / TPR, U = 8;
     const int gi = lane / TPR, d = lane % TPR * 4;
-    const int64_t rec = int64_t(rpw) * (D + 2);
+    const int64_t rec = int64_t(rpw) * (D + extra_of(KIND));
     const float* base = a.part + int64_t(x.y) * 2 * rec;
     const int r = int(blockIdx.y) * 4 + w, s = u * a.spb + r / a.G, h = kh * a.G + r % a.G;
     if (r >= a.spb * a.G || s >= a.S) return;  // (uniform in the wave)
     f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-    float M = -INFINITY, sum = 0.f;
+    float M = -INFINITY, sum = 0.f, sumx = 0.f;
     for (int i0 = 0; i0 < nseg; i0 += U * NG) {
         f32x4 v[U];
-        float mi[U], li[U];
+        float mi[U], li[U], xi[U];
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             const int sg = min(i0 + i * NG + gi, nseg - 1);  // (past the last: read again, not counted)
             const float* p = base + (sg == 0 ? 1 : 2 * sg) * rec;
             mi[i] = p[int64_t(rpw) * D + r];
             li[i] = p[int64_t(rpw) * (D + 1) + r];
+            if (WIN) xi[i] = p[int64_t(rpw) * (D + 2) + r];
             v[i] = *reinterpret_cast<const f32x4*>(p + int64_t(r) * D + d);
         }
         float top = M;
@@ -926,12 +1002,14 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int rpw) {
         const float was = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - top);
         o *= was;
         sum *= was;
+        if (WIN) sumx *= was;
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             if (i0 + i * NG + gi >= nseg) continue;
             // (a partial without an admitted token has sum 0 and O 0)
             const float wi = mi[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi[i] - top);
             sum += li[i] * wi;
+            if (WIN) sumx += xi[i] * wi;
             o += v[i] * wi;
         }
         M = top;
@@ -942,13 +1020,16 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int rpw) {
     const float own = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - top);
     o *= own;
     sum *= own;
+    if (WIN) sumx *= own;
 #pragma unroll
     for (int j = TPR; j < 64; j <<= 1) {
         sum += __shfl_xor(sum, j, 64);
+        if (WIN) sumx += __shfl_xor(sumx, j, 64);
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], j, 64);
     }
     if (gi != 0) return;
+    if (WIN && d == 0) a.lse[(int64_t(b) * a.S + s) * a.H + h] = log_sum<E>(top, sumx);
     const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
     *reinterpret_cast<uint2*>(a.out + ((int64_t(b) * a.S + s) * a.H + h) * D + d) =
         sum == 0.f ? make_uint2(0u, 0u) : make_uint2(E::pair(o[0] * inv, o[1] * inv), E::pair(o[2] * inv, o[3] * inv));
@@ -972,7 +1053,7 @@ __global__ __launch_bounds__(256) void block_score_kernel(PagedArgs a) {
     constexpr int QR = D + 2;  // (rows two doubles further apart: no bank conflicts)
     __shared__ __align__(16) double qs[SCORE_ROWS * QR];
     const int b = blockIdx.z / a.Hk, kh = blockIdx.z % a.Hk, s0 = blockIdx.y * SCORE_ROWS, ns = min(SCORE_ROWS, a.S - s0);
-    const int c = span_of<true>(a, a.length[b]).tail >> a.lt, j_end = c - a.local;
+    const int c = span_of<Kind::SEL>(a, a.length[b], 0).tail >> a.lt, j_end = c - a.local;
     if (c <= a.most || a.sink + int(blockIdx.x) * 64 >= j_end) return;  // (uniform: all pages are selected, or none is scored here)
     const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
     const int j = a.sink + int(blockIdx.x) * 64 + int(threadIdx.x >> 6) * 16 + c16;
@@ -1069,7 +1150,7 @@ __global__ __launch_bounds__(NT) void block_select_kernel(PagedArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const int64_t unit = blockIdx.x;
     const int b = int(unit / (int64_t(a.S) * a.Hk));
-    const int c = span_of<true>(a, a.length[b]).tail >> a.lt;
+    const int c = span_of<Kind::SEL>(a, a.length[b], 0).tail >> a.lt;
     int32_t* sel = a.sel + unit * a.most;
     int32_t* page = a.page + unit * a.most;
     const int32_t* row = a.table + b * a.ts;
@@ -1259,16 +1340,23 @@ __global__ __launch_bounds__(NT) void block_select_kernel(PagedArgs a) {
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------
-// The most tokens a unit can have: all that the table (or a selection) holds, and the rows' own.
-int64_t most_tokens(const PagedArgs& a, bool sel) {
-    const int64_t pages = sel && a.most < a.W ? a.most + 1 : a.W;
+// The most tokens a unit can have: all that the table (or a selection) holds, and the rows' own; in a window, that of its rows
+// and the first tokens, in whole stages.
+int64_t window_tokens(int64_t held, int64_t S, int64_t spb, int64_t window, int64_t first) {
+    const int64_t rows = S < 64 ? S : spb > 64 ? spb : 64, most = first + window + (rows < S ? rows : S) + 2 * WIN_STEP;
+    return most < held + S ? most : held + S;
+}
+template <Kind KIND>
+int64_t most_tokens(const PagedArgs& a) {
+    if (KIND == Kind::WIN) return window_tokens(int64_t(a.W) << a.lt, a.S, a.spb, a.window, a.first);
+    const int64_t pages = KIND == Kind::SEL && a.most < a.W ? a.most + 1 : a.W;
     return (pages << a.lt) + a.S;
 }
 
-template <class E, int D, int TPW, int RTW, int P, int WPC, bool SEL, int SUB = 1>
+template <class E, int D, int TPW, int RTW, int P, int WPC, Kind KIND, int SUB = 1>
 int launch(PagedArgs& a, hipStream_t st) {
     using Geo = Geometry<D, TPW, RTW, P, WPC, SUB>;
-    constexpr int joined = (RTW * P * 16 * (D + 4) + 2 * RTW * P * 16) * 4;
+    constexpr int joined = (RTW * P * 16 * (D + 4) + extra_of(KIND) * RTW * P * 16) * 4;
     constexpr int lds = Geo::RING > joined ? Geo::RING : joined;
     // (once per device and kernel: the call costs about a microsecond)
     static std::atomic<uint64_t> allowed{0};
@@ -1276,22 +1364,22 @@ int launch(PagedArgs& a, hipStream_t st) {
     MDX_HIP(hipGetDevice(&dev));
     const uint64_t bit = uint64_t(1) << (dev & 63);
     if (dev > 63 || !(allowed.load(std::memory_order_relaxed) & bit)) {
-        allow_smem(reinterpret_cast<const void*>(&paged_attn_kernel<E, D, TPW, RTW, P, WPC, SUB, SEL>), lds);
+        allow_smem(reinterpret_cast<const void*>(&paged_attn_kernel<E, D, TPW, RTW, P, WPC, SUB, KIND>), lds);
         allowed.fetch_or(bit, std::memory_order_relaxed);
     }
     // Row blocks enough for every work-group there is room for: whole ones, without partials, as long as no unit can be much
     // longer than the others (2048 rows over 1000 tokens: 122 us in shares, 90 whole; 16 x 128 rows over 1000 each: 87 and 52;
     // over 0 to 6000: 166 and 161; but with one sequence of 60000 among 15 of 500: 211 and 1437).
     const int units = a.B * a.Hk * a.units;
-    const int64_t most = most_tokens(a, SEL);
+    const int64_t most = most_tokens<KIND>(a);
     if (a.units > 1 && units >= CUS * WPC && (a.B == 1 || most <= EVEN_TOKENS || int64_t(units) * a.S >= most * CUS * WPC)) a.whole = 1;
     const int grid = a.whole ? units : CUS * WPC;
     a.by_unit = units <= grid;  // (every unit is begun by one share, which writes its entry)
-    hipLaunchKernelGGL((paged_attn_kernel<E, D, TPW, RTW, P, WPC, SUB, SEL>), dim3(unsigned(grid)), dim3(Geo::NT), lds, st, a);
+    hipLaunchKernelGGL((paged_attn_kernel<E, D, TPW, RTW, P, WPC, SUB, KIND>), dim3(unsigned(grid)), dim3(Geo::NT), lds, st, a);
     MDX_LAUNCHED();
     if (a.whole) return MDX_OK;
     const int rows = (a.spb < a.S ? a.spb : a.S) * a.G;
-    hipLaunchKernelGGL((paged_join_kernel<E, D>), dim3(unsigned(units < grid ? units : grid), unsigned((rows + 3) / 4)), dim3(256), 0, st, a,
+    hipLaunchKernelGGL((paged_join_kernel<E, D, KIND>), dim3(unsigned(units < grid ? units : grid), unsigned((rows + 3) / 4)), dim3(256), 0, st, a,
                        Geo::RPW);
     MDX_LAUNCHED();
     return MDX_OK;
@@ -1304,44 +1392,45 @@ int rpw_of(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64
 // but have fewer instructions one after the other (32 and 64 rows in one wave's registers: 20 against 15 us for 16 rows over
 // 1000 tokens of 8 kv heads, 120 against 106 for 16 sequences over 8000); only at head_dim 64 LDS is what bounds 64 rows where
 // there is much to stream (32 sequences of 16 rows over 8000: 106 us in one wave's registers, 117 in waves of their own).
-template <class E, int D, bool SEL>
+template <class E, int D, Kind KIND>
 int launch_rows(PagedArgs& a, hipStream_t st) {
+    constexpr bool SEL = KIND == Kind::SEL;
     const int rows = SEL ? a.G : a.units > 1 ? 128 : a.S * a.G;
-    const int64_t steps = int64_t(a.B) * a.Hk * a.units * ((most_tokens(a, SEL) + 127) / 128);
+    const int64_t steps = int64_t(a.B) * a.Hk * a.units * ((most_tokens<KIND>(a) + 127) / 128);
     const bool few = steps <= FEW_STEPS;
     // Two work-groups per CU where there is much to stream: one goes on while the other changes units (16 x 8 rows' selections
     // of 16 blocks: 121 -> 109 us, 200 single tokens over 10 to 500: 50 -> 46, 64 over at most 8192 at head_dim 64: 98 -> 93, at
     // 128: 195 -> 198; one token over 2000: 11.7 -> 12.1; at head_dim 256 a stage of 32 KiB leaves no ring for it).
     if (rows <= 16) {
-        if (few || D == 256) return launch<E, D, 1, 1, 4, 1, SEL>(a, st);
-        if constexpr (D != 256) return launch<E, D, 1, 1, 4, 2, SEL>(a, st);
+        if (few || D == 256) return launch<E, D, 1, 1, 4, 1, KIND>(a, st);
+        if constexpr (D != 256) return launch<E, D, 1, 1, 4, 2, KIND>(a, st);
     }
-    if (rows <= 32) return launch<E, D, 1, 2, (D == 256 ? 2 : 4), 1, SEL>(a, st);
+    if (rows <= 32) return launch<E, D, 1, 2, (D == 256 ? 2 : 4), 1, KIND>(a, st);
     if (rows <= 64) {
         if constexpr (D == 64)
-            if (!few) return launch<E, D, 4, 1, 4, 1, SEL>(a, st);
-        return launch<E, D, 1, 4, (D == 256 ? 1 : 2), 1, SEL>(a, st);
+            if (!few) return launch<E, D, 4, 1, 4, 1, KIND>(a, st);
+        return launch<E, D, 1, 4, (D == 256 ? 1 : 2), 1, KIND>(a, st);
     }
-    if constexpr (!SEL) return launch<E, D, 2, 4, 1, (D == 256 ? 1 : 2), SEL, (D == 256 ? 1 : 2)>(a, st);
+    if constexpr (!SEL) return launch<E, D, 2, 4, 1, (D == 256 ? 1 : 2), KIND, (D == 256 ? 1 : 2)>(a, st);
     set_error("at most 64 query heads per kv head");
     return MDX_EINVAL;
 }
 
-template <bool SEL>
+template <Kind KIND>
 int launch_any(PagedArgs& a, int D, int dtype, hipStream_t st) {
     if (dtype == MDX_DT_BF16) {
-        if (D == 64) return launch_rows<Bf16, 64, SEL>(a, st);
-        if (D == 128) return launch_rows<Bf16, 128, SEL>(a, st);
-        return launch_rows<Bf16, 256, SEL>(a, st);
+        if (D == 64) return launch_rows<Bf16, 64, KIND>(a, st);
+        if (D == 128) return launch_rows<Bf16, 128, KIND>(a, st);
+        return launch_rows<Bf16, 256, KIND>(a, st);
     }
-    if (D == 64) return launch_rows<Fp16, 64, SEL>(a, st);
-    if (D == 128) return launch_rows<Fp16, 128, SEL>(a, st);
-    return launch_rows<Fp16, 256, SEL>(a, st);
+    if (D == 64) return launch_rows<Fp16, 64, KIND>(a, st);
+    if (D == 128) return launch_rows<Fp16, 128, KIND>(a, st);
+    return launch_rows<Fp16, 256, KIND>(a, st);
 }
 
-size_t base_bytes(int64_t rows, int64_t D) {
+size_t base_bytes(int64_t rows, int64_t D, Kind kind) {
     const int rpw = rpw_of(rows), shares = rpw == 16 || rpw == 128 ? 2 * CUS : CUS;
-    return size_t(2 * CUS) * sizeof(int4) + size_t(shares) * 2 * rpw * (D + 2) * 4;
+    return size_t(2 * CUS) * sizeof(int4) + size_t(shares) * 2 * rpw * (D + extra_of(kind)) * 4;
 }
 
 int log2_of(int64_t T) {
@@ -1407,14 +1496,14 @@ static int64_t rows_of_unit(int64_t S, int64_t G) { return rpw_of(S * G) / G; }
 static int64_t blocks_of(int64_t S, int64_t G) { return G > 128 ? 0 : (S + rows_of_unit(S, G) - 1) / rows_of_unit(S, G); }
 
 // One work-group per unit, without a join: where a unit has few steps at most.
-static bool whole_units(int64_t B, int64_t S, int64_t H, int64_t Hk, int64_t T, int64_t W) {
+static bool whole_units(int64_t B, int64_t S, int64_t H, int64_t Hk, int64_t most) {
     const int64_t units = B * Hk * blocks_of(S, H / Hk);
-    return W * T + S <= (2 * units >= CUS && units <= CUS ? 2 : 1) * WHOLE_TOKENS && units <= 65536;
+    return most <= (2 * units >= CUS && units <= CUS ? 2 : 1) * WHOLE_TOKENS && units <= 65536;
 }
 
 extern "C" size_t mdx_attn_paged_workspace(int64_t B, int64_t S, int64_t H, int64_t Hk, int64_t D, int64_t T, int64_t W) {
     if (B < 1 || S < 1 || Hk < 1 || H < 1 || H % Hk != 0 || D < 1 || T < 1 || W < 1 || W > (int64_t(1) << 30)) return 0;
-    return whole_units(B, S, H, Hk, T, W) ? 0 : base_bytes(S * (H / Hk), D);
+    return whole_units(B, S, H, Hk, W * T + S) ? 0 : base_bytes(S * (H / Hk), D, Kind::ALL);
 }
 
 extern "C" int mdx_attn_paged(const void* q, int64_t q_seq_stride, int64_t q_row_stride, int64_t q_head_stride, const void* key,
@@ -1433,19 +1522,58 @@ extern "C" int mdx_attn_paged(const void* q, int64_t q_seq_stride, int64_t q_row
     const int64_t rows = S * (H / Hk), blocks = blocks_of(S, H / Hk);
     MDX_CHECK(rows < (int64_t(1) << 30) && B * Hk * blocks < (int64_t(1) << 30) && B * Hk * blocks * ((W * T + S) / STEP + 8) < MAX_LINE,
               "too many rows times tokens for one call");
-    a.whole = whole_units(B, S, H, Hk, T, W);
-    MDX_CHECK(a.whole || (workspace && aligned(workspace, 16) && workspace_bytes >= base_bytes(rows, D)),
-              "workspace: %zu bytes, 16-byte aligned", base_bytes(rows, D));
+    a.whole = whole_units(B, S, H, Hk, W * T + S);
+    MDX_CHECK(a.whole || (workspace && aligned(workspace, 16) && workspace_bytes >= base_bytes(rows, D, Kind::ALL)),
+              "workspace: %zu bytes, 16-byte aligned", base_bytes(rows, D, Kind::ALL));
     a.spb = int(rows_of_unit(S, H / Hk));
     a.units = int(blocks);
     a.info = static_cast<int4*>(workspace);
     a.part = reinterpret_cast<float*>(a.info + 2 * CUS);
-    return launch_any<false>(a, int(D), dtype, static_cast<hipStream_t>(stream));
+    return launch_any<Kind::ALL>(a, int(D), dtype, static_cast<hipStream_t>(stream));
+}
+
+extern "C" size_t mdx_attn_window_workspace(int64_t B, int64_t S, int64_t H, int64_t Hk, int64_t D, int64_t T, int64_t W,
+                                            int64_t window, int64_t sinks) {
+    if (B < 1 || S < 1 || Hk < 1 || H < 1 || H % Hk != 0 || H / Hk > 128 || D < 1 || T < 1 || W < 1 || W > (int64_t(1) << 30) || window < 1 ||
+        sinks < 0 || window > (int64_t(1) << 30) || sinks > (int64_t(1) << 30))
+        return 0;
+    const int64_t most = window_tokens(W * T, S, rows_of_unit(S, H / Hk), window, sinks);
+    return whole_units(B, S, H, Hk, most) ? 0 : base_bytes(S * (H / Hk), D, Kind::WIN);
+}
+
+extern "C" int mdx_attn_window(const void* q, int64_t q_seq_stride, int64_t q_row_stride, int64_t q_head_stride, const void* key,
+                               int64_t k_head_stride, int64_t k_page_stride, int64_t k_row_stride, const void* value,
+                               int64_t v_head_stride, int64_t v_page_stride, int64_t v_row_stride, int32_t dtype,
+                               const int32_t* table, int64_t table_stride, const int32_t* length, const int64_t* mask, void* out,
+                               float* lse, int64_t window, int64_t sinks, int64_t B, int64_t S, int64_t H, int64_t Hk, int64_t D,
+                               int64_t P, int64_t T, int64_t W, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+    MDX_CHECK(S >= 1 && (mask ? S <= 64 : S <= 65535), "1..64 rows with masks, 1..65535 without");
+    MDX_CHECK(lse && aligned(lse, 4), "null pointer");
+    MDX_CHECK(window >= 1 && window <= (int64_t(1) << 30) && sinks >= 0 && sinks <= (int64_t(1) << 30), "a window of 1..2^30 tokens, 0..2^30 first ones");
+    PagedArgs a{};
+    const int rc = fill(a, q, q_seq_stride, q_row_stride, q_head_stride, key, k_head_stride, k_page_stride, k_row_stride, value,
+                        v_head_stride, v_page_stride, v_row_stride, dtype, table, table_stride, length, mask, out, B, S, H, Hk, D, P,
+                        T, W, scale);
+    if (rc != MDX_OK) return rc;
+    MDX_CHECK(H / Hk <= 128, "at most 128 query heads per kv head");
+    const int64_t rows = S * (H / Hk), blocks = blocks_of(S, H / Hk), most = window_tokens(W * T, S, rows_of_unit(S, H / Hk), window, sinks);
+    MDX_CHECK(rows < (int64_t(1) << 30) && B * Hk * blocks < (int64_t(1) << 30) && B * Hk * blocks * (most / STEP + 8) < MAX_LINE,
+              "too many rows times tokens for one call");
+    a.whole = whole_units(B, S, H, Hk, most);
+    MDX_CHECK(a.whole || (workspace && aligned(workspace, 16) && workspace_bytes >= base_bytes(rows, D, Kind::WIN)),
+              "workspace: %zu bytes, 16-byte aligned", base_bytes(rows, D, Kind::WIN));
+    a.spb = int(rows_of_unit(S, H / Hk));
+    a.units = int(blocks);
+    a.first = int(sinks), a.window = int(window);
+    a.lse = lse;
+    a.info = static_cast<int4*>(workspace);
+    a.part = reinterpret_cast<float*>(a.info + 2 * CUS);
+    return launch_any<Kind::WIN>(a, int(D), dtype, static_cast<hipStream_t>(stream));
 }
 
 extern "C" size_t mdx_attn_blocks_workspace(int64_t B, int64_t S, int64_t H, int64_t Hk, int64_t D, int64_t W, int64_t most) {
     if (B < 1 || S < 1 || Hk < 1 || H < 1 || H % Hk != 0 || D < 1 || W < 1 || most < 1) return 0;
-    return base_bytes(H / Hk, D) + size_t(B * S * Hk) * (size_t(W) * 8 + size_t((most + 3) / 4 * 4) * 4);
+    return base_bytes(H / Hk, D, Kind::SEL) + size_t(B * S * Hk) * (size_t(W) * 8 + size_t((most + 3) / 4 * 4) * 4);
 }
 
 extern "C" int mdx_attn_blocks(const void* q, int64_t q_seq_stride, int64_t q_row_stride, int64_t q_head_stride, const void* key,
@@ -1482,7 +1610,7 @@ extern "C" int mdx_attn_blocks(const void* q, int64_t q_seq_stride, int64_t q_ro
     a.sel = sel;
     a.info = static_cast<int4*>(workspace);
     a.part = reinterpret_cast<float*>(a.info + 2 * CUS);
-    a.keys = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + base_bytes(a.G, D));
+    a.keys = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + base_bytes(a.G, D, Kind::SEL));
     a.page = reinterpret_cast<int32_t*>(a.keys + units * W);
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (W > most) {  // (else every full page is selected)
@@ -1506,5 +1634,5 @@ extern "C" int mdx_attn_blocks(const void* q, int64_t q_seq_stride, int64_t q_ro
     else if (W <= 16384) hipLaunchKernelGGL((block_select_kernel<1024, 16>), dim3(unsigned(units)), dim3(1024), 0, st, a);
     else hipLaunchKernelGGL((block_select_kernel<1024, 64>), dim3(unsigned(units)), dim3(1024), 0, st, a);
     MDX_LAUNCHED();
-    return launch_any<true>(a, int(D), dtype, st);
+    return launch_any<Kind::SEL>(a, int(D), dtype, st);
 }

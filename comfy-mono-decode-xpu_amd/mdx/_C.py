@@ -1349,6 +1349,14 @@ def attn_blocks(q, key, value, ksum, table, length, blocks, sink=1, local=1, mas
     return (_bind or _bound()).attn_blocks(q, key, value, ksum, table, length, blocks, sink, local, mask, scale, out, sel)
 
 
+def attn_window(q, key, value, table, length, window, sinks=0, mask=None, scale=None, out=None, lse=None):
+    """attn_paged within a sliding window: of the tokens that a row attends there, in order (the committed ones, then those of
+    the rows' own that its mask admits), it attends the first `sinks` and the last `window` (None: all). The other operands
+    are attn_paged's. Returns (out [B, S, H, D], lse float32 [B, S, H]): lse is the log of the row's sum of
+    exp(scale q . k), -inf for a row that admits nothing (attn_mass takes it). No counterpart in the reference."""
+    return (_bind or _bound()).attn_window(q, key, value, table, length, window, sinks, mask, scale, out, lse)
+
+
 def verify_drafts(logits, tokens, uniform, draft=None, parent=None, temperature=1.0):
     """The step's drafted tokens against the target's probabilities p_r = softmax(logits[b, r] / temperature): logits [B, R, V]
     (bf16, fp16 or fp32), row 0 the last committed token's, row r >= 1 holding the drafted token tokens[b, r] (int64; outside

@@ -649,6 +649,19 @@ int mdx_attn_blocks(const void* q, int64_t q_seq_stride, int64_t q_row_stride, i
                     int64_t S, int64_t H, int64_t Hk, int64_t D, int64_t P, int64_t T, int64_t W, float scale, void* workspace,
                     size_t workspace_bytes, void* stream);
 
+/* mdx_attn_paged within a window: of the tokens that a row attends there, in order (the committed ones, then the own ones it
+ * admits), the first `sinks` and the last `window` (sinks 0..2^30, window 1..2^30). lse f32 [B, S, H]: log of the sum of
+ * exp(scale q . k) over them, -inf for none. A token in no page keeps its place in the order. No counterpart in the
+ * reference. */
+size_t mdx_attn_window_workspace(int64_t B, int64_t S, int64_t H, int64_t Hk, int64_t D, int64_t T, int64_t W, int64_t window,
+                                 int64_t sinks);
+int mdx_attn_window(const void* q, int64_t q_seq_stride, int64_t q_row_stride, int64_t q_head_stride, const void* key,
+                    int64_t k_head_stride, int64_t k_page_stride, int64_t k_row_stride, const void* value,
+                    int64_t v_head_stride, int64_t v_page_stride, int64_t v_row_stride, int32_t dtype, const int32_t* table,
+                    int64_t table_stride, const int32_t* length, const int64_t* mask, void* out, float* lse, int64_t window,
+                    int64_t sinks, int64_t B, int64_t S, int64_t H, int64_t Hk, int64_t D, int64_t P, int64_t T, int64_t W,
+                    float scale, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- a step's answers --------------------------------------------------------------------------------
  * Verification of drafted tokens against the target's probabilities. p_r = softmax(logits[b][r] / T), T the sequence's
  * temperature (temperatures f32 [B], or `temperature` for all with NULL; 0 and below: 1 at the lowest index of the maximum); a

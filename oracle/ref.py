@@ -986,6 +986,41 @@ def paged_attention(q, key, value, table, length, mask, scale, keep=None):
     return out, spread, mass, heft
 
 
+def window_keep(mask, length, S, window, sinks):
+    """paged_attention's `keep` of rows that attend, of their tokens in order (committed, then own admitted ones), the first
+    `sinks` and the last `window`."""
+    def keep(b, s, kh, pos):
+        n = int(length[b])
+        own = list(range(s + 1)) if mask is None else [j for j in range(S) if (int(mask[b, s]) >> j) & 1]
+        count = n + len(own)
+        place = {n + j: n + i for i, j in enumerate(own)}  # a token's number among the row's
+        number = np.array([int(p) if p < n else place.get(int(p), -1) for p in pos], dtype=np.int64)
+        return (number >= 0) & ((number < sinks) | (number >= count - window))
+    return keep
+
+
+def paged_lse(q, key, table, length, mask, scale, keep=None):
+    """float64 log-sum-exp of every row's scores [B, S, H], -inf where it attends nothing (operands: paged_attention's)."""
+    B, S, H, _ = q.shape
+    Hk, P, T, _ = key.shape
+    G = H // Hk
+    out = np.full((B, S, H), -np.inf)
+    for b in range(B):
+        n = int(length[b])
+        pos, page, row = paged_tokens(table, length, T, P, b, S)
+        for s in range(S):
+            own = pos - n
+            seen = own <= s if mask is None else np.array([o < 0 or (int(mask[b, s]) >> int(o)) & 1 == 1 for o in own], dtype=bool)
+            for kh in range(Hk):
+                use = seen if keep is None else seen & keep(b, s, kh, pos)
+                if not use.any():
+                    continue
+                z = key[kh, page[use], row[use]] @ q[b, s, kh * G:(kh + 1) * G].T * scale
+                top = z.max(0)
+                out[b, s, kh * G:(kh + 1) * G] = top + np.log(np.exp(z - top).sum(0))
+    return out
+
+
 def block_selection(q, ksum, table, length, T, blocks, sink, local):
     """The pages that each row and kv head selects: int [B, S, Hk, sink + local + blocks], ascending, -1 behind. q [B, S, H, D]
     and ksum [Hk, P, D] float64."""
