@@ -9,6 +9,7 @@
 #include <Python.h>
 
 #include <ATen/ops/empty.h>
+#include <ATen/ops/zeros.h>
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -35,8 +36,9 @@ struct Entries {
     decltype(&mdx_verify_drafts) verify;
     decltype(&mdx_attn_window_workspace) window_workspace;
     decltype(&mdx_attn_window) window;
+    decltype(&mdx_attn_mass) mass;
 } g;
-constexpr int ENTRIES = 13;
+constexpr int ENTRIES = 14;
 PyObject* g_error = nullptr;  // _lib.MdxError
 
 struct Refused : std::runtime_error {
@@ -376,6 +378,70 @@ PyObject* attn_window(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     });
 }
 
+// q, key, table, length, lse, prior, count, path, window, sinks, scale, out -> out
+PyObject* attn_mass(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    EXPECT(12, "attn_mass")
+    return guarded([&]() -> PyObject* {
+        const at::Tensor& q = tensor(a[0], "q");
+        const c10::Device d = rocm_device(q);
+        const at::Tensor &key = on(a[1], "key", d), &table = on(a[2], "table", d), &length = on(a[3], "length", d), &lse = on(a[4], "lse", d);
+        const int32_t dt = code_of(q);
+        check(dt >= 0 && key.scalar_type() == q.scalar_type(), "q and key: bf16 or fp16, one type");
+        check(q.dim() == 4 && q.stride(3) == 1, "q: [sequences, rows, heads, head_dim], the last dim contiguous");
+        const int64_t B = q.size(0), S = q.size(1), H = q.size(2), D = q.size(3);
+        check(key.dim() == 4 && key.size(3) == D && key.stride(3) == 1, "key: [kv_heads, pages, page rows, head_dim], the last dim contiguous");
+        const int64_t Hk = key.size(0), P = key.size(1), T = key.size(2);
+        check(Hk >= 1 && H % Hk == 0, "query heads: a multiple of the kv heads");
+        check(table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) == B && table.stride(1) == 1 && table.stride(0) >= table.size(1),
+              "table: int32 [sequences, W], rows contiguous");
+        const int64_t W = table.size(1);
+        ints(length, "length", {B});
+        check(lse.scalar_type() == at::kFloat && lse.sizes() == at::IntArrayRef({B, S, H}) && lse.is_contiguous(),
+              "lse: contiguous float32 [sequences, rows, heads]");
+        const int32_t *count = nullptr, *path = nullptr;
+        if (given(a[6])) {
+            const at::Tensor& t = on(a[6], "count", d);
+            ints(t, "count", {B});
+            count = t.data_ptr<int32_t>();
+        }
+        if (given(a[7])) {
+            const at::Tensor& t = on(a[7], "path", d);
+            ints(t, "path", {B, S});
+            path = t.data_ptr<int32_t>();
+        }
+        const int64_t window = window_of(a[8]), sinks = number(a[9]);
+        check(sinks >= 0 && sinks <= (int64_t(1) << 30), "sinks: 0..2^30 tokens");
+        const float scale = scale_of(a[10], D);
+        auto sums = [&](const at::Tensor& t, const char* what) {
+            check(t.scalar_type() == at::kFloat && t.dim() == 3 && t.size(0) == B && t.size(1) == Hk && t.size(2) >= 1 && t.stride(2) == 1, what);
+        };
+        const float* prior = nullptr;
+        int64_t pb = 0, ph = 0, N = W * T;
+        if (given(a[5])) {
+            const at::Tensor& t = on(a[5], "prior", d);
+            sums(t, "prior: float32 [sequences, kv_heads, places], rows contiguous");
+            prior = t.data_ptr<float>();
+            pb = t.stride(0), ph = t.stride(1), N = t.size(2);
+        }
+        at::Tensor out;
+        if (given(a[11])) {
+            out = on(a[11], "out", d);
+            sums(out, "out: float32 [sequences, kv_heads, places], rows contiguous");
+            check(!prior || out.size(2) == N, "prior and out: as many places");
+            N = out.size(2);
+        } else {
+            out = at::zeros({B, Hk, N}, at::TensorOptions().dtype(at::kFloat).device(d));
+        }
+        if (B > 0 && S > 0)
+            call("mdx_attn_mass", d, [&](void* st) {
+                return g.mass(data(q), q.stride(0), q.stride(1), q.stride(2), data(key), key.stride(0), key.stride(1), key.stride(2), dt,
+                              table.data_ptr<int32_t>(), table.stride(0), length.data_ptr<int32_t>(), lse.data_ptr<float>(), prior, pb, ph, count,
+                              path, window, sinks, out.data_ptr<float>(), out.stride(0), out.stride(1), N, B, S, H, Hk, D, P, T, W, scale, st);
+            });
+        return same_or_new(a[11], out);
+    });
+}
+
 // ---- a step's answers ----
 // logits, tokens, uniform, draft, parent, temperature -> (count, path, next)
 PyObject* verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
@@ -463,6 +529,7 @@ PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     g.verify = reinterpret_cast<decltype(g.verify)>(p[i++]);
     g.window_workspace = reinterpret_cast<decltype(g.window_workspace)>(p[i++]);
     g.window = reinterpret_cast<decltype(g.window)>(p[i++]);
+    g.mass = reinterpret_cast<decltype(g.mass)>(p[i++]);
     Py_XINCREF(a[ENTRIES]);
     Py_XDECREF(g_error);
     g_error = a[ENTRIES];
@@ -476,6 +543,7 @@ PyMethodDef methods[] = {{"init", FAST(init), METH_FASTCALL, nullptr},
                          {"attn_paged", FAST(attn_paged), METH_FASTCALL, nullptr},
                          {"attn_blocks", FAST(attn_blocks), METH_FASTCALL, nullptr},
                          {"attn_window", FAST(attn_window), METH_FASTCALL, nullptr},
+                         {"attn_mass", FAST(attn_mass), METH_FASTCALL, nullptr},
                          {"verify_drafts", FAST(verify_drafts), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_bind", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -1,0 +1,275 @@
+// The attention weight that cached tokens draw, summed up (mdx_attn_mass): what an eviction goes by (mdx_page_evict).
+//
+// out[b][g][t] = (t < n ? prior[b][g][t] : 0) + sum over rows k < count[b] that attend t and the heads h of kv head g of
+// exp(scale q[b][path[b][k]][h] . key_t - lse[b][path[b][k]][h]); row k attends the tokens t <= n + k (n = length[b]; a row's own
+// place is n + k), of these the first `sinks` and the last `window`. lse is the rows' log-sum-exp of mdx_attn_window, so a
+// weight needs nothing but its own score: the keys are read once and no token waits for another.
+//
+// S^T = K Q^T by v_mfma_f32_16x16x32 (A: 16 tokens x 32 dims, B: 16 query rows, the lane holds scores of one row and four
+// tokens), keys straight from the pages to registers (16 bytes per lane and load, whole 64-byte pieces of 16 tokens), one
+// exponential per score, fp32 sums per token in the lane, joined over the 16 rows' lanes at the end by exchanges that halve the
+// values (45 instructions for 64 tokens instead of 64 sums). A token's sum is one wave's (or a work-group's waves', joined in their
+// order): no atomics, the same bits every time. What a row does not attend is selected out, not multiplied: non-finite keys
+// there do not reach it.
+//
+// Few rows: a wave per 16 TT tokens, bound by the keys' bytes. Many rows: the four waves of a work-group take the row tiles of one
+// run of 16 TT tokens in turn; bound by the exponentials and the matrix instructions in about equal parts.
+//
+// Reference: none (its cache is never thinned).
+#include "mdx_common.hpp"
+
+namespace mdx {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+struct Bf16 {
+    static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+};
+struct Fp16 {
+    static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+};
+
+struct MassArgs {
+    const uint16_t* q;  // [B, S, H, D], strides qb, qs, qh
+    int64_t qb, qs, qh;
+    const uint16_t* key;  // [Hk, P, T, D], strides kh, kp, kt
+    int64_t kh, kp, kt;
+    const int32_t* table;  // [B, W], row stride ts
+    int64_t ts;
+    const int32_t* length;  // [B]
+    const float* lse;       // [B, S, H]
+    const float* prior;     // [B, Hk, N], strides pb, ph; null: zeros
+    int64_t pb, ph;
+    const int32_t* count;  // [B] or null (S)
+    const int32_t* path;   // [B, S] or null (row k is k)
+    float* out;            // [B, Hk, N], strides ob, oh
+    int64_t ob, oh;
+    int B, S, H, Hk, G, W, P, lt, N;
+    int window, sinks;
+    int tiles;  // runs of tokens that the grid covers at once
+    float zs;   // scale * log2(e)
+};
+
+// the sums of 16 (V = 16) or 8 values over a row of 16 lanes: lane c16 receives value c16 (V = 8: value c16 % 8)
+template <int CTRL>
+__device__ __forceinline__ float other(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, false));
+}
+template <int N, int CTRL>
+__device__ __forceinline__ void halve(float* v, bool up) {  // (the partner across has the other half's sums)
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const float keep = up ? v[j + N] : v[j], give = up ? v[j] : v[j + N];
+        v[j] = keep + other<CTRL>(give);
+    }
+}
+constexpr int ROR8 = 0x128, HALF_MIRROR = 0x141, QUAD_REVERSE = 0x1B, QUAD_SWAP = 0xB1;  // lane ^ 8, ^ 7, ^ 3, ^ 1
+template <int V>
+__device__ __forceinline__ float row_sums(float* v, int c16) {
+    if constexpr (V == 16) {
+        halve<8, ROR8>(v, c16 & 8);
+    } else {
+        static_assert(V == 8, "");
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += other<ROR8>(v[j]);
+    }
+    halve<4, HALF_MIRROR>(v, c16 & 4);
+    halve<2, QUAD_REVERSE>(v, c16 & 2);
+    halve<1, QUAD_SWAP>(v, c16 & 1);
+    return v[0];
+}
+
+typedef __attribute__((address_space(4))) const int32_t* const_i32p;
+__device__ __forceinline__ int uload(const int32_t* p) { return *(const_i32p)(p); }  // (a scalar load: uniform addresses)
+
+// TT tiles of 16 tokens per wave; SPLIT: the four waves of the work-group share them and take the row tiles in turn.
+template <class E, int D, int TT, bool SPLIT>
+__global__ __launch_bounds__(256) void attn_mass_kernel(MassArgs a) {
+    constexpr int KK = D / 32, TOK = 16 * TT, RUN = SPLIT ? TOK : 4 * TOK;
+    static_assert(TT == 2 || TT == 4, "");
+    __shared__ float part[SPLIT ? 4 : 1][TOK];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c16 = lane & 15;
+    // (kv heads in turn: an XCD's work-groups share the queries of one)
+    const int kh = int(blockIdx.x) % a.Hk, rest = int(blockIdx.x) / a.Hk, b = rest / a.tiles;
+    const int n = max(0, min(uload(a.length + b), a.W << a.lt));
+    const int rows = a.count ? max(0, min(uload(a.count + b), a.S)) : a.S;
+    const int end = min(min(n + rows, a.W << a.lt), a.N);
+    const int32_t* trow = a.table + b * a.ts;
+    for (int run = rest % a.tiles; run * RUN < end; run += a.tiles) {
+        const int t0 = run * RUN + (SPLIT ? 0 : w * TOK);
+        if (!SPLIT && t0 >= end) continue;
+        // ---- the tokens' keys, as A operands
+        u32x4 kf[TT][KK];
+        uint32_t there = 0;  // tiles that stand in a page
+#pragma unroll
+        for (int i = 0; i < TT; ++i) {
+            const int t = t0 + 16 * i, e = t < end ? uload(trow + (t >> a.lt)) : -1;
+            const bool in = uint32_t(e) < uint32_t(a.P);
+            there |= in ? 1u << i : 0u;
+            // (a tile without a page reads the pool's first rows: in bounds, and selected out)
+            const uint16_t* src = a.key + kh * a.kh + (in ? int64_t(e) * a.kp + int64_t(t & ((1 << a.lt) - 1)) * a.kt : 0) + c16 * a.kt + 8 * g;
+#pragma unroll
+            for (int k = 0; k < KK; ++k) kf[i][k] = *reinterpret_cast<const u32x4*>(src + 32 * k);
+        }
+        f32x4 sum[TT];
+#pragma unroll
+        for (int i = 0; i < TT; ++i) sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        // ---- row tiles that can attend a token of the run: rows k from t0 - n on, and in a window up to the last token's
+        const int k_first = max(0, t0 - n);
+        const int64_t k_last = t0 < a.sinks ? rows - 1 : min(int64_t(rows) - 1, int64_t(t0) + TOK - 2 - n + a.window);
+        const int r_first = k_first * a.G / 16, r_end = k_last < 0 || there == 0 ? 0 : int((k_last + 1) * a.G + 15) / 16;
+        for (int rt = r_first + (SPLIT ? w : 0); rt < r_end; rt += SPLIT ? 4 : 1) {
+            const int r = rt * 16 + c16, k = r / a.G, h = kh * a.G + r % a.G;
+            const bool row = k < rows;
+            int s = row ? k : 0;
+            if (a.path) s = a.path[int64_t(b) * a.S + s];
+            const bool in = row && uint32_t(s) < uint32_t(a.S);
+            s = in ? s : 0;
+            const float base = a.lse[(int64_t(b) * a.S + s) * a.H + (row ? h : kh * a.G)];
+            const bool live = in && base > -INFINITY;
+            const uint16_t* src = a.q + b * a.qb + s * a.qs + (row ? h : kh * a.G) * a.qh + 8 * g;
+            u32x4 qf[KK];
+#pragma unroll
+            for (int i = 0; i < KK; ++i) qf[i] = *reinterpret_cast<const u32x4*>(src + 32 * i);
+            const float sub = base * 1.44269504088896340736f;
+            // this row's tokens: t < lim, and t < sinks or t >= lim - window
+            const int lim = n + k + 1, lo = lim - a.window;
+            // (uniform) every row of the tile attends every token of the run
+            const bool whole = there == (1u << TT) - 1u && __builtin_amdgcn_ballot_w64(!live) == 0 &&
+                               t0 + TOK <= n + rt * 16 / a.G + 1 &&
+                               (t0 + TOK <= a.sinks || t0 >= n + (rt * 16 + 15) / a.G + 1 - a.window);
+#pragma unroll
+            for (int i = 0; i < TT; ++i) {
+                f32x4 z = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int x = 0; x < KK; ++x) z = E::mfma(kf[i][x], qf[x], z);
+                if (whole) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum[i][e] += __builtin_amdgcn_exp2f(fmaf(z[e], a.zs, -sub));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int t = t0 + 16 * i + 4 * g + e;
+                        const bool seen = live && ((there >> i) & 1u) && t < lim && (t < a.sinks || t >= lo);
+                        const float x = __builtin_amdgcn_exp2f(fmaf(z[e], a.zs, -sub));
+                        sum[i][e] += seen ? x : 0.f;
+                    }
+                }
+            }
+        }
+        float v[4 * TT];
+#pragma unroll
+        for (int i = 0; i < TT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[4 * i + e] = sum[i][e];
+        const float mine = row_sums<4 * TT>(v, c16);
+        const int token = 16 * ((c16 % (4 * TT)) >> 2) + 4 * g + (c16 & 3);
+        auto put = [&](int t, float x) {
+            if (t >= end) return;
+            const float p = t < n && a.prior ? a.prior[b * a.pb + kh * a.ph + t] : 0.f;
+            a.out[b * a.ob + kh * a.oh + t] = p + x;
+        };
+        if constexpr (SPLIT) {
+            if (c16 < 4 * TT) part[w][token] = mine;
+            __syncthreads();
+            if (threadIdx.x < TOK)
+                put(t0 + int(threadIdx.x), (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]));
+            __syncthreads();
+        } else {
+            if (c16 < 4 * TT) put(t0 + token, mine);
+        }
+    }
+}
+
+constexpr int64_t MOST_GROUPS = 65536;  // work-groups of a launch at most (further runs in a loop)
+template <class E, int D, int TT, bool SPLIT>
+int launch(MassArgs& a, hipStream_t st) {
+    const int64_t most = int64_t(a.W) << a.lt, tokens = most < a.N ? most : a.N, run = SPLIT ? 16 * TT : 64 * TT, pairs = int64_t(a.B) * a.Hk;
+    int64_t tiles = (tokens + run - 1) / run;
+    if (tiles * pairs > MOST_GROUPS) tiles = MOST_GROUPS / pairs > 0 ? MOST_GROUPS / pairs : 1;
+    a.tiles = int(tiles);
+    hipLaunchKernelGGL((attn_mass_kernel<E, D, TT, SPLIT>), dim3(unsigned(tiles * pairs)), dim3(256), 0, st, a);
+    MDX_LAUNCHED();
+    return MDX_OK;
+}
+template <class E, int D>
+int launch_rows(MassArgs& a, hipStream_t st) {
+    constexpr int TT = D == 256 ? 2 : 4;
+    if (int64_t(a.S) * a.G <= 64) return launch<E, D, TT, false>(a, st);
+    return launch<E, D, TT, true>(a, st);
+}
+template <class E>
+int launch_any(MassArgs& a, int64_t D, hipStream_t st) {
+    return D == 64 ? launch_rows<E, 64>(a, st) : D == 128 ? launch_rows<E, 128>(a, st) : launch_rows<E, 256>(a, st);
+}
+
+int log2_of(int64_t T) {
+    for (int i = 4; i <= 10; ++i)
+        if (T == int64_t(1) << i) return i;
+    return -1;
+}
+
+}  // namespace
+}  // namespace mdx
+
+using namespace mdx;
+
+extern "C" int mdx_attn_mass(const void* q, int64_t q_seq_stride, int64_t q_row_stride, int64_t q_head_stride, const void* key,
+                             int64_t k_head_stride, int64_t k_page_stride, int64_t k_row_stride, int32_t dtype, const int32_t* table,
+                             int64_t table_stride, const int32_t* length, const float* lse, const float* prior, int64_t prior_seq_stride,
+                             int64_t prior_head_stride, const int32_t* count, const int32_t* path, int64_t window, int64_t sinks,
+                             float* out, int64_t out_seq_stride, int64_t out_head_stride, int64_t N, int64_t B, int64_t S, int64_t H,
+                             int64_t Hk, int64_t D, int64_t P, int64_t T, int64_t W, float scale, void* stream) {
+    MDX_CHECK(q && key && table && length && lse && out, "null pointer");
+    MDX_CHECK(dtype == MDX_DT_BF16 || dtype == MDX_DT_F16, "bf16 or fp16");
+    MDX_CHECK(D == 64 || D == 128 || D == 256, "head_dim must be 64, 128 or 256");
+    const int lt = log2_of(T);
+    MDX_CHECK(lt >= 0, "page rows: a power of two in 16..1024");
+    MDX_CHECK(B >= 1 && B <= 1024 && S >= 1 && S <= 65535 && Hk >= 1 && Hk <= 1024 && H >= 1 && H % Hk == 0 && H <= 65536 && H / Hk <= 128,
+              "1..1024 sequences, 1..65535 rows, heads (at most 128 per kv head)");
+    MDX_CHECK(P >= 1 && P <= (int64_t(1) << 30) && W >= 1 && (W << lt) < (int64_t(1) << 30) && table_stride >= W &&
+                  table_stride <= (int64_t(1) << 26),
+              "pages, table [sequences, W], under 2^30 tokens a sequence");
+    const int64_t lim = int64_t(1) << 40;
+    MDX_CHECK(k_row_stride >= D && k_row_stride <= (int64_t(1) << 24) && k_head_stride >= 0 && k_page_stride >= 0 && k_head_stride < lim &&
+                  k_page_stride < lim && q_seq_stride >= 0 && q_row_stride >= 0 && q_head_stride >= 0 && q_seq_stride < lim &&
+                  q_row_stride < lim && q_head_stride < lim,
+              "strides");
+    MDX_CHECK(aligned(q, 16) && aligned(key, 16) && q_seq_stride % 8 == 0 && q_row_stride % 8 == 0 && q_head_stride % 8 == 0 &&
+                  k_head_stride % 8 == 0 && k_page_stride % 8 == 0 && k_row_stride % 8 == 0 && aligned(lse, 4) && aligned(out, 4) && aligned(prior, 4),
+              "16-byte aligned rows");
+    MDX_CHECK(N >= 1 && N <= (int64_t(1) << 30) && out_head_stride >= N && out_seq_stride >= 0 && out_head_stride < lim && out_seq_stride < lim &&
+                  (Hk == 1 || B == 1 || out_seq_stride >= (Hk - 1) * out_head_stride + N) && (B == 1 || out_seq_stride >= N),
+              "sums [sequences, kv heads, places]: apart from one another");
+    MDX_CHECK(!prior || (prior_seq_stride >= 0 && prior_head_stride >= 0 && prior_seq_stride < lim && prior_head_stride < lim), "prior strides");
+    MDX_CHECK(window >= 1 && window <= (int64_t(1) << 30) && sinks >= 0 && sinks <= (int64_t(1) << 30), "a window of 1..2^30 tokens, 0..2^30 first ones");
+    MDX_CHECK(scale > 0.f && scale < INFINITY, "a positive, finite scale");
+    MassArgs a{};
+    a.q = static_cast<const uint16_t*>(q);
+    a.qb = q_seq_stride, a.qs = q_row_stride, a.qh = q_head_stride;
+    a.key = static_cast<const uint16_t*>(key);
+    a.kh = k_head_stride, a.kp = k_page_stride, a.kt = k_row_stride;
+    a.table = table;
+    a.ts = table_stride;
+    a.length = length;
+    a.lse = lse;
+    a.prior = prior;
+    a.pb = prior_seq_stride, a.ph = prior_head_stride;
+    a.count = count;
+    a.path = path;
+    a.out = out;
+    a.ob = out_seq_stride, a.oh = out_head_stride;
+    a.B = int(B), a.S = int(S), a.H = int(H), a.Hk = int(Hk), a.G = int(H / Hk), a.W = int(W), a.P = int(P), a.lt = lt, a.N = int(N);
+    a.window = int(window), a.sinks = int(sinks);
+    a.zs = float(double(scale) * 1.4426950408889634);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    return dtype == MDX_DT_BF16 ? launch_any<Bf16>(a, D, st) : launch_any<Fp16>(a, D, st);
+}

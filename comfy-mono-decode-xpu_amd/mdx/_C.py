@@ -1357,6 +1357,18 @@ def attn_window(q, key, value, table, length, window, sinks=0, mask=None, scale=
     return (_bind or _bound()).attn_window(q, key, value, table, length, window, sinks, mask, scale, out, lse)
 
 
+def attn_mass(q, key, table, length, lse, prior=None, count=None, path=None, window=None, sinks=0, scale=None, out=None):
+    """The attention weight that cached tokens have drawn, summed up over the rows and query heads of a kv head (page_evict goes
+    by it): out[b, g, t] = prior[b, g, t] (0 for the step's own tokens, t >= length[b]) + the sum over rows k < count[b] (None:
+    all S) and the heads h of kv head g of exp(scale q[b, r, h] . key_t - lse[b, r, h]), r = path[b, k] (None: k). Row k stands
+    at place length[b] + k and attends what is not behind it, of that the first `sinks` and the last `window` (None: all). q
+    [B, S, H, D] and lse [B, S, H] are attn_window's, count and path verify_drafts' and page_commit's: the call goes behind the
+    commit, with the lengths of before, and refused rows give nothing. key [Hk, P, T, D]: a layer's keys. prior, out float32
+    [B, Hk, N] (out may be prior; default: new, zeros elsewhere); places from length[b] + count[b] on stay. No counterpart in
+    the reference."""
+    return (_bind or _bound()).attn_mass(q, key, table, length, lse, prior, count, path, window, sinks, scale, out)
+
+
 def verify_drafts(logits, tokens, uniform, draft=None, parent=None, temperature=1.0):
     """The step's drafted tokens against the target's probabilities p_r = softmax(logits[b, r] / temperature): logits [B, R, V]
     (bf16, fp16 or fp32), row 0 the last committed token's, row r >= 1 holding the drafted token tokens[b, r] (int64; outside

@@ -662,6 +662,20 @@ int mdx_attn_window(const void* q, int64_t q_seq_stride, int64_t q_row_stride, i
                     int64_t sinks, int64_t B, int64_t S, int64_t H, int64_t Hk, int64_t D, int64_t P, int64_t T, int64_t W,
                     float scale, void* workspace, size_t workspace_bytes, void* stream);
 
+/* The attention weight that tokens draw, summed up: out[b][g][t] = (t < n ? prior[b][g][t] : 0) + the sum over the rows
+ * k < count[b] (NULL: S) that attend t and the heads h of kv head g of exp(scale q[b][r][h] . key_t - lse[b][r][h]), r =
+ * path[b][k] (int32 [B][S]; NULL: k), for t < n + count[b], n = length[b]; places behind stay. Row k's own place is n + k (as
+ * mdx_page_commit leaves a path's rows): it attends t <= n + k, of these the first `sinks` and the last `window`
+ * (mdx_attn_window's). lse f32 [B, S, H] contiguous; a row whose lse is -inf or whose r is none gives nothing, a token in no
+ * page draws nothing. prior, out f32 [B, Hk, N] (strides in elements; rows contiguous; out may be prior, with its strides).
+ * fp32 sums, the same bits every time. Other operands as mdx_attn_paged. No counterpart in the reference. */
+int mdx_attn_mass(const void* q, int64_t q_seq_stride, int64_t q_row_stride, int64_t q_head_stride, const void* key,
+                  int64_t k_head_stride, int64_t k_page_stride, int64_t k_row_stride, int32_t dtype, const int32_t* table,
+                  int64_t table_stride, const int32_t* length, const float* lse, const float* prior, int64_t prior_seq_stride,
+                  int64_t prior_head_stride, const int32_t* count, const int32_t* path, int64_t window, int64_t sinks,
+                  float* out, int64_t out_seq_stride, int64_t out_head_stride, int64_t N, int64_t B, int64_t S, int64_t H,
+                  int64_t Hk, int64_t D, int64_t P, int64_t T, int64_t W, float scale, void* stream);
+
 /* ---- a step's answers --------------------------------------------------------------------------------
  * Verification of drafted tokens against the target's probabilities. p_r = softmax(logits[b][r] / T), T the sequence's
  * temperature (temperatures f32 [B], or `temperature` for all with NULL; 0 and below: 1 at the lowest index of the maximum); a

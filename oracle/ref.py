@@ -1021,6 +1021,39 @@ def paged_lse(q, key, table, length, mask, scale, keep=None):
     return out
 
 
+def attention_mass(q, key, table, length, lse, prior, count, path, window, sinks, scale, places):
+    """The summed attention weights [B, Hk, places] in float64, for error bounds the sum of weight times what a score's rounding
+    scales with (1 + scale sum |q k| + |lse|), and the written places (bool [B, places]). path [B, S] or None."""
+    B, S, H, _ = q.shape
+    Hk, P, T, _ = key.shape
+    G = H // Hk
+    out, heft, written = np.zeros((B, Hk, places)), np.zeros((B, Hk, places)), np.zeros((B, places), dtype=bool)
+    for b in range(B):
+        n = max(0, min(int(length[b]), table.shape[1] * T))
+        c = S if count is None else max(0, min(int(count[b]), S))
+        end = min(n + c, places, table.shape[1] * T)
+        written[b, :end] = True
+        if prior is not None:
+            out[b, :, :min(n, end)] = prior[b, :, :min(n, end)]
+        pos, page, row = paged_tokens(table[b:b + 1], [n], T, P, 0, c)
+        live = pos < end
+        pos, page, row = pos[live], page[live], row[live]
+        for k in range(c):
+            r = k if path is None else int(path[b, k])
+            if not 0 <= r < S:
+                continue
+            use = (pos <= n + k) & ((pos < sinks) | (pos >= n + k + 1 - window))
+            for g in range(Hk):
+                keys = key[g, page[use], row[use]]
+                for h in range(g * G, (g + 1) * G):
+                    if not lse[b, r, h] > -np.inf:
+                        continue
+                    w = np.exp(keys @ q[b, r, h] * scale - lse[b, r, h])
+                    out[b, g, pos[use]] += w
+                    heft[b, g, pos[use]] += w * (1 + scale * (np.abs(keys) @ np.abs(q[b, r, h])) + np.abs(lse[b, r, h]))
+    return out, heft, written
+
+
 def block_selection(q, ksum, table, length, T, blocks, sink, local):
     """The pages that each row and kv head selects: int [B, S, Hk, sink + local + blocks], ascending, -1 behind. q [B, S, H, D]
     and ksum [Hk, P, D] float64."""

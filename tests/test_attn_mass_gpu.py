@@ -1,0 +1,182 @@
+"""attn_mass on the GPU against the float64 oracle, over pages whose unused rows hold NaN."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import ref
+from paged_cases import cache, f64, tree_masks
+
+pytestmark = pytest.mark.gpu
+BF, FH = torch.bfloat16, torch.float16
+
+
+def check(got, before, q, key, table, lens, lse, prior, count, path, window, sinks, scale):
+    """A weight's relative error: its score's D products and sums (fp32, each within 2^-23 of the sum of magnitudes), the argument
+    of its exponential (three roundings of the score's and the lse's size, 2^-23 each) and exp2 (2^-22); the sums of weights:
+    one rounding per row tile and join, (rows / 16 + 40) 2^-24 of the sum. `heft` holds sum w (1 + |q k| + |lse|)."""
+    D, rows = q.shape[3], q.shape[1] * q.shape[2] // key.shape[0]
+    want, heft, written = ref.attention_mass(f64(q), f64(key), table.numpy(), lens, f64(lse), None if prior is None else f64(prior),
+                                             None if count is None else count.numpy(), None if path is None else path.numpy(), window, sinks, scale,
+                                             got.shape[2])
+    lim = ((D + 4) * 2.0 ** -23 + 6 * 2.0 ** -23) * heft + (rows / 16 + 40) * 2.0 ** -24 * want
+    got = f64(got)
+    bad = ~(np.abs(got - want) <= lim) & written[:, None]
+    assert not bad.any(), (int(bad.sum()), np.argwhere(bad)[:4].tolist(), got[bad][:4].tolist(), want[bad][:4].tolist())
+    stay = ~written[:, None] & np.ones_like(got, dtype=bool)
+    assert np.array_equal(got[stay], f64(before)[stay], equal_nan=True)
+
+
+def operands(g, dt, H, Hk, D, T, lens, S, width=1, spread=1.5):
+    key, value, table = cache(g, dt, Hk, T, D, lens, S, width=width)
+    q = (torch.randn(len(lens), S, H, D, generator=g) * spread).to(dt)
+    return q, key, value, table
+
+
+def _run(C, dev, dt, H, Hk, D, T, lens, S, tree=False, window=None, sinks=0, seed=0, width=1):
+    print(f"attn_mass {dt} H={H} Hk={Hk} D={D} T={T} lens={lens} S={S} tree={tree} window={window} sinks={sinks} width={width}", flush=True)
+    g = torch.Generator().manual_seed(seed + D + T + S)
+    q, key, value, table = operands(g, dt, H, Hk, D, T, lens, S, width)
+    B, N = len(lens), table.shape[1] * T
+    n = torch.tensor(lens, dtype=torch.int32)
+    count = path = None
+    if tree:  # (some of the rows, in order; the lse of any rows will do)
+        count = torch.tensor([i % (S + 1) for i in range(1, B + 1)], dtype=torch.int32)
+        path = torch.stack([torch.randperm(S, generator=g).sort().values if i % 2 else torch.randperm(S, generator=g) for i in range(B)]).to(torch.int32)
+    _, lse = C.attn_window(q.to(dev), key.to(dev), value.to(dev), table.to(dev), n.to(dev), window, sinks)
+    prior = torch.rand(B, Hk, N, generator=g) * 3
+    out = torch.full((B, Hk, N), float("nan"))
+    up = lambda t: None if t is None else t.to(dev)  # noqa: E731
+    got = C.attn_mass(*map(up, (q, key, table, n, lse)), prior=up(prior), count=up(count), path=up(path), window=window, sinks=sinks, out=up(out))
+    check(got, out, q, key, table, lens, lse, prior, count, path, window or 1 << 30, sinks, D ** -0.5)
+
+
+@pytest.mark.parametrize("dt", [BF, FH])
+@pytest.mark.parametrize("H,Hk,D", [(32, 8, 128), (16, 4, 256), (16, 8, 64), (7, 1, 128), (3, 3, 64)])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (1, 0), (70, 5), (300, 64)])
+def test_single_tokens(C, dev, dt, H, Hk, D, window, sinks):
+    _run(C, dev, dt, H, Hk, D, 16, [0, 1, 15, 16, 17, 63, 64, 255, 256, 257, 700], 1, False, window, sinks)
+
+
+@pytest.mark.parametrize("T", [16, 32, 128, 1024])
+def test_page_sizes(C, dev, T):
+    _run(C, dev, BF, 8, 2, 128, T, [T - 1, T, T + 1, 3 * T + 5, 0], 5, True, None, 0, T)
+
+
+@pytest.mark.parametrize("H,Hk,D,S", [(32, 8, 128, 8), (16, 4, 256, 16), (16, 8, 64, 9), (32, 4, 128, 33), (4, 4, 256, 64), (128, 1, 128, 3)])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (9, 3), (200, 130)])
+def test_paths(C, dev, H, Hk, D, S, window, sinks):
+    _run(C, dev, BF if S % 2 else FH, H, Hk, D, 32, [0, 300, 70, 5, 129], S, True, window, sinks, 3)
+
+
+@pytest.mark.parametrize("H,Hk,D,S,lens", [(32, 8, 128, 100, [0, 40]), (8, 2, 64, 500, [129]), (4, 1, 256, 130, [7, 640]), (6, 2, 128, 333, [33]), (33, 1, 256, 12, [90])])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (1, 1), (100, 70)])
+def test_prompts(C, dev, H, Hk, D, S, lens, window, sinks):
+    _run(C, dev, BF, H, Hk, D, 64, lens, S, False, window, sinks, 4)
+
+
+def test_wide_tables(C, dev):
+    """More runs of tokens than the grid holds at once."""
+    _run(C, dev, BF, 2, 2, 64, 16, [5000, 0] + [3] * 60, 2, False, None, 0, 5, width=9000)
+    _run(C, dev, BF, 40, 2, 64, 16, [3000] + [9] * 100, 3, False, None, 0, 5, width=9000)
+
+
+def test_whole_weight(C, dev):
+    """A row's weights sum to one: the tokens' sums over everything are the number of rows and heads."""
+    g = torch.Generator().manual_seed(6)
+    q, key, value, table = (t.to(dev) for t in operands(g, BF, 16, 4, 128, 32, [77, 300, 0], 9))
+    n = torch.tensor([77, 300, 0], dtype=torch.int32, device=dev)
+    for window, sinks in ((None, 0), (50, 4)):
+        _, lse = C.attn_window(q, key, value, table, n, window, sinks)
+        got = C.attn_mass(q, key, table, n, lse, window=window, sinks=sinks)
+        assert (got.sum(2) - 9 * 4).abs().max().item() < 1e-3
+
+
+def test_in_place_and_strides(C, dev):
+    g = torch.Generator().manual_seed(7)
+    lens = [100, 37]
+    q, key, value, table = operands(g, BF, 8, 2, 128, 16, lens, 4)
+    n = torch.tensor(lens, dtype=torch.int32)
+    wide = torch.randn(2, 4, 3, 8, 128, generator=g).to(BF)
+    wide[:, :, 1] = q
+    a = [wide.to(dev)[:, :, 1], key.to(dev), table.to(dev), n.to(dev)]
+    _, lse = C.attn_window(a[0], a[1], value.to(dev), *a[2:], None)
+    layers = torch.rand(2, 3, 2, 5, 1000, generator=g)
+    state = layers.to(dev)
+    view, prior = state[:, 1, :, 2], layers[:, 1, :, 2]
+    got = C.attn_mass(*a, lse, prior=view, out=view)
+    assert got is view
+    check(view, prior, q, key, table, lens, lse, prior, None, None, 1 << 30, 0, 128 ** -0.5)
+    rest = torch.ones_like(layers, dtype=torch.bool)
+    rest[:, 1, :, 2] = False
+    assert torch.equal(state.cpu()[rest], layers[rest])
+    # fewer places than tokens: those there are
+    short = torch.zeros(2, 2, 50, device=dev)
+    C.attn_mass(*a, lse, prior=torch.zeros_like(short), out=short)
+    check(short, short, q, key, table, lens, lse, torch.zeros(2, 2, 50), None, None, 1 << 30, 0, 128 ** -0.5)
+
+
+def test_rows_and_tokens_that_are_none(C, dev):
+    """Counts out of range, paths out of range, rows that attended nothing, NaN queries behind the count, pages that are none,
+    NaN keys in places that a row does not attend."""
+    g = torch.Generator().manual_seed(8)
+    lens, S = [90, 90, 90, 90], 5
+    q, key, value, table = operands(g, BF, 8, 2, 64, 16, lens, S)
+    n = torch.tensor(lens, dtype=torch.int32)
+    _, lse = C.attn_window(*(t.to(dev) for t in (q, key, value, table, n)), 30, 2)
+    lse = lse.cpu()
+    count, path = torch.tensor([3, -2, 99, 4], dtype=torch.int32), torch.arange(S, dtype=torch.int32).repeat(4, 1)
+    path[2, 1], path[2, 3] = -1, S
+    q[0, 3:] = float("nan")
+    lse[3, 2] = -float("inf")
+    table[3, 4] = -1
+    table[2, 5] = key.shape[1]
+    key[:, table[0, 2], 0] = float("nan")  # token 32: every row's window has passed it
+    prior = torch.rand(4, 2, table.shape[1] * 16, generator=g)
+    out = torch.full_like(prior, 7.0)
+    up = lambda t: t.to(dev)  # noqa: E731
+    got = C.attn_mass(*map(up, (q, key, table, n, lse)), prior=up(prior), count=up(count), path=up(path), window=30, sinks=2, out=up(out))
+    q2, key2 = q.clone(), key.clone()
+    q2[0, 3:] = 0
+    key2[key2.isnan()] = 0
+    check(got, out, q2, key2, table, lens, lse, prior, count, path, 30, 2, 0.125)
+
+
+def test_replay_follows_the_lengths(C, dev):
+    g = torch.Generator().manual_seed(9)
+    q, key, value, table = operands(g, BF, 8, 2, 128, 16, [600, 600], 3)
+    key.nan_to_num_(0.5), value.nan_to_num_(0.5)
+    n = torch.tensor([600, 600], dtype=torch.int32, device=dev)
+    a = [q.to(dev), key.to(dev), table.to(dev), n]
+    lse = torch.randn(2, 3, 8, generator=g).to(dev) + 10
+    state, start = torch.zeros(2, 2, 700, device=dev), torch.rand(2, 2, 700, generator=g)
+    C.attn_mass(*a, lse, prior=state, out=state)
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        C.attn_mass(*a, lse, prior=state, out=state)
+    for now in ([0, 1], [599, 77], [64, 300]):
+        n.copy_(torch.tensor(now, dtype=torch.int32))
+        state.copy_(start)
+        torch.cuda.synchronize()
+        graph.replay()
+        with torch.cuda.stream(side):
+            other = C.attn_mass(*a, lse, prior=start.to(dev), out=start.to(dev))
+        torch.cuda.synchronize()
+        assert torch.equal(other, state)
+        check(state, start, q, key, table, now, lse, start, None, None, 1 << 30, 0, 128 ** -0.5)
+
+
+def test_refusals(C, dev):
+    g = torch.Generator().manual_seed(10)
+    q, key, _, table = (t.to(dev) for t in operands(g, BF, 4, 2, 64, 16, [20], 2))
+    n, lse = torch.tensor([20], dtype=torch.int32, device=dev), torch.zeros(1, 2, 4, device=dev)
+    ok = torch.zeros(1, 2, 64, device=dev)
+    for kw in (dict(prior=ok.double()), dict(prior=ok[:, :1]), dict(out=ok[0]), dict(out=ok[:, :, ::2]), dict(prior=ok, out=ok[:, :, :32]), dict(window=0),
+               dict(sinks=-1), dict(count=torch.ones(1, device=dev)), dict(path=torch.ones(1, 3, dtype=torch.int32, device=dev)), dict(scale=-1.0),
+               dict(out=ok[:, :1].expand(1, 2, 64)), dict(out=ok.cpu())):
+        with pytest.raises(RuntimeError):
+            C.attn_mass(q, key, table, n, lse, **kw)
+    for args in ((q.half(), key, table, n, lse), (q, key, table, n, lse.double()), (q, key, table, n, lse[:, :1]), (q, key, table[:, ::2], n, lse), (q, key, table, n.long(), lse)):
+        with pytest.raises(RuntimeError):
+            C.attn_mass(*args)
+    assert C.attn_mass(q[:0], key, table[:0], n[:0], lse[:0]).shape[0] == 0
