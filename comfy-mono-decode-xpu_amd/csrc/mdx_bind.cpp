@@ -37,8 +37,10 @@ struct Entries {
     decltype(&mdx_attn_window_workspace) window_workspace;
     decltype(&mdx_attn_window) window;
     decltype(&mdx_attn_mass) mass;
+    decltype(&mdx_page_evict_workspace) evict_workspace;
+    decltype(&mdx_page_evict) evict;
 } g;
-constexpr int ENTRIES = 14;
+constexpr int ENTRIES = 16;
 PyObject* g_error = nullptr;  // _lib.MdxError
 
 struct Refused : std::runtime_error {
@@ -442,6 +444,44 @@ PyObject* attn_mass(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     });
 }
 
+// kv, ksum, table, length, refs, mass, dst, src, keep, sinks, recent, room, slots -> (status, kept)
+PyObject* page_evict(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    EXPECT(13, "page_evict")
+    return guarded([&]() -> PyObject* {
+        const Pool p = pool(a);
+        const at::Tensor &mass = on(a[5], "mass", p.d), &dst = on(a[6], "dst", p.d), &src = on(a[7], "src", p.d);
+        check(mass.scalar_type() == at::kFloat && mass.dim() == 4 && mass.size(0) == p.L && mass.size(1) == p.B && mass.size(2) == p.Hk &&
+                  mass.is_contiguous(),
+              "mass: contiguous float32 [layers, sequences, kv_heads, places]");
+        const int64_t M = dst.numel(), keep = number(a[8]), sinks = number(a[9]), recent = number(a[10]), room = number(a[11]);
+        ints(dst, "dst", {M});
+        ints(src, "src", {M});
+        const int64_t cap = int64_t(1) << 29;
+        check(keep >= 0 && sinks >= 0 && recent >= 0 && keep <= cap && sinks <= cap && recent <= cap && keep + sinks + recent >= 1,
+              "1..2^29 kept tokens of each kind");
+        const int64_t most = keep + sinks + recent;
+        check(M * p.L * p.Hk * most < (int64_t(1) << 31), "too many pairs times heads times kept tokens for one call");
+        void* slots = slots_of(a[12], p, M, room);
+        const auto kind = at::TensorOptions().dtype(at::kInt).device(p.d);
+        at::Tensor status = at::empty({M}, kind), kept = at::empty({M, p.L, p.Hk, most}, kind);
+        if (M > 0) {
+            const size_t n = g.evict_workspace(M, p.W, p.L, p.Hk, most);
+            at::Tensor ws = scratch(n, p.d);
+            call("mdx_page_evict", p.d, [&](void* st) {
+                return g.evict(p.kv, p.ksum, p.dt, p.L, p.Hk, p.P, p.T, p.D, static_cast<int32_t*>(p.table), p.ts, p.B, p.W,
+                               static_cast<int32_t*>(p.length), static_cast<int32_t*>(p.refs), mass.data_ptr<float>(), mass.size(3),
+                               dst.data_ptr<int32_t>(), src.data_ptr<int32_t>(), M, keep, sinks, recent, room, static_cast<int64_t*>(slots),
+                               status.data_ptr<int32_t>(), kept.data_ptr<int32_t>(), data(ws), n, st);
+            });
+        }
+        PyObject *s = THPVariable_Wrap(std::move(status)), *k = s ? THPVariable_Wrap(std::move(kept)) : nullptr;
+        PyObject* both = k ? PyTuple_Pack(2, s, k) : nullptr;
+        Py_XDECREF(s);
+        Py_XDECREF(k);
+        return both;
+    });
+}
+
 // ---- a step's answers ----
 // logits, tokens, uniform, draft, parent, temperature -> (count, path, next)
 PyObject* verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
@@ -530,6 +570,8 @@ PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     g.window_workspace = reinterpret_cast<decltype(g.window_workspace)>(p[i++]);
     g.window = reinterpret_cast<decltype(g.window)>(p[i++]);
     g.mass = reinterpret_cast<decltype(g.mass)>(p[i++]);
+    g.evict_workspace = reinterpret_cast<decltype(g.evict_workspace)>(p[i++]);
+    g.evict = reinterpret_cast<decltype(g.evict)>(p[i++]);
     Py_XINCREF(a[ENTRIES]);
     Py_XDECREF(g_error);
     g_error = a[ENTRIES];
@@ -544,6 +586,7 @@ PyMethodDef methods[] = {{"init", FAST(init), METH_FASTCALL, nullptr},
                          {"attn_blocks", FAST(attn_blocks), METH_FASTCALL, nullptr},
                          {"attn_window", FAST(attn_window), METH_FASTCALL, nullptr},
                          {"attn_mass", FAST(attn_mass), METH_FASTCALL, nullptr},
+                         {"page_evict", FAST(page_evict), METH_FASTCALL, nullptr},
                          {"verify_drafts", FAST(verify_drafts), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_bind", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

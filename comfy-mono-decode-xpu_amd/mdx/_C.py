@@ -1369,6 +1369,20 @@ def attn_mass(q, key, table, length, lse, prior=None, count=None, path=None, win
     return (_bind or _bound()).attn_mass(q, key, table, length, lse, prior, count, path, window, sinks, scale, out)
 
 
+def page_evict(kv, ksum, table, length, refs, mass, dst, src, keep, sinks=0, recent=0, room=0, slots=None):
+    """Sequence dst[i] becomes src[i] thinned, for every pair i at once: of src's tokens it keeps, for every layer and kv head by
+    itself, the first `sinks`, the last `recent` and, of the others, the `keep` of largest mass (attn_mass's sums, float32
+    [layers, B, kv_heads, N >= W T]; ties: the lowest; NaN last), in their order, and has them at places 0, 1, ..: all of
+    them if there are no more than that (dst[i] == src[i] then stays as it is, only its room is given). Keys keep the
+    rotation of the positions they had. The tokens go to fresh pages, the lowest free ones in the pairs' order, with pages
+    for `room` more tokens; the pages that dst had go back and are free for the next call; all pairs read the state before
+    the call. The mean keys of full pages (ksum, or None) and the rows of mass follow. slots as page_fork's.
+    Returns (status int32 [pairs] as page_fork's; -1 also for src[i] < 0, kept int32 [pairs, layers, kv_heads, sinks + recent
+    + keep]: the numbers the tokens had in src, -1 behind, all -1 where the pair is not done). No counterpart in the
+    reference."""
+    return (_bind or _bound()).page_evict(kv, ksum, table, length, refs, mass, dst, src, keep, sinks, recent, room, slots)
+
+
 def verify_drafts(logits, tokens, uniform, draft=None, parent=None, temperature=1.0):
     """The step's drafted tokens against the target's probabilities p_r = softmax(logits[b, r] / temperature): logits [B, R, V]
     (bf16, fp16 or fp32), row 0 the last committed token's, row r >= 1 holding the drafted token tokens[b, r] (int64; outside

@@ -676,6 +676,22 @@ int mdx_attn_mass(const void* q, int64_t q_seq_stride, int64_t q_row_stride, int
                   float* out, int64_t out_seq_stride, int64_t out_head_stride, int64_t N, int64_t B, int64_t S, int64_t H,
                   int64_t Hk, int64_t D, int64_t P, int64_t T, int64_t W, float scale, void* stream);
 
+/* Eviction: sequence dst[i] <- of the n tokens of src[i] (0..B - 1), for every layer and kv head by itself, the first `sinks`,
+ * the last `recent` and, of the others, the `keep` of largest mass[l][src[i]][g][t] (f32 [L][B][Hk][N], N >= W T; ties: the
+ * lowest t; NaN last), in order; all of them if n <= sinks + recent + keep (dst[i] == src[i] then stays as it is and only
+ * its room is given). The tokens go to fresh pages (the lowest free ones, in pair order, with pages for `room` more
+ * tokens); the pages that dst[i] had are given back and free from the next call on. All pairs read the state before the
+ * call. mass[l][dst[i]][g] and the mean keys of full pages (ksum, may be NULL) follow; length[dst[i]] is the number kept.
+ * kept int32 [pairs][L][Hk][sinks + recent + keep]: their numbers t in src[i], -1 behind. A kept token that stood in no page
+ * leaves its place as it was. slots and status as mdx_page_fork (status -1 also for src[i] < 0; kept is then -1). P T <
+ * 2^31, pairs L Hk <= 2^24, D in {64, 128, 256}; dtype MDX_DT_BF16 or MDX_DT_F16. No counterpart in the reference. */
+size_t mdx_page_evict_workspace(int64_t pairs, int64_t W, int64_t L, int64_t Hk, int64_t most);
+int mdx_page_evict(void* kv, void* ksum, int32_t dtype, int64_t L, int64_t Hk, int64_t P, int64_t T, int64_t D, int32_t* table,
+                   int64_t table_stride, int64_t B, int64_t W, int32_t* length, int32_t* refs, float* mass, int64_t N,
+                   const int32_t* dst, const int32_t* src, int64_t pairs, int64_t keep, int64_t sinks, int64_t recent,
+                   int64_t room, int64_t* slots, int32_t* status, int32_t* kept, void* workspace, size_t workspace_bytes,
+                   void* stream);
+
 /* ---- a step's answers --------------------------------------------------------------------------------
  * Verification of drafted tokens against the target's probabilities. p_r = softmax(logits[b][r] / T), T the sequence's
  * temperature (temperatures f32 [B], or `temperature` for all with NULL; 0 and below: 1 at the lowest index of the maximum); a

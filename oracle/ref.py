@@ -1134,6 +1134,72 @@ def page_fork(kv, ksum, table, length, refs, dst, src, room, share):
     return kv, ksum, new_table, new_length, refs, np.array(status), np.array(slots).reshape(len(status), room)
 
 
+def kept_tokens(mass, n, keep, sinks, recent):
+    """The tokens that an eviction keeps of n, by their masses [>= n]: ascending."""
+    if n <= keep + sinks + recent:
+        return list(range(n))
+    middle = list(range(sinks, n - recent))
+    worth = [-np.inf if np.isnan(mass[t]) else float(mass[t]) for t in middle]
+    nan = [bool(np.isnan(mass[t])) for t in middle]
+    best = sorted(range(len(middle)), key=lambda i: (nan[i], -worth[i], i))[:keep]
+    return sorted(list(range(sinks)) + [middle[i] for i in best] + list(range(n - recent, n)))
+
+
+def page_evict(kv, ksum, table, length, refs, mass, dst, src, keep, sinks, recent, room):
+    """The pairs of an eviction one after the other, every read from the state before the call (operands as page_fork's, mass
+    [L, B, Hk, N]). Returns the new (kv, ksum in float64, table, length, refs, mass), the status, the kept tokens and the
+    slots."""
+    (L, _, Hk, _, T, _), (B, W), most = kv.shape, table.shape, keep + sinks + recent
+    old_kv, old_mass = kv, mass
+    kv, ksum, refs, mass = kv.copy(), ksum.astype(np.float64), refs.copy(), mass.copy()
+    new_table, new_length = table.copy(), length.copy()
+    free = [p for p in range(len(refs)) if refs[p] == 0]
+    page_in = lambda e: 0 <= e < len(refs)  # noqa: E731
+    status, slots, wanted, seen = [], [], 0, set()
+    kept = np.full((len(dst), L, Hk, most), -1, dtype=np.int64)
+    for i, (d, s) in enumerate(zip(dst, src)):
+        d, s = int(d), int(s)
+        ok = 0 <= d < B and d not in seen and 0 <= s < B
+        seen.add(d)
+        had = min(max(int(length[s]), 0), W * T) if ok else 0
+        n, stays = min(had, most), s == d and had <= most
+        total = -(-(n + room) // T)
+        if not ok or total > W:
+            status.append(-1)
+            slots.append([-1] * room)
+            continue
+        places = [j for j in range(n // T, total) if not page_in(table[d, j])] if stays else list(range(total))
+        wanted += len(places)
+        if places and wanted > len(free):
+            status.append(0)
+            slots.append([-1] * room)
+            continue
+        row = [int(e) for e in table[d]] if stays else [-1] * W
+        for j, e in zip(places, free[wanted - len(places):wanted]):
+            row[j] = e
+            refs[e] = 1
+        for l in range(L):
+            for h in range(Hk):
+                stay = kept_tokens(old_mass[l, s, h], had, keep, sinks, recent)
+                kept[i, l, h, :n] = stay
+                if stays:
+                    continue
+                for k, t in enumerate(stay):
+                    if page_in(table[s, t // T]):
+                        kv[l, :, h, row[k // T], k % T] = old_kv[l, :, h, table[s, t // T], t % T]
+                mass[l, d, h, :n] = old_mass[l, s, h, stay]
+                for j in range(n // T):
+                    ksum[l, h, row[j]] = kv[l, 0, h, row[j]].astype(np.float64).mean(0)
+        if not stays:
+            for e in table[d]:
+                if page_in(e):
+                    refs[e] -= 1
+        new_table[d], new_length[d] = row, n
+        status.append(1)
+        slots.append([row[t // T] * T + t % T if page_in(row[t // T]) else -1 for t in range(n, n + room)])
+    return kv, ksum, new_table, new_length, refs, mass, np.array(status), kept, np.array(slots).reshape(len(status), room)
+
+
 def page_commit(kv, table, length, refs, count, path, room):
     """A commit, sequence by sequence. Returns the new (kv, table, length, refs), the status, the slots and the pages that filled:
     a list of (page, float64 mean of its keys [L, Hk, D])."""
