@@ -16,6 +16,8 @@
 // run of 16 TT tokens in turn; bound by the exponentials and the matrix instructions in about equal parts.
 //
 // Reference: none (its cache is never thinned).
+#include <limits.h>
+
 #include "mdx_common.hpp"
 
 namespace mdx {
@@ -90,9 +92,10 @@ __device__ __forceinline__ float row_sums(float* v, int c16) {
 typedef __attribute__((address_space(4))) const int32_t* const_i32p;
 __device__ __forceinline__ int uload(const int32_t* p) { return *(const_i32p)(p); }  // (a scalar load: uniform addresses)
 
-// TT tiles of 16 tokens per wave; SPLIT: the four waves of the work-group share them and take the row tiles in turn.
-template <class E, int D, int TT, bool SPLIT>
-__global__ __launch_bounds__(256) void attn_mass_kernel(MassArgs a) {
+// TT tiles of 16 tokens per wave; SPLIT: the four waves of the work-group share them and take the row tiles in turn; PATH: the
+// rows go by a.path.
+template <class E, int D, int TT, bool SPLIT, bool PATH>
+__global__ __launch_bounds__(256, 3) void attn_mass_kernel(MassArgs a) {
     constexpr int KK = D / 32, TOK = 16 * TT, RUN = SPLIT ? TOK : 4 * TOK;
     static_assert(TT == 2 || TT == 4, "");
     __shared__ float part[SPLIT ? 4 : 1][TOK];
@@ -103,65 +106,117 @@ __global__ __launch_bounds__(256) void attn_mass_kernel(MassArgs a) {
     const int rows = a.count ? max(0, min(uload(a.count + b), a.S)) : a.S;
     const int end = min(min(n + rows, a.W << a.lt), a.N);
     const int32_t* trow = a.table + b * a.ts;
+    const float* lse = a.lse + int64_t(b) * a.S * a.H + kh * a.G;
+    const uint16_t* queries = a.q + b * a.qb + kh * a.G * a.qh + 8 * g;
+    const int32_t* path = PATH ? a.path + int64_t(b) * a.S : nullptr;
+    constexpr int STEP = SPLIT ? 4 : 1;  // a wave's row tiles are so far apart
+    const int step_k = 16 * STEP / a.G, step_h = 16 * STEP % a.G;
+    const int64_t q_step = step_k * a.qs + step_h * a.qh, q_over = q_step + a.qs - a.G * a.qh;
     for (int run = rest % a.tiles; run * RUN < end; run += a.tiles) {
         const int t0 = run * RUN + (SPLIT ? 0 : w * TOK);
         if (!SPLIT && t0 >= end) continue;
-        // ---- the tokens' keys, as A operands
-        u32x4 kf[TT][KK];
-        uint32_t there = 0;  // tiles that stand in a page
-#pragma unroll
-        for (int i = 0; i < TT; ++i) {
-            const int t = t0 + 16 * i, e = t < end ? uload(trow + (t >> a.lt)) : -1;
-            const bool in = uint32_t(e) < uint32_t(a.P);
-            there |= in ? 1u << i : 0u;
-            // (a tile without a page reads the pool's first rows: in bounds, and selected out)
-            const uint16_t* src = a.key + kh * a.kh + (in ? int64_t(e) * a.kp + int64_t(t & ((1 << a.lt) - 1)) * a.kt : 0) + c16 * a.kt + 8 * g;
-#pragma unroll
-            for (int k = 0; k < KK; ++k) kf[i][k] = *reinterpret_cast<const u32x4*>(src + 32 * k);
-        }
-        f32x4 sum[TT];
-#pragma unroll
-        for (int i = 0; i < TT; ++i) sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
         // ---- row tiles that can attend a token of the run: rows k from t0 - n on, and in a window up to the last token's
         const int k_first = max(0, t0 - n);
         const int64_t k_last = t0 < a.sinks ? rows - 1 : min(int64_t(rows) - 1, int64_t(t0) + TOK - 2 - n + a.window);
-        const int r_first = k_first * a.G / 16, r_end = k_last < 0 || there == 0 ? 0 : int((k_last + 1) * a.G + 15) / 16;
-        for (int rt = r_first + (SPLIT ? w : 0); rt < r_end; rt += SPLIT ? 4 : 1) {
-            const int r = rt * 16 + c16, k = r / a.G, h = kh * a.G + r % a.G;
-            const bool row = k < rows;
-            int s = row ? k : 0;
-            if (a.path) s = a.path[int64_t(b) * a.S + s];
-            const bool in = row && uint32_t(s) < uint32_t(a.S);
-            s = in ? s : 0;
-            const float base = a.lse[(int64_t(b) * a.S + s) * a.H + (row ? h : kh * a.G)];
-            const bool live = in && base > -INFINITY;
-            const uint16_t* src = a.q + b * a.qb + s * a.qs + (row ? h : kh * a.G) * a.qh + 8 * g;
-            u32x4 qf[KK];
+        const int r_first = k_first * a.G / 16 + (SPLIT ? w : 0), r_end = k_last < k_first ? 0 : int((k_last + 1) * a.G + 15) / 16;
+        f32x4 sum[TT];
 #pragma unroll
-            for (int i = 0; i < KK; ++i) qf[i] = *reinterpret_cast<const u32x4*>(src + 32 * i);
-            const float sub = base * 1.44269504088896340736f;
-            // this row's tokens: t < lim, and t < sinks or t >= lim - window
-            const int lim = n + k + 1, lo = lim - a.window;
-            // (uniform) every row of the tile attends every token of the run
-            const bool whole = there == (1u << TT) - 1u && __builtin_amdgcn_ballot_w64(!live) == 0 &&
-                               t0 + TOK <= n + rt * 16 / a.G + 1 &&
-                               (t0 + TOK <= a.sinks || t0 >= n + (rt * 16 + 15) / a.G + 1 - a.window);
+        for (int i = 0; i < TT; ++i) sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (r_first < r_end) {  // (uniform in the wave)
+            // ---- a tile's queries and log-sum-exps, one tile ahead of their use
+            struct Rows {
+                u32x4 q[KK];
+                float base;  // its log-sum-exp, as loaded: its first use waits for it, a tile later
+                int k;       // -1: no row
+            };
+            const int r0 = r_first * 16 + c16;
+            int k_at = r0 / a.G, h_at = r0 % a.G;
+            const uint16_t* q_at = queries + k_at * a.qs + h_at * a.qh;  // (without a path: row k's queries, advanced by sums)
+            auto fetch = [&]() {
+                Rows x;
+                bool live = k_at < rows;
+                int s = live ? k_at : 0;
+                const uint16_t* src = live ? q_at : queries;
+                int h = live ? h_at : 0;
+                if constexpr (PATH) {
+                    s = path[s];
+                    live = live && uint32_t(s) < uint32_t(a.S);
+                    s = live ? s : 0;
+                    src = queries + s * a.qs + h * a.qh;
+                }
+                x.base = lse[uint32_t(s) * uint32_t(a.H) + uint32_t(h)];
+                x.k = live ? k_at : -1;
+#pragma unroll
+                for (int i = 0; i < KK; ++i) x.q[i] = *reinterpret_cast<const u32x4*>(src + 32 * i);
+                h_at += step_h;
+                const bool over = h_at >= a.G;
+                h_at -= over ? a.G : 0;
+                k_at += step_k + (over ? 1 : 0);
+                q_at += over ? q_over : q_step;
+                return x;
+            };
+            Rows next = fetch();
+            // ---- the tokens' keys, as A operands
+            u32x4 kf[TT][KK];
+            uint32_t there = 0;  // tiles that stand in a page
 #pragma unroll
             for (int i = 0; i < TT; ++i) {
-                f32x4 z = f32x4{0.f, 0.f, 0.f, 0.f};
+                const int t = t0 + 16 * i, e = t < end ? uload(trow + (t >> a.lt)) : -1;
+                const bool in = uint32_t(e) < uint32_t(a.P);
+                there |= in ? 1u << i : 0u;
+                // (a tile without a page reads the pool's first rows: in bounds, and selected out)
+                const uint16_t* src = a.key + kh * a.kh + (in ? int64_t(e) * a.kp + int64_t(t & ((1 << a.lt) - 1)) * a.kt : 0) + c16 * a.kt + 8 * g;
 #pragma unroll
-                for (int x = 0; x < KK; ++x) z = E::mfma(kf[i][x], qf[x], z);
-                if (whole) {
+                for (int k = 0; k < KK; ++k) kf[i][k] = *reinterpret_cast<const u32x4*>(src + 32 * k);
+            }
+            // they have arrived before the loop: the waits for them in it would be for the next tile's queries too
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) sum[i][e] += __builtin_amdgcn_exp2f(fmaf(z[e], a.zs, -sub));
+            for (int i = 0; i < TT; ++i)
+#pragma unroll
+                for (int k = 0; k < KK; ++k) asm volatile("" : "+v"(kf[i][k]));
+            // Row tiles in which every row attends every token of the run: k >= the last token's own row, and in a window k up to
+            // the first token's last one.
+            const int all_k = t0 + TOK - 1 - n;
+            const int64_t near_k = int64_t(t0) - n - 1 + a.window;
+            const int whole_from = there != (1u << TT) - 1u ? INT_MAX : all_k <= 0 ? 0 : (all_k * a.G + 15) / 16;
+            const int whole_end = t0 + TOK <= a.sinks ? INT_MAX : int(((near_k + 1) * a.G) >> 4);
+            uint64_t pages = 0;  // tokens of the run that stand in pages
+#pragma unroll
+            for (int i = 0; i < TT; ++i) pages |= (there >> i) & 1u ? uint64_t(0xFFFF) << (16 * i) : 0;
+            auto scores = [&](const Rows& x, f32x4 (&z)[TT]) {
+#pragma unroll
+                for (int i = 0; i < TT; ++i) z[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < KK; ++k)
+#pragma unroll
+                    for (int i = 0; i < TT; ++i) z[i] = E::mfma(kf[i][k], x.q[k], z[i]);
+            };
+            for (int rt = r_first; rt < r_end; rt += STEP) {
+                const Rows row = next;
+                if (rt + STEP < r_end) next = fetch();
+                f32x4 z[TT];
+                scores(row, z);
+                // (+inf: the row gives nothing)
+                const float sub = row.k >= 0 && row.base > -INFINITY ? row.base * 1.44269504088896340736f : INFINITY;
+                if (rt >= whole_from && rt < whole_end && __builtin_amdgcn_ballot_w64(sub == INFINITY) == 0) {  // (uniform)
+#pragma unroll
+                    for (int i = 0; i < TT; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sum[i][e] += __builtin_amdgcn_exp2f(fmaf(z[i][e], a.zs, -sub));
                 } else {
+                    // the run's tokens that this row attends: t < lim, of these t < sinks or t >= lim - window
+                    const int lim = n + row.k + 1 - t0, lo = lim - a.window, f = a.sinks - t0;
+                    auto below = [](int m) -> uint64_t { return m <= 0 ? 0 : m >= 64 ? ~uint64_t(0) : (uint64_t(1) << m) - 1; };
+                    uint64_t in = sub == INFINITY ? 0 : below(lim) & (below(f) | ~below(lo)) & pages;
+                    in >>= 4 * g;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int t = t0 + 16 * i + 4 * g + e;
-                        const bool seen = live && ((there >> i) & 1u) && t < lim && (t < a.sinks || t >= lo);
-                        const float x = __builtin_amdgcn_exp2f(fmaf(z[e], a.zs, -sub));
-                        sum[i][e] += seen ? x : 0.f;
-                    }
+                    for (int i = 0; i < TT; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float p = __builtin_amdgcn_exp2f(fmaf(z[i][e], a.zs, -sub));
+                            sum[i][e] += (in >> (16 * i + e)) & 1 ? p : 0.f;
+                        }
                 }
             }
         }
@@ -196,7 +251,8 @@ int launch(MassArgs& a, hipStream_t st) {
     int64_t tiles = (tokens + run - 1) / run;
     if (tiles * pairs > MOST_GROUPS) tiles = MOST_GROUPS / pairs > 0 ? MOST_GROUPS / pairs : 1;
     a.tiles = int(tiles);
-    hipLaunchKernelGGL((attn_mass_kernel<E, D, TT, SPLIT>), dim3(unsigned(tiles * pairs)), dim3(256), 0, st, a);
+    if (a.path) hipLaunchKernelGGL((attn_mass_kernel<E, D, TT, SPLIT, true>), dim3(unsigned(tiles * pairs)), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((attn_mass_kernel<E, D, TT, SPLIT, false>), dim3(unsigned(tiles * pairs)), dim3(256), 0, st, a);
     MDX_LAUNCHED();
     return MDX_OK;
 }
