@@ -8,7 +8,7 @@
 //
 // Two launches. evict_plan_kernel: one work-group gives the fresh pages (as page_fork's plan does), the others, one per (pair,
 // layer, kv head), find the keep-th largest mass by a radix search over its order-preserving bits (11 + 11 + 10, the masses in
-// registers up to 16384 tokens, read again beyond) and write the kept tokens' numbers, places in the pool and masses in
+// registers and LDS up to 16384 tokens, read again beyond) and write the kept tokens' numbers, places in the pool and masses in
 // order. evict_move_kernel: work-groups of whole new pages gather the kept rows, 16 bytes a lane, and take the full pages'
 // mean keys; the first ones change the tables.
 //
@@ -91,19 +91,44 @@ __device__ __forceinline__ uint32_t order_of(float x) {
     return x != x ? 0u : (u >> 31 ? ~u : u | 0x80000000u);
 }
 
-constexpr int EACH = 16;  // tokens of a thread per round: a page's (pages have at least 16 rows)
-constexpr int ROUND = PLAN_T * EACH;
+// EACH tokens of a thread per round, side by side (of one page: those have at least 16 rows)
 constexpr int BINS = 2048;
 
+template <int EACH>
 __device__ void evict_select(const EvictArgs& a, int unit) {
+    constexpr int ROUND = PLAN_T * EACH;
     __shared__ int hist[BINS];
-    __shared__ int tmp[PLAN_T / 64], pick[2];
+    __shared__ int tmp[PLAN_T / 64], pick[3];
+    __shared__ float held[EACH][PLAN_T];  // the round's masses
     const int t = threadIdx.x, h = unit % a.Hk, l = unit / a.Hk % a.L, i = unit / (a.Hk * a.L);
     const int s = a.src[i], d = a.dst[i];
     int32_t* kept = a.kept + int64_t(unit) * a.most;
     if (s < 0 || s >= a.B) return;  // (refused: the move writes what is due)
-    const int n = clamp_len(a.length[s], a.W, a.lt), first = min(a.sinks, n), last = max(first, n - a.recent);
     const float* mass = a.mass + ((int64_t(l) * a.B + s) * a.Hk + h) * a.N;
+    const bool even = (reinterpret_cast<uintptr_t>(mass) & 15) == 0;
+    const int places = a.W << a.lt;  // (there are as many masses: loaded ahead of the length)
+    uint32_t key[EACH];
+    auto load = [&](int from) {  // this thread's masses of the round
+        const int t0 = from + t * EACH;
+        float x[EACH];
+        if (even && t0 + EACH <= places) {
+#pragma unroll
+            for (int j = 0; j < EACH; j += 4) {
+                const float4 v = *reinterpret_cast<const float4*>(mass + t0 + j);
+                x[j] = v.x, x[j + 1] = v.y, x[j + 2] = v.z, x[j + 3] = v.w;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < EACH; ++j) x[j] = t0 + j < places ? mass[t0 + j] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) {
+            held[j][t] = x[j];  // (read by this thread alone)
+            key[j] = order_of(x[j]);
+        }
+    };
+    load(0);
+    const int n = clamp_len(a.length[s], a.W, a.lt), first = min(a.sinks, n), last = max(first, n - a.recent);
     const int32_t* row = a.table + s * a.ts;
     int32_t* place = a.place + int64_t(unit) * a.most;
     float* drawn = a.drawn + int64_t(unit) * a.most;
@@ -113,39 +138,27 @@ __device__ void evict_select(const EvictArgs& a, int unit) {
         for (int k = t; k < n; k += PLAN_T) kept[k] = k;
         return;
     }
-    const bool even = (reinterpret_cast<uintptr_t>(mass) & 15) == 0;
-    float x[EACH];
-    auto load = [&](int from) {  // this thread's masses of the round
-        const int t0 = from + t * EACH;
-        if (even && t0 + EACH <= n) {
-#pragma unroll
-            for (int j = 0; j < EACH; j += 4) {
-                const float4 v = *reinterpret_cast<const float4*>(mass + t0 + j);
-                x[j] = v.x, x[j + 1] = v.y, x[j + 2] = v.z, x[j + 3] = v.w;
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < EACH; ++j) x[j] = t0 + j < n ? mass[t0 + j] : 0.f;
-        }
+    // which of this thread's tokens of the round are below `end`
+    auto below = [&](int from, int end) -> uint32_t {
+        const int m = end - from - t * EACH;
+        return m <= 0 ? 0u : m >= EACH ? (1u << EACH) - 1u : (1u << m) - 1u;
     };
-    // ---- the order of the keep-th largest, and how many of that order are kept
-    uint32_t prefix = 0;  // its bits above `shift`
-    int shift = 32, left = a.keep;
+    // ---- the order from which on keys are kept, and how many of the order just below it (ties)
     const bool once = n <= ROUND;
-    load(0);
+    uint32_t prefix = 0, from_key = 0;
+    int left = a.keep;
+    bool ties = false;
     if (!all && a.keep > 0) {
-        while (shift > 0) {
+        for (int shift = 32; shift > 0;) {
             const int bits = shift == 10 ? 10 : 11, low = shift - bits;
             for (int k = t; k < BINS; k += PLAN_T) hist[k] = 0;
             __syncthreads();
             for (int from = 0; from < n; from += ROUND) {
                 if (!once) load(from);
+                const uint32_t in = below(from, last) & ~below(from, first);
 #pragma unroll
-                for (int j = 0; j < EACH; ++j) {
-                    const int at = from + t * EACH + j;
-                    const uint32_t o = order_of(x[j]);
-                    if (at >= first && at < last && (shift == 32 || (o >> shift) == prefix)) atomicAdd(&hist[(o >> low) & ((1u << bits) - 1u)], 1);
-                }
+                for (int j = 0; j < EACH; ++j)
+                    if (((in >> j) & 1u) && (shift == 32 || (key[j] >> shift) == prefix)) atomicAdd(&hist[(key[j] >> low) & ((1u << bits) - 1u)], 1);
             }
             __syncthreads();
             // two bins per thread, from the top
@@ -156,58 +169,62 @@ __device__ void evict_select(const EvictArgs& a, int unit) {
                 const bool upper = left <= before + h0;
                 pick[0] = BINS - 1 - 2 * t - (upper ? 0 : 1);
                 pick[1] = left - before - (upper ? 0 : h0);
+                pick[2] = upper ? h0 : h1;
             }
             __syncthreads();
             prefix = (prefix << bits) | uint32_t(pick[0]);
             left = pick[1];
             shift = low;
+            ties = pick[2] != left;
+            from_key = prefix << shift;
+            if (!ties) break;  // (uniform: the whole bin is kept)
         }
     }
-    // ---- the kept tokens in order: per thread how many lie above the threshold or are forced, and how many at it
-    int above = 0, ties = 0;  // in the rounds before
+    // ---- the kept tokens in order
+    int above = 0, equal = 0;  // kept ones and ties in the rounds before
     for (int from = 0; from < n; from += ROUND) {
         if (!once) load(from);
-        int up = 0, at_it = 0;
-#pragma unroll
-        for (int j = 0; j < EACH; ++j) {
-            const int at = from + t * EACH + j;
-            if (at >= n) continue;
-            const bool forced = all || at < first || at >= last;
-            const uint32_t o = order_of(x[j]);
-            up += forced || (a.keep > 0 && o > prefix);
-            at_it += !forced && a.keep > 0 && o == prefix;
-        }
-        int total;
-        const int upto = block_sum_incl(up | (at_it << 16), tmp, total);
-        int u = above + (upto & 0xFFFF) - up, e = ties + (upto >> 16) - at_it;
-        if (up + at_it > 0) {
-            const int t0 = from + t * EACH, page = row[t0 >> a.lt];
-            const int base = uint32_t(page) < uint32_t(a.P) ? (page << a.lt) + (t0 & (a.T - 1)) : -1;
+        const uint32_t in = below(from, n), forced = all ? in : in & (below(from, first) | ~below(from, last));
+        uint32_t over = 0, same = 0;
+        if (!all && a.keep > 0) {
 #pragma unroll
             for (int j = 0; j < EACH; ++j) {
-                const int at = t0 + j;
-                if (at >= n) continue;
-                const bool forced = all || at < first || at >= last;
-                const uint32_t o = order_of(x[j]);
-                const bool over = forced || (a.keep > 0 && o > prefix), tie = !over && a.keep > 0 && o == prefix;
-                if (over || (tie && e < left)) {
-                    const int k = u + min(e, left);
-                    kept[k] = at;
-                    place[k] = base < 0 ? -1 : base + j;
-                    drawn[k] = x[j];
-                }
-                u += over;
-                e += tie;
+                over |= key[j] >= from_key ? 1u << j : 0u;
+                same |= key[j] == from_key ? 1u << j : 0u;
             }
         }
+        same = ties ? same & in & ~forced : 0;
+        over = (over & in & ~same) | forced;
+        const int up = __popc(over), at_it = __popc(same);
+        int total;
+        const int upto = block_sum_incl(up | (at_it << 16), tmp, total);
+        int u = above + (upto & 0xFFFF) - up, e = equal + (upto >> 16) - at_it;
         above += total & 0xFFFF;
-        ties += total >> 16;
+        equal += total >> 16;
+        uint32_t todo = over | same;
+        if (todo == 0) continue;
+        const int t0 = from + t * EACH, page = row[t0 >> a.lt];
+        const int base = uint32_t(page) < uint32_t(a.P) ? (page << a.lt) + (t0 & (a.T - 1)) : -1;
+        while (todo) {
+            const int j = __builtin_ctz(todo);
+            todo &= todo - 1;
+            const bool tie = (same >> j) & 1u;
+            if (!tie || e < left) {
+                const int k = u + min(e, left);
+                kept[k] = t0 + j;
+                place[k] = base < 0 ? -1 : base + j;
+                drawn[k] = held[j][t];
+            }
+            u += tie ? 0 : 1;
+            e += tie ? 1 : 0;
+        }
     }
 }
 
+template <int EACH>
 __global__ __launch_bounds__(PLAN_T) void evict_plan_kernel(EvictArgs a) {
     if (blockIdx.x == 0) evict_plan(a);
-    else evict_select(a, int(blockIdx.x) - 1);
+    else evict_select<EACH>(a, int(blockIdx.x) - 1);
 }
 
 // ---- the tables and the rows --------------------------------------------------------------------------------------
@@ -255,6 +272,7 @@ __device__ void evict_tables(const EvictArgs& a, int i) {
     }
 }
 
+constexpr int MOVE_BYTES = 16384;  // of a work-group of the move: whole pages of at least that
 __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
     if (int(blockIdx.x) < a.M) {
         evict_tables(a, blockIdx.x);
@@ -264,35 +282,57 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
     const int4 p = a.pair[i];
     const int k0 = x % a.units * a.unit << a.lt, k1 = min(p.y, k0 + (a.unit << a.lt));
     if (p.x != 1 || p.w || k0 >= k1) return;  // (uniform)
+    // keys whose pages are to be summed up here are kept in LDS on their way
+    __shared__ __align__(16) unsigned char rows[MOVE_BYTES];
+    const bool in_lds = !part && a.ksum && (int64_t(a.unit) << a.lt) * a.D * 2 <= MOVE_BYTES;
     const int64_t list = ((int64_t(i) * a.L + l) * a.Hk + h) * a.most;
     const int32_t *place = a.place + list, *fresh = a.fresh + p.z;
     const int lanes = a.D / 8, step = 256 / lanes, sub = int(threadIdx.x) / lanes, in = int(threadIdx.x) % lanes * 16;
     const int64_t chunk = (int64_t(l) * 2 + part) * a.Hk + h;
     unsigned char* base = a.kv + ((chunk * a.P) << a.lt) * a.D * 2 + in;
     constexpr int U = 4;
+    int missing = 0;
     for (int k = k0 + sub; k < k1; k += U * step) {
         u32x4 v[U];
-        int from[U];
+        int from[U], to[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) from[u] = k + u * step < k1 ? place[k + u * step] : -1;
+        for (int u = 0; u < U; ++u) {
+            const int at = min(k + u * step, k1 - 1);
+            from[u] = place[at];
+            to[u] = fresh[at >> a.lt];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            to[u] = (to[u] << a.lt) + ((k + u * step) & (a.T - 1));
+            missing |= from[u] < 0;
+            if (k + u * step >= k1) from[u] = -1;
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (from[u] >= 0) v[u] = *reinterpret_cast<const u32x4*>(base + int64_t(from[u]) * a.D * 2);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int to = k + u * step;
-            if (from[u] >= 0) *reinterpret_cast<u32x4*>(base + ((int64_t(fresh[to >> a.lt]) << a.lt) + (to & (a.T - 1))) * a.D * 2) = v[u];
-        }
+        for (int u = 0; u < U; ++u)
+            if (from[u] >= 0) {
+                *reinterpret_cast<u32x4*>(base + int64_t(to[u]) * a.D * 2) = v[u];
+                if (in_lds) *reinterpret_cast<u32x4*>(rows + (k + u * step - k0) * a.D * 2 + in) = v[u];
+            }
     }
     if (part) return;
     float* mass = a.mass + ((int64_t(l) * a.B + a.dst[i]) * a.Hk + h) * a.N;
     for (int k = k0 + int(threadIdx.x); k < k1; k += 256) mass[k] = a.drawn[list + k];
     if (!a.ksum) return;
-    __syncthreads();  // (the rows above, read by other waves)
-    for (int j = (k0 >> a.lt) + int(threadIdx.x >> 6); j < k1 >> a.lt; j += 4) mean_key(a, int64_t(l) * a.Hk + h, fresh[j], threadIdx.x & 63);
+    const bool whole = !__syncthreads_or(missing);  // (and the rows above, read by other waves)
+    for (int j = (k0 >> a.lt) + int(threadIdx.x >> 6); j < k1 >> a.lt; j += 4) {
+        const int64_t kc = int64_t(l) * a.Hk + h;
+        if (in_lds && whole) {
+            const uint16_t* at = reinterpret_cast<const uint16_t*>(rows) + ((j << a.lt) - k0) * a.D;
+            mean_rows(at, a.ksum + (kc * a.P + fresh[j]) * a.D, a.T, a.D, a.half, threadIdx.x & 63);
+        } else {  // (a page larger than that; or rows that stand in no page, whose places stay as they were)
+            mean_key(a, kc, fresh[j], threadIdx.x & 63);
+        }
+    }
 }
 
-constexpr int64_t MOVE_BYTES = 16384;  // of a work-group of the move: whole pages of at least that
 int64_t lists(int64_t M, int64_t L, int64_t Hk, int64_t most) { return (M * L * Hk * most + 3) / 4 * 4; }
 int64_t given(int64_t M, int64_t W) { return (M * W + 3) / 4 * 4; }
 
@@ -360,7 +400,9 @@ extern "C" int mdx_page_evict(void* kv, void* ksum, int32_t dtype, int64_t L, in
     const int64_t grid = pairs + pairs * L * 2 * Hk * a.units;
     MDX_CHECK(grid < (int64_t(1) << 31), "too many pairs times heads times kept tokens for one call");
     hipStream_t st = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(evict_plan_kernel, dim3(unsigned(1 + pairs * L * Hk)), dim3(PLAN_T), 0, st, a);
+    // (four tokens a thread where a round of them holds a sequence)
+    if ((W << lt) <= 4 * PLAN_T) hipLaunchKernelGGL((evict_plan_kernel<4>), dim3(unsigned(1 + pairs * L * Hk)), dim3(PLAN_T), 0, st, a);
+    else hipLaunchKernelGGL((evict_plan_kernel<16>), dim3(unsigned(1 + pairs * L * Hk)), dim3(PLAN_T), 0, st, a);
     MDX_LAUNCHED();
     hipLaunchKernelGGL(evict_move_kernel, dim3(unsigned(grid)), dim3(256), 0, st, a);
     MDX_LAUNCHED();

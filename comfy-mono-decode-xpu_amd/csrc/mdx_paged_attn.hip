@@ -1343,7 +1343,8 @@ __global__ __launch_bounds__(NT) void block_select_kernel(PagedArgs a) {
 // The most tokens a unit can have: all that the table (or a selection) holds, and the rows' own; in a window, that of its rows
 // and the first tokens, in whole stages.
 int64_t window_tokens(int64_t held, int64_t S, int64_t spb, int64_t window, int64_t first) {
-    const int64_t rows = S < 64 ? S : spb > 64 ? spb : 64, most = first + window + (rows < S ? rows : S) + 2 * WIN_STEP;
+    const int64_t rows = S < 64 ? S : spb > 64 ? spb : 64, heads = (first + WIN_STEP - 1) / WIN_STEP * WIN_STEP;
+    const int64_t most = heads + window + (rows < S ? rows : S) + WIN_STEP - 1;
     return most < held + S ? most : held + S;
 }
 template <Kind KIND>

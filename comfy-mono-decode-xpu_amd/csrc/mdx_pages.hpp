@@ -11,14 +11,26 @@ constexpr int PLAN_T = 1024;      // threads of the planning work-group
 constexpr int MAX_SEQS = 1024;    // pairs of a fork or an eviction, sequences of a commit: one planning thread each
 
 // ---- the free pages -------------------------------------------------------------------------------------
+// Inclusive sum over a wave's lanes in order, by DPP: the lane 1, 2, 4, 8 ahead in its row of 16, then the rows' last lanes (the
+// LDS crossbar's steps are six times as long).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int lane_ahead(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int wave_sum_incl(int v) {
+    v += lane_ahead<0x111, 0xF>(v);
+    v += lane_ahead<0x112, 0xF>(v);
+    v += lane_ahead<0x114, 0xF>(v);
+    v += lane_ahead<0x118, 0xF>(v);
+    v += lane_ahead<0x142, 0xA>(v);
+    v += lane_ahead<0x143, 0xC>(v);
+    return v;
+}
+
 // Inclusive sum over the work-group's threads (16 waves), and the total; `tmp` of 16 ints. Every thread calls it.
 __device__ __forceinline__ int block_sum_incl(int v, int* tmp, int& total) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int u = __shfl_up(v, d, 64);
-        if (lane >= d) v += u;
-    }
+    v = wave_sum_incl(v);
     __syncthreads();  // (tmp may be in use by the call before)
     if (lane == 63) tmp[w] = v;
     __syncthreads();
@@ -74,24 +86,21 @@ __device__ __forceinline__ uint16_t to_el(float f, int half) {
     return half ? __builtin_bit_cast(uint16_t, static_cast<_Float16>(f)) : f2bf(f);
 }
 
-// The mean key of page e in chunk kc (layer, kv head), by one wave: a lane holds eight dims of every (64 / (D / 8))-th row,
-// fp32 sums, the row groups joined by lane exchanges, one rounding to the cache's type.
-template <class Args>
-__device__ void mean_key(const Args& a, int64_t kc, int e, int lane) {
-    const int lanes = a.D / 8, step = 64 / lanes, sub = lane / lanes, d8 = lane % lanes * 8;
-    const float inv = 1.f / float(a.T);  // (a power of two: exact)
-    const int64_t layer = kc / a.Hk, h = kc % a.Hk;
-    const uint16_t* keys = reinterpret_cast<const uint16_t*>(a.kv) + (((layer * 2 * a.Hk + h) * a.P + e) << a.lt) * a.D + d8;
+// The mean of T rows of D elements at `keys` (the cache or LDS), to `mean`, by one wave: a lane holds eight dims of every
+// (64 / (D / 8))-th row, fp32 sums, the row groups joined by lane exchanges, one rounding to the cache's type.
+__device__ __forceinline__ void mean_rows(const uint16_t* keys, uint16_t* mean, int T, int D, int half, int lane) {
+    const int lanes = D / 8, step = 64 / lanes, sub = lane / lanes, d8 = lane % lanes * 8;
+    const float inv = 1.f / float(T);  // (a power of two: exact)
     float s[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) s[i] = 0.f;
 #pragma unroll 8
-    for (int r = sub; r < a.T; r += step) {
-        const u32x4 v = *reinterpret_cast<const u32x4*>(keys + int64_t(r) * a.D);
+    for (int r = sub; r < T; r += step) {
+        const u32x4 v = *reinterpret_cast<const u32x4*>(keys + int64_t(r) * D + d8);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            s[2 * i] += el(uint16_t(v[i] & 0xFFFFu), a.half);
-            s[2 * i + 1] += el(uint16_t(v[i] >> 16), a.half);
+            s[2 * i] += el(uint16_t(v[i] & 0xFFFFu), half);
+            s[2 * i + 1] += el(uint16_t(v[i] >> 16), half);
         }
     }
     for (int d = lanes; d < 64; d <<= 1)
@@ -100,10 +109,16 @@ __device__ void mean_key(const Args& a, int64_t kc, int e, int lane) {
     if (sub == 0) {
         u32x4 o;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            o[i] = unsigned(to_el(s[2 * i] * inv, a.half)) | (unsigned(to_el(s[2 * i + 1] * inv, a.half)) << 16);
-        *reinterpret_cast<u32x4*>(a.ksum + (kc * a.P + e) * a.D + d8) = o;
+        for (int i = 0; i < 4; ++i) o[i] = unsigned(to_el(s[2 * i] * inv, half)) | (unsigned(to_el(s[2 * i + 1] * inv, half)) << 16);
+        *reinterpret_cast<u32x4*>(mean + d8) = o;
     }
+}
+// The mean key of page e in chunk kc (layer, kv head), by one wave.
+template <class Args>
+__device__ void mean_key(const Args& a, int64_t kc, int e, int lane) {
+    const int64_t layer = kc / a.Hk, h = kc % a.Hk;
+    mean_rows(reinterpret_cast<const uint16_t*>(a.kv) + (((layer * 2 * a.Hk + h) * a.P + e) << a.lt) * a.D, a.ksum + (kc * a.P + e) * a.D, a.T, a.D, a.half,
+              lane);
 }
 
 int log2_of(int64_t T) {
