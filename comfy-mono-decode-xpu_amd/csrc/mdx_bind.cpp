@@ -36,11 +36,12 @@ struct Entries {
     decltype(&mdx_verify_drafts) verify;
     decltype(&mdx_attn_window_workspace) window_workspace;
     decltype(&mdx_attn_window) window;
+    decltype(&mdx_attn_mass_workspace) mass_workspace;
     decltype(&mdx_attn_mass) mass;
     decltype(&mdx_page_evict_workspace) evict_workspace;
     decltype(&mdx_page_evict) evict;
 } g;
-constexpr int ENTRIES = 16;
+constexpr int ENTRIES = 17;
 PyObject* g_error = nullptr;  // _lib.MdxError
 
 struct Refused : std::runtime_error {
@@ -434,12 +435,17 @@ PyObject* attn_mass(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
         } else {
             out = at::zeros({B, Hk, N}, at::TensorOptions().dtype(at::kFloat).device(d));
         }
-        if (B > 0 && S > 0)
+        if (B > 0 && S > 0) {
+            const size_t n = g.mass_workspace(B, S, H, Hk, D, T, W, N);
+            at::Tensor ws;
+            if (n) ws = scratch(n, d);
             call("mdx_attn_mass", d, [&](void* st) {
                 return g.mass(data(q), q.stride(0), q.stride(1), q.stride(2), data(key), key.stride(0), key.stride(1), key.stride(2), dt,
                               table.data_ptr<int32_t>(), table.stride(0), length.data_ptr<int32_t>(), lse.data_ptr<float>(), prior, pb, ph, count,
-                              path, window, sinks, out.data_ptr<float>(), out.stride(0), out.stride(1), N, B, S, H, Hk, D, P, T, W, scale, st);
+                              path, window, sinks, out.data_ptr<float>(), out.stride(0), out.stride(1), N, B, S, H, Hk, D, P, T, W, scale,
+                              n ? data(ws) : nullptr, n, st);
             });
+        }
         return same_or_new(a[11], out);
     });
 }
@@ -569,6 +575,7 @@ PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     g.verify = reinterpret_cast<decltype(g.verify)>(p[i++]);
     g.window_workspace = reinterpret_cast<decltype(g.window_workspace)>(p[i++]);
     g.window = reinterpret_cast<decltype(g.window)>(p[i++]);
+    g.mass_workspace = reinterpret_cast<decltype(g.mass_workspace)>(p[i++]);
     g.mass = reinterpret_cast<decltype(g.mass)>(p[i++]);
     g.evict_workspace = reinterpret_cast<decltype(g.evict_workspace)>(p[i++]);
     g.evict = reinterpret_cast<decltype(g.evict)>(p[i++]);

@@ -33,7 +33,7 @@
 
 #include <atomic>
 
-#include "mdx_common.hpp"
+#include "mdx_lds.hpp"
 
 namespace mdx {
 namespace {
@@ -42,7 +42,6 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 
 // The two element types: their MFMA, and P's rounding. fp16 holds weights down to 2^-14 at full precision only: P is
@@ -139,10 +138,6 @@ constexpr int64_t FEW_STEPS = 2048;
 constexpr int64_t WHOLE_TOKENS = 640;
 constexpr int64_t EVEN_TOKENS = 4096;  // and where there are as many row blocks as work-groups
 
-__device__ __forceinline__ uint32_t lds_addr(const void* p) {
-    return uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const unsigned char*)p));
-}
-
 // LDS layout of a 32-token stage, K and V alike: the tokens' rows of 2 D bytes one after the other, as they stand in a page,
 // so that a direct load's KiB is one KiB of the page (64-byte pieces of 16 tokens per load took 2 % longer, 200 us against 196
 // for 64 single-token sequences of 262 thousand tokens in all). Within a row the 16-byte pieces are exchanged by
@@ -152,35 +147,6 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
 //      receives dim c16 of tokens 4 g .. 4 g + 3) meet every bank alike;
 // both from one lane address: piece bits above the lane's own enter by an exclusive or with a constant.
 // The reads are inline asm that ends with its wait: the builtins would wait for every direct load in flight.
-template <int D>
-__device__ __forceinline__ int swizzle(int token) {  // exchanged piece = piece ^ swizzle(token)
-    return D == 64 ? (token >> 1) & 7 : token & 15;
-}
-// tokens of half h: k-operands kk of the D / 32
-template <int D>
-__device__ __forceinline__ void read_k(u32x4 (&kf)[D / 32], uint32_t at) {
-    if constexpr (D == 256) {
-        asm volatile(
-            "ds_read_b128 %0, %8\n\tds_read_b128 %1, %9\n\tds_read_b128 %2, %10\n\tds_read_b128 %3, %11\n\t"
-            "ds_read_b128 %4, %8 offset:256\n\tds_read_b128 %5, %9 offset:256\n\tds_read_b128 %6, %10 offset:256\n\t"
-            "ds_read_b128 %7, %11 offset:256\n\ts_waitcnt lgkmcnt(0)"
-            : "=&v"(kf[0]), "=&v"(kf[1]), "=&v"(kf[2]), "=&v"(kf[3]), "=&v"(kf[4]), "=&v"(kf[5]), "=&v"(kf[6]), "=&v"(kf[7])
-            : "v"(at), "v"(at ^ 64), "v"(at ^ 128), "v"(at ^ 192)
-            : "memory");
-    } else if constexpr (D == 128) {
-        asm volatile(
-            "ds_read_b128 %0, %4\n\tds_read_b128 %1, %5\n\tds_read_b128 %2, %6\n\tds_read_b128 %3, %7\n\ts_waitcnt lgkmcnt(0)"
-            : "=&v"(kf[0]), "=&v"(kf[1]), "=&v"(kf[2]), "=&v"(kf[3])
-            : "v"(at), "v"(at ^ 64), "v"(at ^ 128), "v"(at ^ 192)
-            : "memory");
-    } else {
-        static_assert(D == 64, "head_dim 64, 128 or 256");
-        asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %3\n\ts_waitcnt lgkmcnt(0)"
-                     : "=&v"(kf[0]), "=&v"(kf[1])
-                     : "v"(at), "v"(at ^ 64)
-                     : "memory");
-    }
-}
 // both halves at once
 template <int D>
 __device__ __forceinline__ void read_k2(u32x4 (&kf)[2][D / 32], uint32_t at) {
@@ -236,13 +202,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
     return r;
-}
-
-// what a wave may have in flight behind the load it waits for (vmcnt only)
-template <int N>
-__device__ __forceinline__ void wait_vm() {
-    static_assert(N <= 63, "vmcnt");
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
 // The tokens a unit's steps run over, as virtual tokens v: the first `nsel` of them are selected blocks' (Kind::SEL) or the

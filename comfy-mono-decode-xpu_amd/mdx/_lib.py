@@ -174,7 +174,9 @@ SIGNATURES = {
                         [c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p] + [c_int64] * 10 +
                         [ctypes.c_float, c_void_p, c_size_t, c_void_p]),
     "mdx_attn_mass": (ctypes.c_int, [c_void_p] + [c_int64] * 3 + [c_void_p] + [c_int64] * 3 + [c_int32, c_void_p, c_int64, c_void_p, c_void_p,
-                      c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p] + [c_int64] * 11 + [ctypes.c_float, c_void_p]),
+                      c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p] + [c_int64] * 11 +
+                      [ctypes.c_float, c_void_p, c_size_t, c_void_p]),
+    "mdx_attn_mass_workspace": (c_size_t, [c_int64] * 8),
     "mdx_page_evict_workspace": (c_size_t, [c_int64] * 5),
     "mdx_page_evict": (ctypes.c_int, [c_void_p, c_void_p, c_int32] + [c_int64] * 5 + [c_void_p] + [c_int64] * 3 + [c_void_p] * 3 +
                        [c_int64, c_void_p, c_void_p] + [c_int64] * 5 + [c_void_p] * 4 + [c_size_t, c_void_p]),
@@ -273,7 +275,7 @@ def bind():
         except ImportError as e:
             raise MdxError(f"mdx/_bind.so not built or not loadable ({e}); run comfy-mono-decode-xpu_amd/build.py") from None
         names = ("last_error", "page_fork_workspace", "page_fork", "page_commit_workspace", "page_commit", "attn_paged_workspace",
-                 "attn_paged", "attn_blocks_workspace", "attn_blocks", "verify_drafts_workspace", "verify_drafts", "attn_window_workspace", "attn_window", "attn_mass", "page_evict_workspace", "page_evict")
+                 "attn_paged", "attn_blocks_workspace", "attn_blocks", "verify_drafts_workspace", "verify_drafts", "attn_window_workspace", "attn_window", "attn_mass_workspace", "attn_mass", "page_evict_workspace", "page_evict")
         m.init(*(ctypes.cast(getattr(L, "mdx_" + n), c_void_p).value for n in names), MdxError)
         _bound = m
     return _bound

@@ -668,13 +668,16 @@ int mdx_attn_window(const void* q, int64_t q_seq_stride, int64_t q_row_stride, i
  * mdx_page_commit leaves a path's rows): it attends t <= n + k, of these the first `sinks` and the last `window`
  * (mdx_attn_window's). lse f32 [B, S, H] contiguous; a row whose lse is -inf or whose r is none gives nothing, a token in no
  * page draws nothing. prior, out f32 [B, Hk, N] (strides in elements; rows contiguous; out may be prior, with its strides).
- * fp32 sums, the same bits every time. Other operands as mdx_attn_paged. No counterpart in the reference. */
+ * fp32 sums, the same bits every time. Other operands as mdx_attn_paged; a workspace of 0 bytes may be NULL. No counterpart in
+ * the reference. */
+size_t mdx_attn_mass_workspace(int64_t B, int64_t S, int64_t H, int64_t Hk, int64_t D, int64_t T, int64_t W, int64_t N);
 int mdx_attn_mass(const void* q, int64_t q_seq_stride, int64_t q_row_stride, int64_t q_head_stride, const void* key,
                   int64_t k_head_stride, int64_t k_page_stride, int64_t k_row_stride, int32_t dtype, const int32_t* table,
                   int64_t table_stride, const int32_t* length, const float* lse, const float* prior, int64_t prior_seq_stride,
                   int64_t prior_head_stride, const int32_t* count, const int32_t* path, int64_t window, int64_t sinks,
                   float* out, int64_t out_seq_stride, int64_t out_head_stride, int64_t N, int64_t B, int64_t S, int64_t H,
-                  int64_t Hk, int64_t D, int64_t P, int64_t T, int64_t W, float scale, void* stream);
+                  int64_t Hk, int64_t D, int64_t P, int64_t T, int64_t W, float scale, void* workspace, size_t workspace_bytes,
+                  void* stream);
 
 /* Eviction: sequence dst[i] <- of the n tokens of src[i] (0..B - 1), for every layer and kv head by itself, the first `sinks`,
  * the last `recent` and, of the others, the `keep` of largest mass[l][src[i]][g][t] (f32 [L][B][Hk][N], N >= W T; ties: the

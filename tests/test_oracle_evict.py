@@ -58,13 +58,13 @@ def test_refusals_before_any_device_work():
 
     def mass(**k):
         a = dict(q=p, qb=128, qs=128, qh=64, key=p, kh=1024, kp=1024, kt=64, dt=_lib.DT_F16, table=p, ts=8, length=p, lse=p, prior=None, pb=0, ph=0, count=None,
-                 path=None, window=4, sinks=0, out=p, ob=256, oh=128, N=128, B=2, S=3, H=4, Hk=2, D=64, P=20, T=16, W=8, scale=0.1)
+                 path=None, window=4, sinks=0, out=p, ob=256, oh=128, N=128, B=2, S=3, H=4, Hk=2, D=64, P=20, T=16, W=8, scale=0.1, ws=None, n=0)
         a.update(k)
         return L.mdx_attn_mass(*a.values(), None), L.mdx_last_error().decode()
 
     for k in (dict(q=None), dict(lse=None), dict(dt=_lib.DT_F32), dict(D=32), dict(T=8), dict(S=0), dict(S=65536), dict(H=3), dict(H=258), dict(kt=60), dict(qs=4),
               dict(key=p + 8), dict(N=0), dict(oh=100), dict(ob=200), dict(prior=p, pb=-1), dict(window=0), dict(sinks=-1), dict(scale=0.0), dict(W=1 << 27),
-              dict(out=p + 2)):
+              dict(out=p + 2), dict(S=2000, N=1024, oh=1024, ob=2048, W=64, ts=64)):
         rc, msg = mass(**k)
         assert rc == _lib.MDX_EINVAL and msg, k
 
