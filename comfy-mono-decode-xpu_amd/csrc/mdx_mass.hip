@@ -533,8 +533,10 @@ extern "C" int mdx_attn_mass(const void* q, int64_t q_seq_stride, int64_t q_row_
     MDX_CHECK(aligned(q, 16) && aligned(key, 16) && q_seq_stride % 8 == 0 && q_row_stride % 8 == 0 && q_head_stride % 8 == 0 &&
                   k_head_stride % 8 == 0 && k_page_stride % 8 == 0 && k_row_stride % 8 == 0 && aligned(lse, 4) && aligned(out, 4) && aligned(prior, 4),
               "16-byte aligned rows");
-    MDX_CHECK(N >= 1 && N <= (int64_t(1) << 30) && out_head_stride >= N && out_seq_stride >= 0 && out_head_stride < lim && out_seq_stride < lim &&
-                  (Hk == 1 || B == 1 || out_seq_stride >= (Hk - 1) * out_head_stride + N) && (B == 1 || out_seq_stride >= N),
+    // (rows apart from one another, the sequences' or the kv heads' side by side)
+    const int64_t ob = B == 1 ? 0 : out_seq_stride, oh = Hk == 1 ? 0 : out_head_stride;
+    MDX_CHECK(N >= 1 && N <= (int64_t(1) << 30) && ob >= 0 && oh >= 0 && ob < lim && oh < lim && (B == 1 || ob >= (Hk - 1) * oh + N || oh >= (B - 1) * ob + N) &&
+                  (Hk == 1 || oh >= N) && (B == 1 || ob >= N),
               "sums [sequences, kv heads, places]: apart from one another");
     MDX_CHECK(!prior || (prior_seq_stride >= 0 && prior_head_stride >= 0 && prior_seq_stride < lim && prior_head_stride < lim), "prior strides");
     MDX_CHECK(window >= 1 && window <= (int64_t(1) << 30) && sinks >= 0 && sinks <= (int64_t(1) << 30), "a window of 1..2^30 tokens, 0..2^30 first ones");
@@ -553,7 +555,7 @@ extern "C" int mdx_attn_mass(const void* q, int64_t q_seq_stride, int64_t q_row_
     a.count = count;
     a.path = path;
     a.out = out;
-    a.ob = out_seq_stride, a.oh = out_head_stride;
+    a.ob = ob, a.oh = oh;
     a.B = int(B), a.S = int(S), a.H = int(H), a.Hk = int(Hk), a.G = int(H / Hk), a.W = int(W), a.P = int(P), a.lt = lt, a.N = int(N);
     a.window = int(window), a.sinks = int(sinks);
     a.zs = float(double(scale) * 1.4426950408889634);

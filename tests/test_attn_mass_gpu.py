@@ -180,3 +180,70 @@ def test_refusals(C, dev):
         with pytest.raises(RuntimeError):
             C.attn_mass(*args)
     assert C.attn_mass(q[:0], key, table[:0], n[:0], lse[:0]).shape[0] == 0
+
+
+@pytest.mark.parametrize("H,Hk,D,S,lens", [(32, 8, 128, 300, [700]), (16, 4, 256, 200, [300, 0, 90]), (16, 8, 64, 1000, [50]), (128, 1, 128, 70, [600]), (9, 3, 128, 411, [1000, 3])])
+@pytest.mark.parametrize("dt", [BF, FH])
+@pytest.mark.parametrize("width", [1, 700])
+def test_many_rows_with_counts(C, dev, H, Hk, D, S, lens, dt, width):
+    """Rows through LDS: runs shared by several work-groups (short tables) and by one (wide ones), counts that end inside a stage."""
+    g = torch.Generator().manual_seed(S)
+    q, key, value, table = operands(g, dt, H, Hk, D, 16, lens, S, width)
+    n = torch.tensor(lens, dtype=torch.int32)
+    _, lse = C.attn_window(*(t.to(dev) for t in (q, key, value, table, n)), 400, 20)
+    N = table.shape[1] * 16
+    prior, out = torch.rand(len(lens), Hk, N, generator=g), torch.full((len(lens), Hk, N), 5.0)
+    up = lambda t: t.to(dev)  # noqa: E731
+    for c in (S, S - 1, S // 2 + 3, 17, 1, 0):
+        count = torch.tensor([max(0, c - 5 * i) for i in range(len(lens))], dtype=torch.int32)
+        got = C.attn_mass(*map(up, (q, key, table, n, lse)), prior=up(prior), count=up(count), window=400, sinks=20, out=up(out))
+        again = C.attn_mass(*map(up, (q, key, table, n, lse)), prior=up(prior), count=up(count), window=400, sinks=20, out=up(out))
+        assert torch.equal(got, again)
+        if c in (S - 1, 17):
+            check(got, out, q, key, table, lens, lse, prior, count, None, 400, 20, D ** -0.5)
+        elif c < 2:
+            assert torch.equal(got.cpu()[0, :, :lens[0]], prior[0, :, :lens[0]]) or c == 1
+
+
+def test_heads_side_by_side(C, dev):
+    """Sums kept as [kv heads, sequences, places]."""
+    g = torch.Generator().manual_seed(11)
+    q, key, value, table = (t.to(dev) for t in operands(g, BF, 8, 4, 64, 16, [70, 9], 3))
+    n = torch.tensor([70, 9], dtype=torch.int32, device=dev)
+    _, lse = C.attn_window(q, key, value, table, n, None)
+    want = C.attn_mass(q, key, table, n, lse)
+    got = torch.zeros(4, 2, want.shape[2], device=dev).transpose(0, 1)
+    assert torch.equal(C.attn_mass(q, key, table, n, lse, out=got), want)
+
+
+def test_longest_chain(C, dev):
+    """65535 rows: every row's weights sum to one."""
+    g = torch.Generator().manual_seed(12)
+    S = 65535
+    q, key, value, table = (t.to(dev) for t in operands(g, BF, 1, 1, 64, 1024, [100], S))
+    n = torch.tensor([100], dtype=torch.int32, device=dev)
+    _, lse = C.attn_window(q, key, value, table, n, 200, 4)
+    got = C.attn_mass(q, key, table, n, lse, window=200, sinks=4)
+    assert abs(got.double().sum().item() / S - 1) < 1e-5
+    few = C.attn_mass(q[:, -40:].contiguous(), key, table, n + S - 40, lse[:, -40:].contiguous(), window=200, sinks=4)
+    part = C.attn_mass(q, key, table, n, lse, count=torch.tensor([S - 40], dtype=torch.int32, device=dev), window=200, sinks=4)
+    assert (part + few - got).abs().max().item() < 1e-2 and (few[0, 0, 4:S - 200] == 0).all()
+
+
+def test_offsets_past_32_bits(C, dev):
+    """Keys, and their sums, past 2^32 elements and bytes of their bases."""
+    g = torch.Generator().manual_seed(13)
+    q, key, value, table = operands(g, BF, 4, 2, 128, 1024, [1500], 70)
+    n = torch.tensor([1500], dtype=torch.int32)
+    P, small = 16500, key.shape[1]  # a kv head of 4.3 GB
+    pool = torch.empty(2, P, 1024, 128, dtype=BF, device=dev)
+    pool[:, P - small:] = key.to(dev)
+    high = torch.where(table >= 0, table + (P - small), table)
+    _, lse = C.attn_window(*(t.to(dev) for t in (q, key, value, table, n)), None)
+    wide = torch.empty(2, 1 << 30, dtype=torch.float32, device=dev)[:, -4096:][None]
+    wide.fill_(3.0)
+    for rows in (70, 1):
+        a = (q[:, :rows].contiguous(), lse[:, :rows].contiguous())
+        got = C.attn_mass(a[0].to(dev), pool, high.to(dev), n.to(dev), a[1], out=wide)
+        check(got, torch.full((1, 2, 4096), 3.0), a[0], key, table, [1500], a[1], None, None, None, 1 << 30, 0, 128 ** -0.5)
+        wide.fill_(3.0)

@@ -206,3 +206,38 @@ def test_refusals(C, dev):
         C.attn_window(q, key, value, table, n, 2.5)
     out, lse = C.attn_window(q[:0], key, value, table[:0], n[:0], 4)
     assert out.shape == (0, 2, 4, 64) and lse.shape == (0, 2, 4)
+
+
+@pytest.mark.parametrize("width", [1, 3000])
+def test_lengths_out_of_range_are_clamped(C, dev, width):
+    g = torch.Generator().manual_seed(13)
+    key, value, table = cache(g, BF, 2, 16, 64, [60, 40], 4, width=width)
+    q = torch.randn(2, 4, 8, 64, generator=g).to(BF)
+    a = [t.to(dev) for t in (q, key, value, table)]
+    n = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    top = table.shape[1] * 16
+    for got, want in ((n(-5, 40), n(0, 40)), (n(60, 2 ** 31 - 1), n(60, top)), (n(-2 ** 31, top + 1), n(0, top))):
+        x, y = C.attn_window(*a, got, 20, 3), C.attn_window(*a, want, 20, 3)
+        assert torch.equal(x[0], y[0]) and torch.equal(x[1], y[1])
+
+
+def test_the_most_sequences(C, dev):
+    g = torch.Generator().manual_seed(14)
+    lens = [i % 50 for i in range(1024)]
+    key, value, table = cache(g, BF, 1, 16, 64, lens, 2)
+    q = torch.randn(1024, 2, 2, 64, generator=g).to(BF)
+    got = C.attn_window(*(t.to(dev) for t in (q, key, value, table)), torch.tensor(lens, dtype=torch.int32, device=dev), 20, 3)
+    check(got, BF, q, key, value, table, lens, None, 0.125, 20, 3)
+
+
+def test_longest_chain(C, dev):
+    """65535 rows: the first and the last are as those of short calls over the same tokens."""
+    g = torch.Generator().manual_seed(15)
+    S, T = 65535, 1024
+    key, value, table = (t.to(dev) for t in cache(g, BF, 1, T, 64, [100], S))
+    q = torch.randn(1, S, 1, 64, generator=g).to(BF).to(dev)
+    n = torch.tensor([100], dtype=torch.int32, device=dev)
+    out, lse = C.attn_window(q, key, value, table, n, 300, 5)
+    for s in (0, 1, 40000, S - 3):
+        a, b = C.attn_window(q[:, s:s + 3].contiguous(), key, value, table, n + s, 300, 5)
+        assert (a.float() - out[:, s:s + 3].float()).abs().max().item() <= 2.0 ** -6 and (b - lse[:, s:s + 3]).abs().max().item() <= 1e-5

@@ -208,3 +208,33 @@ def test_refusals(C, dev):
         C.page_evict(*d, two, two, 5, room=3, slots=torch.zeros(2, 2, dtype=torch.int64, device=dev))
     status, kept = C.page_evict(*d, two[:0], two[:0], 5)
     assert status.shape == (0,) and kept.shape == (0, 2, 2, 5)
+
+
+def test_offsets_past_32_bits(C, dev):
+    """Kept rows and fresh pages past 2^32 bytes of a chunk's base."""
+    st = State(15, [90, 0, 40], L=1, Hk=1, P=12, T=32, D=256, W=4)
+    P = 270000  # a chunk of 4.4 GB
+    base = P - 12
+    kv = torch.empty(1, 2, 1, P, 32, 256, dtype=BF, device=dev)
+    kv[:, :, :, base:] = st.kv.to(dev)
+    ksum = torch.zeros(1, 1, P, 256, dtype=BF, device=dev)
+    ksum[:, :, base:] = st.ksum.to(dev)
+    refs = torch.ones(P, dtype=torch.int32, device=dev)
+    refs[base:] = st.refs.to(dev)
+    table = torch.where(st.table >= 0, st.table + base, st.table).to(dev)
+    length, mass = st.length.to(dev), st.mass.to(dev)
+    slots = torch.zeros(2, 3, dtype=torch.int64, device=dev)
+    status, kept = C.page_evict(kv, ksum, table, length, refs, mass, i32([0, 1], dev), i32([0, 2], dev), 30, 2, 5, 3, slots)
+    want = ref.page_evict(*st.host(), [0, 1], [0, 2], 30, 2, 5, 3)
+    got = [kv[:, :, :, base:], ksum[:, :, base:], torch.where(table >= 0, table - base, table), length, refs[base:], mass]
+    compare(st, got, want, status, kept, torch.where(slots >= 0, slots - base * 32, slots))
+
+
+def test_the_most_pairs(C, dev):
+    st = State(16, [(5 * i) % 33 for i in range(1024)], L=1, Hk=1, P=4000, W=3)
+    evict(C, dev, st, list(range(1024)), list(range(1024)), 7, 1, 3, 2)
+
+
+def test_more_kept_than_a_table_holds(C, dev):
+    st = State(17, [100, 128, 0], P=60)
+    assert evict(C, dev, st, [0, 1, 2], [1, 1, 0], 5000, 100, 100) == [1, 1, 1]

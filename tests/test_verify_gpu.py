@@ -179,3 +179,39 @@ def test_refusals(C, dev):
         C.verify_drafts(logits, tokens, uniform, temperature="warm")
     count, path, answer = C.verify_drafts(logits[:0], tokens[:0], uniform[:0])
     assert count.shape == (0,) and path.shape == (0, 3) and answer.shape == (0,)
+
+
+def test_padded_batches(C):
+    """Chains of unequal lengths in one batch: a token of -1 (or any outside of the vocabulary) ends a sequence's chain."""
+    logits, draft, tokens, uniform = inputs(16, 6, 6, 3000, "bf16")
+    for b in range(6):
+        tokens[b, 1 + b:] = (-1, 3000, 2 ** 40, -(2 ** 40), -5, 0)[b]
+    uniform[:, :6] *= 0.2
+    want = check(C, logits, tokens, uniform, draft)
+    assert want[0].tolist()[0] == 1 and want[0].max() > 2
+    check(C, logits, tokens, uniform)
+
+
+def test_no_drafted_rows(C, dev):
+    logits, _, tokens, uniform = inputs(17, 5, 1, 7777, "fp16")
+    want = check(C, logits, tokens, uniform)
+    got = C.verify_drafts(logits.to(dev), tokens.to(dev), uniform.to(dev), draft=torch.empty(5, 0, 7777, dtype=torch.float16, device=dev))
+    assert got[2].tolist() == want[2].tolist() and got[0].tolist() == [1] * 5
+
+
+@pytest.mark.parametrize("B,R,V", [(1024, 3, 40), (1, 2, (1 << 24) - 1), (2, 64, 2100)])
+def test_the_largest(C, B, R, V):
+    """The most sequences, the largest vocabulary (more runs than the draw holds at once), the most rows."""
+    logits, draft, tokens, uniform = inputs(18, B, R, V, "bf16")
+    check(C, logits, tokens, uniform, draft, heat=0.9)
+
+
+def test_draws_in_every_run(C, dev):
+    """Equal weights: the draw is u of the vocabulary itself, at either side of every run's border."""
+    V, B = 151936, 1024
+    logits = torch.zeros(1, 1, V, dtype=torch.bfloat16, device=dev).expand(B, 1, V)
+    u = torch.zeros(B, 2, dtype=torch.float64)
+    at = torch.tensor([min(V - 1, i // 2 * 512 + (i % 2) * 511) for i in range(B)])
+    u[:, 1] = (at.double() + 0.5) / V
+    got = C.verify_drafts(logits, torch.zeros(B, 1, dtype=torch.int64, device=dev), u.to(dev))
+    assert torch.equal(got[2].cpu(), at)
