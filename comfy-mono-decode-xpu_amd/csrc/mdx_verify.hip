@@ -10,14 +10,15 @@
 // All of it in 64 bits: a drawn token is a whole number that changes where u falls between two sums, and at a vocabulary of 150
 // thousand 32-bit sums (1e-7 of the whole) would move one draw in thirty across a border; 64-bit ones (1e-13) one in 1e8.
 //
-// Three launches. verify_rows_kernel: a work-group per slice of a row (8192 logits, 2048 where there are few) sums their
+// Three launches. verify_rows_kernel: a work-group per slice of a row (16384 logits, fewer where there are few) sums their
 // exponentials. verify_walk_kernel: a work-group per piece of a sequence's vocabulary joins the rows' sums, walks the tree (every
 // work-group of a sequence alike, from LDS) and sums the weights of its piece of the row that answers. verify_draw_kernel: a
-// work-group per sequence finds the piece that the draw falls in and the token in it. (The last work-group of the second
+// work-group per sequence finds the run of 512 that the draw falls in and the token in it. (The last work-group of the second
 // launch can not do that cheaply: a release to the other XCDs' caches by each of 600 cost 30 us.)
 //
-// What bounds it: the logits' bytes, each read once (the row that answers again, out of the caches), and at about the same rate
-// the exponentials (18 vector instructions each, float64 at the rate of float32 on this chip).
+// What bounds it: many rows the exponentials, 14 vector instructions each, eight of them float64 (7 rows of 32 sequences and their
+// drafts over 151936: 37 us for 126 MB, 25 at the rate of a large copy; with 20 instructions 51), then the walk and the draw, 18
+// and 10 us, chains of dependent loads; one short chain those alone (16 us a call).
 // Exponentials: 2^(a / 128) = table[k % 128] 2^(k / 128) poly(a - k), k = rint(a): a table of 1 KiB in LDS, a polynomial of degree 3
 // through the Chebyshev points of [-1/2, 1/2] (2.8e-13 relative); x / T as it stands, without a maximum, as long as none is past
 // 2^900 (then the row is read again less its largest).
@@ -290,9 +291,9 @@ __global__ __launch_bounds__(NT) void verify_rows_kernel(VerifyArgs a) {
         __builtin_amdgcn_sched_barrier(0);  // (eight at a time are enough in flight: more cost registers, and waves)
     }
     double s = s0 + s1;
-    // (a NaN makes the sum one)
-    const bool near = c > 0.0 && top >= 0.f && double(top) * c < FAR && s == s;
-    if (__builtin_amdgcn_ballot_w64(!near) != 0) {  // (uniform in the wave)
+    // (a NaN makes the sum one; a lane past the row's end has top -1)
+    const bool near = c > 0.0 && double(top) * c < FAR && s == s;
+    if (__builtin_amdgcn_ballot_w64(!near) != 0 || __builtin_amdgcn_ballot_w64(top >= 0.f) == 0) {  // (uniform in the wave)
         // once more: the largest, and whether a reference of 0 will do with the others raised to weights of 2^-1020
         ref = -INFINITY;
 #pragma unroll 1
