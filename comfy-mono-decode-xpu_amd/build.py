@@ -1,5 +1,5 @@
-"""Build libmdx.so (every HIP kernel of the package, gfx950) and _bind.so (the torch binding of the paged cache's calls)
-in-tree, next to the Python shim.
+"""Build libmdx.so (every HIP kernel of the package, gfx950) and _bind.so (the torch binding of the serving
+step's calls: the paged cache's and verify_drafts) in-tree, next to the Python shim.
 
     python comfy-mono-decode-xpu_amd/build.py [--jobs N]
 

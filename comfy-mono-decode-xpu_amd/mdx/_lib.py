@@ -275,7 +275,8 @@ def bind():
         except ImportError as e:
             raise MdxError(f"mdx/_bind.so not built or not loadable ({e}); run comfy-mono-decode-xpu_amd/build.py") from None
         names = ("last_error", "page_fork_workspace", "page_fork", "page_commit_workspace", "page_commit", "attn_paged_workspace",
-                 "attn_paged", "attn_blocks_workspace", "attn_blocks", "verify_drafts_workspace", "verify_drafts", "attn_window_workspace", "attn_window", "attn_mass_workspace", "attn_mass", "page_evict_workspace", "page_evict")
+                 "attn_paged", "attn_blocks_workspace", "attn_blocks", "verify_drafts_workspace", "verify_drafts", "attn_window_workspace",
+                 "attn_window", "attn_mass_workspace", "attn_mass", "page_evict_workspace", "page_evict")
         m.init(*(ctypes.cast(getattr(L, "mdx_" + n), c_void_p).value for n in names), MdxError)
         _bound = m
     return _bound

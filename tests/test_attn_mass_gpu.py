@@ -247,3 +247,26 @@ def test_offsets_past_32_bits(C, dev):
         got = C.attn_mass(a[0].to(dev), pool, high.to(dev), n.to(dev), a[1], out=wide)
         check(got, torch.full((1, 2, 4096), 3.0), a[0], key, table, [1500], a[1], None, None, None, 1 << 30, 0, 128 ** -0.5)
         wide.fill_(3.0)
+
+
+def test_no_rows(C, dev):
+    """A step without rows: the committed tokens' sums pass through, places behind stay."""
+    g = torch.Generator().manual_seed(14)
+    q, key, _, table = (t.to(dev) for t in operands(g, BF, 4, 2, 64, 16, [40, 0], 1))
+    n, lse = torch.tensor([40, 0], dtype=torch.int32, device=dev), torch.zeros(2, 0, 4, device=dev)
+    prior = torch.rand(2, 2, 60, generator=g).to(dev)
+    none = torch.zeros(2, 0, dtype=torch.int32, device=dev)
+    for kw in ({}, dict(count=n, path=none)):
+        out = torch.full_like(prior, 7.0)
+        C.attn_mass(q[:, :0], key, table, n, lse, prior=prior, out=out, **kw)
+        assert torch.equal(out[0, :, :40], prior[0, :, :40]) and (out[0, :, 40:] == 7).all() and (out[1] == 7).all()
+        assert (C.attn_mass(q[:, :0], key, table, n, lse, **kw) == 0).all()
+
+
+def test_in_place_needs_the_same_strides(C, dev):
+    g = torch.Generator().manual_seed(15)
+    q, key, _, table = (t.to(dev) for t in operands(g, BF, 4, 2, 64, 16, [20, 9], 2))
+    n, lse = torch.tensor([20, 9], dtype=torch.int32, device=dev), torch.zeros(2, 2, 4, device=dev)
+    state = torch.zeros(2, 2, 64, device=dev)
+    with pytest.raises(RuntimeError, match="in place"):
+        C.attn_mass(q, key, table, n, lse, prior=state, out=state.transpose(0, 1))
