@@ -10,15 +10,16 @@
 // All of it in 64 bits: a drawn token is a whole number that changes where u falls between two sums, and at a vocabulary of 150
 // thousand 32-bit sums (1e-7 of the whole) would move one draw in thirty across a border; 64-bit ones (1e-13) one in 1e8.
 //
-// Three launches. verify_rows_kernel: a work-group per slice of a row (16384 logits, fewer where there are few) sums their
-// exponentials. verify_walk_kernel: a work-group per piece of a sequence's vocabulary joins the rows' sums, walks the tree (every
-// work-group of a sequence alike, from LDS) and sums the weights of its piece of the row that answers. verify_draw_kernel: a
-// work-group per sequence finds the run of 512 that the draw falls in and the token in it. (The last work-group of the second
-// launch can not do that cheaply: a release to the other XCDs' caches by each of 600 cost 30 us.)
+// verify_rows_kernel: a work-group per slice of a row (16384 logits, fewer where there are few) sums their exponentials. Without q
+// it leaves the sums of every run of 512 logits too, and verify_answer_kernel, a work-group per sequence, joins the rows' sums,
+// walks the tree, finds the run that the draw falls in, and the token in it. With q the weights of the row that answers are known
+// after the walk alone: verify_walk_kernel, a work-group per piece of a sequence's vocabulary, joins and walks (every work-group of
+// a sequence alike, from LDS) and sums the weights of its piece; verify_draw_kernel, a work-group per sequence, draws. (The last
+// work-group of the second launch can not do that cheaply: a release to the other XCDs' caches by each of 600 cost 30 us.)
 //
 // What bounds it: many rows the exponentials, 14 vector instructions each, eight of them float64 (7 rows of 32 sequences and their
 // drafts over 151936: 37 us for 126 MB, 25 at the rate of a large copy; with 20 instructions 51), then the walk and the draw, 18
-// and 10 us, chains of dependent loads; one short chain those alone (16 us a call).
+// and 5 us, chains of dependent loads; one short chain those alone (14 us a call). 8 rows of 16 trees: 17 us and 11.
 // Exponentials: 2^(a / 128) = table[k % 128] 2^(k / 128) poly(a - k), k = rint(a): a table of 1 KiB in LDS, a polynomial of degree 3
 // through the Chebyshev points of [-1/2, 1/2] (2.8e-13 relative); x / T as it stands, without a maximum, as long as none is past
 // 2^900 (then the row is read again less its largest).
@@ -64,8 +65,9 @@ struct VerifyArgs {
     int32_t* path;   // [B, R]
     int64_t* next;   // [B]
     Part* part;      // [B][2 R - 1 or R][slices]
-    double* sums;    // [B][runs of SUB logits]
-    struct Answer* answer;  // [B]
+    Part* run;       // without drafts [B][R][runs of SUB logits], `at` unused
+    double* sums;    // with drafts [B][runs]
+    struct Answer* answer;  // with drafts [B]
     int B, R, V, rows;   // rows: of a sequence, the draft's behind the target's
     int slices, pieces;  // of a row: work-groups of the first launch, of the second
 };
@@ -240,7 +242,8 @@ __device__ __forceinline__ float max3_abs(float a, float b, float c) {
 }
 
 // A slice of a row. The sums are taken as if no x / T were far from 0, nor -inf; where one is, or T is 0, the slice is read again.
-template <class E, int EACH>
+// RUNS: the sums of every run too, for the draw.
+template <class E, int EACH, bool RUNS>
 __global__ __launch_bounds__(NT) void verify_rows_kernel(VerifyArgs a) {
     __shared__ double tab[STEPS], sum_w[NT / 64];
     __shared__ float ref_w[NT / 64];
@@ -265,13 +268,18 @@ __global__ __launch_bounds__(NT) void verify_rows_kernel(VerifyArgs a) {
     fill_table(tab);
     const double c = rate_of(a, b);
     __syncthreads();  // (the table)
-    double s0 = 0, s1 = 0;
+    // the wave's run i
+    auto put = [&](int i, double sum, float from) {
+        if (lane == 0) a.run[((int64_t(b) * a.R + r) * a.slices + slice) * (EACH * (NT / 64)) + i * (NT / 64) + w] = Part{sum, from, 0};
+    };
+    double s = 0, s0 = 0, s1 = 0;
     float top = -1.f, ref = 0.f;
     int at = 0x7FFFFFFF;
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
         const int e = first + i * NT * 8;
         if (e >= a.V) break;  // (uniform)
+        if constexpr (RUNS) s0 = s1 = 0;
         if (e >= 0 && e + SUB <= a.V) {
 #pragma unroll
             for (int k = 0; k < 8; k += 2) {
@@ -288,9 +296,14 @@ __global__ __launch_bounds__(NT) void verify_rows_kernel(VerifyArgs a) {
                 s0 += exp2_steps(double(y) * c, tab);
             }
         }
+        if constexpr (RUNS) {
+            s0 = wave_sum(s0 + s1);
+            put(i, s0, 0.f);
+            s += s0;
+        }
         __builtin_amdgcn_sched_barrier(0);  // (eight at a time are enough in flight: more cost registers, and waves)
     }
-    double s = s0 + s1;
+    if constexpr (!RUNS) s = s0 + s1;
     // (a NaN makes the sum one; a lane past the row's end has top -1)
     const bool near = c > 0.0 && double(top) * c < FAR && s == s;
     if (__builtin_amdgcn_ballot_w64(!near) != 0 || __builtin_amdgcn_ballot_w64(top >= 0.f) == 0) {  // (uniform in the wave)
@@ -315,16 +328,24 @@ __global__ __launch_bounds__(NT) void verify_rows_kernel(VerifyArgs a) {
         if (ref > -INFINITY && c > 0.0) {
             const bool zero = __builtin_fabs(double(ref) * c) < FAR;
             const double less = zero ? 0.0 : double(ref);
+            if (zero) ref = 0.f;
 #pragma unroll 1
             for (int i = 0; i < EACH; ++i) {
                 const Piece<E> y = piece_at<E>(row, a.V, at0<EACH>(slice, i, shift), true);
+                double si = 0;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) s += exp2_steps((double(clean(y[k])) - less) * c, tab);
+                for (int k = 0; k < 8; ++k) si += exp2_steps((double(clean(y[k])) - less) * c, tab);
+                if constexpr (RUNS) {
+                    si = wave_sum(si);
+                    put(i, si, ref);
+                }
+                s += si;
             }
-            if (zero) ref = 0.f;
+        } else if constexpr (RUNS) {
+            for (int i = 0; i < EACH; ++i) put(i, 0.0, -INFINITY);
         }
     }
-    s = wave_sum(s);
+    if constexpr (!RUNS) s = wave_sum(s);
     if (lane == 0) {
         sum_w[w] = s;
         ref_w[w] = ref;
@@ -360,13 +381,16 @@ struct Soft {
         const double e = ref == 0.0 ? add_exp(0.0, y, c, tab) : exp2_steps((double(fminf(y, 3.402823466e38f)) - ref) * c, tab);
         return x >= cut && !none ? e * z : 0.0;
     }
+    __device__ __forceinline__ double once(float x, const double* tab) const {  // (less code)
+        const double e = exp2_steps((double(fminf(x, 3.402823466e38f)) - ref) * c, tab);
+        return x >= cut && !none ? e * z : 0.0;
+    }
 };
 
-// The weights of the eight logits from e0 on (8 lanes apart in a wave) of the row that answers. up, tok (LDS): the rows' parents
-// and tokens, -1: none.
+// The weights of the eight logits from e0 on (8 lanes apart in a wave) of the row that answers.
 template <class E, int N>
-__device__ __forceinline__ void weights(const VerifyArgs& a, int b, const Answer& w, double c, const int (&e0)[N], bool rest, const int* up,
-                                        const int64_t* tok, const double* tab, double (&wt)[N][8]) {
+__device__ __forceinline__ void weights(const VerifyArgs& a, int b, const Answer& w, double c, const int (&e0)[N], bool rest, const double* tab,
+                                        double (&wt)[N][8]) {
     const typename E::type *pr = row_of<E>(a, b, w.row), *qr = rest ? row_of<E>(a, b, a.R + w.row) : pr;
     const bool alike = shift_of<E>(pr) == shift_of<E>(qr);  // (to the 16-byte boundaries)
     Piece<E> x[N], y[N];
@@ -385,15 +409,6 @@ __device__ __forceinline__ void weights(const VerifyArgs& a, int b, const Answer
         }
         __builtin_amdgcn_sched_barrier(0);
     }
-    if (a.draft) return;
-    for (int s = w.row + 1; s < a.R; ++s) {  // the children that were tried
-        if (up[s] != w.row) continue;
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (int(tok[s]) == e0[i] + k) wt[i][k] = 0.0;
-    }
 }
 // row t's token and parent (thread t): what can be reached
 __device__ __forceinline__ void row_at(const VerifyArgs& a, int b, int t, int64_t& x, int& parent) {
@@ -402,15 +417,18 @@ __device__ __forceinline__ void row_at(const VerifyArgs& a, int b, int t, int64_
     if (!(t > 0 && x >= 0 && x < a.V && parent >= 0 && parent < t)) x = parent = -1;
 }
 
-template <class E, int EACH>
-__global__ __launch_bounds__(NT) void verify_walk_kernel(VerifyArgs a) {
-    __shared__ double tab[STEPS], z[2 * MAX_ROWS], share[MAX_ROWS];
-    __shared__ float ref[2 * MAX_ROWS];
-    __shared__ int best[2 * MAX_ROWS], up[MAX_ROWS], took[MAX_ROWS], line[MAX_ROWS], pick[2];
-    __shared__ int64_t tok[MAX_ROWS];
-    const int slice = int(blockIdx.x % unsigned(a.pieces)), b = int(blockIdx.x / unsigned(a.pieces));
+// What a sequence's walk leaves in LDS.
+struct Tree {
+    double z[2 * MAX_ROWS], share[MAX_ROWS];  // 1 / the rows' sums (the draft's behind the target's)
+    int64_t tok[MAX_ROWS];
+    float ref[2 * MAX_ROWS];
+    int best[2 * MAX_ROWS], up[MAX_ROWS], took[MAX_ROWS], line[MAX_ROWS];
+    int row, n;  // the row that answers, the accepted ones with row 0 (in line)
+};
+// By THREADS threads, all of them; tab: filled here.
+template <class E, bool DRAFT, int THREADS>
+__device__ __forceinline__ void walk(const VerifyArgs& a, int b, double c, double* tab, Tree& tree) {
     const int t = threadIdx.x;
-    const double c = rate_of(a, b);
     const bool cold = greedy(a, b);
     // thread r: row r's token, its parent, and the token's logits there
     int64_t x = -1;
@@ -419,19 +437,19 @@ __global__ __launch_bounds__(NT) void verify_walk_kernel(VerifyArgs a) {
     double own_u = 0;
     if (t < a.R) {
         row_at(a, b, t, x, parent);
-        tok[t] = x;
-        up[t] = parent;
-        took[t] = -1;
+        tree.tok[t] = x;
+        tree.up[t] = parent;
+        tree.took[t] = -1;
         if (parent >= 0) {
             own_p = E::f32(row_of<E>(a, b, parent)[x]);
-            if (a.draft) own_q = E::f32(row_of<E>(a, b, a.R + parent)[x]);
+            if (DRAFT) own_q = E::f32(row_of<E>(a, b, a.R + parent)[x]);
             own_u = a.uniform[int64_t(b) * (a.R + 1) + parent];
         }
     }
     fill_table(tab);
     __syncthreads();
     // 16 lanes a row: its reference and sum out of the slices', four of them in flight
-    for (int r = t >> 4; r < a.rows; r += NT / 16) {
+    for (int r = t >> 4; r < a.rows; r += THREADS / 16) {
         const Part* part = a.part + (int64_t(b) * a.rows + r) * a.slices;
         float m = -INFINITY;
         double s = 0;
@@ -464,49 +482,59 @@ __global__ __launch_bounds__(NT) void verify_walk_kernel(VerifyArgs a) {
             at = min(at, __shfl_xor(at, d, 64));
         }
         if ((t & 15) == 0) {
-            ref[r] = all;
-            z[r] = all == -INFINITY ? 0.0 : 1.0 / s;
-            best[r] = all == -INFINITY ? -1 : at;
+            tree.ref[r] = all;
+            tree.z[r] = all == -INFINITY ? 0.0 : 1.0 / s;
+            tree.best[r] = all == -INFINITY ? -1 : at;
         }
     }
     __syncthreads();
     // probability of this thread's token in its parent's row (r >= R: the draft's)
-    auto prob = [&](int r, float l) -> double { return cold ? (x == best[r] ? 1.0 : 0.0) : Soft(c, z[r], ref[r]).of(l, tab); };
+    auto prob = [&](int r, float l) -> double { return cold ? (x == tree.best[r] ? 1.0 : 0.0) : Soft(c, tree.z[r], tree.ref[r]).once(l, tab); };
     if (parent >= 0) {
         bool again = false;  // (a token that a sibling ahead has tried)
-        for (int s = 1; s < t && !a.draft; ++s) again = again || (up[s] == parent && tok[s] == x);
-        share[t] = again ? 0.0 : prob(parent, own_p);
+        for (int s = 1; s < t && !DRAFT; ++s) again = again || (tree.up[s] == parent && tree.tok[s] == x);
+        tree.share[t] = again ? 0.0 : prob(parent, own_p);
     }
     __syncthreads();
     if (parent >= 0) {
         bool ok;
-        if (a.draft) {
-            ok = own_u * prob(a.R + parent, own_q) < share[t];
+        if (DRAFT) {
+            ok = own_u * prob(a.R + parent, own_q) < tree.share[t];
         } else {  // the siblings ahead have [0, from)
             double from = 0;
-            for (int s = 1; s < t; ++s) from += up[s] == parent ? share[s] : 0.0;
-            ok = own_u < from + share[t] && !(own_u < from);
+            for (int s = 1; s < t; ++s) from += tree.up[s] == parent ? tree.share[s] : 0.0;
+            ok = own_u < from + tree.share[t] && !(own_u < from);
         }
-        if (ok) took[parent] = t;  // (one child at most: their parts of [0, 1) do not meet)
+        if (ok) tree.took[parent] = t;  // (one child at most: their parts of [0, 1) do not meet)
     }
     __syncthreads();
     if (t == 0) {
         int n = 0, at = 0;
-        line[n++] = 0;
-        while (took[at] >= 0) line[n++] = at = took[at];  // (a child's row is behind its parent's)
-        pick[0] = at;
-        pick[1] = n;
+        tree.line[n++] = 0;
+        while (tree.took[at] >= 0) tree.line[n++] = at = tree.took[at];  // (a child's row is behind its parent's)
+        tree.row = at;
+        tree.n = n;
     }
     __syncthreads();
-    const int row = pick[0], n = pick[1];
-    const bool refused = a.draft && row + 1 < a.R && up[row + 1] == row;
-    const Answer w{z[row], refused ? z[a.R + row] : 0.0, ref[row], refused ? ref[a.R + row] : 0.f, row, refused};
+}
+
+template <class E, int EACH>
+__global__ __launch_bounds__(NT) void verify_walk_kernel(VerifyArgs a) {
+    __shared__ double tab[STEPS];
+    __shared__ Tree tree;
+    const int slice = int(blockIdx.x % unsigned(a.pieces)), b = int(blockIdx.x / unsigned(a.pieces));
+    const int t = threadIdx.x;
+    const double c = rate_of(a, b);
+    walk<E, true, NT>(a, b, c, tab, tree);
+    const int row = tree.row;
+    const bool refused = row + 1 < a.R && tree.up[row + 1] == row, cold = greedy(a, b);
+    const Answer w{tree.z[row], refused ? tree.z[a.R + row] : 0.0, tree.ref[row], refused ? tree.ref[a.R + row] : 0.f, row, refused};
     if (slice == 0) {
-        if (t < a.R) a.path[int64_t(b) * a.R + t] = t < n ? line[t] : -1;
+        if (t < a.R) a.path[int64_t(b) * a.R + t] = t < tree.n ? tree.line[t] : -1;
         if (t == 0) {
-            a.count[b] = n;
+            a.count[b] = tree.n;
             a.answer[b] = w;
-            if (cold) a.next[b] = best[row];
+            if (cold) a.next[b] = tree.best[row];
         }
     }
     if (cold) return;  // (uniform)
@@ -516,7 +544,7 @@ __global__ __launch_bounds__(NT) void verify_walk_kernel(VerifyArgs a) {
     const int shift = shift_of<E>(row_of<E>(a, b, row));
 #pragma unroll
     for (int i = 0; i < EACH; ++i) e0[i] = at0<EACH>(slice, i, shift);
-    weights<E, EACH>(a, b, w, c, e0, refused, up, tok, tab, wt);
+    weights<E, EACH>(a, b, w, c, e0, refused, tab, wt);
     double* sums = a.sums + (int64_t(b) * a.pieces + slice) * (EACH * (NT / 64)) + (t >> 6);
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
@@ -528,120 +556,234 @@ __global__ __launch_bounds__(NT) void verify_walk_kernel(VerifyArgs a) {
     }
 }
 
-constexpr int DT = 512;  // threads of the draw: all runs of a vocabulary of 262144 at once
+// ---- the draw -----------------------------------------------------------------------------------------------------
+// One work-group per sequence goes through this code once: besides the loads that wait for each other its instructions' own way
+// from memory counts, so there are few of them (a logit per thread and one loop for the run and the token, 5 KB, against eight logits per lane of
+// one wave, 18 KB: 9.8 -> 4.9 us).
+constexpr int DT = 512;  // threads of the draw: all runs of a vocabulary of 262144 at once, all logits of a run
+static_assert(DT == SUB, "");
+struct Scan {
+    double tmp[DT / 64], aim;
+    int first[DT / 64], last[DT / 64];
+};
+// inclusive sum over the work-group's threads in order, and the total (every thread calls it)
+__device__ __forceinline__ double block_scan(double v, double& total, Scan& sc) {
+    const int w = threadIdx.x >> 6;
+    v = wave_scan(v);
+    __syncthreads();  // (tmp may be in use by the call before)
+    if ((threadIdx.x & 63) == 63) sc.tmp[w] = v;
+    __syncthreads();
+    double before = 0;
+    total = 0;
+#pragma unroll
+    for (int i = 0; i < DT / 64; ++i) {
+        before = i == w ? total : before;
+        total += sc.tmp[i];
+    }
+    return v + before;
+}
+// The first thread whose weight, with those ahead (upto), passes `to`; `passed`: there is one; else the last that has any (-1:
+// none).
+__device__ __forceinline__ int pick(double v, double upto, double to, bool& passed, Scan& sc) {
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint64_t any = __builtin_amdgcn_ballot_w64(v > 0), past = __builtin_amdgcn_ballot_w64(v > 0 && upto > to);
+    if ((threadIdx.x & 63) == 0) {
+        sc.first[w] = past ? w * 64 + __builtin_ctzll(past) : 0x7FFFFFFF;
+        sc.last[w] = any ? w * 64 + 63 - __builtin_clzll(any) : -1;
+    }
+    __syncthreads();
+    int first = 0x7FFFFFFF, last = -1;
+#pragma unroll
+    for (int i = 0; i < DT / 64; ++i) {
+        first = min(first, sc.first[i]);
+        last = max(last, sc.last[i]);
+    }
+    passed = first < DT;
+    return passed ? first : last;
+}
+// The same over more runs than threads: sum_at(i), 0 behind the last. The aim within the run goes to sc.aim.
+template <class F>
+__device__ int pick_long(F sum_at, int runs, double u, Scan& sc) {
+    const int t = threadIdx.x;
+    double total = 0, before = 0, part;
+    for (int i0 = 0; i0 < runs; i0 += DT) {
+        block_scan(sum_at(i0 + t), part, sc);
+        total += part;
+    }
+    const double to = u * total;
+    int found = -1;
+    for (int i0 = 0; i0 < runs; i0 += DT) {
+        const double s = sum_at(i0 + t), upto = before + block_scan(s, part, sc);
+        before += part;
+        bool passed;
+        const int at = pick(s, upto, to, passed, sc);
+        if (at == t) sc.aim = to - (upto - s);  // (of the last with any as long as none passes)
+        if (at >= 0) found = i0 + at;
+        if (passed) break;  // (uniform)
+    }
+    __syncthreads();
+    return found;
+}
+// The weight of a logit of the row that answers.
+template <class E>
+struct Weight {
+    const typename E::type *p, *q;
+    Soft sp, sq;
+    int V;
+    bool rest;
+    __device__ __forceinline__ Weight(const VerifyArgs& a, int b, const Answer& w, double c)
+        : p(row_of<E>(a, b, w.row)), q(w.refused ? row_of<E>(a, b, a.R + w.row) : p), sp(c, w.zp, w.rp), sq(c, w.zq, w.rq), V(a.V), rest(w.refused) {}
+    struct Logit {
+        typename E::type x, y;
+        bool in;
+    };
+    __device__ __forceinline__ Logit load(int e) const {
+        const bool in = e >= 0 && e < V;
+        return {p[in ? e : 0], q[in ? e : 0], in};
+    }
+    __device__ __forceinline__ double of(const Logit& l, const double* tab) const {
+        double v = sp.once(E::f32(l.x), tab);
+        if (rest) v = __builtin_fmax(v - sq.once(E::f32(l.y), tab), 0.0);  // (uniform)
+        return l.in ? v : 0.0;
+    }
+    __device__ __forceinline__ double at(int e, const double* tab) const { return of(load(e), tab); }
+};
+// The draw: of the runs, then of the run's logits. mine: sum_at(t); weight(e): logit e's; none(): nothing has any, true: sum_at has
+// changed.
+template <class F, class G, class N>
+__device__ __forceinline__ int64_t drawn(double mine, F sum_at, int runs, double u, int shift, G weight, N none, Scan& sc) {
+    const int t = threadIdx.x;
+    int e0 = 0;  // level 1: the run's first logit
+    bool runs_left = true;
+#pragma unroll 1
+    for (double v = mine;;) {
+        int at;
+        if (runs_left && runs > DT) {
+            at = pick_long(sum_at, runs, u, sc);
+        } else {
+            double total;
+            const double upto = block_scan(v, total, sc), to = runs_left ? u * total : sc.aim;
+            bool passed;
+            at = pick(v, upto, to, passed, sc);
+            if (runs_left && at == t) sc.aim = to - (upto - v);
+        }
+        if (!runs_left) return at < 0 ? -1 : e0 + at;  // (not reached without one: the run's sum is not zero)
+        if (at < 0) {
+            if (!none()) return -1;
+            v = sum_at(t);
+            continue;
+        }
+        runs_left = false;
+        e0 = at * SUB - shift;
+        v = weight(e0 + t);
+    }
+}
+
 template <class E>
 __global__ __launch_bounds__(DT) void verify_draw_kernel(VerifyArgs a, int runs) {
-    __shared__ double tab[STEPS], tmp[DT / 64], aim;
-    __shared__ int up[MAX_ROWS], pick[2];
-    __shared__ int64_t tok[MAX_ROWS];
-    const int t = threadIdx.x, b = int(blockIdx.x), lane = t & 63;
+    __shared__ double tab[STEPS];
+    __shared__ Scan sc;
+    const int t = threadIdx.x, b = int(blockIdx.x);
     const double c = rate_of(a, b);
     if (greedy(a, b)) return;  // (uniform: the walk has written the answer)
     double* sums = a.sums + int64_t(b) * runs;
-    const double mine = t < runs ? sums[t] : 0.0;
+    auto sum_at = [&](int i) { return i < runs ? sums[i] : 0.0; };
+    const double mine = sum_at(t);
     const Answer w = a.answer[b];
     const double u = a.uniform[int64_t(b) * (a.R + 1) + a.R];
-    if (t < a.R) row_at(a, b, t, tok[t], up[t]);
     fill_table(tab);
-    const int shift = shift_of<E>(row_of<E>(a, b, w.row));
-    // inclusive sum over the work-group's threads in order, and the total (every thread calls it)
-    auto block_scan = [&](double v, double& total) {
-        v = wave_scan(v);
-        __syncthreads();  // (tmp may be in use by the call before)
-        if (lane == 63) tmp[t >> 6] = v;
-        __syncthreads();
-        double before = 0;
-        total = 0;
-#pragma unroll
-        for (int i = 0; i < DT / 64; ++i) {
-            before += i < (t >> 6) ? tmp[i] : 0.0;
-            total += tmp[i];
-        }
-        return v + before;
-    };
-    // The run that the draw falls in: the first whose sum, with those ahead, passes u of all (the last that has any); the aim
-    // within it.
-    auto find = [&](double s) {
-        double total, part;
-        double upto = block_scan(s, total);
-        const bool once = runs <= DT;
-        if (!once) {
-            for (int i0 = DT; i0 < runs; i0 += DT) {
-                block_scan(i0 + t < runs ? sums[i0 + t] : 0.0, part);
-                total += part;
-            }
-        }
-        const double to = u * total;
-        if (t == 0) pick[0] = 0x7FFFFFFF, pick[1] = -1;
-        double before = 0;
-        for (int i0 = 0; i0 < runs; i0 += DT) {
-            if (!once) {
-                s = i0 + t < runs ? sums[i0 + t] : 0.0;
-                upto = before + block_scan(s, part);
-                before += part;
-            }
-            __syncthreads();
-            if (s > 0) {
-                atomicMax(&pick[1], i0 + t);
-                if (upto > to) atomicMin(&pick[0], i0 + t);
-            }
-            __syncthreads();
-            const bool passed = pick[0] < runs;
-            if ((passed ? pick[0] : pick[1]) == i0 + t) aim = to - (upto - s);  // (of the last with any as long as none passes)
-            if (passed) break;  // (uniform)
-        }
-        __syncthreads();
-        return pick[0] < runs ? pick[0] : pick[1];
-    };
-    bool rest = w.refused;
-    double wt[1][8];
-    int from = find(mine);
-    if (from < 0 && rest) {  // (uniform) nothing is left of p - q: the answer is p's
-        rest = false;
+    Weight<E> weight(a, b, w, c);
+    const int shift = shift_of<E>(weight.p);
+    const int64_t x = drawn(mine, sum_at, runs, u, shift, [&](int e) { return weight.at(e, tab); }, [&]() {
+        if (!weight.rest) return false;
+        weight.rest = false;  // nothing is left of p - q: the answer is p's
+#pragma unroll 1
         for (int i = t >> 6; i < runs; i += DT / 64) {
-            const int e0[1] = {i * SUB + lane * 8 - shift};
-            weights<E, 1>(a, b, w, c, e0, false, up, tok, tab, wt);
             double s = 0;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) s += wt[0][k];
+#pragma unroll 1
+            for (int j = t & 63; j < SUB; j += 64) s += weight.at(i * SUB - shift + j, tab);
             s = wave_sum(s);
-            if (lane == 0) sums[i] = s;
+            if ((t & 63) == 0) sums[i] = s;
         }
         __syncthreads();
-        from = find(t < runs ? sums[t] : 0.0);
-    }
-    if (t >= 64) return;
-    if (from < 0) {
-        if (t == 0) a.next[b] = -1;
+        return true;
+    }, sc);
+    if (t == 0) a.next[b] = x;
+}
+
+// Without drafts' probabilities: the walk and the draw. The runs' sums are the rows kernel's, but those with a child's token,
+// which are taken again without it (subtracted, a likely child would leave its rounding).
+constexpr double LEAST_RUN = 0x1p-1009;  // a run's sum that counts as none: all its logits could be ones that do
+template <class E>
+__global__ __launch_bounds__(DT) void verify_answer_kernel(VerifyArgs a, int per_row) {
+    __shared__ double tab[STEPS], less[MAX_ROWS], part[MAX_ROWS][DT / 64];
+    __shared__ int child[MAX_ROWS], children;
+    __shared__ Tree tree;
+    __shared__ Scan sc;
+    const int t = threadIdx.x, b = int(blockIdx.x);
+    const double c = rate_of(a, b);
+    const double u = a.uniform[int64_t(b) * (a.R + 1) + a.R];
+    walk<E, false, DT>(a, b, c, tab, tree);
+    const int row = tree.row;
+    if (t < a.R) a.path[int64_t(b) * a.R + t] = t < tree.n ? tree.line[t] : -1;
+    if (t == 0) a.count[b] = tree.n;
+    if (greedy(a, b)) {  // (uniform)
+        if (t == 0) a.next[b] = tree.best[row];
         return;
     }
-    // ---- and the token in it, by the first wave
-    const int e0[1] = {from * SUB + lane * 8 - shift};
-    weights<E, 1>(a, b, w, c, e0, rest, up, tok, tab, wt);
-    double s = 0;
-    int last = -1;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        s += wt[0][k];
-        if (wt[0][k] > 0) last = k;
+    const Weight<E> weight(a, b, Answer{tree.z[row], 0.0, tree.ref[row], 0.f, row, 0}, c);
+    const int shift = shift_of<E>(weight.p), runs = (a.V + shift + SUB - 1) / SUB;
+    const Part* run = a.run + (int64_t(b) * a.R + row) * per_row;
+    Part first{0.0, -INFINITY, 0};  // (on its way while the children's runs are)
+    if (t < runs) first = run[t];
+    // ---- the children that were tried, and the sums of their runs without them
+    if (t < 64) {
+        const bool is = t < a.R && tree.up[t] == row;
+        const uint64_t m = __builtin_amdgcn_ballot_w64(is);
+        if (is) child[__popcll(m & ((uint64_t(1) << t) - 1))] = int(tree.tok[t]);
+        if (t == 0) children = __popcll(m);
     }
-    const double upto = wave_scan(s), to = aim;
-    const uint64_t past = __builtin_amdgcn_ballot_w64(last >= 0 && upto > to), any = __builtin_amdgcn_ballot_w64(last >= 0);
-    if (any == 0) return;  // (not reached: the run's sum is not zero)
-    if (lane != (past ? __builtin_ctzll(past) : 63 - __builtin_clzll(any))) return;
-    double run = upto - s;
-    int at = -1;
+    __syncthreads();
+    const int kids = children;
+    auto without = [&](int e, double v) {
+#pragma unroll 1
+        for (int k = 0; k < kids; ++k) v = child[k] == e ? 0.0 : v;
+        return v;
+    };
+    if (kids > 0) {  // (uniform)
+        auto at = [&](int k) { return (child[k] + shift) / SUB * SUB - shift + t; };  // this thread's logit of child k's run
+        auto next = weight.load(at(0));
+#pragma unroll 1
+        for (int k = 0; k < kids; ++k) {
+            const auto l = next;
+            next = weight.load(at(min(k + 1, kids - 1)));
+            const double s = wave_sum(without(at(k), weight.of(l, tab)));
+            if ((t & 63) == 0) part[k][t >> 6] = s;
+        }
+        __syncthreads();
+        if (t < kids) {
+            double s = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        run += wt[0][k];
-        if (at < 0 && wt[0][k] > 0 && run > to) at = k;
+            for (int w = 0; w < DT / 64; ++w) s += part[t][w];
+            less[t] = s;
+        }
+        __syncthreads();
     }
-    a.next[b] = e0[0] + (at < 0 || !past ? last : at);  // (the last with a weight, where rounding lets none pass)
+    auto sum_of = [&](int i, const Part& p) {
+        double s = p.ref == weight.sp.ref ? p.sum : p.ref == -INFINITY ? 0.0 : p.sum * exp2_steps((double(p.ref) - weight.sp.ref) * c, tab);
+        s = s >= LEAST_RUN ? s * weight.sp.z : 0.0;
+#pragma unroll 1
+        for (int k = 0; k < kids; ++k) s = (child[k] + shift) / SUB == i ? less[k] : s;
+        return s;
+    };
+    const int64_t x = drawn(t < runs ? sum_of(t, first) : 0.0, [&](int i) { return i < runs ? sum_of(i, run[i]) : 0.0; }, runs, u, shift,
+                            [&](int e) { return without(e, weight.at(e, tab)); }, [&]() { return false; }, sc);
+    if (t == 0) a.next[b] = x;
 }
 
 template <class E, int ROWS, int WALK>
 int launch(const VerifyArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL((verify_rows_kernel<E, ROWS>), dim3(unsigned(int64_t(a.slices) * a.rows * a.B)), dim3(NT), 0, st, a);
+    hipLaunchKernelGGL((verify_rows_kernel<E, ROWS, false>), dim3(unsigned(int64_t(a.slices) * a.rows * a.B)), dim3(NT), 0, st, a);
     MDX_LAUNCHED();
     hipLaunchKernelGGL((verify_walk_kernel<E, WALK>), dim3(unsigned(a.pieces * a.B)), dim3(NT), 0, st, a);
     MDX_LAUNCHED();
@@ -649,18 +791,25 @@ int launch(const VerifyArgs& a, hipStream_t st) {
     MDX_LAUNCHED();
     return MDX_OK;
 }
+template <class E, int ROWS>
+int launch_rows(const VerifyArgs& a, int walk, hipStream_t st) {
+    if (a.draft) return walk == 4 ? launch<E, ROWS, 4>(a, st) : launch<E, ROWS, 1>(a, st);
+    hipLaunchKernelGGL((verify_rows_kernel<E, ROWS, true>), dim3(unsigned(int64_t(a.slices) * a.rows * a.B)), dim3(NT), 0, st, a);
+    MDX_LAUNCHED();
+    hipLaunchKernelGGL((verify_answer_kernel<E>), dim3(unsigned(a.B)), dim3(DT), 0, st, a, a.slices * ROWS * (NT / 64));
+    MDX_LAUNCHED();
+    return MDX_OK;
+}
 template <class E>
 int launch_any(const VerifyArgs& a, int rows, int walk, hipStream_t st) {
-    if (rows == 8) return walk == 4 ? launch<E, 8, 4>(a, st) : launch<E, 8, 1>(a, st);
-    if (rows == 4) return walk == 4 ? launch<E, 4, 4>(a, st) : launch<E, 4, 1>(a, st);
-    return walk == 4 ? launch<E, 1, 4>(a, st) : launch<E, 1, 1>(a, st);
+    return rows == 8 ? launch_rows<E, 8>(a, walk, st) : rows == 4 ? launch_rows<E, 4>(a, walk, st) : launch_rows<E, 1>(a, walk, st);
 }
 
 int64_t slices_of(int64_t V, int each) { return (V + 7 + slice_of(each) - 1) / slice_of(each); }
 // Pieces of eight logits per thread: as many as leave work-groups enough (their exponentials are a chain of 2 us).
 int rows_each(int64_t B, int64_t rows, int64_t V) { return B * rows * slices_of(V, 8) >= 2048 ? 8 : B * rows * slices_of(V, 4) >= 1024 ? 4 : 1; }
 int walk_each(int64_t B, int64_t V) { return B * slices_of(V, 1) > 2048 ? 4 : 1; }
-int64_t runs_of(int64_t B, int64_t V) { return slices_of(V, walk_each(B, V)) * walk_each(B, V) * (NT / 64); }  // (a multiple of 4)
+int64_t runs_of(int64_t V, int each) { return slices_of(V, each) * each * (NT / 64); }  // (a multiple of 4)
 
 }  // namespace
 }  // namespace mdx
@@ -669,8 +818,10 @@ using namespace mdx;
 
 extern "C" size_t mdx_verify_drafts_workspace(int64_t B, int64_t R, int64_t V, int32_t drafted) {
     if (B < 1 || B > 1024 || R < 1 || R > MAX_ROWS || V < 1 || V >= (int64_t(1) << 24)) return 0;
-    const int64_t rows = drafted ? 2 * R - 1 : R, slices = slices_of(V, rows_each(B, rows, V));
-    return size_t(B * rows * slices) * sizeof(Part) + size_t(B * runs_of(B, V)) * 8 + size_t(B) * sizeof(Answer);
+    const int64_t rows = drafted ? 2 * R - 1 : R;
+    const int each = rows_each(B, rows, V);
+    const size_t parts = size_t(B * rows * slices_of(V, each)) * sizeof(Part);
+    return parts + (drafted ? size_t(B * runs_of(V, walk_each(B, V))) * 8 + size_t(B) * sizeof(Answer) : size_t(B * R * runs_of(V, each)) * sizeof(Part));
 }
 
 extern "C" int mdx_verify_drafts(const void* logits, int64_t seq_stride, int64_t row_stride, const void* draft,
@@ -709,8 +860,12 @@ extern "C" int mdx_verify_drafts(const void* logits, int64_t seq_stride, int64_t
     a.slices = int(slices_of(V, rows)), a.pieces = int(slices_of(V, walk));
     MDX_CHECK(B * a.rows * a.slices < (int64_t(1) << 30), "too many rows times logits for one call");
     a.part = static_cast<Part*>(workspace);
-    a.sums = reinterpret_cast<double*>(a.part + B * a.rows * a.slices);
-    a.answer = reinterpret_cast<Answer*>(a.sums + B * runs_of(B, V));
+    if (drafted) {
+        a.sums = reinterpret_cast<double*>(a.part + B * a.rows * a.slices);
+        a.answer = reinterpret_cast<Answer*>(a.sums + B * runs_of(V, walk));
+    } else {
+        a.run = a.part + B * a.rows * a.slices;
+    }
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (dtype == MDX_DT_BF16) return launch_any<Bf>(a, rows, walk, st);
     if (dtype == MDX_DT_F16) return launch_any<Hf>(a, rows, walk, st);
