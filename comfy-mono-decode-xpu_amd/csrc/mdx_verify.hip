@@ -18,7 +18,7 @@
 // work-group of the second launch can not do that cheaply: a release to the other XCDs' caches by each of 600 cost 30 us.)
 //
 // What bounds it: many rows the exponentials, 14 vector instructions each, eight of them float64 (7 rows of 32 sequences and their
-// drafts over 151936: 37 us for 126 MB, 25 at the rate of a large copy; with 20 instructions 51), then the walk and the draw, 18
+// drafts over 151936: 37 us for 126 MB, 25 at the rate of a large copy; with 20 instructions 51), then the walk and the draw, 16
 // and 5 us, chains of dependent loads; one short chain those alone (14 us a call). 8 rows of 16 trees: 17 us and 11.
 // Exponentials: 2^(a / 128) = table[k % 128] 2^(k / 128) poly(a - k), k = rint(a): a table of 1 KiB in LDS, a polynomial of degree 3
 // through the Chebyshev points of [-1/2, 1/2] (2.8e-13 relative); x / T as it stands, without a maximum, as long as none is past
@@ -377,39 +377,11 @@ struct Soft {
         cut = fmaxf(-3.402823466e38f, float(ref + LEAST / c));
     }
     __device__ __forceinline__ double of(float x, const double* tab) const {
-        const float y = fmaxf(x, cut);
-        const double e = ref == 0.0 ? add_exp(0.0, y, c, tab) : exp2_steps((double(fminf(y, 3.402823466e38f)) - ref) * c, tab);
-        return x >= cut && !none ? e * z : 0.0;
-    }
-    __device__ __forceinline__ double once(float x, const double* tab) const {  // (less code)
         const double e = exp2_steps((double(fminf(x, 3.402823466e38f)) - ref) * c, tab);
         return x >= cut && !none ? e * z : 0.0;
     }
 };
 
-// The weights of the eight logits from e0 on (8 lanes apart in a wave) of the row that answers.
-template <class E, int N>
-__device__ __forceinline__ void weights(const VerifyArgs& a, int b, const Answer& w, double c, const int (&e0)[N], bool rest, const double* tab,
-                                        double (&wt)[N][8]) {
-    const typename E::type *pr = row_of<E>(a, b, w.row), *qr = rest ? row_of<E>(a, b, a.R + w.row) : pr;
-    const bool alike = shift_of<E>(pr) == shift_of<E>(qr);  // (to the 16-byte boundaries)
-    Piece<E> x[N], y[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = piece_at<E>(pr, a.V, e0[i], true);
-    if (rest)  // (uniform)
-#pragma unroll
-        for (int i = 0; i < N; ++i) y[i] = piece_at<E>(qr, a.V, e0[i], alike);
-    const Soft p(c, w.zp, w.rp), q(c, w.zq, w.rq);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            wt[i][k] = p.of(x[i][k], tab);
-            if (rest) wt[i][k] = __builtin_fmax(wt[i][k] - q.of(y[i][k], tab), 0.0);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-    }
-}
 // row t's token and parent (thread t): what can be reached
 __device__ __forceinline__ void row_at(const VerifyArgs& a, int b, int t, int64_t& x, int& parent) {
     x = a.tokens[int64_t(b) * a.R + t];
@@ -489,7 +461,7 @@ __device__ __forceinline__ void walk(const VerifyArgs& a, int b, double c, doubl
     }
     __syncthreads();
     // probability of this thread's token in its parent's row (r >= R: the draft's)
-    auto prob = [&](int r, float l) -> double { return cold ? (x == tree.best[r] ? 1.0 : 0.0) : Soft(c, tree.z[r], tree.ref[r]).once(l, tab); };
+    auto prob = [&](int r, float l) -> double { return cold ? (x == tree.best[r] ? 1.0 : 0.0) : Soft(c, tree.z[r], tree.ref[r]).of(l, tab); };
     if (parent >= 0) {
         bool again = false;  // (a token that a sibling ahead has tried)
         for (int s = 1; s < t && !DRAFT; ++s) again = again || (tree.up[s] == parent && tree.tok[s] == x);
@@ -538,19 +510,28 @@ __global__ __launch_bounds__(NT) void verify_walk_kernel(VerifyArgs a) {
         }
     }
     if (cold) return;  // (uniform)
-    // the sum of every wave's runs of SUB logits
-    double wt[EACH][8];
-    int e0[EACH];
-    const int shift = shift_of<E>(row_of<E>(a, b, row));
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) e0[i] = at0<EACH>(slice, i, shift);
-    weights<E, EACH>(a, b, w, c, e0, refused, tab, wt);
+    // the sums of every wave's runs of SUB logits, the next one's logits on their way
+    const typename E::type *pr = row_of<E>(a, b, row), *qr = refused ? row_of<E>(a, b, a.R + row) : pr;
+    const int shift = shift_of<E>(pr);
+    const bool alike = shift == shift_of<E>(qr);  // (to the 16-byte boundaries)
+    const Soft p(c, w.zp, w.rp), q(c, w.zq, w.rq);
     double* sums = a.sums + (int64_t(b) * a.pieces + slice) * (EACH * (NT / 64)) + (t >> 6);
-#pragma unroll
+    Piece<E> x = piece_at<E>(pr, a.V, at0<EACH>(slice, 0, shift), true), y = piece_at<E>(qr, a.V, at0<EACH>(slice, 0, shift), alike);
+#pragma unroll 1
     for (int i = 0; i < EACH; ++i) {
+        const Piece<E> x0 = x, y0 = y;
+        if (i + 1 < EACH) {
+            const int e = at0<EACH>(slice, i + 1, shift);
+            x = piece_at<E>(pr, a.V, e, true);
+            y = piece_at<E>(qr, a.V, e, alike);
+        }
         double s = 0;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) s += wt[i][k];
+        for (int k = 0; k < 8; ++k) {
+            double v = p.of(x0[k], tab);
+            if (refused) v = __builtin_fmax(v - q.of(y0[k], tab), 0.0);  // (uniform)
+            s += v;
+        }
         s = wave_sum(s);
         if ((t & 63) == 0) sums[i * (NT / 64)] = s;
     }
@@ -642,8 +623,8 @@ struct Weight {
         return {p[in ? e : 0], q[in ? e : 0], in};
     }
     __device__ __forceinline__ double of(const Logit& l, const double* tab) const {
-        double v = sp.once(E::f32(l.x), tab);
-        if (rest) v = __builtin_fmax(v - sq.once(E::f32(l.y), tab), 0.0);  // (uniform)
+        double v = sp.of(E::f32(l.x), tab);
+        if (rest) v = __builtin_fmax(v - sq.of(E::f32(l.y), tab), 0.0);  // (uniform)
         return l.in ? v : 0.0;
     }
     __device__ __forceinline__ double at(int e, const double* tab) const { return of(load(e), tab); }
@@ -793,7 +774,7 @@ int launch(const VerifyArgs& a, hipStream_t st) {
 }
 template <class E, int ROWS>
 int launch_rows(const VerifyArgs& a, int walk, hipStream_t st) {
-    if (a.draft) return walk == 4 ? launch<E, ROWS, 4>(a, st) : launch<E, ROWS, 1>(a, st);
+    if (a.draft) return walk == 4 ? launch<E, ROWS, 4>(a, st) : walk == 2 ? launch<E, ROWS, 2>(a, st) : launch<E, ROWS, 1>(a, st);
     hipLaunchKernelGGL((verify_rows_kernel<E, ROWS, true>), dim3(unsigned(int64_t(a.slices) * a.rows * a.B)), dim3(NT), 0, st, a);
     MDX_LAUNCHED();
     hipLaunchKernelGGL((verify_answer_kernel<E>), dim3(unsigned(a.B)), dim3(DT), 0, st, a, a.slices * ROWS * (NT / 64));
@@ -808,7 +789,8 @@ int launch_any(const VerifyArgs& a, int rows, int walk, hipStream_t st) {
 int64_t slices_of(int64_t V, int each) { return (V + 7 + slice_of(each) - 1) / slice_of(each); }
 // Pieces of eight logits per thread: as many as leave work-groups enough (their exponentials are a chain of 2 us).
 int rows_each(int64_t B, int64_t rows, int64_t V) { return B * rows * slices_of(V, 8) >= 2048 ? 8 : B * rows * slices_of(V, 4) >= 1024 ? 4 : 1; }
-int walk_each(int64_t B, int64_t V) { return B * slices_of(V, 1) > 2048 ? 4 : 1; }
+// (the walk, over 151936: 32 sequences 17.2 us with one, 16.0 with two, 17.4 with four; 64: 24.0 with two, 21.9 with four)
+int walk_each(int64_t B, int64_t V) { return B * slices_of(V, 1) > 4096 ? 4 : B * slices_of(V, 1) > 2048 ? 2 : 1; }
 int64_t runs_of(int64_t V, int each) { return slices_of(V, each) * each * (NT / 64); }  // (a multiple of 4)
 
 }  // namespace

@@ -1392,8 +1392,8 @@ def verify_drafts(logits, tokens, uniform, draft=None, parent=None, temperature=
     Without draft (drafts that are no samples; trees): of a row's children, in row order, the first is accepted whose token,
     with the distinct ones ahead of it, has more of p_r than uniform[b, r]; if none has, the answer is drawn from p_r without
     their tokens. A row with no drafted token behind it answers from p_r. Drawn: the lowest index whose cumulative weight
-    passes uniform[b, R] of the whole, in 64-bit sums. uniform float64 [B, R + 1] in [0, 1). temperature: a number, or float32
-    [B]; 0: the lowest index of the largest logit has all of p_r. A logit of -inf or NaN has no probability; +inf counts as
+    passes uniform[b, R] of the whole, in 64-bit sums (a weight under 2^-100 of the largest may count as
+    none). uniform float64 [B, R + 1] in [0, 1). temperature: a number, or float32 [B]; 0: the lowest index of the largest logit has all of p_r. A logit of -inf or NaN has no probability; +inf counts as
     the largest finite number.
     Returns (count int32 [B]: row 0 and the accepted rows, path int32 [B, R]: those rows, -1 behind, next int64 [B]: the
     answer, -1 where no token has a probability); count and path are page_commit's. The role of mtp_accept's walk

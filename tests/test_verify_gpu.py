@@ -215,3 +215,102 @@ def test_draws_in_every_run(C, dev):
     u[:, 1] = (at.double() + 0.5) / V
     got = C.verify_drafts(logits, torch.zeros(B, 1, dtype=torch.int64, device=dev), u.to(dev))
     assert torch.equal(got[2].cpu(), at)
+
+
+@pytest.mark.parametrize("B,R,V", [(1024, 3, 40), (1, 2, (1 << 24) - 1), (2, 64, 2100), (3, 64, 30000)])
+def test_the_largest_without_draft_probabilities(C, B, R, V):
+    """As chains, and as trees whose rows are all children of the first one, distinct tokens and (in the last sequence) one alone."""
+    logits, _, tokens, uniform = inputs(31, B, R, V, "bf16")
+    check(C, logits, tokens, uniform, heat=0.9)
+    tokens[:, 1:] = logits[:, 0].float().topk(R - 1, -1).indices.flip(-1)
+    tokens[-1, 1:] = tokens[-1, 1]
+    for u in (uniform, 0.9 + 0.1 * uniform):
+        check(C, logits, tokens, u, parent=torch.zeros(B, R, dtype=torch.int32), heat=0.9)
+
+
+@pytest.mark.parametrize("V", [5000, 9000])
+def test_many_short_vocabularies(C, V):
+    """Work-groups of several runs each."""
+    logits, draft, tokens, uniform = inputs(32, 1024, 2, V, "bf16")
+    check(C, logits, tokens, uniform, draft)
+
+
+def test_extreme_temperatures_without_draft_probabilities(C):
+    """References far from zero that differ between the waves of a row, runs far below it, masked ones."""
+    logits, _, tokens, uniform = inputs(33, 8, 3, 60000, "fp32")
+    logits[6, :, :30000] -= 3000.0
+    logits[7, :, 700:] = float("-inf")
+    heat = torch.tensor([1e-30, 1e-3, 50.0, 1e30, 2.0 ** -140, 0.004, 1.0, 0.01])
+    best = logits.topk(3, -1).indices
+    for rank in (0, 1):
+        tokens[:, 1:] = best[:, :2, rank]
+        check(C, logits, tokens, uniform, heat=heat)
+        # A uniform of 0 is passed by any weight. Which ones there are depends on where the range of a 64-bit exponential ends:
+        # the oracle's at 2^-1074 of the largest; the kernel's at 2^-1009 of a reference that is up to 2^900 above that (0 while
+        # the largest logit's own exponent is within 900 of it). No weight below the answer's is 2^(900 - 1009) of the largest.
+        out = C.verify_drafts(logits.cuda(), tokens.cuda(), uniform.cuda() * 0, temperature=heat.cuda())
+        want = ref.verify_drafts(f64(logits), tokens.numpy(), uniform.numpy() * 0, heat=heat.numpy())
+        assert out[0].tolist() == want[0].tolist() and out[1].tolist() == want[1].tolist()
+        for b, got in enumerate(out[2].tolist()):
+            x = f64(logits[b, int(want[1][b][want[0][b] - 1])])
+            steps = (x - x.max()) / float(heat[b]) / np.log(2.0)
+            assert 0 <= got and np.isfinite(x[got]) and (steps[:got] < 900 - 1009 + 1e-6).all()
+    check(C, logits, tokens, 1.0 - (1.0 - uniform) * 2.0 ** -20, heat=heat)
+
+
+def test_likely_children_refused(C):
+    """A child that has nearly all of a run's weight, or of the row's, is refused: the draw is from what its run has beside it."""
+    B, V = 12, 4096
+    logits, _, tokens, uniform = inputs(34, B, 3, V, "fp32", spread=0.2)
+    at = torch.arange(B) * 341 + 5
+    for b in range(B):
+        logits[b, :, at[b]] = 8.0 + 3.0 * b  # (up to e^41 times the others)
+        tokens[b, 1] = at[b]
+        tokens[b, 2] = at[b] + 1
+    parent = torch.zeros(B, 3, dtype=torch.int32)
+    p = torch.tensor([1.0 - ref.token_probabilities(f64(logits[b, 0]), 1.0)[[int(at[b]), int(at[b]) + 1]].sum() for b in range(B)], dtype=torch.float64)
+    uniform[:, 0] = torch.clamp(1.0 - p * 0.25, max=1.0 - 2.0 ** -53)
+    want = check(C, logits, tokens, uniform, parent=parent)
+    assert (want[0][:9] == 1).all()
+    assert all(int(t) not in (int(i), int(i) + 1) for t, i in zip(want[2][:9], at[:9]))
+
+
+def test_strided_rows_without_draft_probabilities(C, dev):
+    for dt in ("bf16", "fp32"):
+        logits, _, tokens, uniform = inputs(35, 3, 4, 8190, dt)
+        tokens[:, 1:] = logits[:, :3].float().argmax(-1)
+        for off, pad in ((1, 3), (3, 0), (5, 8), (7, 1)):
+            wide = torch.full((3, 4, 8190 + off + pad), 99.0, dtype=DT[dt], device=dev)
+            view = wide[:, :, off:off + 8190]
+            view.copy_(logits)
+            got = C.verify_drafts(view, tokens.to(dev), uniform.to(dev), temperature=0.9)
+            want = ref.verify_drafts(f64(logits), tokens.numpy(), uniform.numpy(), heat=0.9)
+            assert [g.cpu().tolist() for g in got] == [w.tolist() for w in want]
+
+
+def test_replay_without_draft_probabilities(C, dev):
+    a = [inputs(40 + i, 5, 6, 40000, "bf16") for i in range(3)]
+    parent = torch.tensor([[0, 0, 0, 1, 1, 2]] * 5, dtype=torch.int32)
+    for _, _, tokens, uniform in a:
+        uniform[:, :6] *= 0.3
+    for x in a:
+        best = x[0].float().topk(2, -1).indices
+        for r in range(1, 6):
+            x[2][:, r] = best[:, parent[0, r], r % 2]
+    hold = [t.to(dev) for t in (a[0][0], a[0][2], a[0][3], parent)]
+    C.verify_drafts(*hold[:3], parent=hold[3])
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        out = C.verify_drafts(*hold[:3], parent=hold[3])
+    for i in (1, 2, 0, 1):
+        for h, t in zip(hold, (a[i][0], a[i][2], a[i][3])):
+            h.copy_(t)
+        torch.cuda.synchronize()
+        graph.replay()
+        with torch.cuda.stream(side):
+            beside = C.verify_drafts(a[2][0].to(dev), a[2][2].to(dev), a[2][3].to(dev), parent=parent.to(dev))
+        torch.cuda.synchronize()
+        for got, x in ((out, a[i]), (beside, a[2])):
+            want = ref.verify_drafts(f64(x[0]), x[2].numpy(), x[3].numpy(), parent=parent.numpy())
+            assert [g.cpu().tolist() for g in got] == [w.tolist() for w in want]
