@@ -19,7 +19,7 @@
 //
 // What bounds it: many rows the exponentials, 14 vector instructions each, eight of them float64 (7 rows of 32 sequences and their
 // drafts over 151936: 37 us for 126 MB, 25 at the rate of a large copy; with 20 instructions 51), then the walk and the draw, 16
-// and 5 us, chains of dependent loads; one short chain those alone (14 us a call). 8 rows of 16 trees: 17 us and 11.
+// and 5 us, chains of dependent loads; one short chain those alone (14 us a call). 8 rows of 16 trees: 16 us and 11.
 // Exponentials: 2^(a / 128) = table[k % 128] 2^(k / 128) poly(a - k), k = rint(a): a table of 1 KiB in LDS, a polynomial of degree 3
 // through the Chebyshev points of [-1/2, 1/2] (2.8e-13 relative); x / T as it stands, without a maximum, as long as none is past
 // 2^900 (then the row is read again less its largest).
@@ -211,17 +211,29 @@ __device__ __forceinline__ double across(double v) {  // 0 where there is no suc
     return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, ROWS, 0xF, false),
                             __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, ROWS, 0xF, false));
 }
-__device__ __forceinline__ double wave_sum(double v) {  // in every lane
+// a's sums over the rows of 16 lanes 2 i and 2 i + 1, in row 2 i, b's in row 2 i + 1
+__device__ __forceinline__ double join16(double a, double b) {
+    const auto l = __builtin_amdgcn_permlane16_swap(unsigned(__double2loint(a)), unsigned(__double2loint(b)), false, false);
+    const auto h = __builtin_amdgcn_permlane16_swap(unsigned(__double2hiint(a)), unsigned(__double2hiint(b)), false, false);
+    return __hiloint2double(int(h[0]), int(l[0])) + __hiloint2double(int(h[1]), int(l[1]));
+}
+// a's sums over the halves of the wave, in the lower one, b's in the upper one
+__device__ __forceinline__ double join32(double a, double b) {
+    const auto l = __builtin_amdgcn_permlane32_swap(unsigned(__double2loint(a)), unsigned(__double2loint(b)), false, false);
+    const auto h = __builtin_amdgcn_permlane32_swap(unsigned(__double2hiint(a)), unsigned(__double2hiint(b)), false, false);
+    return __hiloint2double(int(h[0]), int(l[0])) + __hiloint2double(int(h[1]), int(l[1]));
+}
+__device__ __forceinline__ double row_sum(double v) {  // over 16 lanes, in each of them
     v += across<0x128>(v);  // lane ^ 8 of the 16, ^ 7, ^ 3, ^ 1
     v += across<0x141>(v);
     v += across<0x1B>(v);
     v += across<0xB1>(v);
-    const auto l16 = __builtin_amdgcn_permlane16_swap(unsigned(__double2loint(v)), unsigned(__double2loint(v)), false, false);
-    const auto h16 = __builtin_amdgcn_permlane16_swap(unsigned(__double2hiint(v)), unsigned(__double2hiint(v)), false, false);
-    v = __hiloint2double(int(h16[0]), int(l16[0])) + __hiloint2double(int(h16[1]), int(l16[1]));
-    const auto l32 = __builtin_amdgcn_permlane32_swap(unsigned(__double2loint(v)), unsigned(__double2loint(v)), false, false);
-    const auto h32 = __builtin_amdgcn_permlane32_swap(unsigned(__double2hiint(v)), unsigned(__double2hiint(v)), false, false);
-    return __hiloint2double(int(h32[0]), int(l32[0])) + __hiloint2double(int(h32[1]), int(l32[1]));
+    return v;
+}
+__device__ __forceinline__ double wave_sum(double v) {  // in every lane
+    v = row_sum(v);
+    v = join16(v, v);
+    return join32(v, v);
 }
 __device__ __forceinline__ double wave_scan(double v) {  // inclusive, in lane order
     v += across<0x111>(v);  // the lane 1, 2, 4, 8 ahead in the row of 16
@@ -270,15 +282,15 @@ __global__ __launch_bounds__(NT) void verify_rows_kernel(VerifyArgs a) {
     __syncthreads();  // (the table)
     // the wave's run i
     auto put = [&](int i, double sum, float from) {
-        if (lane == 0) a.run[((int64_t(b) * a.R + r) * a.slices + slice) * (EACH * (NT / 64)) + i * (NT / 64) + w] = Part{sum, from, 0};
+        a.run[((int64_t(b) * a.R + r) * a.slices + slice) * (EACH * (NT / 64)) + i * (NT / 64) + w] = Part{sum, from, 0};
     };
-    double s = 0, s0 = 0, s1 = 0;
+    double s = 0, s0 = 0, s1 = 0, one = 0, two = 0;
     float top = -1.f, ref = 0.f;
     int at = 0x7FFFFFFF;
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
         const int e = first + i * NT * 8;
-        if (e >= a.V) break;  // (uniform)
+        if (!RUNS && e >= a.V) break;  // (uniform)
         if constexpr (RUNS) s0 = s1 = 0;
         if (e >= 0 && e + SUB <= a.V) {
 #pragma unroll
@@ -288,7 +300,7 @@ __global__ __launch_bounds__(NT) void verify_rows_kernel(VerifyArgs a) {
                 s0 = add_exp(s0, x0, c, tab);
                 s1 = add_exp(s1, x1, c, tab);
             }
-        } else {  // (an end of the row: what is -inf counts as 2^-1020)
+        } else if (!RUNS || e < a.V) {  // (an end of the row: what is -inf counts as 2^-1020)
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 const float y = x[i][k];
@@ -296,17 +308,31 @@ __global__ __launch_bounds__(NT) void verify_rows_kernel(VerifyArgs a) {
                 s0 += exp2_steps(double(y) * c, tab);
             }
         }
-        if constexpr (RUNS) {
-            s0 = wave_sum(s0 + s1);
-            put(i, s0, 0.f);
-            s += s0;
+        // Runs' sums over the wave, four together: two, then four of them side by side in the lanes, a row of 16 lanes each in the
+        // order 0, 2, 1, 3 (one by one: 17.4 us for 8 rows of 16 sequences over 151936, so 15.8,
+        // without any 15.2).
+        if constexpr (RUNS && EACH == 1) {
+            s = wave_sum(s0 + s1);
+            if (lane == 0) put(0, s, 0.f);
+        } else if constexpr (RUNS) {
+            if (i % 2 == 0) {
+                one = s0 + s1;
+            } else if (i % 4 == 1) {
+                two = join32(one, s0 + s1);
+            } else {
+                const double four = row_sum(join16(two, join32(one, s0 + s1)));
+                if ((lane & 15) == 0) put(i - 3 + (lane >> 5) + (lane >> 4 & 1) * 2, four, 0.f);
+                s += four;
+            }
         }
         __builtin_amdgcn_sched_barrier(0);  // (eight at a time are enough in flight: more cost registers, and waves)
     }
     if constexpr (!RUNS) s = s0 + s1;
+    else if (EACH > 1) s = join16(s, s), s = join32(s, s);
     // (a NaN makes the sum one; a lane past the row's end has top -1)
     const bool near = c > 0.0 && double(top) * c < FAR && s == s;
     if (__builtin_amdgcn_ballot_w64(!near) != 0 || __builtin_amdgcn_ballot_w64(top >= 0.f) == 0) {  // (uniform in the wave)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the runs above are written before they are again)
         // once more: the largest, and whether a reference of 0 will do with the others raised to weights of 2^-1020
         ref = -INFINITY;
 #pragma unroll 1
@@ -337,12 +363,12 @@ __global__ __launch_bounds__(NT) void verify_rows_kernel(VerifyArgs a) {
                 for (int k = 0; k < 8; ++k) si += exp2_steps((double(clean(y[k])) - less) * c, tab);
                 if constexpr (RUNS) {
                     si = wave_sum(si);
-                    put(i, si, ref);
+                    if (lane == 0) put(i, si, ref);
                 }
                 s += si;
             }
         } else if constexpr (RUNS) {
-            for (int i = 0; i < EACH; ++i) put(i, 0.0, -INFINITY);
+            for (int i = lane; i < EACH; i += 64) put(i, 0.0, -INFINITY);
         }
     }
     if constexpr (!RUNS) s = wave_sum(s);
