@@ -435,7 +435,15 @@ PyObject* attn_mass(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
         } else {
             out = at::zeros({B, Hk, N}, at::TensorOptions().dtype(at::kFloat).device(d));
         }
-        if (B > 0) {  // (no rows: the prior sums)
+        if (B > 0 && S == 0) {  // the prior sums: a row that does not count
+            const auto of = [&](at::ScalarType type) { return at::TensorOptions().dtype(type).device(d); };
+            const at::Tensor none = at::zeros({B}, of(at::kInt)), row = at::empty({B, 1, H, D}, of(q.scalar_type())), sum = at::empty({B, 1, H}, of(at::kFloat));
+            call("mdx_attn_mass", d, [&](void* st) {
+                return g.mass(data(row), H * D, H * D, D, data(key), key.stride(0), key.stride(1), key.stride(2), dt, table.data_ptr<int32_t>(),
+                              table.stride(0), length.data_ptr<int32_t>(), sum.data_ptr<float>(), prior, pb, ph, none.data_ptr<int32_t>(), nullptr,
+                              window, sinks, out.data_ptr<float>(), out.stride(0), out.stride(1), N, B, 1, H, Hk, D, P, T, W, scale, nullptr, 0, st);
+            });
+        } else if (B > 0) {
             const size_t n = g.mass_workspace(B, S, H, Hk, D, T, W, N);
             at::Tensor ws;
             if (n) ws = scratch(n, d);

@@ -516,13 +516,13 @@ extern "C" int mdx_attn_mass(const void* q, int64_t q_seq_stride, int64_t q_row_
                              float* out, int64_t out_seq_stride, int64_t out_head_stride, int64_t N, int64_t B, int64_t S, int64_t H,
                              int64_t Hk, int64_t D, int64_t P, int64_t T, int64_t W, float scale, void* workspace,
                              size_t workspace_bytes, void* stream) {
-    MDX_CHECK(key && table && length && out && (S == 0 || (q && lse)), "null pointer");
+    MDX_CHECK(q && key && table && length && lse && out, "null pointer");
     MDX_CHECK(dtype == MDX_DT_BF16 || dtype == MDX_DT_F16, "bf16 or fp16");
     MDX_CHECK(D == 64 || D == 128 || D == 256, "head_dim must be 64, 128 or 256");
     const int lt = log2_of(T);
     MDX_CHECK(lt >= 0, "page rows: a power of two in 16..1024");
-    MDX_CHECK(B >= 1 && B <= 1024 && S >= 0 && S <= 65535 && Hk >= 1 && Hk <= 1024 && H >= 1 && H % Hk == 0 && H <= 65536 && H / Hk <= 128,
-              "1..1024 sequences, 0..65535 rows, heads (at most 128 per kv head)");
+    MDX_CHECK(B >= 1 && B <= 1024 && S >= 1 && S <= 65535 && Hk >= 1 && Hk <= 1024 && H >= 1 && H % Hk == 0 && H <= 65536 && H / Hk <= 128,
+              "1..1024 sequences, 1..65535 rows, heads (at most 128 per kv head)");
     MDX_CHECK(P >= 1 && P <= (int64_t(1) << 30) && W >= 1 && (W << lt) < (int64_t(1) << 30) && table_stride >= W &&
                   table_stride <= (int64_t(1) << 26),
               "pages, table [sequences, W], under 2^30 tokens a sequence");
