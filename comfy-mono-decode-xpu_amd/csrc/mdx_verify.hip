@@ -674,7 +674,7 @@ __device__ __forceinline__ int64_t drawn(double mine, F sum_at, int runs, double
             at = pick(v, upto, to, passed, sc);
             if (runs_left && at == t) sc.aim = to - (upto - v);
         }
-        if (!runs_left) return at < 0 ? -1 : e0 + at;  // (not reached without one: the run's sum is not zero)
+        if (!runs_left) return at < 0 ? -1 : e0 + at;  // (a run with a sum has a logit with a weight)
         if (at < 0) {
             if (!none()) return -1;
             v = sum_at(t);
@@ -776,8 +776,11 @@ __global__ __launch_bounds__(DT) void verify_answer_kernel(VerifyArgs a, int per
         }
         __syncthreads();
     }
+    // (Of a run whose reference is 2^1020 or more below the row's nothing is left, 2^-111 at most; the exponential, which ends at
+    // 2^-1020, would leave a sum where no logit has a weight.)
     auto sum_of = [&](int i, const Part& p) {
-        double s = p.ref == weight.sp.ref ? p.sum : p.ref == -INFINITY ? 0.0 : p.sum * exp2_steps((double(p.ref) - weight.sp.ref) * c, tab);
+        const double down = (double(p.ref) - weight.sp.ref) * c;
+        double s = p.ref == weight.sp.ref ? p.sum : !(down > LEAST) ? 0.0 : p.sum * exp2_steps(down, tab);
         s = s >= LEAST_RUN ? s * weight.sp.z : 0.0;
 #pragma unroll 1
         for (int k = 0; k < kids; ++k) s = (child[k] + shift) / SUB == i ? less[k] : s;

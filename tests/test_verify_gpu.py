@@ -314,3 +314,22 @@ def test_replay_without_draft_probabilities(C, dev):
         for got, x in ((out, a[i]), (beside, a[2])):
             want = ref.verify_drafts(f64(x[0]), x[2].numpy(), x[3].numpy(), parent=parent.numpy())
             assert [g.cpu().tolist() for g in got] == [w.tolist() for w in want]
+
+
+@pytest.mark.parametrize("B,R,V", [(1, 1, 9000), (3, 3, 9000), (64, 3, 60000), (512, 2, 20000), (1, 2, 600000)])
+def test_runs_that_the_largest_leaves_nothing_of(C, B, R, V):
+    """Runs within the exponentials' range by themselves, ahead of a logit that leaves them less than that range holds: a uniform of
+    0 passes none of them. (Weights of 2^-1154 of the largest at most: none in 64 bits.)"""
+    g = torch.Generator().manual_seed(36)
+    logits = torch.rand(B, R, V, generator=g) * 12 - 6  # (866 octaves at most at a temperature of 0.01)
+    at = 2048 + torch.randint(0, V - 2048, (B, R), generator=g)
+    logits.scatter_(2, at[..., None], 14.0)  # 2020
+    tokens = torch.zeros(B, R, dtype=torch.int64)
+    uniform = torch.rand(B, R + 1, generator=g, dtype=torch.float64)
+    uniform[:, R] = 0.0
+    tokens[:, 1:] = at[:, :R - 1]
+    want = check(C, logits, tokens, uniform, heat=0.01)
+    assert (want[0] == R).all() and want[2].tolist() == at[:, -1].tolist()
+    tokens[:, 1:] = 7  # (refused)
+    want = check(C, logits, tokens, uniform, heat=0.01)
+    assert (want[0] == 1).all() and want[2].tolist() == at[:, 0].tolist()
