@@ -39,6 +39,9 @@ void set_error(const char* fmt, ...);
         }                                                                           \
     } while (0)
 
+// Work-groups of `threads` that one launch can have (its threads have to be under 2^32).
+constexpr int64_t most_groups(int threads) { return ((int64_t(1) << 32) - 1) / threads; }
+
 inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 // ---- scalar conversions (device) ---------------------------------------------------------------

@@ -820,6 +820,7 @@ int64_t slices_of(int64_t V, int each) { return (V + 7 + slice_of(each) - 1) / s
 int rows_each(int64_t B, int64_t rows, int64_t V) { return B * rows * slices_of(V, 8) >= 2048 ? 8 : B * rows * slices_of(V, 4) >= 1024 ? 4 : 1; }
 // (the walk, over 151936: 32 sequences 17.2 us with one, 16.0 with two, 17.4 with four; 64: 24.0 with two, 21.9 with four)
 int walk_each(int64_t B, int64_t V) { return B * slices_of(V, 1) > 4096 ? 4 : B * slices_of(V, 1) > 2048 ? 2 : 1; }
+bool fits(int64_t B, int64_t rows, int64_t V) { return B * rows * slices_of(V, rows_each(B, rows, V)) <= most_groups(NT); }  // (of a walk's pieces there are fewer)
 int64_t runs_of(int64_t V, int each) { return slices_of(V, each) * each * (NT / 64); }  // (a multiple of 4)
 
 }  // namespace
@@ -830,6 +831,7 @@ using namespace mdx;
 extern "C" size_t mdx_verify_drafts_workspace(int64_t B, int64_t R, int64_t V, int32_t drafted) {
     if (B < 1 || B > 1024 || R < 1 || R > MAX_ROWS || V < 1 || V >= (int64_t(1) << 24)) return 0;
     const int64_t rows = drafted ? 2 * R - 1 : R;
+    if (!fits(B, rows, V)) return 0;
     const int each = rows_each(B, rows, V);
     const size_t parts = size_t(B * rows * slices_of(V, each)) * sizeof(Part);
     return parts + (drafted ? size_t(B * runs_of(V, walk_each(B, V))) * 8 + size_t(B) * sizeof(Answer) : size_t(B * R * runs_of(V, each)) * sizeof(Part));
@@ -851,6 +853,7 @@ extern "C" int mdx_verify_drafts(const void* logits, int64_t seq_stride, int64_t
               "strides");
     MDX_CHECK(temperatures || (temperature >= 0.f && temperature < INFINITY), "a temperature of 0 or more, finite");
     const bool drafted = draft && R > 1;
+    MDX_CHECK(fits(B, drafted ? 2 * R - 1 : R, V), "too many rows times logits for one call");
     const size_t need = mdx_verify_drafts_workspace(B, R, V, drafted);
     MDX_CHECK(workspace && aligned(workspace, 16) && workspace_bytes >= need, "workspace: %zu bytes, 16-byte aligned", need);
     VerifyArgs a{};
@@ -869,7 +872,6 @@ extern "C" int mdx_verify_drafts(const void* logits, int64_t seq_stride, int64_t
     a.B = int(B), a.R = int(R), a.V = int(V), a.rows = int(drafted ? 2 * R - 1 : R);
     const int rows = rows_each(B, a.rows, V), walk = walk_each(B, V);
     a.slices = int(slices_of(V, rows)), a.pieces = int(slices_of(V, walk));
-    MDX_CHECK(B * a.rows * a.slices < (int64_t(1) << 30), "too many rows times logits for one call");
     a.part = static_cast<Part*>(workspace);
     if (drafted) {
         a.sums = reinterpret_cast<double*>(a.part + B * a.rows * a.slices);

@@ -706,9 +706,10 @@ int mdx_page_evict(void* kv, void* ksum, int32_t dtype, int64_t L, int64_t Hk, i
  * accepted; if none is, the answer is drawn from p_r without their tokens. A row with no drafted token behind it answers
  * from p_r. Drawn is the lowest index whose cumulative weight passes uniform[b][R] of the whole (the last with a weight where
  * rounding leaves none; -1 where there is no weight); a weight under 2^-100 of the largest may count as none. 64-bit sums.
- * logits, draft: dtype MDX_DT_BF16, _F16 or _F32, rows contiguous, any strides; uniform f64 [B][R + 1] in [0, 1). count int32 [B]: row 0 and the accepted rows; path int32 [B][R]:
- * those rows, -1 behind (mdx_page_commit's); next int64 [B]: the answer. B <= 1024, R <= 64, V < 2^24. The role of
- * mdx_mtp_accept's walk (csrc/mtp_loop.sycl:86-196), by probabilities and for a batch. */
+ * logits, draft: dtype MDX_DT_BF16, _F16 or _F32, rows contiguous, any strides; uniform f64 [B][R + 1] in [0, 1). count int32
+ * [B]: row 0 and the accepted rows; path int32 [B][R]: those rows, -1 behind (mdx_page_commit's); next int64 [B]: the answer.
+ * B <= 1024, R <= 64, V < 2^24, and under 2^24 pieces of 16384 logits in all rows together (the draft's too; a row's last one may
+ * be short). The role of mdx_mtp_accept's walk (csrc/mtp_loop.sycl:86-196), by probabilities and for a batch. */
 size_t mdx_verify_drafts_workspace(int64_t B, int64_t R, int64_t V, int32_t drafted);
 int mdx_verify_drafts(const void* logits, int64_t seq_stride, int64_t row_stride, const void* draft, int64_t draft_seq_stride,
                       int64_t draft_row_stride, int32_t dtype, const int64_t* tokens, const int32_t* parent, const double* uniform,

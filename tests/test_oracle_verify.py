@@ -79,3 +79,18 @@ def test_refusals_before_any_device_work():
         _C.verify_drafts(torch.zeros(1, 2, 8), torch.zeros(1, 2, dtype=torch.int64), torch.zeros(1, 3, dtype=torch.float64))
     with pytest.raises(RuntimeError, match="logits"):
         _C.verify_drafts(None, None, None)
+
+
+def test_more_rows_times_logits_than_a_launch_holds():
+    """Rows of one broadcast buffer: the launch would have 2^32 threads or more. Refused before any device work."""
+    lib = os.path.join(PKG, "mdx", "libmdx.so")
+    if not os.path.exists(lib):
+        pytest.skip("libmdx.so not built")
+    from mdx import _lib
+    L, p = _lib.lib(), 4096  # (never read)
+    most = 255 * 16384  # logits of a row: 255 work-groups of 16384
+    for R, draft, V in ((64, None, most + 16384 - 6), (64, None, (1 << 24) - 1), (33, p, most + 16384), (64, p, most)):
+        assert L.mdx_verify_drafts_workspace(1024, R, V, draft is not None) == 0, (R, V)
+        rc = L.mdx_verify_drafts(p, 0, 0, draft, 0, 0, _lib.DT_BF16, p, None, p, None, 1.0, p, p, p, 1024, R, V, p, 1 << 50, None)
+        assert rc == _lib.MDX_EINVAL and "too many" in L.mdx_last_error().decode(), (R, V)
+    assert L.mdx_verify_drafts_workspace(1024, 64, most - 7, 0) > 0 and L.mdx_verify_drafts_workspace(1024, 32, most - 7, 1) > 0
