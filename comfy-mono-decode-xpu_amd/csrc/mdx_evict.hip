@@ -223,9 +223,9 @@ __device__ void evict_select(const EvictArgs& a, int unit) {
 }
 
 template <int EACH>
-__global__ __launch_bounds__(PLAN_T) void evict_plan_kernel(EvictArgs a) {
-    if (blockIdx.x == 0) evict_plan(a);
-    else evict_select<EACH>(a, int(blockIdx.x) - 1);
+__global__ __launch_bounds__(PLAN_T) void evict_plan_kernel(EvictArgs a, int first) {
+    if (first == 0 && blockIdx.x == 0) evict_plan(a);
+    else evict_select<EACH>(a, first + int(blockIdx.x) - 1);
 }
 
 // ---- the tables and the rows --------------------------------------------------------------------------------------
@@ -274,12 +274,13 @@ __device__ void evict_tables(const EvictArgs& a, int i) {
 }
 
 constexpr int MOVE_BYTES = 16384;  // of a work-group of the move: whole pages of at least that
-__global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
-    if (int(blockIdx.x) < a.M) {
-        evict_tables(a, blockIdx.x);
+__global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a, int first) {
+    const int x = first + int(blockIdx.x) - a.M;
+    if (x < 0) {
+        evict_tables(a, x + a.M);
         return;
     }
-    const int x = int(blockIdx.x) - a.M, c = x / a.units, h = c % a.Hk, part = c / a.Hk % 2, l = c / (2 * a.Hk) % a.L, i = c / (2 * a.Hk * a.L);
+    const int c = x / a.units, h = c % a.Hk, part = c / a.Hk % 2, l = c / (2 * a.Hk) % a.L, i = c / (2 * a.Hk * a.L);
     const int4 p = a.pair[i];
     const int k0 = x % a.units * a.unit << a.lt, k1 = min(p.y, k0 + (a.unit << a.lt));
     if (p.x != 1 || p.w || k0 >= k1) return;  // (uniform)
@@ -332,6 +333,21 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
             mean_key(a, kc, fresh[j], threadIdx.x & 63);
         }
     }
+}
+
+// Selections and moves of a launch: more of them take further launches. (A launch holds under 2^32 threads, and the moves go by what
+// the tables could hold: 1024 pairs of 32 layers of 8 kv heads thinned to 2048 tokens are 2^24 work-groups of 256. A loop in the
+// kernels cost every call registers: the move of 4 sequences of 16100 tokens 116 -> 122 us.)
+constexpr int MOST_GROUPS = 1 << 20;
+static_assert(MOST_GROUPS <= most_groups(PLAN_T), "");
+// f(first work-group, work-groups) of every launch
+template <class F>
+int launches(int groups, F f) {
+    for (int first = 0; first < groups; first += MOST_GROUPS) {
+        f(first, dim3(unsigned(groups - first < MOST_GROUPS ? groups - first : MOST_GROUPS)));
+        MDX_LAUNCHED();
+    }
+    return MDX_OK;
 }
 
 int64_t lists(int64_t M, int64_t L, int64_t Hk, int64_t most) { return (M * L * Hk * most + 3) / 4 * 4; }
@@ -398,14 +414,14 @@ extern "C" int mdx_page_evict(void* kv, void* ksum, int32_t dtype, int64_t L, in
     a.fresh = reinterpret_cast<int32_t*>(a.pair + pairs);
     a.place = a.fresh + given(pairs, W);
     a.drawn = reinterpret_cast<float*>(a.place + lists(pairs, L, Hk, most));
-    const int64_t grid = pairs + pairs * L * 2 * Hk * a.units;
-    MDX_CHECK(grid < (int64_t(1) << 31), "too many pairs times heads times kept tokens for one call");
+    const int64_t moves = pairs * L * 2 * Hk * a.units;  // (of at least 32 of the kept rows each, or all: under 2^28)
+    MDX_CHECK(pairs + moves < (int64_t(1) << 30), "too many pairs times heads times kept tokens for one call");
     hipStream_t st = static_cast<hipStream_t>(stream);
-    // (four tokens a thread where a round of them holds a sequence)
-    if ((W << lt) <= 4 * PLAN_T) hipLaunchKernelGGL((evict_plan_kernel<4>), dim3(unsigned(1 + pairs * L * Hk)), dim3(PLAN_T), 0, st, a);
-    else hipLaunchKernelGGL((evict_plan_kernel<16>), dim3(unsigned(1 + pairs * L * Hk)), dim3(PLAN_T), 0, st, a);
-    MDX_LAUNCHED();
-    hipLaunchKernelGGL(evict_move_kernel, dim3(unsigned(grid)), dim3(256), 0, st, a);
-    MDX_LAUNCHED();
-    return MDX_OK;
+    const bool few = (W << lt) <= 4 * PLAN_T;  // (four tokens a thread where a round of them holds a sequence)
+    const int rc = launches(int(1 + pairs * L * Hk), [&](int first, dim3 groups) {
+        if (few) hipLaunchKernelGGL((evict_plan_kernel<4>), groups, dim3(PLAN_T), 0, st, a, first);
+        else hipLaunchKernelGGL((evict_plan_kernel<16>), groups, dim3(PLAN_T), 0, st, a, first);
+    });
+    if (rc != MDX_OK) return rc;
+    return launches(int(pairs + moves), [&](int first, dim3 groups) { hipLaunchKernelGGL(evict_move_kernel, groups, dim3(256), 0, st, a, first); });
 }

@@ -238,3 +238,57 @@ def test_the_most_pairs(C, dev):
 def test_more_kept_than_a_table_holds(C, dev):
     st = State(17, [100, 128, 0], P=60)
     assert evict(C, dev, st, [0, 1, 2], [1, 1, 0], 5000, 100, 100) == [1, 1, 1]
+
+
+@pytest.mark.parametrize("L,Hk,T,D,W,B,long,keep,sinks,recent", [(129, 8, 16, 64, 2, 1024, 0, 5, 1, 2), (32, 8, 16, 128, 133, 1024, 2100, 2043, 1, 4)])
+def test_more_units_than_a_launch_has_work_groups(C, dev, L, Hk, T, D, W, B, long, keep, sinks, recent):
+    """1024 pairs of many layers and heads: over 2^20 selections; 2^24 moves, as the table's width has it. The sequences become thinned
+    copies of 40 short ones (and of a long one)."""
+    g = torch.Generator().manual_seed(19)
+    src = torch.randint(0, 40, (B,), generator=g)
+    lens = torch.randint(0, min(33, W * T + 1), (B,), generator=g)
+    lens[40:] = 0
+    if long:
+        lens[3] = long
+        src[src == 3] = 4
+        src[7] = src[B - 1] = 3
+    used, most = -(-lens // T), keep + sinks + recent
+    P = int(used.sum()) + int((-(-lens.clamp(max=most) // T))[src].sum())
+    print(f"page_evict {B} pairs of {L} layers of {Hk} heads, {P} pages", flush=True)
+    order, table, at = torch.randperm(P, generator=g), torch.full((B, W), -1, dtype=torch.int32), 0
+    refs = torch.zeros(P, dtype=torch.int32)
+    for b in range(40):
+        e = int(used[b])
+        table[b, :e] = order[at:at + e]
+        refs[order[at:at + e]] = 1
+        at += e
+    kv = torch.empty(L, 2, Hk, P, T, D, dtype=BF, device=dev)
+    for part in kv.view(L, -1):
+        part.normal_()
+    mass = torch.rand(L, 40, Hk, W * T, generator=g).to(dev)
+    whole = torch.zeros(L, B, Hk, W * T, device=dev)
+    whole[:, :40] = mass
+    rows = []  # (what the sources' tokens hold, before the call)
+    for b in range(40):
+        t = torch.arange(int(lens[b]))
+        rows.append(kv[:, :, :, table[b, t // T].long().to(dev), (t % T).to(dev)])
+    table, refs = table.to(dev), refs.to(dev)
+    status, kept = C.page_evict(kv, None, table, lens.to(torch.int32).to(dev), refs, whole, i32(range(B), dev), i32(src.tolist(), dev), keep, sinks, recent)
+    assert (status == 1).all()
+    want = []  # the kept tokens of every source: forced ones ahead of the masses, ties at the lowest
+    for b in range(40):
+        n = int(lens[b])
+        worth = mass[:, b, :, :n].clone()
+        worth[..., :sinks] = worth[..., max(0, n - recent):] = 2.0
+        want.append(worth.sort(dim=-1, descending=True, stable=True).indices[..., :most].sort(-1).values)
+    table = table.cpu()
+    for i in range(B):
+        keys, held = want[int(src[i])], rows[int(src[i])]
+        n = keys.shape[-1]
+        if int(src[i]) == i and n == int(lens[i]):
+            continue  # (it stays)
+        assert torch.equal(kept[i, :, :, :n].long(), keys) and (kept[i, :, :, n:] == -1).all(), i
+        t = torch.arange(n)
+        got = kv[:, :, :, table[i, t // T].long().to(dev), (t % T).to(dev)]
+        assert torch.equal(got, held.gather(3, keys[:, None, :, :, None].expand(L, 2, Hk, n, D))), i
+        assert torch.equal(whole[:, i, :, :n], mass[:, int(src[i])].gather(2, keys)), i
