@@ -42,14 +42,14 @@ struct EvictArgs {
     // workspace
     int4* pair;      // [M]: state (1 served, 0 too few pages, -1 refused), tokens, first fresh page, the sequence stays as it is
     int32_t* fresh;  // the free pages given out
-    int32_t* place;  // [M][L][Hk][most]: row page * T + t of the pool; -1: none
+    int32_t* place;  // [M][L][Hk][most]: row page * T + t of the pool; -1: none (such a pair is refused)
     float* drawn;    // [M][L][Hk][most]
 };
 
 // ---- the plan -----------------------------------------------------------------------------------------------
 __device__ void evict_plan(const EvictArgs& a) {
     __shared__ int tmp[PLAN_T / 64];
-    __shared__ int sdst[MAX_SEQS];
+    __shared__ int sdst[MAX_SEQS], source[MAX_SEQS], pages[MAX_SEQS];
     const int i = threadIdx.x;
     const int d = i < a.M ? a.dst[i] : -1, s = i < a.M ? a.src[i] : -1;
     sdst[i] = d;
@@ -71,7 +71,24 @@ __device__ void evict_plan(const EvictArgs& a) {
         } else {
             need = int(total);
         }
+        source[i] = s;
+        pages[i] = valid && !stays ? (had + a.T - 1) >> a.lt : 0;
+    } else {
+        pages[i] = 0;
     }
+    // Every token that may move has to stand in a page: its new place would be attended, with what another sequence left there. The
+    // pairs' entries by as many threads each.
+    __syncthreads();
+    int each = PLAN_T;
+    while (each * a.M > PLAN_T) each >>= 1;
+    const int mine = i / each;  // (a thread of no pair: its pages are 0)
+    const int32_t* row = a.table + (pages[mine] ? source[mine] : 0) * a.ts;
+    bool hole = false;
+#pragma unroll 4
+    for (int j = i % each; j < pages[mine]; j += each) hole |= uint32_t(row[j]) >= uint32_t(a.P);
+    if (hole) sdst[mine] = -1;  // (a valid pair's is not)
+    __syncthreads();
+    valid = valid && sdst[i] >= 0;
     if (!valid) n = need = 0;
     int want = 0, upto = 0, have = 0;
     if (__syncthreads_or(need)) {
@@ -293,7 +310,6 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a, int first)
     const int64_t chunk = (int64_t(l) * 2 + part) * a.Hk + h;
     unsigned char* base = a.kv + ((chunk * a.P) << a.lt) * a.D * 2 + in;
     constexpr int U = 4;
-    int missing = 0;
     for (int k = k0 + sub; k < k1; k += U * step) {
         u32x4 v[U];
         int from[U], to[U];
@@ -306,7 +322,6 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a, int first)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             to[u] = (to[u] << a.lt) + ((k + u * step) & (a.T - 1));
-            missing |= from[u] < 0;
             if (k + u * step >= k1) from[u] = -1;
         }
 #pragma unroll
@@ -323,13 +338,13 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a, int first)
     float* mass = a.mass + ((int64_t(l) * a.B + a.dst[i]) * a.Hk + h) * a.N;
     for (int k = k0 + int(threadIdx.x); k < k1; k += 256) mass[k] = a.drawn[list + k];
     if (!a.ksum) return;
-    const bool whole = !__syncthreads_or(missing);  // (and the rows above, read by other waves)
+    __syncthreads();  // (the rows above, read by other waves)
     for (int j = (k0 >> a.lt) + int(threadIdx.x >> 6); j < k1 >> a.lt; j += 4) {
         const int64_t kc = int64_t(l) * a.Hk + h;
-        if (in_lds && whole) {
+        if (in_lds) {
             const uint16_t* at = reinterpret_cast<const uint16_t*>(rows) + ((j << a.lt) - k0) * a.D;
             mean_rows(at, a.ksum + (kc * a.P + fresh[j]) * a.D, a.T, a.D, a.half, threadIdx.x & 63);
-        } else {  // (a page larger than that; or rows that stand in no page, whose places stay as they were)
+        } else {  // (a page larger than that)
             mean_key(a, kc, fresh[j], threadIdx.x & 63);
         }
     }

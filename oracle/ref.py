@@ -1164,7 +1164,8 @@ def page_evict(kv, ksum, table, length, refs, mass, dst, src, keep, sinks, recen
         had = min(max(int(length[s]), 0), W * T) if ok else 0
         n, stays = min(had, most), s == d and had <= most
         total = -(-(n + room) // T)
-        if not ok or total > W:
+        holes = not stays and any(not page_in(table[s, j]) for j in range(-(-had // T)))  # tokens in no page have no rows to move
+        if not ok or total > W or holes:
             status.append(-1)
             slots.append([-1] * room)
             continue
@@ -1185,8 +1186,7 @@ def page_evict(kv, ksum, table, length, refs, mass, dst, src, keep, sinks, recen
                 if stays:
                     continue
                 for k, t in enumerate(stay):
-                    if page_in(table[s, t // T]):
-                        kv[l, :, h, row[k // T], k % T] = old_kv[l, :, h, table[s, t // T], t % T]
+                    kv[l, :, h, row[k // T], k % T] = old_kv[l, :, h, table[s, t // T], t % T]
                 mass[l, d, h, :n] = old_mass[l, s, h, stay]
                 for j in range(n // T):
                     ksum[l, h, row[j]] = kv[l, 0, h, row[j]].astype(np.float64).mean(0)

@@ -292,3 +292,29 @@ def test_more_units_than_a_launch_has_work_groups(C, dev, L, Hk, T, D, W, B, lon
         got = kv[:, :, :, table[i, t // T].long().to(dev), (t % T).to(dev)]
         assert torch.equal(got, held.gather(3, keys[:, None, :, :, None].expand(L, 2, Hk, n, D))), i
         assert torch.equal(whole[:, i, :, :n], mass[:, int(src[i])].gather(2, keys)), i
+
+
+@pytest.mark.parametrize("pairs", [1, 3, 4, 300])
+def test_sources_with_a_token_in_no_page_are_refused(C, dev, pairs):
+    """Its place in a fresh page would be attended, with the rows that a sequence before left there. What is behind the source's last
+    token, and a sequence that stays, need no page."""
+    st = State(20, [100, 100, 90, 40] + [20 + i % 13 for i in range(296)], P=1000)
+    st.kv[:, :, :, st.refs == 0] = 7.0  # (the pool's free pages hold something)
+    for bad in (-1, 1000, 2 ** 31 - 1, -2 ** 31):
+        for at, refused in ((0, 1), (6, 1), (7, 0)):  # (the first, the last of 100 tokens, one behind them)
+            st.table[1, at], was = bad, st.table[1, at].clone()
+            src = [1, 0, 2, 1] if pairs < 300 else [(i * 7 + 1) % 300 for i in range(300)]
+            status = evict(C, dev, st, list(range(pairs)), src[:pairs], 50, 2, 8, 3)
+            assert [x == -1 for x in status] == [bool(refused) and s == 1 for s in src[:pairs]]  # (of 300 the last find too few pages)
+            st.table[1, at] = was
+    st.table[3, 1], st.table[2, 0] = -1, -1
+    assert evict(C, dev, st, [3, 2, 0], [3, 2, 0], 50, 2, 8, 3) == [1, -1, 1]  # (40 tokens stay as they are)
+
+
+def test_a_hole_in_a_long_table(C, dev):
+    """The last entry of 3001."""
+    st = State(21, [48010, 0], L=1, Hk=1, P=3010, T=16, W=3002)
+    for at, want in ((3000, -1), (1500, -1), (3001, 1)):
+        st.table[0, at], was = -1, st.table[0, at].clone()
+        assert evict(C, dev, st, [1], [0], 20, 1, 5) == [want]
+        st.table[0, at] = was
