@@ -43,6 +43,11 @@ void set_error(const char* fmt, ...);
 constexpr int64_t most_groups(int threads) { return ((int64_t(1) << 32) - 1) / threads; }
 
 inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+// whether the n bytes at p and the m bytes at q have none in common
+inline bool apart(const void* p, uint64_t n, const void* q, uint64_t m) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+    return a + n <= b || b + m <= a;
+}
 
 // ---- scalar conversions (device) ---------------------------------------------------------------
 __device__ __forceinline__ float bf2f(uint16_t b) { return __uint_as_float(uint32_t(b) << 16); }

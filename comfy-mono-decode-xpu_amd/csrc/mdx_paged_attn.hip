@@ -1427,9 +1427,8 @@ int fill(PagedArgs& a, const void* q, int64_t q_seq_stride, int64_t q_row_stride
     MDX_CHECK(q_seq_stride >= 0 && q_row_stride >= 0 && q_head_stride >= 0 && q_seq_stride < lim && q_row_stride < lim && q_head_stride < lim,
               "query strides");
     // (a row is written while work-groups that have a part of it may still have its query to read)
-    const uintptr_t q0 = reinterpret_cast<uintptr_t>(q), o0 = reinterpret_cast<uintptr_t>(out);
     const uint64_t q_bytes = uint64_t((B - 1) * q_seq_stride + (S - 1) * q_row_stride + (H - 1) * q_head_stride + D) * 2;
-    MDX_CHECK(o0 + uint64_t(B * S * H * D) * 2 <= q0 || q0 + q_bytes <= o0, "out: apart from q");
+    MDX_CHECK(apart(out, uint64_t(B * S * H * D) * 2, q, q_bytes), "out: apart from q");
     a.q = static_cast<const uint16_t*>(q);
     a.qb = q_seq_stride, a.qs = q_row_stride, a.qh = q_head_stride;
     a.key = static_cast<const uint16_t*>(key);
@@ -1522,6 +1521,9 @@ extern "C" int mdx_attn_window(const void* q, int64_t q_seq_stride, int64_t q_ro
     a.whole = whole_units(B, S, H, Hk, most);
     MDX_CHECK(a.whole || (workspace && aligned(workspace, 16) && workspace_bytes >= base_bytes(rows, D, Kind::WIN)),
               "workspace: %zu bytes, 16-byte aligned", base_bytes(rows, D, Kind::WIN));
+    // (written while other rows' outputs and queries are)
+    const uint64_t q_bytes = uint64_t((B - 1) * q_seq_stride + (S - 1) * q_row_stride + (H - 1) * q_head_stride + D) * 2, l_bytes = uint64_t(B * S * H) * 4;
+    MDX_CHECK(apart(lse, l_bytes, out, uint64_t(B * S * H * D) * 2) && apart(lse, l_bytes, q, q_bytes), "lse: apart from out and q");
     a.spb = int(rows_of_unit(S, H / Hk));
     a.units = int(blocks);
     a.first = int(sinks), a.window = int(window);

@@ -1352,8 +1352,8 @@ def attn_blocks(q, key, value, ksum, table, length, blocks, sink=1, local=1, mas
 def attn_window(q, key, value, table, length, window, sinks=0, mask=None, scale=None, out=None, lse=None):
     """attn_paged within a sliding window: of the tokens that a row attends there, in order (the committed ones, then those of
     the rows' own that its mask admits), it attends the first `sinks` and the last `window` (None: all). The other operands
-    are attn_paged's. Returns (out [B, S, H, D], lse float32 [B, S, H]): lse is the log of the row's sum of
-    exp(scale q . k), -inf for a row that admits nothing (attn_mass takes it). No counterpart in the reference."""
+    are attn_paged's. Returns (out [B, S, H, D], lse float32 [B, S, H], apart from q and out): lse is the log of the row's sum
+    of exp(scale q . k), -inf for a row that admits nothing (attn_mass takes it). No counterpart in the reference."""
     return (_bind or _bound()).attn_window(q, key, value, table, length, window, sinks, mask, scale, out, lse)
 
 

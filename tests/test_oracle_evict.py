@@ -80,3 +80,23 @@ def test_refusals_before_any_device_work():
         assert rc == _lib.MDX_EINVAL and msg, k
     assert L.mdx_attn_window_workspace(2, 3, 4, 2, 64, 16, 8, 4, 0) == 0 < L.mdx_attn_window_workspace(2, 3, 4, 2, 64, 16, 4000, 60000, 0)
     assert L.mdx_attn_window_workspace(2, 3, 4, 2, 64, 16, 4000, 300, 4) == 0
+
+
+def test_log_sum_exps_over_the_outputs_or_queries_are_refused():
+    """Rows are written while others' queries are read: 12 rows of 64 elements of 2 bytes, 12 log-sum-exps of 4."""
+    if not os.path.exists(os.path.join(PKG, "mdx", "libmdx.so")):
+        pytest.skip("libmdx.so not built")
+    from mdx import _lib
+    L, q, out = _lib.lib(), 1 << 20, 1 << 21  # (never read: the checks come first)
+
+    def window(lse, qs=256):
+        rc = L.mdx_attn_window(q, 3 * qs, qs, 64, 1 << 24, 1024, 1024, 64, 1 << 25, 1024, 1024, 64, _lib.DT_BF16, 1 << 26, 8, 1 << 26, None, out, lse, 4, 0, 2, 3, 4,
+                               2, 64, 20, 16, 8, 0.1, None, 0, None)
+        return rc, L.mdx_last_error().decode()
+
+    rows, sums = 2 * 3 * 4 * 64 * 2, 2 * 3 * 4 * 4
+    for lse in (out, out + 4, out + rows - 4, out - sums + 4, q, q + rows - 4, q - sums + 4):
+        rc, msg = window(lse)
+        assert rc == _lib.MDX_EINVAL and "apart" in msg, lse
+    rc, msg = window(q + 2 * rows - 4, 512 + 64)  # (rows further apart)
+    assert rc == _lib.MDX_EINVAL and "apart" in msg
