@@ -489,6 +489,34 @@ int launch_any(MassArgs& a, int64_t D, hipStream_t st) {
     return D == 64 ? launch_rows<E, 64>(a, st) : D == 128 ? launch_rows<E, 128>(a, st) : launch_rows<E, 256>(a, st);
 }
 
+// Rows of N sums [B, Hk] and their strides.
+struct Sums {
+    const float* at;
+    int64_t sb, sh;
+};
+// Whether a row of `prior` meets one of `out`, whose rows are apart from one another (views of one buffer may lie in each other's
+// gaps): looked up among them row by row, where the ranges meet at all.
+bool rows_meet(const Sums& prior, const Sums& out, int64_t B, int64_t Hk, int64_t N) {
+    auto bytes = [&](const Sums& x) { return uint64_t((B - 1) * x.sb + (Hk - 1) * x.sh + N) * 4; };
+    if (apart(prior.at, bytes(prior), out.at, bytes(out))) return false;
+    // out's rows stand at i1 s1 + i2 s2, those of one i1 within s1
+    const bool by_head = out.sb < out.sh;
+    const int64_t s1 = by_head ? out.sh : out.sb, s2 = by_head ? out.sb : out.sh, n1 = by_head ? Hk : B, n2 = by_head ? B : Hk;
+    const int64_t from = (int64_t(reinterpret_cast<uintptr_t>(prior.at)) - int64_t(reinterpret_cast<uintptr_t>(out.at))) / 4;
+    // the two rows of stride s that a row at x can meet: those at or ahead of its first place and of its last
+    auto near = [](int64_t x, int64_t s, int64_t n) { return s == 0 || x < 0 ? int64_t(0) : x / s < n ? x / s : n - 1; };
+    for (int64_t b = 0; b < B; ++b)
+        for (int64_t h = 0; h < Hk; ++h) {
+            const int64_t x = from + b * prior.sb + h * prior.sh;
+            for (const int64_t i1 : {near(x, s1, n1), near(x + N - 1, s1, n1)}) {
+                const int64_t y = x - i1 * s1;
+                for (const int64_t i2 : {near(y, s2, n2), near(y + N - 1, s2, n2)})
+                    if (y - i2 * s2 < N && i2 * s2 - y < N) return true;
+            }
+        }
+    return false;
+}
+
 int log2_of(int64_t T) {
     for (int i = 4; i <= 10; ++i)
         if (T == int64_t(1) << i) return i;
@@ -541,7 +569,8 @@ extern "C" int mdx_attn_mass(const void* q, int64_t q_seq_stride, int64_t q_row_
               "sums [sequences, kv heads, places]: apart from one another");
     MDX_CHECK(!prior || (prior_seq_stride >= 0 && prior_head_stride >= 0 && prior_seq_stride < lim && prior_head_stride < lim), "prior strides");
     // (a place is read and written by the same lane)
-    MDX_CHECK(prior != out || ((B == 1 || prior_seq_stride == ob) && (Hk == 1 || prior_head_stride == oh)), "sums in place: prior's strides");
+    const int64_t pb = B == 1 ? 0 : prior_seq_stride, ph = Hk == 1 ? 0 : prior_head_stride;
+    MDX_CHECK(prior != out || (pb == ob && ph == oh), "sums in place: prior's strides");
     MDX_CHECK(window >= 1 && window <= (int64_t(1) << 30) && sinks >= 0 && sinks <= (int64_t(1) << 30), "a window of 1..2^30 tokens, 0..2^30 first ones");
     MDX_CHECK(scale > 0.f && scale < INFINITY, "a positive, finite scale");
     MassArgs a{};
@@ -554,7 +583,7 @@ extern "C" int mdx_attn_mass(const void* q, int64_t q_seq_stride, int64_t q_row_
     a.length = length;
     a.lse = lse;
     a.prior = prior;
-    a.pb = prior_seq_stride, a.ph = prior_head_stride;
+    a.pb = pb, a.ph = ph;
     a.count = count;
     a.path = path;
     a.out = out;
@@ -564,6 +593,11 @@ extern "C" int mdx_attn_mass(const void* q, int64_t q_seq_stride, int64_t q_row_
     a.zs = float(double(scale) * 1.4426950408889634);
     const size_t need = mdx_attn_mass_workspace(B, S, H, Hk, D, T, W, N);
     MDX_CHECK(!need || (workspace && aligned(workspace, 16) && workspace_bytes >= need), "workspace: %zu bytes, 16-byte aligned", need);
+    // (places are written while others, and queries, are read)
+    MDX_CHECK(!prior || prior == out || !rows_meet({prior, pb, ph}, {out, ob, oh}, B, Hk, N), "out: prior itself, or apart from it");
+    const uint64_t out_bytes = uint64_t((B - 1) * ob + (Hk - 1) * oh + N) * 4;
+    const uint64_t q_bytes = uint64_t((B - 1) * q_seq_stride + (S - 1) * q_row_stride + (H - 1) * q_head_stride + D) * 2;
+    MDX_CHECK(apart(out, out_bytes, lse, uint64_t(B * S * H) * 4) && apart(out, out_bytes, q, q_bytes), "out: apart from q and lse");
     a.shares = need ? shares_of(B, S, H, Hk, D, (W << lt) < N ? W << lt : N) : 1;
     a.part = static_cast<float*>(workspace);
     hipStream_t st = static_cast<hipStream_t>(stream);

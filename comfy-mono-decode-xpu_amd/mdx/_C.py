@@ -1364,8 +1364,8 @@ def attn_mass(q, key, table, length, lse, prior=None, count=None, path=None, win
     at place length[b] + k and attends what is not behind it, of that the first `sinks` and the last `window` (None: all). q
     [B, S, H, D] and lse [B, S, H] are attn_window's, count and path verify_drafts' and page_commit's: the call goes behind the
     commit, with the lengths of before, and refused rows give nothing. key [Hk, P, T, D]: a layer's keys. prior, out float32
-    [B, Hk, N] (out may be prior; default: new, zeros elsewhere); places from length[b] + count[b] on stay. No counterpart in
-    the reference."""
+    [B, Hk, N] (out: prior itself, or apart from it, from q and lse; default: new, zeros elsewhere); places from length[b] +
+    count[b] on stay. No counterpart in the reference."""
     return (_bind or _bound()).attn_mass(q, key, table, length, lse, prior, count, path, window, sinks, scale, out)
 
 

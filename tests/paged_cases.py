@@ -66,3 +66,18 @@ def check(got, dt, q, key, value, table, lens, mask, scale, keep=None, rows=slic
     bad = ~(err <= lim)
     assert not bad.any(), (int(bad.sum()), np.argwhere(bad)[:4].tolist(), float(np.nanmax(err / np.maximum(lim, 1e-30))))
     return float(np.nanmax(err / np.maximum(lim, 1e-30)))
+
+
+def views():
+    """Strides of rows of 100 places [sequences, kv heads] apart from one another, of a second view of the buffer, and how many
+    places ahead that begins."""
+    for ob, oh in ((200, 100), (500, 210), (100, 300), (150, 460)):
+        for pb, ph in ((ob, oh), (0, 0), (100, 0), (oh, ob), (1000, 7)):
+            for d in (-2001, -901, -250, -101, -100, -99, -1, 1, 50, 99, 100, 101, 199, 250, 320, 410, 499, 700, 1200):
+                yield ob, oh, pb, ph, d
+
+
+def rows_meet(B, Hk, N, d, pb, ph, ob, oh):
+    """Whether a row of the view at d meets one of the view at 0, place by place."""
+    written = {b * ob + h * oh + t for b in range(B) for h in range(Hk) for t in range(N)}
+    return any(d + b * pb + h * ph + t in written for b in range(B) for h in range(Hk) for t in range(N))

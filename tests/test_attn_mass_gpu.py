@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from oracle import ref
-from paged_cases import cache, f64, tree_masks
+from paged_cases import cache, f64, rows_meet, tree_masks, views
 
 pytestmark = pytest.mark.gpu
 BF, FH = torch.bfloat16, torch.float16
@@ -270,3 +270,23 @@ def test_in_place_needs_the_same_strides(C, dev):
     state = torch.zeros(2, 2, 64, device=dev)
     with pytest.raises(RuntimeError, match="in place"):
         C.attn_mass(q, key, table, n, lse, prior=state, out=state.transpose(0, 1))
+
+
+def test_sums_in_the_gaps_of_others(C, dev):
+    """prior and out as views of one buffer whose ranges meet and whose rows do not: as with buffers of their own."""
+    g = torch.Generator().manual_seed(16)
+    start = torch.rand(9000, generator=g).to(dev)
+    tried = 0
+    for B, Hk in ((3, 2), (1, 2), (3, 1)):
+        q, key, value, table = (t.to(dev) for t in operands(g, BF, 4, Hk, 64, 16, [20, 9, 0][:B], 2))
+        n = torch.tensor([20, 9, 0][:B], dtype=torch.int32, device=dev)
+        _, lse = C.attn_window(q, key, value, table, n, None)
+        for ob, oh, pb, ph, d in views():
+            if rows_meet(B, Hk, 100, d, pb, ph, ob, oh):
+                continue
+            buf = start.clone()
+            prior, out = buf.as_strided((B, Hk, 100), (pb, ph, 1), 4000 + d), buf.as_strided((B, Hk, 100), (ob, oh, 1), 4000)
+            want = C.attn_mass(q, key, table, n, lse, prior=prior.clone(), out=out.clone())
+            assert torch.equal(C.attn_mass(q, key, table, n, lse, prior=prior, out=out), want), (B, Hk, ob, oh, pb, ph, d)
+            tried += 1
+    assert tried > 300

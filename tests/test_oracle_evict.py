@@ -6,6 +6,7 @@ import pytest
 
 from conftest import PKG
 from oracle import ref
+from paged_cases import rows_meet, views
 
 
 def test_kept_tokens_by_hand():
@@ -100,3 +101,28 @@ def test_log_sum_exps_over_the_outputs_or_queries_are_refused():
         assert rc == _lib.MDX_EINVAL and "apart" in msg, lse
     rc, msg = window(q + 2 * rows - 4, 512 + 64)  # (rows further apart)
     assert rc == _lib.MDX_EINVAL and "apart" in msg
+
+
+def test_sums_over_what_is_read_are_refused():
+    """prior and out of [3, 2, 100] places in one buffer: views that meet without being one; out over q or lse."""
+    if not os.path.exists(os.path.join(PKG, "mdx", "libmdx.so")):
+        pytest.skip("libmdx.so not built")
+    from mdx import _lib
+    L, q, lse, base = _lib.lib(), 1 << 20, 1 << 21, 1 << 28  # (never read: the checks come first)
+
+    def mass(prior, pb, ph, out, ob, oh, B=3, Hk=2, N=100):
+        rc = L.mdx_attn_mass(q, 768, 256, 64, 1 << 24, 1024, 1024, 64, _lib.DT_BF16, 1 << 26, 8, 1 << 26, lse, prior, pb, ph, None, None, 4, 0, out, ob, oh, N, B,
+                             3, 4, Hk, 64, 20, 16, 8, 0.1, None, 0, None)
+        return rc, L.mdx_last_error().decode()
+
+    tried = 0
+    for B, Hk in ((3, 2), (1, 2), (3, 1)):
+        for ob, oh, pb, ph, d in views():
+            if rows_meet(B, Hk, 100, d, pb, ph, ob, oh):
+                rc, msg = mass(base + 4 * d, pb, ph, base, ob, oh, B, Hk)
+                assert rc == _lib.MDX_EINVAL and "apart" in msg, (B, Hk, ob, oh, pb, ph, d)
+                tried += 1
+    assert tried > 300
+    for out in (lse, lse + 140, q, q + 4, lse - 2396):
+        rc, msg = mass(None, 0, 0, out, 200, 100)
+        assert rc == _lib.MDX_EINVAL and "apart" in msg, out
