@@ -444,7 +444,7 @@ PyObject* attn_mass(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
                               window, sinks, out.data_ptr<float>(), out.stride(0), out.stride(1), N, B, 1, H, Hk, D, P, T, W, scale, nullptr, 0, st);
             });
         } else if (B > 0) {
-            const size_t n = g.mass_workspace(B, S, H, Hk, D, T, W, N);
+            const size_t n = path ? 0 : g.mass_workspace(B, S, H, Hk, D, T, W, N);
             at::Tensor ws;
             if (n) ws = scratch(n, d);
             call("mdx_attn_mass", d, [&](void* st) {

@@ -591,7 +591,7 @@ extern "C" int mdx_attn_mass(const void* q, int64_t q_seq_stride, int64_t q_row_
     a.B = int(B), a.S = int(S), a.H = int(H), a.Hk = int(Hk), a.G = int(H / Hk), a.W = int(W), a.P = int(P), a.lt = lt, a.N = int(N);
     a.window = int(window), a.sinks = int(sinks);
     a.zs = float(double(scale) * 1.4426950408889634);
-    const size_t need = mdx_attn_mass_workspace(B, S, H, Hk, D, T, W, N);
+    const size_t need = path ? 0 : mdx_attn_mass_workspace(B, S, H, Hk, D, T, W, N);  // (rows of a path are not shared out)
     MDX_CHECK(!need || (workspace && aligned(workspace, 16) && workspace_bytes >= need), "workspace: %zu bytes, 16-byte aligned", need);
     // (places are written while others, and queries, are read)
     MDX_CHECK(!prior || prior == out || !rows_meet({prior, pb, ph}, {out, ob, oh}, B, Hk, N), "out: prior itself, or apart from it");

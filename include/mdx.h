@@ -669,7 +669,7 @@ int mdx_attn_window(const void* q, int64_t q_seq_stride, int64_t q_row_stride, i
  * (mdx_attn_window's). lse f32 [B, S, H] contiguous; a row whose lse is -inf or whose r is none gives nothing, a token in no
  * page draws nothing. prior, out f32 [B, Hk, N] (strides in elements; rows contiguous); out is prior itself, with its strides,
  * or no row of it meets one of prior's, and it is apart from q and lse. fp32 sums, the same bits every time. Other operands as
- * mdx_attn_paged; a workspace of 0 bytes may be NULL. No counterpart in the reference. */
+ * mdx_attn_paged; a workspace of 0 bytes may be NULL, with a path too (none is used). No counterpart in the reference. */
 size_t mdx_attn_mass_workspace(int64_t B, int64_t S, int64_t H, int64_t Hk, int64_t D, int64_t T, int64_t W, int64_t N);
 int mdx_attn_mass(const void* q, int64_t q_seq_stride, int64_t q_row_stride, int64_t q_head_stride, const void* key,
                   int64_t k_head_stride, int64_t k_page_stride, int64_t k_row_stride, int32_t dtype, const int32_t* table,

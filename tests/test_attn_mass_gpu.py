@@ -290,3 +290,24 @@ def test_sums_in_the_gaps_of_others(C, dev):
             assert torch.equal(C.attn_mass(q, key, table, n, lse, prior=prior, out=out), want), (B, Hk, ob, oh, pb, ph, d)
             tried += 1
     assert tried > 300
+
+
+def test_paths_of_many_rows_need_no_workspace(C, dev):
+    """Only rows without a path are shared out to several work-groups, which leave their sums in the workspace."""
+    from mdx import _lib
+    g = torch.Generator().manual_seed(17)
+    lens, S, H, Hk, D, T = [300, 40], 200, 8, 2, 64, 16  # (seven stages of rows: without a path two work-groups a run)
+    q, key, value, table = (t.to(dev) for t in operands(g, BF, H, Hk, D, T, lens, S))
+    n = torch.tensor(lens, dtype=torch.int32, device=dev)
+    path = torch.arange(S, dtype=torch.int32, device=dev).repeat(2, 1)
+    count = torch.tensor([17, 133], dtype=torch.int32, device=dev)
+    _, lse = C.attn_window(q, key, value, table, n, None)
+    want = C.attn_mass(q, key, table, n, lse, count=count, path=path)
+    out, (P, W, N) = torch.zeros_like(want), (key.shape[1], table.shape[1], want.shape[2])
+    L = _lib.lib()
+    assert L.mdx_attn_mass_workspace(2, S, H, Hk, D, T, W, N) > 0
+    p = lambda t: t.data_ptr()  # noqa: E731
+    rc = L.mdx_attn_mass(p(q), *q.stride()[:3], p(key), *key.stride()[:3], _lib.DT_BF16, p(table), W, p(n), p(lse), None, 0, 0, p(count), p(path), 1 << 30, 0, p(out),
+                         *out.stride()[:2], N, 2, S, H, Hk, D, P, T, W, D ** -0.5, None, 0, torch.cuda.current_stream().cuda_stream)
+    assert rc == _lib.MDX_OK, L.mdx_last_error()
+    assert torch.equal(out, want)
