@@ -311,3 +311,42 @@ def test_paths_of_many_rows_need_no_workspace(C, dev):
                          *out.stride()[:2], N, 2, S, H, Hk, D, P, T, W, D ** -0.5, None, 0, torch.cuda.current_stream().cuda_stream)
     assert rc == _lib.MDX_OK, L.mdx_last_error()
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("H,Hk,D,S,lens", [(32, 8, 128, 300, [700]), (16, 4, 256, 200, [300, 0, 90]), (16, 8, 64, 1000, [50]), (128, 1, 128, 70, [600]), (9, 3, 128, 411, [1000, 3])])
+@pytest.mark.parametrize("width", [1, 700])
+def test_every_count_against_the_oracle(C, dev, H, Hk, D, S, lens, width):
+    """All rows, half of them, one, none; each sequence with fewer than the one ahead."""
+    g = torch.Generator().manual_seed(S + 1)
+    q, key, value, table = operands(g, BF, H, Hk, D, 16, lens, S, width)
+    n = torch.tensor(lens, dtype=torch.int32)
+    _, lse = C.attn_window(*(t.to(dev) for t in (q, key, value, table, n)), 400, 20)
+    N = table.shape[1] * 16
+    prior, out = torch.rand(len(lens), Hk, N, generator=g), torch.full((len(lens), Hk, N), 5.0)
+    up = lambda t: t.to(dev)  # noqa: E731
+    for c in (S, S // 2 + 3, 1, 0):
+        count = torch.tensor([max(0, c - 5 * i) for i in range(len(lens))], dtype=torch.int32)
+        got = C.attn_mass(*map(up, (q, key, table, n, lse)), prior=up(prior), count=up(count), window=400, sinks=20, out=up(out))
+        check(got, out, q, key, table, lens, lse, prior, count, None, 400, 20, D ** -0.5)
+
+
+@pytest.mark.parametrize("D,path,dt", [(128, False, BF), (256, False, FH), (64, False, BF), (128, True, FH), (256, True, BF)])
+def test_many_rows_over_wide_tables(C, dev, D, path, dt):
+    """More runs of tokens than the grid holds at once, at 68 query rows per kv head: 4096 pairs leave 16 runs each, and two of the
+    sequences have more."""
+    B, S, H, Hk, T = 1024, 17, 16, 4, 16
+    g = torch.Generator().manual_seed(18)
+    lens = [i % 7 for i in range(B)]
+    lens[5], lens[700] = 4600, 4300  # (runs of 256 tokens, 128 at head_dim 256, 64 and 32 with a path)
+    q, key, value, table = operands(g, dt, H, Hk, D, T, lens, S)
+    n = torch.tensor(lens, dtype=torch.int32)
+    _, lse = C.attn_window(*(t.to(dev) for t in (q, key, value, table, n)), None)
+    count = torch.zeros(B, dtype=torch.int32)
+    for b in (0, 5, 6, 300, 700, 701, 1023):
+        count[b] = S - b % 2
+    rows = torch.stack([torch.randperm(S, generator=g) for _ in range(B)]).to(torch.int32) if path else None
+    prior = torch.rand(B, Hk, table.shape[1] * T, generator=g)
+    out = torch.full_like(prior, 7.0)
+    up = lambda t: None if t is None else t.to(dev)  # noqa: E731
+    got = C.attn_mass(*map(up, (q, key, table, n, lse)), prior=up(prior), count=up(count), path=up(rows), out=up(out))
+    check(got, out, q, key, table, lens, lse, prior, count, rows, 1 << 30, 0, D ** -0.5)
