@@ -8,7 +8,8 @@
 // The draw: the lowest index whose cumulative weight passes u_R of the whole.
 //
 // All of it in 64 bits: a drawn token is a whole number that changes where u falls between two sums, and at a vocabulary of 150
-// thousand 32-bit sums (1e-7 of the whole) would move one draw in thirty across a border; 64-bit ones (1e-13) one in 1e8.
+// thousand 32-bit sums (1e-7 of the whole) would move one draw in thirty across a border. Here a weight is good to some 2e-15 and
+// 3e-16 |x / T|, a border to half of that: at most one draw in 1e9.
 //
 // verify_rows_kernel: a work-group per slice of a row (16384 logits, fewer where there are few) sums their exponentials. Without q
 // it leaves the sums of every run of 512 logits too, and verify_answer_kernel, a work-group per sequence, joins the rows' sums,
@@ -20,9 +21,10 @@
 // What bounds it: many rows the exponentials, 14 vector instructions each, eight of them float64 (7 rows of 32 sequences and their
 // drafts over 151936: 37 us for 126 MB, 25 at the rate of a large copy; with 20 instructions 51), then the walk and the draw, 16
 // and 5 us, chains of dependent loads; one short chain those alone (14 us a call). 8 rows of 16 trees: 16 us and 11.
-// Exponentials: 2^(a / 128) = table[k % 128] 2^(k / 128) poly(a - k), k = rint(a): a table of 1 KiB in LDS, a polynomial of degree 3
-// through the Chebyshev points of [-1/2, 1/2] (2.8e-13 relative); x / T as it stands, without a maximum, as long as none is past
-// 2^900 (then the row is read again less its largest).
+// Exponentials: 2^(a / 512) = table[k % 512] 2^(k / 512) poly(a - k), k = rint(a): a table of 4 KiB in LDS, a polynomial of degree 3
+// through the Chebyshev points of [-1/2, 1/2] (1.1e-15 relative; a table of 128, 2.8e-13, takes the rows of 32 sequences 35 us for 37,
+// one of 1024, 1.1e-16, 37.6); x / T as it stands, without a maximum, as long as none is past 2^900 (then the row is read again
+// less its largest).
 //
 // Reference: the walk's role is csrc/mtp_loop.sycl:86-196's accept (which compares with one sampled token per row).
 #include "mdx_common.hpp"
@@ -74,53 +76,45 @@ struct VerifyArgs {
 
 // ---- exponentials -----------------------------------------------------------------------------------------
 constexpr double MAGIC = 6755399441055744.0;  // 1.5 2^52: the low word of MAGIC + x is rint(x)
-constexpr int STEPS = 128;                      // of an octave
+constexpr int STEPS = 512;                    // of an octave
 constexpr float FAR = 900.f * STEPS;          // references past which 2^(a / STEPS) is taken less the largest a
 constexpr double LEAST = -1020.0 * STEPS;     // a weight that counts as none
 
-__device__ const double POWERS[STEPS] = {  // 2^(j / STEPS)
-    0x1.0000000000000p+0, 0x1.0163da9fb3335p+0, 0x1.02c9a3e778061p+0, 0x1.04315e86e7f85p+0, 0x1.059b0d3158574p+0,
-    0x1.0706b29ddf6dep+0, 0x1.0874518759bc8p+0, 0x1.09e3ecac6f383p+0, 0x1.0b5586cf9890fp+0, 0x1.0cc922b7247f7p+0,
-    0x1.0e3ec32d3d1a2p+0, 0x1.0fb66affed31bp+0, 0x1.11301d0125b51p+0, 0x1.12abdc06c31ccp+0, 0x1.1429aaea92de0p+0,
-    0x1.15a98c8a58e51p+0, 0x1.172b83c7d517bp+0, 0x1.18af9388c8deap+0, 0x1.1a35beb6fcb75p+0, 0x1.1bbe084045cd4p+0,
-    0x1.1d4873168b9aap+0, 0x1.1ed5022fcd91dp+0, 0x1.2063b88628cd6p+0, 0x1.21f49917ddc96p+0, 0x1.2387a6e756238p+0,
-    0x1.251ce4fb2a63fp+0, 0x1.26b4565e27cddp+0, 0x1.284dfe1f56381p+0, 0x1.29e9df51fdee1p+0, 0x1.2b87fd0dad990p+0,
-    0x1.2d285a6e4030bp+0, 0x1.2ecafa93e2f56p+0, 0x1.306fe0a31b715p+0, 0x1.32170fc4cd831p+0, 0x1.33c08b26416ffp+0,
-    0x1.356c55f929ff1p+0, 0x1.371a7373aa9cbp+0, 0x1.38cae6d05d866p+0, 0x1.3a7db34e59ff7p+0, 0x1.3c32dc313a8e5p+0,
-    0x1.3dea64c123422p+0, 0x1.3fa4504ac801cp+0, 0x1.4160a21f72e2ap+0, 0x1.431f5d950a897p+0, 0x1.44e086061892dp+0,
-    0x1.46a41ed1d0057p+0, 0x1.486a2b5c13cd0p+0, 0x1.4a32af0d7d3dep+0, 0x1.4bfdad5362a27p+0, 0x1.4dcb299fddd0dp+0,
-    0x1.4f9b2769d2ca7p+0, 0x1.516daa2cf6642p+0, 0x1.5342b569d4f82p+0, 0x1.551a4ca5d920fp+0, 0x1.56f4736b527dap+0,
-    0x1.58d12d497c7fdp+0, 0x1.5ab07dd485429p+0, 0x1.5c9268a5946b7p+0, 0x1.5e76f15ad2148p+0, 0x1.605e1b976dc09p+0,
-    0x1.6247eb03a5585p+0, 0x1.6434634ccc320p+0, 0x1.6623882552225p+0, 0x1.68155d44ca973p+0, 0x1.6a09e667f3bcdp+0,
-    0x1.6c012750bdabfp+0, 0x1.6dfb23c651a2fp+0, 0x1.6ff7df9519484p+0, 0x1.71f75e8ec5f74p+0, 0x1.73f9a48a58174p+0,
-    0x1.75feb564267c9p+0, 0x1.780694fde5d3fp+0, 0x1.7a11473eb0187p+0, 0x1.7c1ed0130c132p+0, 0x1.7e2f336cf4e62p+0,
-    0x1.80427543e1a12p+0, 0x1.82589994cce13p+0, 0x1.8471a4623c7adp+0, 0x1.868d99b4492edp+0, 0x1.88ac7d98a6699p+0,
-    0x1.8ace5422aa0dbp+0, 0x1.8cf3216b5448cp+0, 0x1.8f1ae99157736p+0, 0x1.9145b0b91ffc6p+0, 0x1.93737b0cdc5e5p+0,
-    0x1.95a44cbc8520fp+0, 0x1.97d829fde4e50p+0, 0x1.9a0f170ca07bap+0, 0x1.9c49182a3f090p+0, 0x1.9e86319e32323p+0,
-    0x1.a0c667b5de565p+0, 0x1.a309bec4a2d33p+0, 0x1.a5503b23e255dp+0, 0x1.a799e1330b358p+0, 0x1.a9e6b5579fdbfp+0,
-    0x1.ac36bbfd3f37ap+0, 0x1.ae89f995ad3adp+0, 0x1.b0e07298db666p+0, 0x1.b33a2b84f15fbp+0, 0x1.b59728de5593ap+0,
-    0x1.b7f76f2fb5e47p+0, 0x1.ba5b030a1064ap+0, 0x1.bcc1e904bc1d2p+0, 0x1.bf2c25bd71e09p+0, 0x1.c199bdd85529cp+0,
-    0x1.c40ab5fffd07ap+0, 0x1.c67f12e57d14bp+0, 0x1.c8f6d9406e7b5p+0, 0x1.cb720dcef9069p+0, 0x1.cdf0b555dc3fap+0,
-    0x1.d072d4a07897cp+0, 0x1.d2f87080d89f2p+0, 0x1.d5818dcfba487p+0, 0x1.d80e316c98398p+0, 0x1.da9e603db3285p+0,
-    0x1.dd321f301b460p+0, 0x1.dfc97337b9b5fp+0, 0x1.e264614f5a129p+0, 0x1.e502ee78b3ff6p+0, 0x1.e7a51fbc74c83p+0,
-    0x1.ea4afa2a490dap+0, 0x1.ecf482d8e67f1p+0, 0x1.efa1bee615a27p+0, 0x1.f252b376bba97p+0, 0x1.f50765b6e4540p+0,
-    0x1.f7bfdad9cbe14p+0, 0x1.fa7c1819e90d8p+0, 0x1.fd3c22b8f71f1p+0};
-// 2^(j / STEPS), the exponent less j << 13 in the high word: k << 13 added gives 2^(k / STEPS) for k % STEPS = j
+constexpr int FINE = 32;
+__device__ const double COARSE[STEPS / FINE] = {  // 2^(j FINE / STEPS)
+    0x1.0000000000000p+0, 0x1.0b5586cf9890fp+0, 0x1.172b83c7d517bp+0, 0x1.2387a6e756238p+0, 0x1.306fe0a31b715p+0,
+    0x1.3dea64c123422p+0, 0x1.4bfdad5362a27p+0, 0x1.5ab07dd485429p+0, 0x1.6a09e667f3bcdp+0, 0x1.7a11473eb0187p+0,
+    0x1.8ace5422aa0dbp+0, 0x1.9c49182a3f090p+0, 0x1.ae89f995ad3adp+0, 0x1.c199bdd85529cp+0, 0x1.d5818dcfba487p+0,
+    0x1.ea4afa2a490dap+0};
+__device__ const double POWERS[FINE] = {  // 2^(j / STEPS)
+    0x1.0000000000000p+0, 0x1.0058c86da1c0ap+0, 0x1.00b1afa5abcbfp+0, 0x1.010ab5b2cbd11p+0, 0x1.0163da9fb3335p+0,
+    0x1.01bd1e77170b4p+0, 0x1.02168143b0281p+0, 0x1.027003103b10ep+0, 0x1.02c9a3e778061p+0, 0x1.032363d42b027p+0,
+    0x1.037d42e11bbccp+0, 0x1.03d7411915a8ap+0, 0x1.04315e86e7f85p+0, 0x1.048b9b35659d8p+0, 0x1.04e5f72f654b1p+0,
+    0x1.0540727fc1762p+0, 0x1.059b0d3158574p+0, 0x1.05f5c74f0bec2p+0, 0x1.0650a0e3c1f89p+0, 0x1.06ab99fa6407cp+0,
+    0x1.0706b29ddf6dep+0, 0x1.0761ead925493p+0, 0x1.07bd42b72a836p+0, 0x1.0818ba42e7d30p+0, 0x1.0874518759bc8p+0,
+    0x1.08d0088f8093fp+0, 0x1.092bdf66607e0p+0, 0x1.0987d61701716p+0, 0x1.09e3ecac6f383p+0, 0x1.0a402331b9715p+0,
+    0x1.0a9c79b1f3919p+0, 0x1.0af8f03834e52p+0};
+// 2^(j / STEPS), the exponent less j << SHIFT in the high word: k << SHIFT added gives 2^(k / STEPS) for k % STEPS = j
+constexpr int SHIFT = 20 - 9;
+static_assert(STEPS << SHIFT == 1 << 20, "");
+template <int THREADS>
 __device__ __forceinline__ void fill_table(double* tab) {  // (the caller's barrier follows)
-    const int j = threadIdx.x;
-    if (j < STEPS) {
-        const double v = POWERS[j];
-        tab[j] = __hiloint2double(__double2hiint(v) - (j << 13), __double2loint(v));
+#pragma unroll
+    for (int i = 0; i < STEPS; i += THREADS) {
+        const int j = i + int(threadIdx.x);
+        if (STEPS % THREADS != 0 && j >= STEPS) break;
+        const double v = COARSE[j / FINE] * POWERS[j % FINE];
+        tab[j] = __hiloint2double(__double2hiint(v) - (j << SHIFT), __double2loint(v));
     }
 }
 __device__ __forceinline__ double poly(double f) {
-    double p = __builtin_fma(f, 0x1.c6b0985c8a1bcp-26, 0x1.ebfbf3aad80f5p-17);
-    p = __builtin_fma(p, f, 0x1.62e42fefa3892p-8);
-    return __builtin_fma(p, f, 0x1.ffffffffff627p-1);
+    double p = __builtin_fma(f, 0x1.c6b08e52035e3p-32, 0x1.ebfbe133587d2p-21);
+    p = __builtin_fma(p, f, 0x1.62e42fefa39efp-10);
+    return __builtin_fma(p, f, 0x1.ffffffffffff6p-1);
 }
 __device__ __forceinline__ double power(int k, const double* tab) {
     const double v = tab[k & (STEPS - 1)];
-    return __hiloint2double(__double2hiint(v) + (k << 13), __double2loint(v));
+    return __hiloint2double(__double2hiint(v) + (k << SHIFT), __double2loint(v));
 }
 // 2^(a / STEPS); below 2^-1020 (NaN too) that
 __device__ __forceinline__ double exp2_steps(double a, const double* tab) {
@@ -277,7 +271,7 @@ __global__ __launch_bounds__(NT) void verify_rows_kernel(VerifyArgs a) {
 #pragma unroll
         for (int i = 0; i < EACH; ++i) x[i] = piece_at<E>(row, a.V, at0<EACH>(slice, i, shift), true);
     }
-    fill_table(tab);
+    fill_table<NT>(tab);
     const double c = rate_of(a, b);
     __syncthreads();  // (the table)
     // the wave's run i
@@ -444,7 +438,7 @@ __device__ __forceinline__ void walk(const VerifyArgs& a, int b, double c, doubl
             own_u = a.uniform[int64_t(b) * (a.R + 1) + parent];
         }
     }
-    fill_table(tab);
+    fill_table<THREADS>(tab);
     __syncthreads();
     // 16 lanes a row: its reference and sum out of the slices', four of them in flight
     for (int r = t >> 4; r < a.rows; r += THREADS / 16) {
@@ -698,7 +692,7 @@ __global__ __launch_bounds__(DT) void verify_draw_kernel(VerifyArgs a, int runs)
     const double mine = sum_at(t);
     const Answer w = a.answer[b];
     const double u = a.uniform[int64_t(b) * (a.R + 1) + a.R];
-    fill_table(tab);
+    fill_table<DT>(tab);
     Weight<E> weight(a, b, w, c);
     const int shift = shift_of<E>(weight.p);
     const int64_t x = drawn(mine, sum_at, runs, u, shift, [&](int e) { return weight.at(e, tab); }, [&]() {

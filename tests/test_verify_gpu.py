@@ -1,5 +1,5 @@
 """verify_drafts against its oracle in float64: every output is a whole number and has to be equal. (A draw or an acceptance could
-only differ where a uniform lies within about 1e-13 of a border, relative to the whole: with the fixed inputs here none does.)"""
+only differ where a uniform lies within some 1e-14 of a border, relative to the whole: with the fixed inputs here none does.)"""
 import numpy as np
 import pytest
 import torch
@@ -333,3 +333,43 @@ def test_runs_that_the_largest_leaves_nothing_of(C, B, R, V):
     tokens[:, 1:] = 7  # (refused)
     want = check(C, logits, tokens, uniform, heat=0.01)
     assert (want[0] == 1).all() and want[2].tolist() == at[:, 0].tolist()
+
+
+def test_uniforms_beside_the_borders(C, dev):
+    """Uniforms 1e-14 to either side of a border of the cumulative probabilities (80-bit oracle), logits within 4 of 0. A weight's
+    relative error: the exponential's polynomial 1.2e-15 and table 3.4e-16, the argument's two roundings (4 2^-53 each, and the rate's
+    4 2^-52), its own 2^-53: under 4e-15 in all; a border moves by at most half of that and some roundings of 2^-53: under 3e-15."""
+    g = torch.Generator().manual_seed(37)
+    B, V = 1024, 5
+    logits = torch.rand(B, 1, V, generator=g) * 8 - 4
+    w = np.exp(logits[:, 0].double().numpy().astype(np.longdouble))
+    p = w / w.sum(1, keepdims=True)
+    upto = np.cumsum(p, 1)
+    at = np.arange(B) % (V - 1)
+    border = upto[np.arange(B), at]
+    none = torch.full((B, 2), -1, dtype=torch.int64)
+    for side, want in ((-1, at), (1, at + 1)):
+        uniform = torch.zeros(B, 3, dtype=torch.float64)
+        uniform[:, 1] = uniform[:, 2] = torch.from_numpy((border + side * np.longdouble(1e-14)).astype(np.float64))
+        one = C.verify_drafts(logits.to(dev), none[:, :1].to(dev), uniform[:, :2].contiguous().to(dev))
+        assert one[2].tolist() == want.tolist()
+        two = logits.expand(B, 2, V).to(dev)  # (with draft probabilities: no token behind row 0)
+        assert C.verify_drafts(two, none.to(dev), uniform.to(dev), draft=two[:, :1])[2].tolist() == want.tolist()
+        # children of one row split [0, 1) at the same borders
+        tokens = torch.arange(-1, V).repeat(B, 1)
+        uniform = torch.zeros(B, V + 2, dtype=torch.float64)
+        uniform[:, 0] = torch.from_numpy((border + side * np.longdouble(1e-14)).astype(np.float64))
+        got = C.verify_drafts(logits.expand(B, V + 1, V).to(dev), tokens.to(dev), uniform.to(dev), parent=torch.zeros(B, V + 1, dtype=torch.int32, device=dev))
+        assert got[1][:, 1].tolist() == (want + 1).tolist()
+    # acceptance: u q(x) against p(x)
+    other = torch.rand(B, 1, V, generator=g) * 8 - 4
+    w = np.exp(other[:, 0].double().numpy().astype(np.longdouble))
+    q = w / w.sum(1, keepdims=True)
+    x = (q - p).argmax(1)
+    ratio = p[np.arange(B), x] / q[np.arange(B), x]
+    tokens = torch.stack([torch.zeros(B, dtype=torch.int64), torch.from_numpy(x)], 1)
+    for side, want in ((-1, 2), (1, 1)):
+        uniform = torch.full((B, 3), 0.5, dtype=torch.float64)
+        uniform[:, 0] = torch.from_numpy((ratio * (1 + side * np.longdouble(2e-14))).astype(np.float64))
+        got = C.verify_drafts(logits.expand(B, 2, V).to(dev), tokens.to(dev), uniform.to(dev), draft=other.to(dev))
+        assert got[0].tolist() == [want] * B
