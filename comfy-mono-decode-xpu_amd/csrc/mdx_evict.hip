@@ -66,7 +66,8 @@ __device__ void evict_plan(const EvictArgs& a) {
         const int64_t total = (int64_t(n) + a.room + a.T - 1) >> a.lt;
         if (total > a.W) {
             valid = false;
-        } else if (stays) {  // only the pages of its room
+        } else if (stays) {  // only the pages of its room (and none for tokens that it has)
+            valid = (n & (a.T - 1)) == 0 || uint32_t(a.table[d * a.ts + (n >> a.lt)]) < uint32_t(a.P);
             for (int j = n >> a.lt; j < int(total); ++j) need += uint32_t(a.table[d * a.ts + j]) >= uint32_t(a.P);
         } else {
             need = int(total);

@@ -1377,8 +1377,8 @@ def page_evict(kv, ksum, table, length, refs, mass, dst, src, keep, sinks=0, rec
     rotation of the positions they had. The tokens go to fresh pages, the lowest free ones in the pairs' order, with pages
     for `room` more tokens; the pages that dst had go back and are free for the next call; all pairs read the state before
     the call. The mean keys of full pages (ksum, or None) and the rows of mass follow. slots as page_fork's.
-    Returns (status int32 [pairs] as page_fork's; -1 also for src[i] < 0, and for a source with a token in no page unless it
-    stays as it is, kept int32 [pairs, layers, kv_heads, sinks + recent + keep]: the numbers the tokens had in src, -1 behind,
+    Returns (status int32 [pairs] as page_fork's; -1 also for src[i] < 0, and for a source with a token in no page (of a
+    sequence that stays: in the page that its length ends in), kept int32 [pairs, layers, kv_heads, sinks + recent + keep]: the numbers the tokens had in src, -1 behind,
     all -1 where the pair is not done). No counterpart in the reference."""
     return (_bind or _bound()).page_evict(kv, ksum, table, length, refs, mass, dst, src, keep, sinks, recent, room, slots)
 

@@ -686,9 +686,9 @@ int mdx_attn_mass(const void* q, int64_t q_seq_stride, int64_t q_row_stride, int
  * tokens); the pages that dst[i] had are given back and free from the next call on. All pairs read the state before the
  * call. mass[l][dst[i]][g] and the mean keys of full pages (ksum, may be NULL) follow; length[dst[i]] is the number kept.
  * kept int32 [pairs][L][Hk][sinks + recent + keep]: their numbers t in src[i], -1 behind. slots and status as mdx_page_fork
- * (status -1 also for src[i] < 0, and where one of src[i]'s tokens stands in no page, unless the sequence stays as it is; kept is
- * then -1). P T < 2^31, pairs L Hk <= 2^24, D in {64, 128, 256}; dtype MDX_DT_BF16 or MDX_DT_F16. No counterpart in the
- * reference. */
+ * (status -1 also for src[i] < 0, and where one of src[i]'s tokens stands in no page: of a sequence that stays, in the page that
+ * its length ends in; kept is then -1). P T < 2^31, pairs L Hk <= 2^24, D in {64, 128, 256}; dtype MDX_DT_BF16 or MDX_DT_F16.
+ * No counterpart in the reference. */
 size_t mdx_page_evict_workspace(int64_t pairs, int64_t W, int64_t L, int64_t Hk, int64_t most);
 int mdx_page_evict(void* kv, void* ksum, int32_t dtype, int64_t L, int64_t Hk, int64_t P, int64_t T, int64_t D, int32_t* table,
                    int64_t table_stride, int64_t B, int64_t W, int32_t* length, int32_t* refs, float* mass, int64_t N,

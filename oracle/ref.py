@@ -1164,7 +1164,8 @@ def page_evict(kv, ksum, table, length, refs, mass, dst, src, keep, sinks, recen
         had = min(max(int(length[s]), 0), W * T) if ok else 0
         n, stays = min(had, most), s == d and had <= most
         total = -(-(n + room) // T)
-        holes = not stays and any(not page_in(table[s, j]) for j in range(-(-had // T)))  # tokens in no page have no rows to move
+        # tokens in no page have no rows to move, and a sequence that stays is given no page for tokens that it has
+        holes = any(not page_in(table[s, j]) for j in range(n // T if stays else 0, -(-had // T)))
         if not ok or total > W or holes:
             status.append(-1)
             slots.append([-1] * room)

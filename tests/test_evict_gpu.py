@@ -318,3 +318,12 @@ def test_a_hole_in_a_long_table(C, dev):
         st.table[0, at], was = -1, st.table[0, at].clone()
         assert evict(C, dev, st, [1], [0], 20, 1, 5) == [want]
         st.table[0, at] = was
+
+
+def test_no_page_for_tokens_that_a_staying_sequence_has(C, dev):
+    """The page that its length ends in is missing: a fresh one would make its tokens another sequence's rows."""
+    st = State(22, [40, 48, 40, 33], P=60)
+    st.kv[:, :, :, st.refs == 0] = 7.0
+    st.table[0, 2], st.table[1, 2], st.table[2, 1] = -1, -1, 60
+    for room in (0, 20):
+        assert evict(C, dev, st, [0, 1, 2, 3], [0, 1, 2, 3], 50, 2, 8, room) == [-1, 1, 1, 1]  # (48 tokens end at a page's end)
