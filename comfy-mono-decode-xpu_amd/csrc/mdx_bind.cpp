@@ -1,6 +1,6 @@
-// mdx._bind: the paged cache's calls and verify_drafts from Python without a Python-level check of every operand. The module checks torch
-// tensors (type, shape, strides, device), takes outputs and workspaces from torch's allocator and calls libmdx's C entry
-// points on the current stream of the tensors' device. These calls are a few microseconds of GPU work in a serving loop
+// mdx._bind: the paged cache's calls and verify_drafts from Python without a Python-level check of every operand. The module
+// checks torch tensors (type, shape, strides, device), takes outputs and workspaces from torch's allocator and calls libmdx's C
+// entry points on the current stream of the tensors' device. These calls are a few microseconds of GPU work in a serving loop
 // that captures no graph: with the checks in Python a call of attn_paged took 14.5 us of host time, two thirds of them
 // outside the launches.
 //

@@ -1,5 +1,6 @@
 // Attention over the paged cache (layout: mdx_pages.hip): single tokens, drafted trees and prompt rows of several
-// sequences (mdx_attn_paged), and the same over the blocks of a long context that a score selects (mdx_attn_blocks).
+// sequences (mdx_attn_paged), the same over the blocks of a long context that a score selects (mdx_attn_blocks), and within a
+// sliding window and a few first tokens, with the rows' log-sum-exps (mdx_attn_window).
 //
 // Row (b, s, h) attends the committed tokens t < n = length[b] and the rows' own tokens n + j (j < S, their K/V in the
 // pages already) that bit j of mask[b][s] admits, or j <= s without masks: softmax(q . k / sqrt(D)) v, 0 where no token
@@ -18,7 +19,8 @@
 // scores; softmax against an earlier maximum, renewed when a score passes it by a slack; O^T += V^T P^T with A = V^T by transposing LDS reads in the token order the
 // S^T accumulators hold, B = P^T from registers. A wave holds up to four tiles of 16 query rows and reads each K and V
 // operand once for all of them. Sums, maxima and O in fp32; P is rounded to the cache's type for the product (half a
-// step of each weight; the normaliser sums the rounded weights, so that equal values come out unchanged).
+// step of each weight; the normaliser sums the rounded weights, so that equal values come out unchanged; a log-sum-exp is that of
+// the weights as they were).
 //
 // What bounds it. Few rows: the cache's bytes, where there are many (64 single tokens over 262 thousand: 193 us, 5.6 TB/s),
 // else the latency of one work-group's chain of queries, pages, first stage, products, meeting and join (one token of a

@@ -21,10 +21,10 @@
 // What bounds it: many rows the exponentials, 14 vector instructions each, eight of them float64 (7 rows of 32 sequences and their
 // drafts over 151936: 37 us for 126 MB, 25 at the rate of a large copy; with 20 instructions 51), then the walk and the draw, 16
 // and 5 us, chains of dependent loads; one short chain those alone (14 us a call). 8 rows of 16 trees: 16 us and 11.
-// Exponentials: 2^(a / 512) = table[k % 512] 2^(k / 512) poly(a - k), k = rint(a): a table of 4 KiB in LDS, a polynomial of degree 3
-// through the Chebyshev points of [-1/2, 1/2] (1.1e-15 relative; a table of 128, 2.8e-13, takes the rows of 32 sequences 35 us for 37,
-// one of 1024, 1.1e-16, 37.6); x / T as it stands, without a maximum, as long as none is past 2^900 (then the row is read again
-// less its largest).
+// Exponentials: 2^(a / 512) = table[k % 512] 2^((k - k % 512) / 512) poly(a - k), k = rint(a): a table of 4 KiB in LDS, a polynomial
+// of degree 3 through the Chebyshev points of [-1/2, 1/2] (1.1e-15 relative; the rows of 32 sequences take 37 us, 35 with a table of
+// 128 and 2.8e-13, 37.6 with one of 1024 and 1.1e-16); x / T as it stands, without a maximum, as long as none is past 2^900 (then the
+// row is read again less its largest).
 //
 // Reference: the walk's role is csrc/mtp_loop.sycl:86-196's accept (which compares with one sampled token per row).
 #include "mdx_common.hpp"

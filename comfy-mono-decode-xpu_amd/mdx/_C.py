@@ -1352,8 +1352,9 @@ def attn_blocks(q, key, value, ksum, table, length, blocks, sink=1, local=1, mas
 def attn_window(q, key, value, table, length, window, sinks=0, mask=None, scale=None, out=None, lse=None):
     """attn_paged within a sliding window: of the tokens that a row attends there, in order (the committed ones, then those of
     the rows' own that its mask admits), it attends the first `sinks` and the last `window` (None: all). The other operands
-    are attn_paged's. Returns (out [B, S, H, D], lse float32 [B, S, H], apart from q and out): lse is the log of the row's sum
-    of exp(scale q . k), -inf for a row that admits nothing (attn_mass takes it). No counterpart in the reference."""
+    are attn_paged's, and so is the rounding of the weights to the cache's type for the product with the values. Returns (out
+    [B, S, H, D], lse float32 [B, S, H], apart from q and out): lse is the log of the row's sum of exp(scale q . k), before any
+    rounding, -inf for a row that admits nothing (attn_mass takes it). No counterpart in the reference."""
     return (_bind or _bound()).attn_window(q, key, value, table, length, window, sinks, mask, scale, out, lse)
 
 
@@ -1392,9 +1393,10 @@ def verify_drafts(logits, tokens, uniform, draft=None, parent=None, temperature=
     Without draft (drafts that are no samples; trees): of a row's children, in row order, the first is accepted whose token,
     with the distinct ones ahead of it, has more of p_r than uniform[b, r]; if none has, the answer is drawn from p_r without
     their tokens. A row with no drafted token behind it answers from p_r. Drawn: the lowest index whose cumulative weight
-    passes uniform[b, R] of the whole, in 64-bit sums (a weight under 2^-100 of the largest may count as
-    none). uniform float64 [B, R + 1] in [0, 1). temperature: a number, or float32 [B]; 0: the lowest index of the largest logit has all of p_r. A logit of -inf or NaN has no probability; +inf counts as
-    the largest finite number.
+    passes uniform[b, R] of the whole, in 64-bit sums (a weight under 2^-100 of the largest may count as none). uniform float64
+    [B, R + 1] in [0, 1). temperature: a number, or float32 [B]; 0: the lowest index of the largest logit has all of p_r. A
+    logit of -inf or NaN has no probability; +inf counts as the largest finite number. At most 1024 sequences, 64 rows, and
+    2^24 - 1 pieces of 16384 logits in all rows together.
     Returns (count int32 [B]: row 0 and the accepted rows, path int32 [B, R]: those rows, -1 behind, next int64 [B]: the
     answer, -1 where no token has a probability); count and path are page_commit's. The role of mtp_accept's walk
     (csrc/mtp_loop.sycl:86-196 of the reference), by probabilities and for a batch."""

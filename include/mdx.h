@@ -651,8 +651,8 @@ int mdx_attn_blocks(const void* q, int64_t q_seq_stride, int64_t q_row_stride, i
 
 /* mdx_attn_paged within a window: of the tokens that a row attends there, in order (the committed ones, then the own ones it
  * admits), the first `sinks` and the last `window` (sinks 0..2^30, window 1..2^30). lse f32 [B, S, H], apart from q and out: log
- * of the sum of exp(scale q . k) over them, -inf for none. A token in no page keeps its place in the order. No counterpart in
- * the reference. */
+ * of the sum of exp(scale q . k) over them (of the weights before their rounding), -inf for none. A token in no page keeps its
+ * place in the order. No counterpart in the reference. */
 size_t mdx_attn_window_workspace(int64_t B, int64_t S, int64_t H, int64_t Hk, int64_t D, int64_t T, int64_t W, int64_t window,
                                  int64_t sinks);
 int mdx_attn_window(const void* q, int64_t q_seq_stride, int64_t q_row_stride, int64_t q_head_stride, const void* key,
