@@ -7,11 +7,10 @@
 // another pair of the call reads, and src may be thinned in place or as a copy.
 //
 // Two launches (several of 2^20 work-groups where there are more). evict_plan_kernel: one work-group looks the sources' pages over
-// and gives the fresh ones (as page_fork's plan does), the others, one per (pair,
-// layer, kv head), find the keep-th largest mass by a radix search over its order-preserving bits (11 + 11 + 10, the masses in
-// registers and LDS up to 16384 tokens, read again beyond) and write the kept tokens' numbers, places in the pool and masses in
-// order. evict_move_kernel: work-groups of whole new pages gather the kept rows, 16 bytes a lane, and take the full pages'
-// mean keys; the first ones change the tables.
+// and gives the fresh ones (as page_fork's plan does), the others, one per (pair, layer, kv head), find the keep-th largest mass by a
+// radix search over its order-preserving bits (11 + 11 + 10, the masses in registers and LDS up to 16384 tokens, read again beyond)
+// and write the kept tokens' numbers, places in the pool and masses in order. evict_move_kernel: work-groups of whole new pages
+// gather the kept rows, 16 bytes a lane, and take the full pages' mean keys; the first ones change the tables.
 //
 // What bounds it: the kept rows' bytes, read and written (4 sequences of 16100 tokens to 2048 in 8 layers of 8 kv heads of 128: the
 // move 115 us at 4.6 TB/s behind a plan of 21); for one short sequence the latency of the plan's and the search's dependent

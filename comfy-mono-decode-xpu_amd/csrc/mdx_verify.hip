@@ -8,7 +8,7 @@
 // The draw: the lowest index whose cumulative weight passes u_R of the whole.
 //
 // All of it in 64 bits: a drawn token is a whole number that changes where u falls between two sums, and at a vocabulary of 150
-// thousand 32-bit sums (1e-7 of the whole) would move one draw in thirty across a border. Here a weight is good to some 2e-15 and
+// thousand 32-bit weights and sums (1e-7 of the whole) would move one draw in a hundred across a border. Here a weight is good to some 2e-15 and
 // 3e-16 |x / T|, a border to half of that: at most one draw in 1e9.
 //
 // verify_rows_kernel: a work-group per slice of a row (16384 logits, fewer where there are few) sums their exponentials. Without q
